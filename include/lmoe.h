@@ -417,6 +417,58 @@ int lmoe_trace_simple_gla_fwd(const lmoe_args* a, int64_t* trace, int32_t work_g
  * gla/gla.py:58-59, deltanet/deltanet.py:81-82, basic_linear_attention/basic_linear_attention.py:99-100). */
 int lmoe_fused_recurrent_fwd(const lmoe_args* a, int32_t op, void* stream);
 
+/* Softmax attention, the layers between the linear ones of a hybrid model (the reference's core:
+ * linear_moe/sequence_modeling/attention/dot_product_attention.py:139-183).
+ *   x = scale q_i . k_j;  x = softcap tanh(x / softcap) where softcap > 0;  s_ij = x - slopes[h] |i - j| where slopes is given
+ *   o_i = sum_j softmax_j(s_ij) v_j  over the j of the same sequence with (causal = 0, or j <= i, or j < prefix_lens[n])
+ * Query head h reads key and value head h / (HQ / HKV).  i, j count inside the sequence.  Packed input (cu_seqlens, chunk_map,
+ * nt_dev, N, NT) as for the chunk ops, B = 1; rows behind the last sequence are zero in o, dq, dk, dv.
+ * K, V <= 128, multiples of 16 bytes; q, k, v, o and their gradients with 16-byte aligned rows. */
+typedef struct lmoe_attn_args {
+  int32_t dtype;       /* of q, k, v, o and their gradients                            */
+  int32_t causal;
+  int32_t B, T, HQ, HKV, K, V;
+  int32_t N, NT;       /* sequences, 64-token chunks (as in lmoe_args)                 */
+  float scale, softcap;
+  const int32_t *cu_seqlens, *chunk_map, *nt_dev;
+  const float* slopes;         /* [HQ] or NULL                                         */
+  const int32_t* prefix_lens;  /* [N] or NULL (causal calls); beyond 0 .. length: clamped */
+  lmoe_tensor q, k, v, o;      /* [B,T,HQ,K], [B,T,HKV,K], [B,T,HKV,V], [B,T,HQ,V]     */
+  float* lse;          /* [B,HQ,T]: log2 of the sum of e^s per row; written by fwd (NULL: not kept), read by bwd */
+  /* backward: o, lse of the forward call, d_o in; dq, dk, dv out (dk.ptr and dv.ptr NULL: dq alone)      */
+  lmoe_tensor d_o, dq, dk, dv;
+  float* delta;        /* [B,HQ,T] workspace: sum of d_o o per row                     */
+} lmoe_attn_args;
+int lmoe_softmax_attn_fwd(const lmoe_attn_args* a, void* stream);
+int lmoe_softmax_attn_bwd(const lmoe_attn_args* a, void* stream);
+
+/* One new token per sequence over a paged cache of keys and values, and the writing of that cache.  Position j of sequence n
+ * lies in slot j % S of page table[n * table_stride + j / S].  A position whose page is not in [0, P) or whose column is
+ * not in [0, M) does not exist: it is neither read (it takes no part) nor written.  lens below 0 count as 0.
+ * kp, vp: [P, S, HKV, K] and [P, S, HKV, V] with sb the stride of a page, st of a slot, sh of a head.
+ * lmoe_paged_attn_decode: q, o [N, 1, HQ, K | V]; the token attends to the lens[n] tokens of the cache and, where kn, vn
+ *   ([N, 1, HKV, K | V]) are given, to itself, and they are written at position lens[n].  slopes: distance to the last token.
+ *   Nothing to attend to: o = 0.  ws: lmoe_paged_attn_floats fp32 numbers (0: may be NULL), 16-byte aligned.
+ * lmoe_paged_kv_append: kn, vn [B, T, HKV, K | V]: token t of row n goes to position lens[n] + t (cu_seqlens NULL, N = B), or
+ *   packed, B = 1: token cu_seqlens[n] + t of sequence n; tokens behind the last sequence are left out.
+ * Two tokens of one call that share a position leave one of them there.  No counterpart in the reference, whose generation
+ * keeps dense caches (linear_moe/generation). */
+typedef struct lmoe_paged_args {
+  int32_t dtype;       /* of q, kp, vp, kn, vn, o                                      */
+  int32_t N, HQ, HKV, K, V;
+  int32_t P, S, M;     /* pages, tokens per page, columns of the table                 */
+  int32_t B, T;        /* append only                                                  */
+  float scale, softcap;
+  int64_t table_stride;
+  const int32_t *table, *lens, *cu_seqlens;
+  const float* slopes; /* [HQ] or NULL                                                 */
+  lmoe_tensor q, o, kp, vp, kn, vn;
+  float* ws;
+} lmoe_paged_args;
+int64_t lmoe_paged_attn_floats(const lmoe_paged_args* a);
+int lmoe_paged_attn_decode(const lmoe_paged_args* a, void* stream);
+int lmoe_paged_kv_append(const lmoe_paged_args* a, void* stream);
+
 /* Toolkit self-test over one pair of 64 x kd tiles A, B (element type by dtype, kd in {64,128}),
  * through the same tile loaders, MFMA fragments and accumulator stores the kernels use:
  * C[64][64] (fp32) = A B^T (contraction along tile columns), G[kd][kd] (fp32) = A^T B

@@ -48,6 +48,23 @@ class Args(C.Structure):
     ]
 
 
+class AttnArgs(C.Structure):
+    """``lmoe_attn_args`` -- field order must match include/lmoe.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "causal", "B", "T", "HQ", "HKV", "K", "V", "N", "NT")]
+                + [("scale", C.c_float), ("softcap", C.c_float)]
+                + [(n, C.c_void_p) for n in ("cu_seqlens", "chunk_map", "nt_dev", "slopes", "prefix_lens")]
+                + [(n, Tensor4) for n in ("q", "k", "v", "o")] + [("lse", C.c_void_p)]
+                + [(n, Tensor4) for n in ("d_o", "dq", "dk", "dv")] + [("delta", C.c_void_p)])
+
+
+class PagedArgs(C.Structure):
+    """``lmoe_paged_args`` -- field order must match include/lmoe.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "N", "HQ", "HKV", "K", "V", "P", "S", "M", "B", "T")]
+                + [("scale", C.c_float), ("softcap", C.c_float), ("table_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("table", "lens", "cu_seqlens", "slopes")]
+                + [(n, Tensor4) for n in ("q", "o", "kp", "vp", "kn", "vn")] + [("ws", C.c_void_p)])
+
+
 ENTRY_POINTS = (
     "lmoe_version", "lmoe_last_error",
     "lmoe_chunk_simple_gla_fwd", "lmoe_chunk_simple_gla_bwd",
@@ -61,6 +78,7 @@ ENTRY_POINTS = (
     "lmoe_quad_featmap_bwd",
     "lmoe_fused_recurrent_fwd", "lmoe_trace_gdn_state_fwd", "lmoe_trace_simple_gla_fwd", "lmoe_mom_gather", "lmoe_mom_combine", "lmoe_mom_rowdot",
     "lmoe_mom_combine_bwd", "lmoe_mom_plan_ints", "lmoe_mom_plan", "lmoe_seq_tables",
+    "lmoe_softmax_attn_fwd", "lmoe_softmax_attn_bwd", "lmoe_paged_attn_floats", "lmoe_paged_attn_decode", "lmoe_paged_kv_append",
 )
 
 _lib = None
@@ -158,6 +176,11 @@ def load() -> C.CDLL:
     lib.lmoe_mom_plan.restype = C.c_int
     lib.lmoe_seq_tables.argtypes = [C.c_void_p] + [C.c_int32] * 3 + [C.c_void_p] * 6
     lib.lmoe_seq_tables.restype = C.c_int
+    for fn in (lib.lmoe_softmax_attn_fwd, lib.lmoe_softmax_attn_bwd):
+        fn.argtypes, fn.restype = [C.POINTER(AttnArgs), C.c_void_p], C.c_int
+    for fn in (lib.lmoe_paged_attn_decode, lib.lmoe_paged_kv_append):
+        fn.argtypes, fn.restype = [C.POINTER(PagedArgs), C.c_void_p], C.c_int
+    lib.lmoe_paged_attn_floats.argtypes, lib.lmoe_paged_attn_floats.restype = [C.POINTER(PagedArgs)], C.c_int64
     lib.lmoe_split_floats.argtypes = [C.POINTER(Args), C.c_int32, C.c_int32]
     lib.lmoe_split_floats.restype = C.c_int64
     lib.lmoe_split_lengths.argtypes = [C.POINTER(Args), C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]

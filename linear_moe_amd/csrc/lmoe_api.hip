@@ -667,6 +667,101 @@ int lmoe_launch_stage(const lmoe_args* a, int32_t op, int32_t stage, void* strea
   return launched(nm);
 }
 
+constexpr int64_t MAX_GROUPS = 1 << 24;      // of 256 threads: a launch has less than 2^32
+static int check_attn(const lmoe_attn_args* a, const char* op, bool bwd) {
+  if (!a) return fail(-1, "%s: null argument block", op);
+  if (a->dtype != LMOE_BF16 && a->dtype != LMOE_F32) return fail(-2, "%s: dtype must be LMOE_BF16 or LMOE_F32", op);
+  const int64_t vec = a->dtype == LMOE_BF16 ? 8 : 4;            // elements per 16 bytes
+  if (a->K <= 0 || a->V <= 0 || a->K > 128 || a->V > 128 || a->K % vec || a->V % vec)
+    return fail(-3, "%s: head dims K=%d V=%d unsupported (at most 128, multiples of 16 bytes)", op, a->K, a->V);
+  if (a->B < 0 || a->T < 0 || a->HQ <= 0 || a->HKV <= 0 || a->N < 0 || a->NT < 0) return fail(-4, "%s: negative dimension", op);
+  if (a->HQ % a->HKV) return fail(-3, "%s: HQ=%d is no multiple of HKV=%d", op, a->HQ, a->HKV);
+  if (a->HQ > 65535 || a->N > 65535) return fail(-8, "%s: HQ and N must be <= 65535", op);
+  const int64_t per_row = ((int64_t)a->T + LMOE_CHUNK - 1) / LMOE_CHUNK;
+  if (a->cu_seqlens) {
+    if (a->B != 1 || !a->chunk_map) return fail(-5, "%s: packed input needs B == 1 and chunk_map", op);
+    if ((int64_t)a->NT > per_row + a->N) return fail(-4, "%s: packed input of T=%d, N=%d has at most %lld chunks, NT=%d given", op, a->T, a->N, (long long)(per_row + a->N), a->NT);
+  } else {
+    if (a->N != a->B) return fail(-6, "%s: dense input needs N == B", op);
+    if ((int64_t)a->NT != a->B * per_row) return fail(-4, "%s: dense input of B=%d, T=%d has %lld chunks, NT=%d given", op, a->B, a->T, (long long)(a->B * per_row), a->NT);
+  }
+  if (!a->q.ptr || !a->k.ptr || !a->v.ptr || !a->o.ptr) return fail(-7, "%s: q, k, v, o must not be null", op);
+  if (bwd && (!a->lse || !a->delta || !a->d_o.ptr || !a->dq.ptr)) return fail(-11, "%s: lse, delta, d_o and dq must not be null", op);
+  if ((a->dk.ptr != nullptr) != (a->dv.ptr != nullptr)) return fail(-11, "%s: dk and dv go together", op);
+  if (!(a->softcap >= 0.f) || a->softcap > 3e38f) return fail(-15, "%s: softcap must be finite and not negative", op);
+  if (a->prefix_lens && !a->causal) return fail(-15, "%s: prefix_lens belongs to a causal call", op);
+  const lmoe_tensor* rows[] = {&a->q, &a->k, &a->v, &a->o, &a->d_o, &a->dq, &a->dk, &a->dv};
+  for (const lmoe_tensor* t : rows)
+    if (t->ptr && (((uintptr_t)t->ptr & 15) || t->sb % vec || t->st % vec || t->sh % vec))
+      return fail(-9, "%s: q, k, v, o and their gradients need 16-byte aligned rows (pointer and strides)", op);
+  if (lmoe::attn_groups(*a) >= MAX_GROUPS) return fail(-8, "%s: more than 2^24 - 1 work-groups", op);
+  return 0;
+}
+int lmoe_softmax_attn_fwd(const lmoe_attn_args* a, void* stream) {
+  const char* op = "lmoe_softmax_attn_fwd";
+  if (int r = check_attn(a, op, false)) return r;
+  if (a->B == 0 || a->T == 0) return 0;
+  lmoe::launch_attn_fwd(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_softmax_attn_bwd(const lmoe_attn_args* a, void* stream) {
+  const char* op = "lmoe_softmax_attn_bwd";
+  if (int r = check_attn(a, op, true)) return r;
+  if (a->B == 0 || a->T == 0) return 0;
+  lmoe::launch_attn_bwd(*a, (hipStream_t)stream);
+  return launched(op);
+}
+
+static int check_paged(const lmoe_paged_args* a, const char* op) {
+  if (!a) return fail(-1, "%s: null argument block", op);
+  if (a->dtype != LMOE_BF16 && a->dtype != LMOE_F32) return fail(-2, "%s: dtype must be LMOE_BF16 or LMOE_F32", op);
+  const int64_t vec = a->dtype == LMOE_BF16 ? 8 : 4;
+  if (a->K <= 0 || a->V <= 0 || a->K > 128 || a->V > 128 || a->K % vec || a->V % vec)
+    return fail(-3, "%s: head dims K=%d V=%d unsupported (at most 128, multiples of 16 bytes)", op, a->K, a->V);
+  if (a->N < 0 || a->HKV <= 0 || a->P < 0 || a->M < 0 || a->S <= 0) return fail(-4, "%s: negative dimension", op);
+  if (a->HKV > 65535 || a->N > 65535) return fail(-8, "%s: heads and N must be <= 65535", op);
+  if ((int64_t)a->M * a->S >= INT32_MAX) return fail(-8, "%s: %d pages of %d tokens per sequence: positions must stay below 2^31 - 1", op, a->M, a->S);
+  if (!a->kp.ptr || !a->vp.ptr || (!a->table && a->M > 0) || !a->lens) return fail(-7, "%s: pages, table and lens must not be null", op);
+  if ((a->kn.ptr != nullptr) != (a->vn.ptr != nullptr)) return fail(-11, "%s: kn and vn go together", op);
+  const lmoe_tensor* rows[] = {&a->q, &a->o, &a->kp, &a->vp, &a->kn, &a->vn};
+  for (const lmoe_tensor* t : rows)
+    if (t->ptr && (((uintptr_t)t->ptr & 15) || t->sb % vec || t->st % vec || t->sh % vec))
+      return fail(-9, "%s: q, o, the pages and the new tokens need 16-byte aligned rows (pointer and strides)", op);
+  return 0;
+}
+static int check_decode(const lmoe_paged_args* a, const char* op) {
+  if (int r = check_paged(a, op)) return r;
+  if (a->HQ <= 0 || a->HQ % a->HKV) return fail(-3, "%s: HQ=%d is no multiple of HKV=%d", op, a->HQ, a->HKV);
+  if (a->HQ > 65535) return fail(-8, "%s: heads and N must be <= 65535", op);
+  if ((int64_t)a->N * a->HQ >= MAX_GROUPS) return fail(-8, "%s: more than 2^24 - 1 rows of q", op);
+  if (!(a->softcap >= 0.f) || a->softcap > 3e38f) return fail(-15, "%s: softcap must be finite and not negative", op);
+  return 0;
+}
+int64_t lmoe_paged_attn_floats(const lmoe_paged_args* a) {
+  if (int r = check_decode(a, "lmoe_paged_attn_floats")) return r;
+  return lmoe::paged_attn_floats(*a);
+}
+int lmoe_paged_attn_decode(const lmoe_paged_args* a, void* stream) {
+  const char* op = "lmoe_paged_attn_decode";
+  if (int r = check_decode(a, op)) return r;
+  if (!a->q.ptr || !a->o.ptr) return fail(-7, "%s: q and o must not be null", op);
+  if (a->N == 0) return 0;
+  if (lmoe::paged_attn_floats(*a) > 0 && (!a->ws || ((uintptr_t)a->ws & 15))) return fail(-11, "%s: ws must be a 16-byte aligned pointer", op);
+  lmoe::launch_paged_decode(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged_kv_append(const lmoe_paged_args* a, void* stream) {
+  const char* op = "lmoe_paged_kv_append";
+  if (int r = check_paged(a, op)) return r;
+  if (a->B < 0 || a->T < 0) return fail(-4, "%s: negative dimension", op);
+  if (!a->kn.ptr) return fail(-7, "%s: kn and vn must not be null", op);
+  if (a->cu_seqlens ? a->B != 1 : a->N != a->B) return fail(-6, "%s: N == B for dense input, B == 1 for packed", op);
+  if ((int64_t)a->B * a->T >= 4 * MAX_GROUPS) return fail(-8, "%s: more than 2^26 - 1 tokens", op);
+  if (a->B == 0 || a->T == 0 || a->N == 0) return 0;
+  lmoe::launch_paged_append(*a, (hipStream_t)stream);
+  return launched(op);
+}
+
 int lmoe_selftest_gemm(int32_t dtype, int32_t kd, const void* A, const void* B, float* C, float* G, void* stream) {
   if (!A || !B || !C || !G) return fail(-1, "lmoe_selftest_gemm: null pointer");
   if ((dtype != LMOE_BF16 && dtype != LMOE_F32) || (kd != 64 && kd != 128))

@@ -1,0 +1,115 @@
+// Softmax attention: what its kernels share.
+//
+//   x_ij = scale q_i . k_j                            (query head h reads key / value head h / (HQ / HKV))
+//   x_ij = cap tanh(x_ij / cap)                       with a cap
+//   s_ij = x_ij - slope_h |i - j|                     with slopes
+//   allowed(i, j): same sequence and (not causal, or j <= i, or j < prefix of the sequence)
+//   p_ij = 2^(log2(e) s_ij - lse_i),  lse_i = log2 sum_j e^{s_ij},   o_i = sum_j p_ij v_j
+// Backward, with delta_i = do_i . o_i and dp_ij = do_i . v_j:
+//   ds_ij = p_ij (dp_ij - delta_i) [(1 - tanh^2(x_ij / cap))]
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_{h, i} ds_ij q_i,   dv_j = sum_{h, i} p_ij do_i
+// (stands where the reference's softmax layers call their attention core:
+// linear_moe/sequence_modeling/attention/dot_product_attention.py:139-183).
+//
+// All exponents are to the base 2: log2(e) is a factor of the scale, the cap and the slope.  Statistics, the sums and the
+// accumulators are fp32.  Every row of a sequence is allowed to see itself (causal) or everything, so no row is empty;
+// rows that a mask leaves nothing of inside one tile are handled by a finite lowest maximum (M_LOW): 2^(-inf - M_LOW) = 0.
+#pragma once
+#include "lmoe_launch.hpp"
+#include "lmoe_seq.hpp"
+
+namespace lmoe {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float M_LOW = -1e30f;
+
+// What turns a product q . k into a score to the base 2.  CAP, BIAS: the call has a cap / slopes.
+template <bool CAP, bool BIAS, bool FAST> struct Score {
+  float mul;       // without a cap: scale log2(e);  with one: scale / cap (fast: 2 log2(e) scale / cap)
+  float out;       // cap log2(e)
+  float slope;     // slope log2(e)
+  __device__ __forceinline__ Score(const lmoe_attn_args& a, int h) {
+    mul = CAP ? a.scale / a.softcap * (FAST ? 2.0f * LOG2E : 1.0f) : a.scale * LOG2E;
+    out = a.softcap * LOG2E;
+    slope = BIAS ? a.slopes[h] * LOG2E : 0.f;
+  }
+  // tanh(x / cap) of a product.  Fast: 1 - 2 / (1 + e^{2z}), whose error of an ulp of 1 is an ulp of the cap in the score.
+  __device__ __forceinline__ float squash(float qk) const {
+    if constexpr (FAST) return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(qk * mul)), 1.0f);
+    else return tanhf(qk * mul);
+  }
+  // dist = i - j, th = squash(qk) where there is a cap
+  __device__ __forceinline__ float of(float qk, float th, float dist) const {
+    float s = CAP ? th * out : qk * mul;
+    if constexpr (BIAS) s = __builtin_fmaf(-slope, fabsf(dist), s);
+    return s;
+  }
+};
+
+template <bool FAST> __device__ __forceinline__ float pow2(float x) {
+  if constexpr (FAST) return __builtin_amdgcn_exp2f(x); else return exp2f(x);
+}
+
+// The sequence a tile of rows lies in, and the tile's first row inside it
+struct AttnTile {
+  int n, b;        // sequence, batch row
+  int tok0, len;   // first token of the sequence inside the batch row, tokens of the sequence
+  int r0;          // first row of the tile inside the sequence
+  int prefix;      // tokens every row of the sequence sees (causal calls)
+};
+// Tile `idx` of ROWS rows (a multiple of 64), counted from the end: with a causal mask the late rows see most, and work-groups
+// are dispatched in order of their index.  Packed input: the chunk map names 64-token chunks; a tile begins at every
+// ROWS / 64-th of a sequence, the work-groups of the others leave.
+template <int ROWS> __device__ __forceinline__ bool attn_tile(const lmoe_attn_args& a, int idx, bool from_end, AttnTile& t) {
+  if (a.cu_seqlens) {
+    const int nt = a.nt_dev ? as_const(a.nt_dev)[0] : a.NT;
+    const int c = from_end ? nt - 1 - idx : idx;
+    if (c < 0 || c >= nt) return false;
+    t.n = as_const(a.chunk_map)[2 * c];
+    t.r0 = as_const(a.chunk_map)[2 * c + 1] * CH;
+    if (t.r0 % ROWS) return false;
+    t.b = 0;
+    t.tok0 = as_const(a.cu_seqlens)[t.n];
+    t.len = as_const(a.cu_seqlens)[t.n + 1] - t.tok0;
+  } else {
+    const int tiles = (a.T + ROWS - 1) / ROWS, i = idx / a.B;
+    t.n = t.b = idx - i * a.B;
+    t.r0 = (from_end ? tiles - 1 - i : i) * ROWS;
+    t.tok0 = 0; t.len = a.T;
+  }
+  t.prefix = 0;
+  if (a.prefix_lens) {
+    const int p = as_const(a.prefix_lens)[t.n];
+    t.prefix = p < 0 ? 0 : p > t.len ? t.len : p;
+  }
+  return true;
+}
+template <int ROWS> inline int64_t attn_tiles(const lmoe_attn_args& a) {
+  return a.cu_seqlens ? (int64_t)a.NT : (int64_t)a.B * ((a.T + ROWS - 1) / ROWS);
+}
+
+// Rows that belong to no sequence (packed input whose last offset is below T) are zero in the outputs: the work-groups of a
+// launch share them.  out: [1, T, H, D] with D = V or K.
+template <typename T> __device__ __forceinline__ void zero_behind(const lmoe_attn_args& a, const lmoe_tensor& x, int H, int D) {
+  if (!a.cu_seqlens) return;
+  const int end = as_const(a.cu_seqlens)[a.N];
+  if (end >= a.T) return;
+  const typename ET<T>::vec z = ET<T>::zero();
+  const int per = H * (D / ET<T>::VEC);
+  for (int t = end + blockIdx.x; t < a.T; t += gridDim.x)
+    for (int i = threadIdx.x; i < per; i += blockDim.x) {
+      const int h = i / (D / ET<T>::VEC), c = i % (D / ET<T>::VEC) * ET<T>::VEC;
+      *(typename ET<T>::vec*)((T*)x.ptr + (int64_t)t * x.st + (int64_t)h * x.sh + c) = z;
+    }
+}
+
+// largest value of 16 neighbouring lanes (a row of the wave), in all of them
+__device__ __forceinline__ float row16_max(float x) {
+  x = fmaxf(x, dpp_or_zero<0xB1, 0xf>(x));
+  x = fmaxf(x, dpp_or_zero<0x4E, 0xf>(x));
+  x = fmaxf(x, dpp_or_zero<0x141, 0xf>(x));
+  x = fmaxf(x, dpp_or_zero<0x140, 0xf>(x));
+  return x;
+}
+
+}  // namespace lmoe

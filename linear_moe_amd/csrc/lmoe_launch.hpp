@@ -124,5 +124,13 @@ void launch_mom_plan(const void* sel, int is64, int B, int per_row, int topk, in
                      hipStream_t st);
 // token-by-token forward (decoding); delta = the (gated) delta rule
 void launch_recurrent(const lmoe_args& a, bool delta, hipStream_t st);
+// softmax attention; bwd: dk, dv too where their pointers are given
+void launch_attn_fwd(const lmoe_attn_args& a, hipStream_t st);
+void launch_attn_bwd(const lmoe_attn_args& a, hipStream_t st);
+int64_t attn_groups(const lmoe_attn_args& a);                     // work-groups of the largest launch of a call
+// one token per sequence over a paged cache
+int64_t paged_attn_floats(const lmoe_paged_args& a);
+void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st);
+void launch_paged_append(const lmoe_paged_args& a, hipStream_t st);
 void launch_selftest(int dtype, int kd, const void* A, const void* B, float* C, float* G, hipStream_t st);
 }  // namespace lmoe

@@ -1,0 +1,352 @@
+// One new token per sequence over a paged cache of keys and values (include/lmoe.h, lmoe_paged_args), and the writing of the
+// cache.
+//
+// k_paged_attn: a work-group of four waves takes up to 16 query heads of one key head and a stretch of the sequence's cache;
+// each wave takes 32 positions at a time.  Everything a product needs lies in the wave's registers as it comes from memory:
+//   S^T [32 keys][16 heads] = K Q^T:  the rows of K are the A operand (lane l: key l % 16, eight columns), 16 keys twice;
+//     the result leaves lane l with head l % 16 and the keys 4g + e and 16 + 4g + e (g = l / 16, e = 0..3);
+//   O^T [V columns][16 heads] += V^T P^T:  P^T as it is (the contraction index may be numbered freely, so those eight keys are the
+//     lane's share), and V^T from the lane's own loads: lane l loads those eight keys at columns VW n .. VW n + VW - 1
+//     (n = l % 16, VW = W / 16), so element i of all eight is the A operand whose row n is column VW n + i.
+// So there is no LDS traffic and no barrier per step, and 16 lanes read 256 adjacent bytes of a value row.
+// HBM-bound: the keys and values of the live tokens are read once for all heads that share them.
+// The stretches of a sequence are joined by k_paged_join where there is more than one.
+#include "lmoe_attn.hpp"
+
+namespace lmoe {
+
+constexpr int PSTEP = 32;              // positions a wave takes at a time
+constexpr int PGROUP = 4 * PSTEP;      // and a work-group
+constexpr int PHEADS = 16;             // query heads of a work-group
+
+struct PagedPlan {
+  int splits;      // stretches per sequence at most
+  int chunk;       // positions of a stretch at least
+  int blocks;      // work-groups that share a key head's query heads
+  uint32_t div_m;  // j / S = (umulhi(j, div_m) + j) >> div_s for 0 <= j < 2^31
+  int div_s;
+};
+static PagedPlan paged_plan(const lmoe_paged_args& a) {
+  PagedPlan p;
+  p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
+  const int64_t bound = (int64_t)a.M * a.S + 1, groups = (int64_t)a.N * a.HKV * p.blocks;
+  int64_t chunk = bound * groups / (8 * (int64_t)cu_count());
+  chunk = chunk < 2 * PGROUP ? 2 * PGROUP : chunk > 2048 ? 2048 : chunk;
+  chunk = (chunk + PGROUP - 1) / PGROUP * PGROUP;
+  int64_t splits = (bound + chunk - 1) / chunk;
+  const int64_t most = groups >= 16384 ? 1 : 16384 / groups;
+  p.splits = (int)(splits < most ? splits : most);
+  p.chunk = (int)chunk;
+  p.div_s = 0;
+  while ((1ll << p.div_s) < a.S) ++p.div_s;
+  p.div_m = (uint32_t)((((1ull << p.div_s) - (uint64_t)a.S) << 32) / (uint64_t)a.S + 1);
+  return p;
+}
+int64_t paged_attn_floats(const lmoe_paged_args& a) {
+  const PagedPlan p = paged_plan(a);
+  // per (sequence, head, stretch): V columns, maximum, sum -- rounded up so that rows stay on 16 bytes
+  return p.splits > 1 ? (int64_t)a.N * a.HQ * p.splits * (a.V + 4) : 0;
+}
+
+// Tokens the new one attends to in the cache, and the length of a stretch
+struct PagedSeq { int len, chunk, used; };
+__device__ __forceinline__ PagedSeq paged_seq(const lmoe_paged_args& a, const PagedPlan& p, int n) {
+  PagedSeq s;
+  const int len = as_const(a.lens)[n], room = a.M * a.S;
+  s.len = len < 0 ? 0 : len > room ? room : len;
+  const int total = s.len + (a.kn.ptr ? 1 : 0);
+  const int per = (total + p.splits - 1) / p.splits;
+  s.chunk = per <= p.chunk ? p.chunk : (per + PGROUP - 1) / PGROUP * PGROUP;
+  s.used = (total + s.chunk - 1) / s.chunk;
+  return s;
+}
+
+template <typename T, int W> struct PagedTile {
+  static constexpr int KS = W / 32, VW = W / 16;
+  typename ET<T>::frag k[2][KS];
+  T v[8][VW];
+};
+
+template <typename T> __device__ __forceinline__ typename ET<T>::frag zero_frag() {
+  typename ET<T>::frag f;
+  if constexpr (sizeof(T) == 2) f = ET<T>::zero(); else { f.lo = ET<T>::zero(); f.hi = ET<T>::zero(); }
+  return f;
+}
+
+template <typename T, int W, bool CAP, bool BIAS>
+__global__ __launch_bounds__(NTHR) void k_paged_attn(const lmoe_paged_args a, const PagedPlan p) {
+  typedef PagedTile<T, W> Tile;
+  constexpr int KS = Tile::KS, VW = Tile::VW, PIECE = VW < ET<T>::VEC ? VW : ET<T>::VEC;
+  constexpr bool FAST = sizeof(T) == 2;
+  typedef T piece __attribute__((ext_vector_type(PIECE)));
+  __shared__ __attribute__((aligned(16))) float s_o[4][PHEADS][W + 4];
+  __shared__ float s_m[4][PHEADS], s_l[4][PHEADS];
+  const int n = blockIdx.x / (a.HKV * p.blocks), hb = blockIdx.x % (a.HKV * p.blocks), hk = hb / p.blocks, G = a.HQ / a.HKV;
+  const int h0 = hb % p.blocks * PHEADS, heads = min(PHEADS, G - h0);      // of the key head's group
+  const PagedSeq sq = paged_seq(a, p, n);
+  const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = blockIdx.y * sq.chunk;
+  if (begin >= total && blockIdx.y > 0) return;
+  const int end = min(total, begin + sq.chunk);
+  const int l = lane_id(), w = wave_id(), c = l & 15, g = l >> 4;
+  const int32_t* table = a.table + (int64_t)n * a.table_stride;
+  const T* kn = a.kn.ptr ? (const T*)a.kn.ptr + (int64_t)n * a.kn.sb + (int64_t)hk * a.kn.sh : nullptr;
+  const T* vn = a.kn.ptr ? (const T*)a.vn.ptr + (int64_t)n * a.vn.sb + (int64_t)hk * a.vn.sh : nullptr;
+
+  // the new token into its page: by the work-group whose stretch ends with it
+  if (kn && end == total && h0 == 0) {
+    const int page = sq.len / a.S, slot = sq.len % a.S;
+    const bool there = as_const(a.lens)[n] == sq.len && page < a.M;
+    const int id = there ? as_const(table)[page] : -1;
+    if (id >= 0 && id < a.P) {
+      T* kp = (T*)a.kp.ptr + (int64_t)id * a.kp.sb + (int64_t)slot * a.kp.st + (int64_t)hk * a.kp.sh;
+      T* vp = (T*)a.vp.ptr + (int64_t)id * a.vp.sb + (int64_t)slot * a.vp.st + (int64_t)hk * a.vp.sh;
+      if ((int)threadIdx.x < a.K) kp[threadIdx.x] = kn[threadIdx.x];
+      else if (threadIdx.x >= 128 && (int)threadIdx.x - 128 < a.V) vp[threadIdx.x - 128] = vn[threadIdx.x - 128];
+    }
+  }
+
+  typename ET<T>::frag q[KS];
+  {
+    const T* row = (const T*)a.q.ptr + (int64_t)n * a.q.sb + (int64_t)(hk * G + h0 + min(c, heads - 1)) * a.q.sh;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      q[j] = zero_frag<T>();
+      const int d = 32 * j + 8 * g;
+      if (c < heads && d < a.K) {
+        if constexpr (FAST) q[j] = ET<T>::load_frag(row + d);
+        else { q[j].lo = *(const f32x4*)(row + d); if (d + 4 < a.K) q[j].hi = *(const f32x4*)(row + d + 4); }
+      }
+    }
+  }
+  const Score<CAP, BIAS, FAST> sc = [&] {
+    lmoe_attn_args s = {};
+    s.scale = a.scale; s.softcap = a.softcap; s.slopes = a.slopes;
+    return Score<CAP, BIAS, FAST>(s, hk * G + h0 + min(c, heads - 1));
+  }();
+
+  // page of position j, -1 where there is none
+  auto page_of = [&](int j, int& slot) {
+    const int col = (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s);
+    slot = j - col * a.S;
+    const int id = table[col];
+    return id >= 0 && id < a.P ? id : -1;
+  };
+  // the row of keys (VAL: values) of position j, or null
+  auto row_of = [&](int j, bool val) -> const T* {
+    if (j >= end) return nullptr;
+    if (j >= sq.len) return val ? vn : kn;
+    int slot;
+    const int id = page_of(j, slot);
+    if (id < 0) return nullptr;
+    const lmoe_tensor& x = val ? a.vp : a.kp;
+    return (const T*)x.ptr + (int64_t)id * x.sb + (int64_t)slot * x.st + (int64_t)hk * x.sh;
+  };
+  auto load = [&](Tile& t, int j0) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const T* row = row_of(j0 + 16 * b + c, false);
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        t.k[b][j] = zero_frag<T>();
+        const int d = 32 * j + 8 * g;
+        if (row && d < a.K) {
+          if constexpr (FAST) t.k[b][j] = ET<T>::load_frag(row + d);
+          else { t.k[b][j].lo = *(const f32x4*)(row + d); if (d + 4 < a.K) t.k[b][j].hi = *(const f32x4*)(row + d + 4); }
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const T* row = row_of(j0 + 16 * (e >> 2) + 4 * g + (e & 3), true);
+#pragma unroll
+      for (int i = 0; i < VW; i += PIECE) {
+        piece x;
+#pragma unroll
+        for (int y = 0; y < PIECE; ++y) x[y] = (T)0.0f;
+        if (row && VW * c + i < a.V) x = *(const piece*)(row + VW * c + i);
+#pragma unroll
+        for (int y = 0; y < PIECE; ++y) t.v[e][i + y] = x[y];
+      }
+    }
+  };
+
+  f32x4 o[VW];
+#pragma unroll
+  for (int i = 0; i < VW; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = M_LOW, sum = 0.f;
+  auto take = [&](const Tile& t, int j0) {
+    f32x4 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KS; ++j) ET<T>::mma(s[b], t.k[b][j], q[j]);
+    }
+    float mx = M_LOW;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = j0 + 16 * b + 4 * g + e;
+        bool ok = j < end;
+        if (j < min(sq.len, end)) { int slot; ok = page_of(j, slot) >= 0; }
+        s[b][e] = ok ? sc.of(s[b][e], CAP ? sc.squash(s[b][e]) : 0.f, (float)(total - 1 - j)) : -INFINITY;
+        mx = fmaxf(mx, s[b][e]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float next = fmaxf(m, mx), f = pow2<FAST>(m - next);
+    m = next;
+    sum *= f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[b][e] = pow2<FAST>(s[b][e] - m);
+        sum += s[b][e];
+      }
+    // (P rounded to the element type, as the products take it; the sum is of the numbers before)
+    typename ET<T>::frag pf;
+    if constexpr (FAST) pf = frag_of_blocks(s[0], s[1]); else { pf.lo = s[0]; pf.hi = s[1]; }
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+      o[i] *= f;
+      typename ET<T>::frag vf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (FAST) vf[e] = t.v[e][i]; else { if (e < 4) vf.lo[e] = t.v[e][i]; else vf.hi[e - 4] = t.v[e][i]; }
+      }
+      ET<T>::mma(o[i], vf, pf);
+    }
+  };
+
+  Tile t[2];
+  int j0 = begin + PSTEP * w;
+  if (j0 < end) load(t[0], j0);
+  while (j0 < end) {
+    if (j0 + PGROUP < end) load(t[1], j0 + PGROUP);
+    take(t[0], j0);
+    j0 += PGROUP;
+    if (j0 >= end) break;
+    if (j0 + PGROUP < end) load(t[0], j0 + PGROUP);
+    take(t[1], j0);
+    j0 += PGROUP;
+  }
+
+  // the four waves: lane (c, g) holds head c, columns VW (4g + r) + i
+  sum += __shfl_xor(sum, 16, 64);
+  sum += __shfl_xor(sum, 32, 64);
+  if (g == 0) { s_m[w][c] = m; s_l[w][c] = sum; }
+#pragma unroll
+  for (int i = 0; i < VW; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_o[w][c][VW * (4 * g + r) + i] = o[i][r];
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < heads * W; idx += NTHR) {
+    const int hh = idx / W, d = idx % W;
+    if (d >= a.V) continue;
+    const float mm = fmaxf(fmaxf(s_m[0][hh], s_m[1][hh]), fmaxf(s_m[2][hh], s_m[3][hh]));
+    float ll = 0.f, x = 0.f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float f = pow2<FAST>(s_m[y][hh] - mm);
+      ll += f * s_l[y][hh];
+      x += f * s_o[y][hh][d];
+    }
+    const int h = hk * G + h0 + hh;
+    if (sq.used <= 1) {
+      ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll > 0.f ? x / ll : ll == 0.f ? 0.f : ll);
+    } else {
+      float* ws = a.ws + (((int64_t)n * a.HQ + h) * p.splits + blockIdx.y) * (a.V + 4);
+      ws[d] = x;
+      if (d == 0) { ws[a.V] = mm; ws[a.V + 1] = ll; }
+    }
+  }
+}
+
+// o = sum over the stretches of 2^(m_s - m) x_s, divided by the same sum of the l_s
+template <typename T>
+__global__ __launch_bounds__(128) void k_paged_join(const lmoe_paged_args a, const PagedPlan p) {
+  const int n = blockIdx.x / a.HQ, h = blockIdx.x % a.HQ, d = threadIdx.x;
+  const PagedSeq sq = paged_seq(a, p, n);
+  if (sq.used <= 1 || d >= a.V) return;
+  const float* ws = a.ws + ((int64_t)n * a.HQ + h) * p.splits * (a.V + 4);
+  float m = M_LOW;
+  for (int s = 0; s < sq.used; ++s) m = fmaxf(m, ws[(int64_t)s * (a.V + 4) + a.V]);
+  float x = 0.f, ll = 0.f;
+  for (int s = 0; s < sq.used; ++s) {
+    const float* y = ws + (int64_t)s * (a.V + 4);
+    const float f = pow2<sizeof(T) == 2>(y[a.V] - m);
+    ll += f * y[a.V + 1];
+    x += f * y[d];
+  }
+  ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll > 0.f ? x / ll : ll == 0.f ? 0.f : ll);
+}
+
+template <typename T, int W> static void paged_decode(const lmoe_paged_args& a, hipStream_t st) {
+  const PagedPlan p = paged_plan(a);
+  const dim3 grid((uint32_t)((int64_t)a.N * a.HKV * p.blocks), (uint32_t)p.splits);
+  if (a.softcap > 0.f) {
+    if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, true, true>), grid, dim3(NTHR), 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged_attn<T, W, true, false>), grid, dim3(NTHR), 0, st, a, p);
+  } else if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, false, true>), grid, dim3(NTHR), 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged_attn<T, W, false, false>), grid, dim3(NTHR), 0, st, a, p);
+  if (p.splits > 1) hipLaunchKernelGGL((k_paged_join<T>), dim3((uint32_t)((int64_t)a.N * a.HQ)), dim3(128), 0, st, a, p);
+}
+void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st) {
+  const bool narrow = a.K <= 64 && a.V <= 64;
+  if (a.dtype == LMOE_BF16) { if (narrow) paged_decode<bf16, 64>(a, st); else paged_decode<bf16, 128>(a, st); }
+  else if (narrow) paged_decode<float, 64>(a, st);
+  else paged_decode<float, 128>(a, st);
+}
+
+// ------------------------------------------------------------------------- //
+// the cache is written: a wave per token, 16 bytes per lane
+// ------------------------------------------------------------------------- //
+template <typename T> __global__ __launch_bounds__(NTHR) void k_paged_append(const lmoe_paged_args a) {
+  constexpr int VEC = ET<T>::VEC;
+  typedef typename ET<T>::vec vec;
+  const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
+  const int l = lane_id();
+  if (tok >= (int64_t)a.B * a.T) return;
+  int n, b, t, at;       // sequence; row and token in memory; token inside the sequence
+  if (a.cu_seqlens) {
+    // the last sequence that begins at or before the token (of several, all but the last are empty): 64 candidates a round
+    b = 0; t = (int)tok;
+    if (t >= a.cu_seqlens[a.N] || t < a.cu_seqlens[0]) return;
+    int lo = 0, hi = a.N;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, i = lo + l * step;
+      const int cnt = __popcll(__ballot(i < hi && a.cu_seqlens[min(i, a.N)] <= t));
+      lo += (cnt - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    n = lo;
+    at = t - a.cu_seqlens[n];
+  } else {
+    n = b = (int)(tok / a.T);
+    t = at = (int)(tok - (int64_t)b * a.T);
+  }
+  const int64_t pos = (int64_t)a.lens[n] + at;
+  if (a.lens[n] < 0 || pos >= (int64_t)a.M * a.S) return;
+  const int id = a.table[(int64_t)n * a.table_stride + (int)pos / a.S], slot = (int)pos % a.S;
+  if (id < 0 || id >= a.P) return;
+  auto copy = [&](const lmoe_tensor& from, const lmoe_tensor& to, int D) {
+    const T* s = (const T*)from.ptr + (int64_t)b * from.sb + (int64_t)t * from.st;
+    T* d = (T*)to.ptr + (int64_t)id * to.sb + (int64_t)slot * to.st;
+    const int per = D / VEC;
+    for (int i = l; i < a.HKV * per; i += 64) {
+      const int h = i / per, c = i % per * VEC;
+      *(vec*)(d + (int64_t)h * to.sh + c) = *(const vec*)(s + (int64_t)h * from.sh + c);
+    }
+  };
+  copy(a.kn, a.kp, a.K);
+  copy(a.vn, a.vp, a.V);
+}
+void launch_paged_append(const lmoe_paged_args& a, hipStream_t st) {
+  const dim3 grid((uint32_t)(((int64_t)a.B * a.T + NTHR / 64 - 1) / (NTHR / 64)));
+  if (a.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_append<bf16>), grid, dim3(NTHR), 0, st, a);
+  else hipLaunchKernelGGL((k_paged_append<float>), grid, dim3(NTHR), 0, st, a);
+}
+
+}  // namespace lmoe
