@@ -1,5 +1,8 @@
 // Softmax attention: instances and dispatch (kernels in lmoe_attn_any.hpp).
+#include <type_traits>
+
 #include "lmoe_attn_any.hpp"
+#include "lmoe_attn_fwd.hpp"
 
 namespace lmoe {
 
@@ -15,6 +18,14 @@ template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
   }
 };
 
+template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
+  static void fwd(const lmoe_attn_args& a, hipStream_t st) {
+    if (a.T > 1024) hipLaunchKernelGGL((k_attn_fwd<W, 8, CAP, BIAS>), dim3(attn_tiles<256>(a) * a.HQ), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_fwd<W, 4, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HQ), dim3(256), 0, st, a);
+  }
+  static void bwd(const lmoe_attn_args& a, hipStream_t st) { AttnAny<T, W, CAP, BIAS>::bwd(a, st); }
+};
+
 template <template <typename, int, bool, bool> class F, typename T, int W> static void by_score(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
   auto run = [&](auto f) { if (bwd) f.bwd(a, st); else f.fwd(a, st); };
   if (a.softcap > 0.f) { if (a.slopes) run(F<T, W, true, true>()); else run(F<T, W, true, false>()); }
@@ -23,7 +34,7 @@ template <template <typename, int, bool, bool> class F, typename T, int W> stati
 }
 static void attn(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;
-  if (a.dtype == LMOE_BF16) { if (narrow) by_score<AttnAny, bf16, 64>(a, bwd, st); else by_score<AttnAny, bf16, 128>(a, bwd, st); }
+  if (a.dtype == LMOE_BF16) { if (narrow) by_score<Attn16, bf16, 64>(a, bwd, st); else by_score<Attn16, bf16, 128>(a, bwd, st); }
   else if (narrow) by_score<AttnAny, float, 64>(a, bwd, st);
   else by_score<AttnAny, float, 128>(a, bwd, st);
 }

@@ -57,13 +57,20 @@ struct AttnTile {
   int r0;          // first row of the tile inside the sequence
   int prefix;      // tokens every row of the sequence sees (causal calls)
 };
-// Tile `idx` of ROWS rows (a multiple of 64), counted from the end: with a causal mask the late rows see most, and work-groups
-// are dispatched in order of their index.  Packed input: the chunk map names 64-token chunks; a tile begins at every
-// ROWS / 64-th of a sequence, the work-groups of the others leave.
-template <int ROWS> __device__ __forceinline__ bool attn_tile(const lmoe_attn_args& a, int idx, bool from_end, AttnTile& t) {
+// The tile of ROWS rows (a multiple of 64) and the head of H that the work-group takes.  from_end: the last tiles first (with a
+// causal mask the late rows see most, and work-groups are dispatched in the order of their index; the keys of a causal call the
+// other way round).  The (row of the batch, head) pairs change fastest, so that neighbouring work-groups do alike; where
+// their number allows it, an XCD (work-groups go round them) keeps the same pairs, and with them the same keys in its L2.
+// Packed input: the chunk map names 64-token chunks; a tile begins at every ROWS / 64-th of a sequence, the work-groups of
+// the others leave.
+template <int ROWS> __device__ __forceinline__ bool attn_place(const lmoe_attn_args& a, int H, bool from_end, int& h, AttnTile& t) {
+  const int pairs = a.cu_seqlens ? H : a.B * H, i = blockIdx.x / pairs;
+  int x = blockIdx.x - i * pairs;
+  if (pairs % 8 == 0) x = (x & 7) * (pairs / 8) + (x >> 3);
+  h = x % H;
   if (a.cu_seqlens) {
     const int nt = a.nt_dev ? as_const(a.nt_dev)[0] : a.NT;
-    const int c = from_end ? nt - 1 - idx : idx;
+    const int c = from_end ? nt - 1 - i : i;
     if (c < 0 || c >= nt) return false;
     t.n = as_const(a.chunk_map)[2 * c];
     t.r0 = as_const(a.chunk_map)[2 * c + 1] * CH;
@@ -72,9 +79,8 @@ template <int ROWS> __device__ __forceinline__ bool attn_tile(const lmoe_attn_ar
     t.tok0 = as_const(a.cu_seqlens)[t.n];
     t.len = as_const(a.cu_seqlens)[t.n + 1] - t.tok0;
   } else {
-    const int tiles = (a.T + ROWS - 1) / ROWS, i = idx / a.B;
-    t.n = t.b = idx - i * a.B;
-    t.r0 = (from_end ? tiles - 1 - i : i) * ROWS;
+    t.n = t.b = x / H;
+    t.r0 = (from_end ? (a.T + ROWS - 1) / ROWS - 1 - i : i) * ROWS;
     t.tok0 = 0; t.len = a.T;
   }
   t.prefix = 0;
@@ -86,6 +92,9 @@ template <int ROWS> __device__ __forceinline__ bool attn_tile(const lmoe_attn_ar
 }
 template <int ROWS> inline int64_t attn_tiles(const lmoe_attn_args& a) {
   return a.cu_seqlens ? (int64_t)a.NT : (int64_t)a.B * ((a.T + ROWS - 1) / ROWS);
+}
+template <typename T> __device__ __forceinline__ T* attn_row(const lmoe_tensor& x, int b, int t, int h) {
+  return (T*)x.ptr + (int64_t)b * x.sb + (int64_t)t * x.st + (int64_t)h * x.sh;
 }
 
 // Rows that belong to no sequence (packed input whose last offset is below T) are zero in the outputs: the work-groups of a

@@ -35,18 +35,15 @@ template <typename T, int NB> __device__ __forceinline__ void attn_store(const f
     }
   }
 }
-template <typename T> __device__ __forceinline__ T* attn_row(const lmoe_tensor& x, int b, int t, int h) {
-  return (T*)x.ptr + (int64_t)b * x.sb + (int64_t)t * x.st + (int64_t)h * x.sh;
-}
-
 template <typename T, int W, bool CAP, bool BIAS>
 __global__ __launch_bounds__(NTHR) void k_attn_fwd_any(const lmoe_attn_args a) {
   constexpr int LD = W + LPAD, PLD = CH + LPAD, NB = W / 16;
   __shared__ __attribute__((aligned(16))) T s_q[CH * LD], s_k[CH * LD], s_v[CH * LD], s_p[CH * PLD];
   zero_behind<T>(a, a.o, a.HQ, a.V);
-  const int h = blockIdx.x % a.HQ, hk = h / (a.HQ / a.HKV);
   AttnTile t;
-  if (!attn_tile<CH>(a, blockIdx.x / a.HQ, true, t)) return;
+  int h;
+  if (!attn_place<CH>(a, a.HQ, true, h, t)) return;
+  const int hk = h / (a.HQ / a.HKV);
   const Score<CAP, BIAS, false> sc(a, h);
   const int l = lane_id(), w = wave_id(), row = t.r0 + 16 * w + 4 * (l >> 4);
   const int rows = min(CH, t.len - t.r0);
@@ -130,9 +127,10 @@ __global__ __launch_bounds__(NTHR) void k_attn_bwd_dq_any(const lmoe_attn_args a
   // (q, then keys; do, then values: the strips of q and do a wave needs stay with it as LDS tiles of their own)
   __shared__ __attribute__((aligned(16))) T s_q[CH * LD], s_k[CH * LD], s_v[CH * LD], s_do[CH * LD], s_p[CH * PLD];
   zero_behind<T>(a, a.dq, a.HQ, a.K);
-  const int h = blockIdx.x % a.HQ, hk = h / (a.HQ / a.HKV);
   AttnTile t;
-  if (!attn_tile<CH>(a, blockIdx.x / a.HQ, true, t)) return;
+  int h;
+  if (!attn_place<CH>(a, a.HQ, true, h, t)) return;
+  const int hk = h / (a.HQ / a.HKV);
   const Score<CAP, BIAS, false> sc(a, h);
   const int l = lane_id(), w = wave_id(), row = t.r0 + 16 * w + 4 * (l >> 4);
   const int rows = min(CH, t.len - t.r0);
@@ -193,9 +191,10 @@ __global__ __launch_bounds__(NTHR) void k_attn_bwd_dkv_any(const lmoe_attn_args 
   __shared__ __attribute__((aligned(16))) T s_q[CH * LD], s_k[CH * LD], s_v[CH * LD], s_do[CH * LD], s_p[CH * PLD];
   zero_behind<T>(a, a.dk, a.HKV, a.K);
   zero_behind<T>(a, a.dv, a.HKV, a.V);
-  const int hk = blockIdx.x % a.HKV, G = a.HQ / a.HKV;
+  const int G = a.HQ / a.HKV;
   AttnTile t;
-  if (!attn_tile<CH>(a, blockIdx.x / a.HKV, false, t)) return;
+  int hk;
+  if (!attn_place<CH>(a, a.HKV, false, hk, t)) return;
   const int l = lane_id(), w = wave_id(), key = t.r0 + 16 * w + 4 * (l >> 4);
   const int keys = min(CH, t.len - t.r0);
   attn_load<T, W>(s_k, attn_row<T>(a.k, t.b, t.tok0 + t.r0, hk), a.k.st, keys, a.K);
