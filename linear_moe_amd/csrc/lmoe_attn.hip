@@ -2,7 +2,7 @@
 #include <type_traits>
 
 #include "lmoe_attn_any.hpp"
-#include "lmoe_attn_fwd.hpp"
+#include "lmoe_attn_bwd.hpp"
 
 namespace lmoe {
 
@@ -23,7 +23,12 @@ template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
     if (a.T > 1024) hipLaunchKernelGGL((k_attn_fwd<W, 8, CAP, BIAS>), dim3(attn_tiles<256>(a) * a.HQ), dim3(512), 0, st, a);
     else hipLaunchKernelGGL((k_attn_fwd<W, 4, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HQ), dim3(256), 0, st, a);
   }
-  static void bwd(const lmoe_attn_args& a, hipStream_t st) { AttnAny<T, W, CAP, BIAS>::bwd(a, st); }
+  static void bwd(const lmoe_attn_args& a, hipStream_t st) {
+    if (a.T > 1024) hipLaunchKernelGGL((k_attn_bwd_dq<W, 8, CAP, BIAS>), dim3(attn_tiles<256>(a) * a.HQ), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_bwd_dq<W, 4, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HQ), dim3(256), 0, st, a);
+    if (!a.dk.ptr) return;
+    hipLaunchKernelGGL((k_attn_bwd_dkv<W, 4, 64, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HKV), dim3(256), 0, st, a);
+  }
 };
 
 template <template <typename, int, bool, bool> class F, typename T, int W> static void by_score(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
