@@ -28,11 +28,12 @@ template <bool CAP, bool BIAS, bool FAST> struct Score {
   float mul;       // without a cap: scale log2(e);  with one: scale / cap (fast: 2 log2(e) scale / cap)
   float out;       // cap log2(e)
   float slope;     // slope log2(e)
-  __device__ __forceinline__ Score(const lmoe_attn_args& a, int h) {
-    mul = CAP ? a.scale / a.softcap * (FAST ? 2.0f * LOG2E : 1.0f) : a.scale * LOG2E;
-    out = a.softcap * LOG2E;
-    slope = BIAS ? a.slopes[h] * LOG2E : 0.f;
+  __device__ __forceinline__ Score(float scale, float softcap, const float* slopes, int h) {
+    mul = CAP ? scale / softcap * (FAST ? 2.0f * LOG2E : 1.0f) : scale * LOG2E;
+    out = softcap * LOG2E;
+    slope = BIAS ? slopes[h] * LOG2E : 0.f;
   }
+  __device__ __forceinline__ Score(const lmoe_attn_args& a, int h) : Score(a.scale, a.softcap, a.slopes, h) {}
   // tanh(x / cap) of a product.  Fast: 1 - 2 / (1 + e^{2z}), whose error of an ulp of 1 is an ulp of the cap in the score.
   __device__ __forceinline__ float squash(float qk) const {
     if constexpr (FAST) return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(qk * mul)), 1.0f);

@@ -62,9 +62,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const lmoe_paged_args& a, const Pa
 }
 
 template <typename T, int W> struct PagedTile {
-  static constexpr int KS = W / 32, VW = W / 16;
+  static constexpr int KS = W / 32, VW = W / 16, PIECE = VW < ET<T>::VEC ? VW : ET<T>::VEC;
+  typedef T piece __attribute__((ext_vector_type(PIECE)));
   typename ET<T>::frag k[2][KS];
-  T v[8][VW];
+  piece v[8][VW / PIECE];
+  uint32_t live;         // which of the 32 positions exist
 };
 
 template <typename T> __device__ __forceinline__ typename ET<T>::frag zero_frag() {
@@ -72,13 +74,22 @@ template <typename T> __device__ __forceinline__ typename ET<T>::frag zero_frag(
   if constexpr (sizeof(T) == 2) f = ET<T>::zero(); else { f.lo = ET<T>::zero(); f.hi = ET<T>::zero(); }
   return f;
 }
+// eight columns from d of a row of D (a multiple of 16 bytes), zeros behind its end
+template <typename T, bool ALL> __device__ __forceinline__ typename ET<T>::frag load_cols(const T* row, int d, int D) {
+  if constexpr (ALL) return ET<T>::load_frag(row + d);
+  typename ET<T>::frag f = zero_frag<T>();
+  if constexpr (sizeof(T) == 2) { if (d < D) f = ET<T>::load_frag(row + d); }
+  else { if (d < D) f.lo = *(const f32x4*)(row + d); if (d + 4 < D) f.hi = *(const f32x4*)(row + d + 4); }
+  return f;
+}
 
-template <typename T, int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NTHR) void k_paged_attn(const lmoe_paged_args a, const PagedPlan p) {
+// ALL: the head dimension of q and k is W.
+template <typename T, int W, bool CAP, bool BIAS, bool ALL>
+__global__ __launch_bounds__(NTHR, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(const lmoe_paged_args a, const PagedPlan p) {
   typedef PagedTile<T, W> Tile;
-  constexpr int KS = Tile::KS, VW = Tile::VW, PIECE = VW < ET<T>::VEC ? VW : ET<T>::VEC;
+  constexpr int KS = Tile::KS, VW = Tile::VW, PIECE = Tile::PIECE;
   constexpr bool FAST = sizeof(T) == 2;
-  typedef T piece __attribute__((ext_vector_type(PIECE)));
+  typedef typename Tile::piece piece;
   __shared__ __attribute__((aligned(16))) float s_o[4][PHEADS][W + 4];
   __shared__ float s_m[4][PHEADS], s_l[4][PHEADS];
   const int n = blockIdx.x / (a.HKV * p.blocks), hb = blockIdx.x % (a.HKV * p.blocks), hk = hb / p.blocks, G = a.HQ / a.HKV;
@@ -89,8 +100,77 @@ __global__ __launch_bounds__(NTHR) void k_paged_attn(const lmoe_paged_args a, co
   const int end = min(total, begin + sq.chunk);
   const int l = lane_id(), w = wave_id(), c = l & 15, g = l >> 4;
   const int32_t* table = a.table + (int64_t)n * a.table_stride;
+  const T* kp = (const T*)a.kp.ptr + (int64_t)hk * a.kp.sh;
+  const T* vp = (const T*)a.vp.ptr + (int64_t)hk * a.vp.sh;
   const T* kn = a.kn.ptr ? (const T*)a.kn.ptr + (int64_t)n * a.kn.sb + (int64_t)hk * a.kn.sh : nullptr;
   const T* vn = a.kn.ptr ? (const T*)a.vn.ptr + (int64_t)n * a.vn.sb + (int64_t)hk * a.vn.sh : nullptr;
+
+  // Where the lane's position (j0 + l % 32) lies.  A page number is asked for two steps before its rows are used and one before they
+  // are asked for, in front of the rows of the step between: loads return in order, so that waiting for it waits for no rows.
+  struct Where { int id, slot; };
+  auto ask = [&](int j0) {
+    Where x = {-1, 0};
+    const int j = j0 + (l & 31);
+    if (j < min(sq.len, end)) {
+      const int col = (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s);
+      x.slot = j - col * a.S;
+      x.id = table[col];
+    }
+    return x;
+  };
+  auto load = [&](Tile& t, int j0, const Where& x) {
+    // offsets of the lane's position, and the other lanes' through the LDS crossbar.  The new token: its own rows.
+    const bool there = x.id >= 0 && x.id < a.P, fresh = j0 + (l & 31) == sq.len && sq.len < end;
+    const int id = there ? x.id : 0;
+    const T* kr = fresh ? kn : kp + (int64_t)id * a.kp.sb + (int64_t)x.slot * a.kp.st;
+    const T* vr = fresh ? vn : vp + (int64_t)id * a.vp.sb + (int64_t)x.slot * a.vp.st;
+    t.live = (uint32_t)__ballot(there || fresh);
+    const uint64_t ki = (uint64_t)(uintptr_t)kr, vi = (uint64_t)(uintptr_t)vr;
+    auto of = [&](uint64_t v, int lane) {
+      const uint32_t lo = __shfl((int)(uint32_t)v, lane, 64), hi = __shfl((int)(uint32_t)(v >> 32), lane, 64);
+      return (const T*)(uintptr_t)((uint64_t)hi << 32 | lo);
+    };
+    const T* kq[2];
+    const T* vq[8];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) kq[b] = of(ki, 16 * b + c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vq[e] = of(vi, 16 * (e >> 2) + 4 * g + (e & 3));
+    const int vc = VW * c;
+    if (t.live == ~0u) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < KS; ++j) t.k[b][j] = load_cols<T, ALL>(kq[b], 32 * j + 8 * g, a.K);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < VW; i += PIECE)
+          // (columns behind the head dimension: any of the row, they are not stored)
+          t.v[e][i / PIECE] = *(const piece*)(vq[e] + (vc + i < a.V ? vc + i : 0));
+    } else {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          t.k[b][j] = zero_frag<T>();
+          if (t.live >> (16 * b + c) & 1) t.k[b][j] = load_cols<T, ALL>(kq[b], 32 * j + 8 * g, a.K);
+        }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < VW; i += PIECE) {
+          piece y;
+#pragma unroll
+          for (int z = 0; z < PIECE; ++z) y[z] = (T)0.0f;
+          if (t.live >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1) y = *(const piece*)(vq[e] + (vc + i < a.V ? vc + i : 0));
+          t.v[e][i / PIECE] = y;
+        }
+    }
+  };
+
+  int j0 = begin + PSTEP * w;
+  Where at = ask(j0), ahead = ask(j0 + PGROUP);
 
   // the new token into its page: by the work-group whose stretch ends with it
   if (kn && end == total && h0 == 0) {
@@ -98,77 +178,21 @@ __global__ __launch_bounds__(NTHR) void k_paged_attn(const lmoe_paged_args a, co
     const bool there = as_const(a.lens)[n] == sq.len && page < a.M;
     const int id = there ? as_const(table)[page] : -1;
     if (id >= 0 && id < a.P) {
-      T* kp = (T*)a.kp.ptr + (int64_t)id * a.kp.sb + (int64_t)slot * a.kp.st + (int64_t)hk * a.kp.sh;
-      T* vp = (T*)a.vp.ptr + (int64_t)id * a.vp.sb + (int64_t)slot * a.vp.st + (int64_t)hk * a.vp.sh;
-      if ((int)threadIdx.x < a.K) kp[threadIdx.x] = kn[threadIdx.x];
-      else if (threadIdx.x >= 128 && (int)threadIdx.x - 128 < a.V) vp[threadIdx.x - 128] = vn[threadIdx.x - 128];
+      T* kd = (T*)a.kp.ptr + (int64_t)id * a.kp.sb + (int64_t)slot * a.kp.st + (int64_t)hk * a.kp.sh;
+      T* vd = (T*)a.vp.ptr + (int64_t)id * a.vp.sb + (int64_t)slot * a.vp.st + (int64_t)hk * a.vp.sh;
+      if ((int)threadIdx.x < a.K) kd[threadIdx.x] = kn[threadIdx.x];
+      else if (threadIdx.x >= 128 && (int)threadIdx.x - 128 < a.V) vd[threadIdx.x - 128] = vn[threadIdx.x - 128];
     }
   }
 
   typename ET<T>::frag q[KS];
+  const int hq = hk * G + h0 + min(c, heads - 1);
   {
-    const T* row = (const T*)a.q.ptr + (int64_t)n * a.q.sb + (int64_t)(hk * G + h0 + min(c, heads - 1)) * a.q.sh;
+    const T* row = (const T*)a.q.ptr + (int64_t)n * a.q.sb + (int64_t)hq * a.q.sh;
 #pragma unroll
-    for (int j = 0; j < KS; ++j) {
-      q[j] = zero_frag<T>();
-      const int d = 32 * j + 8 * g;
-      if (c < heads && d < a.K) {
-        if constexpr (FAST) q[j] = ET<T>::load_frag(row + d);
-        else { q[j].lo = *(const f32x4*)(row + d); if (d + 4 < a.K) q[j].hi = *(const f32x4*)(row + d + 4); }
-      }
-    }
+    for (int j = 0; j < KS; ++j) q[j] = load_cols<T, ALL>(row, 32 * j + 8 * g, a.K);
   }
-  const Score<CAP, BIAS, FAST> sc = [&] {
-    lmoe_attn_args s = {};
-    s.scale = a.scale; s.softcap = a.softcap; s.slopes = a.slopes;
-    return Score<CAP, BIAS, FAST>(s, hk * G + h0 + min(c, heads - 1));
-  }();
-
-  // page of position j, -1 where there is none
-  auto page_of = [&](int j, int& slot) {
-    const int col = (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s);
-    slot = j - col * a.S;
-    const int id = table[col];
-    return id >= 0 && id < a.P ? id : -1;
-  };
-  // the row of keys (VAL: values) of position j, or null
-  auto row_of = [&](int j, bool val) -> const T* {
-    if (j >= end) return nullptr;
-    if (j >= sq.len) return val ? vn : kn;
-    int slot;
-    const int id = page_of(j, slot);
-    if (id < 0) return nullptr;
-    const lmoe_tensor& x = val ? a.vp : a.kp;
-    return (const T*)x.ptr + (int64_t)id * x.sb + (int64_t)slot * x.st + (int64_t)hk * x.sh;
-  };
-  auto load = [&](Tile& t, int j0) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const T* row = row_of(j0 + 16 * b + c, false);
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        t.k[b][j] = zero_frag<T>();
-        const int d = 32 * j + 8 * g;
-        if (row && d < a.K) {
-          if constexpr (FAST) t.k[b][j] = ET<T>::load_frag(row + d);
-          else { t.k[b][j].lo = *(const f32x4*)(row + d); if (d + 4 < a.K) t.k[b][j].hi = *(const f32x4*)(row + d + 4); }
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const T* row = row_of(j0 + 16 * (e >> 2) + 4 * g + (e & 3), true);
-#pragma unroll
-      for (int i = 0; i < VW; i += PIECE) {
-        piece x;
-#pragma unroll
-        for (int y = 0; y < PIECE; ++y) x[y] = (T)0.0f;
-        if (row && VW * c + i < a.V) x = *(const piece*)(row + VW * c + i);
-#pragma unroll
-        for (int y = 0; y < PIECE; ++y) t.v[e][i + y] = x[y];
-      }
-    }
-  };
+  const Score<CAP, BIAS, FAST> sc(a.scale, a.softcap, a.slopes, hq);
 
   f32x4 o[VW];
 #pragma unroll
@@ -188,9 +212,8 @@ __global__ __launch_bounds__(NTHR) void k_paged_attn(const lmoe_paged_args a, co
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = j0 + 16 * b + 4 * g + e;
-        bool ok = j < end;
-        if (j < min(sq.len, end)) { int slot; ok = page_of(j, slot) >= 0; }
-        s[b][e] = ok ? sc.of(s[b][e], CAP ? sc.squash(s[b][e]) : 0.f, (float)(total - 1 - j)) : -INFINITY;
+        const float x = sc.of(s[b][e], CAP ? sc.squash(s[b][e]) : 0.f, (float)(total - 1 - j));
+        s[b][e] = t.live >> (16 * b + 4 * g + e) & 1 ? x : -INFINITY;
         mx = fmaxf(mx, s[b][e]);
       }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
@@ -214,21 +237,25 @@ __global__ __launch_bounds__(NTHR) void k_paged_attn(const lmoe_paged_args a, co
       typename ET<T>::frag vf;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if constexpr (FAST) vf[e] = t.v[e][i]; else { if (e < 4) vf.lo[e] = t.v[e][i]; else vf.hi[e - 4] = t.v[e][i]; }
+        const T x = t.v[e][i / PIECE][i % PIECE];
+        if constexpr (FAST) vf[e] = x; else { if (e < 4) vf.lo[e] = x; else vf.hi[e - 4] = x; }
       }
       ET<T>::mma(o[i], vf, pf);
     }
   };
 
   Tile t[2];
-  int j0 = begin + PSTEP * w;
-  if (j0 < end) load(t[0], j0);
+  if (j0 < end) load(t[0], j0, at);
   while (j0 < end) {
-    if (j0 + PGROUP < end) load(t[1], j0 + PGROUP);
+    at = ahead;
+    ahead = ask(j0 + 2 * PGROUP);
+    if (j0 + PGROUP < end) load(t[1], j0 + PGROUP, at);
     take(t[0], j0);
     j0 += PGROUP;
     if (j0 >= end) break;
-    if (j0 + PGROUP < end) load(t[0], j0 + PGROUP);
+    at = ahead;
+    ahead = ask(j0 + 2 * PGROUP);
+    if (j0 + PGROUP < end) load(t[0], j0 + PGROUP, at);
     take(t[1], j0);
     j0 += PGROUP;
   }
@@ -283,15 +310,18 @@ __global__ __launch_bounds__(128) void k_paged_join(const lmoe_paged_args a, con
   ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll > 0.f ? x / ll : ll == 0.f ? 0.f : ll);
 }
 
-template <typename T, int W> static void paged_decode(const lmoe_paged_args& a, hipStream_t st) {
+template <typename T, int W, bool ALL> static void paged_decode_all(const lmoe_paged_args& a, hipStream_t st) {
   const PagedPlan p = paged_plan(a);
   const dim3 grid((uint32_t)((int64_t)a.N * a.HKV * p.blocks), (uint32_t)p.splits);
   if (a.softcap > 0.f) {
-    if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, true, true>), grid, dim3(NTHR), 0, st, a, p);
-    else hipLaunchKernelGGL((k_paged_attn<T, W, true, false>), grid, dim3(NTHR), 0, st, a, p);
-  } else if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, false, true>), grid, dim3(NTHR), 0, st, a, p);
-  else hipLaunchKernelGGL((k_paged_attn<T, W, false, false>), grid, dim3(NTHR), 0, st, a, p);
+    if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, true, true, ALL>), grid, dim3(NTHR), 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged_attn<T, W, true, false, ALL>), grid, dim3(NTHR), 0, st, a, p);
+  } else if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, false, true, ALL>), grid, dim3(NTHR), 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged_attn<T, W, false, false, ALL>), grid, dim3(NTHR), 0, st, a, p);
   if (p.splits > 1) hipLaunchKernelGGL((k_paged_join<T>), dim3((uint32_t)((int64_t)a.N * a.HQ)), dim3(128), 0, st, a, p);
+}
+template <typename T, int W> static void paged_decode(const lmoe_paged_args& a, hipStream_t st) {
+  if (a.K == W) paged_decode_all<T, W, true>(a, st); else paged_decode_all<T, W, false>(a, st);
 }
 void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;
