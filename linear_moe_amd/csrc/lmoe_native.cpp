@@ -43,6 +43,11 @@ struct Library {
   decltype(&lmoe_mom_plan_ints) mom_plan_ints;
   decltype(&lmoe_mom_plan) mom_plan;
   decltype(&lmoe_seq_tables) seq_tables;
+  decltype(&lmoe_softmax_attn_fwd) attn_fwd;
+  decltype(&lmoe_softmax_attn_bwd) attn_bwd;
+  decltype(&lmoe_paged_attn_floats) paged_floats;
+  decltype(&lmoe_paged_attn_decode) paged_decode;
+  decltype(&lmoe_paged_kv_append) paged_append;
 } lib;
 
 constexpr int OP_SIMPLE = LMOE_OP_SIMPLE_GLA, OP_GLA = LMOE_OP_GLA, OP_GDN = LMOE_OP_GATED_DELTA_RULE;
@@ -735,6 +740,193 @@ PyObject* seq_tables(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- softmax attention and the paged cache ----
+bool number(float& to, PyObject* o, float otherwise) {
+  if (o == Py_None) { to = otherwise; return true; }
+  const double x = PyFloat_AsDouble(o);
+  if (x == -1.0 && PyErr_Occurred()) return false;
+  to = (float)x;
+  return true;
+}
+// slopes or None: one fp32 number per head, not trained
+bool slopes_from(Tensor& to, PyObject* o, int dev, int64_t H) {
+  NEED(plain_or_none(to, o, dev));
+  return !to.defined() || (f32(to) && to.is_contiguous() && to.numel() == H && !to.requires_grad());
+}
+// one int32 per sequence
+bool ints_from(const Tensor& x, int64_t n) { return x.dim() == 1 && x.scalar_type() == at::kInt && x.is_contiguous() && x.numel() == n; }
+
+struct Attn {
+  int dev;
+  bool head_first;
+  int64_t B, T, HQ, HKV, K, V;
+  lmoe_attn_args a = {};
+  Tensor q, k, v, slopes, prefix, tables[5];
+  // o: q, k, v, scale, causal, softcap, slopes, prefix_lens, plan, head_first
+  bool take(PyObject* const* o) {
+    dev = current_device(o[0]);
+    NEED(dev >= 0 && plain(q, o[0], dev) && plain(k, o[1], dev) && plain(v, o[2], dev));
+    head_first = yes(o[9]);
+    NEED(q.dim() == 4 && k.dim() == 4 && v.dim() == 4 && (bf16(q) || f32(q)) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
+    const int h = head_first ? 1 : 2, t = head_first ? 2 : 1;
+    B = q.size(0); T = q.size(t); HQ = q.size(h); HKV = k.size(h); K = q.size(3); V = v.size(3);
+    NEED(k.size(0) == B && k.size(t) == T && k.size(3) == K && v.sizes().slice(0, 3) == k.sizes().slice(0, 3));
+    const int64_t vec = 16 / q.element_size();
+    NEED(q.numel() > 0 && v.numel() > 0 && HQ % HKV == 0 && K <= 128 && V <= 128 && K % vec == 0 && V % vec == 0);
+    NEED(rows_aligned(q) && rows_aligned(k) && rows_aligned(v));
+    NEED(B <= INT32_MAX && T <= INT32_MAX && HQ <= INT32_MAX);
+    int64_t N = B, NT = B * ((T + LMOE_CHUNK - 1) / LMOE_CHUNK);
+    PyObject* const plan = o[8];
+    if (plan != Py_None) {
+      NEED(PyTuple_Check(plan) && PyTuple_GET_SIZE(plan) == 7 && !head_first && B == 1);
+      N = PyLong_AsLongLong(PyTuple_GET_ITEM(plan, 0)); NT = PyLong_AsLongLong(PyTuple_GET_ITEM(plan, 1));
+      for (int i = 0; i < 5; ++i) NEED(plain_or_none(tables[i], PyTuple_GET_ITEM(plan, 2 + i), dev));
+      a.cu_seqlens = (const int32_t*)ptr(tables[0]); a.chunk_map = (const int32_t*)ptr(tables[1]); a.nt_dev = (const int32_t*)ptr(tables[4]);
+    }
+    NEED(NT <= INT32_MAX);
+    NEED(number(a.scale, o[3], (float)std::pow((double)K, -0.5)) && number(a.softcap, o[5], 0.f) && a.softcap >= 0.f && a.softcap < 3e38f);
+    a.causal = yes(o[4]);
+    NEED(slopes_from(slopes, o[6], dev, HQ) && plain_or_none(prefix, o[7], dev));
+    if (prefix.defined()) NEED(a.causal && ints_from(prefix, N));
+    a.dtype = bf16(q) ? LMOE_BF16 : LMOE_F32;
+    a.B = B; a.T = T; a.HQ = HQ; a.HKV = HKV; a.K = K; a.V = V; a.N = N; a.NT = NT;
+    a.slopes = (const float*)ptr(slopes); a.prefix_lens = (const int32_t*)ptr(prefix);
+    a.q = desc(q, head_first); a.k = desc(k, head_first); a.v = desc(v, head_first);
+    return true;
+  }
+  bool lies_like_o(const Tensor& x) const {
+    return x.dim() == 4 && x.sizes().slice(0, 3) == q.sizes().slice(0, 3) && x.size(3) == V && x.scalar_type() == q.scalar_type() && rows_aligned(x);
+  }
+};
+
+// attn_forward(q, k, v, scale, causal, softcap, slopes, prefix_lens, plan, head_first, save, stream) -> (o, lse or None)
+PyObject* attn_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Attn c;
+  if (n != 12 || !c.take(o)) return elsewhere();
+  const bool save = yes(o[10]);
+  void* st = stream_of(o[11]);
+  if (PyErr_Occurred()) return elsewhere();
+  Tensor out, lse;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const auto s = c.q.sizes();
+    out = at::empty({s[0], s[1], s[2], c.V}, c.q.options().requires_grad(false));
+    if (save) lse = at::empty({c.B, c.HQ, c.T}, c.q.options().dtype(at::kFloat).requires_grad(false));
+    c.a.o = desc(out, c.head_first); c.a.lse = (float*)ptr(lse);
+    rc = lib.attn_fwd(&c.a, st);
+  }
+  return result(rc, {out, lse});
+  END_HANDLE_TH_ERRORS
+}
+
+// attn_backward(the first ten of attn_forward, o, lse, do, keys: whether dk and dv are wanted, stream) -> (dq, dk, dv)
+PyObject* attn_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Attn c;
+  Tensor out, lse, dout;
+  if (n != 15 || !c.take(o) || !plain(out, o[10], c.dev) || !plain(lse, o[11], c.dev) || !plain(dout, o[12], c.dev)) return elsewhere();
+  if (!c.lies_like_o(out) || !c.lies_like_o(dout) || !f32(lse) || !lse.is_contiguous() || lse.sizes() != at::IntArrayRef({c.B, c.HQ, c.T})) return elsewhere();
+  const bool keys = yes(o[13]);
+  void* st = stream_of(o[14]);
+  if (PyErr_Occurred()) return elsewhere();
+  Tensor dq, dk, dv;
+  int rc;
+  {
+    const Unlocked unlocked;
+    dq = at::empty_like(c.q.detach());
+    const Tensor delta = at::empty_like(lse);
+    if (keys) { dk = at::empty_like(c.k.detach()); dv = at::empty_like(c.v.detach()); }
+    c.a.o = desc(out, c.head_first); c.a.lse = (float*)lse.data_ptr(); c.a.d_o = desc(dout, c.head_first); c.a.delta = (float*)delta.data_ptr();
+    c.a.dq = desc(dq, c.head_first); c.a.dk = desc(dk, c.head_first); c.a.dv = desc(dv, c.head_first);
+    rc = lib.attn_bwd(&c.a, st);
+  }
+  return result(rc, {dq, dk, dv});
+  END_HANDLE_TH_ERRORS
+}
+
+struct Paged {
+  int dev;
+  lmoe_paged_args a = {};
+  Tensor kp, vp, table, lens;
+  // o: k_pages, v_pages, page_table, lens
+  bool take(PyObject* const* o) {
+    dev = current_device(o[0]);
+    NEED(dev >= 0 && plain(kp, o[0], dev) && plain(vp, o[1], dev) && plain(table, o[2], dev) && plain(lens, o[3], dev));
+    NEED(kp.dim() == 4 && vp.dim() == 4 && dtype_of(kp) >= 0 && vp.scalar_type() == kp.scalar_type() && kp.sizes().slice(0, 3) == vp.sizes().slice(0, 3));
+    const int64_t vec = 16 / kp.element_size(), K = kp.size(3), V = vp.size(3);
+    NEED(kp.numel() > 0 && vp.numel() > 0 && K <= 128 && V <= 128 && K % vec == 0 && V % vec == 0 && rows_aligned(kp) && rows_aligned(vp));
+    NEED(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(1) > 0 && (table.size(1) == 1 || table.stride(1) == 1));
+    NEED(ints_from(lens, table.size(0)) && table.size(0) > 0);
+    for (const int64_t x : {kp.size(0), kp.size(1), kp.size(2), table.size(0), table.size(1)}) NEED(fits(x));
+    a.dtype = dtype_of(kp);
+    a.N = table.size(0); a.M = table.size(1); a.P = kp.size(0); a.S = kp.size(1); a.HKV = kp.size(2); a.K = K; a.V = V;
+    a.table_stride = table.stride(0); a.table = (const int32_t*)table.data_ptr(); a.lens = (const int32_t*)lens.data_ptr();
+    a.kp = desc(kp, false); a.vp = desc(vp, false);
+    return true;
+  }
+  // [B, T, H, D] (or [B, H, T, D]) as it lies
+  bool tokens(Tensor& x, PyObject* o, int64_t B, int64_t T, int64_t H, int64_t D, bool hf) const {
+    NEED(plain(x, o, dev) && x.dim() == 4 && x.scalar_type() == kp.scalar_type());
+    return x.size(0) == B && x.size(hf ? 2 : 1) == T && x.size(hf ? 1 : 2) == H && x.size(3) == D && rows_aligned(x);
+  }
+};
+
+// paged_decode(k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first, stream) -> (o,)
+PyObject* paged_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged c;
+  Tensor q, k, v, slopes;
+  if (n != 12 || !c.take(o)) return elsewhere();
+  const bool hf = yes(o[10]);
+  void* st = stream_of(o[11]);
+  if (PyErr_Occurred() || !plain(q, o[4], c.dev) || q.dim() != 4) return elsewhere();
+  const int64_t HQ = q.size(hf ? 1 : 2);
+  if (HQ < 1 || !fits(HQ) || HQ % c.a.HKV || !c.tokens(q, o[4], c.a.N, 1, HQ, c.a.K, hf) || (o[5] == Py_None) != (o[6] == Py_None)) return elsewhere();
+  if (o[5] != Py_None && !(c.tokens(k, o[5], c.a.N, 1, c.a.HKV, c.a.K, hf) && c.tokens(v, o[6], c.a.N, 1, c.a.HKV, c.a.V, hf))) return elsewhere();
+  c.a.HQ = HQ;
+  if (!number(c.a.scale, o[7], (float)std::pow((double)c.a.K, -0.5)) || !number(c.a.softcap, o[8], 0.f) || !(c.a.softcap >= 0.f && c.a.softcap < 3e38f) ||
+      !slopes_from(slopes, o[9], c.dev, HQ)) return elsewhere();
+  c.a.slopes = (const float*)ptr(slopes);
+  c.a.q = desc(q, hf); c.a.kn = desc(k, hf); c.a.vn = desc(v, hf);
+  const int64_t floats = lib.paged_floats(&c.a);
+  if (floats < 0) return PyLong_FromLong((long)floats);
+  Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const auto s = q.sizes();
+    out = at::empty({s[0], s[1], s[2], c.a.V}, q.options().requires_grad(false));
+    Tensor ws;
+    if (floats) ws = at::empty({floats}, q.options().dtype(at::kFloat).requires_grad(false));
+    c.a.o = desc(out, hf); c.a.ws = (float*)ptr(ws);
+    rc = lib.paged_decode(&c.a, st);
+  }
+  if (rc == 0 && k.defined()) for (const Tensor* x : {&c.kp, &c.vp}) if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  return result(rc, {out});
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(k_pages, v_pages, page_table, lens, k, v, cu_seqlens or None, head_first, stream) -> ()
+PyObject* paged_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged c;
+  Tensor k, v, cu;
+  if (n != 9 || !c.take(o)) return elsewhere();
+  const bool hf = yes(o[7]);
+  void* st = stream_of(o[8]);
+  if (PyErr_Occurred() || !plain(k, o[4], c.dev) || k.dim() != 4 || !plain_or_none(cu, o[6], c.dev)) return elsewhere();
+  const int64_t B = cu.defined() ? 1 : c.a.N, T = k.size(hf ? 2 : 1);
+  if (T < 1 || !fits(T) || !c.tokens(k, o[4], B, T, c.a.HKV, c.a.K, hf) || !c.tokens(v, o[5], B, T, c.a.HKV, c.a.V, hf)) return elsewhere();
+  if (cu.defined() && (hf || !ints_from(cu, (int64_t)c.a.N + 1))) return elsewhere();
+  c.a.B = B; c.a.T = T; c.a.kn = desc(k, hf); c.a.vn = desc(v, hf); c.a.cu_seqlens = (const int32_t*)ptr(cu);
+  const int rc = lib.paged_append(&c.a, st);
+  if (rc == 0) for (const Tensor* x : {&c.kp, &c.vp}) if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  return result(rc, {});
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path): the library's entry points
 PyObject* bind(PyObject*, PyObject* path) {
   const char* p = PyUnicode_AsUTF8(path);
@@ -759,6 +951,8 @@ PyObject* bind(PyObject*, PyObject* path) {
   get(l.swish_fwd, "lmoe_swish_gate_relayout_fwd"); get(l.swish_bwd, "lmoe_swish_gate_relayout_bwd");
   get(l.gates_partials, "lmoe_gdn_gates_partials"); get(l.gates_fwd, "lmoe_gdn_gates_fwd"); get(l.gates_bwd, "lmoe_gdn_gates_bwd");
   get(l.mom_gather, "lmoe_mom_gather"); get(l.mom_combine, "lmoe_mom_combine"); get(l.mom_combine_bwd, "lmoe_mom_combine_bwd");
+  get(l.attn_fwd, "lmoe_softmax_attn_fwd"); get(l.attn_bwd, "lmoe_softmax_attn_bwd"); get(l.paged_floats, "lmoe_paged_attn_floats");
+  get(l.paged_decode, "lmoe_paged_attn_decode"); get(l.paged_append, "lmoe_paged_kv_append");
   get(l.mom_plan_ints, "lmoe_mom_plan_ints"); get(l.mom_plan, "lmoe_mom_plan"); get(l.seq_tables, "lmoe_seq_tables");
   if (!all) return PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point", p);
   lib = l;
@@ -774,6 +968,7 @@ PyMethodDef methods[] = {
     LMOE_METHOD(mixer_forward), LMOE_METHOD(mixer_backward), LMOE_METHOD(swish_forward), LMOE_METHOD(swish_backward),
     LMOE_METHOD(gates_forward), LMOE_METHOD(gates_backward), LMOE_METHOD(mom_gather), LMOE_METHOD(mom_combine),
     LMOE_METHOD(mom_combine_backward), LMOE_METHOD(mom_plan), LMOE_METHOD(seq_tables),
+    LMOE_METHOD(attn_forward), LMOE_METHOD(attn_backward), LMOE_METHOD(paged_decode), LMOE_METHOD(paged_append),
 #undef LMOE_METHOD
     {"intact", (PyCFunction)(void (*)(void))intact, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -1,7 +1,7 @@
 // One new token per sequence over a paged cache of keys and values (include/lmoe.h, lmoe_paged_args), and the writing of the
 // cache.
 //
-// k_paged_attn: a work-group of four waves takes up to 16 query heads of one key head and a stretch of the sequence's cache;
+// k_paged_attn: a work-group of four or eight waves takes up to 16 query heads of one key head and a stretch of the sequence's cache;
 // each wave takes 32 positions at a time.  Everything a product needs lies in the wave's registers as it comes from memory:
 //   S^T [32 keys][16 heads] = K Q^T:  the rows of K are the A operand (lane l: key l % 16, eight columns), 16 keys twice;
 //     the result leaves lane l with head l % 16 and the keys 4g + e and 16 + 4g + e (g = l / 16, e = 0..3);
@@ -16,12 +16,13 @@
 namespace lmoe {
 
 constexpr int PSTEP = 32;              // positions a wave takes at a time
-constexpr int PGROUP = 4 * PSTEP;      // and a work-group
 constexpr int PHEADS = 16;             // query heads of a work-group
+constexpr int PSPLITS = 2048;          // stretches of a sequence at most
 
 struct PagedPlan {
   int splits;      // stretches per sequence at most
   int chunk;       // positions of a stretch at least
+  int waves;       // of a work-group
   int blocks;      // work-groups that share a key head's query heads
   uint32_t div_m;  // j / S = (umulhi(j, div_m) + j) >> div_s for 0 <= j < 2^31
   int div_s;
@@ -30,11 +31,15 @@ static PagedPlan paged_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
   const int64_t bound = (int64_t)a.M * a.S + 1, groups = (int64_t)a.N * a.HKV * p.blocks;
-  int64_t chunk = bound * groups / (8 * (int64_t)cu_count());
-  chunk = chunk < 2 * PGROUP ? 2 * PGROUP : chunk > 2048 ? 2048 : chunk;
-  chunk = (chunk + PGROUP - 1) / PGROUP * PGROUP;
+  // A short cache: one stretch of eight waves, at most four steps each, and no second launch (one sequence of 500 tokens, 16 / 4
+  // heads of 128: 9.2 us, in stretches of 256 and joined 13).  4-byte elements have no registers for eight waves.
+  // Else stretches of one length, whatever the call: us for stretches of 256, 384, 512, 1024 positions (64 sequences of 1024 to 4096
+  // tokens, 32 / 8 heads of 128; 2 of 32 K and 128 K, 16 / 4 heads of 128; 9 of 750 to 3001 tokens, 12 / 3 heads of 64,
+  // 4-byte elements): 140 135 134 136; 80 76 74 78; 20.3 17.4 19.9 31.1.
+  p.waves = a.dtype == LMOE_BF16 && bound <= 1024 ? 8 : 4;
+  const int64_t chunk = p.waves == 8 ? 1024 : a.dtype == LMOE_BF16 ? 512 : 384;
   int64_t splits = (bound + chunk - 1) / chunk;
-  const int64_t most = groups >= 16384 ? 1 : 16384 / groups;
+  const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;
   p.splits = (int)(splits < most ? splits : most);
   p.chunk = (int)chunk;
   p.div_s = 0;
@@ -44,19 +49,20 @@ static PagedPlan paged_plan(const lmoe_paged_args& a) {
 }
 int64_t paged_attn_floats(const lmoe_paged_args& a) {
   const PagedPlan p = paged_plan(a);
-  // per (sequence, head, stretch): V columns, maximum, sum -- rounded up so that rows stay on 16 bytes
-  return p.splits > 1 ? (int64_t)a.N * a.HQ * p.splits * (a.V + 4) : 0;
+  // per (sequence, head, stretch): V columns; behind them all the maxima and sums
+  return p.splits > 1 ? (int64_t)a.N * a.HQ * p.splits * (a.V + 2) : 0;
 }
 
 // Tokens the new one attends to in the cache, and the length of a stretch
 struct PagedSeq { int len, chunk, used; };
 __device__ __forceinline__ PagedSeq paged_seq(const lmoe_paged_args& a, const PagedPlan& p, int n) {
   PagedSeq s;
+  const int step = p.waves * PSTEP;
   const int len = as_const(a.lens)[n], room = a.M * a.S;
   s.len = len < 0 ? 0 : len > room ? room : len;
   const int total = s.len + (a.kn.ptr ? 1 : 0);
   const int per = (total + p.splits - 1) / p.splits;
-  s.chunk = per <= p.chunk ? p.chunk : (per + PGROUP - 1) / PGROUP * PGROUP;
+  s.chunk = per <= p.chunk ? p.chunk : (per + step - 1) / step * step;
   s.used = (total + s.chunk - 1) / s.chunk;
   return s;
 }
@@ -84,19 +90,24 @@ template <typename T, bool ALL> __device__ __forceinline__ typename ET<T>::frag 
 }
 
 // ALL: the head dimension of q and k is W.
-template <typename T, int W, bool CAP, bool BIAS, bool ALL>
-__global__ __launch_bounds__(NTHR, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(const lmoe_paged_args a, const PagedPlan p) {
+template <typename T, int W, int NW, bool CAP, bool BIAS, bool ALL>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(const lmoe_paged_args a, const PagedPlan p) {
   typedef PagedTile<T, W> Tile;
   constexpr int KS = Tile::KS, VW = Tile::VW, PIECE = Tile::PIECE;
   constexpr bool FAST = sizeof(T) == 2;
+  constexpr int PGROUP = NW * PSTEP;        // positions the work-group takes at a time
   typedef typename Tile::piece piece;
-  __shared__ __attribute__((aligned(16))) float s_o[4][PHEADS][W + 4];
-  __shared__ float s_m[4][PHEADS], s_l[4][PHEADS];
-  const int n = blockIdx.x / (a.HKV * p.blocks), hb = blockIdx.x % (a.HKV * p.blocks), hk = hb / p.blocks, G = a.HQ / a.HKV;
+  __shared__ __attribute__((aligned(16))) float s_o[NW][PHEADS][W + 4];
+  __shared__ float s_m[NW][PHEADS], s_l[NW][PHEADS];
+  // The stretches of one head follow each other in the grid, so that an XCD (work-groups go round them) has stretches of all
+  // heads: with the heads next to each other, each XCD had some heads only, and those of the longest sequence took their
+  // XCDs' time (the two documents of the comment above: 94 -> 74 us).
+  const int part = blockIdx.x % p.splits, group = blockIdx.x / p.splits;
+  const int n = group / (a.HKV * p.blocks), hb = group % (a.HKV * p.blocks), hk = hb / p.blocks, G = a.HQ / a.HKV;
   const int h0 = hb % p.blocks * PHEADS, heads = min(PHEADS, G - h0);      // of the key head's group
   const PagedSeq sq = paged_seq(a, p, n);
-  const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = blockIdx.y * sq.chunk;
-  if (begin >= total && blockIdx.y > 0) return;
+  const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = part * sq.chunk;
+  if (begin >= total && part > 0) return;
   const int end = min(total, begin + sq.chunk);
   const int l = lane_id(), w = wave_id(), c = l & 15, g = l >> 4;
   const int32_t* table = a.table + (int64_t)n * a.table_stride;
@@ -260,7 +271,7 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(con
     j0 += PGROUP;
   }
 
-  // the four waves: lane (c, g) holds head c, columns VW (4g + r) + i
+  // the waves together: lane (c, g) holds head c, columns VW (4g + r) + i
   sum += __shfl_xor(sum, 16, 64);
   sum += __shfl_xor(sum, 32, 64);
   if (g == 0) { s_m[w][c] = m; s_l[w][c] = sum; }
@@ -269,59 +280,97 @@ __global__ __launch_bounds__(NTHR, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(con
 #pragma unroll
     for (int r = 0; r < 4; ++r) s_o[w][c][VW * (4 * g + r) + i] = o[i][r];
   __syncthreads();
-  for (int idx = threadIdx.x; idx < heads * W; idx += NTHR) {
+  for (int idx = threadIdx.x; idx < heads * W; idx += NW * 64) {
     const int hh = idx / W, d = idx % W;
     if (d >= a.V) continue;
-    const float mm = fmaxf(fmaxf(s_m[0][hh], s_m[1][hh]), fmaxf(s_m[2][hh], s_m[3][hh]));
+    float mm = M_LOW;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) mm = fmaxf(mm, s_m[y][hh]);
     float ll = 0.f, x = 0.f;
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < NW; ++y) {
       const float f = pow2<FAST>(s_m[y][hh] - mm);
       ll += f * s_l[y][hh];
       x += f * s_o[y][hh][d];
     }
     const int h = hk * G + h0 + hh;
     if (sq.used <= 1) {
-      ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll > 0.f ? x / ll : ll == 0.f ? 0.f : ll);
+      ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll != 0.f ? x / ll : 0.f);
     } else {
-      float* ws = a.ws + (((int64_t)n * a.HQ + h) * p.splits + blockIdx.y) * (a.V + 4);
-      ws[d] = x;
-      if (d == 0) { ws[a.V] = mm; ws[a.V + 1] = ll; }
+      const int64_t at = ((int64_t)n * a.HQ + h) * p.splits + part, rows = (int64_t)a.N * a.HQ * p.splits;
+      a.ws[at * a.V + d] = x;
+      if (d == 0) *(f32x2*)(a.ws + rows * a.V + 2 * at) = f32x2{mm, ll};
     }
   }
 }
 
-// o = sum over the stretches of 2^(m_s - m) x_s, divided by the same sum of the l_s
+// The stretches of one (sequence, head) joined: o = sum 2^(m_s - m) x_s / sum 2^(m_s - m) l_s.  Eight rows of 32 lanes, four columns a
+// lane; a row takes every eighth stretch.
 template <typename T>
-__global__ __launch_bounds__(128) void k_paged_join(const lmoe_paged_args a, const PagedPlan p) {
-  const int n = blockIdx.x / a.HQ, h = blockIdx.x % a.HQ, d = threadIdx.x;
+__global__ __launch_bounds__(NTHR) void k_paged_join(const lmoe_paged_args a, const PagedPlan p) {
+  __shared__ float s_f[PSPLITS], s_r[NTHR / 64];
+  __shared__ __attribute__((aligned(16))) f32x4 s_x[8][32];
+  const int n = blockIdx.x / a.HQ, h = blockIdx.x % a.HQ, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(a, p, n);
-  if (sq.used <= 1 || d >= a.V) return;
-  const float* ws = a.ws + ((int64_t)n * a.HQ + h) * p.splits * (a.V + 4);
+  if (sq.used <= 1) return;
+  const int64_t at = ((int64_t)n * a.HQ + h) * p.splits, rows = (int64_t)a.N * a.HQ * p.splits;
+  const f32x2* ml = (const f32x2*)(a.ws + rows * a.V) + at;
   float m = M_LOW;
-  for (int s = 0; s < sq.used; ++s) m = fmaxf(m, ws[(int64_t)s * (a.V + 4) + a.V]);
-  float x = 0.f, ll = 0.f;
-  for (int s = 0; s < sq.used; ++s) {
-    const float* y = ws + (int64_t)s * (a.V + 4);
-    const float f = pow2<sizeof(T) == 2>(y[a.V] - m);
-    ll += f * y[a.V + 1];
-    x += f * y[d];
+  for (int s = tid; s < sq.used; s += NTHR) m = fmaxf(m, ml[s][0]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  if ((tid & 63) == 0) s_r[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_r[0], s_r[1]), fmaxf(s_r[2], s_r[3]));
+  float ll = 0.f;
+  for (int s = tid; s < sq.used; s += NTHR) {
+    const f32x2 y = ml[s];
+    const float f = pow2<sizeof(T) == 2>(y[0] - m);
+    s_f[s] = f;
+    ll += f * y[1];
   }
-  ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll > 0.f ? x / ll : ll == 0.f ? 0.f : ll);
+  ll = wave_sum(ll);
+  __syncthreads();                       // s_r has been read, s_f is whole
+  if ((tid & 63) == 0) s_r[tid >> 6] = ll;
+  const int c = tid & 31, r = tid >> 5;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (4 * c < a.V) {
+    const float* ws = a.ws + at * a.V + 4 * c;
+#pragma unroll 4
+    for (int s = r; s < sq.used; s += 8) x += s_f[s] * *(const f32x4*)(ws + (int64_t)s * a.V);
+  }
+  s_x[r][c] = x;
+  __syncthreads();
+  if (r == 0 && 4 * c < a.V) {
+    ll = (s_r[0] + s_r[1]) + (s_r[2] + s_r[3]);
+#pragma unroll
+    for (int y = 1; y < 8; ++y) x += s_x[y][c];
+    typename ET<T>::vec4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = ET<T>::from_f(ll != 0.f ? x[i] / ll : 0.f);
+    *(typename ET<T>::vec4*)((T*)a.o.ptr + (int64_t)n * a.o.sb + (int64_t)h * a.o.sh + 4 * c) = y;
+  }
 }
 
-template <typename T, int W, bool ALL> static void paged_decode_all(const lmoe_paged_args& a, hipStream_t st) {
-  const PagedPlan p = paged_plan(a);
-  const dim3 grid((uint32_t)((int64_t)a.N * a.HKV * p.blocks), (uint32_t)p.splits);
+template <typename T, int W, int NW, bool ALL> static void paged_parts(const lmoe_paged_args& a, const PagedPlan& p, hipStream_t st) {
+  const dim3 grid((uint32_t)((int64_t)a.N * a.HKV * p.blocks * p.splits)), block(64 * NW);
   if (a.softcap > 0.f) {
-    if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, true, true, ALL>), grid, dim3(NTHR), 0, st, a, p);
-    else hipLaunchKernelGGL((k_paged_attn<T, W, true, false, ALL>), grid, dim3(NTHR), 0, st, a, p);
-  } else if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, false, true, ALL>), grid, dim3(NTHR), 0, st, a, p);
-  else hipLaunchKernelGGL((k_paged_attn<T, W, false, false, ALL>), grid, dim3(NTHR), 0, st, a, p);
-  if (p.splits > 1) hipLaunchKernelGGL((k_paged_join<T>), dim3((uint32_t)((int64_t)a.N * a.HQ)), dim3(128), 0, st, a, p);
+    if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, NW, true, true, ALL>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged_attn<T, W, NW, true, false, ALL>), grid, block, 0, st, a, p);
+  } else if (a.slopes) hipLaunchKernelGGL((k_paged_attn<T, W, NW, false, true, ALL>), grid, block, 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged_attn<T, W, NW, false, false, ALL>), grid, block, 0, st, a, p);
 }
 template <typename T, int W> static void paged_decode(const lmoe_paged_args& a, hipStream_t st) {
-  if (a.K == W) paged_decode_all<T, W, true>(a, st); else paged_decode_all<T, W, false>(a, st);
+  const PagedPlan p = paged_plan(a);
+  if constexpr (sizeof(T) == 2) {
+    if (p.waves == 8) {
+      if (a.K == W) paged_parts<T, W, 8, true>(a, p, st); else paged_parts<T, W, 8, false>(a, p, st);
+    }
+  }
+  if (p.waves == 4) {
+    if (a.K == W) paged_parts<T, W, 4, true>(a, p, st); else paged_parts<T, W, 4, false>(a, p, st);
+  }
+  if (p.splits > 1) hipLaunchKernelGGL((k_paged_join<T>), dim3((uint32_t)((int64_t)a.N * a.HQ)), dim3(NTHR), 0, st, a, p);
 }
 void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;

@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._host import _DT, _desc, ptr, stream_ptr
+from ._host import _DT, _desc, native_call, ptr, stream_ptr
 from .softmax_attn import MAX_DIM, cap_of, has_rows16, ints_of, on_current_device, rows16, slopes_of
 
 
@@ -74,6 +74,13 @@ def _no_grad(name, *xs):
         raise RuntimeError(f"{name} is for generation and has no backward: call it under torch.no_grad(), or train with softmax_attn")
 
 
+def _written(*pages):
+    """Autograd's count of writes (a backward that saved the pages notices them)."""
+    for x in pages:
+        if not x.is_inference():
+            torch.autograd.graph.increment_version(x)
+
+
 def paged_attn_decode(
     q: torch.Tensor,
     k_pages: torch.Tensor,
@@ -95,6 +102,9 @@ def paged_attn_decode(
     sequence with nothing to attend to gives zeros.  A position beyond the table is attended to but not kept."""
     name = "paged_attn_decode"
     _no_grad(name, q, k, v, k_pages, v_pages, slopes)
+    r = native_call("paged_decode", name, k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first)
+    if r is not None:
+        return r[0]
     if (k is None) != (v is None):
         raise ValueError(f"{name}: k and v go together")
     a, held = _pages(k_pages, v_pages, page_table, lens, name)
@@ -121,6 +131,8 @@ def paged_attn_decode(
     ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     a.ws = ptr(ws)
     _lib.check(lib.lmoe_paged_attn_decode(C.byref(a), stream_ptr()), name)
+    if k is not None:
+        _written(k_pages, v_pages)
     return o
 
 
@@ -139,6 +151,8 @@ def paged_kv_append(
     last packed sequence, and positions that have no page, are left out."""
     name = "paged_kv_append"
     _no_grad(name, k, v, k_pages, v_pages)
+    if native_call("paged_append", name, k_pages, v_pages, page_table, lens, k, v, cu_seqlens, head_first) is not None:
+        return
     a, held = _pages(k_pages, v_pages, page_table, lens, name)
     if k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"{name}: k and v must be 4-dimensional")
@@ -161,3 +175,4 @@ def paged_kv_append(
     a.B, a.T, a.kn, a.vn = B, T, _desc(k, head_first), _desc(v, head_first)
     if k.numel() and a.N:
         _lib.check(_lib.load().lmoe_paged_kv_append(C.byref(a), stream_ptr()), name)
+        _written(k_pages, v_pages)

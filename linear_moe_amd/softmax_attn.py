@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._host import _DT, _desc, no_node, ptr, seq_plan, stream_ptr
+from ._host import _DT, _desc, native_call, no_node, ptr, seq_plan, stream_ptr
 
 MAX_DIM = 128      # columns of a head
 
@@ -105,6 +105,9 @@ def _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, pre
 
 def _forward(q, k, v, dims, head_first, scale, causal, softcap, slopes, prefix, plan, save):
     B, T, HQ, HKV, K, V = dims
+    r = native_call("attn_forward", "softmax_attn forward", q, k, v, scale, causal, softcap, slopes, prefix, plan.tables, head_first, save)
+    if r is not None:
+        return (q, k, v, *r)
     q, k, v = rows16(q.detach()), rows16(k.detach()), rows16(v.detach())
     o = torch.empty((*q.shape[:3], V), dtype=q.dtype, device=q.device)
     lse = torch.empty(B, HQ, T, dtype=torch.float32, device=q.device) if save else None
@@ -137,6 +140,12 @@ class _SoftmaxAttn(torch.autograd.Function):
         dims, head_first, scale, causal, softcap, plan = ctx.call
         B, T, HQ, HKV, K, V = dims
         q, k, v, o, lse, slopes, prefix = ctx.saved_tensors
+        keys = any(ctx.needs_input_grad[1:3])
+        if (q.shape, k.shape, v.shape, o.shape) == ctx.shapes and (slopes is not None, prefix is not None) == ctx.options:
+            r = native_call("attn_backward", "softmax_attn backward", q, k, v, scale, causal, softcap, slopes, prefix, plan.tables,
+                            head_first, o, lse, do, keys)
+            if r is not None:
+                return (*r, *(None,) * 8)
         dev, dt = do.device, ctx.dtype
         q, k, v, o = (_back(x, s, dt, dev, n) for x, s, n in zip((q, k, v, o), ctx.shapes, "qkvo"))
         do = _back(do, ctx.shapes[3], dt, dev, "the gradient")
@@ -146,7 +155,7 @@ class _SoftmaxAttn(torch.autograd.Function):
         if ctx.options[1]:
             prefix = _back(prefix, (plan.N,), torch.int32, dev, "prefix_lens")
         dq = torch.empty_like(q)
-        dk, dv = (torch.empty_like(k), torch.empty_like(v)) if any(ctx.needs_input_grad[1:3]) else (None, None)
+        dk, dv = (torch.empty_like(k), torch.empty_like(v)) if keys else (None, None)
         if B * T:
             a = _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, prefix, plan)
             delta = torch.empty(B, HQ, T, dtype=torch.float32, device=dev)
@@ -180,6 +189,10 @@ def softmax_attn(
     cu_seqlens: packed documents as in the chunk ops; rows of one never see another's (nor what it holds: a NaN stays in its
     document).  Rows behind the last document are zero in o and in the gradients.
     Without atomics: the gradients of a key head are summed over its query heads in a fixed order."""
+    if cu_seqlens is None and no_node(q, k, v):      # (what the native path takes as it is, it also checks)
+        r = native_call("attn_forward", "softmax_attn forward", q, k, v, scale, causal, softcap, slopes, prefix_lens, None, head_first, False)
+        if r is not None:
+            return r[0]
     dims = _check(q, k, v, head_first, cu_seqlens)
     B, T, HQ, HKV, K, V = dims
     on_current_device(q.device, "softmax_attn")
