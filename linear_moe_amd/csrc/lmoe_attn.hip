@@ -1,4 +1,6 @@
 // Softmax attention: instances and dispatch (kernels in lmoe_attn_any.hpp).
+#include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "lmoe_attn_any.hpp"
@@ -27,7 +29,8 @@ template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
     if (a.T > 1024) hipLaunchKernelGGL((k_attn_bwd_dq<W, 8, CAP, BIAS>), dim3(attn_tiles<256>(a) * a.HQ), dim3(512), 0, st, a);
     else hipLaunchKernelGGL((k_attn_bwd_dq<W, 4, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HQ), dim3(256), 0, st, a);
     if (!a.dk.ptr) return;
-    hipLaunchKernelGGL((k_attn_bwd_dkv<W, 4, 64, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HKV), dim3(256), 0, st, a);
+    if (a.T > 1024) hipLaunchKernelGGL((k_attn_bwd_dkv<W, 8, CAP, BIAS>), dim3(attn_tiles<256>(a) * a.HKV), dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_bwd_dkv<W, 4, CAP, BIAS>), dim3(attn_tiles<128>(a) * a.HKV), dim3(256), 0, st, a);
   }
 };
 
@@ -39,7 +42,11 @@ template <template <typename, int, bool, bool> class F, typename T, int W> stati
 }
 static void attn(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;
-  if (a.dtype == LMOE_BF16) { if (narrow) by_score<Attn16, bf16, 64>(a, bwd, st); else by_score<Attn16, bf16, 128>(a, bwd, st); }
+  // (the kernels on 2-byte elements reach the rows of a tile by 32-bit offsets)
+  int64_t stride = 0;
+  for (const lmoe_tensor* x : {&a.q, &a.k, &a.v, &a.d_o}) stride = std::max(stride, std::abs(x->st));
+  if (a.dtype == LMOE_BF16 && stride >= (1 << 24)) { if (narrow) by_score<AttnAny, bf16, 64>(a, bwd, st); else by_score<AttnAny, bf16, 128>(a, bwd, st); }
+  else if (a.dtype == LMOE_BF16) { if (narrow) by_score<Attn16, bf16, 64>(a, bwd, st); else by_score<Attn16, bf16, 128>(a, bwd, st); }
   else if (narrow) by_score<AttnAny, float, 64>(a, bwd, st);
   else by_score<AttnAny, float, 128>(a, bwd, st);
 }

@@ -47,6 +47,29 @@ template <bool CAP, bool BIAS, bool FAST> struct Score {
   }
 };
 
+// The same for the kernels on 2-byte elements, which keep a number u per pair that grows with the score, s = a u + b, so that a score
+// less a maximum (or lse) is one multiply-add:  u = q . k (q negated for a negative scale);  with a cap u = -1 / (1 + e^{2x / cap}),
+// tanh = 1 + 2 u, a = 2 b = 2 cap;  with slopes u = s.
+template <bool CAP, bool BIAS> struct Score16 {
+  float mul, cap2, slope, a, b;
+  bool negate;
+  __device__ __forceinline__ Score16(const lmoe_attn_args& x, int h) {
+    negate = !CAP && !BIAS && x.scale < 0.f;
+    mul = CAP ? x.scale / x.softcap * (2.0f * LOG2E) : x.scale * LOG2E;
+    cap2 = 2.0f * x.softcap * LOG2E;
+    slope = BIAS ? x.slopes[h] * LOG2E : 0.f;
+    // (a > 0 also for a scale of 0: a hidden score of -infinity stays one)
+    a = BIAS ? 1.0f : CAP ? cap2 : fmaxf(fabsf(mul), 1e-37f);
+    b = !BIAS && CAP ? 0.5f * cap2 : 0.f;
+  }
+  // r: the factor of the cap, (1 - tanh^2) / 4 = -r (1 + r); dist = i - j
+  __device__ __forceinline__ float operator()(float qk, float dist, float& r) const {
+    if constexpr (CAP) r = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(qk * mul));
+    if constexpr (BIAS) return __builtin_fmaf(-slope, fabsf(dist), CAP ? __builtin_fmaf(r, cap2, 0.5f * cap2) : qk * mul);
+    return CAP ? r : qk;
+  }
+};
+
 template <bool FAST> __device__ __forceinline__ float pow2(float x) {
   if constexpr (FAST) return __builtin_amdgcn_exp2f(x); else return exp2f(x);
 }

@@ -10,18 +10,17 @@ namespace lmoe {
 // whose lse and delta are one number, and dS^T as the B operand of dQ^T += K^T dS^T.
 template <int W, int NW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
-  constexpr int LD = W + LPAD, KS = W / 16, DB = W / 32, NT = NW * 64, ROWS = NW * 32, TILE = CH * LD;
-  typedef RowStage<CH, W, NT> St;
-  __shared__ __attribute__((aligned(16))) bf16 s_kv[4 * TILE];
-  static_assert(ROWS * LD <= 4 * TILE, "the strips of the waves");
+  constexpr int KS = W / 16, DB = W / 32, ROWS = NW * 32, TILE = CH * W;
+  __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
   zero_behind<bf16>(a, a.dq, a.HQ, a.K);
   AttnTile t;
   int h;
   if (!attn_place<ROWS>(a, a.HQ, true, h, t)) return;
-  const int hk = h / (a.HQ / a.HKV), tid = threadIdx.x, l = lane_id(), w = wave_id(), g = l >> 5;
-  const Score<CAP, BIAS, true> sc(a, h);
-  const int w0 = t.r0 + 32 * w, rows = t.len - w0, row = w0 + (l & 31);
-  const int64_t at = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0;
+  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 5;
+  const Score16<CAP, BIAS> sc(a, h);
+  const int w0 = t.r0 + 32 * w, rows = t.len - w0, row_ = w0 + (l & 31);
+  const int64_t first = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0;
+  const Swz<W> lane(l);
   bf16x8 q[KS], d_o[KS];
   rows32<W>(d_o, attn_row<bf16>(a.d_o, t.b, t.tok0 + min(w0, t.len - 1), h), a.d_o.st, max(rows, 1), a.V, l);
   rows32<W>(q, attn_row<bf16>(a.o, t.b, t.tok0 + min(w0, t.len - 1), h), a.o.st, max(rows, 1), a.V, l);
@@ -29,190 +28,234 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
 #pragma unroll
   for (int j = 0; j < KS; ++j) delta = dot_vec(q[j], d_o[j], delta);
   delta = both_sum(delta);
-  const float lse = a.lse[at + min(row, t.len - 1)];
-  if (g == 0 && row < t.len) a.delta[at + row] = delta;
+  const float lse = a.lse[first + min(row_, t.len - 1)];
+  if (g == 0 && row_ < t.len) a.delta[first + row_] = delta;
   rows32<W>(q, attn_row<bf16>(a.q, t.b, t.tok0 + min(w0, t.len - 1), h), a.q.st, max(rows, 1), a.K, l);
+  if (sc.negate) {
+#pragma unroll
+    for (int j = 0; j < KS; ++j) frag_negate(q[j]);
+  }
+  const float off = sc.b - lse;
   f32x16 dq[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) dq[b] = zero16();
 
   const int end = a.causal ? min(t.len, max(t.r0 + ROWS, t.prefix)) : t.len;
   const int wend = rows <= 0 ? 0 : a.causal ? min(t.len, max(w0 + 32, t.prefix)) : t.len;
-  const int whole = a.causal ? max(w0 + 1, t.prefix) : t.len;
+  const int whole = min(a.causal ? max(t.r0 + 1, t.prefix) : t.len, end);
   const bf16* kp = attn_row<bf16>(a.k, t.b, t.tok0, hk);
   const bf16* vp = attn_row<bf16>(a.v, t.b, t.tok0, hk);
 
   auto block = [&](const bf16* sk, const bf16* sv, int j0, auto part_c) {
     constexpr bool PART = decltype(part_c)::value;
+    const Swz<W> at = lane.fresh();
+    const int row = fresh_index(row_);
+    bf16x8 kf[2], vf[2], kt[2 * DB];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       __builtin_amdgcn_sched_barrier(0);
       f32x16 s = zero16(), dp = zero16();
+      // (pieces of two steps at a time: the registers hold no more)
 #pragma unroll
-      for (int j = 0; j < KS; ++j) s = mfma32(*(const bf16x8*)(sk + (32 * b + (l & 31)) * LD + 16 * j + 8 * g), q[j], s);
+      for (int j = 0; j < KS; j += 2) {
 #pragma unroll
-      for (int j = 0; j < KS; ++j) dp = mfma32(*(const bf16x8*)(sv + (32 * b + (l & 31)) * LD + 16 * j + 8 * g), d_o[j], dp);
+        for (int x = 0; x < 2; ++x) { kf[x] = at.frag(sk, b, j + x); vf[x] = at.frag(sv, b, j + x); }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { s = mfma32(kf[x], q[j + x], s); dp = mfma32(vf[x], d_o[j + x], dp); }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) kt[x * DB + d] = at.frag_t(sk, 2 * b + x, d);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int j = j0 + 32 * b + row32(i) + 4 * g;
-        const float th = CAP ? sc.squash(s[i]) : 0.f;
-        float ds = pow2<true>(sc.of(s[i], th, (float)(row - j)) - lse) * (dp[i] - delta);
-        if constexpr (CAP) ds *= __builtin_fmaf(-th, th, 1.0f);
+        float r;
+        const float u = sc(s[i], (float)(row - j), r);
+        float ds = pow2<true>(__builtin_fmaf(u, sc.a, off)) * (dp[i] - delta);
+        if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
         if constexpr (PART) ds = j < t.len && (!a.causal || j <= row || j < t.prefix) ? ds : 0.f;
         s[i] = ds;
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const bf16x8 ds = frag_of_acc(s, x);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) dq[d] = mfma32(frag32_t(sk, LD, 32 * b + 16 * x, 32 * d, l), ds, dq[d]);
+        for (int d = 0; d < DB; ++d) dq[d] = mfma32(kt[x * DB + d], ds, dq[d]);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  St sk, sv;
-  sk.load(kp, a.k.st, t.len, a.K, tid);
-  sv.load(vp, a.v.st, t.len, a.V, tid);
-  sk.store(s_kv, t.len, a.K, tid);
-  sv.store(s_kv + TILE, t.len, a.V, tid);
-  if (CH < end) {
-    sk.load(kp + CH * a.k.st, a.k.st, t.len - CH, a.K, tid);
-    sv.load(vp + CH * a.v.st, a.v.st, t.len - CH, a.V, tid);
-  }
-  for (int j0 = 0; j0 < end; j0 += CH) {
-    const int cur = (j0 / CH) & 1;
+  const TileLoad<W, NW> lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
+  auto fetch = [&](bf16* sk, bf16* sv, int j0) {
+    lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, a.K, w);
+    lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, a.V, w);
+  };
+  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) {
+    wait_all_loads();
+    lk.clear(ck, t.len - j0, a.K, w, l);
+    lv.clear(cv, t.len - j0, a.V, w, l);
     lds_barrier();
-    if (j0 + CH < end) {
-      sk.store(s_kv + (2 - 2 * cur) * TILE, t.len - j0 - CH, a.K, tid);
-      sv.store(s_kv + (3 - 2 * cur) * TILE, t.len - j0 - CH, a.V, tid);
-      if (j0 + 2 * CH < end) {
-        sk.load(kp + (int64_t)(j0 + 2 * CH) * a.k.st, a.k.st, t.len - j0 - 2 * CH, a.K, tid);
-        sv.load(vp + (int64_t)(j0 + 2 * CH) * a.v.st, a.v.st, t.len - j0 - 2 * CH, a.V, tid);
-      }
-    }
-    const bf16 *ck = s_kv + 2 * cur * TILE, *cv = ck + TILE;
-    if (j0 + CH <= whole && j0 + CH <= t.len) { if (rows > 0) block(ck, cv, j0, std::false_type()); }
-    else if (j0 < wend) block(ck, cv, j0, std::true_type());
+    if (j0 + CH < end) fetch(nk, nv, j0 + CH);
+    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, part_c);
+  };
+  fetch(s_k0, s_v0, 0);
+  int j0 = 0;
+  for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
+    tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::false_type());
   }
-  lds_barrier();
+  for (; j0 < end; j0 += 2 * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
+    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
+  }
   if (rows > 0)
-    store_rows32<W>(dq, a.scale, s_kv + w * 32 * LD, attn_row<bf16>(a.dq, t.b, t.tok0 + w0, h), a.dq.st, rows, a.K, l);
+    store_rows32<W>(dq, a.scale, attn_row<bf16>(a.dq, t.b, t.tok0 + w0, h), a.dq.st, rows, a.K, l);
 }
 
-// dk, dv of NW x 32 keys, over the rows of all query heads that share the key head, one after the other.  A wave holds its 32 keys
-// and values as B operands: S = Q K^T and dP = dO V^T leave a lane with one key, P and dS as the B operands of dV^T += dO^T P and
-// dK^T += Q^T dS.  QR rows of q and do at a time lie in LDS, twice, with their lse and delta.  Rows behind the sequence come with
-// lse = infinity, so that their p is 0.
-template <int W, int NW, int QR, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NW * 64, W == 64 ? 2 : 1) void k_attn_bwd_dkv(const lmoe_attn_args a) {
-  constexpr int LD = W + LPAD, KS = W / 16, DB = W / 32, NT = NW * 64, KEYS = NW * 32, TILE = QR * LD;
-  typedef RowStage<QR, W, NT> St;
-  constexpr int AREA = 4 * TILE > KEYS * LD ? 4 * TILE : KEYS * LD;
-  __shared__ __attribute__((aligned(16))) bf16 s_qd[AREA];
-  __shared__ __attribute__((aligned(16))) float s_row[2][2][QR];          // lse, delta
+// dk, dv of NW x 32 keys, over the rows of all query heads that share the key head.  S = Q K^T and dP = dO V^T leave a lane with one
+// key, P and dS as the B operands of dV^T += dO^T P and dK^T += Q^T dS.  A wave holds its keys as B operands in registers; its
+// values, for which there is no room beside both sums, lie in LDS.  64 rows of q and do at a time lie there too, twice, with
+// their lse and delta.  Rows behind the sequence come with lse = infinity, so that their p is 0.
+// From the last row to the first, the heads of a row tile one after the other: the work-groups of a key head, whose rows begin at
+// different places but end at one, read the same tiles at about the same time, and an XCD's L2 holds them for all.
+template <int W, int NW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_args a) {
+  constexpr int KS = W / 16, DB = W / 32, KEYS = NW * 32, TILE = CH * W;
+  __shared__ __attribute__((aligned(1024))) bf16 s_q0[TILE], s_d0[TILE], s_q1[TILE], s_d1[TILE], s_v[KEYS * W];
+  __shared__ __attribute__((aligned(16))) float s_row[2][2][CH];          // lse, delta
   zero_behind<bf16>(a, a.dk, a.HKV, a.K);
   zero_behind<bf16>(a, a.dv, a.HKV, a.V);
   AttnTile t;
   int hk;
   if (!attn_place<KEYS>(a, a.HKV, false, hk, t)) return;
   const int G = a.HQ / a.HKV, tid = threadIdx.x, l = lane_id(), w = wave_id(), g = l >> 5;
-  const int w0 = t.r0 + 32 * w, keys = t.len - w0, key = w0 + (l & 31);
-  bf16x8 k[KS], v[KS];
+  const Swz<W> lane(l);
+  const int w0 = t.r0 + 32 * w, keys = t.len - w0, key_ = w0 + (l & 31);
+  bf16x8 k[KS];
+  bf16* const sv = s_v + 32 * w * W;                                      // (of the wave's own: no barrier)
+  rows32<W>(k, attn_row<bf16>(a.v, t.b, t.tok0 + min(w0, t.len - 1), hk), a.v.st, max(keys, 1), a.V, l);
+#pragma unroll
+  for (int j = 0; j < KS; ++j) *(bf16x8*)((char*)sv + (lane.rows ^ 32 * j)) = k[j];
   rows32<W>(k, attn_row<bf16>(a.k, t.b, t.tok0 + min(w0, t.len - 1), hk), a.k.st, max(keys, 1), a.K, l);
-  rows32<W>(v, attn_row<bf16>(a.v, t.b, t.tok0 + min(w0, t.len - 1), hk), a.v.st, max(keys, 1), a.V, l);
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) { dk[b] = zero16(); dv[b] = zero16(); }
-  const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;
-  const int wbegin = keys <= 0 ? t.len : a.causal && w0 >= t.prefix ? w0 : 0;             // the first row that sees one of the wave's keys
-  const int whole = a.causal && w0 + 32 > t.prefix ? w0 + 31 : 0;                         // from it on rows see all of them
+  const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;                              // the first row that sees a key of the tile
+  const int wbegin = keys <= 0 ? t.len : a.causal && w0 >= t.prefix ? w0 : 0;             // ... of the wave
+  const int whole = a.causal && t.r0 + KEYS > t.prefix ? t.r0 + KEYS - 1 : 0;             // from it on rows see all keys of the tile
 
-  auto block = [&](const Score<CAP, BIAS, true>& sc, const bf16* sq, const bf16* sd, const float* s_lse, const float* s_delta, int i0, auto part_c) {
+  auto block = [&](const Score16<CAP, BIAS>& sc, const bf16* sq, const bf16* sd, const float* s_lse, const float* s_delta, int i0, auto part_c) {
     constexpr bool PART = decltype(part_c)::value;
 #pragma unroll
-    for (int b = 0; b < QR / 32; ++b) {
-      if constexpr (W == 64) __builtin_amdgcn_sched_barrier(0);
+    for (int b = 0; b < CH / 32; ++b) {
+      const Swz<W> at = lane.fresh();
+      const int key = fresh_index(key_);
       f32x16 s = zero16(), dp = zero16();
+      bf16x8 f[2 * DB], y[2], z[2];
+      __builtin_amdgcn_sched_barrier(0);
+      // (pieces of two steps at a time: the registers hold no more)
 #pragma unroll
-      for (int j = 0; j < KS; ++j) s = mfma32(*(const bf16x8*)(sq + (32 * b + (l & 31)) * LD + 16 * j + 8 * g), k[j], s);
+      for (int j = 0; j < KS; j += 2) {
 #pragma unroll
-      for (int j = 0; j < KS; ++j) dp = mfma32(*(const bf16x8*)(sd + (32 * b + (l & 31)) * LD + 16 * j + 8 * g), v[j], dp);
+        for (int x = 0; x < 2; ++x) { f[x] = at.frag(sq, b, j + x); y[x] = at.frag(sd, b, j + x); z[x] = at.frag(sv, 0, j + x); }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { s = mfma32(f[x], k[j + x], s); dp = mfma32(y[x], z[x], dp); }
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const f32x4 lse = *(const f32x4*)(s_lse + 32 * b + row32(e) + 4 * g), delta = *(const f32x4*)(s_delta + 32 * b + row32(e) + 4 * g);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = i0 + 32 * b + row32(e + x) + 4 * g;
-          const float th = CAP ? sc.squash(s[e + x]) : 0.f;
-          float p = pow2<true>(sc.of(s[e + x], th, (float)(i - key)) - lse[x]);
+          float r;
+          const float u = sc(s[e + x], (float)(i - key), r);
+          float p = pow2<true>(__builtin_fmaf(u, sc.a, sc.b - lse[x]));
           if constexpr (PART) p = key <= i || key < t.prefix ? p : 0.f;
           float ds = p * (dp[e + x] - delta[x]);
-          if constexpr (CAP) ds *= __builtin_fmaf(-th, th, 1.0f);
+          if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
           s[e + x] = p;
           dp[e + x] = ds;
         }
       }
+      const bf16x8 p0 = frag_of_acc(s, 0), p1 = frag_of_acc(s, 1), ds0 = frag_of_acc(dp, 0), ds1 = frag_of_acc(dp, 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const bf16x8 p = frag_of_acc(s, x), ds = frag_of_acc(dp, x);
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int d = 0; d < DB; ++d) dv[d] = mfma32(frag32_t(sd, LD, 32 * b + 16 * x, 32 * d, l), p, dv[d]);
+        for (int d = 0; d < DB; ++d) f[x * DB + d] = at.frag_t(sd, 2 * b + x, d);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) dk[d] = mfma32(frag32_t(sq, LD, 32 * b + 16 * x, 32 * d, l), ds, dk[d]);
-      }
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) dv[d] = mfma32(f[x * DB + d], x ? p1 : p0, dv[d]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) f[x * DB + d] = at.frag_t(sq, 2 * b + x, d);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) dk[d] = mfma32(f[x * DB + d], x ? ds1 : ds0, dk[d]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // rows of the group's heads, one after the other: what is fetched next
-  struct { int h, i; } next = {hk * G, begin};
-  St sq, sd;
-  float stat = 0.f;
-  const int last = hk * G + G;
-  auto fetch = [&] {
-    sq.load(attn_row<bf16>(a.q, t.b, t.tok0 + next.i, next.h), a.q.st, t.len - next.i, a.K, tid);
-    sd.load(attn_row<bf16>(a.d_o, t.b, t.tok0 + next.i, next.h), a.d_o.st, t.len - next.i, a.V, tid);
-    if (tid < 2 * QR) {
-      const int i = next.i + tid % QR;
-      const float* p = (tid < QR ? a.lse : a.delta) + ((int64_t)t.b * a.HQ + next.h) * a.T + t.tok0;
-      stat = i < t.len ? p[i] : tid < QR ? INFINITY : 0.f;
+  const TileLoad<W, NW> lq(a.q.st, a.K, w, l), ld(a.d_o.st, a.V, w, l);
+  float lse_ = 0.f, delta_ = 0.f;
+  // rows from the last tile to the first, per tile the heads; n: tiles of rows and heads that are still to be fetched
+  const int first = begin / CH * CH;
+  int h = 0, i = (t.len - 1) / CH * CH, n = ((i - first) / CH + 1) * G;
+  auto fetch = [&](bf16* sq, bf16* sd) {
+    const int hq = hk * G + h;
+    lq.load(sq, attn_row<bf16>(a.q, t.b, t.tok0 + i, hq), a.q.st, t.len - i, a.K, w);
+    ld.load(sd, attn_row<bf16>(a.d_o, t.b, t.tok0 + i, hq), a.d_o.st, t.len - i, a.V, w);
+    if (tid < CH) {
+      const int64_t row = ((int64_t)t.b * a.HQ + hq) * a.T + t.tok0 + i;
+      const bool in = i + tid < t.len;
+      lse_ = in ? (a.lse + row)[(uint32_t)tid] : INFINITY;
+      delta_ = in ? (a.delta + row)[(uint32_t)tid] : 0.f;
     }
+    --n;
+    if (++h == G) { h = 0; i -= CH; }
   };
-  auto put = [&](int buf, int i) {
-    sq.store(s_qd + 2 * buf * TILE, t.len - i, a.K, tid);
-    sd.store(s_qd + (2 * buf + 1) * TILE, t.len - i, a.V, tid);
-    if (tid < 2 * QR) s_row[buf][tid / QR][tid % QR] = stat;
-  };
-  auto advance = [&] {
-    next.i += QR;
-    if (next.i >= t.len) { next.i = begin; ++next.h; }
-  };
-  fetch();
-  put(0, next.i);
-  int h = next.h, i0 = next.i, cur = 0;
-  advance();
-  if (next.h < last) fetch();
-  Score<CAP, BIAS, true> sc(a, h);
-  while (h < last) {
+  int hc = 0, ic = i;                    // the tile that is worked on
+  auto tile = [&](bf16* cq, bf16* cd, bf16* nq, bf16* nd, float (&rows)[2][CH], auto part_c) {
+    wait_all_loads();
+    lq.clear(cq, t.len - ic, a.K, w, l);
+    ld.clear(cd, t.len - ic, a.V, w, l);
+    if (tid < CH) { rows[0][tid] = lse_; rows[1][tid] = delta_; }
     lds_barrier();
-    const int hn = next.h, in = next.i;
-    if (hn < last) {
-      put(cur ^ 1, in);
-      advance();
-      if (next.h < last) fetch();
+    if (n > 0) fetch(nq, nd);
+    if (!decltype(part_c)::value || ic + CH > wbegin) {
+      const Score16<CAP, BIAS> sc(a, hk * G + hc);
+      block(sc, cq, cd, rows[0], rows[1], ic, part_c);
     }
-    const bf16 *cq = s_qd + 2 * cur * TILE, *cd = cq + TILE;
-    if (i0 + QR > wbegin) {
-      if (i0 >= whole) block(sc, cq, cd, s_row[cur][0], s_row[cur][1], i0, std::false_type());
-      else block(sc, cq, cd, s_row[cur][0], s_row[cur][1], i0, std::true_type());
-    }
-    if (hn != h && hn < last) sc = Score<CAP, BIAS, true>(a, hn);
-    h = hn; i0 = in; cur ^= 1;
+    if (++hc == G) { hc = 0; ic -= CH; }
+  };
+  if (!CAP && !BIAS && a.scale < 0.f) {
+#pragma unroll
+    for (int j = 0; j < KS; ++j) frag_negate(k[j]);
   }
-  lds_barrier();
+  fetch(s_q0, s_d0);
+  // pairs of tiles; those with rows that see only some of the keys last
+  const int all = n + 1, clear = whole > t.len ? 0 : ((t.len - 1) / CH - (whole + CH - 1) / CH + 1) * G;
+  int m = 0;
+  for (; m + 2 <= clear; m += 2) {
+    tile(s_q0, s_d0, s_q1, s_d1, s_row[0], std::false_type());
+    tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::false_type());
+  }
+  for (; m < all; m += 2) {
+    tile(s_q0, s_d0, s_q1, s_d1, s_row[0], std::true_type());
+    if (m + 1 < all) tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::true_type());
+  }
   if (keys > 0) {
-    store_rows32<W>(dv, 1.0f, s_qd + w * 32 * LD, attn_row<bf16>(a.dv, t.b, t.tok0 + w0, hk), a.dv.st, keys, a.V, l);
-    __builtin_amdgcn_wave_barrier();
-    store_rows32<W>(dk, a.scale, s_qd + w * 32 * LD, attn_row<bf16>(a.dk, t.b, t.tok0 + w0, hk), a.dk.st, keys, a.K, l);
+    store_rows32<W>(dv, 1.0f, attn_row<bf16>(a.dv, t.b, t.tok0 + w0, hk), a.dv.st, keys, a.V, l);
+    store_rows32<W>(dk, a.scale, attn_row<bf16>(a.dk, t.b, t.tok0 + w0, hk), a.dk.st, keys, a.K, l);
   }
 }
 

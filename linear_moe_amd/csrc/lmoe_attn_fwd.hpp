@@ -6,9 +6,6 @@
 // that a lane has one row of the scores (with its neighbour 32 lanes on): maximum, sum and scale factors are one number per
 // lane.  O^T += V^T P^T takes P^T from the registers it is in (the contraction index may be numbered freely) and V^T through
 // the transposing LDS read.
-//
-// The running maximum is raised (and O, sum scaled) only when a row exceeds it by more than 2^8: p <= 256 then, which changes
-// neither the relative rounding of p nor that of the sums.
 #pragma once
 #include "lmoe_attn.hpp"
 
@@ -36,16 +33,43 @@ __device__ __forceinline__ void halves(float x, float& lo, float& hi) {
 __device__ __forceinline__ float both_max(float x) { float a, b; halves(x, a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float both_sum(float x) { float a, b; halves(x, a, b); return a + b; }
 
-// A operand of a product that contracts over the rows of a tile (32 of its columns, from n0): the rows k0 + 4 g + {0..3} and
-// k0 + 8 + 4 g + {0..3}, g = lane / 32 -- the numbering in which elements 8 s .. 8 s + 7 of an accumulator block are a B operand.
-__device__ __forceinline__ bf16x8 frag32_t(const bf16* tile, int ld, int k0, int n0, int l) {
-  const int s = l & 15;
-  const bf16* p = tile + (k0 + 4 * (l >> 5) + (s >> 2)) * ld + n0 + 16 * ((l >> 4) & 1) + 4 * (s & 3);
-  typedef __attribute__((address_space(3))) bf16x4 lds_b4;
-  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4*)p);
-  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4*)(p + 8 * ld));
-  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// A tile of rows of W columns in LDS, without padding: the 16-byte piece c of row r lies at piece c ^ f(r), so that neither 16 lanes that
+// read one piece of 16 successive rows (A operands that contract over the columns) nor 32 lanes that read 64 bytes of four
+// successive rows (the transposing read, for those that contract over the rows) meet in a bank.  (Rows padded by 16 bytes: the
+// transposing reads lay in wait of each other for a quarter of the forward kernel's time.)
+// Both kinds of address are a number per lane, xor a constant, plus a constant.
+template <int W> struct Swz {
+  static constexpr int RB = W * 2;
+  static __device__ __forceinline__ int f(int r) { return W == 128 ? (r & 3) << 2 | (r >> 2 & 3) : (r >> 1 & 1) << 2 | (r >> 2 & 3); }
+  int rows, cols;       // byte offsets of the lane
+  __device__ __forceinline__ explicit Swz(int l) {
+    rows = (l & 31) * RB + ((l >> 5 ^ f(l & 15)) << 4);
+    const int s = l & 15, r = 4 * (l >> 5) + (s >> 2);
+    cols = r * RB + ((2 * (l >> 4 & 1) + (s >> 1 & 1) ^ f(r)) << 4) + 8 * (s & 1);
+  }
+  // the same numbers, in a form the compiler cannot prove invariant: what is formed from them stays in the iteration, in place of
+  // sixteen addresses in registers for the whole loop
+  __device__ __forceinline__ Swz fresh() const {
+    Swz x = *this;
+    x.rows = fresh_index(x.rows); x.cols = fresh_index(x.cols);
+    return x;
+  }
+  // row 32 b + l % 32, columns 16 j + 8 (l / 32) ..
+  __device__ __forceinline__ bf16x8 frag(const bf16* tile, int b, int j) const {
+    return *(const bf16x8*)((const char*)tile + (rows ^ 32 * j) + 32 * RB * b);
+  }
+  // 32 columns from 32 d, rows 16 x + 4 g + {0..3} and 16 x + 8 + 4 g + {0..3}, g = lane / 32 -- the numbering in which elements
+  // 8 s .. 8 s + 7 of an accumulator block are a B operand
+  __device__ __forceinline__ bf16x8 frag_t(const bf16* tile, int x, int d) const {
+    typedef __attribute__((address_space(3))) bf16x4 lds_b4;
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4*)((const char*)tile + (cols ^ 64 * d) + 16 * RB * x));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_b4*)((const char*)tile + (cols ^ 64 * d ^ 32) + 16 * RB * x + 8 * RB));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  static __device__ __forceinline__ const bf16* at(const bf16* tile, int r, int c) {
+    return (const bf16*)((const char*)tile + r * RB + ((c >> 3 ^ f(r)) << 4) + 2 * (c & 7));
+  }
+};
 // elements 8 s .. 8 s + 7 of an accumulator block as a B operand
 __device__ __forceinline__ bf16x8 frag_of_acc(const f32x16& x, int s) {
   bf16x8 f;
@@ -54,27 +78,36 @@ __device__ __forceinline__ bf16x8 frag_of_acc(const f32x16& x, int s) {
   return f;
 }
 
-// ROWS rows of W columns on their way from memory to LDS, NT threads: rows at or behind nvalid and columns at or behind D
-// arrive as zeros.
-template <int ROWS, int W, int NT> struct RowStage {
-  static constexpr int VPR = W / 8, PASSES = ROWS * VPR / NT, LD = W + LPAD;
-  static_assert(PASSES * NT == ROWS * VPR, "whole passes");
-  bf16x8 v[PASSES];
-  __device__ __forceinline__ void load(const bf16* src, int64_t stride, int nvalid, int D, int tid) {
+// Loads straight into LDS: a wave's instruction fills 1 KB, 16 bytes a lane, in the order of the lanes; the order of a row's pieces comes
+// from the addresses the lanes read.  NW waves share a tile of 64 rows.  Rows at or behind nvalid repeat the last one and columns
+// at or behind D the first, until clear() (once they have arrived) makes zeros of them.  Offsets in a full tile fit 32 bits: the
+// launch sees to it.
+typedef __attribute__((address_space(1))) const void global_void;
+typedef __attribute__((address_space(3))) void lds_void;
+template <int W, int NW> struct TileLoad {
+  static constexpr int VPR = W / 8, RPI = 64 / VPR, PASSES = CH / RPI / NW;      // pieces per row, rows per instruction
+  static_assert(PASSES * RPI * NW == CH && NW * RPI % 16 == 0, "whole passes; the order of the pieces repeats after 16 rows");
+  int row, col;      // of the lane in the first pass
+  uint32_t at;       // bytes
+  __device__ __forceinline__ TileLoad(int64_t stride, int D, int w, int l) {
+    row = w * RPI + l / VPR;
+    col = (l % VPR ^ Swz<W>::f(row)) * 8;
+    at = ((uint32_t)row * (uint32_t)stride + (col < D ? col : 0)) * 2;
+  }
+  __device__ __forceinline__ void load(bf16* tile, const bf16* src, int64_t stride, int nvalid, int D, int w) const {
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
-      const int idx = p * NT + tid, c = idx % VPR * 8;
-      const int r = min(idx / VPR, nvalid - 1);
-      v[p] = *(const bf16x8*)(src + (int64_t)r * stride + (c < D ? c : 0));
+      const char* g = (const char*)src + (int64_t)(p * NW * RPI) * stride * 2;
+      if (nvalid >= CH) g += at;
+      else g = (const char*)(src + (int64_t)min(row + p * NW * RPI, nvalid - 1) * stride + (col < D ? col : 0));
+      __builtin_amdgcn_global_load_lds((global_void*)g, (lds_void*)(tile + (p * NW + w) * 512), 16, 0, 0);
     }
   }
-  __device__ __forceinline__ void store(bf16* tile, int nvalid, int D, int tid) {
+  __device__ __forceinline__ void clear(bf16* tile, int nvalid, int D, int w, int l) const {
+    if (nvalid >= CH && D >= W) return;
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int idx = p * NT + tid, r = idx / VPR, c = idx % VPR * 8;
-      frag_keep_if(v[p], r < nvalid && c < D);
-      *(bf16x8*)(tile + r * LD + c) = v[p];
-    }
+    for (int p = 0; p < PASSES; ++p)
+      if (row + p * NW * RPI >= nvalid || col >= D) *(bf16x8*)(tile + (p * NW + w) * 512 + l * 8) = ET<bf16>::zero();
   }
 };
 
@@ -88,27 +121,23 @@ template <int W> __device__ __forceinline__ void rows32(bf16x8 (&f)[W / 16], con
   }
 }
 
-// a transposed block of 32 rows and W columns (acc[b]: columns 32 b ..) to rows [0, rows) and columns [0, D) of dst, through a
-// strip of LDS that only this wave uses
-template <int W> __device__ __forceinline__ void store_rows32(const f32x16 (&acc)[W / 32], float mul, bf16* strip, bf16* dst, int64_t stride, int rows, int D, int l) {
-  constexpr int LD = W + LPAD;
+// a transposed block of 32 rows and W columns (acc[b]: columns 32 b ..) to rows [0, rows) and columns [0, D) of dst: two lanes of a
+// row exchange halves, so that each has 16 adjacent bytes
+template <int W> __device__ __forceinline__ void store_rows32(const f32x16 (&acc)[W / 32], float mul, bf16* dst, int64_t stride, int rows, int D, int l) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  bf16* p = dst + (int64_t)(l & 31) * stride + 8 * (l >> 5);
 #pragma unroll
   for (int b = 0; b < W / 32; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      bf16x4 x;
+    for (int i = 0; i < 16; i += 8) {
+      bf16x8 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = (bf16)(acc[b][i + e] * mul);
-      *(bf16x4*)(strip + (l & 31) * LD + 32 * b + row32(i) + 4 * (l >> 5)) = x;
+      for (int e = 0; e < 8; ++e) x[e] = (bf16)(acc[b][i + e] * mul);
+      const u32x4 y = __builtin_bit_cast(u32x4, x);
+      const u32x2 lo = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false), hi = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
+      if ((l & 31) < rows && 32 * b + 2 * i + 8 * (l >> 5) < D) *(u32x4*)(p + 32 * b + 2 * i) = u32x4{lo[0], hi[0], lo[1], hi[1]};
     }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-  for (int i = 0; i < 32 * (W / 8) / 64; ++i) {
-    const int idx = i * 64 + l, r = idx / (W / 8), c = idx % (W / 8) * 8;
-    if (r < rows && c < D) *(bf16x8*)(dst + (int64_t)r * stride + c) = *(const bf16x8*)(strip + r * LD + c);
-  }
 }
 
 __device__ __forceinline__ bool all_finite(const bf16x8& f) {
@@ -122,20 +151,24 @@ __device__ __forceinline__ bool all_finite(const bf16x8& f) {
 
 template <int W, int NW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
-  constexpr int LD = W + LPAD, KS = W / 16, DB = W / 32, NT = NW * 64, ROWS = NW * 32, TILE = CH * LD;
-  typedef RowStage<CH, W, NT> St;
-  __shared__ __attribute__((aligned(16))) bf16 s_kv[4 * TILE];       // K, V of even tiles, of odd tiles
-  static_assert(ROWS * LD <= 4 * TILE, "the strips of the waves");
+  constexpr int KS = W / 16, DB = W / 32, ROWS = NW * 32, TILE = CH * W;
+  // (arrays of their own, so that the compiler sees that reads of one tile need not wait for loads into the other)
+  __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
   zero_behind<bf16>(a, a.o, a.HQ, a.V);
   AttnTile t;
   int h;
   if (!attn_place<ROWS>(a, a.HQ, true, h, t)) return;
-  const int hk = h / (a.HQ / a.HKV), tid = threadIdx.x, l = lane_id(), w = wave_id(), g = l >> 5;
-  const Score<CAP, BIAS, true> sc(a, h);
+  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 5;
+  const Score16<CAP, BIAS> sc(a, h);
+  const Swz<W> lane(l);
   const int w0 = t.r0 + 32 * w, rows = t.len - w0;                   // the wave's first row, its rows (may be none)
-  const int row = w0 + (l & 31);
+  const int row_ = w0 + (l & 31);
   bf16x8 q[KS];
   rows32<W>(q, attn_row<bf16>(a.q, t.b, t.tok0 + min(w0, t.len - 1), h), a.q.st, max(rows, 1), a.K, l);
+  if (sc.negate) {
+#pragma unroll
+    for (int j = 0; j < KS; ++j) frag_negate(q[j]);
+  }
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) o[b] = zero16();
@@ -143,45 +176,66 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
 
   const int end = a.causal ? min(t.len, max(t.r0 + ROWS, t.prefix)) : t.len;       // keys that some row sees
   const int wend = rows <= 0 ? 0 : a.causal ? min(t.len, max(w0 + 32, t.prefix)) : t.len;
-  const int whole = a.causal ? max(w0 + 1, t.prefix) : t.len;                      // keys before it: seen by all rows of the wave
+  const int whole = min(a.causal ? max(t.r0 + 1, t.prefix) : t.len, end);          // keys before it: seen by all rows
   const bf16* kp = attn_row<bf16>(a.k, t.b, t.tok0, hk);
   const bf16* vp = attn_row<bf16>(a.v, t.b, t.tok0, hk);
 
+  // Fragments are read a phase ahead of their products: the second half of K under the products of the first, half of V before the
+  // exponentials, the rest of it under the products of that half.
   auto block = [&](const bf16* sk, const bf16* sv, int j0, auto part_c) {
     constexpr bool PART = decltype(part_c)::value;                   // some of the tile's keys are hidden from some rows
+    const Swz<W> at = lane.fresh();
+    const int row = fresh_index(row_);
     f32x16 s[2];
+    bf16x8 kf[2][KS];
+    auto read_k = [&](int b) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = zero16();
+      for (int j = 0; j < KS; ++j) kf[b][j] = at.frag(sk, b, j);
+    };
+    bf16x8 vf[2][2 * DB];
+    auto read_v = [&](int b) {
 #pragma unroll
-      for (int j = 0; j < KS; ++j) s[b] = mfma32(*(const bf16x8*)(sk + (32 * b + (l & 31)) * LD + 16 * j + 8 * g), q[j], s[b]);
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vf[b][x * DB + d] = at.frag_t(sv, 2 * b + x, d);
+    };
+    read_k(0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_k(1);
+    s[0] = zero16(); s[1] = zero16();
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      s[0] = mfma32(kf[0][j], q[j], s[0]);
+      s[1] = mfma32(kf[1][j], q[j], s[1]);
     }
-    float mx = M_LOW;
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(0);
+    float mx = -INFINITY;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int j = j0 + 32 * b + row32(i) + 4 * g;
-        float x = sc.of(s[b][i], CAP ? sc.squash(s[b][i]) : 0.f, (float)(row - j));
+        float r, x = sc(s[b][i], (float)(row - j), r);
         if constexpr (PART) x = j < t.len && (!a.causal || j <= row || j < t.prefix) ? x : -INFINITY;
         s[b][i] = x;
         mx = fmaxf(mx, x);
       }
-    mx = both_max(mx);
-    if (__any(mx > m + 8.0f)) {
-      const float next = mx > m + 8.0f ? mx : m, f = pow2<true>(m - next);      // (row by row: what a row gets depends on no other)
-      m = next;
-      sum *= f;
-#pragma unroll
-      for (int b = 0; b < DB; ++b) o[b] *= f;
-    }
+    const float next = fmaxf(m, __builtin_fmaf(sc.a, both_max(mx), sc.b)), f = pow2<true>(m - next), off = sc.b - next;
+    m = next;
+    float part = 0.f;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[b][i] = pow2<true>(s[b][i] - m);
-        sum += s[b][i];
+        s[b][i] = pow2<true>(__builtin_fmaf(s[b][i], sc.a, off));
+        part += s[b][i];
       }
+    sum = __builtin_fmaf(sum, f, part);
+#pragma unroll
+    for (int b = 0; b < DB; ++b) o[b] *= f;
+    __builtin_amdgcn_sched_barrier(0);
+    read_v(1);
     bool finite = true;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -190,7 +244,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
         const bf16x8 p = frag_of_acc(s[b], x);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
-          bf16x8 v = frag32_t(sv, LD, 32 * b + 16 * x, 32 * d, l);
+          bf16x8 v = vf[b][x * DB + d];
           if constexpr (PART) {
             // A product with 0 for what the mask hides would make NaN of a hidden NaN or infinity: such numbers are left out here ...
             if (!all_finite(v)) {
@@ -202,6 +256,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
           o[d] = mfma32(v, p, o[d]);
         }
       }
+    __builtin_amdgcn_sched_barrier(0);
     if constexpr (PART) {
       if (__any(!finite)) {                                          // ... and reach the rows that see them by themselves
         for (int j = 0; j < CH; ++j) {
@@ -210,7 +265,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
           for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float x = (float)sv[j * LD + 32 * d + row32(i) + 4 * g];
+              const float x = (float)*at.at(sv, j, 32 * d + row32(i) + 4 * g);
               if (ok && !(fabsf(x) < INFINITY)) o[d][i] += x;
             }
         }
@@ -218,35 +273,35 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
     }
   };
 
-  St sk, sv;
-  sk.load(kp, a.k.st, t.len, a.K, tid);
-  sv.load(vp, a.v.st, t.len, a.V, tid);
-  sk.store(s_kv, t.len, a.K, tid);
-  sv.store(s_kv + TILE, t.len, a.V, tid);
-  if (CH < end) {
-    sk.load(kp + CH * a.k.st, a.k.st, t.len - CH, a.K, tid);
-    sv.load(vp + CH * a.v.st, a.v.st, t.len - CH, a.V, tid);
-  }
-  for (int j0 = 0; j0 < end; j0 += CH) {
-    const int cur = (j0 / CH) & 1;
+  const TileLoad<W, NW> lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
+  auto fetch = [&](bf16* sk, bf16* sv, int j0) {
+    lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, a.K, w);
+    lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, a.V, w);
+  };
+  // the tile from j0 on, in ck and cv; the next one goes to nk and nv
+  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) {
+    wait_all_loads();
+    lk.clear(ck, t.len - j0, a.K, w, l);
+    lv.clear(cv, t.len - j0, a.V, w, l);
     lds_barrier();
-    if (j0 + CH < end) {
-      sk.store(s_kv + (2 - 2 * cur) * TILE, t.len - j0 - CH, a.K, tid);
-      sv.store(s_kv + (3 - 2 * cur) * TILE, t.len - j0 - CH, a.V, tid);
-      if (j0 + 2 * CH < end) {
-        sk.load(kp + (int64_t)(j0 + 2 * CH) * a.k.st, a.k.st, t.len - j0 - 2 * CH, a.K, tid);
-        sv.load(vp + (int64_t)(j0 + 2 * CH) * a.v.st, a.v.st, t.len - j0 - 2 * CH, a.V, tid);
-      }
-    }
-    const bf16 *ck = s_kv + 2 * cur * TILE, *cv = ck + TILE;
-    if (j0 + CH <= whole && j0 + CH <= t.len) { if (rows > 0) block(ck, cv, j0, std::false_type()); }
-    else if (j0 < wend) block(ck, cv, j0, std::true_type());
+    if (j0 + CH < end) fetch(nk, nv, j0 + CH);
+    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, part_c);
+  };
+  fetch(s_k0, s_v0, 0);
+  // (two loops: with both bodies in one, the accumulators move between them)
+  int j0 = 0;
+  for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
+    tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::false_type());
+  }
+  for (; j0 < end; j0 += 2 * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
+    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
   }
   sum = both_sum(sum);
-  if (a.lse && g == 0 && row < t.len) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + row] = m + __builtin_amdgcn_logf(sum);
-  lds_barrier();
+  if (a.lse && g == 0 && row_ < t.len) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + row_] = m + __builtin_amdgcn_logf(sum);
   if (rows > 0)
-    store_rows32<W>(o, 1.0f / sum, s_kv + w * 32 * LD, attn_row<bf16>(a.o, t.b, t.tok0 + w0, h), a.o.st, rows, a.V, l);
+    store_rows32<W>(o, 1.0f / sum, attn_row<bf16>(a.o, t.b, t.tok0 + w0, h), a.o.st, rows, a.V, l);
 }
 
 }  // namespace lmoe
