@@ -89,10 +89,13 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  const TileLoad<W, NW> lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
+  typedef TileLoad<W, NW, CH> Load;
+  const Load lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
   auto fetch = [&](bf16* sk, bf16* sv, int j0) {
-    lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, a.K, w);
-    lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, a.V, w);
+#pragma unroll
+    for (int p = 0; p < Load::PASSES; ++p) lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, w, p);
+#pragma unroll
+    for (int p = 0; p < Load::PASSES; ++p) lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, w, p);
   };
   auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) {
     wait_all_loads();
@@ -205,15 +208,18 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
     }
   };
 
-  const TileLoad<W, NW> lq(a.q.st, a.K, w, l), ld(a.d_o.st, a.V, w, l);
+  typedef TileLoad<W, NW, CH> Load;
+  const Load lq(a.q.st, a.K, w, l), ld(a.d_o.st, a.V, w, l);
   float lse_ = 0.f, delta_ = 0.f;
   // rows from the last tile to the first, per tile the heads; n: tiles of rows and heads that are still to be fetched
   const int first = begin / CH * CH;
   int h = 0, i = (t.len - 1) / CH * CH, n = ((i - first) / CH + 1) * G;
   auto fetch = [&](bf16* sq, bf16* sd) {
     const int hq = hk * G + h;
-    lq.load(sq, attn_row<bf16>(a.q, t.b, t.tok0 + i, hq), a.q.st, t.len - i, a.K, w);
-    ld.load(sd, attn_row<bf16>(a.d_o, t.b, t.tok0 + i, hq), a.d_o.st, t.len - i, a.V, w);
+#pragma unroll
+    for (int p = 0; p < Load::PASSES; ++p) lq.load(sq, attn_row<bf16>(a.q, t.b, t.tok0 + i, hq), a.q.st, t.len - i, w, p);
+#pragma unroll
+    for (int p = 0; p < Load::PASSES; ++p) ld.load(sd, attn_row<bf16>(a.d_o, t.b, t.tok0 + i, hq), a.d_o.st, t.len - i, w, p);
     if (tid < CH) {
       const int64_t row = ((int64_t)t.b * a.HQ + hq) * a.T + t.tok0 + i;
       const bool in = i + tid < t.len;

@@ -84,27 +84,23 @@ __device__ __forceinline__ bf16x8 frag_of_acc(const f32x16& x, int s) {
 // launch sees to it.
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
-template <int W, int NW> struct TileLoad {
-  static constexpr int VPR = W / 8, RPI = 64 / VPR, PASSES = CH / RPI / NW;      // pieces per row, rows per instruction
-  static_assert(PASSES * RPI * NW == CH && NW * RPI % 16 == 0, "whole passes; the order of the pieces repeats after 16 rows");
+template <int W, int NW, int BK> struct TileLoad {
+  static constexpr int VPR = W / 8, RPI = 64 / VPR, PASSES = BK / RPI / NW;      // pieces per row, rows per instruction
+  static_assert(PASSES * RPI * NW == BK && NW * RPI % 16 == 0, "whole passes; the order of the pieces repeats after 16 rows");
   int row, col;      // of the lane in the first pass
-  uint32_t at;       // bytes
+  uint32_t first;    // bytes
   __device__ __forceinline__ TileLoad(int64_t stride, int D, int w, int l) {
     row = w * RPI + l / VPR;
     col = (l % VPR ^ Swz<W>::f(row)) * 8;
-    at = ((uint32_t)row * (uint32_t)stride + (col < D ? col : 0)) * 2;
+    first = (col < D ? col : 0) * 2;
   }
-  __device__ __forceinline__ void load(bf16* tile, const bf16* src, int64_t stride, int nvalid, int D, int w) const {
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const char* g = (const char*)src + (int64_t)(p * NW * RPI) * stride * 2;
-      if (nvalid >= CH) g += at;
-      else g = (const char*)(src + (int64_t)min(row + p * NW * RPI, nvalid - 1) * stride + (col < D ? col : 0));
-      __builtin_amdgcn_global_load_lds((global_void*)g, (lds_void*)(tile + (p * NW + w) * 512), 16, 0, 0);
-    }
+  // pass p of the tile from src on (nvalid >= 1)
+  __device__ __forceinline__ void load(bf16* tile, const bf16* src, int64_t stride, int nvalid, int w, int p) const {
+    const uint32_t r = min(row + p * NW * RPI, nvalid - 1);
+    __builtin_amdgcn_global_load_lds((global_void*)((const char*)src + (r * (uint32_t)(2 * stride) + first)), (lds_void*)(tile + (p * NW + w) * 512), 16, 0, 0);
   }
   __device__ __forceinline__ void clear(bf16* tile, int nvalid, int D, int w, int l) const {
-    if (nvalid >= CH && D >= W) return;
+    if (nvalid >= BK && D >= W) return;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p)
       if (row + p * NW * RPI >= nvalid || col >= D) *(bf16x8*)(tile + (p * NW + w) * 512 + l * 8) = ET<bf16>::zero();
@@ -151,7 +147,7 @@ __device__ __forceinline__ bool all_finite(const bf16x8& f) {
 
 template <int W, int NW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
-  constexpr int KS = W / 16, DB = W / 32, ROWS = NW * 32, TILE = CH * W;
+  constexpr int KS = W / 16, DB = W / 32, ROWS = NW * 32, BK = NW == 8 ? 128 : 64, TILE = BK * W;
   // (arrays of their own, so that the compiler sees that reads of one tile need not wait for loads into the other)
   __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
   zero_behind<bf16>(a, a.o, a.HQ, a.V);
@@ -182,7 +178,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
 
   // Fragments are read a phase ahead of their products: the second half of K under the products of the first, half of V before the
   // exponentials, the rest of it under the products of that half.
-  auto block = [&](const bf16* sk, const bf16* sv, int j0, auto part_c) {
+  auto block = [&](const bf16* sk, const bf16* sv, int j0, auto issue, auto part_c) __attribute__((always_inline)) {
     constexpr bool PART = decltype(part_c)::value;                   // some of the tile's keys are hidden from some rows
     const Swz<W> at = lane.fresh();
     const int row = fresh_index(row_);
@@ -207,7 +203,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
     for (int j = 0; j < KS; ++j) {
       s[0] = mfma32(kf[0][j], q[j], s[0]);
       s[1] = mfma32(kf[1][j], q[j], s[1]);
+      if (j == KS / 2) issue(0);
     }
+    issue(1);
     __builtin_amdgcn_sched_barrier(0);
     read_v(0);
     float mx = -INFINITY;
@@ -236,9 +234,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
     for (int b = 0; b < DB; ++b) o[b] *= f;
     __builtin_amdgcn_sched_barrier(0);
     read_v(1);
+    issue(2);
     bool finite = true;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b) {
+      if (b == 1) issue(3);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const bf16x8 p = frag_of_acc(s[b], x);
@@ -256,6 +256,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
           o[d] = mfma32(v, p, o[d]);
         }
       }
+    }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (PART) {
       if (__any(!finite)) {                                          // ... and reach the rows that see them by themselves
@@ -273,31 +274,47 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
     }
   };
 
-  const TileLoad<W, NW> lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
-  auto fetch = [&](bf16* sk, bf16* sv, int j0) {
-    lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, a.K, w);
-    lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, a.V, w);
+  typedef TileLoad<W, NW, BK> Load;
+  const Load lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
+  // instruction i of those that load the tile from j0 on
+  auto fetch = [&](bf16* sk, bf16* sv, int j0, int i) __attribute__((always_inline)) {
+    if (i < Load::PASSES) lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, w, i);
+    else lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, w, i - Load::PASSES);
   };
-  // the tile from j0 on, in ck and cv; the next one goes to nk and nv
-  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) {
+  // The tile from j0 on, in ck and cv; the next one goes to nk and nv.  Its loads are spread over the products: the CU takes 64 bytes
+  // a cycle, and waves that hand over a whole tile at once wait for each other in front of it.
+  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) __attribute__((always_inline)) {
+    constexpr int SUB = BK / CH, ALL = 2 * Load::PASSES, POINTS = 4 * SUB;
+    const int next = min(j0 + BK, (end - 1) / BK * BK);      // (behind the last tile: that one once more, so that there is no branch)
     wait_all_loads();
     lk.clear(ck, t.len - j0, a.K, w, l);
     lv.clear(cv, t.len - j0, a.V, w, l);
     lds_barrier();
-    if (j0 + CH < end) fetch(nk, nv, j0 + CH);
-    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, part_c);
+#pragma unroll
+    for (int y = 0; y < SUB; ++y) {
+      auto issue = [&](int point) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = (4 * y + point) * ALL / POINTS; e < (4 * y + point + 1) * ALL / POINTS; ++e) fetch(nk, nv, next, e);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      if (!decltype(part_c)::value || j0 + y * CH < wend) block(ck + y * CH * W, cv + y * CH * W, j0 + y * CH, issue, part_c);
+      else { issue(0); issue(1); issue(2); issue(3); }
+    }
   };
-  fetch(s_k0, s_v0, 0);
+#pragma unroll
+  for (int i = 0; i < 2 * Load::PASSES; ++i) fetch(s_k0, s_v0, 0, i);
   // (two loops: with both bodies in one, the accumulators move between them)
   int j0 = 0;
-  for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
+  for (; j0 + 2 * BK <= whole; j0 += 2 * BK) {
     tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
-    tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::false_type());
+    tile(s_k1, s_v1, s_k0, s_v0, j0 + BK, std::false_type());
   }
-  for (; j0 < end; j0 += 2 * CH) {
+  for (; j0 < end; j0 += 2 * BK) {
     tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
-    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
+    if (j0 + BK < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + BK, std::true_type());
   }
+  wait_all_loads();                      // (none may arrive in an LDS that is another's)
   sum = both_sum(sum);
   if (a.lse && g == 0 && row_ < t.len) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + row_] = m + __builtin_amdgcn_logf(sum);
   if (rows > 0)
