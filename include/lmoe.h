@@ -430,7 +430,7 @@ typedef struct lmoe_attn_args {
   int32_t B, T, HQ, HKV, K, V;
   int32_t N, NT;       /* sequences, 64-token chunks (as in lmoe_args)                 */
   float scale, softcap;
-  const int32_t *cu_seqlens, *chunk_map, *nt_dev;
+  const int32_t *cu_seqlens, *chunk_map, *nt_dev, *seq_order;      /* as in lmoe_args */
   const float* slopes;         /* [HQ] or NULL                                         */
   const int32_t* prefix_lens;  /* [N] or NULL (causal calls); beyond 0 .. length: clamped */
   lmoe_tensor q, k, v, o;      /* [B,T,HQ,K], [B,T,HKV,K], [B,T,HKV,V], [B,T,HQ,V]     */
@@ -438,7 +438,9 @@ typedef struct lmoe_attn_args {
   /* backward: o, lse of the forward call, d_o in; dq, dk, dv out (dk.ptr and dv.ptr NULL: dq alone)      */
   lmoe_tensor d_o, dq, dk, dv;
   float* delta;        /* [B,HQ,T] workspace: sum of d_o o per row                     */
+  float* ws;           /* workspace of lmoe_softmax_attn_bwd_floats fp32 numbers (0: may be NULL), 16-byte aligned */
 } lmoe_attn_args;
+int64_t lmoe_softmax_attn_bwd_floats(const lmoe_attn_args* a);
 int lmoe_softmax_attn_fwd(const lmoe_attn_args* a, void* stream);
 int lmoe_softmax_attn_bwd(const lmoe_attn_args* a, void* stream);
 

@@ -52,9 +52,9 @@ class AttnArgs(C.Structure):
     """``lmoe_attn_args`` -- field order must match include/lmoe.h."""
     _fields_ = ([(n, C.c_int32) for n in ("dtype", "causal", "B", "T", "HQ", "HKV", "K", "V", "N", "NT")]
                 + [("scale", C.c_float), ("softcap", C.c_float)]
-                + [(n, C.c_void_p) for n in ("cu_seqlens", "chunk_map", "nt_dev", "slopes", "prefix_lens")]
+                + [(n, C.c_void_p) for n in ("cu_seqlens", "chunk_map", "nt_dev", "seq_order", "slopes", "prefix_lens")]
                 + [(n, Tensor4) for n in ("q", "k", "v", "o")] + [("lse", C.c_void_p)]
-                + [(n, Tensor4) for n in ("d_o", "dq", "dk", "dv")] + [("delta", C.c_void_p)])
+                + [(n, Tensor4) for n in ("d_o", "dq", "dk", "dv")] + [("delta", C.c_void_p), ("ws", C.c_void_p)])
 
 
 class PagedArgs(C.Structure):
@@ -78,7 +78,7 @@ ENTRY_POINTS = (
     "lmoe_quad_featmap_bwd",
     "lmoe_fused_recurrent_fwd", "lmoe_trace_gdn_state_fwd", "lmoe_trace_simple_gla_fwd", "lmoe_mom_gather", "lmoe_mom_combine", "lmoe_mom_rowdot",
     "lmoe_mom_combine_bwd", "lmoe_mom_plan_ints", "lmoe_mom_plan", "lmoe_seq_tables",
-    "lmoe_softmax_attn_fwd", "lmoe_softmax_attn_bwd", "lmoe_paged_attn_floats", "lmoe_paged_attn_decode", "lmoe_paged_kv_append",
+    "lmoe_softmax_attn_fwd", "lmoe_softmax_attn_bwd", "lmoe_softmax_attn_bwd_floats", "lmoe_paged_attn_floats", "lmoe_paged_attn_decode", "lmoe_paged_kv_append",
 )
 
 _lib = None
@@ -178,6 +178,7 @@ def load() -> C.CDLL:
     lib.lmoe_seq_tables.restype = C.c_int
     for fn in (lib.lmoe_softmax_attn_fwd, lib.lmoe_softmax_attn_bwd):
         fn.argtypes, fn.restype = [C.POINTER(AttnArgs), C.c_void_p], C.c_int
+    lib.lmoe_softmax_attn_bwd_floats.argtypes, lib.lmoe_softmax_attn_bwd_floats.restype = [C.POINTER(AttnArgs)], C.c_int64
     for fn in (lib.lmoe_paged_attn_decode, lib.lmoe_paged_kv_append):
         fn.argtypes, fn.restype = [C.POINTER(PagedArgs), C.c_void_p], C.c_int
     lib.lmoe_paged_attn_floats.argtypes, lib.lmoe_paged_attn_floats.restype = [C.POINTER(PagedArgs)], C.c_int64

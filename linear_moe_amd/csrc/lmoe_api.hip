@@ -704,10 +704,15 @@ int lmoe_softmax_attn_fwd(const lmoe_attn_args* a, void* stream) {
   lmoe::launch_attn_fwd(*a, (hipStream_t)stream);
   return launched(op);
 }
+int64_t lmoe_softmax_attn_bwd_floats(const lmoe_attn_args* a) {
+  if (int r = check_attn(a, "lmoe_softmax_attn_bwd_floats", true)) return r;
+  return a->B == 0 || a->T == 0 ? 0 : lmoe::attn_bwd_floats(*a);
+}
 int lmoe_softmax_attn_bwd(const lmoe_attn_args* a, void* stream) {
   const char* op = "lmoe_softmax_attn_bwd";
   if (int r = check_attn(a, op, true)) return r;
   if (a->B == 0 || a->T == 0) return 0;
+  if (lmoe::attn_bwd_floats(*a) > 0 && (!a->ws || ((uintptr_t)a->ws & 15))) return fail(-11, "%s: ws must be a 16-byte aligned pointer", op);
   lmoe::launch_attn_bwd(*a, (hipStream_t)stream);
   return launched(op);
 }

@@ -15,6 +15,8 @@
 // accumulators are fp32.  Every row of a sequence is allowed to see itself (causal) or everything, so no row is empty;
 // rows that a mask leaves nothing of inside one tile are handled by a finite lowest maximum (M_LOW): 2^(-inf - M_LOW) = 0.
 #pragma once
+#include <algorithm>
+
 #include "lmoe_launch.hpp"
 #include "lmoe_seq.hpp"
 
@@ -81,18 +83,46 @@ struct AttnTile {
   int r0;          // first row of the tile inside the sequence
   int prefix;      // tokens every row of the sequence sees (causal calls)
 };
+// Packed input of at most so many sequences is walked through by every work-group (64 sequences at a time) to find its tile; of
+// more, the chunk map names 64-token chunks, a tile begins at every ROWS / 64-th of a sequence, and the work-groups of the
+// other chunks leave.
+constexpr int WALK_SEQS = 256;
+
 // The tile of ROWS rows (a multiple of 64) and the head of H that the work-group takes.  from_end: the last tiles first (with a
 // causal mask the late rows see most, and work-groups are dispatched in the order of their index; the keys of a causal call the
-// other way round).  The (row of the batch, head) pairs change fastest, so that neighbouring work-groups do alike; where
-// their number allows it, an XCD (work-groups go round them) keeps the same pairs, and with them the same keys in its L2.
-// Packed input: the chunk map names 64-token chunks; a tile begins at every ROWS / 64-th of a sequence, the work-groups of
-// the others leave.
+// other way round); of packed sequences the longest first, where the walk finds the tile.  The (row of the batch, head) pairs
+// change fastest, so that neighbouring work-groups do alike; where their number allows it, an XCD (work-groups go round them) keeps
+// the same pairs, and with them the same keys in its L2.  All lanes of the wave call it.
 template <int ROWS> __device__ __forceinline__ bool attn_place(const lmoe_attn_args& a, int H, bool from_end, int& h, AttnTile& t) {
   const int pairs = a.cu_seqlens ? H : a.B * H, i = blockIdx.x / pairs;
   int x = blockIdx.x - i * pairs;
   if (pairs % 8 == 0) x = (x & 7) * (pairs / 8) + (x >> 3);
   h = x % H;
-  if (a.cu_seqlens) {
+  if (a.cu_seqlens && a.N <= WALK_SEQS) {
+    int before = 0;
+    for (int n0 = 0;; n0 += 64) {
+      if (n0 >= a.N) return false;
+      const int y = n0 + lane_id(), n = y < a.N ? (a.seq_order ? a.seq_order[y] : y) : 0;
+      const int first = a.cu_seqlens[n], len = y < a.N ? a.cu_seqlens[n + 1] - first : 0, tiles = (len + ROWS - 1) / ROWS;
+      int upto = tiles;                                    // tiles of the sequences up to the lane's
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int z = __shfl_up(upto, d, 64);
+        if (lane_id() >= d) upto += z;
+      }
+      const uint64_t behind = __ballot(before + upto > i);
+      if (behind) {
+        const int l = __builtin_ctzll(behind), at = i - before - __shfl(upto, l, 64) + __shfl(tiles, l, 64);
+        t.n = __shfl(n, l, 64); t.tok0 = __shfl(first, l, 64); t.len = __shfl(len, l, 64);
+        t.r0 = (from_end ? (t.len + ROWS - 1) / ROWS - 1 - at : at) * ROWS;
+        t.n = __builtin_amdgcn_readfirstlane(t.n); t.tok0 = __builtin_amdgcn_readfirstlane(t.tok0);
+        t.len = __builtin_amdgcn_readfirstlane(t.len); t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
+        t.b = 0;
+        break;
+      }
+      before += __shfl(upto, 63, 64);
+    }
+  } else if (a.cu_seqlens) {
     const int nt = a.nt_dev ? as_const(a.nt_dev)[0] : a.NT;
     const int c = from_end ? nt - 1 - i : i;
     if (c < 0 || c >= nt) return false;
@@ -114,8 +144,10 @@ template <int ROWS> __device__ __forceinline__ bool attn_place(const lmoe_attn_a
   }
   return true;
 }
+// tiles of a call, all rows of the batch together (packed input: no fewer)
 template <int ROWS> inline int64_t attn_tiles(const lmoe_attn_args& a) {
-  return a.cu_seqlens ? (int64_t)a.NT : (int64_t)a.B * ((a.T + ROWS - 1) / ROWS);
+  if (!a.cu_seqlens) return (int64_t)a.B * ((a.T + ROWS - 1) / ROWS);
+  return a.N <= WALK_SEQS ? std::min<int64_t>((int64_t)a.T / ROWS + a.N, a.NT) : (int64_t)a.NT;
 }
 template <typename T> __device__ __forceinline__ T* attn_row(const lmoe_tensor& x, int b, int t, int h) {
   return (T*)x.ptr + (int64_t)b * x.sb + (int64_t)t * x.st + (int64_t)h * x.sh;

@@ -6,16 +6,16 @@
 
 namespace lmoe {
 
-// dq of NW x 32 rows; delta of those rows beside it.  As the forward kernel: S^T = K Q^T and dP^T = V dO^T leave a lane with one row,
+// dq of 128 rows; delta of those rows beside it.  As the forward kernel: S^T = K Q^T and dP^T = V dO^T leave a lane with one row,
 // whose lse and delta are one number, and dS^T as the B operand of dQ^T += K^T dS^T.
-template <int W, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
-  constexpr int KS = W / 16, DB = W / 32, ROWS = NW * 32, TILE = CH * W;
+template <int W, bool CAP, bool BIAS>
+__global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
+  constexpr int KS = W / 16, DB = W / 32, TILE = CH * W;
   __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
   zero_behind<bf16>(a, a.dq, a.HQ, a.K);
   AttnTile t;
   int h;
-  if (!attn_place<ROWS>(a, a.HQ, true, h, t)) return;
+  if (!attn_place<ATTN_ROWS>(a, a.HQ, true, h, t)) return;
   const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 5;
   const Score16<CAP, BIAS> sc(a, h);
   const int w0 = t.r0 + 32 * w, rows = t.len - w0, row_ = w0 + (l & 31);
@@ -40,13 +40,13 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
 #pragma unroll
   for (int b = 0; b < DB; ++b) dq[b] = zero16();
 
-  const int end = a.causal ? min(t.len, max(t.r0 + ROWS, t.prefix)) : t.len;
+  const int end = a.causal ? min(t.len, max(t.r0 + ATTN_ROWS, t.prefix)) : t.len;
   const int wend = rows <= 0 ? 0 : a.causal ? min(t.len, max(w0 + 32, t.prefix)) : t.len;
   const int whole = min(a.causal ? max(t.r0 + 1, t.prefix) : t.len, end);
   const bf16* kp = attn_row<bf16>(a.k, t.b, t.tok0, hk);
   const bf16* vp = attn_row<bf16>(a.v, t.b, t.tok0, hk);
 
-  auto block = [&](const bf16* sk, const bf16* sv, int j0, auto part_c) {
+  auto block = [&](const bf16* sk, const bf16* sv, int j0, auto issue, auto part_c) __attribute__((always_inline)) {
     constexpr bool PART = decltype(part_c)::value;
     const Swz<W> at = lane.fresh();
     const int row = fresh_index(row_);
@@ -63,6 +63,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
 #pragma unroll
         for (int x = 0; x < 2; ++x) { s = mfma32(kf[x], q[j + x], s); dp = mfma32(vf[x], d_o[j + x], dp); }
       }
+      issue(2 * b);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
         if constexpr (PART) ds = j < t.len && (!a.causal || j <= row || j < t.prefix) ? ds : 0.f;
         s[i] = ds;
       }
-      __builtin_amdgcn_sched_barrier(0);
+      issue(2 * b + 1);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const bf16x8 ds = frag_of_acc(s, x);
@@ -89,23 +90,14 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  typedef TileLoad<W, NW, CH> Load;
-  const Load lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
-  auto fetch = [&](bf16* sk, bf16* sv, int j0) {
-#pragma unroll
-    for (int p = 0; p < Load::PASSES; ++p) lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, w, p);
-#pragma unroll
-    for (int p = 0; p < Load::PASSES; ++p) lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, w, p);
+  KeyTiles<W> load(a, kp, vp, t.len, end, w, l);
+  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) __attribute__((always_inline)) {
+    load.arrived(ck, cv, j0);
+    auto issue = [&](int point) __attribute__((always_inline)) { load.next(nk, nv, j0, point); };
+    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, issue, part_c);
+    else { issue(0); issue(1); issue(2); issue(3); }
   };
-  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) {
-    wait_all_loads();
-    lk.clear(ck, t.len - j0, a.K, w, l);
-    lv.clear(cv, t.len - j0, a.V, w, l);
-    lds_barrier();
-    if (j0 + CH < end) fetch(nk, nv, j0 + CH);
-    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, part_c);
-  };
-  fetch(s_k0, s_v0, 0);
+  load.first(s_k0, s_v0);
   int j0 = 0;
   for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
     tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
@@ -115,8 +107,20 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
     tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
     if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
   }
+  wait_all_loads();                      // (none may arrive in an LDS that is another's)
   if (rows > 0)
     store_rows32<W>(dq, a.scale, attn_row<bf16>(a.dq, t.b, t.tok0 + w0, h), a.dq.st, rows, a.K, l);
+}
+
+// the lane's numbers of a transposed block of 32 rows, times mul, as they are: four adjacent columns at a time
+template <int W> __device__ __forceinline__ void store_sums(const f32x16 (&acc)[W / 32], float mul, float* row, int D, int g) {
+#pragma unroll
+  for (int b = 0; b < W / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int c = 32 * b + row32(i) + 4 * g;
+      if (c < D) *(f32x4*)(row + c) = f32x4{acc[b][i], acc[b][i + 1], acc[b][i + 2], acc[b][i + 3]} * mul;
+    }
 }
 
 // dk, dv of NW x 32 keys, over the rows of all query heads that share the key head.  S = Q K^T and dP = dO V^T leave a lane with one
@@ -125,13 +129,17 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args
 // their lse and delta.  Rows behind the sequence come with lse = infinity, so that their p is 0.
 // From the last row to the first, the heads of a row tile one after the other: the work-groups of a key head, whose rows begin at
 // different places but end at one, read the same tiles at about the same time, and an XCD's L2 holds them for all.
+// Where the keys are too few for the card, `parts` work-groups share them, each with its part of that stream, and leave fp32 sums
+// for k_attn_join (parts = 1: the gradients themselves).
 template <int W, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_args a) {
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_args a, int parts) {
   constexpr int KS = W / 16, DB = W / 32, KEYS = NW * 32, TILE = CH * W;
   __shared__ __attribute__((aligned(1024))) bf16 s_q0[TILE], s_d0[TILE], s_q1[TILE], s_d1[TILE], s_v[KEYS * W];
   __shared__ __attribute__((aligned(16))) float s_row[2][2][CH];          // lse, delta
-  zero_behind<bf16>(a, a.dk, a.HKV, a.K);
-  zero_behind<bf16>(a, a.dv, a.HKV, a.V);
+  if (blockIdx.y == 0) {
+    zero_behind<bf16>(a, a.dk, a.HKV, a.K);
+    zero_behind<bf16>(a, a.dv, a.HKV, a.V);
+  }
   AttnTile t;
   int hk;
   if (!attn_place<KEYS>(a, a.HKV, false, hk, t)) return;
@@ -151,7 +159,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   const int wbegin = keys <= 0 ? t.len : a.causal && w0 >= t.prefix ? w0 : 0;             // ... of the wave
   const int whole = a.causal && t.r0 + KEYS > t.prefix ? t.r0 + KEYS - 1 : 0;             // from it on rows see all keys of the tile
 
-  auto block = [&](const Score16<CAP, BIAS>& sc, const bf16* sq, const bf16* sd, const float* s_lse, const float* s_delta, int i0, auto part_c) {
+  auto block = [&](const Score16<CAP, BIAS>& sc, const bf16* sq, const bf16* sd, const float* s_lse, const float* s_delta, int i0, auto issue, auto part_c) __attribute__((always_inline)) {
     constexpr bool PART = decltype(part_c)::value;
 #pragma unroll
     for (int b = 0; b < CH / 32; ++b) {
@@ -168,7 +176,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
 #pragma unroll
         for (int x = 0; x < 2; ++x) { s = mfma32(f[x], k[j + x], s); dp = mfma32(y[x], z[x], dp); }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      issue(2 * b);
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
         const f32x4 lse = *(const f32x4*)(s_lse + 32 * b + row32(e) + 4 * g), delta = *(const f32x4*)(s_delta + 32 * b + row32(e) + 4 * g);
@@ -178,7 +186,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
           float r;
           const float u = sc(s[e + x], (float)(i - key), r);
           float p = pow2<true>(__builtin_fmaf(u, sc.a, sc.b - lse[x]));
-          if constexpr (PART) p = key <= i || key < t.prefix ? p : 0.f;
+          if constexpr (PART) p = !a.causal || key <= i || key < t.prefix ? p : 0.f;
           float ds = p * (dp[e + x] - delta[x]);
           if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
           s[e + x] = p;
@@ -195,7 +203,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int d = 0; d < DB; ++d) dv[d] = mfma32(f[x * DB + d], x ? p1 : p0, dv[d]);
-      __builtin_amdgcn_sched_barrier(0);
+      issue(2 * b + 1);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -208,60 +216,100 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
     }
   };
 
-  typedef TileLoad<W, NW, CH> Load;
+  typedef TileLoad<W, NW> Load;
   const Load lq(a.q.st, a.K, w, l), ld(a.d_o.st, a.V, w, l);
+  // The stream: tiles of 64 rows from the last to the first, per tile the heads.  Of it the work-group takes pieces m0 .. m1 - 1.
+  const int top = (t.len - 1) / CH, all = (top - begin / CH + 1) * G;
+  const int m0 = (int)((int64_t)all * blockIdx.y / parts), m1 = (int)((int64_t)all * (blockIdx.y + 1) / parts);
+  const int clear = whole > t.len ? 0 : (top - (whole + CH - 1) / CH + 1) * G;            // pieces whose rows see all keys, the first ones
+  struct Place { int m, h, i; } cur = {m0, m0 % G, (top - m0 / G) * CH}, next = cur;
+  auto advance = [&](Place& x) { ++x.m; if (++x.h == G) { x.h = 0; x.i -= CH; } };
   float lse_ = 0.f, delta_ = 0.f;
-  // rows from the last tile to the first, per tile the heads; n: tiles of rows and heads that are still to be fetched
-  const int first = begin / CH * CH;
-  int h = 0, i = (t.len - 1) / CH * CH, n = ((i - first) / CH + 1) * G;
-  auto fetch = [&](bf16* sq, bf16* sd) {
-    const int hq = hk * G + h;
-#pragma unroll
-    for (int p = 0; p < Load::PASSES; ++p) lq.load(sq, attn_row<bf16>(a.q, t.b, t.tok0 + i, hq), a.q.st, t.len - i, w, p);
-#pragma unroll
-    for (int p = 0; p < Load::PASSES; ++p) ld.load(sd, attn_row<bf16>(a.d_o, t.b, t.tok0 + i, hq), a.d_o.st, t.len - i, w, p);
+  auto piece = [&](bf16* sq, bf16* sd, int i) __attribute__((always_inline)) {
+    const int hq = hk * G + next.h;
+    if (i < Load::PASSES) lq.load(sq, attn_row<bf16>(a.q, t.b, t.tok0 + next.i, hq), a.q.st, t.len - next.i, w, i);
+    else ld.load(sd, attn_row<bf16>(a.d_o, t.b, t.tok0 + next.i, hq), a.d_o.st, t.len - next.i, w, i - Load::PASSES);
+  };
+  auto stats = [&] {
     if (tid < CH) {
-      const int64_t row = ((int64_t)t.b * a.HQ + hq) * a.T + t.tok0 + i;
-      const bool in = i + tid < t.len;
+      const int64_t row = ((int64_t)t.b * a.HQ + hk * G + next.h) * a.T + t.tok0 + next.i;
+      const bool in = next.i + tid < t.len;
       lse_ = in ? (a.lse + row)[(uint32_t)tid] : INFINITY;
       delta_ = in ? (a.delta + row)[(uint32_t)tid] : 0.f;
     }
-    --n;
-    if (++h == G) { h = 0; i -= CH; }
   };
-  int hc = 0, ic = i;                    // the tile that is worked on
-  auto tile = [&](bf16* cq, bf16* cd, bf16* nq, bf16* nd, float (&rows)[2][CH], auto part_c) {
+  auto tile = [&](bf16* cq, bf16* cd, bf16* nq, bf16* nd, float (&rows)[2][CH], auto part_c) __attribute__((always_inline)) {
     wait_all_loads();
-    lq.clear(cq, t.len - ic, a.K, w, l);
-    ld.clear(cd, t.len - ic, a.V, w, l);
+    lq.clear(cq, t.len - cur.i, a.K, w, l);
+    ld.clear(cd, t.len - cur.i, a.V, w, l);
     if (tid < CH) { rows[0][tid] = lse_; rows[1][tid] = delta_; }
     lds_barrier();
-    if (n > 0) fetch(nq, nd);
-    if (!decltype(part_c)::value || ic + CH > wbegin) {
-      const Score16<CAP, BIAS> sc(a, hk * G + hc);
-      block(sc, cq, cd, rows[0], rows[1], ic, part_c);
+    if (next.m + 1 < m1) advance(next);                  // (behind the last piece: that one once more, so that there is no branch)
+    stats();
+    auto issue = [&](int point) __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = point * 2 * Load::PASSES / 4; i < (point + 1) * 2 * Load::PASSES / 4; ++i) piece(nq, nd, i);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (!decltype(part_c)::value || cur.i + CH > wbegin) {
+      const Score16<CAP, BIAS> sc(a, hk * G + cur.h);
+      block(sc, cq, cd, rows[0], rows[1], cur.i, issue, part_c);
+    } else {
+      issue(0); issue(1); issue(2); issue(3);
     }
-    if (++hc == G) { hc = 0; ic -= CH; }
+    advance(cur);
   };
   if (!CAP && !BIAS && a.scale < 0.f) {
 #pragma unroll
     for (int j = 0; j < KS; ++j) frag_negate(k[j]);
   }
-  fetch(s_q0, s_d0);
-  // pairs of tiles; those with rows that see only some of the keys last
-  const int all = n + 1, clear = whole > t.len ? 0 : ((t.len - 1) / CH - (whole + CH - 1) / CH + 1) * G;
-  int m = 0;
-  for (; m + 2 <= clear; m += 2) {
+  if (m0 < m1) {
+#pragma unroll
+    for (int i = 0; i < 2 * Load::PASSES; ++i) piece(s_q0, s_d0, i);
+    stats();
+  }
+  const int whole_to = min(clear, m1);
+  while (cur.m + 2 <= whole_to) {
     tile(s_q0, s_d0, s_q1, s_d1, s_row[0], std::false_type());
     tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::false_type());
   }
-  for (; m < all; m += 2) {
+  while (cur.m < m1) {
     tile(s_q0, s_d0, s_q1, s_d1, s_row[0], std::true_type());
-    if (m + 1 < all) tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::true_type());
+    if (cur.m < m1) tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::true_type());
   }
-  if (keys > 0) {
+  wait_all_loads();                      // (none may arrive in an LDS that is another's)
+  if (keys <= 0) return;
+  if (parts == 1) {
     store_rows32<W>(dv, 1.0f, attn_row<bf16>(a.dv, t.b, t.tok0 + w0, hk), a.dv.st, keys, a.V, l);
     store_rows32<W>(dk, a.scale, attn_row<bf16>(a.dk, t.b, t.tok0 + w0, hk), a.dk.st, keys, a.K, l);
+  } else {
+    const int64_t rows = (int64_t)a.B * a.T * a.HKV, row = ((int64_t)t.b * a.T + t.tok0 + key_) * a.HKV + hk;
+    float* sums = a.ws + ((int64_t)blockIdx.y * rows + row) * (a.K + a.V);
+    if ((l & 31) < keys) {
+      store_sums<W>(dk, a.scale, sums, a.K, g);
+      store_sums<W>(dv, 1.0f, sums + a.K, a.V, g);
+    }
+  }
+}
+
+// dk and dv of a key head's rows from the sums of the parts: [parts][B, T, HKV][K + V]
+__global__ __launch_bounds__(NTHR) void k_attn_join(const lmoe_attn_args a, int parts) {
+  const int per = (a.K + a.V) / 4;
+  const int64_t rows = (int64_t)a.B * a.T * a.HKV, all = rows * per;
+  const int end = a.cu_seqlens ? as_const(a.cu_seqlens)[a.N] : a.T;
+  for (int64_t i = (int64_t)blockIdx.x * NTHR + threadIdx.x; i < all; i += (int64_t)gridDim.x * NTHR) {
+    const int64_t row = i / per;
+    const int c = (int)(i - row * per) * 4, h = (int)(row % a.HKV);
+    const int64_t tok = row / a.HKV;
+    const int b = (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
+    if (t >= end) continue;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; ++p) x += *(const f32x4*)(a.ws + ((int64_t)p * rows + row) * (a.K + a.V) + c);
+    bf16x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (bf16)x[e];
+    *(bf16x4*)(c < a.K ? attn_row<bf16>(a.dk, b, t, h) + c : attn_row<bf16>(a.dv, b, t, h) + c - a.K) = y;
   }
 }
 

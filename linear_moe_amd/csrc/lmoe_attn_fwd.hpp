@@ -1,8 +1,10 @@
 // Softmax attention, forward pass on 2-byte elements.
 //
-// A work-group of NW waves takes NW x 32 rows of one query head; 64 keys and values at a time lie in LDS, twice: while the
-// waves work on one pair of tiles, the next is written from registers into the other and the one after it is on its way
-// into those registers.  A wave works on S^T = K Q^T (32 x 32 blocks of v_mfma_f32_32x32x16_bf16, q held in registers), so
+// A work-group of four waves takes 128 rows of one query head; 64 keys and values at a time lie in LDS, twice: while the waves work
+// on one pair of tiles, the next is loaded into the other.  Two work-groups share a CU, and no barrier holds them to one
+// another: while one wave of a SIMD has the matrix unit, the other has the vector unit.  (One work-group of eight waves, 128 keys
+// between two barriers: 2 x 8192 tokens, 16 heads of 128, 580 us in place of 556, of 64 362 in place of 322; with its two
+// halves held half a step apart by barriers, and the tiles of one step in one phase, 20 % more.)  A wave works on S^T = K Q^T (32 x 32 blocks of v_mfma_f32_32x32x16_bf16, q held in registers), so
 // that a lane has one row of the scores (with its neighbour 32 lanes on): maximum, sum and scale factors are one number per
 // lane.  O^T += V^T P^T takes P^T from the registers it is in (the contraction index may be numbered freely) and V^T through
 // the transposing LDS read.
@@ -80,13 +82,13 @@ __device__ __forceinline__ bf16x8 frag_of_acc(const f32x16& x, int s) {
 
 // Loads straight into LDS: a wave's instruction fills 1 KB, 16 bytes a lane, in the order of the lanes; the order of a row's pieces comes
 // from the addresses the lanes read.  NW waves share a tile of 64 rows.  Rows at or behind nvalid repeat the last one and columns
-// at or behind D the first, until clear() (once they have arrived) makes zeros of them.  Offsets in a full tile fit 32 bits: the
+// at or behind D the first, until clear() (once they have arrived) makes zeros of them.  Offsets inside a tile fit 32 bits: the
 // launch sees to it.
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
-template <int W, int NW, int BK> struct TileLoad {
-  static constexpr int VPR = W / 8, RPI = 64 / VPR, PASSES = BK / RPI / NW;      // pieces per row, rows per instruction
-  static_assert(PASSES * RPI * NW == BK && NW * RPI % 16 == 0, "whole passes; the order of the pieces repeats after 16 rows");
+template <int W, int NW> struct TileLoad {
+  static constexpr int VPR = W / 8, RPI = 64 / VPR, PASSES = CH / RPI / NW;      // pieces per row, rows per instruction
+  static_assert(PASSES * RPI * NW == CH && NW * RPI % 16 == 0, "whole passes; the order of the pieces repeats after 16 rows");
   int row, col;      // of the lane in the first pass
   uint32_t first;    // bytes
   __device__ __forceinline__ TileLoad(int64_t stride, int D, int w, int l) {
@@ -100,10 +102,47 @@ template <int W, int NW, int BK> struct TileLoad {
     __builtin_amdgcn_global_load_lds((global_void*)((const char*)src + (r * (uint32_t)(2 * stride) + first)), (lds_void*)(tile + (p * NW + w) * 512), 16, 0, 0);
   }
   __device__ __forceinline__ void clear(bf16* tile, int nvalid, int D, int w, int l) const {
-    if (nvalid >= BK && D >= W) return;
+    if (nvalid >= CH && D >= W) return;
 #pragma unroll
     for (int p = 0; p < PASSES; ++p)
       if (row + p * NW * RPI >= nvalid || col >= D) *(bf16x8*)(tile + (p * NW + w) * 512 + l * 8) = ET<bf16>::zero();
+  }
+};
+
+// The tiles of 64 keys and values that a work-group of ATTN_WAVES waves goes through.  The loads of a tile are spread over the products
+// of the one before it, a quarter at each of four points: a CU takes 64 bytes a cycle, and waves that hand over a whole tile at once
+// wait for each other in front of it.
+constexpr int ATTN_WAVES = 4, ATTN_ROWS = 32 * ATTN_WAVES;
+template <int W> struct KeyTiles {
+  typedef TileLoad<W, ATTN_WAVES> Load;
+  const lmoe_attn_args& a;
+  const bf16 *kp, *vp;
+  int len, last, w, l;       // last: first key of the last tile
+  Load lk, lv;
+  __device__ __forceinline__ KeyTiles(const lmoe_attn_args& a, const bf16* kp, const bf16* vp, int len, int end, int w, int l)
+      : a(a), kp(kp), vp(vp), len(len), last((end - 1) / CH * CH), w(w), l(l), lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l) {}
+  __device__ __forceinline__ void piece(bf16* sk, bf16* sv, int j0, int i) const {
+    if (i < Load::PASSES) lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, len - j0, w, i);
+    else lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, len - j0, w, i - Load::PASSES);
+  }
+  __device__ __forceinline__ void first(bf16* sk, bf16* sv) const {
+#pragma unroll
+    for (int i = 0; i < 2 * Load::PASSES; ++i) piece(sk, sv, 0, i);
+  }
+  // of the tile behind the one from j0 on (behind the last one: that once more, so that there is no branch)
+  __device__ __forceinline__ void next(bf16* sk, bf16* sv, int j0, int point) const {
+    const int j = min(j0 + CH, last);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = point * 2 * Load::PASSES / 4; i < (point + 1) * 2 * Load::PASSES / 4; ++i) piece(sk, sv, j, i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // the tile from j0 on is whole, for all waves
+  __device__ __forceinline__ void arrived(bf16* sk, bf16* sv, int j0) const {
+    wait_all_loads();
+    lk.clear(sk, len - j0, a.K, w, l);
+    lv.clear(sv, len - j0, a.V, w, l);
+    lds_barrier();
   }
 };
 
@@ -145,15 +184,15 @@ __device__ __forceinline__ bool all_finite(const bf16x8& f) {
   return ok;
 }
 
-template <int W, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
-  constexpr int KS = W / 16, DB = W / 32, ROWS = NW * 32, BK = NW == 8 ? 128 : 64, TILE = BK * W;
+template <int W, bool CAP, bool BIAS>
+__global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
+  constexpr int KS = W / 16, DB = W / 32, TILE = CH * W;
   // (arrays of their own, so that the compiler sees that reads of one tile need not wait for loads into the other)
   __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
   zero_behind<bf16>(a, a.o, a.HQ, a.V);
   AttnTile t;
   int h;
-  if (!attn_place<ROWS>(a, a.HQ, true, h, t)) return;
+  if (!attn_place<ATTN_ROWS>(a, a.HQ, true, h, t)) return;
   const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 5;
   const Score16<CAP, BIAS> sc(a, h);
   const Swz<W> lane(l);
@@ -170,7 +209,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
   for (int b = 0; b < DB; ++b) o[b] = zero16();
   float m = M_LOW, sum = 0.f;
 
-  const int end = a.causal ? min(t.len, max(t.r0 + ROWS, t.prefix)) : t.len;       // keys that some row sees
+  const int end = a.causal ? min(t.len, max(t.r0 + ATTN_ROWS, t.prefix)) : t.len;       // keys that some row sees
   const int wend = rows <= 0 ? 0 : a.causal ? min(t.len, max(w0 + 32, t.prefix)) : t.len;
   const int whole = min(a.causal ? max(t.r0 + 1, t.prefix) : t.len, end);          // keys before it: seen by all rows
   const bf16* kp = attn_row<bf16>(a.k, t.b, t.tok0, hk);
@@ -274,45 +313,23 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_fwd(const lmoe_attn_args a)
     }
   };
 
-  typedef TileLoad<W, NW, BK> Load;
-  const Load lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l);
-  // instruction i of those that load the tile from j0 on
-  auto fetch = [&](bf16* sk, bf16* sv, int j0, int i) __attribute__((always_inline)) {
-    if (i < Load::PASSES) lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, t.len - j0, w, i);
-    else lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, t.len - j0, w, i - Load::PASSES);
-  };
-  // The tile from j0 on, in ck and cv; the next one goes to nk and nv.  Its loads are spread over the products: the CU takes 64 bytes
-  // a cycle, and waves that hand over a whole tile at once wait for each other in front of it.
+  KeyTiles<W> load(a, kp, vp, t.len, end, w, l);
   auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) __attribute__((always_inline)) {
-    constexpr int SUB = BK / CH, ALL = 2 * Load::PASSES, POINTS = 4 * SUB;
-    const int next = min(j0 + BK, (end - 1) / BK * BK);      // (behind the last tile: that one once more, so that there is no branch)
-    wait_all_loads();
-    lk.clear(ck, t.len - j0, a.K, w, l);
-    lv.clear(cv, t.len - j0, a.V, w, l);
-    lds_barrier();
-#pragma unroll
-    for (int y = 0; y < SUB; ++y) {
-      auto issue = [&](int point) __attribute__((always_inline)) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int e = (4 * y + point) * ALL / POINTS; e < (4 * y + point + 1) * ALL / POINTS; ++e) fetch(nk, nv, next, e);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      if (!decltype(part_c)::value || j0 + y * CH < wend) block(ck + y * CH * W, cv + y * CH * W, j0 + y * CH, issue, part_c);
-      else { issue(0); issue(1); issue(2); issue(3); }
-    }
+    load.arrived(ck, cv, j0);
+    auto issue = [&](int point) __attribute__((always_inline)) { load.next(nk, nv, j0, point); };
+    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, issue, part_c);
+    else { issue(0); issue(1); issue(2); issue(3); }
   };
-#pragma unroll
-  for (int i = 0; i < 2 * Load::PASSES; ++i) fetch(s_k0, s_v0, 0, i);
+  load.first(s_k0, s_v0);
   // (two loops: with both bodies in one, the accumulators move between them)
   int j0 = 0;
-  for (; j0 + 2 * BK <= whole; j0 += 2 * BK) {
+  for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
     tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
-    tile(s_k1, s_v1, s_k0, s_v0, j0 + BK, std::false_type());
+    tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::false_type());
   }
-  for (; j0 < end; j0 += 2 * BK) {
+  for (; j0 < end; j0 += 2 * CH) {
     tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
-    if (j0 + BK < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + BK, std::true_type());
+    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
   }
   wait_all_loads();                      // (none may arrive in an LDS that is another's)
   sum = both_sum(sum);

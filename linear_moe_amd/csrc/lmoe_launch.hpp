@@ -127,6 +127,7 @@ void launch_recurrent(const lmoe_args& a, bool delta, hipStream_t st);
 // softmax attention; bwd: dk, dv too where their pointers are given
 void launch_attn_fwd(const lmoe_attn_args& a, hipStream_t st);
 void launch_attn_bwd(const lmoe_attn_args& a, hipStream_t st);
+int64_t attn_bwd_floats(const lmoe_attn_args& a);                 // fp32 numbers of ws
 int64_t attn_groups(const lmoe_attn_args& a);                     // work-groups of the largest launch of a call
 // one token per sequence over a paged cache
 int64_t paged_attn_floats(const lmoe_paged_args& a);

@@ -45,6 +45,7 @@ struct Library {
   decltype(&lmoe_seq_tables) seq_tables;
   decltype(&lmoe_softmax_attn_fwd) attn_fwd;
   decltype(&lmoe_softmax_attn_bwd) attn_bwd;
+  decltype(&lmoe_softmax_attn_bwd_floats) attn_bwd_floats;
   decltype(&lmoe_paged_attn_floats) paged_floats;
   decltype(&lmoe_paged_attn_decode) paged_decode;
   decltype(&lmoe_paged_kv_append) paged_append;
@@ -781,7 +782,8 @@ struct Attn {
       NEED(PyTuple_Check(plan) && PyTuple_GET_SIZE(plan) == 7 && !head_first && B == 1);
       N = PyLong_AsLongLong(PyTuple_GET_ITEM(plan, 0)); NT = PyLong_AsLongLong(PyTuple_GET_ITEM(plan, 1));
       for (int i = 0; i < 5; ++i) NEED(plain_or_none(tables[i], PyTuple_GET_ITEM(plan, 2 + i), dev));
-      a.cu_seqlens = (const int32_t*)ptr(tables[0]); a.chunk_map = (const int32_t*)ptr(tables[1]); a.nt_dev = (const int32_t*)ptr(tables[4]);
+      a.cu_seqlens = (const int32_t*)ptr(tables[0]); a.chunk_map = (const int32_t*)ptr(tables[1]);
+      a.seq_order = (const int32_t*)ptr(tables[3]); a.nt_dev = (const int32_t*)ptr(tables[4]);
     }
     NEED(NT <= INT32_MAX);
     NEED(number(a.scale, o[3], (float)std::pow((double)K, -0.5)) && number(a.softcap, o[5], 0.f) && a.softcap >= 0.f && a.softcap < 3e38f);
@@ -840,7 +842,14 @@ PyObject* attn_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (keys) { dk = at::empty_like(c.k.detach()); dv = at::empty_like(c.v.detach()); }
     c.a.o = desc(out, c.head_first); c.a.lse = (float*)lse.data_ptr(); c.a.d_o = desc(dout, c.head_first); c.a.delta = (float*)delta.data_ptr();
     c.a.dq = desc(dq, c.head_first); c.a.dk = desc(dk, c.head_first); c.a.dv = desc(dv, c.head_first);
-    rc = lib.attn_bwd(&c.a, st);
+    const int64_t floats = lib.attn_bwd_floats(&c.a);
+    rc = (int)std::min<int64_t>(floats, 0);
+    if (rc == 0) {
+      Tensor ws;
+      if (floats) ws = at::empty({floats}, lse.options());
+      c.a.ws = (float*)ptr(ws);
+      rc = lib.attn_bwd(&c.a, st);
+    }
   }
   return result(rc, {dq, dk, dv});
   END_HANDLE_TH_ERRORS
@@ -951,7 +960,7 @@ PyObject* bind(PyObject*, PyObject* path) {
   get(l.swish_fwd, "lmoe_swish_gate_relayout_fwd"); get(l.swish_bwd, "lmoe_swish_gate_relayout_bwd");
   get(l.gates_partials, "lmoe_gdn_gates_partials"); get(l.gates_fwd, "lmoe_gdn_gates_fwd"); get(l.gates_bwd, "lmoe_gdn_gates_bwd");
   get(l.mom_gather, "lmoe_mom_gather"); get(l.mom_combine, "lmoe_mom_combine"); get(l.mom_combine_bwd, "lmoe_mom_combine_bwd");
-  get(l.attn_fwd, "lmoe_softmax_attn_fwd"); get(l.attn_bwd, "lmoe_softmax_attn_bwd"); get(l.paged_floats, "lmoe_paged_attn_floats");
+  get(l.attn_fwd, "lmoe_softmax_attn_fwd"); get(l.attn_bwd, "lmoe_softmax_attn_bwd"); get(l.attn_bwd_floats, "lmoe_softmax_attn_bwd_floats"); get(l.paged_floats, "lmoe_paged_attn_floats");
   get(l.paged_decode, "lmoe_paged_attn_decode"); get(l.paged_append, "lmoe_paged_kv_append");
   get(l.mom_plan_ints, "lmoe_mom_plan_ints"); get(l.mom_plan, "lmoe_mom_plan"); get(l.seq_tables, "lmoe_seq_tables");
   if (!all) return PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point", p);

@@ -96,7 +96,8 @@ def _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, pre
     a.B, a.T, a.HQ, a.HKV, a.K, a.V, a.N, a.NT = B, T, HQ, HKV, K, V, plan.N, plan.NT
     a.scale, a.softcap = scale, softcap
     if plan.cu is not None:
-        a.cu_seqlens, a.chunk_map, a.nt_dev = plan.cu.data_ptr(), plan.chunk_map.data_ptr(), ptr(plan.nt_dev)
+        a.cu_seqlens, a.chunk_map, a.nt_dev, a.seq_order = (plan.cu.data_ptr(), plan.chunk_map.data_ptr(), ptr(plan.nt_dev),
+                                                            ptr(plan.seq_order))
     a.slopes, a.prefix_lens = ptr(slopes), ptr(prefix)
     a.q, a.k, a.v, a.o = (_desc(x, head_first) for x in (q, k, v, o))
     a.lse = ptr(lse)
@@ -161,7 +162,12 @@ class _SoftmaxAttn(torch.autograd.Function):
             delta = torch.empty(B, HQ, T, dtype=torch.float32, device=dev)
             a.d_o, a.dq, a.dk, a.dv, a.delta = (_desc(do, head_first), _desc(dq, head_first), _desc(dk, head_first),
                                                 _desc(dv, head_first), delta.data_ptr())
-            _lib.check(_lib.load().lmoe_softmax_attn_bwd(C.byref(a), stream_ptr()), "softmax_attn backward")
+            lib = _lib.load()
+            floats = lib.lmoe_softmax_attn_bwd_floats(C.byref(a))
+            _lib.check(min(floats, 0), "softmax_attn backward")
+            ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+            a.ws = ptr(ws)
+            _lib.check(lib.lmoe_softmax_attn_bwd(C.byref(a), stream_ptr()), "softmax_attn backward")
         return (dq, dk, dv) + (None,) * 8
 
 

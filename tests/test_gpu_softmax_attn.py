@@ -42,6 +42,36 @@ def test_lengths(cuda, dtype, T, causal):
     run_and_check(cuda, *inputs(T, 2, T, 2, 1, 64, 64, dtype), causal=causal)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,HQ", [(129, 1), (321, 1), (321, 3), (700, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_odd_numbers_of_tiles(cuda, D, T, HQ, causal):
+    run_and_check(cuda, *inputs(T + HQ, 1, T, HQ, 1, D, D, BF16), causal=causal)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["causal", "whole", "prefix", "packed", "packed_prefix", "cap_bias"])
+def test_a_thousand_tokens(cuda, D, kind):
+    """Several work-groups to a sequence in every kernel, the gradients of keys shared by some, unequal documents."""
+    T, HQ, HKV = 1091, 2, 1
+    cu = [0, 3, 3, 131, 900, 1091]
+    kw = {"causal": {}, "whole": dict(causal=False), "prefix": dict(prefix=[700]), "packed": dict(cu=cu),
+          "packed_prefix": dict(cu=cu, prefix=[2, 5, 128, 130, 64]), "cap_bias": dict(softcap=4.0, slopes=alibi(2))}[kind]
+    run_and_check(cuda, *inputs(83, 1, T, HQ, HKV, D, D, BF16), **kw)
+
+
+@pytest.mark.parametrize("N", [64, 65, 256, 257])
+def test_many_documents(cuda, N):
+    """Up to and beyond the number of documents that a work-group looks through for its tile."""
+    lens = [(7 * n) % 5 + (130 if n % 50 == 9 else 0) for n in range(N)]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    x = inputs(89, 1, cu[-1] + 3, 2, 1, 64, 64, BF16)
+    x[3][:, cu[-1]:] = 0                        # (rows behind the last document)
+    run_and_check(cuda, *x, cu=cu)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("K,V", [(128, 128), (64, 128), (128, 64), (96, 96), (32, 8), (8, 128), (20, 13), (1, 1), (127, 72)])
 def test_head_dims(cuda, dtype, K, V):
