@@ -42,12 +42,11 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
 
   const int end = a.causal ? min(t.len, max(t.r0 + ATTN_ROWS, t.prefix)) : t.len;
   const int wend = rows <= 0 ? 0 : a.causal ? min(t.len, max(w0 + 32, t.prefix)) : t.len;
-  const int whole = min(a.causal ? max(t.r0 + 1, t.prefix) : t.len, end);
+  const int wwhole = a.causal ? min(t.len, max(w0 + 1, t.prefix)) : t.len;        // all rows of the wave see the keys before it
   const bf16* kp = attn_row<bf16>(a.k, t.b, t.tok0, hk);
   const bf16* vp = attn_row<bf16>(a.v, t.b, t.tok0, hk);
 
-  auto block = [&](const bf16* sk, const bf16* sv, int j0, auto issue, auto part_c) __attribute__((always_inline)) {
-    constexpr bool PART = decltype(part_c)::value;
+  auto block = [&](const bf16* sk, const bf16* sv, int j0, auto issue) __attribute__((always_inline)) {
     const Swz<W> at = lane.fresh();
     const int row = fresh_index(row_);
     bf16x8 kf[2], vf[2], kt[2 * DB];
@@ -76,8 +75,12 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
         const float u = sc(s[i], (float)(row - j), r);
         float ds = pow2<true>(__builtin_fmaf(u, sc.a, off)) * (dp[i] - delta);
         if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
-        if constexpr (PART) ds = j < t.len && (!a.causal || j <= row || j < t.prefix) ? ds : 0.f;
         s[i] = ds;
+      }
+      if (j0 + 32 * b + 32 > wwhole) {
+        const int sees = (a.causal ? min(t.len, max(row + 1, t.prefix)) : t.len) - (j0 + 32 * b + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = row32(i) < sees ? s[i] : 0.f;
       }
       issue(2 * b + 1);
 #pragma unroll
@@ -91,21 +94,16 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
   };
 
   KeyTiles<W> load(a, kp, vp, t.len, end, w, l);
-  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) __attribute__((always_inline)) {
+  auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0) __attribute__((always_inline)) {
     load.arrived(ck, cv, j0);
     auto issue = [&](int point) __attribute__((always_inline)) { load.next(nk, nv, j0, point); };
-    if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, issue, part_c);
+    if (j0 < wend) block(ck, cv, j0, issue);
     else { issue(0); issue(1); issue(2); issue(3); }
   };
   load.first(s_k0, s_v0);
-  int j0 = 0;
-  for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
-    tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
-    tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::false_type());
-  }
-  for (; j0 < end; j0 += 2 * CH) {
-    tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
-    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
+  for (int j0 = 0; j0 < end; j0 += 2 * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0);
+    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH);
   }
   wait_all_loads();                      // (none may arrive in an LDS that is another's)
   if (rows > 0)
@@ -157,10 +155,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   for (int b = 0; b < DB; ++b) { dk[b] = zero16(); dv[b] = zero16(); }
   const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;                              // the first row that sees a key of the tile
   const int wbegin = keys <= 0 ? t.len : a.causal && w0 >= t.prefix ? w0 : 0;             // ... of the wave
-  const int whole = a.causal && t.r0 + KEYS > t.prefix ? t.r0 + KEYS - 1 : 0;             // from it on rows see all keys of the tile
+  const int wwhole = a.causal && w0 + 32 > t.prefix ? w0 + 31 : 0;                         // from it on rows see all keys of the wave
 
-  auto block = [&](const Score16<CAP, BIAS>& sc, const bf16* sq, const bf16* sd, const float* s_lse, const float* s_delta, int i0, auto issue, auto part_c) __attribute__((always_inline)) {
-    constexpr bool PART = decltype(part_c)::value;
+  auto block = [&](const Score16<CAP, BIAS>& sc, const bf16* sq, const bf16* sd, const float* s_lse, const float* s_delta, int i0, auto issue) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < CH / 32; ++b) {
       const Swz<W> at = lane.fresh();
@@ -186,11 +183,18 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
           float r;
           const float u = sc(s[e + x], (float)(i - key), r);
           float p = pow2<true>(__builtin_fmaf(u, sc.a, sc.b - lse[x]));
-          if constexpr (PART) p = !a.causal || key <= i || key < t.prefix ? p : 0.f;
           float ds = p * (dp[e + x] - delta[x]);
           if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
           s[e + x] = p;
           dp[e + x] = ds;
+        }
+      }
+      if (i0 + 32 * b < wwhole) {
+        const int from = (key < t.prefix ? 0 : key) - (i0 + 32 * b + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[e] = row32(e) >= from ? s[e] : 0.f;
+          dp[e] = row32(e) >= from ? dp[e] : 0.f;
         }
       }
       const bf16x8 p0 = frag_of_acc(s, 0), p1 = frag_of_acc(s, 1), ds0 = frag_of_acc(dp, 0), ds1 = frag_of_acc(dp, 1);
@@ -221,7 +225,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   // The stream: tiles of 64 rows from the last to the first, per tile the heads.  Of it the work-group takes pieces m0 .. m1 - 1.
   const int top = (t.len - 1) / CH, all = (top - begin / CH + 1) * G;
   const int m0 = (int)((int64_t)all * blockIdx.y / parts), m1 = (int)((int64_t)all * (blockIdx.y + 1) / parts);
-  const int clear = whole > t.len ? 0 : (top - (whole + CH - 1) / CH + 1) * G;            // pieces whose rows see all keys, the first ones
   struct Place { int m, h, i; } cur = {m0, m0 % G, (top - m0 / G) * CH}, next = cur;
   auto advance = [&](Place& x) { ++x.m; if (++x.h == G) { x.h = 0; x.i -= CH; } };
   float lse_ = 0.f, delta_ = 0.f;
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
       delta_ = in ? (a.delta + row)[(uint32_t)tid] : 0.f;
     }
   };
-  auto tile = [&](bf16* cq, bf16* cd, bf16* nq, bf16* nd, float (&rows)[2][CH], auto part_c) __attribute__((always_inline)) {
+  auto tile = [&](bf16* cq, bf16* cd, bf16* nq, bf16* nd, float (&rows)[2][CH]) __attribute__((always_inline)) {
     wait_all_loads();
     lq.clear(cq, t.len - cur.i, a.K, w, l);
     ld.clear(cd, t.len - cur.i, a.V, w, l);
@@ -252,9 +255,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
       for (int i = point * 2 * Load::PASSES / 4; i < (point + 1) * 2 * Load::PASSES / 4; ++i) piece(nq, nd, i);
       __builtin_amdgcn_sched_barrier(0);
     };
-    if (!decltype(part_c)::value || cur.i + CH > wbegin) {
+    if (cur.i + CH > wbegin) {
       const Score16<CAP, BIAS> sc(a, hk * G + cur.h);
-      block(sc, cq, cd, rows[0], rows[1], cur.i, issue, part_c);
+      block(sc, cq, cd, rows[0], rows[1], cur.i, issue);
     } else {
       issue(0); issue(1); issue(2); issue(3);
     }
@@ -269,14 +272,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
     for (int i = 0; i < 2 * Load::PASSES; ++i) piece(s_q0, s_d0, i);
     stats();
   }
-  const int whole_to = min(clear, m1);
-  while (cur.m + 2 <= whole_to) {
-    tile(s_q0, s_d0, s_q1, s_d1, s_row[0], std::false_type());
-    tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::false_type());
-  }
   while (cur.m < m1) {
-    tile(s_q0, s_d0, s_q1, s_d1, s_row[0], std::true_type());
-    if (cur.m < m1) tile(s_q1, s_d1, s_q0, s_d0, s_row[1], std::true_type());
+    tile(s_q0, s_d0, s_q1, s_d1, s_row[0]);
+    if (cur.m < m1) tile(s_q1, s_d1, s_q0, s_d0, s_row[1]);
   }
   wait_all_loads();                      // (none may arrive in an LDS that is another's)
   if (keys <= 0) return;

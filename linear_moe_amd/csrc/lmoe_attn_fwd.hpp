@@ -248,13 +248,14 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn
     __builtin_amdgcn_sched_barrier(0);
     read_v(0);
     float mx = -INFINITY;
+    const int sees = (a.causal ? min(t.len, max(row + 1, t.prefix)) : t.len) - j0;           // (keys from j0 on)
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int j = j0 + 32 * b + row32(i) + 4 * g;
         float r, x = sc(s[b][i], (float)(row - j), r);
-        if constexpr (PART) x = j < t.len && (!a.causal || j <= row || j < t.prefix) ? x : -INFINITY;
+        if constexpr (PART) x = 32 * b + row32(i) < sees - 4 * g ? x : -INFINITY;
         s[b][i] = x;
         mx = fmaxf(mx, x);
       }
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn
     if constexpr (PART) {
       if (__any(!finite)) {                                          // ... and reach the rows that see them by themselves
         for (int j = 0; j < CH; ++j) {
-          const bool ok = j0 + j < t.len && (!a.causal || j0 + j <= row || j0 + j < t.prefix);
+          const bool ok = j < sees;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll
