@@ -1,4 +1,4 @@
-// Softmax attention: instances and dispatch (kernels in lmoe_attn_any.hpp).
+// Softmax attention: instances and dispatch.
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>
@@ -8,15 +8,41 @@
 
 namespace lmoe {
 
-int64_t attn_groups(const lmoe_attn_args& a) { return attn_tiles<CH>(a) * a.HQ; }
+// the kernels on 2-byte elements reach the rows of a tile by 32-bit offsets
+static bool fits16(const lmoe_attn_args& a) {
+  int64_t stride = 0;
+  for (const lmoe_tensor* x : {&a.q, &a.k, &a.v, &a.d_o}) stride = std::max(stride, std::abs(x->st));
+  return a.dtype == LMOE_BF16 && stride < (1 << 24);
+}
+// (without them: four strips to 64 rows, 512 threads each)
+int64_t attn_groups(const lmoe_attn_args& a) { return attn_tiles<CH>(a) * a.HQ * (fits16(a) ? 1 : 8); }
 
+// A strip of 32 rows reads each tile half as often as two of 16, which with 64 columns gains where the strips fill the card all the same:
+// 8 x 2048 tokens, 8 heads, forward 413 us in place of 448, backward 1307 in place of 1652; 2 x 1000, 4 heads on 2, 31 and 127 in
+// place of 25 and 100.  (With 128 columns there are no registers for 32.)
 template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
+  static bool wide(const lmoe_attn_args& a, int H) { return (int64_t)a.B * a.T * H / 32 >= 2 * cu_count(); }
+  template <int RB> static void fwd_strips(const lmoe_attn_args& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_attn_fwd_any<T, W, RB, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB)), dim3(64 * ANY_WAVES), 0, st, a);
+  }
+  template <int RB> static void dq_strips(const lmoe_attn_args& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_attn_bwd_dq_any<T, W, RB, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB)), dim3(64 * ANY_WAVES), 0, st, a);
+  }
+  template <int KB> static void dkv_strips(const lmoe_attn_args& a, hipStream_t st) {
+    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HKV * (CH / 16 / KB)), dim3(64 * ANY_KV_WAVES), 0, st, a);
+  }
   static void fwd(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_fwd_any<T, W, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HQ), dim3(NTHR), 0, st, a);
+    if constexpr (W == 64) { if (wide(a, a.HQ)) return fwd_strips<2>(a, st); }
+    fwd_strips<1>(a, st);
   }
   static void bwd(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_bwd_dq_any<T, W, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HQ), dim3(NTHR), 0, st, a);
-    if (a.dk.ptr) hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HKV), dim3(NTHR), 0, st, a);
+    if constexpr (W == 64) {
+      if (wide(a, a.HQ)) dq_strips<2>(a, st); else dq_strips<1>(a, st);
+      if (a.dk.ptr) { if (wide(a, a.HKV)) dkv_strips<2>(a, st); else dkv_strips<1>(a, st); }
+    } else {
+      dq_strips<1>(a, st);
+      if (a.dk.ptr) dkv_strips<1>(a, st);
+    }
   }
 };
 
@@ -24,14 +50,20 @@ template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
 // its 64 KB of values leave no second work-group room), four with 64 (two work-groups per CU).  2 x 8192 tokens of 16 heads,
 // backward: 8 and 4 waves, 128 columns 1.73 and 2.28 ms, 64 columns 1.04 and 0.94.
 constexpr int attn_kv_waves(int W) { return W == 128 ? 8 : 4; }
-// Work-groups that share the rows of a tile of keys (k_attn_bwd_dkv)
+// Work-groups that share the rows of a tile of keys (k_attn_bwd_dkv): so many that the card is full; and twice (64 columns: up to four
+// times) as many if each then still has 64 pieces or more, since the tiles of a causal call are unequal work, those of documents more
+// so.  Each part costs its sums' way through memory.  Backward, 128 columns, 16 heads on 4, with 1 / 2 / 4 / 8 parts: 1 x 1024 tokens
+// 243 / 155 / 106 / 86 us (16 parts: 83), 1 x 4096 929 / 549 / 365 / 384, 8 x 1024 275 / 203 / 214 / 265, 2 x 8192 2411 / 1844 /
+// 1911 / 2017; 16 on 16, 8 x 1024 162 / 278 / 420 / 686.  64 columns, 16 on 4, 2 x 8192 1316 / 1136 / 1034 / 1072.  16384 tokens in
+// documents of which the longest has 5990, 16 on 4 1635 / 1235 / 1229 / 1290, 16 on 16 1102 / 1280 / 1534 / 2094.
 static int attn_parts(const lmoe_attn_args& a) {
-  if (a.dtype != LMOE_BF16) return 1;
-  const int W = a.K <= 64 && a.V <= 64 ? 64 : 128, keys = 32 * attn_kv_waves(W), per_cu = W == 128 ? 1 : 2;
-  const int64_t rows = a.cu_seqlens ? a.T : (int64_t)a.B * a.T;
-  const int64_t groups = std::max<int64_t>(rows / keys, 1) * a.HKV, want = 2 * per_cu * (int64_t)cu_count() * (a.cu_seqlens ? 2 : 1);
-  const int64_t pieces = ((int64_t)a.T + CH - 1) / CH * (a.HQ / a.HKV);
-  return (int)std::max<int64_t>(1, std::min(std::min<int64_t>((want + groups - 1) / groups, 16), pieces / 4));
+  if (!fits16(a)) return 1;
+  const int W = a.K <= 64 && a.V <= 64 ? 64 : 128, keys = 32 * attn_kv_waves(W);
+  const int64_t groups = (a.cu_seqlens ? std::max<int64_t>(a.T / keys, 1) : (int64_t)a.B * ((a.T + keys - 1) / keys)) * a.HKV;
+  const int64_t full = (W == 128 ? 1 : 2) * (int64_t)cu_count(), pieces = ((int64_t)a.T + CH - 1) / CH * (a.HQ / a.HKV);
+  int64_t parts = (full + groups - 1) / groups;
+  for (int i = W == 128 ? 1 : 2; i > 0 && groups * parts < (W == 128 && !a.cu_seqlens ? 2 : 4) * full && pieces / parts >= 128; --i) parts *= 2;
+  return (int)std::max<int64_t>(1, std::min(std::min<int64_t>(parts, 16), pieces / 4));
 }
 int64_t attn_bwd_floats(const lmoe_attn_args& a) {
   const int parts = a.dk.ptr ? attn_parts(a) : 1;
@@ -62,11 +94,8 @@ template <template <typename, int, bool, bool> class F, typename T, int W> stati
 }
 static void attn(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;
-  // (the kernels on 2-byte elements reach the rows of a tile by 32-bit offsets)
-  int64_t stride = 0;
-  for (const lmoe_tensor* x : {&a.q, &a.k, &a.v, &a.d_o}) stride = std::max(stride, std::abs(x->st));
-  if (a.dtype == LMOE_BF16 && stride >= (1 << 24)) { if (narrow) by_score<AttnAny, bf16, 64>(a, bwd, st); else by_score<AttnAny, bf16, 128>(a, bwd, st); }
-  else if (a.dtype == LMOE_BF16) { if (narrow) by_score<Attn16, bf16, 64>(a, bwd, st); else by_score<Attn16, bf16, 128>(a, bwd, st); }
+  if (fits16(a)) { if (narrow) by_score<Attn16, bf16, 64>(a, bwd, st); else by_score<Attn16, bf16, 128>(a, bwd, st); }
+  else if (a.dtype == LMOE_BF16) { if (narrow) by_score<AttnAny, bf16, 64>(a, bwd, st); else by_score<AttnAny, bf16, 128>(a, bwd, st); }
   else if (narrow) by_score<AttnAny, float, 64>(a, bwd, st);
   else by_score<AttnAny, float, 128>(a, bwd, st);
 }

@@ -93,9 +93,10 @@ constexpr int WALK_SEQS = 256;
 // other way round); of packed sequences the longest first, where the walk finds the tile.  The (row of the batch, head) pairs
 // change fastest, so that neighbouring work-groups do alike; where their number allows it, an XCD (work-groups go round them) keeps
 // the same pairs, and with them the same keys in its L2.  All lanes of the wave call it.
-template <int ROWS> __device__ __forceinline__ bool attn_place(const lmoe_attn_args& a, int H, bool from_end, int& h, AttnTile& t) {
-  const int pairs = a.cu_seqlens ? H : a.B * H, i = blockIdx.x / pairs;
-  int x = blockIdx.x - i * pairs;
+// STRIP < ROWS: the tile's strips of so many rows have work-groups of their own, one after the other; false for one without rows.
+template <int ROWS, int STRIP = ROWS> __device__ __forceinline__ bool attn_place(const lmoe_attn_args& a, int H, bool from_end, int& h, AttnTile& t) {
+  const int pairs = a.cu_seqlens ? H : a.B * H, k = blockIdx.x / pairs, i = k / (ROWS / STRIP), strip = k % (ROWS / STRIP);
+  int x = blockIdx.x - k * pairs;
   if (pairs % 8 == 0) x = (x & 7) * (pairs / 8) + (x >> 3);
   h = x % H;
   if (a.cu_seqlens && a.N <= WALK_SEQS) {
@@ -137,6 +138,10 @@ template <int ROWS> __device__ __forceinline__ bool attn_place(const lmoe_attn_a
     t.r0 = (from_end ? (a.T + ROWS - 1) / ROWS - 1 - i : i) * ROWS;
     t.tok0 = 0; t.len = a.T;
   }
+  if constexpr (STRIP < ROWS) {
+    t.r0 += (from_end ? ROWS / STRIP - 1 - strip : strip) * STRIP;
+    if (t.r0 >= t.len) return false;
+  }
   t.prefix = 0;
   if (a.prefix_lens) {
     const int p = as_const(a.prefix_lens)[t.n];
@@ -166,15 +171,6 @@ template <typename T> __device__ __forceinline__ void zero_behind(const lmoe_att
       const int h = i / (D / ET<T>::VEC), c = i % (D / ET<T>::VEC) * ET<T>::VEC;
       *(typename ET<T>::vec*)((T*)x.ptr + (int64_t)t * x.st + (int64_t)h * x.sh + c) = z;
     }
-}
-
-// largest value of 16 neighbouring lanes (a row of the wave), in all of them
-__device__ __forceinline__ float row16_max(float x) {
-  x = fmaxf(x, dpp_or_zero<0xB1, 0xf>(x));
-  x = fmaxf(x, dpp_or_zero<0x4E, 0xf>(x));
-  x = fmaxf(x, dpp_or_zero<0x141, 0xf>(x));
-  x = fmaxf(x, dpp_or_zero<0x140, 0xf>(x));
-  return x;
 }
 
 }  // namespace lmoe

@@ -1,252 +1,387 @@
-// Softmax attention, the kernels for any element type: 64 rows against 64 rows, four waves of 16 rows, every operand of a
-// product in LDS.  The path of 4-byte elements.
+// Softmax attention with products in fp32: the kernels of 4-byte elements (and of 2-byte elements whose rows lie too far apart for
+// the kernels of those).
+//
+// A wave keeps 16 or 32 rows (dk, dv: keys) and goes through what they meet in tiles of 16 that it loads from memory straight into
+// registers: nothing is staged in LDS, and no wave waits for another before the end.  That works because a product of 16 x 16 x 4
+// adds over four numbers, one per lane group, and does not mind which ones.  Of a tile that is contracted over its columns (S, dP)
+// lane l takes row l % 16 and columns 16 j + 4 (l / 16) .. + 3; of one that is contracted over its rows (o, dq, dk, dv) rows
+// 4 (l / 16) + e and columns 64 x + 4 (l % 16) .. + 3: both 16 bytes per load, and the accumulator of S, whose lane holds rows
+// 4 (l / 16) + e of column l % 16, is the other operand of the second product as it stands.
+//
+// Bound: the fp32 matrix rate.  The waves of a work-group share its rows and take every KW-th tile, since short calls have few
+// rows and many tiles; their sums are joined in LDS in the order of the waves.  2 x 4096 tokens, 16 heads on 4 of 64, causal: forward
+// 0.70 ms, 98 TFLOP/s (a large product of this type reaches 154), backward 2.31 ms, 104 TFLOP/s with the scores formed twice.  2 x
+// 1000 tokens, 4 heads on 2: 25 and 100 us.  (64 rows against 64, every operand staged in LDS: 0.89, 3.40 ms, 80 and 304 us.)
+// 8 waves on the rows of a strip: 2 to 5 % more; tiles loaded two steps ahead: 3 % more.
 #pragma once
-#include "lmoe_attn.hpp"
+#include "lmoe_attn_fwd.hpp"
 
 namespace lmoe {
 
-// tile[64][LD] = rows [0, nvalid) of a matrix with D <= W columns, the rest zero.  Returns whether the thread saw a number that
-// is not finite.
-template <typename T, int W> __device__ __forceinline__ bool attn_load(T* tile, const T* src, int64_t stride, int nvalid, int D) {
-  constexpr int VEC = ET<T>::VEC, VPR = W / VEC, LD = W + LPAD;
-  typedef typename ET<T>::vec vec;
-  bool odd = false;
-#pragma unroll
-  for (int p = 0; p < CH * VPR / NTHR; ++p) {
-    const int idx = p * NTHR + threadIdx.x, r = idx / VPR, c = idx % VPR * VEC;
-    vec x = ET<T>::zero();
-    if (r < nvalid && c < D) x = *(const vec*)(src + (int64_t)r * stride + c);
-    *(vec*)(tile + r * LD + c) = x;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) odd |= !(fabsf(ET<T>::to_f(x[i])) < INFINITY);
-  }
-  return odd;
+template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
+  const typename ET<T>::vec4 x = *(const typename ET<T>::vec4*)p;
+  return f32x4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
 }
-// 16 rows of a wave's accumulators, times mul, to rows [0, nvalid) and columns [0, D) of dst
-template <typename T, int NB> __device__ __forceinline__ void attn_store(const f32x4 (&acc)[1][NB], T* dst, int64_t stride, int nvalid, int D, const float (&mul)[4]) {
-  const int l = lane_id();
+template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 x) {
+  typename ET<T>::vec4 y;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * (l >> 4) + i;
+  for (int i = 0; i < 4; ++i) y[i] = ET<T>::from_f(x[i]);
+  *(typename ET<T>::vec4*)p = y;
+}
+// the two lane groups of 16 (of each half), then the two halves
+__device__ __forceinline__ void pairs16(float x, float& a, float& b) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const u32x2 y = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  a = __builtin_bit_cast(float, (uint32_t)y[0]); b = __builtin_bit_cast(float, (uint32_t)y[1]);
+}
+__device__ __forceinline__ float column_max(float x) { float a, b; pairs16(x, a, b); return both_max(fmaxf(a, b)); }
+__device__ __forceinline__ float column_sum(float x) { float a, b; pairs16(x, a, b); return both_sum(a + b); }
+
+// of a tile of 16 rows, the lane's numbers: contracted over the columns
+template <int W> struct ByCols {
+  f32x4 x[W / 16];
+  template <typename T> __device__ __forceinline__ void load(const T* row, int D, int g) {      // row: l % 16 of the tile
 #pragma unroll
-    for (int ni = 0; ni < NB; ++ni) {
-      const int c = 16 * ni + (l & 15);
-      if (r < nvalid && c < D) dst[(int64_t)r * stride + c] = ET<T>::from_f(acc[0][ni][i] * mul[i]);
+    for (int j = 0; j < W / 16; ++j) {
+      const int c = 16 * j + 4 * g;
+      x[j] = load4(row + (c < D ? c : 0));
+      if (c >= D) x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
+};
+// ... contracted over the rows
+template <int W> struct ByRows {
+  f32x4 x[W / 64][4];
+  template <typename T> __device__ __forceinline__ void load(const T* m, int64_t stride, int r0, int last, int D, int l) {   // rows r0 .. (none behind last)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int b = 0; b < W / 64; ++b) {
+        const int c = 64 * b + 4 * (l & 15);
+        x[b][e] = load4(m + (int64_t)min(r0 + 4 * (l >> 4) + e, last) * stride + (c < D ? c : 0));
+        if (c >= D) x[b][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  }
+};
+// acc (lane: row of y l % 16, rows of x 4 (l / 16) + e) += x y^T
+template <int W> __device__ __forceinline__ f32x4 by_cols(const ByCols<W>& x, const ByCols<W>& y, f32x4 acc) {
+#pragma unroll
+  for (int j = 0; j < W / 16; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x[j][e], y.x[j][e], acc, 0, 0, 0);
+  return acc;
 }
-template <typename T, int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NTHR) void k_attn_fwd_any(const lmoe_attn_args a) {
-  constexpr int LD = W + LPAD, PLD = CH + LPAD, NB = W / 16;
-  __shared__ __attribute__((aligned(16))) T s_q[CH * LD], s_k[CH * LD], s_v[CH * LD], s_p[CH * PLD];
+// acc[b][d] (lane: column of p l % 16, columns 64 b + 4 (4 (l / 16) + e) + d of x) += x^T p
+template <int W> __device__ __forceinline__ void by_rows(f32x4 (&acc)[W / 64][4], const ByRows<W>& x, f32x4 p) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+#pragma unroll
+    for (int b = 0; b < W / 64; ++b)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) acc[b][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x[b][e][d], p[e], acc[b][d], 0, 0, 0);
+}
+template <int W> __device__ __forceinline__ void zero_sums(f32x4 (&acc)[W / 64][4]) {
+#pragma unroll
+  for (int b = 0; b < W / 64; ++b)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) acc[b][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+// such sums to row l % 16 of a tile of LDS
+template <int W> __device__ __forceinline__ void put_sums(const f32x4 (&acc)[W / 64][4], float* row, int l) {
+#pragma unroll
+  for (int b = 0; b < W / 64; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *(f32x4*)(row + 64 * b + 16 * (l >> 4) + 4 * e) = f32x4{acc[b][0][e], acc[b][1][e], acc[b][2][e], acc[b][3][e]};
+}
+
+constexpr int ANY_WAVES = 4;         // that share a strip of rows
+constexpr int ANY_KV_WAVES = 8;      // ... of keys
+
+template <typename T, int W, int RB, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_fwd_any(const lmoe_attn_args a) {
+  constexpr int KW = ANY_WAVES, LD = W + 4;
+  __shared__ __attribute__((aligned(16))) float s_o[KW][16 * RB][LD];
+  __shared__ float s_m[KW][16 * RB], s_sum[KW][16 * RB];
   zero_behind<T>(a, a.o, a.HQ, a.V);
   AttnTile t;
   int h;
-  if (!attn_place<CH>(a, a.HQ, true, h, t)) return;
-  const int hk = h / (a.HQ / a.HKV);
+  if (!attn_place<CH, 16 * RB>(a, a.HQ, true, h, t)) return;
+  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 4, last = t.len - 1;
   const Score<CAP, BIAS, false> sc(a, h);
-  const int l = lane_id(), w = wave_id(), row = t.r0 + 16 * w + 4 * (l >> 4);
-  const int rows = min(CH, t.len - t.r0);
-  attn_load<T, W>(s_q, attn_row<T>(a.q, t.b, t.tok0 + t.r0, h), a.q.st, rows, a.K);
-  f32x4 o[1][NB];
-  acc_zero(o);
-  float m[4], sum[4];
+  const int end = a.causal ? min(t.len, max(t.r0 + 16 * RB, t.prefix)) : t.len, whole = a.causal ? min(t.len, max(t.r0 + 1, t.prefix)) : t.len;
+  const T* kp = attn_row<T>(a.k, t.b, t.tok0, hk);
+  const T* vp = attn_row<T>(a.v, t.b, t.tok0, hk);
+  ByCols<W> q[RB], k;
+  f32x4 o[RB][W / 64][4];
+  int row[RB], sees[RB];                                           // sees: keys that the row sees
+  float m[RB], sum[RB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) { m[i] = M_LOW; sum[i] = 0.f; }
-  const int end = a.causal ? min(t.len, max(t.r0 + CH, t.prefix)) : t.len;
-  for (int j0 = 0; j0 < end; j0 += CH) {
-    const int keys = min(CH, t.len - j0);
-    __syncthreads();
-    attn_load<T, W>(s_k, attn_row<T>(a.k, t.b, t.tok0 + j0, hk), a.k.st, keys, a.K);
-    const bool odd = __syncthreads_or(attn_load<T, W>(s_v, attn_row<T>(a.v, t.b, t.tok0 + j0, hk), a.v.st, keys, a.V));
-    f32x4 s[1][4];
-    acc_zero(s);
-    gemm_nt<T, 1, 4>(s, s_q, LD, 16 * w, s_k, LD, 0, 0, W);
-    float old[4];
+  for (int r = 0; r < RB; ++r) {
+    row[r] = t.r0 + 16 * r + (l & 15);
+    sees[r] = a.causal ? min(t.len, max(row[r] + 1, t.prefix)) : t.len;
+    q[r].load(attn_row<T>(a.q, t.b, t.tok0 + min(row[r], last), h), a.K, g);
+    zero_sums<W>(o[r]);
+    m[r] = M_LOW;
+    sum[r] = 0.f;
+  }
+  auto keys = [&](int j0) { k.load(kp + (int64_t)min(j0 + (l & 15), last) * a.k.st, a.K, g); };
+  keys(16 * w);
+  for (int j0 = 16 * w; j0 < end; j0 += 16 * KW) {
+    ByRows<W> v;
+    v.load(vp, a.v.st, j0, last, a.V, l);
+    f32x4 s[RB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      old[i] = m[i];
-      float mx = M_LOW;
+    for (int r = 0; r < RB; ++r) s[r] = by_cols<W>(k, q[r], f32x4{0.f, 0.f, 0.f, 0.f});
+    keys(j0 + 16 * KW);                                            // (of the next step, under the rest of this one)
+    const bool part = j0 + 16 > whole;                             // some of the tile's keys are hidden from some rows
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        const int j = j0 + 16 * ni + (l & 15);
-        const float qk = s[0][ni][i];
-        const bool ok = j < t.len && (!a.causal || j <= row + i || j < t.prefix);
-        s[0][ni][i] = ok ? sc.of(qk, CAP ? sc.squash(qk) : 0.f, (float)(row + i - j)) : -INFINITY;
-        mx = fmaxf(mx, s[0][ni][i]);
+    for (int r = 0; r < RB; ++r) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[r][e] = sc.of(s[r][e], CAP ? sc.squash(s[r][e]) : 0.f, (float)(row[r] - j0 - 4 * g - e));
+        if (part) s[r][e] = e < sees[r] - j0 - 4 * g ? s[r][e] : -INFINITY;
+        mx = fmaxf(mx, s[r][e]);
       }
-      m[i] = fmaxf(m[i], row16_max(mx));
-      float ps = 0.f;
+      const float next = fmaxf(m[r], column_max(mx)), f = pow2<true>(m[r] - next);
+      m[r] = next;
+      float part = 0.f;
 #pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        const float p = pow2<false>(s[0][ni][i] - m[i]);
-        ps += p;
-        s[0][ni][i] = p;
+      for (int e = 0; e < 4; ++e) {
+        s[r][e] = pow2<true>(s[r][e] - next);
+        part += s[r][e];
       }
-      const float f = pow2<false>(old[i] - m[i]);
-      sum[i] = sum[i] * f + group_sum<16>(ps);
+      sum[r] = sum[r] * f + part;
 #pragma unroll
-      for (int ni = 0; ni < NB; ++ni) o[0][ni][i] *= f;
+      for (int b = 0; b < W / 64; ++b)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[r][b][d] *= f;
+    }
+    if (part) {
+      // A product with 0 for what the mask hides would make NaN of a hidden NaN or infinity: such numbers are left out here, and reach the
+      // rows that see them by themselves.
+      bool finite = true;
+#pragma unroll
+      for (int c = 0; c < W / 64; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const bool ok = fabsf(v.x[c][e][d]) < INFINITY;
+            finite &= ok;
+            v.x[c][e][d] = ok ? v.x[c][e][d] : 0.f;
+          }
+      if (__any(!finite))
+        for (int j = j0; j < min(j0 + 16, t.len); ++j)
+#pragma unroll
+          for (int c = 0; c < W / 64; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int col = 64 * c + 16 * g + 4 * e;
+              const f32x4 x = load4(vp + (int64_t)j * a.v.st + (col < a.V ? col : 0));
+#pragma unroll
+              for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) o[r][c][d][e] += j < sees[r] && col < a.V && !(fabsf(x[d]) < INFINITY) ? x[d] : 0.f;
+            }
     }
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni) acc_to_lds<T>(s[0][ni], s_p, PLD, 16 * w, 16 * ni);
-    __syncthreads();
-    // A product with 0 for what the mask hides would make NaN of a hidden NaN or infinity: such numbers are added by themselves to
-    // the rows that see them and leave the tile.
-    if (odd && a.causal && j0 + CH > t.r0) {
-      for (int j = 0; j < keys; ++j)
+    for (int r = 0; r < RB; ++r) by_rows<W>(o[r], v, s[r]);
+  }
 #pragma unroll
-        for (int ni = 0; ni < NB; ++ni) {
-          const float v = ET<T>::to_f(s_v[j * LD + 16 * ni + (l & 15)]);
-          if (fabsf(v) < INFINITY) continue;
+  for (int r = 0; r < RB; ++r) {
+    const float all = column_sum(sum[r]);
+    put_sums<W>(o[r], s_o[w][16 * r + (l & 15)], l);
+    if (g == 0) { s_m[w][16 * r + l] = m[r]; s_sum[w][16 * r + l] = all; }
+  }
+  __syncthreads();
+  for (int r = threadIdx.x >> 4; r < min(16 * RB, t.len - t.r0); r += 4 * KW) {
+    float f[KW], all = 0.f, top = M_LOW;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (j0 + j <= row + i || j0 + j < t.prefix) o[0][ni][i] += ET<T>::to_f(s_p[(16 * w + 4 * (l >> 4) + i) * PLD + j]) * v;
-        }
-      __syncthreads();
-      for (int i = threadIdx.x; i < CH * LD; i += NTHR)
-        if (!(fabsf(ET<T>::to_f(s_v[i])) < INFINITY)) s_v[i] = (T)0.0f;
-      __syncthreads();
+    for (int i = 0; i < KW; ++i) top = fmaxf(top, s_m[i][r]);
+#pragma unroll
+    for (int i = 0; i < KW; ++i) { f[i] = pow2<true>(s_m[i][r] - top); all += s_sum[i][r] * f[i]; }
+    const int c0 = 4 * (threadIdx.x & 15);
+    if (a.lse && c0 == 0) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + t.r0 + r] = top + __builtin_amdgcn_logf(all);
+    T* const out = attn_row<T>(a.o, t.b, t.tok0 + t.r0 + r, h);
+    const float inv = 1.0f / all;
+    for (int c = c0; c < a.V; c += 64) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KW; ++i) x += *(const f32x4*)&s_o[i][r][c] * f[i];
+      store4(out + c, x * inv);
     }
-    gemm<T, 1, NB, false, true>(o, s_p, PLD, 16 * w, s_v, LD, 0, 0, CH);
   }
-  float inv[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    inv[i] = 1.0f / sum[i];
-    if (a.lse && (l & 15) == 0 && row + i < t.len)
-      a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + row + i] = m[i] + log2f(sum[i]);
-  }
-  attn_store<T, NB>(o, attn_row<T>(a.o, t.b, t.tok0 + t.r0 + 16 * w, h), a.o.st, rows - 16 * w, a.V, inv);
 }
 
-// dq of 64 rows; delta of those rows beside it
-template <typename T, int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NTHR) void k_attn_bwd_dq_any(const lmoe_attn_args a) {
-  constexpr int LD = W + LPAD, PLD = CH + LPAD, NB = W / 16;
-  // (q, then keys; do, then values: the strips of q and do a wave needs stay with it as LDS tiles of their own)
-  __shared__ __attribute__((aligned(16))) T s_q[CH * LD], s_k[CH * LD], s_v[CH * LD], s_do[CH * LD], s_p[CH * PLD];
+// the sums of the waves' rows, times mul, to rows [0, nvalid) of dst
+template <typename T, int KW, int ROWS, int LD> __device__ __forceinline__ void join_rows(const float (&sums)[KW][ROWS][LD], int off, float mul, T* dst, int64_t stride, int nvalid, int D) {
+  for (int r = threadIdx.x >> 4; r < min(nvalid, ROWS); r += 4 * KW)
+    for (int c = 4 * (threadIdx.x & 15); c < D; c += 64) {
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KW; ++i) x += *(const f32x4*)&sums[i][r][off + c];
+      store4(dst + (int64_t)r * stride + c, x * mul);
+    }
+}
+
+// dq of a strip of rows; delta of those rows beside it
+template <typename T, int W, int RB, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmoe_attn_args a) {
+  constexpr int KW = ANY_WAVES, LD = W + 4;
+  __shared__ __attribute__((aligned(16))) float s_dq[KW][16 * RB][LD];
   zero_behind<T>(a, a.dq, a.HQ, a.K);
   AttnTile t;
   int h;
-  if (!attn_place<CH>(a, a.HQ, true, h, t)) return;
-  const int hk = h / (a.HQ / a.HKV);
+  if (!attn_place<CH, 16 * RB>(a, a.HQ, true, h, t)) return;
+  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 4, last = t.len - 1;
   const Score<CAP, BIAS, false> sc(a, h);
-  const int l = lane_id(), w = wave_id(), row = t.r0 + 16 * w + 4 * (l >> 4);
-  const int rows = min(CH, t.len - t.r0);
-  attn_load<T, W>(s_q, attn_row<T>(a.q, t.b, t.tok0 + t.r0, h), a.q.st, rows, a.K);
-  attn_load<T, W>(s_do, attn_row<T>(a.d_o, t.b, t.tok0 + t.r0, h), a.d_o.st, rows, a.V);
-  attn_load<T, W>(s_k, attn_row<T>(a.o, t.b, t.tok0 + t.r0, h), a.o.st, rows, a.V);
-  __syncthreads();
-  float lse[4], delta[4];
-  const int64_t at = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0;
+  const int end = a.causal ? min(t.len, max(t.r0 + 16 * RB, t.prefix)) : t.len, whole = a.causal ? min(t.len, max(t.r0 + 1, t.prefix)) : t.len;
+  const T* kp = attn_row<T>(a.k, t.b, t.tok0, hk);
+  const T* vp = attn_row<T>(a.v, t.b, t.tok0, hk);
+  ByCols<W> q[RB], d_o[RB], k, v;
+  f32x4 dq[RB][W / 64][4];
+  int row[RB], sees[RB];
+  float lse[RB], delta[RB];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 16 * w + 4 * (l >> 4) + i;
+  for (int r = 0; r < RB; ++r) {
+    row[r] = t.r0 + 16 * r + (l & 15);
+    sees[r] = a.causal ? min(t.len, max(row[r] + 1, t.prefix)) : t.len;
+    const int rc = min(row[r], last);
+    q[r].load(attn_row<T>(a.o, t.b, t.tok0 + rc, h), a.V, g);
+    d_o[r].load(attn_row<T>(a.d_o, t.b, t.tok0 + rc, h), a.V, g);
     float d = 0.f;
 #pragma unroll
-    for (int c = 0; c < W; c += 16) d += ET<T>::to_f(s_do[r * LD + c + (l & 15)]) * ET<T>::to_f(s_k[r * LD + c + (l & 15)]);
-    delta[i] = group_sum<16>(d);
-    lse[i] = a.lse[at + min(row + i, t.len - 1)];
-    if ((l & 15) == 0 && row + i < t.len) a.delta[at + row + i] = delta[i];
+    for (int j = 0; j < W / 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d = __builtin_fmaf(q[r].x[j][e], d_o[r].x[j][e], d);
+    delta[r] = column_sum(d);
+    const int64_t at = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + rc;
+    lse[r] = a.lse[at];
+    if (w == 0 && g == 0 && row[r] < t.len) a.delta[at] = delta[r];
+    q[r].load(attn_row<T>(a.q, t.b, t.tok0 + rc, h), a.K, g);
+    zero_sums<W>(dq[r]);
   }
-  f32x4 dq[1][NB];
-  acc_zero(dq);
-  const int end = a.causal ? min(t.len, max(t.r0 + CH, t.prefix)) : t.len;
-  for (int j0 = 0; j0 < end; j0 += CH) {
-    const int keys = min(CH, t.len - j0);
-    __syncthreads();
-    attn_load<T, W>(s_k, attn_row<T>(a.k, t.b, t.tok0 + j0, hk), a.k.st, keys, a.K);
-    attn_load<T, W>(s_v, attn_row<T>(a.v, t.b, t.tok0 + j0, hk), a.v.st, keys, a.V);
-    __syncthreads();
-    f32x4 s[1][4], dp[1][4];
-    acc_zero(s);
-    acc_zero(dp);
-    gemm_nt<T, 1, 4>(s, s_q, LD, 16 * w, s_k, LD, 0, 0, W);
-    gemm_nt<T, 1, 4>(dp, s_do, LD, 16 * w, s_v, LD, 0, 0, W);
+  auto keys = [&](int j0) {
+    const int64_t j = min(j0 + (l & 15), last);
+    k.load(kp + j * a.k.st, a.K, g);
+    v.load(vp + j * a.v.st, a.V, g);
+  };
+  keys(16 * w);
+  for (int j0 = 16 * w; j0 < end; j0 += 16 * KW) {
+    ByRows<W> kr;
+    kr.load(kp, a.k.st, j0, last, a.K, l);
+    f32x4 s[RB], dp[RB];
 #pragma unroll
-    for (int ni = 0; ni < 4; ++ni)
+    for (int r = 0; r < RB; ++r) {
+      s[r] = by_cols<W>(k, q[r], f32x4{0.f, 0.f, 0.f, 0.f});
+      dp[r] = by_cols<W>(v, d_o[r], f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    keys(j0 + 16 * KW);
+    const bool part = j0 + 16 > whole;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = j0 + 16 * ni + (l & 15);
-        const float qk = s[0][ni][i], th = CAP ? sc.squash(qk) : 0.f;
-        const bool ok = j < t.len && (!a.causal || j <= row + i || j < t.prefix);
-        float ds = pow2<false>(sc.of(qk, th, (float)(row + i - j)) - lse[i]) * (dp[0][ni][i] - delta[i]);
+    for (int r = 0; r < RB; ++r) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float th = CAP ? sc.squash(s[r][e]) : 0.f;
+        float ds = pow2<true>(sc.of(s[r][e], th, (float)(row[r] - j0 - 4 * g - e)) - lse[r]) * (dp[r][e] - delta[r]);
         if constexpr (CAP) ds *= 1.0f - th * th;
-        s[0][ni][i] = ok ? ds : 0.f;
+        s[r][e] = ds;
+        if (part) s[r][e] = e < sees[r] - j0 - 4 * g ? ds : 0.f;
       }
-#pragma unroll
-    for (int ni = 0; ni < 4; ++ni) acc_to_lds<T>(s[0][ni], s_p, PLD, 16 * w, 16 * ni);
-    __syncthreads();
-    gemm<T, 1, NB, false, true>(dq, s_p, PLD, 16 * w, s_k, LD, 0, 0, CH);
-  }
-  const float mul[4] = {a.scale, a.scale, a.scale, a.scale};
-  attn_store<T, NB>(dq, attn_row<T>(a.dq, t.b, t.tok0 + t.r0 + 16 * w, h), a.dq.st, rows - 16 * w, a.K, mul);
-}
-
-// dk, dv of 64 keys: over the rows of all query heads that share the key head, one after the other (no atomics)
-template <typename T, int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NTHR) void k_attn_bwd_dkv_any(const lmoe_attn_args a) {
-  constexpr int LD = W + LPAD, PLD = CH + LPAD, NB = W / 16;
-  __shared__ __attribute__((aligned(16))) T s_q[CH * LD], s_k[CH * LD], s_v[CH * LD], s_do[CH * LD], s_p[CH * PLD];
-  zero_behind<T>(a, a.dk, a.HKV, a.K);
-  zero_behind<T>(a, a.dv, a.HKV, a.V);
-  const int G = a.HQ / a.HKV;
-  AttnTile t;
-  int hk;
-  if (!attn_place<CH>(a, a.HKV, false, hk, t)) return;
-  const int l = lane_id(), w = wave_id(), key = t.r0 + 16 * w + 4 * (l >> 4);
-  const int keys = min(CH, t.len - t.r0);
-  attn_load<T, W>(s_k, attn_row<T>(a.k, t.b, t.tok0 + t.r0, hk), a.k.st, keys, a.K);
-  attn_load<T, W>(s_v, attn_row<T>(a.v, t.b, t.tok0 + t.r0, hk), a.v.st, keys, a.V);
-  f32x4 dk[1][NB], dv[1][NB];
-  acc_zero(dk);
-  acc_zero(dv);
-  const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;
-  for (int h = hk * G; h < (hk + 1) * G; ++h) {
-    const Score<CAP, BIAS, false> sc(a, h);
-    const int64_t at = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0;
-    for (int i0 = begin; i0 < t.len; i0 += CH) {
-      const int rows = min(CH, t.len - i0);
-      __syncthreads();
-      attn_load<T, W>(s_q, attn_row<T>(a.q, t.b, t.tok0 + i0, h), a.q.st, rows, a.K);
-      attn_load<T, W>(s_do, attn_row<T>(a.d_o, t.b, t.tok0 + i0, h), a.d_o.st, rows, a.V);
-      __syncthreads();
-      f32x4 s[1][4], dp[1][4];
-      acc_zero(s);
-      acc_zero(dp);
-      gemm_nt<T, 1, 4>(s, s_k, LD, 16 * w, s_q, LD, 0, 0, W);
-      gemm_nt<T, 1, 4>(dp, s_v, LD, 16 * w, s_do, LD, 0, 0, W);
-#pragma unroll
-      for (int ni = 0; ni < 4; ++ni) {
-        const int i = i0 + 16 * ni + (l & 15), ic = min(i, t.len - 1);
-        const float lse = a.lse[at + ic], delta = a.delta[at + ic];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = key + e;
-          const float qk = s[0][ni][e], th = CAP ? sc.squash(qk) : 0.f;
-          const bool ok = i < t.len && (!a.causal || j <= i || j < t.prefix);
-          const float p = ok ? pow2<false>(sc.of(qk, th, (float)(i - j)) - lse) : 0.f;
-          float ds = p * (dp[0][ni][e] - delta);
-          if constexpr (CAP) ds *= 1.0f - th * th;
-          s[0][ni][e] = p;
-          dp[0][ni][e] = ok ? ds : 0.f;
-        }
-      }
-#pragma unroll
-      for (int ni = 0; ni < 4; ++ni) acc_to_lds<T>(s[0][ni], s_p, PLD, 16 * w, 16 * ni);
-      __syncthreads();
-      gemm<T, 1, NB, false, true>(dv, s_p, PLD, 16 * w, s_do, LD, 0, 0, CH);
-      __syncthreads();
-#pragma unroll
-      for (int ni = 0; ni < 4; ++ni) acc_to_lds<T>(dp[0][ni], s_p, PLD, 16 * w, 16 * ni);
-      __syncthreads();
-      gemm<T, 1, NB, false, true>(dk, s_p, PLD, 16 * w, s_q, LD, 0, 0, CH);
+      by_rows<W>(dq[r], kr, s[r]);
     }
   }
-  const float one[4] = {1.f, 1.f, 1.f, 1.f}, mul[4] = {a.scale, a.scale, a.scale, a.scale};
-  attn_store<T, NB>(dv, attn_row<T>(a.dv, t.b, t.tok0 + t.r0 + 16 * w, hk), a.dv.st, keys - 16 * w, a.V, one);
-  attn_store<T, NB>(dk, attn_row<T>(a.dk, t.b, t.tok0 + t.r0 + 16 * w, hk), a.dk.st, keys - 16 * w, a.K, mul);
+#pragma unroll
+  for (int r = 0; r < RB; ++r) put_sums<W>(dq[r], s_dq[w][16 * r + (l & 15)], l);
+  __syncthreads();
+  join_rows<T>(s_dq, 0, a.scale, attn_row<T>(a.dq, t.b, t.tok0 + t.r0, h), a.dq.st, t.len - t.r0, a.K);
+}
+
+// dk, dv of a strip of keys, over the rows of all query heads that share the key head
+template <typename T, int W, int KB, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const lmoe_attn_args a) {
+  constexpr int KW = ANY_KV_WAVES, LD = 2 * W + 4;
+  __shared__ __attribute__((aligned(16))) float s_sum[KW][16 * KB][LD];
+  zero_behind<T>(a, a.dk, a.HKV, a.K);
+  zero_behind<T>(a, a.dv, a.HKV, a.V);
+  AttnTile t;
+  int hk;
+  if (!attn_place<CH, 16 * KB>(a, a.HKV, false, hk, t)) return;
+  const int G = a.HQ / a.HKV, l = lane_id(), w = wave_id(), g = l >> 4, last = t.len - 1;
+  const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0, tiles = (t.len - begin + 15) / 16;
+  const int whole = a.causal && t.r0 + 16 * KB > t.prefix ? t.r0 + 16 * KB - 1 : 0;        // from it on rows see all keys of the strip
+  ByCols<W> k[KB], v[KB], q, d_o;
+  f32x4 dk[KB][W / 64][4], dv[KB][W / 64][4];
+  int key[KB], from[KB];                                           // from: rows that see the key begin here
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    key[b] = t.r0 + 16 * b + (l & 15);
+    from[b] = a.causal && key[b] >= t.prefix ? key[b] : 0;
+    const int kc = min(key[b], last);
+    k[b].load(attn_row<T>(a.k, t.b, t.tok0 + kc, hk), a.K, g);
+    v[b].load(attn_row<T>(a.v, t.b, t.tok0 + kc, hk), a.V, g);
+    zero_sums<W>(dk[b]);
+    zero_sums<W>(dv[b]);
+  }
+  // The stream: the tiles of a head, head by head.  A wave takes every KW-th (behind the last: one of the last head, unused).
+  int x = w % tiles, h = w / tiles;
+  float lse[4], delta[4];
+  auto rows = [&] {
+    const int hq = hk * G + min(h, G - 1), i0 = begin + 16 * x;
+    const int64_t r = t.tok0 + min(i0 + (l & 15), last), at = ((int64_t)t.b * a.HQ + hq) * a.T + t.tok0;
+    q.load(attn_row<T>(a.q, t.b, 0, hq) + r * a.q.st, a.K, g);
+    d_o.load(attn_row<T>(a.d_o, t.b, 0, hq) + r * a.d_o.st, a.V, g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = min(i0 + 4 * g + e, last);
+      lse[e] = a.lse[at + i];
+      delta[e] = a.delta[at + i];
+    }
+  };
+  rows();
+  while (h < G) {
+    const int hq = hk * G + h, i0 = begin + 16 * x;
+    const Score<CAP, BIAS, false> sc(a, hq);
+    ByRows<W> y, z;
+    y.load(attn_row<T>(a.d_o, t.b, t.tok0, hq), a.d_o.st, i0, last, a.V, l);
+    f32x4 p[KB], ds[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      p[b] = by_cols<W>(q, k[b], f32x4{0.f, 0.f, 0.f, 0.f});
+      ds[b] = by_cols<W>(d_o, v[b], f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    z.load(attn_row<T>(a.q, t.b, t.tok0, hq), a.q.st, i0, last, a.K, l);
+    const bool part = i0 + 16 > t.len || i0 < whole;
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + 4 * g + e;
+        const bool ok = !part || (i < t.len && i >= from[b]);
+        const float th = CAP ? sc.squash(p[b][e]) : 0.f;
+        p[b][e] = ok ? pow2<true>(sc.of(p[b][e], th, (float)(i - key[b])) - lse[e]) : 0.f;
+        float d = p[b][e] * (ds[b][e] - delta[e]);
+        if constexpr (CAP) d *= 1.0f - th * th;
+        ds[b][e] = ok ? d : 0.f;
+      }
+    for (x += KW; x >= tiles && h < G; x -= tiles) ++h;
+    rows();                                                        // (of the next step, under the rest of this one)
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+      by_rows<W>(dv[b], y, p[b]);
+      by_rows<W>(dk[b], z, ds[b]);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    put_sums<W>(dk[b], s_sum[w][16 * b + (l & 15)], l);
+    put_sums<W>(dv[b], s_sum[w][16 * b + (l & 15)] + W, l);
+  }
+  __syncthreads();
+  join_rows<T>(s_sum, 0, a.scale, attn_row<T>(a.dk, t.b, t.tok0 + t.r0, hk), a.dk.st, t.len - t.r0, a.K);
+  join_rows<T>(s_sum, W, 1.0f, attn_row<T>(a.dv, t.b, t.tok0 + t.r0, hk), a.dv.st, t.len - t.r0, a.V);
 }
 
 }  // namespace lmoe

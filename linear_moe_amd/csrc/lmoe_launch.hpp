@@ -128,7 +128,7 @@ void launch_recurrent(const lmoe_args& a, bool delta, hipStream_t st);
 void launch_attn_fwd(const lmoe_attn_args& a, hipStream_t st);
 void launch_attn_bwd(const lmoe_attn_args& a, hipStream_t st);
 int64_t attn_bwd_floats(const lmoe_attn_args& a);                 // fp32 numbers of ws
-int64_t attn_groups(const lmoe_attn_args& a);                     // work-groups of the largest launch of a call
+int64_t attn_groups(const lmoe_attn_args& a);                     // work-groups of 256 threads in the largest launch of a call, at most
 // one token per sequence over a paged cache
 int64_t paged_attn_floats(const lmoe_paged_args& a);
 void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st);

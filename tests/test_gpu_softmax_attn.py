@@ -49,15 +49,43 @@ def test_odd_numbers_of_tiles(cuda, D, T, HQ, causal):
     run_and_check(cuda, *inputs(T + HQ, 1, T, HQ, 1, D, D, BF16), causal=causal)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("kind", ["causal", "whole", "prefix", "packed", "packed_prefix", "cap_bias"])
-def test_a_thousand_tokens(cuda, D, kind):
+def test_a_thousand_tokens(cuda, D, kind, dtype):
     """Several work-groups to a sequence in every kernel, the gradients of keys shared by some, unequal documents."""
     T, HQ, HKV = 1091, 2, 1
     cu = [0, 3, 3, 131, 900, 1091]
     kw = {"causal": {}, "whole": dict(causal=False), "prefix": dict(prefix=[700]), "packed": dict(cu=cu),
           "packed_prefix": dict(cu=cu, prefix=[2, 5, 128, 130, 64]), "cap_bias": dict(softcap=4.0, slopes=alibi(2))}[kind]
-    run_and_check(cuda, *inputs(83, 1, T, HQ, HKV, D, D, BF16), **kw)
+    run_and_check(cuda, *inputs(83, 1, T, HQ, HKV, D, D, dtype), **kw)
+
+
+@pytest.mark.parametrize("kind", ["causal", "whole", "packed_prefix", "cap_bias"])
+def test_float32_strips_of_32_rows(cuda, kind):
+    """(16 rows to a wave where there are few, 32 where 512 such strips fill the card)"""
+    B, T, H = (1, 2070, 8) if kind == "packed_prefix" else (2, 1035, 8)
+    kw = {"causal": {}, "whole": dict(causal=False), "packed_prefix": dict(cu=[0, 17, 17, 1300, 2066], prefix=[20, 5, 400, 0]),
+          "cap_bias": dict(softcap=4.0, slopes=alibi(8))}[kind]
+    x = inputs(97, B, T, H, H, 48, 64, F32)
+    if kind == "packed_prefix":
+        x[3][:, 2066:] = 0
+    run_and_check(cuda, *x, **kw)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_far_apart(cuda, causal):
+    """A row stride of 2^24 elements: the offsets inside a tile of 64 rows pass 31 bits."""
+    T, D = 67, 64
+    q, k, v, do = inputs(101, 1, T, 2, 1, D, D, BF16)
+    far = torch.zeros(T * 2 ** 24, dtype=BF16, device=cuda).as_strided((1, T, 1, D), (T * 2 ** 24, 2 ** 24, D, 1))
+    far.copy_(k)
+    want = softmax.attn(q, k, v, do=do, causal=causal)
+    leaves = [q.to(cuda).requires_grad_(True), far.detach().requires_grad_(True), v.to(cuda).requires_grad_(True)]
+    assert leaves[1].stride(1) == 2 ** 24
+    o = L.softmax_attn(*leaves, head_first=False, causal=causal)
+    for name, x in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, do.to(cuda)))):
+        softmax.check(x, want[name], name)
 
 
 @pytest.mark.parametrize("N", [64, 65, 256, 257])
