@@ -725,7 +725,7 @@ static int check_paged(const lmoe_paged_args* a, const char* op) {
     return fail(-3, "%s: head dims K=%d V=%d unsupported (at most 128, multiples of 16 bytes)", op, a->K, a->V);
   if (a->N < 0 || a->HKV <= 0 || a->P < 0 || a->M < 0 || a->S <= 0) return fail(-4, "%s: negative dimension", op);
   if (a->HKV > 65535 || a->N > 65535) return fail(-8, "%s: heads and N must be <= 65535", op);
-  if ((int64_t)a->M * a->S >= INT32_MAX) return fail(-8, "%s: %d pages of %d tokens per sequence: positions must stay below 2^31 - 1", op, a->M, a->S);
+  if ((int64_t)a->M * a->S > 1 << 30) return fail(-8, "%s: %d pages of %d tokens per sequence: positions must stay below 2^30", op, a->M, a->S);
   if (!a->kp.ptr || !a->vp.ptr || (!a->table && a->M > 0) || !a->lens) return fail(-7, "%s: pages, table and lens must not be null", op);
   if ((a->kn.ptr != nullptr) != (a->vn.ptr != nullptr)) return fail(-11, "%s: kn and vn go together", op);
   const lmoe_tensor* rows[] = {&a->q, &a->o, &a->kp, &a->vp, &a->kn, &a->vn};

@@ -72,9 +72,8 @@ template <bool CAP, bool BIAS> struct Score16 {
   }
 };
 
-template <bool FAST> __device__ __forceinline__ float pow2(float x) {
-  if constexpr (FAST) return __builtin_amdgcn_exp2f(x); else return exp2f(x);
-}
+// (to an ulp or so; what lies below 2^-126 becomes 0, beside numbers of which one is 1)
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The sequence a tile of rows lies in, and the tile's first row inside it
 struct AttnTile {

@@ -144,12 +144,12 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_fwd_any(const lmoe_a
         if (part) s[r][e] = e < sees[r] - j0 - 4 * g ? s[r][e] : -INFINITY;
         mx = fmaxf(mx, s[r][e]);
       }
-      const float next = fmaxf(m[r], column_max(mx)), f = pow2<true>(m[r] - next);
+      const float next = fmaxf(m[r], column_max(mx)), f = pow2(m[r] - next);
       m[r] = next;
       float part = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[r][e] = pow2<true>(s[r][e] - next);
+        s[r][e] = pow2(s[r][e] - next);
         part += s[r][e];
       }
       sum[r] = sum[r] * f + part;
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_fwd_any(const lmoe_a
 #pragma unroll
     for (int i = 0; i < KW; ++i) top = fmaxf(top, s_m[i][r]);
 #pragma unroll
-    for (int i = 0; i < KW; ++i) { f[i] = pow2<true>(s_m[i][r] - top); all += s_sum[i][r] * f[i]; }
+    for (int i = 0; i < KW; ++i) { f[i] = pow2(s_m[i][r] - top); all += s_sum[i][r] * f[i]; }
     const int c0 = 4 * (threadIdx.x & 15);
     if (a.lse && c0 == 0) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + t.r0 + r] = top + __builtin_amdgcn_logf(all);
     T* const out = attn_row<T>(a.o, t.b, t.tok0 + t.r0 + r, h);
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmo
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float th = CAP ? sc.squash(s[r][e]) : 0.f;
-        float ds = pow2<true>(sc.of(s[r][e], th, (float)(row[r] - j0 - 4 * g - e)) - lse[r]) * (dp[r][e] - delta[r]);
+        float ds = pow2(sc.of(s[r][e], th, (float)(row[r] - j0 - 4 * g - e)) - lse[r]) * (dp[r][e] - delta[r]);
         if constexpr (CAP) ds *= 1.0f - th * th;
         s[r][e] = ds;
         if (part) s[r][e] = e < sees[r] - j0 - 4 * g ? ds : 0.f;
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const
         const int i = i0 + 4 * g + e;
         const bool ok = !part || (i < t.len && i >= from[b]);
         const float th = CAP ? sc.squash(p[b][e]) : 0.f;
-        p[b][e] = ok ? pow2<true>(sc.of(p[b][e], th, (float)(i - key[b])) - lse[e]) : 0.f;
+        p[b][e] = ok ? pow2(sc.of(p[b][e], th, (float)(i - key[b])) - lse[e]) : 0.f;
         float d = p[b][e] * (ds[b][e] - delta[e]);
         if constexpr (CAP) d *= 1.0f - th * th;
         ds[b][e] = ok ? d : 0.f;

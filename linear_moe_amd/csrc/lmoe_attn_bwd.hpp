@@ -73,7 +73,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
         const int j = j0 + 32 * b + row32(i) + 4 * g;
         float r;
         const float u = sc(s[i], (float)(row - j), r);
-        float ds = pow2<true>(__builtin_fmaf(u, sc.a, off)) * (dp[i] - delta);
+        float ds = pow2(__builtin_fmaf(u, sc.a, off)) * (dp[i] - delta);
         if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
         s[i] = ds;
       }
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
           const int i = i0 + 32 * b + row32(e + x) + 4 * g;
           float r;
           const float u = sc(s[e + x], (float)(i - key), r);
-          float p = pow2<true>(__builtin_fmaf(u, sc.a, sc.b - lse[x]));
+          float p = pow2(__builtin_fmaf(u, sc.a, sc.b - lse[x]));
           float ds = p * (dp[e + x] - delta[x]);
           if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
           s[e + x] = p;

@@ -259,14 +259,14 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn
         s[b][i] = x;
         mx = fmaxf(mx, x);
       }
-    const float next = fmaxf(m, __builtin_fmaf(sc.a, both_max(mx), sc.b)), f = pow2<true>(m - next), off = sc.b - next;
+    const float next = fmaxf(m, __builtin_fmaf(sc.a, both_max(mx), sc.b)), f = pow2(m - next), off = sc.b - next;
     m = next;
     float part = 0.f;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[b][i] = pow2<true>(__builtin_fmaf(s[b][i], sc.a, off));
+        s[b][i] = pow2(__builtin_fmaf(s[b][i], sc.a, off));
         part += s[b][i];
       }
     sum = __builtin_fmaf(sum, f, part);

@@ -229,14 +229,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(
       }
     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float next = fmaxf(m, mx), f = pow2<FAST>(m - next);
+    const float next = fmaxf(m, mx), f = pow2(m - next);
     m = next;
     sum *= f;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[b][e] = pow2<FAST>(s[b][e] - m);
+        s[b][e] = pow2(s[b][e] - m);
         sum += s[b][e];
       }
     // (P rounded to the element type, as the products take it; the sum is of the numbers before)
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged_attn(
     float ll = 0.f, x = 0.f;
 #pragma unroll
     for (int y = 0; y < NW; ++y) {
-      const float f = pow2<FAST>(s_m[y][hh] - mm);
+      const float f = pow2(s_m[y][hh] - mm);
       ll += f * s_l[y][hh];
       x += f * s_o[y][hh][d];
     }
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(NTHR) void k_paged_join(const lmoe_paged_args a, co
   float ll = 0.f;
   for (int s = tid; s < sq.used; s += NTHR) {
     const f32x2 y = ml[s];
-    const float f = pow2<sizeof(T) == 2>(y[0] - m);
+    const float f = pow2(y[0] - m);
     s_f[s] = f;
     ll += f * y[1];
   }
