@@ -435,7 +435,10 @@ typedef struct lmoe_attn_args {
   const int32_t* prefix_lens;  /* [N] or NULL (causal calls); beyond 0 .. length: clamped */
   lmoe_tensor q, k, v, o;      /* [B,T,HQ,K], [B,T,HKV,K], [B,T,HKV,V], [B,T,HQ,V]     */
   float* lse;          /* [B,HQ,T]: log2 of the sum of e^s per row; written by fwd (NULL: not kept), read by bwd */
-  /* backward: o, lse of the forward call, d_o in; dq, dk, dv out (dk.ptr and dv.ptr NULL: dq alone)      */
+  int8_t* o_low;       /* [B,HQ,T,V], 8-byte aligned: what the rounding of o to 2 bytes left, in 2^-8 of its last place;
+                          written by fwd (NULL, or a 4-byte type: not kept), read by bwd, whose sums of d_o o it makes exact to
+                          2^-15 (NULL: o as it is) */
+  /* backward: o, lse (and o_low) of the forward call, d_o in; dq, dk, dv out (dk.ptr and dv.ptr NULL: dq alone)      */
   lmoe_tensor d_o, dq, dk, dv;
   float* delta;        /* [B,HQ,T] workspace: sum of d_o o per row                     */
   float* ws;           /* workspace of lmoe_softmax_attn_bwd_floats fp32 numbers (0: may be NULL), 16-byte aligned */

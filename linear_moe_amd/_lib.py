@@ -53,7 +53,7 @@ class AttnArgs(C.Structure):
     _fields_ = ([(n, C.c_int32) for n in ("dtype", "causal", "B", "T", "HQ", "HKV", "K", "V", "N", "NT")]
                 + [("scale", C.c_float), ("softcap", C.c_float)]
                 + [(n, C.c_void_p) for n in ("cu_seqlens", "chunk_map", "nt_dev", "seq_order", "slopes", "prefix_lens")]
-                + [(n, Tensor4) for n in ("q", "k", "v", "o")] + [("lse", C.c_void_p)]
+                + [(n, Tensor4) for n in ("q", "k", "v", "o")] + [("lse", C.c_void_p), ("o_low", C.c_void_p)]
                 + [(n, Tensor4) for n in ("d_o", "dq", "dk", "dv")] + [("delta", C.c_void_p), ("ws", C.c_void_p)])
 
 

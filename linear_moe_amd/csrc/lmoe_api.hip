@@ -694,6 +694,7 @@ static int check_attn(const lmoe_attn_args* a, const char* op, bool bwd) {
   for (const lmoe_tensor* t : rows)
     if (t->ptr && (((uintptr_t)t->ptr & 15) || t->sb % vec || t->st % vec || t->sh % vec))
       return fail(-9, "%s: q, k, v, o and their gradients need 16-byte aligned rows (pointer and strides)", op);
+  if ((uintptr_t)a->o_low & 7) return fail(-9, "%s: o_low must be 8-byte aligned", op);
   if (lmoe::attn_groups(*a) >= MAX_GROUPS) return fail(-8, "%s: more than 2^24 - 1 work-groups", op);
   return 0;
 }

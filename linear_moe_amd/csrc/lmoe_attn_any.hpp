@@ -211,6 +211,12 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_fwd_any(const lmoe_a
 #pragma unroll
       for (int i = 0; i < KW; ++i) x += *(const f32x4*)&s_o[i][r][c] * f[i];
       store4(out + c, x * inv);
+      if constexpr (sizeof(T) == 2) {
+        uint32_t z = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z |= low_byte(x[e] * inv) << 8 * e;
+        if (a.o_low) *(uint32_t*)(a.o_low + (((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + t.r0 + r) * a.V + c) = z;
+      }
     }
   }
 }
@@ -251,13 +257,19 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmo
     const int rc = min(row[r], last);
     q[r].load(attn_row<T>(a.o, t.b, t.tok0 + rc, h), a.V, g);
     d_o[r].load(attn_row<T>(a.d_o, t.b, t.tok0 + rc, h), a.V, g);
+    const int64_t at = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + rc;
     float d = 0.f;
 #pragma unroll
-    for (int j = 0; j < W / 16; ++j)
+    for (int j = 0; j < W / 16; ++j) {
+      uint32_t low = 0;
+      if (sizeof(T) == 2 && a.o_low && 16 * j + 4 * g < a.V) low = *(const uint32_t*)(a.o_low + at * a.V + 16 * j + 4 * g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) d = __builtin_fmaf(q[r].x[j][e], d_o[r].x[j][e], d);
+      for (int e = 0; e < 4; ++e) {
+        const float o = sizeof(T) == 2 ? with_low((bf16)q[r].x[j][e], low, e) : q[r].x[j][e];
+        d = __builtin_fmaf(o, d_o[r].x[j][e], d);
+      }
+    }
     delta[r] = column_sum(d);
-    const int64_t at = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + rc;
     lse[r] = a.lse[at];
     if (w == 0 && g == 0 && row[r] < t.len) a.delta[at] = delta[r];
     q[r].load(attn_row<T>(a.q, t.b, t.tok0 + rc, h), a.K, g);

@@ -25,8 +25,15 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
   rows32<W>(d_o, attn_row<bf16>(a.d_o, t.b, t.tok0 + min(w0, t.len - 1), h), a.d_o.st, max(rows, 1), a.V, l);
   rows32<W>(q, attn_row<bf16>(a.o, t.b, t.tok0 + min(w0, t.len - 1), h), a.o.st, max(rows, 1), a.V, l);
   float delta = 0.f;
+  const int8_t* low = a.o_low + (first + min(row_, t.len - 1)) * a.V;
 #pragma unroll
-  for (int j = 0; j < KS; ++j) delta = dot_vec(q[j], d_o[j], delta);
+  for (int j = 0; j < KS; ++j) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 x = {0, 0};
+    if (a.o_low && 16 * j + 8 * g < a.V) x = *(const u32x2*)(low + 16 * j + 8 * g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(with_low(q[j][e], x[e / 4], e % 4), (float)d_o[j][e], delta);
+  }
   delta = both_sum(delta);
   const float lse = a.lse[first + min(row_, t.len - 1)];
   if (g == 0 && row_ < t.len) a.delta[first + row_] = delta;

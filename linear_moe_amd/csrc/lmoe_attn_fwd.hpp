@@ -158,7 +158,8 @@ template <int W> __device__ __forceinline__ void rows32(bf16x8 (&f)[W / 16], con
 
 // a transposed block of 32 rows and W columns (acc[b]: columns 32 b ..) to rows [0, rows) and columns [0, D) of dst: two lanes of a
 // row exchange halves, so that each has 16 adjacent bytes
-template <int W> __device__ __forceinline__ void store_rows32(const f32x16 (&acc)[W / 32], float mul, bf16* dst, int64_t stride, int rows, int D, int l) {
+// low (or nullptr): [rows][D], what the rounding leaves (low_byte)
+template <int W> __device__ __forceinline__ void store_rows32(const f32x16 (&acc)[W / 32], float mul, bf16* dst, int64_t stride, int rows, int D, int l, int8_t* low = nullptr) {
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   bf16* p = dst + (int64_t)(l & 31) * stride + 8 * (l >> 5);
@@ -172,6 +173,13 @@ template <int W> __device__ __forceinline__ void store_rows32(const f32x16 (&acc
       const u32x4 y = __builtin_bit_cast(u32x4, x);
       const u32x2 lo = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false), hi = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
       if ((l & 31) < rows && 32 * b + 2 * i + 8 * (l >> 5) < D) *(u32x4*)(p + 32 * b + 2 * i) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+      if (low) {
+        uint32_t z[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e / 4] |= low_byte(acc[b][i + e] * mul) << 8 * (e % 4);
+        const u32x2 q = __builtin_amdgcn_permlane32_swap(z[0], z[1], false, false);
+        if ((l & 31) < rows && 32 * b + 2 * i + 8 * (l >> 5) < D) *(u32x2*)(low + (int64_t)(l & 31) * D + 32 * b + 2 * i + 8 * (l >> 5)) = q;
+      }
     }
 }
 
@@ -336,7 +344,8 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn
   sum = both_sum(sum);
   if (a.lse && g == 0 && row_ < t.len) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + row_] = m + __builtin_amdgcn_logf(sum);
   if (rows > 0)
-    store_rows32<W>(o, 1.0f / sum, attn_row<bf16>(a.o, t.b, t.tok0 + w0, h), a.o.st, rows, a.V, l);
+    store_rows32<W>(o, 1.0f / sum, attn_row<bf16>(a.o, t.b, t.tok0 + w0, h), a.o.st, rows, a.V, l,
+                    a.o_low ? a.o_low + (((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + w0) * a.V : nullptr);
 }
 
 }  // namespace lmoe

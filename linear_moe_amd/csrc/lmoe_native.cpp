@@ -801,7 +801,7 @@ struct Attn {
   }
 };
 
-// attn_forward(q, k, v, scale, causal, softcap, slopes, prefix_lens, plan, head_first, save, stream) -> (o, lse or None)
+// attn_forward(q, k, v, scale, causal, softcap, slopes, prefix_lens, plan, head_first, save, stream) -> (o, lse or None, o_low or None)
 PyObject* attn_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Attn c;
@@ -809,29 +809,31 @@ PyObject* attn_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const bool save = yes(o[10]);
   void* st = stream_of(o[11]);
   if (PyErr_Occurred()) return elsewhere();
-  Tensor out, lse;
+  Tensor out, lse, low;
   int rc;
   {
     const Unlocked unlocked;
     const auto s = c.q.sizes();
     out = at::empty({s[0], s[1], s[2], c.V}, c.q.options().requires_grad(false));
     if (save) lse = at::empty({c.B, c.HQ, c.T}, c.q.options().dtype(at::kFloat).requires_grad(false));
-    c.a.o = desc(out, c.head_first); c.a.lse = (float*)ptr(lse);
+    if (save && bf16(c.q)) low = at::empty({c.B, c.HQ, c.T * c.V}, c.q.options().dtype(at::kChar).requires_grad(false));
+    c.a.o = desc(out, c.head_first); c.a.lse = (float*)ptr(lse); c.a.o_low = (int8_t*)ptr(low);
     rc = lib.attn_fwd(&c.a, st);
   }
-  return result(rc, {out, lse});
+  return result(rc, {out, lse, low});
   END_HANDLE_TH_ERRORS
 }
 
-// attn_backward(the first ten of attn_forward, o, lse, do, keys: whether dk and dv are wanted, stream) -> (dq, dk, dv)
+// attn_backward(the first ten of attn_forward, o, lse, o_low, do, keys: whether dk and dv are wanted, stream) -> (dq, dk, dv)
 PyObject* attn_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Attn c;
-  Tensor out, lse, dout;
-  if (n != 15 || !c.take(o) || !plain(out, o[10], c.dev) || !plain(lse, o[11], c.dev) || !plain(dout, o[12], c.dev)) return elsewhere();
+  Tensor out, lse, low, dout;
+  if (n != 16 || !c.take(o) || !plain(out, o[10], c.dev) || !plain(lse, o[11], c.dev) || !plain_or_none(low, o[12], c.dev) || !plain(dout, o[13], c.dev)) return elsewhere();
+  if (low.defined() != bf16(c.q) || (low.defined() && (low.scalar_type() != at::kChar || !low.is_contiguous() || low.sizes() != at::IntArrayRef({c.B, c.HQ, c.T * c.V})))) return elsewhere();
   if (!c.lies_like_o(out) || !c.lies_like_o(dout) || !f32(lse) || !lse.is_contiguous() || lse.sizes() != at::IntArrayRef({c.B, c.HQ, c.T})) return elsewhere();
-  const bool keys = yes(o[13]);
-  void* st = stream_of(o[14]);
+  const bool keys = yes(o[14]);
+  void* st = stream_of(o[15]);
   if (PyErr_Occurred()) return elsewhere();
   Tensor dq, dk, dv;
   int rc;
@@ -840,7 +842,7 @@ PyObject* attn_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
     dq = at::empty_like(c.q.detach());
     const Tensor delta = at::empty_like(lse);
     if (keys) { dk = at::empty_like(c.k.detach()); dv = at::empty_like(c.v.detach()); }
-    c.a.o = desc(out, c.head_first); c.a.lse = (float*)lse.data_ptr(); c.a.d_o = desc(dout, c.head_first); c.a.delta = (float*)delta.data_ptr();
+    c.a.o = desc(out, c.head_first); c.a.lse = (float*)lse.data_ptr(); c.a.o_low = (int8_t*)ptr(low); c.a.d_o = desc(dout, c.head_first); c.a.delta = (float*)delta.data_ptr();
     c.a.dq = desc(dq, c.head_first); c.a.dk = desc(dk, c.head_first); c.a.dv = desc(dv, c.head_first);
     const int64_t floats = lib.attn_bwd_floats(&c.a);
     rc = (int)std::min<int64_t>(floats, 0);

@@ -89,7 +89,7 @@ def _check(q, k, v, head_first, cu_seqlens):
     return B, T, HQ, HKV, K, V
 
 
-def _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, prefix, plan):
+def _args(q, k, v, o, lse, low, dims, head_first, scale, causal, softcap, slopes, prefix, plan):
     B, T, HQ, HKV, K, V = dims
     a = _lib.AttnArgs()
     a.dtype, a.causal = _DT[q.dtype], int(causal)
@@ -100,7 +100,7 @@ def _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, pre
                                                             ptr(plan.seq_order))
     a.slopes, a.prefix_lens = ptr(slopes), ptr(prefix)
     a.q, a.k, a.v, a.o = (_desc(x, head_first) for x in (q, k, v, o))
-    a.lse = ptr(lse)
+    a.lse, a.o_low = ptr(lse), ptr(low)
     return a
 
 
@@ -112,10 +112,11 @@ def _forward(q, k, v, dims, head_first, scale, causal, softcap, slopes, prefix, 
     q, k, v = rows16(q.detach()), rows16(k.detach()), rows16(v.detach())
     o = torch.empty((*q.shape[:3], V), dtype=q.dtype, device=q.device)
     lse = torch.empty(B, HQ, T, dtype=torch.float32, device=q.device) if save else None
+    low = torch.empty(B, HQ, T * V, dtype=torch.int8, device=q.device) if save and q.dtype == torch.bfloat16 else None
     if B * T:
-        a = _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, prefix, plan)
+        a = _args(q, k, v, o, lse, low, dims, head_first, scale, causal, softcap, slopes, prefix, plan)
         _lib.check(_lib.load().lmoe_softmax_attn_fwd(C.byref(a), stream_ptr()), "softmax_attn forward")
-    return q, k, v, o, lse
+    return q, k, v, o, lse, low
 
 
 def _back(x, shape, dtype, device, name):
@@ -129,8 +130,8 @@ def _back(x, shape, dtype, device, name):
 class _SoftmaxAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, dims, head_first, scale, causal, softcap, slopes, prefix, plan):
-        qs, ks, vs, o, lse = _forward(q, k, v, dims, head_first, scale, causal, softcap, slopes, prefix, plan, True)
-        ctx.save_for_backward(qs, ks, vs, o, lse, slopes, prefix)
+        qs, ks, vs, o, lse, low = _forward(q, k, v, dims, head_first, scale, causal, softcap, slopes, prefix, plan, True)
+        ctx.save_for_backward(qs, ks, vs, o, lse, low, slopes, prefix)
         ctx.call = dims, head_first, scale, causal, softcap, plan
         ctx.shapes, ctx.dtype, ctx.options = (q.shape, k.shape, v.shape, o.shape), q.dtype, (slopes is not None, prefix is not None)
         return o
@@ -140,17 +141,19 @@ class _SoftmaxAttn(torch.autograd.Function):
     def backward(ctx, do):
         dims, head_first, scale, causal, softcap, plan = ctx.call
         B, T, HQ, HKV, K, V = dims
-        q, k, v, o, lse, slopes, prefix = ctx.saved_tensors
+        q, k, v, o, lse, low, slopes, prefix = ctx.saved_tensors
         keys = any(ctx.needs_input_grad[1:3])
         if (q.shape, k.shape, v.shape, o.shape) == ctx.shapes and (slopes is not None, prefix is not None) == ctx.options:
             r = native_call("attn_backward", "softmax_attn backward", q, k, v, scale, causal, softcap, slopes, prefix, plan.tables,
-                            head_first, o, lse, do, keys)
+                            head_first, o, lse, low, do, keys)
             if r is not None:
                 return (*r, *(None,) * 8)
         dev, dt = do.device, ctx.dtype
         q, k, v, o = (_back(x, s, dt, dev, n) for x, s, n in zip((q, k, v, o), ctx.shapes, "qkvo"))
         do = _back(do, ctx.shapes[3], dt, dev, "the gradient")
         lse = _back(lse, (B, HQ, T), torch.float32, dev, "lse")
+        if dt == torch.bfloat16:
+            low = _back(low, (B, HQ, T * V), torch.int8, dev, "o_low")
         if ctx.options[0]:
             slopes = _back(slopes, (HQ,), torch.float32, dev, "slopes")
         if ctx.options[1]:
@@ -158,7 +161,7 @@ class _SoftmaxAttn(torch.autograd.Function):
         dq = torch.empty_like(q)
         dk, dv = (torch.empty_like(k), torch.empty_like(v)) if keys else (None, None)
         if B * T:
-            a = _args(q, k, v, o, lse, dims, head_first, scale, causal, softcap, slopes, prefix, plan)
+            a = _args(q, k, v, o, lse, low, dims, head_first, scale, causal, softcap, slopes, prefix, plan)
             delta = torch.empty(B, HQ, T, dtype=torch.float32, device=dev)
             a.d_o, a.dq, a.dk, a.dv, a.delta = (_desc(do, head_first), _desc(dq, head_first), _desc(dk, head_first),
                                                 _desc(dv, head_first), delta.data_ptr())

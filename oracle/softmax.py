@@ -8,7 +8,8 @@ type relative to the value (``torch.finfo(t).eps / 2``), w the same of float32.
   does the sum: twice the largest of the row, and (n + 16) w for n terms of the sum and the exponentials themselves: ``rel``.
 * o: the products take p rounded to the element type (u), o is rounded once: u |o| + (u + rel + n w) sum_j p |v|.
 * dv: the same with do in place of v, summed over rows (and heads).
-* delta = do . o from the rounded o: sum_d |do_d| err(o_d), and V w sum |do o|;  dp: V w sum_d |do_d v_d|.
+* delta = do . o from o to 2^-15 (2-byte elements: o and what its rounding left, in 2^-8 of the last place): sum_d |do_d| err(o_d)
+  with that in place of the u |o|, and V w sum |do o|;  dp: V w sum_d |do_d v_d|.
 * ds = p (dp - delta) (1 - tanh^2), rounded to the element type: (u + rel) |ds| + p (err(dp) + err(delta)); the factor of the cap has
   an absolute error of 8 w.
 * dq, dk: u |dq| + scale sum err(ds) |k| + n w scale sum |ds k|.
@@ -49,7 +50,7 @@ def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dty
     do = do.double()
     dp, delta = do @ v.T, (do * o).sum(1, keepdim=True)
     err_dp = V * w * (do.abs() @ v.abs().T)
-    err_delta = (do.abs() * err_o).sum(1, keepdim=True) + V * w * (do * o).abs().sum(1, keepdim=True)
+    err_delta = (do.abs() * (err_o - (u - min(u, 2.0 ** -15)) * o.abs())).sum(1, keepdim=True) + V * w * (do * o).abs().sum(1, keepdim=True)
     fac = 1 - th * th
     ds = p * (dp - delta) * fac
     err_ds = (u + rel) * ds.abs() + p * (err_dp + err_delta) + (8 * w * p * (dp - delta).abs() if cap else 0.0)
