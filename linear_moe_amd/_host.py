@@ -411,8 +411,11 @@ def no_node(*xs) -> bool:
     function of autograd, to refuse it there (a transform, forward-mode differentiation) or to run it again (a trace being
     recorded, which would hold the allocations of the steps alone).  Its steps then run without one (5 us of a call that
     takes the GPU 9)."""
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs):
-        return False
+    return not (torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs)) and no_transform()
+
+
+def no_transform() -> bool:
+    """Whether nothing is at work that has to see an op as a function of autograd."""
     return (not torch._C._are_functorch_transforms_active() and forward_ad._current_level < 0
             and torch._C._get_tracing_state() is None)
 

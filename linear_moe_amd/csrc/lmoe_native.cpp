@@ -6,6 +6,7 @@
 // 5 to 100 us, and the same steps through Python objects and ctypes took the host 20 us per forward and as much
 // per backward (figures in linear_moe_amd/_host.py).  The neighbours of the ops (gates, prologue, output gate, routing of a
 // mixture of memories: gates.py, layer_io.py, mom.py) take it too: a mixer's step is four autograd nodes and twelve launches.
+// Softmax attention has its node of the autograd graph here as well (AttnNode).
 #include <Python.h>
 #include <dlfcn.h>
 
@@ -14,9 +15,15 @@
 #include <type_traits>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include "../../include/lmoe.h"
 
@@ -43,6 +50,7 @@ struct Library {
   decltype(&lmoe_mom_plan_ints) mom_plan_ints;
   decltype(&lmoe_mom_plan) mom_plan;
   decltype(&lmoe_seq_tables) seq_tables;
+  decltype(&lmoe_last_error) last_error;
   decltype(&lmoe_softmax_attn_fwd) attn_fwd;
   decltype(&lmoe_softmax_attn_bwd) attn_bwd;
   decltype(&lmoe_softmax_attn_bwd_floats) attn_bwd_floats;
@@ -796,10 +804,35 @@ struct Attn {
     a.q = desc(q, head_first); a.k = desc(k, head_first); a.v = desc(v, head_first);
     return true;
   }
+  // the outputs of a forward pass, and the pass
+  int forward(bool save, Tensor& out, Tensor& lse, Tensor& low, void* st) {
+    const auto s = q.sizes();
+    out = at::empty({s[0], s[1], s[2], V}, q.options().requires_grad(false));
+    if (save) lse = at::empty({B, HQ, T}, q.options().dtype(at::kFloat).requires_grad(false));
+    if (save && bf16(q)) low = at::empty({B, HQ, T * V}, q.options().dtype(at::kChar).requires_grad(false));
+    a.o = desc(out, head_first); a.lse = (float*)ptr(lse); a.o_low = (int8_t*)ptr(low);
+    return lib.attn_fwd(&a, st);
+  }
   bool lies_like_o(const Tensor& x) const {
     return x.dim() == 4 && x.sizes().slice(0, 3) == q.sizes().slice(0, 3) && x.size(3) == V && x.scalar_type() == q.scalar_type() && rows_aligned(x);
   }
 };
+
+// The gradients of a pass whose block holds the options, the tables, and q, k, v; st: the stream
+int attn_gradients(lmoe_attn_args a, bool hf, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& lse, const Tensor& low, const Tensor& dout,
+                   bool keys, Tensor& dq, Tensor& dk, Tensor& dv, void* st) {
+  dq = at::empty_like(q.detach());
+  const Tensor delta = at::empty_like(lse);
+  if (keys) { dk = at::empty_like(k.detach()); dv = at::empty_like(v.detach()); }
+  a.o = desc(out, hf); a.lse = (float*)lse.data_ptr(); a.o_low = (int8_t*)ptr(low); a.d_o = desc(dout, hf); a.delta = (float*)delta.data_ptr();
+  a.dq = desc(dq, hf); a.dk = desc(dk, hf); a.dv = desc(dv, hf);
+  const int64_t floats = lib.attn_bwd_floats(&a);
+  if (floats < 0) return (int)floats;
+  Tensor ws;
+  if (floats) ws = at::empty({floats}, lse.options());
+  a.ws = (float*)ptr(ws);
+  return lib.attn_bwd(&a, st);
+}
 
 // attn_forward(q, k, v, scale, causal, softcap, slopes, prefix_lens, plan, head_first, save, stream) -> (o, lse or None, o_low or None)
 PyObject* attn_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
@@ -813,12 +846,7 @@ PyObject* attn_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   int rc;
   {
     const Unlocked unlocked;
-    const auto s = c.q.sizes();
-    out = at::empty({s[0], s[1], s[2], c.V}, c.q.options().requires_grad(false));
-    if (save) lse = at::empty({c.B, c.HQ, c.T}, c.q.options().dtype(at::kFloat).requires_grad(false));
-    if (save && bf16(c.q)) low = at::empty({c.B, c.HQ, c.T * c.V}, c.q.options().dtype(at::kChar).requires_grad(false));
-    c.a.o = desc(out, c.head_first); c.a.lse = (float*)ptr(lse); c.a.o_low = (int8_t*)ptr(low);
-    rc = lib.attn_fwd(&c.a, st);
+    rc = c.forward(save, out, lse, low, st);
   }
   return result(rc, {out, lse, low});
   END_HANDLE_TH_ERRORS
@@ -839,21 +867,104 @@ PyObject* attn_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   int rc;
   {
     const Unlocked unlocked;
-    dq = at::empty_like(c.q.detach());
-    const Tensor delta = at::empty_like(lse);
-    if (keys) { dk = at::empty_like(c.k.detach()); dv = at::empty_like(c.v.detach()); }
-    c.a.o = desc(out, c.head_first); c.a.lse = (float*)lse.data_ptr(); c.a.o_low = (int8_t*)ptr(low); c.a.d_o = desc(dout, c.head_first); c.a.delta = (float*)delta.data_ptr();
-    c.a.dq = desc(dq, c.head_first); c.a.dk = desc(dk, c.head_first); c.a.dv = desc(dv, c.head_first);
-    const int64_t floats = lib.attn_bwd_floats(&c.a);
-    rc = (int)std::min<int64_t>(floats, 0);
-    if (rc == 0) {
-      Tensor ws;
-      if (floats) ws = at::empty({floats}, lse.options());
-      c.a.ws = (float*)ptr(ws);
-      rc = lib.attn_bwd(&c.a, st);
-    }
+    rc = attn_gradients(c.a, c.head_first, c.q, c.k, c.v, out, lse, low, dout, keys, dq, dk, dv, st);
   }
   return result(rc, {dq, dk, dv});
+  END_HANDLE_TH_ERRORS
+}
+
+// The node of softmax_attn in the autograd graph, for the calls that attn_forward takes: the same passes, without the interpreter
+// on the way (a forward and backward of 37 tokens: 63 us of the host, with the node in Python 105; 48 of them torch's engine starting a pass).  The Python of the op has a node for
+// all other calls; what it does with saved tensors that a hook changed, with a second derivative and with a gradient of
+// another type, this one does.
+struct AttnNode : torch::autograd::Node {
+  using List = torch::autograd::variable_list;
+  lmoe_attn_args a;
+  bool head_first;
+  at::ScalarType type;
+  c10::Device device{c10::DeviceType::CUDA, 0};
+  Tensor tables[5];
+  enum { Q, K, V, O, LSE, LOW, SLOPES, PREFIX, SAVED };
+  torch::autograd::SavedVariable saved[SAVED];
+  c10::SmallVector<int64_t, 4> shapes[SAVED];
+  bool given[SAVED] = {};
+
+  std::string name() const override { return "SoftmaxAttnBackward"; }
+  void save(int i, const Tensor& x) {
+    if (!x.defined()) return;
+    given[i] = true;
+    shapes[i].assign(x.sizes().begin(), x.sizes().end());
+    saved[i] = torch::autograd::SavedVariable(x, i == O);
+  }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& x : saved) x.reset_data();
+  }
+  // as the kernels may read it: a saved-tensor hook hands back what it likes
+  Tensor back(int i, at::ScalarType t) {
+    static const char* const names[SAVED] = {"q", "k", "v", "o", "lse", "o_low", "slopes", "prefix_lens"};
+    if (!given[i]) return Tensor();
+    const Tensor x = saved[i].unpack(i == O ? shared_from_this() : nullptr);
+    TORCH_CHECK(x.defined() && x.sizes() == at::IntArrayRef(shapes[i]) && x.device() == device, names[i], ", saved for the backward with shape ",
+                at::IntArrayRef(shapes[i]), " on ", device, ", came back as another");
+    return as(x, t);
+  }
+  static Tensor as(const Tensor& x, at::ScalarType t) {
+    const Tensor y = x.to(t);
+    return y.dim() == 4 ? rows_aligned(y) ? y : y.clone(at::MemoryFormat::Contiguous) : y.contiguous();
+  }
+  List apply(List&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return List(3);
+    const bool again = at::GradMode::is_enabled();
+    List out(3);
+    {
+      const at::NoGradGuard no_grad;
+      const c10::OptionalDeviceGuard on(device);
+      TORCH_CHECK(grads[0].sizes() == at::IntArrayRef(shapes[O]) && grads[0].device() == device, "softmax_attn backward: a gradient of another shape or device");
+      const Tensor q = back(Q, type), k = back(K, type), v = back(V, type), o = back(O, type), lse = back(LSE, at::kFloat), low = back(LOW, at::kChar),
+                   slopes = back(SLOPES, at::kFloat), prefix = back(PREFIX, at::kInt), dout = as(grads[0], type);
+      lmoe_attn_args b = a;
+      b.q = desc(q, head_first); b.k = desc(k, head_first); b.v = desc(v, head_first);
+      b.slopes = (const float*)ptr(slopes); b.prefix_lens = (const int32_t*)ptr(prefix);
+      const int rc = attn_gradients(b, head_first, q, k, v, o, lse, low, dout, task_should_compute_output(1) || task_should_compute_output(2), out[0], out[1], out[2],
+                                    c10::hip::getCurrentHIPStream(device.index()).stream());
+      TORCH_CHECK(rc == 0, "softmax_attn backward failed (", rc, "): ", lib.last_error());
+    }
+    if (again) {                                   // (create_graph: the gradients are constants to everything but an attempt to derive them)
+      List known;
+      for (auto& x : out) if (x.defined()) known.push_back(x.detach().requires_grad_(true));
+      known = torch::autograd::DelayedError("trying to differentiate softmax_attn twice, which has no second derivative", (int64_t)known.size()).apply(std::move(known));
+      size_t i = 0;
+      for (auto& x : out) if (x.defined()) x = known[i++];
+    }
+    return out;
+  }
+};
+
+// attn_node(the first ten of attn_forward, stream) -> (o,) with its node, for a call that autograd has to see
+PyObject* attn_node(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Attn c;
+  if (n != 11 || !c.take(o)) return elsewhere();
+  void* st = stream_of(o[10]);
+  if (PyErr_Occurred()) return elsewhere();
+  Tensor out, lse, low;
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = c.forward(true, out, lse, low, st);
+    if (rc == 0) {
+      const std::shared_ptr<AttnNode> node(new AttnNode, torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(c.q, c.k, c.v));
+      node->a = c.a; node->head_first = c.head_first; node->type = c.q.scalar_type(); node->device = c.q.device();
+      for (int i = 0; i < 5; ++i) node->tables[i] = c.tables[i];
+      torch::autograd::set_history(out, node);
+      const Tensor* const all[] = {&c.q, &c.k, &c.v, &out, &lse, &low, &c.slopes, &c.prefix};
+      for (int i = 0; i < AttnNode::SAVED; ++i) node->save(i, *all[i]);
+    }
+  }
+  return result(rc, {out});
   END_HANDLE_TH_ERRORS
 }
 
@@ -962,7 +1073,7 @@ PyObject* bind(PyObject*, PyObject* path) {
   get(l.swish_fwd, "lmoe_swish_gate_relayout_fwd"); get(l.swish_bwd, "lmoe_swish_gate_relayout_bwd");
   get(l.gates_partials, "lmoe_gdn_gates_partials"); get(l.gates_fwd, "lmoe_gdn_gates_fwd"); get(l.gates_bwd, "lmoe_gdn_gates_bwd");
   get(l.mom_gather, "lmoe_mom_gather"); get(l.mom_combine, "lmoe_mom_combine"); get(l.mom_combine_bwd, "lmoe_mom_combine_bwd");
-  get(l.attn_fwd, "lmoe_softmax_attn_fwd"); get(l.attn_bwd, "lmoe_softmax_attn_bwd"); get(l.attn_bwd_floats, "lmoe_softmax_attn_bwd_floats"); get(l.paged_floats, "lmoe_paged_attn_floats");
+  get(l.last_error, "lmoe_last_error"); get(l.attn_fwd, "lmoe_softmax_attn_fwd"); get(l.attn_bwd, "lmoe_softmax_attn_bwd"); get(l.attn_bwd_floats, "lmoe_softmax_attn_bwd_floats"); get(l.paged_floats, "lmoe_paged_attn_floats");
   get(l.paged_decode, "lmoe_paged_attn_decode"); get(l.paged_append, "lmoe_paged_kv_append");
   get(l.mom_plan_ints, "lmoe_mom_plan_ints"); get(l.mom_plan, "lmoe_mom_plan"); get(l.seq_tables, "lmoe_seq_tables");
   if (!all) return PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point", p);
@@ -979,7 +1090,7 @@ PyMethodDef methods[] = {
     LMOE_METHOD(mixer_forward), LMOE_METHOD(mixer_backward), LMOE_METHOD(swish_forward), LMOE_METHOD(swish_backward),
     LMOE_METHOD(gates_forward), LMOE_METHOD(gates_backward), LMOE_METHOD(mom_gather), LMOE_METHOD(mom_combine),
     LMOE_METHOD(mom_combine_backward), LMOE_METHOD(mom_plan), LMOE_METHOD(seq_tables),
-    LMOE_METHOD(attn_forward), LMOE_METHOD(attn_backward), LMOE_METHOD(paged_decode), LMOE_METHOD(paged_append),
+    LMOE_METHOD(attn_forward), LMOE_METHOD(attn_backward), LMOE_METHOD(attn_node), LMOE_METHOD(paged_decode), LMOE_METHOD(paged_append),
 #undef LMOE_METHOD
     {"intact", (PyCFunction)(void (*)(void))intact, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._host import _DT, _desc, native_call, no_node, ptr, seq_plan, stream_ptr
+from ._host import _DT, _desc, native_call, no_node, no_transform, ptr, seq_plan, stream_ptr
 
 MAX_DIM = 128      # columns of a head
 
@@ -198,8 +198,11 @@ def softmax_attn(
     cu_seqlens: packed documents as in the chunk ops; rows of one never see another's (nor what it holds: a NaN stays in its
     document).  Rows behind the last document are zero in o and in the gradients.
     Without atomics: the gradients of a key head are summed over its query heads in a fixed order."""
-    if cu_seqlens is None and no_node(q, k, v):      # (what the native path takes as it is, it also checks)
-        r = native_call("attn_forward", "softmax_attn forward", q, k, v, scale, causal, softcap, slopes, prefix_lens, None, head_first, False)
+    grad = not no_node(q, k, v)
+    node = grad and no_transform()                   # (a node of the graph, in native code)
+    if cu_seqlens is None and (node or not grad):    # (what the native path takes as it is, it also checks)
+        call = q, k, v, scale, causal, softcap, slopes, prefix_lens, None, head_first
+        r = native_call("attn_node", "softmax_attn", *call) if node else native_call("attn_forward", "softmax_attn forward", *call, False)
         if r is not None:
             return r[0]
     dims = _check(q, k, v, head_first, cu_seqlens)
@@ -221,5 +224,9 @@ def softmax_attn(
         q, k, v = pad(q, (0, -K % step)), pad(k, (0, -K % step)), pad(v, (0, -V % step))
         dims = B, T, HQ, HKV, q.shape[3], v.shape[3]
     rest = dims, head_first, sc, bool(causal), cap, slopes, prefix_lens, plan
-    o = _forward(q, k, v, *rest, save=False)[3] if no_node(q, k, v) else _SoftmaxAttn.apply(q, k, v, *rest)
+    if grad:
+        r = native_call("attn_node", "softmax_attn", q, k, v, *rest[2:7], plan.tables, head_first) if node else None
+        o = _SoftmaxAttn.apply(q, k, v, *rest) if r is None else r[0]
+    else:
+        o = _forward(q, k, v, *rest, save=False)[3]
     return o if o.shape[3] == V else o[..., :V]

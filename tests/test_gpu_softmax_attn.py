@@ -297,9 +297,13 @@ def test_only_the_gradients_that_are_wanted(cuda):
         assert torch.equal(g, full[i])
 
 
-def test_saved_tensor_hooks_and_checkpoint(cuda):
-    """Hooks that hand back other types and strides: gradients of the same values."""
+@pytest.mark.parametrize("odd", [False, True])
+def test_saved_tensor_hooks_and_checkpoint(cuda, odd):
+    """Hooks that hand back other types and strides: gradients of the same values (odd: rows off 16 bytes, which take the node in
+    Python)."""
     q, k, v, do = (x.to(cuda) for x in inputs(61, 1, 130, 4, 2, 64, 64, BF16))
+    if odd:
+        q, k, v = (torch.empty(x.numel() + 1, dtype=BF16, device=cuda)[1:].view(x.shape).copy_(x) for x in (q, k, v))
 
     def all_of(f):
         leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
@@ -321,11 +325,44 @@ def test_saved_tensor_hooks_and_checkpoint(cuda):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
-def test_second_derivatives_are_refused(cuda):
-    q, k, v, do = (x.to(cuda).requires_grad_(True) for x in inputs(67, 1, 20, 2, 2, 64, 64, F32))
-    (g,) = torch.autograd.grad(L.softmax_attn(q, k, v, head_first=False), q, do, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(g.sum(), q)
+@pytest.mark.parametrize("D", [64, 60])              # (60: padded, 64 as it is)
+def test_second_derivatives_are_refused(cuda, D):
+    q, k, v, do = (x.to(cuda).requires_grad_(True) for x in inputs(67, 1, 20, 2, 2, D, D, F32))
+    plain = torch.autograd.grad(L.softmax_attn(q, k, v, head_first=False), (q, k, v), do)
+    grads = torch.autograd.grad(L.softmax_attn(q, k, v, head_first=False), (q, k, v), do, create_graph=True)
+    for a, b in zip(plain, grads):
+        assert torch.equal(a, b)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(b.sum(), q, retain_graph=True)
+
+
+def test_the_node_keeps_to_the_rules_of_autograd(cuda):
+    q, k, v, do = (x.to(cuda) for x in inputs(71, 1, 40, 4, 2, 64, 64, BF16))
+    q, k, v = (x.requires_grad_(True) for x in (q, k, v))
+    op = lambda: L.softmax_attn(q * 1, k, v, head_first=False)
+    o = op()
+    first = torch.autograd.grad(o, (q, k, v), do, retain_graph=True)
+    for a, b in zip(first, torch.autograd.grad(o, (q, k, v), do)):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(o, (q, k, v), do)
+    for bad in (q, o):                                # what it saved has changed: the inputs, and the output
+        o = op() if bad is q else o
+        x = q * 1
+        o = L.softmax_attn(x, k, v, head_first=False)
+        with torch.no_grad():
+            (x if bad is q else o).add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(o, (q, k, v), do)
+    # outputs in a chain, a gradient that never arrives, and the memory of a node that goes unused
+    y = L.softmax_attn(L.softmax_attn(q, q, q, head_first=False), k.expand(1, 40, 2, 64), v, head_first=False)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(y, (q, k, v), do))
+    assert torch.autograd.grad(op().sum() * 0 + k.sum(), v, allow_unused=True)[0].abs().max() == 0
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    o = op()
+    del o, y
+    assert torch.cuda.memory_allocated() <= before
 
 
 def test_a_captured_step_follows_offsets_and_prefixes(cuda):
