@@ -70,12 +70,24 @@ int64_t attn_bwd_floats(const lmoe_attn_args& a) {
   return parts > 1 ? (int64_t)parts * a.B * a.T * a.HKV * (a.K + a.V) : 0;
 }
 
+// Whether two groups of waves share the rows of a work-group (k_attn_fwd, k_attn_bwd_dq): where the card is not full without, or
+// just so, and the rows see many keys.  Forward, us with one group and with two, 16 heads of 128: 1 x 448 tokens 15.3 15.6, 1 x 512
+// 18.4 17.3, 1 x 1024 28.6 24.8, 1 x 2048 50.6 41.2, 1 x 4096 107 91, 1 x 8192 321 321; 4 x 1024 35.9 41.7, 2 x 2048 60.6 57.1;
+// not causal 1 x 2048 49.9 42.7, 1 x 4096 168 179.  8 heads of 64: 1 x 256 9.1 9.6, 1 x 2048 34.8 27.9, 1 x 4096 63.6 49.7.
+static bool two_groups(const lmoe_attn_args& a, int64_t groups) {
+  return (groups <= cu_count() && a.T >= 384) || (a.causal && groups <= 2 * cu_count() && a.T >= 2048);
+}
+
 template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
   static void fwd(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_fwd<W, CAP, BIAS>), dim3(attn_tiles<ATTN_ROWS>(a) * a.HQ), dim3(64 * ATTN_WAVES), 0, st, a);
+    const int64_t groups = attn_tiles<ATTN_ROWS>(a) * a.HQ;
+    if (two_groups(a, groups)) hipLaunchKernelGGL((k_attn_fwd<W, 2, CAP, BIAS>), dim3(groups), dim3(128 * ATTN_WAVES), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_fwd<W, 1, CAP, BIAS>), dim3(groups), dim3(64 * ATTN_WAVES), 0, st, a);
   }
   static void bwd(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_bwd_dq<W, CAP, BIAS>), dim3(attn_tiles<ATTN_ROWS>(a) * a.HQ), dim3(64 * ATTN_WAVES), 0, st, a);
+    const int64_t groups = attn_tiles<ATTN_ROWS>(a) * a.HQ;
+    if (two_groups(a, groups)) hipLaunchKernelGGL((k_attn_bwd_dq<W, 2, CAP, BIAS>), dim3(groups), dim3(128 * ATTN_WAVES), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_bwd_dq<W, 1, CAP, BIAS>), dim3(groups), dim3(64 * ATTN_WAVES), 0, st, a);
     if (!a.dk.ptr) return;
     constexpr int NW = attn_kv_waves(W);
     const int parts = attn_parts(a);

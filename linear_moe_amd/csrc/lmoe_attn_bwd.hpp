@@ -8,15 +8,17 @@ namespace lmoe {
 
 // dq of 128 rows; delta of those rows beside it.  As the forward kernel: S^T = K Q^T and dP^T = V dO^T leave a lane with one row,
 // whose lse and delta are one number, and dS^T as the B operand of dQ^T += K^T dS^T.
-template <int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
+template <int W, int KG, bool CAP, bool BIAS>
+__global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
   constexpr int KS = W / 16, DB = W / 32, TILE = CH * W;
-  __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
+  __shared__ __attribute__((aligned(1024))) bf16 a_k0[KG * TILE], a_v0[KG * TILE], a_k1[KG * TILE], a_v1[KG * TILE];
   zero_behind<bf16>(a, a.dq, a.HQ, a.K);
   AttnTile t;
   int h;
   if (!attn_place<ATTN_ROWS>(a, a.HQ, true, h, t)) return;
-  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 5;
+  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = KG == 1 ? wave_id() : wave_id() % ATTN_WAVES, g = l >> 5;
+  const int kg = KG == 1 ? 0 : wave_id() / ATTN_WAVES;
+  bf16 *const s_k0 = a_k0 + kg * TILE, *const s_v0 = a_v0 + kg * TILE, *const s_k1 = a_k1 + kg * TILE, *const s_v1 = a_v1 + kg * TILE;
   const Score16<CAP, BIAS> sc(a, h);
   const int w0 = t.r0 + 32 * w, rows = t.len - w0, row_ = w0 + (l & 31);
   const int64_t first = ((int64_t)t.b * a.HQ + h) * a.T + t.tok0;
@@ -36,7 +38,7 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
   }
   delta = both_sum(delta);
   const float lse = a.lse[first + min(row_, t.len - 1)];
-  if (g == 0 && row_ < t.len) a.delta[first + row_] = delta;
+  if (kg == 0 && g == 0 && row_ < t.len) a.delta[first + row_] = delta;
   rows32<W>(q, attn_row<bf16>(a.q, t.b, t.tok0 + min(w0, t.len - 1), h), a.q.st, max(rows, 1), a.K, l);
   if (sc.negate) {
 #pragma unroll
@@ -100,19 +102,28 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_a
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  KeyTiles<W> load(a, kp, vp, t.len, end, w, l);
+  KeyTiles<W> load(a, kp, vp, t.len, end, w, l, KG * CH);
   auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0) __attribute__((always_inline)) {
     load.arrived(ck, cv, j0);
     auto issue = [&](int point) __attribute__((always_inline)) { load.next(nk, nv, j0, point); };
     if (j0 < wend) block(ck, cv, j0, issue);
     else { issue(0); issue(1); issue(2); issue(3); }
   };
-  load.first(s_k0, s_v0);
-  for (int j0 = 0; j0 < end; j0 += 2 * CH) {
-    tile(s_k0, s_v0, s_k1, s_v1, j0);
-    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH);
+  load.first(s_k0, s_v0, kg * CH);
+  for (int j0 = 0; j0 < end; j0 += 2 * KG * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0 + kg * CH);
+    if (j0 + KG * CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + (KG + kg) * CH);
   }
   wait_all_loads();                      // (none may arrive in an LDS that is another's)
+  if constexpr (KG == 2) {
+    const Handed<W> x(a_k0, a_v0, w, l);
+    lds_barrier();
+    if (kg == 1) x.put(dq);
+    lds_barrier();
+    if (kg == 1) return;
+#pragma unroll
+    for (int i = 0; i < 16 * DB; ++i) dq[i / 16][i % 16] += x.at(i);
+  }
   if (rows > 0)
     store_rows32<W>(dq, a.scale, attn_row<bf16>(a.dq, t.b, t.tok0 + w0, h), a.dq.st, rows, a.K, l);
 }

@@ -117,21 +117,21 @@ template <int W> struct KeyTiles {
   typedef TileLoad<W, ATTN_WAVES> Load;
   const lmoe_attn_args& a;
   const bf16 *kp, *vp;
-  int len, last, w, l;       // last: first key of the last tile
+  int len, last, step, w, l;       // last: first key of the last tile; step: keys from one tile to the next
   Load lk, lv;
-  __device__ __forceinline__ KeyTiles(const lmoe_attn_args& a, const bf16* kp, const bf16* vp, int len, int end, int w, int l)
-      : a(a), kp(kp), vp(vp), len(len), last((end - 1) / CH * CH), w(w), l(l), lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l) {}
+  __device__ __forceinline__ KeyTiles(const lmoe_attn_args& a, const bf16* kp, const bf16* vp, int len, int end, int w, int l, int step = CH)
+      : a(a), kp(kp), vp(vp), len(len), last((end - 1) / CH * CH), step(step), w(w), l(l), lk(a.k.st, a.K, w, l), lv(a.v.st, a.V, w, l) {}
   __device__ __forceinline__ void piece(bf16* sk, bf16* sv, int j0, int i) const {
     if (i < Load::PASSES) lk.load(sk, kp + (int64_t)j0 * a.k.st, a.k.st, len - j0, w, i);
     else lv.load(sv, vp + (int64_t)j0 * a.v.st, a.v.st, len - j0, w, i - Load::PASSES);
   }
-  __device__ __forceinline__ void first(bf16* sk, bf16* sv) const {
+  __device__ __forceinline__ void first(bf16* sk, bf16* sv, int j0 = 0) const {
 #pragma unroll
-    for (int i = 0; i < 2 * Load::PASSES; ++i) piece(sk, sv, 0, i);
+    for (int i = 0; i < 2 * Load::PASSES; ++i) piece(sk, sv, min(j0, last), i);
   }
   // of the tile behind the one from j0 on (behind the last one: that once more, so that there is no branch)
   __device__ __forceinline__ void next(bf16* sk, bf16* sv, int j0, int point) const {
-    const int j = min(j0 + CH, last);
+    const int j = min(j0 + step, last);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = point * 2 * Load::PASSES / 4; i < (point + 1) * 2 * Load::PASSES / 4; ++i) piece(sk, sv, j, i);
@@ -192,16 +192,34 @@ __device__ __forceinline__ bool all_finite(const bf16x8& f) {
   return ok;
 }
 
-template <int W, bool CAP, bool BIAS>
-__global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
+// What the second group of waves of a work-group hands to the first: a block of 32 rows per wave, half of a lane's sums through either of
+// two arrays of two tiles
+template <int W> struct Handed {
+  static constexpr int STRIDE = ATTN_WAVES * 64, HALF = W / 4;
+  static_assert(HALF * STRIDE * 4 <= 2 * CH * W * 2, "half of the sums fit an array");
+  float *const x, *const y;
+  __device__ __forceinline__ Handed(bf16* p, bf16* q, int w, int l) : x((float*)p + (w * 64 + l)), y((float*)q + (w * 64 + l)) {}
+  __device__ __forceinline__ float at(int i) const { return (i < HALF ? x : y)[i % HALF * STRIDE]; }
+  __device__ __forceinline__ void put(const f32x16 (&acc)[W / 32]) const {
+#pragma unroll
+    for (int i = 0; i < 2 * HALF; ++i) (i < HALF ? x : y)[i % HALF * STRIDE] = acc[i / 16][i % 16];
+  }
+};
+
+// KG: groups of ATTN_WAVES waves that go through the tiles of the same rows, each through every KG-th; the second hands its sums to the first.
+template <int W, int KG, bool CAP, bool BIAS>
+__global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
+  static_assert(KG == 1 || KG == 2, "one joins the other");
   constexpr int KS = W / 16, DB = W / 32, TILE = CH * W;
   // (arrays of their own, so that the compiler sees that reads of one tile need not wait for loads into the other)
-  __shared__ __attribute__((aligned(1024))) bf16 s_k0[TILE], s_v0[TILE], s_k1[TILE], s_v1[TILE];
+  __shared__ __attribute__((aligned(1024))) bf16 a_k0[KG * TILE], a_v0[KG * TILE], a_k1[KG * TILE], a_v1[KG * TILE];
   zero_behind<bf16>(a, a.o, a.HQ, a.V);
   AttnTile t;
   int h;
   if (!attn_place<ATTN_ROWS>(a, a.HQ, true, h, t)) return;
-  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 5;
+  const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = KG == 1 ? wave_id() : wave_id() % ATTN_WAVES, g = l >> 5;
+  const int kg = KG == 1 ? 0 : wave_id() / ATTN_WAVES;
+  bf16 *const s_k0 = a_k0 + kg * TILE, *const s_v0 = a_v0 + kg * TILE, *const s_k1 = a_k1 + kg * TILE, *const s_v1 = a_v1 + kg * TILE;
   const Score16<CAP, BIAS> sc(a, h);
   const Swz<W> lane(l);
   const int w0 = t.r0 + 32 * w, rows = t.len - w0;                   // the wave's first row, its rows (may be none)
@@ -322,26 +340,40 @@ __global__ __launch_bounds__(ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn
     }
   };
 
-  KeyTiles<W> load(a, kp, vp, t.len, end, w, l);
+  KeyTiles<W> load(a, kp, vp, t.len, end, w, l, KG * CH);
   auto tile = [&](bf16* ck, bf16* cv, bf16* nk, bf16* nv, int j0, auto part_c) __attribute__((always_inline)) {
     load.arrived(ck, cv, j0);
     auto issue = [&](int point) __attribute__((always_inline)) { load.next(nk, nv, j0, point); };
     if (!decltype(part_c)::value || j0 < wend) block(ck, cv, j0, issue, part_c);
     else { issue(0); issue(1); issue(2); issue(3); }
   };
-  load.first(s_k0, s_v0);
-  // (two loops: with both bodies in one, the accumulators move between them)
+  load.first(s_k0, s_v0, kg * CH);
+  // (two loops: with both bodies in one, the accumulators move between them.  The groups take the same number of steps, a last one for
+  // nothing where the tiles do not come out even.)
   int j0 = 0;
-  for (; j0 + 2 * CH <= whole; j0 += 2 * CH) {
-    tile(s_k0, s_v0, s_k1, s_v1, j0, std::false_type());
-    tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::false_type());
+  for (; j0 + 2 * KG * CH <= whole; j0 += 2 * KG * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0 + kg * CH, std::false_type());
+    tile(s_k1, s_v1, s_k0, s_v0, j0 + (KG + kg) * CH, std::false_type());
   }
-  for (; j0 < end; j0 += 2 * CH) {
-    tile(s_k0, s_v0, s_k1, s_v1, j0, std::true_type());
-    if (j0 + CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + CH, std::true_type());
+  for (; j0 < end; j0 += 2 * KG * CH) {
+    tile(s_k0, s_v0, s_k1, s_v1, j0 + kg * CH, std::true_type());
+    if (j0 + KG * CH < end) tile(s_k1, s_v1, s_k0, s_v0, j0 + (KG + kg) * CH, std::true_type());
   }
   wait_all_loads();                      // (none may arrive in an LDS that is another's)
   sum = both_sum(sum);
+  if constexpr (KG == 2) {
+    const Handed<W> x(a_k0, a_v0, w, l);
+    float* const st = (float*)a_k1 + (w * 64 + l);
+    lds_barrier();
+    if (kg == 1) { x.put(o); st[0] = m; st[x.STRIDE] = sum; }
+    lds_barrier();
+    if (kg == 1) return;
+    const float m1 = st[0], next = fmaxf(m, m1), f0 = pow2(m - next), f1 = pow2(m1 - next);
+#pragma unroll
+    for (int i = 0; i < 16 * DB; ++i) o[i / 16][i % 16] = o[i / 16][i % 16] * f0 + x.at(i) * f1;
+    sum = sum * f0 + st[x.STRIDE] * f1;
+    m = next;
+  }
   if (a.lse && g == 0 && row_ < t.len) a.lse[((int64_t)t.b * a.HQ + h) * a.T + t.tok0 + row_] = m + __builtin_amdgcn_logf(sum);
   if (rows > 0)
     store_rows32<W>(o, 1.0f / sum, attn_row<bf16>(a.o, t.b, t.tok0 + w0, h), a.o.st, rows, a.V, l,
