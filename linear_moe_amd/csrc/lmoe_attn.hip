@@ -23,13 +23,16 @@ int64_t attn_groups(const lmoe_attn_args& a) { return attn_tiles<CH>(a) * a.HQ *
 template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
   static bool wide(const lmoe_attn_args& a, int H) { return (int64_t)a.B * a.T * H / 32 >= 2 * cu_count(); }
   template <int RB> static void fwd_strips(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_fwd_any<T, W, RB, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB)), dim3(64 * ANY_WAVES), 0, st, a);
+    const int64_t groups = attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB);
+    hipLaunchKernelGGL((k_attn_fwd_any<T, W, RB, CAP, BIAS>), dim3(groups), dim3(64 * ANY_WAVES), 0, st, a, attn_fold(a, groups, a.HQ, cu_count()));
   }
   template <int RB> static void dq_strips(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_bwd_dq_any<T, W, RB, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB)), dim3(64 * ANY_WAVES), 0, st, a);
+    const int64_t groups = attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB);
+    hipLaunchKernelGGL((k_attn_bwd_dq_any<T, W, RB, CAP, BIAS>), dim3(groups), dim3(64 * ANY_WAVES), 0, st, a, attn_fold(a, groups, a.HQ, cu_count()));
   }
   template <int KB> static void dkv_strips(const lmoe_attn_args& a, hipStream_t st) {
-    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP, BIAS>), dim3(attn_tiles<CH>(a) * a.HKV * (CH / 16 / KB)), dim3(64 * ANY_KV_WAVES), 0, st, a);
+    const int64_t groups = attn_tiles<CH>(a) * a.HKV * (CH / 16 / KB);
+    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP, BIAS>), dim3(groups), dim3(64 * ANY_KV_WAVES), 0, st, a, attn_fold(a, groups, a.HKV, cu_count()));
   }
   static void fwd(const lmoe_attn_args& a, hipStream_t st) {
     if constexpr (W == 64) { if (wide(a, a.HQ)) return fwd_strips<2>(a, st); }

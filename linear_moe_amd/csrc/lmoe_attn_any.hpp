@@ -11,7 +11,7 @@
 // Bound: the fp32 matrix rate.  The waves of a work-group share its rows and take every KW-th tile, since short calls have few
 // rows and many tiles; their sums are joined in LDS in the order of the waves.  2 x 4096 tokens, 16 heads on 4 of 64, causal: forward
 // 0.70 ms, 98 TFLOP/s (a large product of this type reaches 154), backward 2.31 ms, 104 TFLOP/s with the scores formed twice.  2 x
-// 1000 tokens, 4 heads on 2: 25 and 100 us.  (64 rows against 64, every operand staged in LDS: 0.89, 3.40 ms, 80 and 304 us.)
+// 1000 tokens, 4 heads on 2: 22 and 97 us.  (64 rows against 64, every operand staged in LDS: 0.89, 3.40 ms, 80 and 304 us.)
 // 8 waves on the rows of a strip: 2 to 5 % more; tiles loaded two steps ahead: 3 % more.
 #pragma once
 #include "lmoe_attn_fwd.hpp"
@@ -99,14 +99,14 @@ constexpr int ANY_WAVES = 4;         // that share a strip of rows
 constexpr int ANY_KV_WAVES = 8;      // ... of keys
 
 template <typename T, int W, int RB, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_fwd_any(const lmoe_attn_args a) {
+__global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_fwd_any(const lmoe_attn_args a, int fold) {
   constexpr int KW = ANY_WAVES, LD = W + 4;
   __shared__ __attribute__((aligned(16))) float s_o[KW][16 * RB][LD];
   __shared__ float s_m[KW][16 * RB], s_sum[KW][16 * RB];
   zero_behind<T>(a, a.o, a.HQ, a.V);
   AttnTile t;
   int h;
-  if (!attn_place<CH, 16 * RB>(a, a.HQ, true, h, t)) return;
+  if (!attn_place<CH, 16 * RB>(a, a.HQ, true, h, t, fold)) return;
   const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 4, last = t.len - 1;
   const Score<CAP, BIAS, false> sc(a, h);
   const int end = a.causal ? min(t.len, max(t.r0 + 16 * RB, t.prefix)) : t.len, whole = a.causal ? min(t.len, max(t.r0 + 1, t.prefix)) : t.len;
@@ -234,13 +234,13 @@ template <typename T, int KW, int ROWS, int LD> __device__ __forceinline__ void 
 
 // dq of a strip of rows; delta of those rows beside it
 template <typename T, int W, int RB, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmoe_attn_args a) {
+__global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmoe_attn_args a, int fold) {
   constexpr int KW = ANY_WAVES, LD = W + 4;
   __shared__ __attribute__((aligned(16))) float s_dq[KW][16 * RB][LD];
   zero_behind<T>(a, a.dq, a.HQ, a.K);
   AttnTile t;
   int h;
-  if (!attn_place<CH, 16 * RB>(a, a.HQ, true, h, t)) return;
+  if (!attn_place<CH, 16 * RB>(a, a.HQ, true, h, t, fold)) return;
   const int hk = h / (a.HQ / a.HKV), l = lane_id(), w = wave_id(), g = l >> 4, last = t.len - 1;
   const Score<CAP, BIAS, false> sc(a, h);
   const int end = a.causal ? min(t.len, max(t.r0 + 16 * RB, t.prefix)) : t.len, whole = a.causal ? min(t.len, max(t.r0 + 1, t.prefix)) : t.len;
@@ -313,14 +313,14 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmo
 
 // dk, dv of a strip of keys, over the rows of all query heads that share the key head
 template <typename T, int W, int KB, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const lmoe_attn_args a) {
+__global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const lmoe_attn_args a, int fold) {
   constexpr int KW = ANY_KV_WAVES, LD = 2 * W + 4;
   __shared__ __attribute__((aligned(16))) float s_sum[KW][16 * KB][LD];
   zero_behind<T>(a, a.dk, a.HKV, a.K);
   zero_behind<T>(a, a.dv, a.HKV, a.V);
   AttnTile t;
   int hk;
-  if (!attn_place<CH, 16 * KB>(a, a.HKV, false, hk, t)) return;
+  if (!attn_place<CH, 16 * KB>(a, a.HKV, false, hk, t, fold)) return;
   const int G = a.HQ / a.HKV, l = lane_id(), w = wave_id(), g = l >> 4, last = t.len - 1;
   const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0, tiles = (t.len - begin + 15) / 16;
   const int whole = a.causal && t.r0 + 16 * KB > t.prefix ? t.r0 + 16 * KB - 1 : 0;        // from it on rows see all keys of the strip
