@@ -53,23 +53,27 @@ template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
 // its 64 KB of values leave no second work-group room), four with 64 (two work-groups per CU).  2 x 8192 tokens of 16 heads,
 // backward: 8 and 4 waves, 128 columns 1.73 and 2.28 ms, 64 columns 1.04 and 0.94.
 constexpr int attn_kv_waves(int W) { return W == 128 ? 8 : 4; }
-// Work-groups that share the rows of a tile of keys (k_attn_bwd_dkv): so many that the card is full; and twice (64 columns: up to four
-// times) as many if each then still has 64 pieces or more, since the tiles of a causal call are unequal work, those of documents more
-// so.  Each part costs its sums' way through memory.  Backward, 128 columns, 16 heads on 4, with 1 / 2 / 4 / 8 parts: 1 x 1024 tokens
-// 243 / 155 / 106 / 86 us (16 parts: 83), 1 x 4096 929 / 549 / 365 / 384, 8 x 1024 275 / 203 / 214 / 265, 2 x 8192 2411 / 1844 /
-// 1911 / 2017; 16 on 16, 8 x 1024 162 / 278 / 420 / 686.  64 columns, 16 on 4, 2 x 8192 1316 / 1136 / 1034 / 1072.  16384 tokens in
-// documents of which the longest has 5990, 16 on 4 1635 / 1235 / 1229 / 1290, 16 on 16 1102 / 1280 / 1534 / 2094.
-static int attn_parts(const lmoe_attn_args& a) {
-  if (!fits16(a)) return 1;
+// Work-groups that share the rows of a tile of keys (k_attn_bwd_dkv), at most, and the pieces of its stream that each has at least.
+// So many that the card is full; where it is, the tiles of a causal call are unequal work all the same, those of documents more so:
+// two (64 columns: four) for long streams, four for documents of 96 pieces or more.  Each part costs its sums' way through memory.
+// Backward in us, 128 columns, 16 heads on 4, with 1 / 2 / 4 / 8 parts: 1 x 1024 tokens 243 / 155 / 106 / 86 (16 parts: 83), 1 x 4096
+// 929 / 549 / 365 / 384, 8 x 1024 275 / 203 / 214 / 265, 2 x 8192 2411 / 1844 / 1911 / 2017; 16 on 16, 8 x 1024 162 / 278 / 420 / 686.
+// 64 columns, 16 on 4, 2 x 8192 1316 / 1136 / 1034 / 1072.  16384 tokens in documents of which the longest has 5990, one part / two
+// of 4 pieces or more / four of 48: 16 on 4 1677 / 1281 / 1270, 16 on 16 1142 / 1313 / 1159; in 16 equal ones 388 / 448 / 394.
+struct Parts { int most, least; };
+static Parts attn_parts(const lmoe_attn_args& a) {
+  if (!fits16(a)) return {1, 1};
   const int W = a.K <= 64 && a.V <= 64 ? 64 : 128, keys = 32 * attn_kv_waves(W);
   const int64_t groups = (a.cu_seqlens ? std::max<int64_t>(a.T / keys, 1) : (int64_t)a.B * ((a.T + keys - 1) / keys)) * a.HKV;
   const int64_t full = (W == 128 ? 1 : 2) * (int64_t)cu_count(), pieces = ((int64_t)a.T + CH - 1) / CH * (a.HQ / a.HKV);
   int64_t parts = (full + groups - 1) / groups;
-  for (int i = W == 128 ? 1 : 2; i > 0 && groups * parts < (W == 128 && !a.cu_seqlens ? 2 : 4) * full && pieces / parts >= 128; --i) parts *= 2;
-  return (int)std::max<int64_t>(1, std::min(std::min<int64_t>(parts, 16), pieces / 4));
+  const int least = parts == 1 && a.cu_seqlens ? 48 : 4;
+  if (a.cu_seqlens) parts = parts > 1 ? parts : 4;
+  else for (int i = W == 128 ? 1 : 2; i > 0 && groups * parts < (W == 128 ? 2 : 4) * full && pieces / parts >= 128; --i) parts *= 2;
+  return {(int)std::max<int64_t>(1, std::min(std::min<int64_t>(parts, 16), pieces / least)), least};
 }
 int64_t attn_bwd_floats(const lmoe_attn_args& a) {
-  const int parts = a.dk.ptr ? attn_parts(a) : 1;
+  const int parts = a.dk.ptr ? attn_parts(a).most : 1;
   return parts > 1 ? (int64_t)parts * a.B * a.T * a.HKV * (a.K + a.V) : 0;
 }
 
@@ -93,11 +97,10 @@ template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
     else hipLaunchKernelGGL((k_attn_bwd_dq<W, 1, CAP, BIAS>), dim3(groups), dim3(64 * ATTN_WAVES), 0, st, a);
     if (!a.dk.ptr) return;
     constexpr int NW = attn_kv_waves(W);
-    const int parts = attn_parts(a);
-    hipLaunchKernelGGL((k_attn_bwd_dkv<W, NW, CAP, BIAS>), dim3(attn_tiles<32 * NW>(a) * a.HKV, parts), dim3(64 * NW), 0, st, a, parts);
-    if (parts == 1) return;
-    const int64_t blocks = ((int64_t)a.B * a.T * a.HKV * (a.K + a.V) / 4 + NTHR - 1) / NTHR;
-    hipLaunchKernelGGL(k_attn_join, dim3(std::min<int64_t>(blocks, 8 * cu_count())), dim3(NTHR), 0, st, a, parts);
+    const Parts p = attn_parts(a);
+    const dim3 tiles(attn_tiles<32 * NW>(a) * a.HKV);
+    hipLaunchKernelGGL((k_attn_bwd_dkv<W, NW, CAP, BIAS>), dim3(tiles.x, p.most), dim3(64 * NW), 0, st, a, p.most, p.least);
+    if (p.most > 1) hipLaunchKernelGGL((k_attn_join<32 * NW>), dim3(tiles.x, 32 * NW / JOIN_ROWS), dim3(NTHR), 0, st, a, p.most, p.least);
   }
 };
 

@@ -1,6 +1,9 @@
 // Softmax attention, backward pass on 2-byte elements: dq by rows, then dk and dv by keys, each with the scores formed again.
 // (One kernel for all three would add dq up in memory, in an order that changes from run to run, or write every tile's share of
 // it: T / 256 times the bytes of dq.  Two score products more cost less.)
+// Bound: the matrix rate; dk and dv also LDS, from which a wave reads 40 KB for every 32 products of 32 x 32 x 16, more than 128 bytes a
+// cycle of a CU.  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.47 ms, 1120 TFLOP/s, dk and dv 2.04 ms, 1078, counted with the
+// scores each forms again; the whole by the five products that it cannot do without 781.
 #pragma once
 #include "lmoe_attn_fwd.hpp"
 
@@ -145,10 +148,20 @@ template <int W> __device__ __forceinline__ void store_sums(const f32x16 (&acc)[
 // their lse and delta.  Rows behind the sequence come with lse = infinity, so that their p is 0.
 // From the last row to the first, the heads of a row tile one after the other: the work-groups of a key head, whose rows begin at
 // different places but end at one, read the same tiles at about the same time, and an XCD's L2 holds them for all.
-// Where the keys are too few for the card, `parts` work-groups share them, each with its part of that stream, and leave fp32 sums
-// for k_attn_join (parts = 1: the gradients themselves).
+// Where the keys are too few for the card, or unequal work, up to `parts` work-groups share a tile of them, each with its part of that
+// stream (`least` of its pieces or more), and leave fp32 sums for k_attn_join; alone, a work-group leaves the gradients themselves.
+// The stream of a tile of keys: 64-row tiles top .. begin / 64 of G heads
+struct KeyStream {
+  int begin, top, all, parts;
+  __device__ __forceinline__ KeyStream(const lmoe_attn_args& a, const AttnTile& t, int most, int least) {
+    begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;              // the first row that sees a key of the tile
+    top = (t.len - 1) / CH;
+    all = (top - begin / CH + 1) * (a.HQ / a.HKV);
+    parts = max(1, min(most, all / least));
+  }
+};
 template <int W, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_args a, int parts) {
+__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_args a, int most, int least) {
   constexpr int KS = W / 16, DB = W / 32, KEYS = NW * 32, TILE = CH * W;
   __shared__ __attribute__((aligned(1024))) bf16 s_q0[TILE], s_d0[TILE], s_q1[TILE], s_d1[TILE], s_v[KEYS * W];
   __shared__ __attribute__((aligned(16))) float s_row[2][2][CH];          // lse, delta
@@ -159,6 +172,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   AttnTile t;
   int hk;
   if (!attn_place<KEYS>(a, a.HKV, false, hk, t)) return;
+  const KeyStream of(a, t, most, least);
+  const int parts = of.parts;
+  if ((int)blockIdx.y >= parts) return;
   const int G = a.HQ / a.HKV, tid = threadIdx.x, l = lane_id(), w = wave_id(), g = l >> 5;
   const Swz<W> lane(l);
   const int w0 = t.r0 + 32 * w, keys = t.len - w0, key_ = w0 + (l & 31);
@@ -171,7 +187,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b) { dk[b] = zero16(); dv[b] = zero16(); }
-  const int begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;                              // the first row that sees a key of the tile
   const int wbegin = keys <= 0 ? t.len : a.causal && w0 >= t.prefix ? w0 : 0;             // ... of the wave
   const int wwhole = a.causal && w0 + 32 > t.prefix ? w0 + 31 : 0;                         // from it on rows see all keys of the wave
 
@@ -241,7 +256,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   typedef TileLoad<W, NW> Load;
   const Load lq(a.q.st, a.K, w, l), ld(a.d_o.st, a.V, w, l);
   // The stream: tiles of 64 rows from the last to the first, per tile the heads.  Of it the work-group takes pieces m0 .. m1 - 1.
-  const int top = (t.len - 1) / CH, all = (top - begin / CH + 1) * G;
+  const int top = of.top, all = of.all;
   const int m0 = (int)((int64_t)all * blockIdx.y / parts), m1 = (int)((int64_t)all * (blockIdx.y + 1) / parts);
   struct Place { int m, h, i; } cur = {m0, m0 % G, (top - m0 / G) * CH}, next = cur;
   auto advance = [&](Place& x) { ++x.m; if (++x.h == G) { x.h = 0; x.i -= CH; } };
@@ -309,23 +324,27 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
   }
 }
 
-// dk and dv of a key head's rows from the sums of the parts: [parts][B, T, HKV][K + V]
-__global__ __launch_bounds__(NTHR) void k_attn_join(const lmoe_attn_args a, int parts) {
-  const int per = (a.K + a.V) / 4;
-  const int64_t rows = (int64_t)a.B * a.T * a.HKV, all = rows * per;
-  const int end = a.cu_seqlens ? as_const(a.cu_seqlens)[a.N] : a.T;
-  for (int64_t i = (int64_t)blockIdx.x * NTHR + threadIdx.x; i < all; i += (int64_t)gridDim.x * NTHR) {
-    const int64_t row = i / per;
-    const int c = (int)(i - row * per) * 4, h = (int)(row % a.HKV);
-    const int64_t tok = row / a.HKV;
-    const int b = (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
-    if (t >= end) continue;
+// dk and dv of a tile of KEYS keys that several work-groups shared, from their sums: [parts][B, T, HKV][K + V].
+// A work-group takes JOIN_ROWS of the tile (blockIdx.y).
+constexpr int JOIN_ROWS = 8;
+template <int KEYS>
+__global__ __launch_bounds__(NTHR) void k_attn_join(const lmoe_attn_args a, int most, int least) {
+  AttnTile t;
+  int hk;
+  if (!attn_place<KEYS>(a, a.HKV, false, hk, t)) return;
+  const int parts = KeyStream(a, t, most, least).parts, per = (a.K + a.V) / 4;
+  if (parts == 1) return;
+  const int64_t rows = (int64_t)a.B * a.T * a.HKV, first = ((int64_t)t.b * a.T + t.tok0 + t.r0) * a.HKV + hk;
+  const int end = min((int)blockIdx.y * JOIN_ROWS + JOIN_ROWS, t.len - t.r0);
+  for (int i = blockIdx.y * JOIN_ROWS * per + threadIdx.x; i < end * per; i += NTHR) {
+    const int r = i / per, c = (i - r * per) * 4;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) x += *(const f32x4*)(a.ws + ((int64_t)p * rows + row) * (a.K + a.V) + c);
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) x += *(const f32x4*)(a.ws + ((int64_t)p * rows + first + (int64_t)r * a.HKV) * (a.K + a.V) + c);
     bf16x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (bf16)x[e];
-    *(bf16x4*)(c < a.K ? attn_row<bf16>(a.dk, b, t, h) + c : attn_row<bf16>(a.dv, b, t, h) + c - a.K) = y;
+    *(bf16x4*)(c < a.K ? attn_row<bf16>(a.dk, t.b, t.tok0 + t.r0 + r, hk) + c : attn_row<bf16>(a.dv, t.b, t.tok0 + t.r0 + r, hk) + c - a.K) = y;
   }
 }
 

@@ -4,10 +4,14 @@
 // on one pair of tiles, the next is loaded into the other.  Two work-groups share a CU, and no barrier holds them to one
 // another: while one wave of a SIMD has the matrix unit, the other has the vector unit.  (One work-group of eight waves, 128 keys
 // between two barriers: 2 x 8192 tokens, 16 heads of 128, 580 us in place of 556, of 64 362 in place of 322; with its two
-// halves held half a step apart by barriers, and the tiles of one step in one phase, 20 % more.)  A wave works on S^T = K Q^T (32 x 32 blocks of v_mfma_f32_32x32x16_bf16, q held in registers), so
-// that a lane has one row of the scores (with its neighbour 32 lanes on): maximum, sum and scale factors are one number per
-// lane.  O^T += V^T P^T takes P^T from the registers it is in (the contraction index may be numbered freely) and V^T through
-// the transposing LDS read.
+// halves held half a step apart by barriers, and the tiles of one step in one phase, 20 % more.)
+// A wave works on S^T = K Q^T (32 x 32 blocks of v_mfma_f32_32x32x16_bf16, q held in registers), so that a lane has one row of the
+// scores (with its neighbour 32 lanes on): maximum, sum and scale factors are one number per lane.  O^T += V^T P^T takes P^T from
+// the registers it is in (the contraction index may be numbered freely) and V^T through the transposing LDS read.
+//
+// Bound: the matrix rate and, as much, the vector unit's 32 exponentials and 170 other operations per 64 keys of a wave, which take it as
+// long as the products take the matrix unit.  4 x 8192 tokens, 16 heads on 4 of 128, causal: 1.13 ms, 976 TFLOP/s (a product of 8192^3
+// reaches 1133); with a cap, whose two more of the slow operations per score make the vector unit the longer, 760; heads of 64 840.
 #pragma once
 #include "lmoe_attn.hpp"
 
