@@ -1,6 +1,5 @@
 // Softmax attention: instances and dispatch.
 #include <algorithm>
-#include <cstdlib>
 #include <type_traits>
 
 #include "lmoe_attn_any.hpp"
@@ -8,11 +7,11 @@
 
 namespace lmoe {
 
-// the kernels on 2-byte elements reach the rows of a tile by 32-bit offsets
+// the kernels on 2-byte elements reach the rows of a tile by unsigned 32-bit offsets
 static bool fits16(const lmoe_attn_args& a) {
-  int64_t stride = 0;
-  for (const lmoe_tensor* x : {&a.q, &a.k, &a.v, &a.d_o}) stride = std::max(stride, std::abs(x->st));
-  return a.dtype == LMOE_BF16 && stride < (1 << 24);
+  for (const lmoe_tensor* x : {&a.q, &a.k, &a.v, &a.d_o})
+    if (x->st < 0 || x->st >= 1 << 24) return false;
+  return a.dtype == LMOE_BF16;
 }
 // (without them: four strips to 64 rows, 512 threads each)
 int64_t attn_groups(const lmoe_attn_args& a) { return attn_tiles<CH>(a) * a.HQ * (fits16(a) ? 1 : 8); }

@@ -197,7 +197,10 @@ def softmax_attn(
     j < its sequence's prefix.  ``causal=False``: all.
     cu_seqlens: packed documents as in the chunk ops; rows of one never see another's (nor what it holds: a NaN stays in its
     document).  Rows behind the last document are zero in o and in the gradients.
-    Without atomics: the gradients of a key head are summed over its query heads in a fixed order."""
+    Without atomics: the gradients of a key head are summed over its query heads in a fixed order.  A NaN or infinity in the k or v of a
+    token stays out of the outputs of rows that do not see it; out of their gradients it stays in another document only.
+    Forward and backward capture into a HIP graph; capture with leaves of which no graph of an eager step lives any more (torch's
+    accumulation nodes belong to the stream of their first use)."""
     grad = not no_node(q, k, v)
     node = grad and no_transform()                   # (a node of the graph, in native code)
     if cu_seqlens is None and (node or not grad):    # (what the native path takes as it is, it also checks)

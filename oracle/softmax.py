@@ -24,10 +24,10 @@ def _rel(u_sum, smax, K, n, cap):
     return 2 * ((K + 8) * w * u_sum + (6 * smax + 16 * cap) * w) + (n + 16) * w
 
 
-def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dtype=torch.float64):
+def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dtype=torch.float64, low=True):
     """One head of one sequence: q [n, K], k [m, K], v [m, V], the last of the n queries at the last of the m keys.
     Returns o and its bound; with do also (dq, dk, dv) and their bounds (to be rounded and summed by the caller: the bounds
-    leave out the final rounding of dk and dv)."""
+    leave out the final rounding of dk and dv).  low=False: delta from o as it is rounded."""
     w = 2.0 ** -24
     u = 2.0 ** -24 if dtype in (torch.float32, torch.float64) else torch.finfo(dtype).eps / 2
     q, k, v = q.double(), k.double(), v.double()
@@ -50,7 +50,7 @@ def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dty
     do = do.double()
     dp, delta = do @ v.T, (do * o).sum(1, keepdim=True)
     err_dp = V * w * (do.abs() @ v.abs().T)
-    err_delta = (do.abs() * (err_o - (u - min(u, 2.0 ** -15)) * o.abs())).sum(1, keepdim=True) + V * w * (do * o).abs().sum(1, keepdim=True)
+    err_delta = (do.abs() * (err_o - (u - min(u, 2.0 ** -15) if low else 0.0) * o.abs())).sum(1, keepdim=True) + V * w * (do * o).abs().sum(1, keepdim=True)
     fac = 1 - th * th
     ds = p * (dp - delta) * fac
     err_ds = (u + rel) * ds.abs() + p * (err_dp + err_delta) + (8 * w * p * (dp - delta).abs() if cap else 0.0)
@@ -62,7 +62,7 @@ def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dty
     return o, err_o, (dq, dk, dv), (err_dq, err_dk, err_dv)
 
 
-def attn(q, k, v, scale=None, causal=True, softcap=0.0, slopes=None, prefix_lens=None, cu=None, do=None):
+def attn(q, k, v, scale=None, causal=True, softcap=0.0, slopes=None, prefix_lens=None, cu=None, do=None, low=True):
     """[B, T, H, D] on the CPU, in the type the kernel is given.  Returns {name: (value, bound)} for o and, with do, dq, dk, dv."""
     B, T, HQ, K = q.shape
     HKV, G = k.shape[2], q.shape[2] // k.shape[2]
@@ -79,7 +79,7 @@ def attn(q, k, v, scale=None, causal=True, softcap=0.0, slopes=None, prefix_lens
             at, kv = (b, slice(t0, t1), h), (b, slice(t0, t1), h // G)
             prefix = 0 if prefix_lens is None else min(max(int(prefix_lens[n]), 0), t1 - t0)
             r = head(q[at], k[kv], v[kv], scale, causal, softcap, 0.0 if slopes is None else float(slopes[h]), prefix,
-                     None if do is None else do[at], q.dtype)
+                     None if do is None else do[at], q.dtype, low)
             out["o"][0][at], out["o"][1][at] = r[0], r[1]
             if do is not None:
                 for name, where, x, e in zip(("dq", "dk", "dv"), (at, kv, kv), r[2], r[3]):

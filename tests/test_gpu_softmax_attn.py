@@ -1,9 +1,12 @@
 """softmax_attn on the GPU against float64: the outputs and gradients element by element, within the bounds that
 oracle/softmax.py derives from the kernels' roundings."""
+import ctypes as C
+
 import pytest
 import torch
 
 import linear_moe_amd as L
+from linear_moe_amd import _lib
 from oracle import softmax
 from tests.util import gen
 
@@ -275,6 +278,40 @@ def test_repeated_calls_agree_bit_for_bit_and_on_another_stream(cuda, dtype):
     torch.cuda.current_stream().wait_stream(s)
     for a, b, c in zip(first, second, all_of()):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("backwards", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_library_called_for_itself(cuda, D, backwards):
+    """A backward pass without o_low, and rows that lie in memory from the last to the first."""
+    T, HQ, HKV = 300, 4, 2
+    q, k, v, do = inputs(107, 1, T, HQ, HKV, D, D, BF16)
+    want = softmax.attn(q, k, v, do=do, low=False)
+    dev = [x.flip(1).contiguous().to(cuda) if backwards else x.to(cuda) for x in (q, k, v, do)]
+    out = [torch.zeros_like(dev[i]) for i in (0, 0, 1, 2)]
+    lse, delta = (torch.zeros(HQ, T, device=cuda) for _ in range(2))
+
+    def rows(x):
+        at = (T - 1) * x.stride(1) if backwards else 0
+        return _lib.Tensor4(x.data_ptr() + 2 * at, x.stride(0), -x.stride(1) if backwards else x.stride(1), x.stride(2))
+
+    a = _lib.AttnArgs()
+    a.dtype, a.causal, a.scale = _lib.LMOE_BF16, 1, D ** -0.5
+    a.B, a.T, a.HQ, a.HKV, a.K, a.V, a.N, a.NT = 1, T, HQ, HKV, D, D, 1, (T + 63) // 64
+    a.q, a.k, a.v, a.d_o = map(rows, dev)
+    a.o, a.dq, a.dk, a.dv = map(rows, out)
+    a.lse, a.delta = lse.data_ptr(), delta.data_ptr()
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    assert lib.lmoe_softmax_attn_fwd(C.byref(a), st) == 0, lib.lmoe_last_error()
+    floats = lib.lmoe_softmax_attn_bwd_floats(C.byref(a))
+    assert (floats > 0) == (not backwards)                    # (few keys: their rows are shared)
+    if floats:
+        assert lib.lmoe_softmax_attn_bwd(C.byref(a), st) == -11
+    ws = torch.empty(max(floats, 1), device=cuda)
+    a.ws = ws.data_ptr()
+    assert lib.lmoe_softmax_attn_bwd(C.byref(a), st) == 0, lib.lmoe_last_error()
+    for name, x in zip(("o", "dq", "dk", "dv"), out):
+        softmax.check(x.flip(1) if backwards else x, want[name], name)
 
 
 def test_no_tokens(cuda):

@@ -47,7 +47,8 @@ def attn_args(**kw):
     (-5, dict(cu_seqlens=FAKE, chunk_map=FAKE)), (-4, dict(cu_seqlens=FAKE, chunk_map=FAKE, B=1, NT=6)), (-7, dict(k=_lib.Tensor4())),
     (-11, dict(dk=_lib.Tensor4())), (-15, dict(softcap=-1.0)), (-15, dict(softcap=float("nan"))), (-15, dict(softcap=float("inf"))),
     (-15, dict(causal=0, prefix_lens=FAKE)), (-9, dict(q=_lib.Tensor4(FAKE + 2, 0, 256, 64))), (-9, dict(dv=_lib.Tensor4(FAKE, 0, 260, 64))),
-    (-8, dict(T=2 ** 30, NT=2 ** 25))])
+    (-8, dict(T=2 ** 30, NT=2 ** 25)),
+    (-9, dict(o_low=FAKE + 4)), (-8, dict(dtype=_lib.LMOE_F32, T=2 ** 20, HQ=128, HKV=128, NT=2 ** 15))])
 def test_softmax_attn_blocks_that_are_refused(code, kw):
     lib = _lib.load()
     for fn in (lib.lmoe_softmax_attn_fwd, lib.lmoe_softmax_attn_bwd):
@@ -79,7 +80,7 @@ def paged_args(**kw):
 
 @pytest.mark.parametrize("code,kw", [
     (-2, dict(dtype=5)), (-3, dict(K=160)), (-3, dict(V=4)), (-4, dict(S=0)), (-4, dict(M=-1)), (-4, dict(HKV=0)), (-8, dict(N=70000)),
-    (-8, dict(M=2 ** 20, S=2 ** 12)), (-7, dict(lens=None)), (-7, dict(table=None)), (-7, dict(vp=_lib.Tensor4())), (-11, dict(vn=_lib.Tensor4())),
+    (-8, dict(M=2 ** 20, S=2 ** 12)), (-8, dict(M=2 ** 25 + 1, S=2 ** 5)), (-7, dict(lens=None)), (-7, dict(table=None)), (-7, dict(vp=_lib.Tensor4())), (-11, dict(vn=_lib.Tensor4())),
     (-9, dict(kp=_lib.Tensor4(FAKE, 2048, 130, 64))), (-9, dict(kn=_lib.Tensor4(FAKE + 8, 2048, 128, 64)))])
 def test_paged_blocks_that_are_refused(code, kw):
     lib = _lib.load()
