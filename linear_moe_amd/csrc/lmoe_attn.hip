@@ -49,7 +49,7 @@ template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
 };
 
 // Keys of a work-group of k_attn_bwd_dkv: as many waves as have registers for both sums on a CU, eight with 128 columns (two per SIMD;
-// its 64 KB of values leave no second work-group room), four with 64 (two work-groups per CU).  2 x 8192 tokens of 16 heads,
+// its 64 KB of values leave no second work-group room), four with 64 (three work-groups per CU).  2 x 8192 tokens of 16 heads,
 // backward: 8 and 4 waves, 128 columns 1.73 and 2.28 ms, 64 columns 1.04 and 0.94.
 constexpr int attn_kv_waves(int W) { return W == 128 ? 8 : 4; }
 // Work-groups that share the rows of a tile of keys (k_attn_bwd_dkv), at most, and the pieces of its stream that each has at least.

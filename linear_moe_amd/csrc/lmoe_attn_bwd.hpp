@@ -1,9 +1,10 @@
 // Softmax attention, backward pass on 2-byte elements: dq by rows, then dk and dv by keys, each with the scores formed again.
 // (One kernel for all three would add dq up in memory, in an order that changes from run to run, or write every tile's share of
 // it: T / 256 times the bytes of dq.  Two score products more cost less.)
-// Bound: the matrix rate; dk and dv also LDS, from which a wave reads 40 KB for every 32 products of 32 x 32 x 16, more than 128 bytes a
-// cycle of a CU.  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.47 ms, 1120 TFLOP/s, dk and dv 2.04 ms, 1078, counted with the
-// scores each forms again; the whole by the five products that it cannot do without 781.
+// Bound: the matrix rate (the matrix unit is busy for 57 % of the cycles of dq, 49 % of those of dk and dv, in which the waves wait
+// for LDS and the barrier the rest of the time; LDS is busy for 37 %).  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.47 ms,
+// 1120 TFLOP/s, dk and dv 2.01 ms, 1095, counted with the scores each forms again; the whole by the five products that it cannot do
+// without 790.
 #pragma once
 #include "lmoe_attn_fwd.hpp"
 
@@ -161,8 +162,9 @@ struct KeyStream {
   }
 };
 template <int W, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_args a, int most, int least) {
+__global__ __launch_bounds__(NW * 64, W == 64 ? 3 : 2) void k_attn_bwd_dkv(const lmoe_attn_args a, int most, int least) {
   constexpr int KS = W / 16, DB = W / 32, KEYS = NW * 32, TILE = CH * W;
+  constexpr int A1 = 2, A2 = 4;
   __shared__ __attribute__((aligned(1024))) bf16 s_q0[TILE], s_d0[TILE], s_q1[TILE], s_d1[TILE], s_v[KEYS * W];
   __shared__ __attribute__((aligned(16))) float s_row[2][2][CH];          // lse, delta
   if (blockIdx.y == 0) {
@@ -196,16 +198,22 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
       const Swz<W> at = lane.fresh();
       const int key = fresh_index(key_);
       f32x16 s = zero16(), dp = zero16();
-      bf16x8 f[2 * DB], y[2], z[2];
       __builtin_amdgcn_sched_barrier(0);
-      // (pieces of two steps at a time: the registers hold no more)
+      // (128 columns: the pieces of a step are asked for two steps before their products, in this order.  Left to itself the compiler asks for
+      // each right in front of its product and waits for it; with 64 it has registers for more, and three waves a SIMD: 2 x 8192
+      // tokens, 16 heads on 4, backward 1.062 ms, in this order 1.075; of 128 with a cap 2.228 and 2.188)
+      bf16x8 f[A1], y[A1], z[A1];
+      auto read = [&](int j) { f[j % A1] = at.frag(sq, b, j); y[j % A1] = at.frag(sd, b, j); z[j % A1] = at.frag(sv, 0, j); };
 #pragma unroll
-      for (int j = 0; j < KS; j += 2) {
+      for (int j = 0; j < A1; ++j) read(j);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) { f[x] = at.frag(sq, b, j + x); y[x] = at.frag(sd, b, j + x); z[x] = at.frag(sv, 0, j + x); }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) { s = mfma32(f[x], k[j + x], s); dp = mfma32(y[x], z[x], dp); }
+      for (int j = 0; j < KS; ++j) {
+        if constexpr (W == 128) __builtin_amdgcn_sched_barrier(0);
+        s = mfma32(f[j % A1], k[j], s);
+        dp = mfma32(y[j % A1], z[j % A1], dp);
+        if (j + A1 < KS) read(j + A1);
       }
+      __builtin_amdgcn_sched_barrier(0);
       issue(2 * b);
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
@@ -231,24 +239,18 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attn_bwd_dkv(const lmoe_attn_arg
         }
       }
       const bf16x8 p0 = frag_of_acc(s, 0), p1 = frag_of_acc(s, 1), ds0 = frag_of_acc(dp, 0), ds1 = frag_of_acc(dp, 1);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) f[x * DB + d] = at.frag_t(sd, 2 * b + x, d);
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) dv[d] = mfma32(f[x * DB + d], x ? p1 : p0, dv[d]);
       issue(2 * b + 1);
+      bf16x8 t[A2];
+      auto read_t = [&](int n) { t[n % A2] = at.frag_t(n < 2 * DB ? sd : sq, 2 * b + n / DB % 2, n % DB); };
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int n = 0; n < A2; ++n) read_t(n);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) f[x * DB + d] = at.frag_t(sq, 2 * b + x, d);
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) dk[d] = mfma32(f[x * DB + d], x ? ds1 : ds0, dk[d]);
+      for (int n = 0; n < 4 * DB; ++n) {
+        if constexpr (W == 128) __builtin_amdgcn_sched_barrier(0);
+        if (n < 2 * DB) dv[n % DB] = mfma32(t[n % A2], n / DB % 2 ? p1 : p0, dv[n % DB]);
+        else dk[n % DB] = mfma32(t[n % A2], n / DB % 2 ? ds1 : ds0, dk[n % DB]);
+        if (n + A2 < 4 * DB) read_t(n + A2);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
