@@ -1,8 +1,8 @@
 // Softmax attention, backward pass on 2-byte elements: dq by rows, then dk and dv by keys, each with the scores formed again.
 // (One kernel for all three would add dq up in memory, in an order that changes from run to run, or write every tile's share of
 // it: T / 256 times the bytes of dq.  Two score products more cost less.)
-// Bound: the matrix rate (the matrix unit is busy for 57 % of the cycles of dq, 49 % of those of dk and dv, in which the waves wait
-// for LDS and the barrier the rest of the time; LDS is busy for 37 %).  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.47 ms,
+// Bound: the matrix rate (the matrix unit is busy for 59 % of the cycles of dq, 55 % of those of dk and dv, in which a third of the
+// waves' time goes to waiting for LDS and the barrier; LDS itself is busy for 41 %).  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.47 ms,
 // 1120 TFLOP/s, dk and dv 2.01 ms, 1095, counted with the scores each forms again; the whole by the five products that it cannot do
 // without 790.
 #pragma once
