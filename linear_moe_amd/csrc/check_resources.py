@@ -29,6 +29,8 @@ GUARDED = {
     "k_gla_fwd_fused": 3,
     "k_state_bwd": 4,         # two work-groups of 8 waves per CU; see FLOORS
     "k_gla_bwd_dqkg": 2,      # K = 64: two work-groups of 8 waves per CU, see FLOORS
+    "k_attn_fwd": 2,          # two work-groups of 4 waves per CU, or one of 8: a spill in the loop waits for the tiles in flight
+    "k_attn_bwd_dq": 2,
     "k_bwd_dqkv": 2,          # one work-group of 8 waves per CU; its first version spilled loop-invariant lane arithmetic
 }
 ANY_TYPE = ("k_state_bwd", "k_state_fwd_chunks")
@@ -73,7 +75,7 @@ def main(paths):
                 # Itanium mangling: <len><name>I<template args>; DF16b = __bf16
                 if f"{len(kern)}{kern}I" not in name:
                     continue
-                two_byte = f"{kern}IDF16b" in name or kern.endswith("_reg") or "_seg_" in kern     # exist for bf16 only
+                two_byte = f"{kern}IDF16b" in name or kern.endswith("_reg") or "_seg_" in kern or kern.startswith("k_attn")     # exist for bf16 only
                 line = (f"{kern:<18} {'bf16' if two_byte else 'fp32'} vgpr {r.get('vgpr', -1):3d} agpr {r.get('agpr', -1):3d} "
                         f"scratch {r.get('scratch', -1):4d} B  vgpr-spill {r.get('vspill', -1):3d}  waves/SIMD {r.get('occ', -1)}  "
                         f"lds {r.get('lds', -1)}  {name}")
