@@ -2,8 +2,8 @@
 // (One kernel for all three would add dq up in memory, in an order that changes from run to run, or write every tile's share of
 // it: T / 256 times the bytes of dq.  Two score products more cost less.)
 // Bound: the matrix rate (the matrix unit is busy for 59 % of the cycles of dq, 55 % of those of dk and dv, in which a third of the
-// waves' time goes to waiting for LDS and the barrier; LDS itself is busy for 41 %).  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.47 ms,
-// 1120 TFLOP/s, dk and dv 2.01 ms, 1095, counted with the scores each forms again; the whole by the five products that it cannot do
+// waves' time goes to waiting for LDS and the barrier; LDS itself is busy for 41 %).  4 x 8192 tokens, 16 heads on 4 of 128, causal: dq 1.44 ms,
+// 1146 TFLOP/s, dk and dv 2.02 ms, 1089, counted with the scores each forms again; the whole by the five products that it cannot do
 // without 790.
 #pragma once
 #include "lmoe_attn_fwd.hpp"
@@ -14,7 +14,7 @@ namespace lmoe {
 // whose lse and delta are one number, and dS^T as the B operand of dQ^T += K^T dS^T.
 template <int W, int KG, bool CAP, bool BIAS>
 __global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
-  constexpr int KS = W / 16, DB = W / 32, TILE = CH * W;
+  constexpr int KS = W / 16, DB = W / 32, TILE = CH * W, A1 = 3;
   __shared__ __attribute__((aligned(1024))) bf16 a_k0[KG * TILE], a_v0[KG * TILE], a_k1[KG * TILE], a_v1[KG * TILE];
   zero_behind<bf16>(a, a.dq, a.HQ, a.K);
   AttnTile t;
@@ -62,18 +62,22 @@ __global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const l
   auto block = [&](const bf16* sk, const bf16* sv, int j0, auto issue) __attribute__((always_inline)) {
     const Swz<W> at = lane.fresh();
     const int row = fresh_index(row_);
-    bf16x8 kf[2], vf[2], kt[2 * DB];
+    // (pieces are asked for A1 steps before their products, those of the second half under the last products of the first: 4 x 8192
+    // tokens, 16 heads on 4 of 128, 1.44 ms, with each pair asked for right in front of its products 1.47; two or four steps: the same)
+    bf16x8 kf[A1], vf[A1], kt[2 * DB];
+    auto read = [&](int b, int j) { kf[j % A1] = at.frag(sk, b, j); vf[j % A1] = at.frag(sv, b, j); };
+#pragma unroll
+    for (int j = 0; j < A1; ++j) read(0, j);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       __builtin_amdgcn_sched_barrier(0);
       f32x16 s = zero16(), dp = zero16();
-      // (pieces of two steps at a time: the registers hold no more)
 #pragma unroll
-      for (int j = 0; j < KS; j += 2) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) { kf[x] = at.frag(sk, b, j + x); vf[x] = at.frag(sv, b, j + x); }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) { s = mfma32(kf[x], q[j + x], s); dp = mfma32(vf[x], d_o[j + x], dp); }
+      for (int j = 0; j < KS; ++j) {
+        s = mfma32(kf[j % A1], q[j], s);
+        dp = mfma32(vf[j % A1], d_o[j], dp);
+        if (j + A1 < KS) read(b, j + A1);
+        __builtin_amdgcn_sched_barrier(0);
       }
       issue(2 * b);
       __builtin_amdgcn_sched_barrier(0);
@@ -96,6 +100,10 @@ __global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const l
         for (int i = 0; i < 16; ++i) s[i] = row32(i) < sees ? s[i] : 0.f;
       }
       issue(2 * b + 1);
+      if (b == 0) {
+#pragma unroll
+        for (int j = 0; j < A1; ++j) read(1, j);
+      }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const bf16x8 ds = frag_of_acc(s, x);
