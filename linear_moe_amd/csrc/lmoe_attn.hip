@@ -16,6 +16,14 @@ static bool fits16(const lmoe_attn_args& a) {
 // (without them: four strips to 64 rows, 512 threads each)
 int64_t attn_groups(const lmoe_attn_args& a) { return attn_tiles<CH>(a) * a.HQ * (fits16(a) ? 1 : 8); }
 
+// Work-groups that share the rows of a strip of keys (k_attn_bwd_dkv_any): two where there are too few strips for the unequal work of a
+// causal call to come out even, or for half of the card.  Backward with 1 / 2 / 3 / 4 work-groups, us: 2 x 1000 tokens, 4 heads on 2 of
+// 64 98 / 88 / 101 / 101, of 128 191 / 160 / 182 / 178; 1 x 2048 190 / 162 / 177 / 172, not causal 206 / 215 / 220 / 226; 1 x 500, 16 on 4
+// of 128 159 / 113 / 109 / 113.
+static int any_parts(const lmoe_attn_args& a) {
+  const int64_t strips = (int64_t)a.B * ((a.T + 15) / 16) * a.HKV;
+  return a.T >= 256 && strips <= (a.causal ? cu_count() : cu_count() / 2) ? 2 : 1;
+}
 // A strip of 32 rows reads each tile half as often as two of 16, which with 64 columns gains where the strips fill the card all the same:
 // 8 x 2048 tokens, 8 heads, forward 413 us in place of 448, backward 1307 in place of 1652; 2 x 1000, 4 heads on 2, 31 and 127 in
 // place of 25 and 100.  (With 128 columns there are no registers for 32.)
@@ -31,7 +39,9 @@ template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
   }
   template <int KB> static void dkv_strips(const lmoe_attn_args& a, hipStream_t st) {
     const int64_t groups = attn_tiles<CH>(a) * a.HKV * (CH / 16 / KB);
-    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP, BIAS>), dim3(groups), dim3(64 * ANY_KV_WAVES), 0, st, a, attn_fold(a, groups, a.HKV, cu_count()));
+    const int parts = any_parts(a);
+    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP, BIAS>), dim3(groups, parts), dim3(64 * ANY_KV_WAVES), 0, st, a, attn_fold(a, groups, a.HKV, cu_count()), parts);
+    if (parts > 1) hipLaunchKernelGGL((k_attn_join<T, CH>), dim3(attn_tiles<CH>(a) * a.HKV, CH / JOIN_ROWS), dim3(NTHR), 0, st, a, parts, 0);
   }
   static void fwd(const lmoe_attn_args& a, hipStream_t st) {
     if constexpr (W == 64) { if (wide(a, a.HQ)) return fwd_strips<2>(a, st); }
@@ -61,7 +71,7 @@ constexpr int attn_kv_waves(int W) { return W == 128 ? 8 : 4; }
 // of 4 pieces or more / four of 48: 16 on 4 1677 / 1281 / 1270, 16 on 16 1142 / 1313 / 1159; in 16 equal ones 388 / 448 / 394.
 struct Parts { int most, least; };
 static Parts attn_parts(const lmoe_attn_args& a) {
-  if (!fits16(a)) return {1, 1};
+  if (!fits16(a)) return {any_parts(a), 0};
   const int W = a.K <= 64 && a.V <= 64 ? 64 : 128, keys = 32 * attn_kv_waves(W);
   const int64_t groups = (a.cu_seqlens ? std::max<int64_t>(a.T / keys, 1) : (int64_t)a.B * ((a.T + keys - 1) / keys)) * a.HKV;
   const int64_t full = (W == 128 ? 1 : 2) * (int64_t)cu_count(), pieces = ((int64_t)a.T + CH - 1) / CH * (a.HQ / a.HKV);
@@ -99,7 +109,7 @@ template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
     const Parts p = attn_parts(a);
     const dim3 tiles(attn_tiles<32 * NW>(a) * a.HKV);
     hipLaunchKernelGGL((k_attn_bwd_dkv<W, NW, CAP, BIAS>), dim3(tiles.x, p.most), dim3(64 * NW), 0, st, a, p.most, p.least);
-    if (p.most > 1) hipLaunchKernelGGL((k_attn_join<32 * NW>), dim3(tiles.x, 32 * NW / JOIN_ROWS), dim3(NTHR), 0, st, a, p.most, p.least);
+    if (p.most > 1) hipLaunchKernelGGL((k_attn_join<bf16, 32 * NW>), dim3(tiles.x, 32 * NW / JOIN_ROWS), dim3(NTHR), 0, st, a, p.most, p.least);
   }
 };
 

@@ -162,6 +162,12 @@ inline int attn_fold(const lmoe_attn_args& a, int64_t groups, int H, int cus) {
   const int64_t pairs = (int64_t)a.B * H;
   return a.causal && !a.cu_seqlens && groups > cus && groups <= 2 * (int64_t)cus && cus % pairs == 0 ? (int)(cus / pairs) : INT32_MAX;
 }
+template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 x) {
+  typename ET<T>::vec4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = ET<T>::from_f(x[i]);
+  *(typename ET<T>::vec4*)p = y;
+}
 template <typename T> __device__ __forceinline__ T* attn_row(const lmoe_tensor& x, int b, int t, int h) {
   return (T*)x.ptr + (int64_t)b * x.sb + (int64_t)t * x.st + (int64_t)h * x.sh;
 }

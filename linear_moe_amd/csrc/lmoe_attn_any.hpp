@@ -11,22 +11,16 @@
 // Bound: the fp32 matrix rate.  The waves of a work-group share its rows and take every KW-th tile, since short calls have few
 // rows and many tiles; their sums are joined in LDS in the order of the waves.  2 x 4096 tokens, 16 heads on 4 of 64, causal: forward
 // 0.70 ms, 98 TFLOP/s (a large product of this type reaches 154), backward 2.31 ms, 104 TFLOP/s with the scores formed twice.  2 x
-// 1000 tokens, 4 heads on 2: 22 and 97 us.  (64 rows against 64, every operand staged in LDS: 0.89, 3.40 ms, 80 and 304 us.)
+// 1000 tokens, 4 heads on 2: 22 and 88 us.  (64 rows against 64, every operand staged in LDS: 0.89, 3.40 ms, 80 and 304 us.)
 // 8 waves on the rows of a strip: 2 to 5 % more; tiles loaded two steps ahead: 3 % more.
 #pragma once
-#include "lmoe_attn_fwd.hpp"
+#include "lmoe_attn_bwd.hpp"
 
 namespace lmoe {
 
 template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
   const typename ET<T>::vec4 x = *(const typename ET<T>::vec4*)p;
   return f32x4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-}
-template <typename T> __device__ __forceinline__ void store4(T* p, f32x4 x) {
-  typename ET<T>::vec4 y;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = ET<T>::from_f(x[i]);
-  *(typename ET<T>::vec4*)p = y;
 }
 // the two lane groups of 16 (of each half), then the two halves
 __device__ __forceinline__ void pairs16(float x, float& a, float& b) {
@@ -311,13 +305,16 @@ __global__ __launch_bounds__(64 * ANY_WAVES, 2) void k_attn_bwd_dq_any(const lmo
   join_rows<T>(s_dq, 0, a.scale, attn_row<T>(a.dq, t.b, t.tok0 + t.r0, h), a.dq.st, t.len - t.r0, a.K);
 }
 
-// dk, dv of a strip of keys, over the rows of all query heads that share the key head
+// dk, dv of a strip of keys, over the rows of all query heads that share the key head.  parts > 1: that many work-groups share them, and
+// leave fp32 sums for k_attn_join.
 template <typename T, int W, int KB, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const lmoe_attn_args a, int fold) {
+__global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const lmoe_attn_args a, int fold, int parts) {
   constexpr int KW = ANY_KV_WAVES, LD = 2 * W + 4;
   __shared__ __attribute__((aligned(16))) float s_sum[KW][16 * KB][LD];
-  zero_behind<T>(a, a.dk, a.HKV, a.K);
-  zero_behind<T>(a, a.dv, a.HKV, a.V);
+  if (blockIdx.y == 0) {
+    zero_behind<T>(a, a.dk, a.HKV, a.K);
+    zero_behind<T>(a, a.dv, a.HKV, a.V);
+  }
   AttnTile t;
   int hk;
   if (!attn_place<CH, 16 * KB>(a, a.HKV, false, hk, t, fold)) return;
@@ -337,8 +334,10 @@ __global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const
     zero_sums<W>(dk[b]);
     zero_sums<W>(dv[b]);
   }
-  // The stream: the tiles of a head, head by head.  A wave takes every KW-th (behind the last: one of the last head, unused).
-  int x = w % tiles, h = w / tiles;
+  // The stream: the tiles of a head, head by head.  Of the parts' waves each takes every so many-th (behind the last: one of the last head,
+  // unused).
+  const int stride = KW * parts, mine = blockIdx.y * KW + w;
+  int x = mine % tiles, h = mine / tiles;
   float lse[4], delta[4];
   auto rows = [&] {
     const int hq = hk * G + min(h, G - 1), i0 = begin + 16 * x;
@@ -378,7 +377,7 @@ __global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const
         if constexpr (CAP) d *= 1.0f - th * th;
         ds[b][e] = ok ? d : 0.f;
       }
-    for (x += KW; x >= tiles && h < G; x -= tiles) ++h;
+    for (x += stride; x >= tiles && h < G; x -= tiles) ++h;
     rows();                                                        // (of the next step, under the rest of this one)
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
@@ -392,8 +391,15 @@ __global__ __launch_bounds__(64 * ANY_KV_WAVES, 2) void k_attn_bwd_dkv_any(const
     put_sums<W>(dv[b], s_sum[w][16 * b + (l & 15)] + W, l);
   }
   __syncthreads();
-  join_rows<T>(s_sum, 0, a.scale, attn_row<T>(a.dk, t.b, t.tok0 + t.r0, hk), a.dk.st, t.len - t.r0, a.K);
-  join_rows<T>(s_sum, W, 1.0f, attn_row<T>(a.dv, t.b, t.tok0 + t.r0, hk), a.dv.st, t.len - t.r0, a.V);
+  const int n = t.len - t.r0;
+  if (parts == 1) {
+    join_rows<T>(s_sum, 0, a.scale, attn_row<T>(a.dk, t.b, t.tok0 + t.r0, hk), a.dk.st, n, a.K);
+    join_rows<T>(s_sum, W, 1.0f, attn_row<T>(a.dv, t.b, t.tok0 + t.r0, hk), a.dv.st, n, a.V);
+  } else {
+    const int64_t D = a.K + a.V, row = ((int64_t)blockIdx.y * a.B * a.T + (int64_t)t.b * a.T + t.tok0 + t.r0) * a.HKV + hk;
+    join_rows<float>(s_sum, 0, a.scale, a.ws + row * D, a.HKV * D, n, a.K);
+    join_rows<float>(s_sum, W, 1.0f, a.ws + row * D + a.K, a.HKV * D, n, a.V);
+  }
 }
 
 }  // namespace lmoe

@@ -166,7 +166,7 @@ struct KeyStream {
     begin = a.causal && t.r0 >= t.prefix ? t.r0 : 0;              // the first row that sees a key of the tile
     top = (t.len - 1) / CH;
     all = (top - begin / CH + 1) * (a.HQ / a.HKV);
-    parts = max(1, min(most, all / least));
+    parts = least ? max(1, min(most, all / least)) : most;        // (0: all of them, whatever the stream)
   }
 };
 template <int W, int NW, bool CAP, bool BIAS>
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(NW * 64, W == 64 ? 3 : 2) void k_attn_bwd_dkv(const
 // dk and dv of a tile of KEYS keys that several work-groups shared, from their sums: [parts][B, T, HKV][K + V].
 // A work-group takes JOIN_ROWS of the tile (blockIdx.y).
 constexpr int JOIN_ROWS = 8;
-template <int KEYS>
+template <typename T, int KEYS>
 __global__ __launch_bounds__(NTHR) void k_attn_join(const lmoe_attn_args a, int most, int least) {
   AttnTile t;
   int hk;
@@ -351,10 +351,7 @@ __global__ __launch_bounds__(NTHR) void k_attn_join(const lmoe_attn_args a, int 
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) x += *(const f32x4*)(a.ws + ((int64_t)p * rows + first + (int64_t)r * a.HKV) * (a.K + a.V) + c);
-    bf16x4 y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (bf16)x[e];
-    *(bf16x4*)(c < a.K ? attn_row<bf16>(a.dk, t.b, t.tok0 + t.r0 + r, hk) + c : attn_row<bf16>(a.dv, t.b, t.tok0 + t.r0 + r, hk) + c - a.K) = y;
+    store4(c < a.K ? attn_row<T>(a.dk, t.b, t.tok0 + t.r0 + r, hk) + c : attn_row<T>(a.dv, t.b, t.tok0 + t.r0 + r, hk) + c - a.K, x);
   }
 }
 
