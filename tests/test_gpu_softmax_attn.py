@@ -91,14 +91,15 @@ def test_rows_far_apart(cuda, causal):
         softmax.check(x, want[name], name)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("N", [64, 65, 256, 257])
-def test_many_documents(cuda, N):
+def test_many_documents(cuda, N, dtype):
     """Up to and beyond the number of documents that a work-group looks through for its tile."""
     lens = [(7 * n) % 5 + (130 if n % 50 == 9 else 0) for n in range(N)]
     cu = [0]
     for n in lens:
         cu.append(cu[-1] + n)
-    x = inputs(89, 1, cu[-1] + 3, 2, 1, 64, 64, BF16)
+    x = inputs(89, 1, cu[-1] + 3, 2, 1, 64, 64, dtype)
     x[3][:, cu[-1]:] = 0                        # (rows behind the last document)
     run_and_check(cuda, *x, cu=cu)
 
