@@ -27,20 +27,20 @@ static int any_parts(const lmoe_attn_args& a) {
 // A strip of 32 rows reads each tile half as often as two of 16, which with 64 columns gains where the strips fill the card all the same:
 // 8 x 2048 tokens, 8 heads, forward 413 us in place of 448, backward 1307 in place of 1652; 2 x 1000, 4 heads on 2, 31 and 127 in
 // place of 25 and 100.  (With 128 columns there are no registers for 32.)
-template <typename T, int W, bool CAP, bool BIAS> struct AttnAny {
+template <typename T, int W, int CAP, bool BIAS> struct AttnAny {
   static bool wide(const lmoe_attn_args& a, int H) { return (int64_t)a.B * a.T * H / 32 >= 2 * cu_count(); }
   template <int RB> static void fwd_strips(const lmoe_attn_args& a, hipStream_t st) {
     const int64_t groups = attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB);
-    hipLaunchKernelGGL((k_attn_fwd_any<T, W, RB, CAP, BIAS>), dim3(groups), dim3(64 * ANY_WAVES), 0, st, a, attn_fold(a, groups, a.HQ, cu_count()));
+    hipLaunchKernelGGL((k_attn_fwd_any<T, W, RB, CAP != NO_CAP, BIAS>), dim3(groups), dim3(64 * ANY_WAVES), 0, st, a, attn_fold(a, groups, a.HQ, cu_count()));
   }
   template <int RB> static void dq_strips(const lmoe_attn_args& a, hipStream_t st) {
     const int64_t groups = attn_tiles<CH>(a) * a.HQ * (CH / 16 / RB);
-    hipLaunchKernelGGL((k_attn_bwd_dq_any<T, W, RB, CAP, BIAS>), dim3(groups), dim3(64 * ANY_WAVES), 0, st, a, attn_fold(a, groups, a.HQ, cu_count()));
+    hipLaunchKernelGGL((k_attn_bwd_dq_any<T, W, RB, CAP != NO_CAP, BIAS>), dim3(groups), dim3(64 * ANY_WAVES), 0, st, a, attn_fold(a, groups, a.HQ, cu_count()));
   }
   template <int KB> static void dkv_strips(const lmoe_attn_args& a, hipStream_t st) {
     const int64_t groups = attn_tiles<CH>(a) * a.HKV * (CH / 16 / KB);
     const int parts = any_parts(a);
-    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP, BIAS>), dim3(groups, parts), dim3(64 * ANY_KV_WAVES), 0, st, a, attn_fold(a, groups, a.HKV, cu_count()), parts);
+    hipLaunchKernelGGL((k_attn_bwd_dkv_any<T, W, KB, CAP != NO_CAP, BIAS>), dim3(groups, parts), dim3(64 * ANY_KV_WAVES), 0, st, a, attn_fold(a, groups, a.HKV, cu_count()), parts);
     if (parts > 1) hipLaunchKernelGGL((k_attn_join<T, CH>), dim3(attn_tiles<CH>(a) * a.HKV, CH / JOIN_ROWS), dim3(NTHR), 0, st, a, parts, 0);
   }
   static void fwd(const lmoe_attn_args& a, hipStream_t st) {
@@ -94,7 +94,7 @@ static bool two_groups(const lmoe_attn_args& a, int64_t groups) {
   return (groups <= cu_count() && a.T >= 384) || (a.causal && groups <= 2 * cu_count() && a.T >= 2048);
 }
 
-template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
+template <typename T, int W, int CAP, bool BIAS> struct Attn16 {
   static void fwd(const lmoe_attn_args& a, hipStream_t st) {
     const int64_t groups = attn_tiles<ATTN_ROWS>(a) * a.HQ;
     if (two_groups(a, groups)) hipLaunchKernelGGL((k_attn_fwd<W, 2, CAP, BIAS>), dim3(groups), dim3(128 * ATTN_WAVES), 0, st, a);
@@ -113,18 +113,21 @@ template <typename T, int W, bool CAP, bool BIAS> struct Attn16 {
   }
 };
 
-template <template <typename, int, bool, bool> class F, typename T, int W> static void by_score(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
+template <template <typename, int, int, bool> class F, typename T, int W, int FAR> static void by_score(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
   auto run = [&](auto f) { if (bwd) f.bwd(a, st); else f.fwd(a, st); };
-  if (a.softcap > 0.f) { if (a.slopes) run(F<T, W, true, true>()); else run(F<T, W, true, false>()); }
-  else if (a.slopes) run(F<T, W, false, true>());
-  else run(F<T, W, false, false>());
+  if (a.softcap > CAP_NEAR) { if (a.slopes) run(F<T, W, FAR, true>()); else run(F<T, W, FAR, false>()); }
+  else if (a.softcap > 0.f) { if (a.slopes) run(F<T, W, NEAR_CAP, true>()); else run(F<T, W, NEAR_CAP, false>()); }
+  else if (a.slopes) run(F<T, W, NO_CAP, true>());
+  else run(F<T, W, NO_CAP, false>());
 }
+// (the kernels with products in fp32 have one form for all caps)
+template <typename T, int W> static void by_score_any(const lmoe_attn_args& a, bool bwd, hipStream_t st) { by_score<AttnAny, T, W, NEAR_CAP>(a, bwd, st); }
 static void attn(const lmoe_attn_args& a, bool bwd, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;
-  if (fits16(a)) { if (narrow) by_score<Attn16, bf16, 64>(a, bwd, st); else by_score<Attn16, bf16, 128>(a, bwd, st); }
-  else if (a.dtype == LMOE_BF16) { if (narrow) by_score<AttnAny, bf16, 64>(a, bwd, st); else by_score<AttnAny, bf16, 128>(a, bwd, st); }
-  else if (narrow) by_score<AttnAny, float, 64>(a, bwd, st);
-  else by_score<AttnAny, float, 128>(a, bwd, st);
+  if (fits16(a)) { if (narrow) by_score<Attn16, bf16, 64, FAR_CAP>(a, bwd, st); else by_score<Attn16, bf16, 128, FAR_CAP>(a, bwd, st); }
+  else if (a.dtype == LMOE_BF16) { if (narrow) by_score_any<bf16, 64>(a, bwd, st); else by_score_any<bf16, 128>(a, bwd, st); }
+  else if (narrow) by_score_any<float, 64>(a, bwd, st);
+  else by_score_any<float, 128>(a, bwd, st);
 }
 void launch_attn_fwd(const lmoe_attn_args& a, hipStream_t st) { attn(a, false, st); }
 void launch_attn_bwd(const lmoe_attn_args& a, hipStream_t st) { attn(a, true, st); }

@@ -25,20 +25,39 @@ namespace lmoe {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float M_LOW = -1e30f;
 
+// 1 - 2 / (1 + e^{2z}) is off by an ulp of 1 whatever tanh(z) itself is, and a score by an ulp of the cap: 1.2e-4 at a cap of 1024, a
+// thirtieth of the rounding of p to a bfloat16.  The kernels on 2-byte elements take that form for caps up to it, and beyond it one whose
+// error is relative (the near form would be off by 1.2e-3 in the score at a cap of 1e4, by 0.09 at 1e6).
+constexpr float CAP_NEAR = 1024.0f;
+enum { NO_CAP, NEAR_CAP, FAR_CAP };
+// Below 1/4 by the series, whose next term is 2^-27 of the sum; from there on the form above is off by 16 ulps of the number at most.
+__device__ __forceinline__ float tanh_far(float z) {
+  const float y = z * z;
+  float x = __builtin_fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f);
+  x = __builtin_fmaf(y, x, 2.0f / 15.0f);
+  x = __builtin_fmaf(y, x, -1.0f / 3.0f);
+  x = __builtin_fmaf(z * y, x, z);
+  const float t = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * (2.0f * LOG2E))), 1.0f);
+  return fabsf(z) < 0.25f ? x : t;
+}
+// (caps above 2^100 are as good as that one: the cap and scale / cap stay normal numbers)
+__device__ __forceinline__ float cap_in_range(float softcap) { return fminf(softcap, 0x1p100f); }
+
 // What turns a product q . k into a score to the base 2.  CAP, BIAS: the call has a cap / slopes.
 template <bool CAP, bool BIAS, bool FAST> struct Score {
-  float mul;       // without a cap: scale log2(e);  with one: scale / cap (fast: 2 log2(e) scale / cap)
+  float mul;       // without a cap: scale log2(e);  with one: scale / cap
   float out;       // cap log2(e)
   float slope;     // slope log2(e)
   __device__ __forceinline__ Score(float scale, float softcap, const float* slopes, int h) {
-    mul = CAP ? scale / softcap * (FAST ? 2.0f * LOG2E : 1.0f) : scale * LOG2E;
-    out = softcap * LOG2E;
+    const float cap = cap_in_range(softcap);
+    mul = CAP ? scale / cap : scale * LOG2E;
+    out = cap * LOG2E;
     slope = BIAS ? slopes[h] * LOG2E : 0.f;
   }
   __device__ __forceinline__ Score(const lmoe_attn_args& a, int h) : Score(a.scale, a.softcap, a.slopes, h) {}
-  // tanh(x / cap) of a product.  Fast: 1 - 2 / (1 + e^{2z}), whose error of an ulp of 1 is an ulp of the cap in the score.
+  // tanh(x / cap) of a product (fast: with the hardware's exponential and reciprocal)
   __device__ __forceinline__ float squash(float qk) const {
-    if constexpr (FAST) return __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(qk * mul)), 1.0f);
+    if constexpr (FAST) return tanh_far(qk * mul);
     else return tanhf(qk * mul);
   }
   // dist = i - j, th = squash(qk) where there is a cap
@@ -50,26 +69,30 @@ template <bool CAP, bool BIAS, bool FAST> struct Score {
 };
 
 // The same for the kernels on 2-byte elements, which keep a number u per pair that grows with the score, s = a u + b, so that a score
-// less a maximum (or lse) is one multiply-add:  u = q . k (q negated for a negative scale);  with a cap u = -1 / (1 + e^{2x / cap}),
-// tanh = 1 + 2 u, a = 2 b = 2 cap;  with slopes u = s.
-template <bool CAP, bool BIAS> struct Score16 {
-  float mul, cap2, slope, a, b;
+// less a maximum (or lse) is one multiply-add:  u = q . k (q negated for a negative scale);  with a cap up to CAP_NEAR
+// u = -1 / (1 + e^{2x / cap}), tanh = 1 + 2 u, a = 2 b = 2 cap;  with one beyond u = tanh, a = cap, b = 0;  with slopes u = s.
+template <int CAP, bool BIAS> struct Score16 {
+  float mul, wide, slope, a, b;        // wide: cap times two, or the cap
   bool negate;
   __device__ __forceinline__ Score16(const lmoe_attn_args& x, int h) {
-    negate = !CAP && !BIAS && x.scale < 0.f;
-    mul = CAP ? x.scale / x.softcap * (2.0f * LOG2E) : x.scale * LOG2E;
-    cap2 = 2.0f * x.softcap * LOG2E;
+    const float cap = cap_in_range(x.softcap);
+    negate = CAP == NO_CAP && !BIAS && x.scale < 0.f;
+    mul = CAP == NEAR_CAP ? x.scale / cap * (2.0f * LOG2E) : CAP == FAR_CAP ? x.scale / cap : x.scale * LOG2E;
+    wide = (CAP == FAR_CAP ? 1.0f : 2.0f) * cap * LOG2E;
     slope = BIAS ? x.slopes[h] * LOG2E : 0.f;
     // (a > 0 also for a scale of 0: a hidden score of -infinity stays one)
-    a = BIAS ? 1.0f : CAP ? cap2 : fmaxf(fabsf(mul), 1e-37f);
-    b = !BIAS && CAP ? 0.5f * cap2 : 0.f;
+    a = BIAS ? 1.0f : CAP ? wide : fmaxf(fabsf(mul), 1e-37f);
+    b = !BIAS && CAP == NEAR_CAP ? 0.5f * wide : 0.f;
   }
-  // r: the factor of the cap, (1 - tanh^2) / 4 = -r (1 + r); dist = i - j
+  // r: what fade() is made of; dist = i - j
   __device__ __forceinline__ float operator()(float qk, float dist, float& r) const {
-    if constexpr (CAP) r = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(qk * mul));
-    if constexpr (BIAS) return __builtin_fmaf(-slope, fabsf(dist), CAP ? __builtin_fmaf(r, cap2, 0.5f * cap2) : qk * mul);
+    if constexpr (CAP == NEAR_CAP) r = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(qk * mul));
+    if constexpr (CAP == FAR_CAP) r = tanh_far(qk * mul);
+    if constexpr (BIAS) return __builtin_fmaf(-slope, fabsf(dist), CAP == NEAR_CAP ? __builtin_fmaf(r, wide, 0.5f * wide) : CAP == FAR_CAP ? r * wide : qk * mul);
     return CAP ? r : qk;
   }
+  // the factor of the cap, 1 - tanh^2
+  static __device__ __forceinline__ float fade(float r) { return CAP == NEAR_CAP ? -4.0f * __builtin_fmaf(r, r, r) : __builtin_fmaf(-r, r, 1.0f); }
 };
 
 // (to an ulp or so; what lies below 2^-126 becomes 0, beside numbers of which one is 1)

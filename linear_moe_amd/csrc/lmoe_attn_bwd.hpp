@@ -12,7 +12,7 @@ namespace lmoe {
 
 // dq of 128 rows; delta of those rows beside it.  As the forward kernel: S^T = K Q^T and dP^T = V dO^T leave a lane with one row,
 // whose lse and delta are one number, and dS^T as the B operand of dQ^T += K^T dS^T.
-template <int W, int KG, bool CAP, bool BIAS>
+template <int W, int KG, int CAP, bool BIAS>
 __global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const lmoe_attn_args a) {
   constexpr int KS = W / 16, DB = W / 32, TILE = CH * W, A1 = 3;
   __shared__ __attribute__((aligned(1024))) bf16 a_k0[KG * TILE], a_v0[KG * TILE], a_k1[KG * TILE], a_v1[KG * TILE];
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_bwd_dq(const l
         float r;
         const float u = sc(s[i], (float)(row - j), r);
         float ds = pow2(__builtin_fmaf(u, sc.a, off)) * (dp[i] - delta);
-        if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
+        if constexpr (CAP) ds *= sc.fade(r);
         s[i] = ds;
       }
       if (j0 + 32 * b + 32 > wwhole) {
@@ -169,7 +169,7 @@ struct KeyStream {
     parts = least ? max(1, min(most, all / least)) : most;        // (0: all of them, whatever the stream)
   }
 };
-template <int W, int NW, bool CAP, bool BIAS>
+template <int W, int NW, int CAP, bool BIAS>
 __global__ __launch_bounds__(NW * 64, W == 64 ? 3 : 2) void k_attn_bwd_dkv(const lmoe_attn_args a, int most, int least) {
   constexpr int KS = W / 16, DB = W / 32, KEYS = NW * 32, TILE = CH * W;
   constexpr int A1 = 2, A2 = 4;
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(NW * 64, W == 64 ? 3 : 2) void k_attn_bwd_dkv(const
           const float u = sc(s[e + x], (float)(i - key), r);
           float p = pow2(__builtin_fmaf(u, sc.a, sc.b - lse[x]));
           float ds = p * (dp[e + x] - delta[x]);
-          if constexpr (CAP) ds *= -4.0f * __builtin_fmaf(r, r, r);
+          if constexpr (CAP) ds *= sc.fade(r);
           s[e + x] = p;
           dp[e + x] = ds;
         }
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(NW * 64, W == 64 ? 3 : 2) void k_attn_bwd_dkv(const
     }
     advance(cur);
   };
-  if (!CAP && !BIAS && a.scale < 0.f) {
+  if (CAP == NO_CAP && !BIAS && a.scale < 0.f) {
 #pragma unroll
     for (int j = 0; j < KS; ++j) frag_negate(k[j]);
   }

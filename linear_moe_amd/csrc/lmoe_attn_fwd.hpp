@@ -211,7 +211,7 @@ template <int W> struct Handed {
 };
 
 // KG: groups of ATTN_WAVES waves that go through the tiles of the same rows, each through every KG-th; the second hands its sums to the first.
-template <int W, int KG, bool CAP, bool BIAS>
+template <int W, int KG, int CAP, bool BIAS>
 __global__ __launch_bounds__(KG * ATTN_WAVES * 64, 2) void k_attn_fwd(const lmoe_attn_args a) {
   static_assert(KG == 1 || KG == 2, "one joins the other");
   constexpr int KS = W / 16, DB = W / 32, TILE = CH * W;

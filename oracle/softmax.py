@@ -1,4 +1,4 @@
-"""Softmax attention in float64 on the CPU, one pair of tokens at a time in the formulas, and how far a kernel may be off.
+"""Softmax attention in float64, one pair of tokens at a time in the formulas, and how far a kernel may be off.
 
 The bounds follow from the roundings that the kernels make, worst case, element by element.  u is half a step of the element
 type relative to the value (``torch.finfo(t).eps / 2``), w the same of float32.
@@ -6,6 +6,7 @@ type relative to the value (``torch.finfo(t).eps / 2``), w the same of float32.
 * score: a sum of K products in float32, (K + 8) w scale sum_d |q_d k_d|; the cap's tanh and the bias a few w of their size;
   the scale to the base 2 a w of the score.  The exponential turns an absolute error of the score into a relative one of p, and so
   does the sum: twice the largest of the row, and (n + 16) w for n terms of the sum and the exponentials themselves: ``rel``.
+  The tanh of a cap is off by 16 w, of itself where the cap is above 1024 (CAP_NEAR of the kernels), else of 1.
 * o: the products take p rounded to the element type (u), o is rounded once: u |o| + (u + rel + n w) sum_j p |v|.
 * dv: the same with do in place of v, summed over rows (and heads).
 * delta = do . o from o to 2^-15 (2-byte elements: o and what its rounding left, in 2^-8 of the last place): sum_d |do_d| err(o_d)
@@ -21,7 +22,7 @@ import torch
 
 def _rel(u_sum, smax, K, n, cap):
     w = 2.0 ** -24
-    return 2 * ((K + 8) * w * u_sum + (6 * smax + 16 * cap) * w) + (n + 16) * w
+    return 2 * ((K + 8) * w * u_sum + (6 * smax + 16 * (cap if cap <= 1024 else smax)) * w) + (n + 16) * w
 
 
 def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dtype=torch.float64, low=True):
@@ -32,12 +33,12 @@ def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dty
     u = 2.0 ** -24 if dtype in (torch.float32, torch.float64) else torch.finfo(dtype).eps / 2
     q, k, v = q.double(), k.double(), v.double()
     n, m, K, V = q.shape[0], k.shape[0], q.shape[1], v.shape[1]
-    i, j = torch.arange(m - n, m)[:, None], torch.arange(m)[None, :]
-    ok = (j <= i) | (j < prefix) if causal else torch.ones(n, m, dtype=torch.bool)
+    i, j = torch.arange(m - n, m, device=q.device)[:, None], torch.arange(m, device=q.device)[None, :]
+    ok = (j <= i) | (j < prefix) if causal else torch.ones(n, m, dtype=torch.bool, device=q.device)
     x = scale * (q @ k.T)
     th = torch.tanh(x / cap) if cap else torch.zeros_like(x)
     s = (cap * th if cap else x) - slope * (i - j).abs()
-    s = torch.where(ok, s, torch.tensor(-math.inf, dtype=torch.float64))
+    s = torch.where(ok, s, -math.inf)
     p = torch.softmax(s, 1)
     p = torch.where(ok, p, torch.zeros_like(p))
     sums = torch.where(ok, abs(scale) * (q.abs() @ k.abs().T), torch.zeros_like(x)).amax(1, keepdim=True)
@@ -63,11 +64,11 @@ def head(q, k, v, scale, causal=True, cap=0.0, slope=0.0, prefix=0, do=None, dty
 
 
 def attn(q, k, v, scale=None, causal=True, softcap=0.0, slopes=None, prefix_lens=None, cu=None, do=None, low=True):
-    """[B, T, H, D] on the CPU, in the type the kernel is given.  Returns {name: (value, bound)} for o and, with do, dq, dk, dv."""
+    """[B, T, H, D], in the type the kernel is given.  Returns {name: (value, bound)} for o and, with do, dq, dk, dv."""
     B, T, HQ, K = q.shape
     HKV, G = k.shape[2], q.shape[2] // k.shape[2]
     scale = K ** -0.5 if scale is None else scale
-    z = lambda x, c=None: torch.zeros(*x.shape[:3], c or x.shape[3], dtype=torch.float64)
+    z = lambda x, c=None: torch.zeros(*x.shape[:3], c or x.shape[3], dtype=torch.float64, device=x.device)
     out = {"o": (z(q, v.shape[3]), z(q, v.shape[3]))}
     if do is not None:
         out.update(dq=(z(q), z(q)), dk=(z(k), z(k)), dv=(z(v), z(v)))
@@ -94,7 +95,8 @@ def attn(q, k, v, scale=None, causal=True, softcap=0.0, slopes=None, prefix_lens
 
 def check(got, want, what=""):
     """got: tensor; want: (value, bound).  The float64 sums of the oracle are exact beside the bounds."""
-    x, (ref, bound) = got.detach().cpu().double(), want
+    ref, bound = want
+    x = got.detach().to(ref.device).double()
     assert x.shape == ref.shape, (what, x.shape, ref.shape)
     assert torch.isfinite(x).all(), f"{what}: not finite"
     off = (x - ref).abs() - bound - 1e-30
