@@ -42,6 +42,11 @@ __device__ __forceinline__ float tanh_far(float z) {
 }
 // (caps above 2^100 are as good as that one: the cap and scale / cap stay normal numbers)
 __device__ __forceinline__ float cap_in_range(float softcap) { return fminf(softcap, 0x1p100f); }
+// (finite for the least of caps as well: a product of 0 has a score of 0)
+__device__ __forceinline__ float over_cap(float scale, float cap) {
+  const float x = scale / cap;
+  return fabsf(x) > 1e38f ? copysignf(1e38f, x) : x;
+}
 
 // What turns a product q . k into a score to the base 2.  CAP, BIAS: the call has a cap / slopes.
 template <bool CAP, bool BIAS, bool FAST> struct Score {
@@ -50,7 +55,7 @@ template <bool CAP, bool BIAS, bool FAST> struct Score {
   float slope;     // slope log2(e)
   __device__ __forceinline__ Score(float scale, float softcap, const float* slopes, int h) {
     const float cap = cap_in_range(softcap);
-    mul = CAP ? scale / cap : scale * LOG2E;
+    mul = CAP ? over_cap(scale, cap) : scale * LOG2E;
     out = cap * LOG2E;
     slope = BIAS ? slopes[h] * LOG2E : 0.f;
   }
@@ -77,7 +82,7 @@ template <int CAP, bool BIAS> struct Score16 {
   __device__ __forceinline__ Score16(const lmoe_attn_args& x, int h) {
     const float cap = cap_in_range(x.softcap);
     negate = CAP == NO_CAP && !BIAS && x.scale < 0.f;
-    mul = CAP == NEAR_CAP ? x.scale / cap * (2.0f * LOG2E) : CAP == FAR_CAP ? x.scale / cap : x.scale * LOG2E;
+    mul = CAP == NEAR_CAP ? over_cap(x.scale, cap) * (2.0f * LOG2E) : CAP == FAR_CAP ? over_cap(x.scale, cap) : x.scale * LOG2E;
     wide = (CAP == FAR_CAP ? 1.0f : 2.0f) * cap * LOG2E;
     slope = BIAS ? x.slopes[h] * LOG2E : 0.f;
     // (a > 0 also for a scale of 0: a hidden score of -infinity stays one)

@@ -10,6 +10,7 @@
 #include <Python.h>
 #include <dlfcn.h>
 
+#include <cfloat>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
@@ -757,6 +758,17 @@ bool number(float& to, PyObject* o, float otherwise) {
   to = (float)x;
   return true;
 }
+// a cap (None or 0: none); one below the least normal number counts as that, so that it stays one in 32 bits
+bool cap_from(float& to, PyObject* o) {
+  double x = 0.;
+  if (o != Py_None) {
+    x = PyFloat_AsDouble(o);
+    if (x == -1.0 && PyErr_Occurred()) return false;
+  }
+  NEED(x >= 0. && x < 3e38);
+  to = x > 0. ? std::max((float)x, FLT_MIN) : 0.f;
+  return true;
+}
 // slopes or None: one fp32 number per head, not trained
 bool slopes_from(Tensor& to, PyObject* o, int dev, int64_t H) {
   NEED(plain_or_none(to, o, dev));
@@ -794,7 +806,7 @@ struct Attn {
       a.seq_order = (const int32_t*)ptr(tables[3]); a.nt_dev = (const int32_t*)ptr(tables[4]);
     }
     NEED(NT <= INT32_MAX);
-    NEED(number(a.scale, o[3], (float)std::pow((double)K, -0.5)) && number(a.softcap, o[5], 0.f) && a.softcap >= 0.f && a.softcap < 3e38f);
+    NEED(number(a.scale, o[3], (float)std::pow((double)K, -0.5)) && cap_from(a.softcap, o[5]));
     a.causal = yes(o[4]);
     NEED(slopes_from(slopes, o[6], dev, HQ) && plain_or_none(prefix, o[7], dev));
     if (prefix.defined()) NEED(a.causal && ints_from(prefix, N));
@@ -1008,7 +1020,7 @@ PyObject* paged_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (HQ < 1 || !fits(HQ) || HQ % c.a.HKV || !c.tokens(q, o[4], c.a.N, 1, HQ, c.a.K, hf) || (o[5] == Py_None) != (o[6] == Py_None)) return elsewhere();
   if (o[5] != Py_None && !(c.tokens(k, o[5], c.a.N, 1, c.a.HKV, c.a.K, hf) && c.tokens(v, o[6], c.a.N, 1, c.a.HKV, c.a.V, hf))) return elsewhere();
   c.a.HQ = HQ;
-  if (!number(c.a.scale, o[7], (float)std::pow((double)c.a.K, -0.5)) || !number(c.a.softcap, o[8], 0.f) || !(c.a.softcap >= 0.f && c.a.softcap < 3e38f) ||
+  if (!number(c.a.scale, o[7], (float)std::pow((double)c.a.K, -0.5)) || !cap_from(c.a.softcap, o[8]) ||
       !slopes_from(slopes, o[9], c.dev, HQ)) return elsewhere();
   c.a.slopes = (const float*)ptr(slopes);
   c.a.q = desc(q, hf); c.a.kn = desc(k, hf); c.a.vn = desc(v, hf);

@@ -35,7 +35,7 @@ def cap_of(softcap, name: str) -> float:
     cap = 0.0 if softcap is None else float(softcap)
     if not 0.0 <= cap < 3e38:
         raise ValueError(f"{name}: softcap must be positive, or 0 / None for none, got {softcap}")
-    return cap
+    return max(cap, 2.0 ** -126) if cap else 0.0         # (the kernels hold it in 32 bits, where 0 is none)
 
 
 def ints_of(x: torch.Tensor, n: int, device, name: str) -> torch.Tensor:

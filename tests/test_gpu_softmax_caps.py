@@ -1,4 +1,4 @@
-"""Large caps of the scores on the GPU: the error of a score must not grow with a cap that the scores are
+"""Caps of the scores from the least to the largest on the GPU: the error of a score must not grow with a cap that the scores are
 far below.  Against float64, within the bounds of oracle/softmax.py."""
 import pytest
 import torch
@@ -43,7 +43,18 @@ def test_large_caps_in_long_sequences(cuda, D):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("cap", CAPS)
+@pytest.mark.parametrize("cap", [1e-12, 1e-30, 1e-41, 1e-60])
+def test_least_caps(cuda, dtype, cap):
+    """All scores are nothing: every row is the mean of what it sees.  (In 32 bits the last two are denormal and 0, which would be none.)"""
+    x = inputs(137, 1, 130, 2, 1, 64, 64, dtype)
+    run_and_check(cuda, *x, softcap=cap)
+    run_and_check(cuda, *x, softcap=cap, slopes=alibi(2))
+    zero = torch.zeros_like(x[0])
+    run_and_check(cuda, zero, *x[1:], softcap=cap, scale=0.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("cap", CAPS + [1e-30, 1e-60])
 @pytest.mark.parametrize("bias", [False, True])
 def test_decoding(cuda, dtype, cap, bias):
     c = Cache(5, [1, 90, 1000], 32, 2, 64, 64, dtype)
