@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from ._host import _DT, _desc, native_call, ptr, stream_ptr
-from .softmax_attn import MAX_DIM, cap_of, has_rows16, ints_of, on_current_device, rows16, slopes_of
+from .softmax_attn import MAX_DIM, cap_of, has_rows16, ints_of, on_current_device, rows16, slopes_of, to_int32
 
 
 def _pages(k_pages, v_pages, page_table, lens, name):
@@ -49,7 +49,7 @@ def _pages(k_pages, v_pages, page_table, lens, name):
         raise ValueError(f"{name}: page_table must be [N, M] whole numbers on {dev}, got {tuple(page_table.shape)} of {page_table.dtype} on "
                          f"{page_table.device}")
     if page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        page_table = page_table.to(torch.int32).contiguous()
+        page_table = to_int32(page_table).contiguous()
     N, M = page_table.shape
     lens = ints_of(lens, N, dev, f"{name}: lens")
     a = _lib.PagedArgs()

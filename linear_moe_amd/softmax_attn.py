@@ -38,13 +38,19 @@ def cap_of(softcap, name: str) -> float:
     return max(cap, 2.0 ** -126) if cap else 0.0         # (the kernels hold it in 32 bits, where 0 is none)
 
 
+def to_int32(x: torch.Tensor) -> torch.Tensor:
+    """Whole numbers in 32 bits; what those do not hold becomes the nearest they do (out of any range all the same)."""
+    wide = x.dtype in (torch.int64, torch.uint32, torch.uint64)
+    return (x.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1) if wide else x).to(torch.int32)
+
+
 def ints_of(x: torch.Tensor, n: int, device, name: str) -> torch.Tensor:
     """One whole number per sequence, as the kernels read them."""
     if x.dim() != 1 or x.numel() != n or x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
         raise ValueError(f"{name} must be {n} whole numbers, got {tuple(x.shape)} of {x.dtype}")
     if x.device != device:
         raise ValueError(f"{name} must live on {device}, got {x.device}")
-    return x.detach().to(torch.int32).contiguous()
+    return to_int32(x.detach()).contiguous()
 
 
 def on_current_device(device, name: str) -> None:
