@@ -420,5 +420,10 @@ def no_transform() -> bool:
             and torch._C._get_tracing_state() is None)
 
 
+def has_tangent(x: torch.Tensor) -> bool:
+    """Whether forward-mode differentiation carries a derivative along with x."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
 def ptr(x: Optional[torch.Tensor]):
     return None if x is None else x.data_ptr()

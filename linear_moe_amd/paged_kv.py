@@ -22,7 +22,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._host import _DT, _desc, native_call, ptr, stream_ptr
+from ._host import _DT, _desc, has_tangent, native_call, ptr, stream_ptr
 from .softmax_attn import MAX_DIM, cap_of, has_rows16, ints_of, on_current_device, rows16, slopes_of, to_int32
 
 
@@ -72,6 +72,10 @@ def _tokens(x, B, T, H, D, head_first, like, name):
 def _no_grad(name, *xs):
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in xs):
         raise RuntimeError(f"{name} is for generation and has no backward: call it under torch.no_grad(), or train with softmax_attn")
+    if any(x is not None and has_tangent(x) for x in xs):
+        raise RuntimeError(f"{name} is for generation and has no forward-mode derivative")
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{name} cannot be recorded in a trace, which would hold its allocations alone")
 
 
 def _written(*pages):

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._host import _DT, _desc, native_call, no_node, no_transform, ptr, seq_plan, stream_ptr
+from ._host import _DT, _desc, has_tangent, native_call, no_node, no_transform, ptr, seq_plan, stream_ptr
 
 MAX_DIM = 128      # columns of a head
 
@@ -26,6 +26,8 @@ def slopes_of(slopes, H: int, device, name: str):
         return None
     if slopes.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: slopes are constants of the model, there is no gradient for them")
+    if has_tangent(slopes):
+        raise RuntimeError(f"{name}: slopes are constants of the model, there is no forward-mode derivative for them")
     if slopes.numel() != H or slopes.device != device:
         raise ValueError(f"{name}: slopes must be {H} numbers on {device}, got {tuple(slopes.shape)} on {slopes.device}")
     return slopes.detach().reshape(H).to(torch.float32).contiguous()
