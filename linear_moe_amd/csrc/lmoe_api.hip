@@ -762,7 +762,7 @@ int lmoe_paged_kv_append(const lmoe_paged_args* a, void* stream) {
   if (a->B < 0 || a->T < 0) return fail(-4, "%s: negative dimension", op);
   if (!a->kn.ptr) return fail(-7, "%s: kn and vn must not be null", op);
   if (a->cu_seqlens ? a->B != 1 : a->N != a->B) return fail(-6, "%s: N == B for dense input, B == 1 for packed", op);
-  if ((int64_t)a->B * a->T >= 4 * MAX_GROUPS) return fail(-8, "%s: more than 2^26 - 1 tokens", op);
+  if ((int64_t)a->B * a->T > 4 * (MAX_GROUPS - 1)) return fail(-8, "%s: more than 2^26 - 4 tokens", op);       // (four to a work-group)
   if (a->B == 0 || a->T == 0 || a->N == 0) return 0;
   lmoe::launch_paged_append(*a, (hipStream_t)stream);
   return launched(op);

@@ -13,8 +13,12 @@ static bool fits16(const lmoe_attn_args& a) {
     if (x->st < 0 || x->st >= 1 << 24) return false;
   return a.dtype == LMOE_BF16;
 }
-// (without them: four strips to 64 rows, 512 threads each)
-int64_t attn_groups(const lmoe_attn_args& a) { return attn_tiles<CH>(a) * a.HQ * (fits16(a) ? 1 : 8); }
+// (without them: four strips to 64 rows, 512 threads each; with them 256, but 512 for tiles of 256 keys.  Of more than WALK_SEQS documents
+// a tile of any size has as many work-groups as one of 64 rows.)
+int64_t attn_groups(const lmoe_attn_args& a) {
+  if (!fits16(a)) return attn_tiles<CH>(a) * a.HQ * 8;
+  return std::max(attn_tiles<CH>(a) * a.HQ, a.dk.ptr ? 2 * attn_tiles<256>(a) * a.HKV : 0);
+}
 
 // Work-groups that share the rows of a strip of keys (k_attn_bwd_dkv_any): two where there are too few strips for the unequal work of a
 // causal call to come out even, or for half of the card.  Backward with 1 / 2 / 3 / 4 work-groups, us: 2 x 1000 tokens, 4 heads on 2 of

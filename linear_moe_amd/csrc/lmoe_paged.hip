@@ -36,7 +36,8 @@ static PagedPlan paged_plan(const lmoe_paged_args& a) {
   // Else stretches of one length, whatever the call: us for stretches of 256, 384, 512, 1024 positions (64 sequences of 1024 to 4096
   // tokens, 32 / 8 heads of 128; 2 of 32 K and 128 K, 16 / 4 heads of 128; 9 of 750 to 3001 tokens, 12 / 3 heads of 64,
   // 4-byte elements): 140 135 134 136; 80 76 74 78; 20.3 17.4 19.9 31.1.
-  p.waves = a.dtype == LMOE_BF16 && bound <= 1024 ? 8 : 4;
+  // (a launch has less than 2^32 threads: of 2^23 work-groups and more, which N * HQ < 2^24 allows, none has 512)
+  p.waves = a.dtype == LMOE_BF16 && bound <= 1024 && groups < 1 << 23 ? 8 : 4;
   const int64_t chunk = p.waves == 8 ? 1024 : a.dtype == LMOE_BF16 ? 512 : 384;
   int64_t splits = (bound + chunk - 1) / chunk;
   const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;
