@@ -68,11 +68,15 @@ template <typename T, int W, int CAP, bool BIAS> struct AttnAny {
 constexpr int attn_kv_waves(int W) { return W == 128 ? 8 : 4; }
 // Work-groups that share the rows of a tile of keys (k_attn_bwd_dkv), at most, and the pieces of its stream that each has at least.
 // So many that the card is full; where it is, the tiles of a causal call are unequal work all the same, those of documents more so:
-// two (64 columns: four) for long streams, four for documents of 96 pieces or more.  Each part costs its sums' way through memory.
+// two (64 columns: four) for long streams, four for documents of 96 pieces or more where the tiles fill the card twice at most (beyond
+// that the longest documents, which come first, leave enough behind them).  Each part costs its sums' way through memory, and room for
+// them whether a document is long enough or not: 1 GiB at the very most with these limits.
 // Backward in us, 128 columns, 16 heads on 4, with 1 / 2 / 4 / 8 parts: 1 x 1024 tokens 243 / 155 / 106 / 86 (16 parts: 83), 1 x 4096
 // 929 / 549 / 365 / 384, 8 x 1024 275 / 203 / 214 / 265, 2 x 8192 2411 / 1844 / 1911 / 2017; 16 on 16, 8 x 1024 162 / 278 / 420 / 686.
 // 64 columns, 16 on 4, 2 x 8192 1316 / 1136 / 1034 / 1072.  16384 tokens in documents of which the longest has 5990, one part / two
-// of 4 pieces or more / four of 48: 16 on 4 1677 / 1281 / 1270, 16 on 16 1142 / 1313 / 1159; in 16 equal ones 388 / 448 / 394.
+// of 4 pieces or more / four of 48: 16 on 4 1677 / 1281 / 1270, 16 on 16 1142 / 1313 / 1159; in 16 equal ones 388 / 448 / 394.  7, 23
+// and 60 unequal ones, one part / four of 48: 16 on 8 (tiles twice the CUs) 1223 / 1265, 815 / 764, 389 / 423; 12 on 12 (three
+// times) 913 / 1045, 510 / 543, 267 / 325; 32768 tokens, 16 on 8 (four times) 4549 / 4793, 2264 / 2485, 951 / 1101.
 struct Parts { int most, least; };
 static Parts attn_parts(const lmoe_attn_args& a) {
   if (!fits16(a)) return {any_parts(a), 0};
@@ -81,7 +85,7 @@ static Parts attn_parts(const lmoe_attn_args& a) {
   const int64_t full = (W == 128 ? 1 : 2) * (int64_t)cu_count(), pieces = ((int64_t)a.T + CH - 1) / CH * (a.HQ / a.HKV);
   int64_t parts = (full + groups - 1) / groups;
   const int least = parts == 1 && a.cu_seqlens ? 48 : 4;
-  if (a.cu_seqlens) parts = parts > 1 ? parts : 4;
+  if (a.cu_seqlens) parts = parts > 1 ? parts : groups <= 2 * full ? 4 : 1;
   else for (int i = W == 128 ? 1 : 2; i > 0 && groups * parts < (W == 128 ? 2 : 4) * full && pieces / parts >= 128; --i) parts *= 2;
   return {(int)std::max<int64_t>(1, std::min(std::min<int64_t>(parts, 16), pieces / least)), least};
 }
