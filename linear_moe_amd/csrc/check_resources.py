@@ -6,7 +6,7 @@ steering: refreshed lane indices, pinned sums, fenced products).  A compiler or 
 spill, or lowers the number of waves it runs with, costs a large factor in speed without failing any test.  This
 script reads the per-kernel resource reports that ``-Rpass-analysis=kernel-resource-usage`` wrote at compile time
 (``<unit>.remarks``) and fails the build when an instance of a guarded kernel uses scratch memory or spills vector
-registers, or when one for 2-byte elements (the performance path; ANY_TYPE: for any) falls below its minimum occupancy.
+registers (but for TOLERATED), or when one for 2-byte elements (the performance path; ANY_TYPE: for any) falls below its minimum occupancy.
 
 usage: check_resources.py unit.remarks [...]
 """
@@ -31,9 +31,16 @@ GUARDED = {
     "k_gla_bwd_dqkg": 2,      # K = 64: two work-groups of 8 waves per CU, see FLOORS
     "k_attn_fwd": 2,          # two work-groups of 4 waves per CU, or one of 8: a spill in the loop waits for the tiles in flight
     "k_attn_bwd_dq": 2,
+    "k_attn_bwd_dkv": 2,      # one work-group of 8 waves per CU; 64 columns: three of 4, see FLOORS
     "k_bwd_dqkv": 2,          # one work-group of 8 waves per CU; its first version spilled loop-invariant lane arithmetic
 }
 ANY_TYPE = ("k_state_bwd", "k_state_fwd_chunks")
+# What instances of a kernel may spill all the same: bytes of scratch and vector registers.
+TOLERATED = {
+    # one register that is stored before the loop and read behind it, and the address at which rows behind a sequence are cleared in LDS,
+    # read where a tile has such rows; the steps of a whole tile touch neither
+    "k_attn_bwd_dkv": (12, 2),
+}
 # other minima of single instances
 FLOORS = (
     # the instances whose kept places (last argument) cost the second work-group: launched where there is one per CU at most
@@ -42,6 +49,7 @@ FLOORS = (
     (re.compile(r"k_state_bwdIfLi64ELi\d+ELi16ELi0ELb[01]ELb0EE"), 6),
     (re.compile(r"k_state_fwd_chunksILi64E"), 6),
     (re.compile(r"k_gla_bwd_dqkgIDF16b(DF16b|f)Li64E"), 4),
+    (re.compile(r"k_attn_bwd_dkvILi64E"), 3),
 )
 FIELDS = {"ScratchSize [bytes/lane]": "scratch", "VGPRs Spill": "vspill", "Occupancy [waves/SIMD]": "occ",
           "VGPRs": "vgpr", "AGPRs": "agpr", "LDS Size [bytes/block]": "lds"}
@@ -81,7 +89,8 @@ def main(paths):
                         f"lds {r.get('lds', -1)}  {name}")
                 seen[kern] += 1
                 min_occ = next((floor for pat, floor in FLOORS if pat.search(name)), min_occ)
-                if r.get("scratch", 1) != 0 or r.get("vspill", 1) != 0 or ((two_byte or kern in ANY_TYPE) and r.get("occ", 0) < min_occ):
+                scratch, vspill = TOLERATED.get(kern, (0, 0))
+                if r.get("scratch", 1 << 30) > scratch or r.get("vspill", 1 << 30) > vspill or ((two_byte or kern in ANY_TYPE) and r.get("occ", 0) < min_occ):
                     bad.append(line)
     missing = [k for k, n in seen.items() if n == 0]
     if missing:
@@ -89,12 +98,12 @@ def main(paths):
         return 1
     if bad:
         print("check_resources: instances of guarded kernels spill or lost occupancy "
-              "(needed: scratch 0, vgpr-spill 0; waves/SIMD >= " + str(GUARDED) + "):", file=sys.stderr)
+              "(needed: scratch 0, vgpr-spill 0, or at most " + str(TOLERATED) + "; waves/SIMD >= " + str(GUARDED) + "):", file=sys.stderr)
         for b in bad:
             print("  " + b, file=sys.stderr)
         return 1
-    print(f"check_resources: {sum(seen.values())} instances of {len(GUARDED)} guarded kernels: no scratch, no spills, "
-          "occupancy as tuned")
+    print(f"check_resources: {sum(seen.values())} instances of {len(GUARDED)} guarded kernels: no scratch, no spills "
+          f"(at most {TOLERATED} bytes and registers), occupancy as tuned")
     return 0
 
 
