@@ -419,7 +419,8 @@ int lmoe_fused_recurrent_fwd(const lmoe_args* a, int32_t op, void* stream);
 
 /* Softmax attention, the layers between the linear ones of a hybrid model (the reference's core:
  * linear_moe/sequence_modeling/attention/dot_product_attention.py:139-183).
- *   x = scale q_i . k_j;  x = softcap tanh(x / softcap) where softcap > 0;  s_ij = x - slopes[h] |i - j| where slopes is given
+ *   x = scale q_i . k_j;  x = softcap tanh(x / softcap) where softcap > 0 (above 2^100: as 2^100);  s_ij = x - slopes[h] |i - j| where
+ *   slopes is given.  Scores are held in 32 bits: |s| below 2^28
  *   o_i = sum_j softmax_j(s_ij) v_j  over the j of the same sequence with (causal = 0, or j <= i, or j < prefix_lens[n])
  * Query head h reads key and value head h / (HQ / HKV).  i, j count inside the sequence.  Packed input (cu_seqlens, chunk_map,
  * nt_dev, N, NT) as for the chunk ops, B = 1; rows behind the last sequence are zero in o, dq, dk, dv.
@@ -441,7 +442,7 @@ typedef struct lmoe_attn_args {
   /* backward: o, lse (and o_low) of the forward call, d_o in; dq, dk, dv out (dk.ptr and dv.ptr NULL: dq alone)      */
   lmoe_tensor d_o, dq, dk, dv;
   float* delta;        /* [B,HQ,T] workspace: sum of d_o o per row                     */
-  float* ws;           /* workspace of lmoe_softmax_attn_bwd_floats fp32 numbers (0: may be NULL), 16-byte aligned */
+  float* ws;           /* workspace of lmoe_softmax_attn_bwd_floats fp32 numbers (0: may be NULL; at most 2^28), 16-byte aligned */
 } lmoe_attn_args;
 int64_t lmoe_softmax_attn_bwd_floats(const lmoe_attn_args* a);
 int lmoe_softmax_attn_fwd(const lmoe_attn_args* a, void* stream);

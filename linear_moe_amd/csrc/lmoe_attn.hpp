@@ -12,7 +12,7 @@
 // linear_moe/sequence_modeling/attention/dot_product_attention.py:139-183).
 //
 // All exponents are to the base 2: log2(e) is a factor of the scale, the cap and the slope.  Statistics, the sums and the
-// accumulators are fp32.  Every row of a sequence is allowed to see itself (causal) or everything, so no row is empty;
+// accumulators are fp32 (scores of 2^28 and more in size are past that: the rounding of one is a factor of 2^16 in its p).  Every row of a sequence is allowed to see itself (causal) or everything, so no row is empty;
 // rows that a mask leaves nothing of inside one tile are handled by a finite lowest maximum (M_LOW): 2^(-inf - M_LOW) = 0.
 #pragma once
 #include <algorithm>
@@ -27,7 +27,8 @@ constexpr float M_LOW = -1e30f;
 
 // 1 - 2 / (1 + e^{2z}) is off by an ulp of 1 whatever tanh(z) itself is, and a score by an ulp of the cap: 1.2e-4 at a cap of 1024, a
 // thirtieth of the rounding of p to a bfloat16.  The kernels on 2-byte elements take that form for caps up to it, and beyond it one whose
-// error is relative (the near form would be off by 1.2e-3 in the score at a cap of 1e4, by 0.09 at 1e6).
+// error is relative (the near form would be off by 1.2e-3 in the score at a cap of 1e4, by 0.09 at 1e6).  It costs six operations more: 2 x
+// 8192 tokens, 16 heads on 4 of 128, forward and backward 0.88 and 2.57 ms, with a near cap 0.69 to 0.77 and 2.18.
 constexpr float CAP_NEAR = 1024.0f;
 enum { NO_CAP, NEAR_CAP, FAR_CAP };
 // Below 1/4 by the series, whose next term is 2^-27 of the sum; from there on the form above is off by 16 ulps of the number at most.

@@ -200,9 +200,11 @@ def softmax_attn(
     strides; HQ a multiple of HKV: query head h reads key head ``h // (HQ // HKV)``.  K, V up to 128 (others than multiples of
     16 bytes are padded).  Returns o, laid out like q with V columns.
 
-    scale: ``None`` is ``K ** -0.5``.  softcap, slopes (``[HQ]``, not trained): as in the formula, left out where ``None`` (or 0).
+    scale: ``None`` is ``K ** -0.5``.  softcap, slopes (``[HQ]``, not trained): as in the formula, left out where ``None`` (or 0).  A cap may be
+    any number below 3e38 (less than 2^-126 counts as that, more than 2^100 as that).  Scores are held in float32: up to 2^28 in size.
     causal: row i sees j <= i; prefix_lens (``[N]`` whole numbers on the device, clamped to the sequence's length): and every
     j < its sequence's prefix.  ``causal=False``: all.
+    The backward takes a workspace of fp32 sums where several work-groups share a tile of keys: 1 GiB at most, none where the tiles fill the card a few times.
     cu_seqlens: packed documents as in the chunk ops; rows of one never see another's (nor what it holds: a NaN stays in its
     document).  Rows behind the last document are zero in o and in the gradients.
     Without atomics: the gradients of a key head are summed over its query heads in a fixed order.  A NaN or infinity in the k or v of a
