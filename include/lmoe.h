@@ -457,13 +457,15 @@ int lmoe_softmax_attn_bwd(const lmoe_attn_args* a, void* stream);
  *   Nothing to attend to: o = 0.  ws: lmoe_paged_attn_floats fp32 numbers (0: may be NULL), 16-byte aligned.
  * lmoe_paged_kv_append: kn, vn [B, T, HKV, K | V]: token t of row n goes to position lens[n] + t (cu_seqlens NULL, N = B), or
  *   packed, B = 1: token cu_seqlens[n] + t of sequence n; tokens behind the last sequence are left out.
+ * lmoe_paged_kv_read: the way back, into kn, vn (dtype: theirs): token t of row n from position lens[n] + t.  Zero where there is
+ *   no page, and behind the last sequence.
  * Two tokens of one call that share a position leave one of them there.  No counterpart in the reference, whose generation
  * keeps dense caches (linear_moe/generation). */
 typedef struct lmoe_paged_args {
   int32_t dtype;       /* of q, kp, vp, kn, vn, o                                      */
   int32_t N, HQ, HKV, K, V;
   int32_t P, S, M;     /* pages, tokens per page, columns of the table                 */
-  int32_t B, T;        /* append only                                                  */
+  int32_t B, T;        /* append and read only                                         */
   float scale, softcap;
   int64_t table_stride;
   const int32_t *table, *lens, *cu_seqlens;
@@ -474,6 +476,83 @@ typedef struct lmoe_paged_args {
 int64_t lmoe_paged_attn_floats(const lmoe_paged_args* a);
 int lmoe_paged_attn_decode(const lmoe_paged_args* a, void* stream);
 int lmoe_paged_kv_append(const lmoe_paged_args* a, void* stream);
+int lmoe_paged_kv_read(const lmoe_paged_args* a, void* stream);
+
+/* The same with a cache in 4 bits (K, V multiples of 32; p.dtype: of q, kn, vn, o): p.kp, p.vp [P, S, HKV, K/2 | V/2] bytes, column 2i in the
+ * low half of byte i, 16-byte aligned rows; ks, vs [P, S, HKV, K/32 | V/32] bytes; the strides of these in bytes.  A half byte is a
+ * sign (8) and one of 0 0.5 1 1.5 2 3 4 6; the 32 columns of a scale byte x stand for that times 2^(x - 127), for x = 255 for NaN.  What is
+ * written: the least x in 7 .. 252 for which nothing is above 6 (above 6 at 252: 6), the nearest number, of two as near the one whose half
+ * byte is even; 255 where one of the 32 is infinite or NaN.  The new token is attended to as the cache holds it. */
+typedef struct lmoe_paged4_args {
+  lmoe_paged_args p;
+  lmoe_tensor ks, vs;
+} lmoe_paged4_args;
+int64_t lmoe_paged4_attn_floats(const lmoe_paged4_args* a);
+int lmoe_paged4_attn_decode(const lmoe_paged4_args* a, void* stream);
+int lmoe_paged4_kv_append(const lmoe_paged4_args* a, void* stream);
+int lmoe_paged4_kv_read(const lmoe_paged4_args* a, void* stream);
+
+/* Norm and rotation of queries and keys, in one pass:
+ *   y = x / sqrt(mean x^2 + eps) w per row of D (norm; w: qw or kw, NULL: none),
+ *   z_a = y_a cos[p][i] - y_b sin[p][i],  z_b = y_b cos[p][i] + y_a sin[p][i]   for the pairs (a, b) = (i, i + R / 2), interleaved (2i, 2i + 1),
+ * i < R / 2 (R = 0: no rotation); columns from R on as they are.  The position p of token t of row b: positions[b * pos_stride + t] where
+ * given, else t + offsets[b] (offsets NULL: 0); packed input (cu_seqlens [N + 1], B = 1): that inside its sequence.  p outside 0 .. L - 1:
+ * not rotated.  Rows behind the last sequence are zero in every result.  D <= 256, D and R even; any strides with adjacent columns.
+ * bwd: q, k and the gradients dzq, dzk in; dq, dk and (where their pointers are given) dqw, dkw out; ws: lmoe_qk_norm_rope_floats fp32 numbers
+ * (0: may be NULL).  The reference's rotary: linear_moe/model/common_modules/rotary.py:40-98. */
+typedef struct lmoe_rope_args {
+  int32_t dtype;       /* of q, k, their results and gradients                         */
+  int32_t w_dtype;     /* of qw, kw, dqw, dkw                                          */
+  int32_t B, T, HQ, HKV, D, R, N, L;
+  int32_t norm, interleaved;
+  float eps;
+  int64_t pos_stride;
+  const int32_t *cu_seqlens, *offsets, *positions;
+  const float *cos, *sin;      /* [L, R / 2]                                           */
+  const void *qw, *kw;         /* [D]                                                  */
+  lmoe_tensor q, k, zq, zk;
+  lmoe_tensor dzq, dzk, dq, dk;
+  void *dqw, *dkw;
+  float* ws;
+} lmoe_rope_args;
+int64_t lmoe_qk_norm_rope_floats(const lmoe_rope_args* a);
+int lmoe_qk_norm_rope_fwd(const lmoe_rope_args* a, void* stream);
+int lmoe_qk_norm_rope_bwd(const lmoe_rope_args* a, void* stream);
+
+/* The pages of a cache, kept by a table [N, M] (row stride table_stride) of page numbers, lens [N] and refs [P]: how many entries (and
+ * holds of the program itself) name a page, 0 for a free one.  A number outside 0 .. P - 1 names no page.  Every result is the same
+ * whatever order the card takes; nothing is read by the host.
+ * lmoe_paged_free: the rows rows[F] give their pages back (refs - 1, entry -1) and get lens 0; a number outside 0 .. N - 1 is left out.
+ * lmoe_paged_fork: for all i at once row rows[i] becomes what row src[i] was (entries and lens), refs follow; of several for one
+ *   row the last counts.  ws: lmoe_paged_fork_ints int32.
+ * lmoe_paged_reserve: in the order of the rows, positions lens[n] .. lens[n] + tokens[n] - 1 (tokens NULL: each) become writable: an entry that names no
+ *   page, or one with refs above 1, gets the next free page (the lowest number first), the latter with the old one's contents, whose refs
+ *   goes down.  fits[n]: 1, or 0 where the table ends before, or no free page is left for the row: then nothing of it changes, nor
+ *   of a later row that needs pages.
+ * lmoe_paged_compact: the used pages (refs above 0) move to 0 .. live[0] - 1: the k-th free number below takes the k-th used page
+ *   above; moved[P]: where each page went (itself, where it stayed); the table and refs follow.
+ * reserve, compact: the pages' contents are `bufs`, n_bufs tensors of P pages at ptr + page * page_stride, each of rows0 * rows1 runs of
+ * `bytes` bytes at i * stride0 + j * stride1 (all in bytes).  ws: lmoe_paged_pages_ints int32. */
+typedef struct lmoe_page_buf {
+  void* ptr;
+  int64_t page_stride, stride0, stride1, bytes;
+  int32_t rows0, rows1;
+} lmoe_page_buf;
+typedef struct lmoe_pages_args {
+  int32_t N, M, P, S, F, each, n_bufs;
+  int64_t table_stride;
+  int32_t *table, *lens, *refs;
+  const int32_t *rows, *src, *tokens;
+  uint8_t* fits;
+  int32_t *live, *moved, *ws;
+  const lmoe_page_buf* bufs;   /* on the host, read by the call                        */
+} lmoe_pages_args;
+int64_t lmoe_paged_fork_ints(const lmoe_pages_args* a);
+int64_t lmoe_paged_pages_ints(const lmoe_pages_args* a);
+int lmoe_paged_free(const lmoe_pages_args* a, void* stream);
+int lmoe_paged_fork(const lmoe_pages_args* a, void* stream);
+int lmoe_paged_reserve(const lmoe_pages_args* a, void* stream);
+int lmoe_paged_compact(const lmoe_pages_args* a, void* stream);
 
 /* Toolkit self-test over one pair of 64 x kd tiles A, B (element type by dtype, kd in {64,128}),
  * through the same tile loaders, MFMA fragments and accumulator stores the kernels use:

@@ -65,6 +65,33 @@ class PagedArgs(C.Structure):
                 + [(n, Tensor4) for n in ("q", "o", "kp", "vp", "kn", "vn")] + [("ws", C.c_void_p)])
 
 
+class Paged4Args(C.Structure):
+    """``lmoe_paged4_args`` -- field order must match include/lmoe.h."""
+    _fields_ = [("p", PagedArgs), ("ks", Tensor4), ("vs", Tensor4)]
+
+
+class RopeArgs(C.Structure):
+    """``lmoe_rope_args`` -- field order must match include/lmoe.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "w_dtype", "B", "T", "HQ", "HKV", "D", "R", "N", "L", "norm", "interleaved")]
+                + [("eps", C.c_float), ("pos_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("cu_seqlens", "offsets", "positions", "cos", "sin", "qw", "kw")]
+                + [(n, Tensor4) for n in ("q", "k", "zq", "zk", "dzq", "dzk", "dq", "dk")]
+                + [(n, C.c_void_p) for n in ("dqw", "dkw", "ws")])
+
+
+class PageBuf(C.Structure):
+    """``lmoe_page_buf`` -- field order must match include/lmoe.h."""
+    _fields_ = ([("ptr", C.c_void_p)] + [(n, C.c_int64) for n in ("page_stride", "stride0", "stride1", "bytes")]
+                + [("rows0", C.c_int32), ("rows1", C.c_int32)])
+
+
+class PagesArgs(C.Structure):
+    """``lmoe_pages_args`` -- field order must match include/lmoe.h."""
+    _fields_ = ([(n, C.c_int32) for n in ("N", "M", "P", "S", "F", "each", "n_bufs")] + [("table_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("table", "lens", "refs", "rows", "src", "tokens", "fits", "live", "moved", "ws")]
+                + [("bufs", C.POINTER(PageBuf))])
+
+
 ENTRY_POINTS = (
     "lmoe_version", "lmoe_last_error",
     "lmoe_chunk_simple_gla_fwd", "lmoe_chunk_simple_gla_bwd",
@@ -79,6 +106,9 @@ ENTRY_POINTS = (
     "lmoe_fused_recurrent_fwd", "lmoe_trace_gdn_state_fwd", "lmoe_trace_simple_gla_fwd", "lmoe_mom_gather", "lmoe_mom_combine", "lmoe_mom_rowdot",
     "lmoe_mom_combine_bwd", "lmoe_mom_plan_ints", "lmoe_mom_plan", "lmoe_seq_tables",
     "lmoe_softmax_attn_fwd", "lmoe_softmax_attn_bwd", "lmoe_softmax_attn_bwd_floats", "lmoe_paged_attn_floats", "lmoe_paged_attn_decode", "lmoe_paged_kv_append",
+    "lmoe_paged_kv_read", "lmoe_paged4_attn_floats", "lmoe_paged4_attn_decode", "lmoe_paged4_kv_append", "lmoe_paged4_kv_read",
+    "lmoe_qk_norm_rope_floats", "lmoe_qk_norm_rope_fwd", "lmoe_qk_norm_rope_bwd",
+    "lmoe_paged_fork_ints", "lmoe_paged_pages_ints", "lmoe_paged_free", "lmoe_paged_fork", "lmoe_paged_reserve", "lmoe_paged_compact",
 )
 
 _lib = None
@@ -179,9 +209,15 @@ def load() -> C.CDLL:
     for fn in (lib.lmoe_softmax_attn_fwd, lib.lmoe_softmax_attn_bwd):
         fn.argtypes, fn.restype = [C.POINTER(AttnArgs), C.c_void_p], C.c_int
     lib.lmoe_softmax_attn_bwd_floats.argtypes, lib.lmoe_softmax_attn_bwd_floats.restype = [C.POINTER(AttnArgs)], C.c_int64
-    for fn in (lib.lmoe_paged_attn_decode, lib.lmoe_paged_kv_append):
-        fn.argtypes, fn.restype = [C.POINTER(PagedArgs), C.c_void_p], C.c_int
-    lib.lmoe_paged_attn_floats.argtypes, lib.lmoe_paged_attn_floats.restype = [C.POINTER(PagedArgs)], C.c_int64
+    for block, size, names in ((PagedArgs, "lmoe_paged_attn_floats", "lmoe_paged_attn_decode lmoe_paged_kv_append lmoe_paged_kv_read"),
+                               (Paged4Args, "lmoe_paged4_attn_floats", "lmoe_paged4_attn_decode lmoe_paged4_kv_append lmoe_paged4_kv_read"),
+                               (RopeArgs, "lmoe_qk_norm_rope_floats", "lmoe_qk_norm_rope_fwd lmoe_qk_norm_rope_bwd"),
+                               (PagesArgs, "lmoe_paged_fork_ints", "lmoe_paged_free lmoe_paged_fork"),
+                               (PagesArgs, "lmoe_paged_pages_ints", "lmoe_paged_reserve lmoe_paged_compact")):
+        getattr(lib, size).argtypes, getattr(lib, size).restype = [C.POINTER(block)], C.c_int64
+        for name in names.split():
+            fn = getattr(lib, name)
+            fn.argtypes, fn.restype = [C.POINTER(block), C.c_void_p], C.c_int
     lib.lmoe_split_floats.argtypes = [C.POINTER(Args), C.c_int32, C.c_int32]
     lib.lmoe_split_floats.restype = C.c_int64
     lib.lmoe_split_lengths.argtypes = [C.POINTER(Args), C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]

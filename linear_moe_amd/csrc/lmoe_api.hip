@@ -718,7 +718,8 @@ int lmoe_softmax_attn_bwd(const lmoe_attn_args* a, void* stream) {
   return launched(op);
 }
 
-static int check_paged(const lmoe_paged_args* a, const char* op) {
+// pages4: the pages are a cache in 4 bits, checked by the caller
+static int check_paged(const lmoe_paged_args* a, const char* op, bool pages4 = false) {
   if (!a) return fail(-1, "%s: null argument block", op);
   if (a->dtype != LMOE_BF16 && a->dtype != LMOE_F32) return fail(-2, "%s: dtype must be LMOE_BF16 or LMOE_F32", op);
   const int64_t vec = a->dtype == LMOE_BF16 ? 8 : 4;
@@ -727,16 +728,16 @@ static int check_paged(const lmoe_paged_args* a, const char* op) {
   if (a->N < 0 || a->HKV <= 0 || a->P < 0 || a->M < 0 || a->S <= 0) return fail(-4, "%s: negative dimension", op);
   if (a->HKV > 65535 || a->N > 65535) return fail(-8, "%s: heads and N must be <= 65535", op);
   if ((int64_t)a->M * a->S > 1 << 30) return fail(-8, "%s: %d pages of %d tokens per sequence: positions must stay below 2^30", op, a->M, a->S);
-  if (!a->kp.ptr || !a->vp.ptr || (!a->table && a->M > 0) || !a->lens) return fail(-7, "%s: pages, table and lens must not be null", op);
+  if (((!a->kp.ptr || !a->vp.ptr) && !(pages4 && a->P == 0)) || (!a->table && a->M > 0) || !a->lens) return fail(-7, "%s: pages, table and lens must not be null", op);
   if ((a->kn.ptr != nullptr) != (a->vn.ptr != nullptr)) return fail(-11, "%s: kn and vn go together", op);
   const lmoe_tensor* rows[] = {&a->q, &a->o, &a->kp, &a->vp, &a->kn, &a->vn};
   for (const lmoe_tensor* t : rows)
-    if (t->ptr && (((uintptr_t)t->ptr & 15) || t->sb % vec || t->st % vec || t->sh % vec))
+    if (t->ptr && !(pages4 && (t == &a->kp || t == &a->vp)) && (((uintptr_t)t->ptr & 15) || t->sb % vec || t->st % vec || t->sh % vec))
       return fail(-9, "%s: q, o, the pages and the new tokens need 16-byte aligned rows (pointer and strides)", op);
   return 0;
 }
-static int check_decode(const lmoe_paged_args* a, const char* op) {
-  if (int r = check_paged(a, op)) return r;
+static int check_decode(const lmoe_paged_args* a, const char* op, bool pages4 = false) {
+  if (int r = check_paged(a, op, pages4)) return r;
   if (a->HQ <= 0 || a->HQ % a->HKV) return fail(-3, "%s: HQ=%d is no multiple of HKV=%d", op, a->HQ, a->HKV);
   if (a->HQ > 65535) return fail(-8, "%s: heads and N must be <= 65535", op);
   if ((int64_t)a->N * a->HQ >= MAX_GROUPS) return fail(-8, "%s: more than 2^24 - 1 rows of q", op);
@@ -756,15 +757,167 @@ int lmoe_paged_attn_decode(const lmoe_paged_args* a, void* stream) {
   lmoe::launch_paged_decode(*a, (hipStream_t)stream);
   return launched(op);
 }
-int lmoe_paged_kv_append(const lmoe_paged_args* a, void* stream) {
-  const char* op = "lmoe_paged_kv_append";
-  if (int r = check_paged(a, op)) return r;
+static int check_tokens(const lmoe_paged_args* a, const char* op) {
   if (a->B < 0 || a->T < 0) return fail(-4, "%s: negative dimension", op);
   if (!a->kn.ptr) return fail(-7, "%s: kn and vn must not be null", op);
   if (a->cu_seqlens ? a->B != 1 : a->N != a->B) return fail(-6, "%s: N == B for dense input, B == 1 for packed", op);
   if ((int64_t)a->B * a->T > 4 * (MAX_GROUPS - 1)) return fail(-8, "%s: more than 2^26 - 4 tokens", op);       // (four to a work-group)
+  return 0;
+}
+int lmoe_paged_kv_append(const lmoe_paged_args* a, void* stream) {
+  const char* op = "lmoe_paged_kv_append";
+  if (int r = check_paged(a, op)) return r;
+  if (int r = check_tokens(a, op)) return r;
   if (a->B == 0 || a->T == 0 || a->N == 0) return 0;
   lmoe::launch_paged_append(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged_kv_read(const lmoe_paged_args* a, void* stream) {
+  const char* op = "lmoe_paged_kv_read";
+  if (int r = check_paged(a, op)) return r;
+  if (int r = check_tokens(a, op)) return r;
+  if (a->B == 0 || a->T == 0 || a->N == 0) return 0;
+  lmoe::launch_paged_read(lmoe_paged4_args{*a, {}, {}}, false, (hipStream_t)stream);
+  return launched(op);
+}
+
+static int check_paged4(const lmoe_paged4_args* a, const char* op) {
+  if (!a) return fail(-1, "%s: null argument block", op);
+  if (int r = check_paged(&a->p, op, true)) return r;
+  if (a->p.K % 32 || a->p.V % 32) return fail(-3, "%s: head dims K=%d V=%d unsupported in 4 bits (multiples of 32)", op, a->p.K, a->p.V);
+  if ((!a->ks.ptr || !a->vs.ptr) && a->p.P > 0) return fail(-7, "%s: ks and vs must not be null", op);
+  const lmoe_tensor* rows[] = {&a->p.kp, &a->p.vp};
+  for (const lmoe_tensor* t : rows)
+    if (((uintptr_t)t->ptr & 15) || t->sb % 16 || t->st % 16 || t->sh % 16) return fail(-9, "%s: the pages need 16-byte aligned rows (pointer and strides)", op);
+  return 0;
+}
+int64_t lmoe_paged4_attn_floats(const lmoe_paged4_args* a) {
+  const char* op = "lmoe_paged4_attn_floats";
+  if (int r = check_paged4(a, op)) return r;
+  if (int r = check_decode(&a->p, op, true)) return r;
+  return lmoe::paged4_attn_floats(a->p);
+}
+int lmoe_paged4_attn_decode(const lmoe_paged4_args* a, void* stream) {
+  const char* op = "lmoe_paged4_attn_decode";
+  if (int r = check_paged4(a, op)) return r;
+  if (int r = check_decode(&a->p, op, true)) return r;
+  if (!a->p.q.ptr || !a->p.o.ptr) return fail(-7, "%s: q and o must not be null", op);
+  if (a->p.N == 0) return 0;
+  if (lmoe::paged4_attn_floats(a->p) > 0 && (!a->p.ws || ((uintptr_t)a->p.ws & 15))) return fail(-11, "%s: ws must be a 16-byte aligned pointer", op);
+  lmoe::launch_paged4_decode(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged4_kv_append(const lmoe_paged4_args* a, void* stream) {
+  const char* op = "lmoe_paged4_kv_append";
+  if (int r = check_paged4(a, op)) return r;
+  if (int r = check_tokens(&a->p, op)) return r;
+  if (a->p.B == 0 || a->p.T == 0 || a->p.N == 0) return 0;
+  lmoe::launch_paged4_append(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged4_kv_read(const lmoe_paged4_args* a, void* stream) {
+  const char* op = "lmoe_paged4_kv_read";
+  if (int r = check_paged4(a, op)) return r;
+  if (int r = check_tokens(&a->p, op)) return r;
+  if (a->p.B == 0 || a->p.T == 0 || a->p.N == 0) return 0;
+  lmoe::launch_paged_read(*a, true, (hipStream_t)stream);
+  return launched(op);
+}
+
+static int check_rope(const lmoe_rope_args* a, const char* op, bool bwd) {
+  if (!a) return fail(-1, "%s: null argument block", op);
+  for (const int32_t t : {a->dtype, a->w_dtype})
+    if (t != LMOE_BF16 && t != LMOE_F32) return fail(-2, "%s: dtype and w_dtype must be LMOE_BF16 or LMOE_F32", op);
+  if (a->D <= 0 || a->D > 256 || a->D % 2) return fail(-3, "%s: head dim D=%d unsupported (even, at most 256)", op, a->D);
+  if (a->R < 0 || a->R > a->D || a->R % 2) return fail(-3, "%s: R=%d must be even, 0 to D=%d", op, a->R, a->D);
+  if (a->B < 0 || a->T < 0 || a->HQ <= 0 || a->HKV <= 0 || a->N < 0 || a->L < 0) return fail(-4, "%s: negative dimension", op);
+  if (a->HQ > 65535 || a->HKV > 65535) return fail(-8, "%s: heads must be <= 65535", op);
+  if (a->cu_seqlens && (a->B != 1 || a->positions)) return fail(-5, "%s: packed input needs B == 1 and no positions", op);
+  if (a->positions && a->offsets) return fail(-5, "%s: positions and offsets exclude each other", op);
+  if (!a->q.ptr || !a->k.ptr) return fail(-7, "%s: q and k must not be null", op);
+  if (a->R > 0 && a->L > 0 && (!a->cos || !a->sin)) return fail(-7, "%s: cos and sin must not be null", op);
+  if (!(a->eps >= 0.f)) return fail(-15, "%s: eps must not be negative", op);
+  if (!a->norm && (a->qw || a->kw || a->dqw || a->dkw)) return fail(-15, "%s: weights belong to the norm", op);
+  if (!bwd && (!a->zq.ptr || !a->zk.ptr)) return fail(-7, "%s: zq and zk must not be null", op);
+  if (bwd && (!a->dzq.ptr || !a->dzk.ptr || !a->dq.ptr || !a->dk.ptr)) return fail(-11, "%s: dzq, dzk, dq and dk must not be null", op);
+  return 0;
+}
+int64_t lmoe_qk_norm_rope_floats(const lmoe_rope_args* a) {
+  if (int r = check_rope(a, "lmoe_qk_norm_rope_floats", true)) return r;
+  return a->dqw || a->dkw ? lmoe::rope_floats(*a) : 0;
+}
+int lmoe_qk_norm_rope_fwd(const lmoe_rope_args* a, void* stream) {
+  const char* op = "lmoe_qk_norm_rope_fwd";
+  if (int r = check_rope(a, op, false)) return r;
+  if (a->B == 0 || a->T == 0) return 0;
+  lmoe::launch_qk_norm_rope(*a, false, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_qk_norm_rope_bwd(const lmoe_rope_args* a, void* stream) {
+  const char* op = "lmoe_qk_norm_rope_bwd";
+  if (int r = check_rope(a, op, true)) return r;
+  if ((a->dqw || a->dkw) && (!a->ws || ((uintptr_t)a->ws & 15))) return fail(-11, "%s: ws must be a 16-byte aligned pointer", op);
+  if (a->B == 0 || a->T == 0) return 0;
+  lmoe::launch_qk_norm_rope(*a, true, (hipStream_t)stream);
+  return launched(op);
+}
+
+static int check_pages(const lmoe_pages_args* a, const char* op, bool rows, bool bufs) {
+  if (!a) return fail(-1, "%s: null argument block", op);
+  if (a->N < 0 || a->M < 0 || a->P < 0 || a->F < 0 || a->n_bufs < 0 || (bufs && a->S <= 0)) return fail(-4, "%s: negative dimension", op);
+  if ((int64_t)a->N * a->M > 1 << 30) return fail(-8, "%s: a table of %d x %d: at most 2^30 entries", op, a->N, a->M);
+  if (a->F >= MAX_GROUPS) return fail(-8, "%s: more than 2^24 - 1 rows", op);
+  if (bufs && (int64_t)a->M * a->S > 1 << 30) return fail(-8, "%s: %d pages of %d tokens per sequence: positions must stay below 2^30", op, a->M, a->S);
+  if ((!a->table && (int64_t)a->N * a->M > 0) || (!a->refs && a->P > 0)) return fail(-7, "%s: table and refs must not be null", op);
+  if (a->N > 1 && a->table_stride < a->M) return fail(-9, "%s: rows of the table overlap", op);
+  if (rows && a->F > 0 && a->N > 0 && (!a->rows || !a->lens)) return fail(-7, "%s: rows and lens must not be null", op);
+  if (bufs && !a->ws) return fail(-11, "%s: ws must not be null", op);
+  for (int k = 0; bufs && k < a->n_bufs; ++k) {
+    if (!a->bufs) return fail(-7, "%s: bufs must not be null", op);
+    const lmoe_page_buf& b = a->bufs[k];
+    if (!b.ptr && a->P > 0) return fail(-7, "%s: tensor %d of the pages is null", op, k);
+    if (b.bytes < 0 || b.rows0 < 0 || b.rows1 < 0 || (double)b.bytes * b.rows0 * b.rows1 > 1e11 || (int64_t)b.rows0 * b.rows1 > 1 << 24)
+      return fail(-8, "%s: tensor %d: a page of %d x %d runs of %lld bytes", op, k, b.rows0, b.rows1, (long long)b.bytes);
+  }
+  return 0;
+}
+int64_t lmoe_paged_fork_ints(const lmoe_pages_args* a) {
+  if (int r = check_pages(a, "lmoe_paged_fork_ints", false, false)) return r;
+  return lmoe::fork_ints(*a);
+}
+int64_t lmoe_paged_pages_ints(const lmoe_pages_args* a) {
+  if (int r = check_pages(a, "lmoe_paged_pages_ints", false, false)) return r;
+  return lmoe::pages_ints(*a);
+}
+int lmoe_paged_free(const lmoe_pages_args* a, void* stream) {
+  const char* op = "lmoe_paged_free";
+  if (int r = check_pages(a, op, true, false)) return r;
+  if (a->F == 0 || a->N == 0) return 0;
+  lmoe::launch_pages_free(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged_fork(const lmoe_pages_args* a, void* stream) {
+  const char* op = "lmoe_paged_fork";
+  if (int r = check_pages(a, op, true, false)) return r;
+  if (a->F == 0 || a->N == 0) return 0;
+  if (!a->src) return fail(-7, "%s: src must not be null", op);
+  if (!a->ws) return fail(-11, "%s: ws must not be null", op);
+  lmoe::launch_pages_fork(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged_reserve(const lmoe_pages_args* a, void* stream) {
+  const char* op = "lmoe_paged_reserve";
+  if (int r = check_pages(a, op, false, true)) return r;
+  if (a->N == 0) return 0;
+  if (!a->lens || !a->fits) return fail(-7, "%s: lens and fits must not be null", op);
+  lmoe::launch_pages_reserve(*a, (hipStream_t)stream);
+  return launched(op);
+}
+int lmoe_paged_compact(const lmoe_pages_args* a, void* stream) {
+  const char* op = "lmoe_paged_compact";
+  if (int r = check_pages(a, op, false, true)) return r;
+  if (!a->live || (!a->moved && a->P > 0)) return fail(-7, "%s: live and moved must not be null", op);
+  lmoe::launch_pages_compact(*a, (hipStream_t)stream);
   return launched(op);
 }
 

@@ -133,5 +133,20 @@ int64_t attn_groups(const lmoe_attn_args& a);                     // work-groups
 int64_t paged_attn_floats(const lmoe_paged_args& a);
 void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st);
 void launch_paged_append(const lmoe_paged_args& a, hipStream_t st);
+// the same over a cache in 4 bits; reading either back
+int64_t paged4_attn_floats(const lmoe_paged_args& a);
+void launch_paged4_decode(const lmoe_paged4_args& a, hipStream_t st);
+void launch_paged4_append(const lmoe_paged4_args& a, hipStream_t st);
+void launch_paged_read(const lmoe_paged4_args& a, bool bits4, hipStream_t st);
+// norm and rotation of queries and keys
+int64_t rope_floats(const lmoe_rope_args& a);
+void launch_qk_norm_rope(const lmoe_rope_args& a, bool bwd, hipStream_t st);
+// pages of a cache
+int64_t pages_ints(const lmoe_pages_args& a);
+int64_t fork_ints(const lmoe_pages_args& a);
+void launch_pages_free(const lmoe_pages_args& a, hipStream_t st);
+void launch_pages_fork(const lmoe_pages_args& a, hipStream_t st);
+void launch_pages_reserve(const lmoe_pages_args& a, hipStream_t st);
+void launch_pages_compact(const lmoe_pages_args& a, hipStream_t st);
 void launch_selftest(int dtype, int kd, const void* A, const void* B, float* C, float* G, hipStream_t st);
 }  // namespace lmoe

@@ -11,22 +11,10 @@
 // So there is no LDS traffic and no barrier per step, and 16 lanes read 256 adjacent bytes of a value row.
 // HBM-bound: the keys and values of the live tokens are read once for all heads that share them.
 // The stretches of a sequence are joined by k_paged_join where there is more than one.
-#include "lmoe_attn.hpp"
+#include "lmoe_paged.hpp"
 
 namespace lmoe {
 
-constexpr int PSTEP = 32;              // positions a wave takes at a time
-constexpr int PHEADS = 16;             // query heads of a work-group
-constexpr int PSPLITS = 2048;          // stretches of a sequence at most
-
-struct PagedPlan {
-  int splits;      // stretches per sequence at most
-  int chunk;       // positions of a stretch at least
-  int waves;       // of a work-group
-  int blocks;      // work-groups that share a key head's query heads
-  uint32_t div_m;  // j / S = (umulhi(j, div_m) + j) >> div_s for 0 <= j < 2^31
-  int div_s;
-};
 static PagedPlan paged_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
@@ -54,20 +42,6 @@ int64_t paged_attn_floats(const lmoe_paged_args& a) {
   return p.splits > 1 ? (int64_t)a.N * a.HQ * p.splits * (a.V + 2) : 0;
 }
 
-// Tokens the new one attends to in the cache, and the length of a stretch
-struct PagedSeq { int len, chunk, used; };
-__device__ __forceinline__ PagedSeq paged_seq(const lmoe_paged_args& a, const PagedPlan& p, int n) {
-  PagedSeq s;
-  const int step = p.waves * PSTEP;
-  const int len = as_const(a.lens)[n], room = a.M * a.S;
-  s.len = len < 0 ? 0 : len > room ? room : len;
-  const int total = s.len + (a.kn.ptr ? 1 : 0);
-  const int per = (total + p.splits - 1) / p.splits;
-  s.chunk = per <= p.chunk ? p.chunk : (per + step - 1) / step * step;
-  s.used = (total + s.chunk - 1) / s.chunk;
-  return s;
-}
-
 template <typename T, int W> struct PagedTile {
   static constexpr int KS = W / 32, VW = W / 16, PIECE = VW < ET<T>::VEC ? VW : ET<T>::VEC;
   typedef T piece __attribute__((ext_vector_type(PIECE)));
@@ -75,20 +49,6 @@ template <typename T, int W> struct PagedTile {
   piece v[8][VW / PIECE];
   uint32_t live;         // which of the 32 positions exist
 };
-
-template <typename T> __device__ __forceinline__ typename ET<T>::frag zero_frag() {
-  typename ET<T>::frag f;
-  if constexpr (sizeof(T) == 2) f = ET<T>::zero(); else { f.lo = ET<T>::zero(); f.hi = ET<T>::zero(); }
-  return f;
-}
-// eight columns from d of a row of D (a multiple of 16 bytes), zeros behind its end
-template <typename T, bool ALL> __device__ __forceinline__ typename ET<T>::frag load_cols(const T* row, int d, int D) {
-  if constexpr (ALL) return ET<T>::load_frag(row + d);
-  typename ET<T>::frag f = zero_frag<T>();
-  if constexpr (sizeof(T) == 2) { if (d < D) f = ET<T>::load_frag(row + d); }
-  else { if (d < D) f.lo = *(const f32x4*)(row + d); if (d + 4 < D) f.hi = *(const f32x4*)(row + d + 4); }
-  return f;
-}
 
 // ALL: the head dimension of q and k is W.
 template <typename T, int W, int NW, bool CAP, bool BIAS, bool ALL>
@@ -353,6 +313,13 @@ __global__ __launch_bounds__(NTHR) void k_paged_join(const lmoe_paged_args a, co
   }
 }
 
+void launch_paged_join(const lmoe_paged_args& a, const PagedPlan& p, hipStream_t st) {
+  if (p.splits <= 1) return;
+  const dim3 grid((uint32_t)((int64_t)a.N * a.HQ));
+  if (a.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_join<bf16>), grid, dim3(NTHR), 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged_join<float>), grid, dim3(NTHR), 0, st, a, p);
+}
+
 template <typename T, int W, int NW, bool ALL> static void paged_parts(const lmoe_paged_args& a, const PagedPlan& p, hipStream_t st) {
   const dim3 grid((uint32_t)((int64_t)a.N * a.HKV * p.blocks * p.splits)), block(64 * NW);
   if (a.softcap > 0.f) {
@@ -371,7 +338,7 @@ template <typename T, int W> static void paged_decode(const lmoe_paged_args& a, 
   if (p.waves == 4) {
     if (a.K == W) paged_parts<T, W, 4, true>(a, p, st); else paged_parts<T, W, 4, false>(a, p, st);
   }
-  if (p.splits > 1) hipLaunchKernelGGL((k_paged_join<T>), dim3((uint32_t)((int64_t)a.N * a.HQ)), dim3(NTHR), 0, st, a, p);
+  launch_paged_join(a, p, st);
 }
 void launch_paged_decode(const lmoe_paged_args& a, hipStream_t st) {
   const bool narrow = a.K <= 64 && a.V <= 64;

@@ -1,0 +1,483 @@
+// A paged cache of keys and values in 4 bits (include/lmoe.h, lmoe_paged4_args): its writing, its reading, and the attention of one
+// new token over it; and the reading of a cache in elements of 2 and 4 bytes.
+//
+// 32 columns of a row share a power of two 2^e, and each is one of 0 0.5 1 1.5 2 3 4 6 times it, with a sign: the format that the card's
+// conversions v_cvt_scalef32_pk_{bf16,f32}_fp4 and back take.  The values are exact in a bfloat16, so that the products with them are
+// those of a cache of 2-byte elements that holds the same numbers; and whatever order things are done in, what is written is the
+// same bits.  A row of D columns is D / 2 + D / 32 bytes in place of 2 D.
+//
+// k_paged4_attn lies in registers as k_paged_attn does (lmoe_paged.hip); what differs:
+//   K: the contraction index may be numbered freely, so lane (c, g) holds a quarter of key c's columns, W / 4 from W / 4 g on: 16 (8)
+//     adjacent bytes and, with 128 columns, one scale.  Eight columns of them are the A operand of a product.
+//   V: lane (c, g) holds its eight keys at columns VW c .. + VW - 1, VW / 2 bytes and a scale each.
+//   The new token is made into 4 bits by the wave that attends to it, in the registers it is attended from.
+#include "lmoe_paged.hpp"
+
+namespace lmoe {
+
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// ---- 4 bits ----
+// The scale byte of 32 columns whose largest size is `most` (no NaN among them, or `most` is one)
+__device__ __forceinline__ uint32_t scale4(float most) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, most);
+  if (b >= 0x7f800000u) return 255;
+  // 6 2^e >= most: a mantissa up to 1.5 fits at its exponent less 2, another at that less 1.  At least 2^-120, so that no value is
+  // below the normal numbers; at most 2^125, so that 6 2^e is finite.
+  const int x = (int)((b + 0x3fffffu) >> 23) - 2;
+  return x < 7 ? 7 : x > 252 ? 252 : x;
+}
+__device__ __forceinline__ float scale_of(uint32_t x) { return __builtin_bit_cast(float, x << 23); }       // (of 255: makes every value NaN)
+// the larger of two sizes, a NaN where one is
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b))); }
+// eight columns into a word, and back
+template <typename T> __device__ __forceinline__ uint32_t to4(const typename ET<T>::frag& x, float scale) {
+  uint32_t r = 0;
+  if constexpr (sizeof(T) == 2) {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_shufflevector(x, x, 0, 1), scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_shufflevector(x, x, 2, 3), scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_shufflevector(x, x, 4, 5), scale, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_shufflevector(x, x, 6, 7), scale, 3);
+  } else {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.lo[0], x.lo[1], scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.lo[2], x.lo[3], scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.hi[0], x.hi[1], scale, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, x.hi[2], x.hi[3], scale, 3);
+  }
+  return r;
+}
+template <typename T> __device__ __forceinline__ typename ET<T>::frag from4(uint32_t r, float scale) {
+  if constexpr (sizeof(T) == 2) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r, scale, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r, scale, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  } else {
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, scale, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(r, scale, 3);
+    f32frag f;
+    f.lo = f32x4{a[0], a[1], b[0], b[1]};
+    f.hi = f32x4{c[0], c[1], d[0], d[1]};
+    return f;
+  }
+}
+template <typename T> __device__ __forceinline__ float size_of(const typename ET<T>::frag& x) {
+  float m = 0.f;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = larger(m, fabsf((float)x[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = larger(m, larger(fabsf(x.lo[i]), fabsf(x.hi[i])));
+  }
+  return m;
+}
+template <typename T> __device__ __forceinline__ void store_frag(T* p, const typename ET<T>::frag& x) {
+  if constexpr (sizeof(T) == 2) *(bf16x8*)p = x; else { *(f32x4*)p = x.lo; *(f32x4*)(p + 4) = x.hi; }
+}
+
+// ---- written and read: a wave per token ----
+// Token `tok` of a call: its sequence n, its row and place in memory, and its place in the sequence; false: behind the last one
+struct PagedToken { int n, b, t, at; };
+__device__ __forceinline__ bool paged_token(const lmoe_paged_args& a, int64_t tok, PagedToken& x) {
+  if (a.cu_seqlens) {
+    // the last sequence that begins at or before the token (of several, all but the last are empty): 64 candidates a round
+    x.b = 0; x.t = (int)tok;
+    if (x.t >= a.cu_seqlens[a.N] || x.t < a.cu_seqlens[0]) return false;
+    int lo = 0, hi = a.N;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, i = lo + lane_id() * step;
+      const int cnt = __popcll(__ballot(i < hi && a.cu_seqlens[min(i, a.N)] <= x.t));
+      lo += (cnt - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    x.n = lo;
+    x.at = x.t - a.cu_seqlens[lo];
+  } else {
+    x.n = x.b = (int)(tok / a.T);
+    x.t = x.at = (int)(tok - (int64_t)x.b * a.T);
+  }
+  return true;
+}
+// page and slot of a token; -1: it has none
+__device__ __forceinline__ int paged_slot(const lmoe_paged_args& a, const PagedToken& x, int& slot) {
+  const int64_t pos = (int64_t)a.lens[x.n] + x.at;
+  slot = 0;
+  if (a.lens[x.n] < 0 || pos >= (int64_t)a.M * a.S) return -1;
+  const int id = a.table[(int64_t)x.n * a.table_stride + (int)pos / a.S];
+  slot = (int)pos % a.S;
+  return id < 0 || id >= a.P ? -1 : id;
+}
+
+template <typename T> __global__ __launch_bounds__(NTHR) void k_paged4_append(const lmoe_paged4_args a4) {
+  const lmoe_paged_args& a = a4.p;
+  const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
+  if (tok >= (int64_t)a.B * a.T) return;
+  PagedToken x;
+  if (!paged_token(a, tok, x)) return;
+  int slot;
+  const int id = paged_slot(a, x, slot);
+  if (id < 0) return;
+  const int l = lane_id();
+  auto write = [&](const lmoe_tensor& from, const lmoe_tensor& to, const lmoe_tensor& scales, int D) {
+    const T* s = (const T*)from.ptr + (int64_t)x.b * from.sb + (int64_t)x.t * from.st;
+    uint8_t* d = (uint8_t*)to.ptr + (int64_t)id * to.sb + (int64_t)slot * to.st;
+    uint8_t* e = (uint8_t*)scales.ptr + (int64_t)id * scales.sb + (int64_t)slot * scales.st;
+    const int per = D / 8;                 // lanes of a row: four for each scale
+    for (int i0 = 0; i0 < a.HKV * per; i0 += 64) {
+      const int i = i0 + l, h = i / per, c = i % per;
+      const bool on = i < a.HKV * per;
+      typename ET<T>::frag y = zero_frag<T>();
+      if (on) y = ET<T>::load_frag(s + (int64_t)h * from.sh + 8 * c);
+      float most = size_of<T>(y);
+      most = larger(most, __shfl_xor(most, 1, 64));
+      most = larger(most, __shfl_xor(most, 2, 64));
+      const uint32_t sc = scale4(most);
+      if (!on) continue;
+      *(uint32_t*)(d + (int64_t)h * to.sh + 4 * c) = to4<T>(y, scale_of(sc));
+      if ((c & 3) == 0) e[(int64_t)h * scales.sh + (c >> 2)] = (uint8_t)sc;
+    }
+  };
+  write(a.kn, a.kp, a4.ks, a.K);
+  write(a.vn, a.vp, a4.vs, a.V);
+}
+
+// BITS4: of a cache in 4 bits, else of elements of the same type
+template <typename T, bool BITS4> __global__ __launch_bounds__(NTHR) void k_paged_read(const lmoe_paged4_args a4) {
+  constexpr int VEC = BITS4 ? 8 : ET<T>::VEC;
+  const lmoe_paged_args& a = a4.p;
+  const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
+  if (tok >= (int64_t)a.B * a.T) return;
+  PagedToken x;
+  int slot = 0, id = -1;
+  if (paged_token(a, tok, x)) id = paged_slot(a, x, slot);
+  const int l = lane_id();
+  auto read = [&](const lmoe_tensor& from, const lmoe_tensor& scales, const lmoe_tensor& to, int D) {
+    T* d = (T*)to.ptr + (int64_t)x.b * to.sb + (int64_t)x.t * to.st;
+    const int64_t page = id < 0 ? 0 : id;
+    const int per = D / VEC;
+    for (int i = l; i < a.HKV * per; i += 64) {
+      const int h = i / per, c = i % per;
+      T* row = d + (int64_t)h * to.sh + VEC * c;
+      if constexpr (BITS4) {
+        typename ET<T>::frag y = zero_frag<T>();
+        if (id >= 0) {
+          const uint32_t r = *(const uint32_t*)((const uint8_t*)from.ptr + page * from.sb + (int64_t)slot * from.st + (int64_t)h * from.sh + 4 * c);
+          y = from4<T>(r, scale_of(*((const uint8_t*)scales.ptr + page * scales.sb + (int64_t)slot * scales.st + (int64_t)h * scales.sh + (c >> 2))));
+        }
+        store_frag<T>(row, y);
+      } else {
+        typename ET<T>::vec y = ET<T>::zero();
+        if (id >= 0) y = *(const typename ET<T>::vec*)((const T*)from.ptr + page * from.sb + (int64_t)slot * from.st + (int64_t)h * from.sh + VEC * c);
+        *(typename ET<T>::vec*)row = y;
+      }
+    }
+  };
+  read(a.kp, a4.ks, a.kn, a.K);
+  read(a.vp, a4.vs, a.vn, a.V);
+}
+
+static uint32_t token_groups(const lmoe_paged_args& a) { return (uint32_t)(((int64_t)a.B * a.T + NTHR / 64 - 1) / (NTHR / 64)); }
+void launch_paged4_append(const lmoe_paged4_args& a, hipStream_t st) {
+  if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged4_append<bf16>), dim3(token_groups(a.p)), dim3(NTHR), 0, st, a);
+  else hipLaunchKernelGGL((k_paged4_append<float>), dim3(token_groups(a.p)), dim3(NTHR), 0, st, a);
+}
+void launch_paged_read(const lmoe_paged4_args& a, bool bits4, hipStream_t st) {
+  const dim3 grid(token_groups(a.p)), block(NTHR);
+  if (bits4) {
+    if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_read<bf16, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_paged_read<float, true>), grid, block, 0, st, a);
+  } else if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_read<bf16, false>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((k_paged_read<float, false>), grid, block, 0, st, a);
+}
+
+// ---- one new token ----
+static PagedPlan paged4_plan(const lmoe_paged_args& a) {
+  PagedPlan p;
+  p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
+  const int64_t bound = (int64_t)a.M * a.S + 1, groups = (int64_t)a.N * a.HKV * p.blocks;
+  p.waves = 4;
+  const int64_t chunk = 512;
+  const int64_t splits = (bound + chunk - 1) / chunk;
+  const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;
+  p.splits = (int)(splits < most ? splits : most);
+  p.chunk = (int)chunk;
+  p.div_s = 0;
+  while ((1ll << p.div_s) < a.S) ++p.div_s;
+  p.div_m = (uint32_t)((((1ull << p.div_s) - (uint64_t)a.S) << 32) / (uint64_t)a.S + 1);
+  return p;
+}
+int64_t paged4_attn_floats(const lmoe_paged_args& a) {
+  const PagedPlan p = paged4_plan(a);
+  return p.splits > 1 ? (int64_t)a.N * a.HQ * p.splits * (a.V + 2) : 0;        // (as k_paged_join reads it)
+}
+
+// 32 positions of the cache, as a wave holds them
+template <int W> struct Tile4 {
+  static constexpr int KW = W / 32;                // words of a lane's columns of a key
+  uint32_t k[2][KW];
+  uint32_t ks[2];
+  uint32_t v[8];                                   // the low half alone with 64 columns
+  uint32_t vs[8];
+  uint32_t live;                                   // which of the positions exist
+};
+
+template <typename T, int W, int NW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
+  const lmoe_paged_args& a = a4.p;
+  typedef Tile4<W> Tile;
+  constexpr int KW = Tile::KW, KC = W / 4, VW = W / 16;
+  constexpr bool FAST = sizeof(T) == 2;
+  constexpr int PGROUP = NW * PSTEP;        // positions the work-group takes at a time
+  typedef uint32_t words __attribute__((ext_vector_type(KW)));
+  __shared__ __attribute__((aligned(16))) float s_o[NW][PHEADS][W + 4];
+  __shared__ float s_m[NW][PHEADS], s_l[NW][PHEADS];
+  // (the order of the work-groups as in k_paged_attn)
+  const int part = blockIdx.x % p.splits, group = blockIdx.x / p.splits;
+  const int n = group / (a.HKV * p.blocks), hb = group % (a.HKV * p.blocks), hk = hb / p.blocks, G = a.HQ / a.HKV;
+  const int h0 = hb % p.blocks * PHEADS, heads = min(PHEADS, G - h0);      // of the key head's group
+  const PagedSeq sq = paged_seq(a, p, n);
+  const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = part * sq.chunk;
+  if (begin >= total && part > 0) return;
+  const int stop = min(total, begin + sq.chunk), end = min(stop, sq.len);       // the stretch, and its part in the cache
+  const int l = lane_id(), w = wave_id(), c = l & 15, g = l >> 4;
+  const int32_t* table = a.table + (int64_t)n * a.table_stride;
+  const uint8_t* kp = (const uint8_t*)a.kp.ptr + (int64_t)hk * a.kp.sh;
+  const uint8_t* vp = (const uint8_t*)a.vp.ptr + (int64_t)hk * a.vp.sh;
+  const uint8_t* ksp = (const uint8_t*)a4.ks.ptr + (int64_t)hk * a4.ks.sh;
+  const uint8_t* vsp = (const uint8_t*)a4.vs.ptr + (int64_t)hk * a4.vs.sh;
+  const bool kin = KC * g < a.K, vin = VW * c < a.V;           // columns behind the head dimension are zeros
+
+  // Where the lane's position (j0 + l % 32) lies; asked for two steps before its rows are used, as in k_paged_attn
+  struct Where { int id, slot; };
+  auto ask = [&](int j0) {
+    Where x = {-1, 0};
+    const int j = j0 + (l & 31);
+    if (j < end) {
+      const int col = (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s);
+      x.slot = j - col * a.S;
+      x.id = table[col];
+    }
+    return x;
+  };
+  auto load = [&](Tile& t, const Where& x) {
+    const bool there = x.id >= 0 && x.id < a.P;
+    t.live = (uint32_t)__ballot(there);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t id = __shfl(x.id, 16 * b + c, 64), slot = __shfl(x.slot, 16 * b + c, 64);
+      words y;
+#pragma unroll
+      for (int i = 0; i < KW; ++i) y[i] = 0;
+      t.ks[b] = 127;
+      if ((t.live >> (16 * b + c) & 1) && kin) {
+        y = *(const words*)(kp + id * a.kp.sb + slot * a.kp.st + KC / 2 * g);
+        t.ks[b] = ksp[id * a4.ks.sb + slot * a4.ks.st + KC * g / 32];
+      }
+#pragma unroll
+      for (int i = 0; i < KW; ++i) t.k[b][i] = y[i];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int at = 16 * (e >> 2) + 4 * g + (e & 3);
+      const int64_t id = __shfl(x.id, at, 64), slot = __shfl(x.slot, at, 64);
+      t.v[e] = 0;
+      t.vs[e] = 127;
+      if ((t.live >> at & 1) && vin) {
+        const uint8_t* row = vp + id * a.vp.sb + slot * a.vp.st + VW / 2 * c;
+        if constexpr (VW == 8) t.v[e] = *(const uint32_t*)row; else t.v[e] = *(const uint16_t*)row;
+        t.vs[e] = vsp[id * a4.vs.sb + slot * a4.vs.st + VW * c / 32];
+      }
+    }
+  };
+
+  int j0 = begin + PSTEP * w;
+  Where at = ask(j0), ahead = ask(j0 + PGROUP);
+
+  typename ET<T>::frag q[KW];
+  const int hq = hk * G + h0 + min(c, heads - 1);
+  {
+    const T* row = (const T*)a.q.ptr + (int64_t)n * a.q.sb + (int64_t)hq * a.q.sh;
+#pragma unroll
+    for (int j = 0; j < KW; ++j) q[j] = kin ? ET<T>::load_frag(row + KC * g + 8 * j) : zero_frag<T>();
+  }
+  const Score<CAP, BIAS, FAST> sc(a.scale, a.softcap, a.slopes, hq);
+
+  f32x4 o[VW];
+#pragma unroll
+  for (int i = 0; i < VW; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = M_LOW, sum = 0.f;
+  auto take = [&](const Tile& t, int j0) {
+    f32x4 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KW; ++j) ET<T>::mma(s[b], from4<T>(t.k[b][j], scale_of(t.ks[b])), q[j]);
+    }
+    float mx = M_LOW;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = j0 + 16 * b + 4 * g + e;
+        const float x = sc.of(s[b][e], CAP ? sc.squash(s[b][e]) : 0.f, (float)(total - 1 - j));
+        s[b][e] = t.live >> (16 * b + 4 * g + e) & 1 ? x : -INFINITY;
+        mx = fmaxf(mx, s[b][e]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float next = fmaxf(m, mx), f = pow2(m - next);
+    m = next;
+    sum *= f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[b][e] = pow2(s[b][e] - m);
+        sum += s[b][e];
+      }
+    // (P rounded to the element type, as the products take it; the sum is of the numbers before)
+    typename ET<T>::frag pf;
+    if constexpr (FAST) pf = frag_of_blocks(s[0], s[1]); else { pf.lo = s[0]; pf.hi = s[1]; }
+    typename ET<T>::frag v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = from4<T>(t.v[e], scale_of(t.vs[e]));
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+      o[i] *= f;
+      typename ET<T>::frag vf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (FAST) vf[e] = v[e][i];
+        else {
+          const float x = i < 4 ? v[e].lo[i & 3] : v[e].hi[i & 3];
+          if (e < 4) vf.lo[e] = x; else vf.hi[e - 4] = x;
+        }
+      }
+      ET<T>::mma(o[i], vf, pf);
+    }
+  };
+
+  Tile t[2];
+  if (j0 < end) load(t[0], at);
+  // the new token: the first of 32 positions that hold nothing else
+  if (a.kn.ptr && stop == total && w == (end - begin + PSTEP - 1) / PSTEP % NW) {
+    const T* kn = (const T*)a.kn.ptr + (int64_t)n * a.kn.sb + (int64_t)hk * a.kn.sh;
+    const T* vn = (const T*)a.vn.ptr + (int64_t)n * a.vn.sb + (int64_t)hk * a.vn.sh;
+    Tile y = {};
+    y.live = 1;
+    typename ET<T>::frag x[KW];
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      x[j] = kin ? ET<T>::load_frag(kn + KC * g + 8 * j) : zero_frag<T>();
+      most = larger(most, size_of<T>(x[j]));
+    }
+    if constexpr (KC < 32) most = larger(most, __shfl_xor(most, 16, 64));
+    y.ks[0] = scale4(most);
+    y.ks[1] = 127;
+#pragma unroll
+    for (int j = 0; j < KW; ++j) y.k[0][j] = to4<T>(x[j], scale_of(y.ks[0]));
+    typename ET<T>::frag z = zero_frag<T>();
+    if (vin) {
+      if constexpr (VW == 8) z = ET<T>::load_frag(vn + VW * c);
+      else if constexpr (FAST) { const bf16x4 u = *(const bf16x4*)(vn + VW * c); z[0] = u[0]; z[1] = u[1]; z[2] = u[2]; z[3] = u[3]; }
+      else z.lo = *(const f32x4*)(vn + VW * c);
+    }
+    float big = size_of<T>(z);
+#pragma unroll
+    for (int d = 1; d < 32 / VW; d <<= 1) big = larger(big, __shfl_xor(big, d, 64));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y.vs[e] = 127;
+    y.vs[0] = scale4(big);
+    y.v[0] = to4<T>(z, scale_of(y.vs[0]));
+    // into its page, by one of the work-groups that share the key head
+    const int page = sq.len / a.S, slot = sq.len % a.S;
+    const int id = h0 == 0 && as_const(a.lens)[n] == sq.len && page < a.M ? as_const(table)[page] : -1;
+    if (id >= 0 && id < a.P) {
+      if (c == 0 && kin) {
+        words out;
+#pragma unroll
+        for (int i = 0; i < KW; ++i) out[i] = y.k[0][i];
+        *(words*)((uint8_t*)kp + (int64_t)id * a.kp.sb + (int64_t)slot * a.kp.st + KC / 2 * g) = out;
+        if (KC * g % 32 == 0) ((uint8_t*)ksp)[(int64_t)id * a4.ks.sb + (int64_t)slot * a4.ks.st + KC * g / 32] = (uint8_t)y.ks[0];
+      }
+      if (g == 0 && vin) {
+        uint8_t* row = (uint8_t*)vp + (int64_t)id * a.vp.sb + (int64_t)slot * a.vp.st + VW / 2 * c;
+        if constexpr (VW == 8) *(uint32_t*)row = y.v[0]; else *(uint16_t*)row = (uint16_t)y.v[0];
+        if (VW * c % 32 == 0) ((uint8_t*)vsp)[(int64_t)id * a4.vs.sb + (int64_t)slot * a4.vs.st + VW * c / 32] = (uint8_t)y.vs[0];
+      }
+    }
+    if (c != 0) {                     // (the other keys of the 16 and their scales: nothing)
+#pragma unroll
+      for (int j = 0; j < KW; ++j) y.k[0][j] = 0;
+      y.ks[0] = 127;
+    }
+    if (g != 0) { y.v[0] = 0; y.vs[0] = 127; }
+    take(y, sq.len);
+  }
+  while (j0 < end) {
+    at = ahead;
+    ahead = ask(j0 + 2 * PGROUP);
+    if (j0 + PGROUP < end) load(t[1], at);
+    take(t[0], j0);
+    j0 += PGROUP;
+    if (j0 >= end) break;
+    at = ahead;
+    ahead = ask(j0 + 2 * PGROUP);
+    if (j0 + PGROUP < end) load(t[0], at);
+    take(t[1], j0);
+    j0 += PGROUP;
+  }
+
+  // the waves together: lane (c, g) holds head c, columns VW (4g + r) + i
+  sum += __shfl_xor(sum, 16, 64);
+  sum += __shfl_xor(sum, 32, 64);
+  if (g == 0) { s_m[w][c] = m; s_l[w][c] = sum; }
+#pragma unroll
+  for (int i = 0; i < VW; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_o[w][c][VW * (4 * g + r) + i] = o[i][r];
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < heads * W; idx += NW * 64) {
+    const int hh = idx / W, d = idx % W;
+    if (d >= a.V) continue;
+    float mm = M_LOW;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) mm = fmaxf(mm, s_m[y][hh]);
+    float ll = 0.f, x = 0.f;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) {
+      const float f = pow2(s_m[y][hh] - mm);
+      ll += f * s_l[y][hh];
+      x += f * s_o[y][hh][d];
+    }
+    const int h = hk * G + h0 + hh;
+    if (sq.used <= 1) {
+      ((T*)a.o.ptr)[(int64_t)n * a.o.sb + (int64_t)h * a.o.sh + d] = ET<T>::from_f(ll != 0.f ? x / ll : 0.f);
+    } else {
+      const int64_t at = ((int64_t)n * a.HQ + h) * p.splits + part, rows = (int64_t)a.N * a.HQ * p.splits;
+      a.ws[at * a.V + d] = x;
+      if (d == 0) *(f32x2*)(a.ws + rows * a.V + 2 * at) = f32x2{mm, ll};
+    }
+  }
+}
+
+template <typename T, int W, int NW> static void paged4_parts(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
+  const dim3 grid((uint32_t)((int64_t)a.p.N * a.p.HKV * p.blocks * p.splits)), block(64 * NW);
+  if (a.p.softcap > 0.f) {
+    if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, true, true>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, true, false>), grid, block, 0, st, a, p);
+  } else if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, false, true>), grid, block, 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, false, false>), grid, block, 0, st, a, p);
+}
+template <typename T> static void paged4_decode(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
+  if (a.p.K <= 64 && a.p.V <= 64) paged4_parts<T, 64, 4>(a, p, st); else paged4_parts<T, 128, 4>(a, p, st);
+}
+void launch_paged4_decode(const lmoe_paged4_args& a, hipStream_t st) {
+  const PagedPlan p = paged4_plan(a.p);
+  if (a.p.dtype == LMOE_BF16) paged4_decode<bf16>(a, p, st); else paged4_decode<float>(a, p, st);
+  launch_paged_join(a.p, p, st);
+}
+
+}  // namespace lmoe

@@ -12,12 +12,19 @@ dense caches, ``linear_moe/generation``).
 view of ``[P, HKV, S, D]`` is as good).  Position j of sequence n lies in slot ``j % S`` of page ``page_table[n, j // S]``;
 ``page_table`` ``[N, M]`` and ``lens`` ``[N]`` (tokens in the cache) are int32 on the device and are never read by the host, so a
 step captures into a HIP graph and a replay follows what they hold then.  A page number outside 0 .. P - 1 names no page: its
-positions take no part and are not written.
+positions take no part and are not written.  ``paged_pages.py`` gives pages out and takes them back.
+
+In 4 bits (``k_scales``, ``v_scales`` given): ``k_pages`` ``[P, S, HKV, K/2]`` and ``k_scales`` ``[P, S, HKV, K/32]``, uint8, and so for v; K and V
+multiples of 32.  32 columns share a power of two 2^(scale - 127); a column is one of 0 0.5 1 1.5 2 3 4 6 times it, with a sign (8), the even
+column in the low half of a byte.  Written is the least scale for which no column is above 6 (7 to 252), and of the numbers the
+nearest, of two as near the even one; a NaN or infinity makes the 32 columns NaN.  The new token of ``paged_attn_decode`` is attended to as the
+cache holds it.  A row takes 17/64 of the bytes of bfloat16.  Fastest are pages in which all tokens of a head lie next to each other
+(``torch.empty(P, HKV, S, K // 2).transpose(1, 2)``).
 """
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -25,26 +32,40 @@ from . import _lib
 from ._host import _DT, _desc, has_tangent, native_call, ptr, stream_ptr
 from .softmax_attn import MAX_DIM, cap_of, has_rows16, ints_of, on_current_device, rows16, slopes_of, to_int32
 
+GROUP = 32        # columns that share a scale in 4 bits
 
-def _pages(k_pages, v_pages, page_table, lens, name):
+
+def _pages(k_pages, v_pages, page_table, lens, name, scales=(None, None), dtype=None):
+    """The block of a call; dtype: of the tokens, where the pages are in 4 bits."""
     for x, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         if x.dim() != 4:
             raise ValueError(f"{name}: {n} must be [P, S, HKV, D], got {tuple(x.shape)}")
     on_current_device(k_pages.device, name)
     dev, dt = k_pages.device, k_pages.dtype
-    if dt not in _DT or v_pages.dtype != dt:
+    bits4 = scales[0] is not None
+    if bits4:
+        if dt != torch.uint8 or v_pages.dtype != dt:
+            raise ValueError(f"{name}: pages in 4 bits must be uint8, got {dt}, {v_pages.dtype}")
+        if dtype not in _DT:
+            raise ValueError(f"{name}: the tokens must be bfloat16 or float32, got {dtype}")
+    elif dt not in _DT or v_pages.dtype != dt:
         raise ValueError(f"{name}: the pages must share dtype bfloat16 or float32, got {dt}, {v_pages.dtype}")
     if k_pages.shape[:3] != v_pages.shape[:3] or v_pages.device != dev:
         raise ValueError(f"{name}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must agree in pages, tokens and heads")
     P, S, HKV, K = k_pages.shape
     V = v_pages.shape[3]
     step = 16 // k_pages.element_size()
+    if bits4:
+        K, V, step = 2 * K, 2 * V, GROUP
     if not (0 < K <= MAX_DIM and 0 < V <= MAX_DIM) or K % step or V % step:
         raise ValueError(f"{name}: head dimensions K={K}, V={V} unsupported (multiples of {step} up to {MAX_DIM})")
     if S < 1 or HKV < 1:
         raise ValueError(f"{name}: pages of {S} tokens and {HKV} heads")
     if not (has_rows16(k_pages) and has_rows16(v_pages)):
         raise ValueError(f"{name}: the pages must keep 16-byte aligned rows (they are used in place)")
+    for x, n, d in ((scales[0], "k_scales", K), (scales[1], "v_scales", V)) if bits4 else ():
+        if x.dtype != torch.uint8 or x.device != dev or tuple(x.shape) != (P, S, HKV, d // GROUP) or (d > GROUP and x.stride(3) != 1):
+            raise ValueError(f"{name}: {n} must be uint8 {(P, S, HKV, d // GROUP)} on {dev} with adjacent columns, got {x.dtype} {tuple(x.shape)} on {x.device}")
     if page_table.dim() != 2 or page_table.is_floating_point() or page_table.is_complex() or page_table.dtype == torch.bool or page_table.device != dev:
         raise ValueError(f"{name}: page_table must be [N, M] whole numbers on {dev}, got {tuple(page_table.shape)} of {page_table.dtype} on "
                          f"{page_table.device}")
@@ -53,20 +74,55 @@ def _pages(k_pages, v_pages, page_table, lens, name):
     N, M = page_table.shape
     lens = ints_of(lens, N, dev, f"{name}: lens")
     a = _lib.PagedArgs()
-    a.dtype, a.N, a.HKV, a.K, a.V, a.P, a.S, a.M = _DT[dt], N, HKV, K, V, P, S, M
+    a.dtype, a.N, a.HKV, a.K, a.V, a.P, a.S, a.M = _DT[dtype if bits4 else dt], N, HKV, K, V, P, S, M
     a.table_stride, a.table, a.lens = page_table.stride(0), page_table.data_ptr(), lens.data_ptr()
-    a.kp, a.vp = (_lib.Tensor4(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)) for x in (k_pages, v_pages))
+    a.kp, a.vp = (_desc(x, False) for x in (k_pages, v_pages))
     return a, (page_table, lens)
 
 
-def _tokens(x, B, T, H, D, head_first, like, name):
-    """New tokens as the kernels read them."""
+def _both_scales(k_scales, v_scales, name):
+    if (k_scales is None) != (v_scales is None):
+        raise ValueError(f"{name}: k_scales and v_scales go together")
+    return k_scales, v_scales
+
+
+def _call(fn, a, scales, name, st=True):
+    """``lmoe_paged_<fn>``, or what does the same in 4 bits."""
+    lib, bits4 = _lib.load(), scales[0] is not None
+    if bits4:
+        a = _lib.Paged4Args(a, *(_desc(x, False) for x in scales))
+    f = getattr(lib, f"lmoe_paged4_{fn}" if bits4 else f"lmoe_paged_{fn}")
+    if not st:
+        n = f(C.byref(a))
+        _lib.check(min(n, 0), name)
+        return n
+    _lib.check(f(C.byref(a), stream_ptr()), name)
+
+
+def _tokens(x, B, T, H, D, head_first, like, name, dtype=None):
+    """New tokens as the kernels read them, in the type of the pages or (in 4 bits) dtype."""
     want = (B, H, T, D) if head_first else (B, T, H, D)
     if tuple(x.shape) != want:
         raise ValueError(f"{name} must have shape {want}, got {tuple(x.shape)}")
-    if x.dtype != like.dtype or x.device != like.device:
-        raise ValueError(f"{name} must be {like.dtype} on {like.device} like the pages, got {x.dtype} on {x.device}")
+    dtype = dtype or like.dtype
+    if x.dtype != dtype or x.device != like.device:
+        raise ValueError(f"{name} must be {dtype} on {like.device} like the {'pages' if dtype == like.dtype else 'queries'}, got {x.dtype} on {x.device}")
     return rows16(x.detach())
+
+
+def _packed(cu_seqlens, head_first, B, T, a, dev, name):
+    """The offsets of packed tokens as the kernels read them."""
+    if head_first:
+        raise ValueError("cu_seqlens requires head_first=False ([1, T, H, D] packed input)")
+    if B != 1:
+        raise ValueError(f"cu_seqlens requires batch size 1 (packed input), got B={B}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() != a.N + 1:
+        raise ValueError(f"{name}: cu_seqlens must hold {a.N + 1} offsets for the {a.N} rows of page_table, got {tuple(cu_seqlens.shape)}")
+    if not cu_seqlens.is_cuda:
+        offs = cu_seqlens.detach().to(torch.int64)
+        if int(offs[0]) != 0 or int(offs[-1]) != T or bool((offs[1:] < offs[:-1]).any()):
+            raise ValueError("cu_seqlens must start at 0, be non-decreasing and end at T")
+    return cu_seqlens.detach().to(device=dev, dtype=torch.int32).contiguous()
 
 
 def _no_grad(name, *xs):
@@ -97,30 +153,37 @@ def paged_attn_decode(
     softcap: Optional[float] = None,
     slopes: Optional[torch.Tensor] = None,
     head_first: bool = True,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention of one new token per sequence: q ``[N,HQ,1,K]`` (``[N,1,HQ,K]`` with ``head_first=False``) over the ``lens[n]`` tokens
     of the cache and, where its own k and v are given (shaped like q with HKV heads), itself; these are written into the cache at position
     ``lens[n]`` by the same launch (``lens`` itself is the caller's to advance).  Returns o ``[N,HQ,1,V]`` / ``[N,1,HQ,V]``.
 
     scale, softcap, slopes as in ``softmax_attn``; distances count to the new token (the last in the cache where k is not given).  A
-    sequence with nothing to attend to gives zeros.  A position beyond the table is attended to but not kept."""
+    sequence with nothing to attend to gives zeros.  A position beyond the table is attended to but not kept.
+
+    k_scales, v_scales: the cache is in 4 bits (above); q, k, v and o are bfloat16 or float32 all the same."""
     name = "paged_attn_decode"
     _no_grad(name, q, k, v, k_pages, v_pages, slopes)
-    r = native_call("paged_decode", name, k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first)
-    if r is not None:
-        return r[0]
+    scales = _both_scales(k_scales, v_scales, name)
+    if k_scales is None:
+        r = native_call("paged_decode", name, k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first)
+        if r is not None:
+            return r[0]
     if (k is None) != (v is None):
         raise ValueError(f"{name}: k and v go together")
-    a, held = _pages(k_pages, v_pages, page_table, lens, name)
+    a, held = _pages(k_pages, v_pages, page_table, lens, name, scales, q.dtype)
     if q.dim() != 4:
         raise ValueError(f"{name}: q must be 4-dimensional")
     HQ = q.shape[1 if head_first else 2]
     if HQ < 1 or HQ % a.HKV:
         raise ValueError(f"{name}: {HQ} query heads are no multiple of {a.HKV} key heads")
-    q = _tokens(q, a.N, 1, HQ, a.K, head_first, k_pages, f"{name}: q")
+    dt = None if k_scales is None else q.dtype
+    q = _tokens(q, a.N, 1, HQ, a.K, head_first, k_pages, f"{name}: q", dt)
     a.HQ, a.q = HQ, _desc(q, head_first)
     if k is not None:
-        k, v = (_tokens(x, a.N, 1, a.HKV, d, head_first, k_pages, f"{name}: {s}") for x, d, s in ((k, a.K, "k"), (v, a.V, "v")))
+        k, v = (_tokens(x, a.N, 1, a.HKV, d, head_first, k_pages, f"{name}: {s}", dt) for x, d, s in ((k, a.K, "k"), (v, a.V, "v")))
         a.kn, a.vn = _desc(k, head_first), _desc(v, head_first)
     a.scale, a.softcap = float(a.K ** -0.5 if scale is None else scale), cap_of(softcap, name)
     slopes = slopes_of(slopes, HQ, q.device, name)
@@ -129,14 +192,12 @@ def paged_attn_decode(
     a.o = _desc(o, head_first)
     if a.N == 0:
         return o
-    lib = _lib.load()
-    floats = lib.lmoe_paged_attn_floats(C.byref(a))
-    _lib.check(min(floats, 0), name)
+    floats = _call("attn_floats", a, scales, name, st=False)
     ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     a.ws = ptr(ws)
-    _lib.check(lib.lmoe_paged_attn_decode(C.byref(a), stream_ptr()), name)
+    _call("attn_decode", a, scales, name)
     if k is not None:
-        _written(k_pages, v_pages)
+        _written(k_pages, v_pages, *(x for x in scales if x is not None))
     return o
 
 
@@ -149,34 +210,63 @@ def paged_kv_append(
     lens: torch.Tensor,
     cu_seqlens: Optional[torch.Tensor] = None,
     head_first: bool = True,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
 ) -> None:
     """Writes k ``[N,HKV,T,K]`` and v ``[N,HKV,T,V]`` (``[N,T,H,*]`` with ``head_first=False``; packed ``[1,T,H,*]`` with ``cu_seqlens``) into
     the cache: token t of sequence n goes to position ``lens[n] + t``.  ``lens`` itself is the caller's to advance.  Tokens behind the
-    last packed sequence, and positions that have no page, are left out."""
+    last packed sequence, and positions that have no page, are left out.  k_scales, v_scales: the cache is in 4 bits (above)."""
     name = "paged_kv_append"
     _no_grad(name, k, v, k_pages, v_pages)
-    if native_call("paged_append", name, k_pages, v_pages, page_table, lens, k, v, cu_seqlens, head_first) is not None:
+    scales = _both_scales(k_scales, v_scales, name)
+    if k_scales is None and native_call("paged_append", name, k_pages, v_pages, page_table, lens, k, v, cu_seqlens, head_first) is not None:
         return
-    a, held = _pages(k_pages, v_pages, page_table, lens, name)
+    a, held = _pages(k_pages, v_pages, page_table, lens, name, scales, k.dtype)
     if k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"{name}: k and v must be 4-dimensional")
-    cu = None
-    if cu_seqlens is not None:
-        if head_first:
-            raise ValueError("cu_seqlens requires head_first=False ([1, T, H, D] packed input)")
-        if k.shape[0] != 1:
-            raise ValueError(f"cu_seqlens requires batch size 1 (packed input), got B={k.shape[0]}")
-        if cu_seqlens.dim() != 1 or cu_seqlens.numel() != a.N + 1:
-            raise ValueError(f"{name}: cu_seqlens must hold {a.N + 1} offsets for the {a.N} rows of page_table, got {tuple(cu_seqlens.shape)}")
-        if not cu_seqlens.is_cuda:
-            offs = cu_seqlens.detach().to(torch.int64)
-            if int(offs[0]) != 0 or int(offs[-1]) != k.shape[1] or bool((offs[1:] < offs[:-1]).any()):
-                raise ValueError("cu_seqlens must start at 0, be non-decreasing and end at T")
-        cu = cu_seqlens.detach().to(device=k_pages.device, dtype=torch.int32).contiguous()
-        a.cu_seqlens = cu.data_ptr()
-    B, T = (1 if cu is not None else a.N), k.shape[2 if head_first else 1]
-    k, v = (_tokens(x, B, T, a.HKV, d, head_first, k_pages, f"{name}: {s}") for x, d, s in ((k, a.K, "k"), (v, a.V, "v")))
+    dt, T = None if k_scales is None else k.dtype, k.shape[2 if head_first else 1]
+    cu = None if cu_seqlens is None else _packed(cu_seqlens, head_first, k.shape[0], T, a, k_pages.device, name)
+    a.cu_seqlens, B = ptr(cu), a.N if cu is None else 1
+    k, v = (_tokens(x, B, T, a.HKV, d, head_first, k_pages, f"{name}: {s}", dt) for x, d, s in ((k, a.K, "k"), (v, a.V, "v")))
     a.B, a.T, a.kn, a.vn = B, T, _desc(k, head_first), _desc(v, head_first)
     if k.numel() and a.N:
-        _lib.check(_lib.load().lmoe_paged_kv_append(C.byref(a), stream_ptr()), name)
-        _written(k_pages, v_pages)
+        _call("kv_append", a, scales, name)
+        _written(k_pages, v_pages, *(x for x in scales if x is not None))
+
+
+def paged_kv_read(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    starts: torch.Tensor,
+    T: int,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    head_first: bool = True,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
+    dtype: Optional[torch.dtype] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The way back: k ``[N,HKV,T,K]`` and v ``[N,HKV,T,V]`` (``[N,T,H,*]`` with ``head_first=False``; packed ``[1,T,H,*]`` with ``cu_seqlens``,
+    sequence n having ``cu_seqlens[n + 1] - cu_seqlens[n]`` tokens) as the cache holds them from position ``starts[n]`` on: what
+    ``softmax_attn`` takes to see a prompt as the tokens behind it will, or what moves to another machine.  Positions that have no page,
+    and rows behind the last packed sequence, are zero.  dtype: of k and v, where the cache is in 4 bits (``None``: bfloat16)."""
+    name = "paged_kv_read"
+    _no_grad(name, k_pages, v_pages)
+    scales = _both_scales(k_scales, v_scales, name)
+    if k_scales is None:
+        if dtype is not None and dtype != k_pages.dtype:
+            raise ValueError(f"{name}: the pages are {k_pages.dtype}, not {dtype}")
+        dtype = k_pages.dtype
+    dtype, T = dtype or torch.bfloat16, int(T)
+    a, held = _pages(k_pages, v_pages, page_table, starts, name, scales, dtype)
+    if not 0 <= T < 2 ** 31:
+        raise ValueError(f"{name}: T={T}")
+    cu = None if cu_seqlens is None else _packed(cu_seqlens, head_first, 1, T, a, k_pages.device, name)
+    a.cu_seqlens, B = ptr(cu), a.N if cu is None else 1
+    k, v = (torch.empty((B, a.HKV, T, d) if head_first else (B, T, a.HKV, d), dtype=dtype, device=k_pages.device) for d in (a.K, a.V))
+    a.B, a.T, a.kn, a.vn = B, T, _desc(k, head_first), _desc(v, head_first)
+    if k.numel():
+        if a.N == 0:
+            return k.zero_(), v.zero_()
+        _call("kv_read", a, scales, name)
+    return k, v

@@ -1,0 +1,176 @@
+"""The pages of a cache on MI355X: given out to sequences, shared between them, copied when a shared one is written, moved together
+and taken back -- around ``paged_kv_append`` and ``paged_attn_decode`` (``paged_kv.py``), whose ``page_table`` and ``lens`` they keep.
+
+    refs = torch.zeros(P, dtype=torch.int32, device="cuda")                   # how many entries of page_table name each page
+    fits = paged_reserve((k_pages, v_pages), page_table, lens, refs, 1)       # a place for the next token of every sequence
+    ...
+    paged_fork(page_table, lens, refs, src, dst)                              # sequence dst[i] goes on from what src[i] holds
+    paged_free(page_table, lens, refs, rows)                                  # sequences that ended
+    live, moved = paged_compact((k_pages, v_pages), page_table, refs)         # the used pages are 0 .. live - 1
+
+``page_table`` ``[N, M]``, ``lens`` ``[N]`` and ``refs`` ``[P]`` are int32 on the device and changed in place.  An entry outside 0 .. P - 1 names no
+page (-1 where these functions write one).  A page with ``refs`` 0 is free; a program that keeps a page by itself (a prompt that many will
+begin with) adds 1 for its own hold.  The pages' tensors are ``[P, S, ...]`` in any number and type: keys, values and scales, of all layers that share
+a table.  Nothing is read by the host, so the calls capture into a HIP graph; every result is the same whatever order the card
+takes.  (The reference's generation keeps dense caches, ``linear_moe/generation``.)
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+from ._host import ptr, stream_ptr
+from .paged_kv import _no_grad, _written
+from .softmax_attn import ints_of, on_current_device, to_int32
+
+
+def _state(page_table, refs, name, lens=None):
+    """The block of a call on a table and its counts, which are changed in place."""
+    on_current_device(page_table.device, name)
+    dev = page_table.device
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1) \
+            or (page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]):
+        raise ValueError(f"{name}: page_table must be [N, M] int32 with adjacent columns (it is changed in place), got {tuple(page_table.shape)} of "
+                         f"{page_table.dtype} with strides {page_table.stride()}")
+    for x, n, count in ((refs, "refs", None), (lens, "lens", page_table.shape[0])):
+        if x is None:
+            continue
+        if x.dim() != 1 or x.dtype != torch.int32 or x.device != dev or not x.is_contiguous() or (count is not None and x.numel() != count):
+            raise ValueError(f"{name}: {n} must be contiguous int32 on {dev}{'' if count is None else f' of {count} numbers'} (it is changed in place), got "
+                             f"{tuple(x.shape)} of {x.dtype} on {x.device}")
+    a = _lib.PagesArgs()
+    a.N, a.M, a.P = *page_table.shape, refs.numel()
+    a.table_stride = max(page_table.stride(0), a.M)
+    a.table, a.lens, a.refs = page_table.data_ptr(), ptr(lens), refs.data_ptr()
+    return a
+
+
+def _bufs(pages, a, dev, name):
+    """The tensors of the pages: runs of adjacent bytes, one or two steps apart."""
+    pages = (pages,) if isinstance(pages, torch.Tensor) else tuple(pages)
+    bufs, S = (_lib.PageBuf * max(len(pages), 1))(), None
+    for buf, x in zip(bufs, pages):
+        if x.dim() < 2 or x.shape[0] != a.P or x.device != dev or x.shape[1] != (S or x.shape[1]) or x.shape[1] < 1:
+            raise ValueError(f"{name}: the pages must be [P, S, ...] on {dev} with the {a.P} pages of refs and one S, got {tuple(x.shape)} on {x.device}")
+        if x.layout != torch.strided or x.is_conj() or x.is_neg():
+            raise ValueError(f"{name}: the pages must be plain strided tensors")
+        S, size = x.shape[1], x.element_size()
+        dims = sorted(((x.stride(i) * size, x.shape[i], i == 0) for i in range(x.dim()) if x.shape[i] != 1), reverse=True)
+        span, runs = size, [(size, 1)]                      # bytes of what lies further in; [step, count] from the innermost out
+        for step, count, is_page in reversed(dims):
+            if step < span and count > 1 and x.numel():
+                raise ValueError(f"{name}: pages that overlap: {tuple(x.shape)} with strides {x.stride()}")
+            span = step * count
+            if is_page:
+                continue
+            if step == runs[-1][0] * runs[-1][1]:
+                runs[-1] = runs[-1][0], runs[-1][1] * count
+            else:
+                runs.append((step, count))
+        if runs[0][0] != size or len(runs) > 3:
+            raise ValueError(f"{name}: a page must be runs of adjacent numbers at one or two strides: {tuple(x.shape)} with strides {x.stride()}")
+        buf.ptr, buf.page_stride = x.data_ptr(), x.stride(0) * size if a.P > 1 else 0
+        buf.bytes = size * runs[0][1] if x.numel() else 0
+        (buf.stride1, buf.rows1), (buf.stride0, buf.rows0) = (runs[1:] + [(0, 1), (0, 1)])[:2]
+    a.n_bufs, a.bufs, a.S = len(pages), bufs, S or 1
+    return pages, bufs
+
+
+def _rows(x, name, what, dev):
+    if x.dim() != 1:
+        raise ValueError(f"{name}: {what} must be one row of whole numbers, got {tuple(x.shape)}")
+    return ints_of(x, x.numel(), dev, f"{name}: {what}")
+
+
+def paged_reserve(
+    pages: Union[torch.Tensor, Sequence[torch.Tensor]],
+    page_table: torch.Tensor,
+    lens: torch.Tensor,
+    refs: torch.Tensor,
+    tokens: Union[int, torch.Tensor],
+) -> torch.Tensor:
+    """Makes positions ``lens[n] .. lens[n] + tokens[n] - 1`` of every sequence n writable (tokens: a number for all, or ``[N]`` whole numbers on
+    the device; 0 or less: nothing), in the order of the rows: an entry that names no page gets the free page of the lowest number; one
+    whose page is shared (``refs`` above 1) too, with the contents copied (all tensors of ``pages``) and the old page given up.  Returns bool
+    ``[N]``: False where the table ends before, or the free pages do; of such a row nothing changes, nor of a later one that needs pages.
+
+    lens itself is the caller's to advance."""
+    name = "paged_reserve"
+    a = _state(page_table, refs, name, lens)
+    dev = page_table.device
+    pages, held = _bufs(pages, a, dev, name)
+    _no_grad(name, *pages)
+    if isinstance(tokens, torch.Tensor):
+        tokens = ints_of(tokens, a.N, dev, f"{name}: tokens")
+        a.tokens = tokens.data_ptr()
+    else:
+        if not 0 <= int(tokens) < 2 ** 31:
+            raise ValueError(f"{name}: {tokens} tokens")
+        a.each = int(tokens)
+    fits = torch.empty(a.N, dtype=torch.bool, device=dev)
+    lib = _lib.load()
+    ints = lib.lmoe_paged_pages_ints(C.byref(a))
+    _lib.check(min(ints, 0), name)
+    ws = torch.empty(ints, dtype=torch.int32, device=dev)
+    a.ws, a.fits = ws.data_ptr(), fits.data_ptr()
+    _lib.check(lib.lmoe_paged_reserve(C.byref(a), stream_ptr()), name)
+    _written(page_table, refs, *pages)
+    return fits
+
+
+def paged_fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Sequence ``dst[i]`` becomes what ``src[i]`` was (entries and length), for all i at once -- a row may be given away and taken in one call,
+    as a beam search does; the pages are shared from then on, and what a row of dst held before is given up.  src, dst: whole
+    numbers on the device, ``[F]``.  Of several i with one dst the last counts; an i with a row outside 0 .. N - 1 is left out."""
+    name = "paged_fork"
+    a = _state(page_table, refs, name, lens)
+    dev = page_table.device
+    src, dst = _rows(src, name, "src", dev), _rows(dst, name, "dst", dev)
+    if src.numel() != dst.numel():
+        raise ValueError(f"{name}: {src.numel()} rows in src, {dst.numel()} in dst")
+    a.F, a.src, a.rows = src.numel(), src.data_ptr(), dst.data_ptr()
+    lib = _lib.load()
+    ints = lib.lmoe_paged_fork_ints(C.byref(a))
+    _lib.check(min(ints, 0), name)
+    ws = torch.empty(max(ints, 1), dtype=torch.int32, device=dev)
+    a.ws = ws.data_ptr()
+    _lib.check(lib.lmoe_paged_fork(C.byref(a), stream_ptr()), name)
+    _written(page_table, lens, refs)
+
+
+def paged_free(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, rows: torch.Tensor) -> None:
+    """The sequences ``rows`` (``[F]`` whole numbers on the device; the same one twice is as good as once, one outside 0 .. N - 1 is left
+    out) give their pages back: entries become -1, ``lens`` 0."""
+    name = "paged_free"
+    a = _state(page_table, refs, name, lens)
+    rows = _rows(rows, name, "rows", page_table.device)
+    a.F, a.rows = rows.numel(), rows.data_ptr()
+    _lib.check(_lib.load().lmoe_paged_free(C.byref(a), stream_ptr()), name)
+    _written(page_table, lens, refs)
+
+
+def paged_compact(
+    pages: Union[torch.Tensor, Sequence[torch.Tensor]],
+    page_table: torch.Tensor,
+    refs: torch.Tensor,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Moves the used pages to the numbers 0 .. live - 1 (the k-th free number there takes the k-th used page beyond), so that the pages
+    behind can go to another use; ``page_table`` and ``refs`` follow.  Returns live ``[1]`` and moved ``[P]``, int32: where each page went (itself,
+    where it stayed), for what else a program keeps by their numbers."""
+    name = "paged_compact"
+    a = _state(page_table, refs, name)
+    dev = page_table.device
+    pages, held = _bufs(pages, a, dev, name)
+    _no_grad(name, *pages)
+    live, moved = torch.empty(1, dtype=torch.int32, device=dev), torch.empty(a.P, dtype=torch.int32, device=dev)
+    lib = _lib.load()
+    ints = lib.lmoe_paged_pages_ints(C.byref(a))
+    _lib.check(min(ints, 0), name)
+    ws = torch.empty(ints, dtype=torch.int32, device=dev)
+    a.ws, a.live, a.moved = ws.data_ptr(), live.data_ptr(), moved.data_ptr()
+    _lib.check(lib.lmoe_paged_compact(C.byref(a), stream_ptr()), name)
+    _written(page_table, refs, *pages)
+    return live, moved

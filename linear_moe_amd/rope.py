@@ -1,0 +1,218 @@
+"""Norm and rotation of queries and keys on MI355X, in one pass: what a softmax layer of a hybrid model does to q and k between its
+projection and ``softmax_attn``, and while it generates between the projection and ``paged_attn_decode``.
+
+The reference turns them by ``apply_rotary`` (``linear_moe/model/common_modules/rotary.py:40-98``), behind norms of their
+own; here the rows are read and written once, the backward pass reads them and their gradients once, and the angles come
+from a table of positions, so that neither a position nor an offset is read by the host.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._host import _DT, _desc, has_tangent, no_node, ptr, stream_ptr
+from .softmax_attn import ints_of, on_current_device, to_int32
+
+MAX_ROPE_DIM = 256      # columns of a head
+
+
+def rope_table(positions: int, dim: int, base: float = 10000.0, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin ``[positions, dim / 2]`` in float32 of the angles ``position * base ** (-2 i / dim)``, which are formed in 64 bits (in 32, one
+    of a far position is off by as much as it turns between neighbours of a bfloat16).  Any other table (longer contexts by other
+    frequencies) is as good for ``qk_norm_rope``."""
+    if dim < 0 or dim % 2 or positions < 0:
+        raise ValueError(f"rope_table: {positions} positions of {dim} columns (an even number)")
+    freq = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / max(dim, 1))
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return angle.cos().float(), angle.sin().float()
+
+
+def _constant(x, name):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} is a constant of the model, there is no gradient for it")
+    if has_tangent(x):
+        raise RuntimeError(f"{name} is a constant of the model, there is no forward-mode derivative for it")
+    return x.detach()
+
+
+def _adjacent(x):
+    """x, or a copy of it, with adjacent columns."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+class _Call:
+    """What forward and backward of a call share: its tables and options."""
+
+    def __init__(self, dims, head_first, cos, sin, R, positions, offsets, cu, N, eps, norm, interleaved):
+        self.dims, self.head_first, self.R, self.N, self.eps, self.norm, self.interleaved = dims, head_first, R, N, eps, norm, interleaved
+        self.tables = cos, sin, positions, offsets, cu
+
+    def block(self, q, k, qw, kw, tables):
+        B, T, HQ, HKV, D = self.dims
+        cos, sin, positions, offsets, cu = tables
+        a = _lib.RopeArgs()
+        a.dtype = _DT[q.dtype]
+        a.w_dtype = next((_DT[w.dtype] for w in (qw, kw) if w is not None), a.dtype)
+        a.B, a.T, a.HQ, a.HKV, a.D, a.R, a.N, a.L = B, T, HQ, HKV, D, self.R, self.N, 0 if cos is None else cos.shape[0]
+        a.norm, a.interleaved, a.eps = int(self.norm), int(self.interleaved), self.eps
+        a.cu_seqlens, a.offsets, a.positions, a.cos, a.sin, a.qw, a.kw = (ptr(x) for x in (cu, offsets, positions, cos, sin, qw, kw))
+        if positions is not None:
+            a.pos_stride = positions.stride(0) if positions.dim() == 2 else 0
+        a.q, a.k = _desc(q, self.head_first), _desc(k, self.head_first)
+        return a
+
+    def forward(self, q, k, qw, kw):
+        q, k = _adjacent(q.detach()), _adjacent(k.detach())
+        zq, zk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+        if q.numel():
+            a = self.block(q, k, qw, kw, self.tables)
+            a.zq, a.zk = _desc(zq, self.head_first), _desc(zk, self.head_first)
+            _lib.check(_lib.load().lmoe_qk_norm_rope_fwd(C.byref(a), stream_ptr()), "qk_norm_rope")
+        return q, k, zq, zk
+
+
+def _back(x, shape, dtype, device, name):
+    """A tensor that was saved for the backward, as the kernels may read it (a saved-tensor hook hands back what it likes)."""
+    if x is None or tuple(x.shape) != tuple(shape) or x.device != device:
+        raise RuntimeError(f"{name}, saved for the backward with shape {tuple(shape)} on {device}, came back as "
+                           f"{None if x is None else (tuple(x.shape), str(x.device))}")
+    x = x.to(dtype)
+    return _adjacent(x) if x.dim() == 4 else x.contiguous()
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, call):
+        ws = [None if w is None else w.detach().contiguous() for w in (qw, kw)]
+        q_, k_, zq, zk = call.forward(q, k, *ws)
+        ctx.call = call
+        saved = (q_, k_, *ws, *call.tables)
+        ctx.save_for_backward(*saved)
+        ctx.like = [None if x is None else (tuple(x.shape), x.dtype) for x in saved]
+        return zq, zk
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dzq, dzk):
+        call, dev = ctx.call, dzq.device
+        names = "q k q_weight k_weight cos sin positions offsets cu_seqlens".split()
+        q, k, qw, kw, *tables = (None if like is None else _back(x, *like, dev, n) for x, like, n in zip(ctx.saved_tensors, ctx.like, names))
+        dzq, dzk = _back(dzq, q.shape, q.dtype, dev, "the gradient of q"), _back(dzk, k.shape, k.dtype, dev, "the gradient of k")
+        dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
+        dqw, dkw = (torch.empty_like(w) if w is not None and ctx.needs_input_grad[i] else None for i, w in ((2, qw), (3, kw)))
+        if q.numel():
+            a = call.block(q, k, qw, kw, tables)
+            a.dzq, a.dzk, a.dq, a.dk = (_desc(x, call.head_first) for x in (dzq, dzk, dq, dk))
+            a.dqw, a.dkw = ptr(dqw), ptr(dkw)
+            lib = _lib.load()
+            floats = lib.lmoe_qk_norm_rope_floats(C.byref(a))
+            _lib.check(min(floats, 0), "qk_norm_rope backward")
+            ws = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+            a.ws = ptr(ws)
+            _lib.check(lib.lmoe_qk_norm_rope_bwd(C.byref(a), stream_ptr()), "qk_norm_rope backward")
+        else:
+            for w in (dqw, dkw):
+                if w is not None:
+                    w.zero_()
+        return dq, dk, dqw, dkw, None
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    cos: Optional[torch.Tensor] = None,
+    sin: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    offsets: Optional[torch.Tensor] = None,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    norm: bool = True,
+    interleaved: bool = False,
+    head_first: bool = True,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``y = x / sqrt(mean(x^2) + eps) * weight`` per head of q and k, then the first R columns turned by their token's angles:
+    ``z_a = y_a cos - y_b sin``, ``z_b = y_b cos + y_a sin`` for the pairs (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.  Rounded once, at the end.
+
+    q ``[B,HQ,T,D]``, k ``[B,HKV,T,D]`` (``[B,T,H,D]`` with ``head_first=False``), bfloat16 or float32, any strides (views of one projection are
+    read in place); any numbers of heads; D even, up to 256.  Returns both, laid out like q and k, contiguous.
+
+    q_weight, k_weight: ``[D]``, bfloat16 or float32, or none; ``norm=False``: rotation alone.
+    cos, sin: ``[L, R/2]`` (``rope_table``; float32, others are converted), not trained; none: norm alone.  A token's row is its position inside its
+    sequence, and so many more as ``offsets`` (``[N]`` whole numbers on the device: what the cache holds already) says; or what ``positions``
+    (``[T]`` or ``[B,T]`` whole numbers on the device) says.  A position outside the table is not turned.
+    cu_seqlens: packed documents as in the chunk ops; rows behind the last one are zero in the results and the gradients.
+    Backward: gradients of q, k and the weights, these summed over all rows in fp32 in a fixed order, without atomics.
+    Forward and backward capture into a HIP graph; capture with leaves of which no graph of an eager step lives any more (torch's
+    accumulation nodes belong to the stream of their first use)."""
+    name = "qk_norm_rope"
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"{name}: q and k must be 4-dimensional")
+    on_current_device(q.device, name)
+    dev = q.device
+    if k.device != dev:
+        raise RuntimeError(f"{name}: q and k must live on one device, got {dev}, {k.device}")
+    if q.dtype not in _DT or k.dtype != q.dtype:
+        raise ValueError(f"{name}: q and k must share dtype bfloat16 or float32, got {q.dtype}, {k.dtype}")
+    h, t = (1, 2) if head_first else (2, 1)
+    B, T, HQ, D = q.shape[0], q.shape[t], q.shape[h], q.shape[3]
+    HKV = k.shape[h]
+    if (k.shape[0], k.shape[t], k.shape[3]) != (B, T, D) or HQ < 1 or HKV < 1:
+        raise ValueError(f"{name}: shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if not 0 < D <= MAX_ROPE_DIM or D % 2:
+        raise ValueError(f"{name}: head dimension D={D} unsupported (even, at most {MAX_ROPE_DIM})")
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if weights and not norm:
+        raise ValueError(f"{name}: weights belong to the norm")
+    for w in weights:
+        if tuple(w.shape) != (D,) or w.device != dev or w.dtype not in _DT or w.dtype != weights[0].dtype:
+            raise ValueError(f"{name}: weights must be ({D},) on {dev}, both bfloat16 or both float32, got {tuple(w.shape)} {w.dtype} on {w.device}")
+    if not 0.0 <= float(eps) < float("inf"):
+        raise ValueError(f"{name}: eps must not be negative, got {eps}")
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{name}: cos and sin go together")
+    if cos is None and not norm:
+        raise ValueError(f"{name}: neither norm nor rotation")
+    R = 0
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.device != dev or sin.device != dev or not (cos.is_floating_point() and sin.is_floating_point()):
+            raise ValueError(f"{name}: cos and sin must be [positions, R / 2] on {dev}, got {tuple(cos.shape)} on {cos.device}, {tuple(sin.shape)} on {sin.device}")
+        R = 2 * cos.shape[1]
+        if R > D or cos.shape[0] >= 2 ** 31:
+            raise ValueError(f"{name}: a table of {tuple(cos.shape)} for heads of {D} columns")
+        cos, sin = (_constant(x, f"{name}: {n}").to(torch.float32).contiguous() for x, n in ((cos, "cos"), (sin, "sin")))
+    if positions is not None:
+        if offsets is not None or cu_seqlens is not None:
+            raise ValueError(f"{name}: positions exclude offsets and cu_seqlens")
+        if tuple(positions.shape) not in ((T,), (B, T)) or positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool \
+                or positions.device != dev:
+            raise ValueError(f"{name}: positions must be [T] or [B, T] whole numbers on {dev}, got {tuple(positions.shape)} of {positions.dtype} on "
+                             f"{positions.device}")
+        positions = to_int32(positions.detach())
+        if T > 1 and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+    N, cu = B, None
+    if cu_seqlens is not None:
+        if head_first:
+            raise ValueError("cu_seqlens requires head_first=False ([1, T, H, D] packed input)")
+        if B != 1:
+            raise ValueError(f"cu_seqlens requires batch size 1 (packed input), got B={B}")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise ValueError("cu_seqlens must be a 1-D tensor of N+1 offsets")
+        if not cu_seqlens.is_cuda:
+            offs = cu_seqlens.detach().to(torch.int64)
+            if int(offs[0]) != 0 or int(offs[-1]) != T or bool((offs[1:] < offs[:-1]).any()):
+                raise ValueError("cu_seqlens must start at 0, be non-decreasing and end at T")
+        cu = cu_seqlens.detach().to(device=dev, dtype=torch.int32).contiguous()
+        N = cu.numel() - 1
+    if offsets is not None:
+        offsets = ints_of(offsets, N, dev, f"{name}: offsets")
+    call = _Call((B, T, HQ, HKV, D), head_first, cos, sin, R, positions, offsets, cu, N, float(eps), bool(norm), bool(interleaved))
+    if no_node(q, k, *weights):
+        return call.forward(q, k, *(None if w is None else w.detach().contiguous() for w in (q_weight, k_weight)))[2:]
+    return _QkNormRope.apply(q, k, q_weight, k_weight, call)
