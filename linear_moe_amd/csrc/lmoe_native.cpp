@@ -10,10 +10,13 @@
 #include <Python.h>
 #include <dlfcn.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
+#include <utility>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -58,6 +61,20 @@ struct Library {
   decltype(&lmoe_paged_attn_floats) paged_floats;
   decltype(&lmoe_paged_attn_decode) paged_decode;
   decltype(&lmoe_paged_kv_append) paged_append;
+  decltype(&lmoe_paged_kv_read) paged_read;
+  decltype(&lmoe_paged4_attn_floats) paged4_floats;
+  decltype(&lmoe_paged4_attn_decode) paged4_decode;
+  decltype(&lmoe_paged4_kv_append) paged4_append;
+  decltype(&lmoe_paged4_kv_read) paged4_read;
+  decltype(&lmoe_paged_fork_ints) fork_ints;
+  decltype(&lmoe_paged_pages_ints) pages_ints;
+  decltype(&lmoe_paged_free) pages_free;
+  decltype(&lmoe_paged_fork) pages_fork;
+  decltype(&lmoe_paged_reserve) pages_reserve;
+  decltype(&lmoe_paged_compact) pages_compact;
+  decltype(&lmoe_qk_norm_rope_floats) rope_floats;
+  decltype(&lmoe_qk_norm_rope_fwd) rope_fwd;
+  decltype(&lmoe_qk_norm_rope_bwd) rope_bwd;
 } lib;
 
 constexpr int OP_SIMPLE = LMOE_OP_SIMPLE_GLA, OP_GLA = LMOE_OP_GLA, OP_GDN = LMOE_OP_GATED_DELTA_RULE;
@@ -991,10 +1008,13 @@ struct Paged {
     NEED(kp.dim() == 4 && vp.dim() == 4 && dtype_of(kp) >= 0 && vp.scalar_type() == kp.scalar_type() && kp.sizes().slice(0, 3) == vp.sizes().slice(0, 3));
     const int64_t vec = 16 / kp.element_size(), K = kp.size(3), V = vp.size(3);
     NEED(kp.numel() > 0 && vp.numel() > 0 && K <= 128 && V <= 128 && K % vec == 0 && V % vec == 0 && rows_aligned(kp) && rows_aligned(vp));
+    a.dtype = dtype_of(kp);
+    return enter(K, V);
+  }
+  bool enter(int64_t K, int64_t V) {
     NEED(table.dim() == 2 && table.scalar_type() == at::kInt && table.size(1) > 0 && (table.size(1) == 1 || table.stride(1) == 1));
     NEED(ints_from(lens, table.size(0)) && table.size(0) > 0);
     for (const int64_t x : {kp.size(0), kp.size(1), kp.size(2), table.size(0), table.size(1)}) NEED(fits(x));
-    a.dtype = dtype_of(kp);
     a.N = table.size(0); a.M = table.size(1); a.P = kp.size(0); a.S = kp.size(1); a.HKV = kp.size(2); a.K = K; a.V = V;
     a.table_stride = table.stride(0); a.table = (const int32_t*)table.data_ptr(); a.lens = (const int32_t*)lens.data_ptr();
     a.kp = desc(kp, false); a.vp = desc(vp, false);
@@ -1002,7 +1022,7 @@ struct Paged {
   }
   // [B, T, H, D] (or [B, H, T, D]) as it lies
   bool tokens(Tensor& x, PyObject* o, int64_t B, int64_t T, int64_t H, int64_t D, bool hf) const {
-    NEED(plain(x, o, dev) && x.dim() == 4 && x.scalar_type() == kp.scalar_type());
+    NEED(plain(x, o, dev) && x.dim() == 4 && dtype_of(x) == a.dtype);
     return x.size(0) == B && x.size(hf ? 2 : 1) == T && x.size(hf ? 1 : 2) == H && x.size(3) == D && rows_aligned(x);
   }
 };
@@ -1061,6 +1081,460 @@ PyObject* paged_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A cache in 4 bits
+struct Paged4 : Paged {
+  lmoe_paged4_args a4 = {};
+  Tensor ks, vs;
+  // o: k_pages, v_pages, page_table, lens; scales: k_scales, v_scales; t: of the tokens
+  bool take(PyObject* const* o, PyObject* const* scales, at::ScalarType t) {
+    dev = current_device(o[0]);
+    NEED(dev >= 0 && plain(kp, o[0], dev) && plain(vp, o[1], dev) && plain(table, o[2], dev) && plain(lens, o[3], dev));
+    NEED(plain(ks, scales[0], dev) && plain(vs, scales[1], dev));
+    for (const Tensor* x : {&kp, &vp, &ks, &vs}) NEED(x->dim() == 4 && x->scalar_type() == at::kByte && x->sizes().slice(0, 3) == kp.sizes().slice(0, 3) && x->numel() > 0);
+    const int64_t K = 2 * kp.size(3), V = 2 * vp.size(3);
+    NEED(K <= 128 && V <= 128 && K % 32 == 0 && V % 32 == 0 && rows_aligned(kp) && rows_aligned(vp));
+    for (const auto& [x, d] : {std::pair(&ks, K / 32), std::pair(&vs, V / 32)}) NEED(x->size(3) == d && (d == 1 || x->stride(3) == 1));
+    NEED(t == at::kBFloat16 || t == at::kFloat);
+    a.dtype = t == at::kFloat ? LMOE_F32 : LMOE_BF16;
+    return enter(K, V);
+  }
+  const lmoe_paged4_args* block() {
+    a4.p = a; a4.ks = desc(ks, false); a4.vs = desc(vs, false);
+    return &a4;
+  }
+  void written() const {
+    for (const Tensor* x : {&kp, &vp, &ks, &vs}) if (!x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+  }
+};
+bool type_of(at::ScalarType& t, PyObject* o) {
+  NEED(THPVariable_CheckExact(o));
+  t = THPVariable_Unpack(o).scalar_type();
+  return true;
+}
+
+// paged4_decode(k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first, k_scales, v_scales, stream) -> (o,)
+PyObject* paged4_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged4 c;
+  Tensor q, k, v, slopes;
+  at::ScalarType t;
+  if (n != 14 || !type_of(t, o[4]) || !c.take(o, o + 11, t)) return elsewhere();
+  const bool hf = yes(o[10]);
+  void* st = stream_of(o[13]);
+  if (PyErr_Occurred() || !plain(q, o[4], c.dev) || q.dim() != 4) return elsewhere();
+  const int64_t HQ = q.size(hf ? 1 : 2);
+  if (HQ < 1 || !fits(HQ) || HQ % c.a.HKV || !c.tokens(q, o[4], c.a.N, 1, HQ, c.a.K, hf) || (o[5] == Py_None) != (o[6] == Py_None)) return elsewhere();
+  if (o[5] != Py_None && !(c.tokens(k, o[5], c.a.N, 1, c.a.HKV, c.a.K, hf) && c.tokens(v, o[6], c.a.N, 1, c.a.HKV, c.a.V, hf))) return elsewhere();
+  c.a.HQ = HQ;
+  if (!number(c.a.scale, o[7], (float)std::pow((double)c.a.K, -0.5)) || !cap_from(c.a.softcap, o[8]) ||
+      !slopes_from(slopes, o[9], c.dev, HQ)) return elsewhere();
+  c.a.slopes = (const float*)ptr(slopes);
+  c.a.q = desc(q, hf); c.a.kn = desc(k, hf); c.a.vn = desc(v, hf);
+  const int64_t floats = lib.paged4_floats(c.block());
+  if (floats < 0) return PyLong_FromLong((long)floats);
+  Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const auto s = q.sizes();
+    out = at::empty({s[0], s[1], s[2], c.a.V}, q.options().requires_grad(false));
+    Tensor ws;
+    if (floats) ws = at::empty({floats}, q.options().dtype(at::kFloat).requires_grad(false));
+    c.a.o = desc(out, hf); c.a.ws = (float*)ptr(ws);
+    rc = lib.paged4_decode(c.block(), st);
+  }
+  if (rc == 0 && k.defined()) c.written();
+  return result(rc, {out});
+  END_HANDLE_TH_ERRORS
+}
+
+// paged4_append(k_pages, v_pages, page_table, lens, k, v, cu_seqlens or None, head_first, k_scales, v_scales, stream) -> ()
+PyObject* paged4_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged4 c;
+  Tensor k, v, cu;
+  at::ScalarType t;
+  if (n != 11 || !type_of(t, o[4]) || !c.take(o, o + 8, t)) return elsewhere();
+  const bool hf = yes(o[7]);
+  void* st = stream_of(o[10]);
+  if (PyErr_Occurred() || !plain(k, o[4], c.dev) || k.dim() != 4 || !plain_or_none(cu, o[6], c.dev)) return elsewhere();
+  const int64_t B = cu.defined() ? 1 : c.a.N, T = k.size(hf ? 2 : 1);
+  if (T < 1 || !fits(T) || !c.tokens(k, o[4], B, T, c.a.HKV, c.a.K, hf) || !c.tokens(v, o[5], B, T, c.a.HKV, c.a.V, hf)) return elsewhere();
+  if (cu.defined() && (hf || !ints_from(cu, (int64_t)c.a.N + 1))) return elsewhere();
+  c.a.B = B; c.a.T = T; c.a.kn = desc(k, hf); c.a.vn = desc(v, hf); c.a.cu_seqlens = (const int32_t*)ptr(cu);
+  const int rc = lib.paged4_append(c.block(), st);
+  if (rc == 0) c.written();
+  return result(rc, {});
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_read(k_pages, v_pages, page_table, starts, T, cu_seqlens or None, head_first, k_scales, v_scales, whether float32 (in 4 bits), stream) -> (k, v)
+PyObject* paged_read(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Paged4 c;
+  Tensor cu;
+  if (n != 11) return elsewhere();
+  const bool bits4 = o[7] != Py_None, hf = yes(o[6]);
+  if (!(bits4 ? c.take(o, o + 7, yes(o[9]) ? at::kFloat : at::kBFloat16) : c.Paged::take(o))) return elsewhere();
+  const int64_t T = PyLong_AsLongLong(o[4]);
+  void* st = stream_of(o[10]);
+  if (PyErr_Occurred() || T < 1 || !fits(T) || !plain_or_none(cu, o[5], c.dev)) return elsewhere();
+  if (cu.defined() && (hf || !ints_from(cu, (int64_t)c.a.N + 1))) return elsewhere();
+  const int64_t B = cu.defined() ? 1 : c.a.N, H = c.a.HKV;
+  Tensor k, v;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const auto opt = c.kp.options().dtype(c.a.dtype == LMOE_F32 ? at::kFloat : at::kBFloat16).requires_grad(false);
+    auto rows = [&](int64_t d) { return hf ? at::empty({B, H, T, d}, opt) : at::empty({B, T, H, d}, opt); };
+    k = rows(c.a.K); v = rows(c.a.V);
+    c.a.B = B; c.a.T = T; c.a.kn = desc(k, hf); c.a.vn = desc(v, hf); c.a.cu_seqlens = (const int32_t*)ptr(cu);
+    rc = bits4 ? lib.paged4_read(c.block(), st) : lib.paged_read(&c.a, st);
+  }
+  return result(rc, {k, v});
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- the pages of a cache ----
+struct Pages {
+  int dev;
+  lmoe_pages_args a = {};
+  Tensor table, lens, refs;
+  std::vector<Tensor> pages;
+  std::vector<lmoe_page_buf> bufs;
+  // lens_o: null where the call has none
+  bool take(PyObject* table_o, PyObject* lens_o, PyObject* refs_o) {
+    dev = current_device(table_o);
+    NEED(dev >= 0 && plain(table, table_o, dev) && plain(refs, refs_o, dev) && (!lens_o || plain(lens, lens_o, dev)));
+    NEED(table.dim() == 2 && table.scalar_type() == at::kInt && table.numel() > 0 && (table.size(1) == 1 || table.stride(1) == 1));
+    const int64_t N = table.size(0), M = table.size(1);
+    NEED((N == 1 || table.stride(0) >= M) && ints_from(refs, refs.numel()) && refs.numel() > 0 && (!lens_o || ints_from(lens, N)));
+    for (const int64_t x : {N, M, refs.numel()}) NEED(fits(x));
+    a.N = N; a.M = M; a.P = refs.numel(); a.S = 1;
+    a.table_stride = std::max(table.stride(0), M);
+    a.table = (int32_t*)table.data_ptr(); a.lens = (int32_t*)ptr(lens); a.refs = (int32_t*)refs.data_ptr();
+    return true;
+  }
+  // the tensors of the pages: as paged_pages.py takes them apart
+  bool take_pages(PyObject* o) {
+    const bool one = THPVariable_CheckExact(o);
+    NEED(one || PyTuple_CheckExact(o) || PyList_CheckExact(o));
+    const Py_ssize_t count = one ? 1 : PySequence_Fast_GET_SIZE(o);
+    pages.resize(count); bufs.resize(count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      Tensor& x = pages[i];
+      NEED(plain(x, one ? o : PySequence_Fast_GET_ITEM(o, i), dev) && !x.requires_grad() && !x.is_conj() && !x.is_neg());
+      NEED(x.dim() >= 2 && x.dim() <= 8 && x.size(0) == a.P && x.numel() > 0 && (i == 0 || x.size(1) == a.S) && fits(x.size(1)));
+      a.S = x.size(1);
+      struct Dim { int64_t step, count; bool page; } dims[8];
+      const int64_t size = x.element_size();
+      int n = 0;
+      for (int64_t d = 0; d < x.dim(); ++d) if (x.size(d) != 1) dims[n++] = {x.stride(d) * size, x.size(d), d == 0};
+      std::sort(dims, dims + n, [](const Dim& u, const Dim& v) { return u.step < v.step; });
+      Dim runs[3] = {{size, 1, false}, {0, 1, false}, {0, 1, false}};
+      int k = 0;
+      int64_t span = size;
+      for (int d = 0; d < n; ++d) {
+        NEED(dims[d].step >= span);
+        span = dims[d].step * dims[d].count;
+        if (dims[d].page) continue;
+        if (dims[d].step == runs[k].step * runs[k].count) runs[k].count *= dims[d].count;
+        else {
+          NEED(++k < 3);
+          runs[k] = dims[d];
+        }
+      }
+      NEED(fits(runs[1].count) && fits(runs[2].count));
+      bufs[i] = lmoe_page_buf{x.data_ptr(), a.P > 1 ? x.stride(0) * size : 0, runs[2].step, runs[1].step, size * runs[0].count, (int32_t)runs[2].count, (int32_t)runs[1].count};
+    }
+    a.n_bufs = (int32_t)count; a.bufs = bufs.data();
+    return true;
+  }
+  bool rows(Tensor& x, PyObject* o) const { return plain(x, o, dev) && x.numel() > 0 && ints_from(x, x.numel()) && fits(x.numel()); }
+  Tensor ints(int64_t n) const { return at::empty({n}, table.options()); }
+  void written() const {
+    auto bump = [](const Tensor& x) { if (x.defined() && !x.is_inference()) x.unsafeGetTensorImpl()->bump_version(); };
+    bump(table); bump(lens); bump(refs);
+    for (const Tensor& x : pages) bump(x);
+  }
+};
+
+// pages_free(page_table, lens, refs, rows, stream) -> ()
+PyObject* pages_free(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  Tensor rows;
+  if (n != 5 || !c.take(o[0], o[1], o[2]) || !c.rows(rows, o[3])) return elsewhere();
+  void* st = stream_of(o[4]);
+  if (PyErr_Occurred()) return elsewhere();
+  c.a.F = rows.numel(); c.a.rows = (const int32_t*)rows.data_ptr();
+  const int rc = lib.pages_free(&c.a, st);
+  if (rc == 0) c.written();
+  return result(rc, {});
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_fork(page_table, lens, refs, src, dst, stream) -> ()
+PyObject* pages_fork(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  Tensor src, dst;
+  if (n != 6 || !c.take(o[0], o[1], o[2]) || !c.rows(src, o[3]) || !c.rows(dst, o[4]) || src.numel() != dst.numel()) return elsewhere();
+  void* st = stream_of(o[5]);
+  if (PyErr_Occurred()) return elsewhere();
+  c.a.F = src.numel(); c.a.src = (const int32_t*)src.data_ptr(); c.a.rows = (const int32_t*)dst.data_ptr();
+  const int64_t ints = lib.fork_ints(&c.a);
+  if (ints < 0) return PyLong_FromLong((long)ints);
+  int rc;
+  {
+    const Unlocked unlocked;
+    const Tensor ws = c.ints(ints);
+    c.a.ws = (int32_t*)ws.data_ptr();
+    rc = lib.pages_fork(&c.a, st);
+  }
+  if (rc == 0) c.written();
+  return result(rc, {});
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_reserve(page_table, lens, refs, pages, tokens, stream) -> (fits,)
+PyObject* pages_reserve(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  Tensor tokens;
+  if (n != 6 || !c.take(o[0], o[1], o[2]) || !c.take_pages(o[3])) return elsewhere();
+  if (PyLong_CheckExact(o[4])) {
+    const int64_t each = PyLong_AsLongLong(o[4]);
+    if (PyErr_Occurred() || !fits(each)) return elsewhere();
+    c.a.each = each;
+  } else {
+    if (!plain(tokens, o[4], c.dev) || !ints_from(tokens, c.a.N)) return elsewhere();
+    c.a.tokens = (const int32_t*)tokens.data_ptr();
+  }
+  void* st = stream_of(o[5]);
+  if (PyErr_Occurred()) return elsewhere();
+  const int64_t ints = lib.pages_ints(&c.a);
+  if (ints < 0) return PyLong_FromLong((long)ints);
+  Tensor out;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const Tensor ws = c.ints(ints);
+    out = at::empty({c.a.N}, c.table.options().dtype(at::kBool));
+    c.a.ws = (int32_t*)ws.data_ptr(); c.a.fits = (uint8_t*)out.data_ptr();
+    rc = lib.pages_reserve(&c.a, st);
+  }
+  if (rc == 0) c.written();
+  return result(rc, {out});
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_compact(page_table, refs, pages, stream) -> (live, moved)
+PyObject* pages_compact(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Pages c;
+  if (n != 4 || !c.take(o[0], nullptr, o[1]) || !c.take_pages(o[2])) return elsewhere();
+  void* st = stream_of(o[3]);
+  if (PyErr_Occurred()) return elsewhere();
+  const int64_t ints = lib.pages_ints(&c.a);
+  if (ints < 0) return PyLong_FromLong((long)ints);
+  Tensor live, moved;
+  int rc;
+  {
+    const Unlocked unlocked;
+    const Tensor ws = c.ints(ints);
+    live = c.ints(1); moved = c.ints(c.a.P);
+    c.a.ws = (int32_t*)ws.data_ptr(); c.a.live = (int32_t*)live.data_ptr(); c.a.moved = (int32_t*)moved.data_ptr();
+    rc = lib.pages_compact(&c.a, st);
+  }
+  if (rc == 0) c.written();
+  return result(rc, {live, moved});
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- norm and rotation of queries and keys ----
+struct Rope {
+  int dev;
+  bool head_first;
+  lmoe_rope_args a = {};
+  Tensor q, k, qw, kw, tables[5];      // cos, sin, positions, offsets, cu_seqlens
+  // o: q, k, q_weight, k_weight, cos, sin, positions, offsets, cu_seqlens, eps, norm, interleaved, head_first
+  bool take(PyObject* const* o) {
+    dev = current_device(o[0]);
+    NEED(dev >= 0 && plain(q, o[0], dev) && plain(k, o[1], dev) && plain_or_none(qw, o[2], dev) && plain_or_none(kw, o[3], dev));
+    for (int i = 0; i < 5; ++i) NEED(plain_or_none(tables[i], o[4 + i], dev));
+    head_first = yes(o[12]);
+    NEED(q.dim() == 4 && k.dim() == 4 && dtype_of(q) >= 0 && k.scalar_type() == q.scalar_type() && q.numel() > 0 && k.numel() > 0);
+    const int h = head_first ? 1 : 2, t = head_first ? 2 : 1;
+    const int64_t B = q.size(0), T = q.size(t), D = q.size(3);
+    NEED(k.size(0) == B && k.size(t) == T && k.size(3) == D && D <= 256 && D % 2 == 0 && q.stride(3) == 1 && k.stride(3) == 1);
+    for (const int64_t x : {B, T, q.size(h), k.size(h)}) NEED(fits(x));
+    a.dtype = a.w_dtype = dtype_of(q);
+    a.B = B; a.T = T; a.HQ = q.size(h); a.HKV = k.size(h); a.D = D; a.N = B;
+    a.norm = yes(o[10]); a.interleaved = yes(o[11]);
+    NEED(number(a.eps, o[9], 0.f) && o[9] != Py_None && a.eps >= 0.f && a.eps < INFINITY);
+    NEED(a.norm || (!qw.defined() && !kw.defined()));
+    if (qw.defined() && kw.defined()) NEED(qw.scalar_type() == kw.scalar_type());
+    for (const Tensor* w : {&qw, &kw}) {
+      if (!w->defined()) continue;
+      NEED(dtype_of(*w) >= 0 && w->dim() == 1 && w->numel() == D && w->is_contiguous());
+      a.w_dtype = dtype_of(*w);
+    }
+    const Tensor &cos = tables[0], &sin = tables[1], &positions = tables[2], &offsets = tables[3], &cu = tables[4];
+    NEED(cos.defined() == sin.defined() && (cos.defined() || a.norm));
+    if (cos.defined()) {
+      for (const Tensor* x : {&cos, &sin}) NEED(f32(*x) && x->is_contiguous() && !x->requires_grad() && x->dim() == 2 && x->sizes() == cos.sizes() && x->numel() > 0);
+      NEED(2 * cos.size(1) <= D && fits(cos.size(0)));
+      a.R = 2 * cos.size(1); a.L = cos.size(0);
+    }
+    if (positions.defined()) {
+      NEED(!offsets.defined() && !cu.defined() && positions.scalar_type() == at::kInt && positions.is_contiguous());
+      NEED(positions.dim() == 1 ? positions.numel() == T : positions.dim() == 2 && positions.size(0) == B && positions.size(1) == T);
+      a.pos_stride = positions.dim() == 2 ? positions.stride(0) : 0;
+    }
+    if (cu.defined()) {
+      NEED(!head_first && B == 1 && cu.numel() > 1 && ints_from(cu, cu.numel()));
+      a.N = cu.numel() - 1;
+    }
+    if (offsets.defined()) NEED(ints_from(offsets, a.N));
+    a.cos = (const float*)ptr(cos); a.sin = (const float*)ptr(sin);
+    a.positions = (const int32_t*)ptr(positions); a.offsets = (const int32_t*)ptr(offsets); a.cu_seqlens = (const int32_t*)ptr(cu);
+    a.qw = ptr(qw); a.kw = ptr(kw);
+    a.q = desc(q, head_first); a.k = desc(k, head_first);
+    return true;
+  }
+  int forward(Tensor& zq, Tensor& zk, void* st) {
+    zq = at::empty(q.sizes(), q.options().requires_grad(false));
+    zk = at::empty(k.sizes(), k.options().requires_grad(false));
+    a.zq = desc(zq, head_first); a.zk = desc(zk, head_first);
+    return lib.rope_fwd(&a, st);
+  }
+};
+
+// rope_forward(q, k, q_weight, k_weight, cos, sin, positions, offsets, cu_seqlens, eps, norm, interleaved, head_first, stream) -> (q, k)
+PyObject* rope_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Rope c;
+  if (n != 14 || !c.take(o)) return elsewhere();
+  void* st = stream_of(o[13]);
+  if (PyErr_Occurred()) return elsewhere();
+  Tensor zq, zk;
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = c.forward(zq, zk, st);
+  }
+  return result(rc, {zq, zk});
+  END_HANDLE_TH_ERRORS
+}
+
+// The node of qk_norm_rope in the autograd graph, for the calls that rope_forward takes (as AttnNode is softmax_attn's).
+struct RopeNode : torch::autograd::Node {
+  using List = torch::autograd::variable_list;
+  lmoe_rope_args a;
+  bool head_first;
+  c10::Device device{c10::DeviceType::CUDA, 0};
+  enum { Q, K, QW, KW, COS, SIN, POSITIONS, OFFSETS, CU, SAVED };
+  torch::autograd::SavedVariable saved[SAVED];
+  c10::SmallVector<int64_t, 4> shapes[SAVED];
+  at::ScalarType types[SAVED];
+  bool given[SAVED] = {};
+
+  std::string name() const override { return "QkNormRopeBackward"; }
+  void save(int i, const Tensor& x) {
+    if (!x.defined()) return;
+    given[i] = true;
+    types[i] = x.scalar_type();
+    shapes[i].assign(x.sizes().begin(), x.sizes().end());
+    saved[i] = torch::autograd::SavedVariable(x, false);
+  }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    for (auto& x : saved) x.reset_data();
+  }
+  static Tensor as(const Tensor& x, at::ScalarType t) {
+    const Tensor y = x.to(t);
+    return y.dim() == 4 && y.stride(3) == 1 ? y : y.contiguous();
+  }
+  // as the kernels may read it: a saved-tensor hook hands back what it likes
+  Tensor back(int i) {
+    static const char* const names[SAVED] = {"q", "k", "q_weight", "k_weight", "cos", "sin", "positions", "offsets", "cu_seqlens"};
+    if (!given[i]) return Tensor();
+    const Tensor x = saved[i].unpack(nullptr);
+    TORCH_CHECK(x.defined() && x.sizes() == at::IntArrayRef(shapes[i]) && x.device() == device, names[i], ", saved for the backward with shape ",
+                at::IntArrayRef(shapes[i]), " on ", device, ", came back as another");
+    return as(x, types[i]);
+  }
+  List apply(List&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined() && !grads[1].defined()) return List(4);
+    const bool again = at::GradMode::is_enabled();
+    List out(4);
+    {
+      const at::NoGradGuard no_grad;
+      const c10::OptionalDeviceGuard on(device);
+      Tensor x[SAVED];
+      for (int i = 0; i < SAVED; ++i) x[i] = back(i);
+      Tensor dz[2];
+      for (int i = 0; i < 2; ++i) {
+        if (grads[i].defined()) {
+          TORCH_CHECK(grads[i].sizes() == at::IntArrayRef(shapes[i]) && grads[i].device() == device, "qk_norm_rope backward: a gradient of another shape or device");
+          dz[i] = as(grads[i], types[i]);
+        } else dz[i] = at::zeros(shapes[i], x[i].options().requires_grad(false));
+      }
+      lmoe_rope_args b = a;
+      b.q = desc(x[Q], head_first); b.k = desc(x[K], head_first); b.qw = ptr(x[QW]); b.kw = ptr(x[KW]);
+      b.cos = (const float*)ptr(x[COS]); b.sin = (const float*)ptr(x[SIN]);
+      b.positions = (const int32_t*)ptr(x[POSITIONS]); b.offsets = (const int32_t*)ptr(x[OFFSETS]); b.cu_seqlens = (const int32_t*)ptr(x[CU]);
+      b.dzq = desc(dz[0], head_first); b.dzk = desc(dz[1], head_first);
+      for (int i = 0; i < 2; ++i) out[i] = at::empty(shapes[i], x[i].options().requires_grad(false));
+      for (int i = QW; i <= KW; ++i) if (given[i] && task_should_compute_output(i)) out[i] = at::empty(shapes[i], x[i].options().requires_grad(false));
+      b.dq = desc(out[0], head_first); b.dk = desc(out[1], head_first); b.dqw = ptr(out[QW]); b.dkw = ptr(out[KW]);
+      const int64_t floats = lib.rope_floats(&b);
+      TORCH_CHECK(floats >= 0, "qk_norm_rope backward failed (", floats, "): ", lib.last_error());
+      Tensor ws;
+      if (floats) ws = at::empty({floats}, x[Q].options().dtype(at::kFloat).requires_grad(false));
+      b.ws = (float*)ptr(ws);
+      const int rc = lib.rope_bwd(&b, c10::hip::getCurrentHIPStream(device.index()).stream());
+      TORCH_CHECK(rc == 0, "qk_norm_rope backward failed (", rc, "): ", lib.last_error());
+    }
+    if (again) {                                   // (create_graph: the gradients are constants to everything but an attempt to derive them)
+      List known;
+      for (auto& x : out) if (x.defined()) known.push_back(x.detach().requires_grad_(true));
+      known = torch::autograd::DelayedError("trying to differentiate qk_norm_rope twice, which has no second derivative", (int64_t)known.size()).apply(std::move(known));
+      size_t i = 0;
+      for (auto& x : out) if (x.defined()) x = known[i++];
+    }
+    return out;
+  }
+};
+
+// rope_node(as rope_forward) -> (q, k) with their node, for a call that autograd has to see
+PyObject* rope_node(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Rope c;
+  if (n != 14 || !c.take(o)) return elsewhere();
+  void* st = stream_of(o[13]);
+  if (PyErr_Occurred()) return elsewhere();
+  Tensor zq, zk;
+  int rc;
+  {
+    const Unlocked unlocked;
+    rc = c.forward(zq, zk, st);
+    if (rc == 0) {
+      const std::shared_ptr<RopeNode> node(new RopeNode, torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(c.q, c.k, c.qw, c.kw));
+      node->a = c.a; node->head_first = c.head_first; node->device = c.q.device();
+      torch::autograd::set_history(zq, node);
+      torch::autograd::set_history(zk, node);
+      const Tensor* const all[] = {&c.q, &c.k, &c.qw, &c.kw, &c.tables[0], &c.tables[1], &c.tables[2], &c.tables[3], &c.tables[4]};
+      for (int i = 0; i < RopeNode::SAVED; ++i) node->save(i, *all[i]);
+    }
+  }
+  return result(rc, {zq, zk});
+  END_HANDLE_TH_ERRORS
+}
+
 // bind(path): the library's entry points
 PyObject* bind(PyObject*, PyObject* path) {
   const char* p = PyUnicode_AsUTF8(path);
@@ -1086,7 +1560,12 @@ PyObject* bind(PyObject*, PyObject* path) {
   get(l.gates_partials, "lmoe_gdn_gates_partials"); get(l.gates_fwd, "lmoe_gdn_gates_fwd"); get(l.gates_bwd, "lmoe_gdn_gates_bwd");
   get(l.mom_gather, "lmoe_mom_gather"); get(l.mom_combine, "lmoe_mom_combine"); get(l.mom_combine_bwd, "lmoe_mom_combine_bwd");
   get(l.last_error, "lmoe_last_error"); get(l.attn_fwd, "lmoe_softmax_attn_fwd"); get(l.attn_bwd, "lmoe_softmax_attn_bwd"); get(l.attn_bwd_floats, "lmoe_softmax_attn_bwd_floats"); get(l.paged_floats, "lmoe_paged_attn_floats");
-  get(l.paged_decode, "lmoe_paged_attn_decode"); get(l.paged_append, "lmoe_paged_kv_append");
+  get(l.paged_decode, "lmoe_paged_attn_decode"); get(l.paged_append, "lmoe_paged_kv_append"); get(l.paged_read, "lmoe_paged_kv_read");
+  get(l.paged4_floats, "lmoe_paged4_attn_floats"); get(l.paged4_decode, "lmoe_paged4_attn_decode");
+  get(l.paged4_append, "lmoe_paged4_kv_append"); get(l.paged4_read, "lmoe_paged4_kv_read");
+  get(l.fork_ints, "lmoe_paged_fork_ints"); get(l.pages_ints, "lmoe_paged_pages_ints"); get(l.pages_free, "lmoe_paged_free");
+  get(l.pages_fork, "lmoe_paged_fork"); get(l.pages_reserve, "lmoe_paged_reserve"); get(l.pages_compact, "lmoe_paged_compact");
+  get(l.rope_floats, "lmoe_qk_norm_rope_floats"); get(l.rope_fwd, "lmoe_qk_norm_rope_fwd"); get(l.rope_bwd, "lmoe_qk_norm_rope_bwd");
   get(l.mom_plan_ints, "lmoe_mom_plan_ints"); get(l.mom_plan, "lmoe_mom_plan"); get(l.seq_tables, "lmoe_seq_tables");
   if (!all) return PyErr_Format(PyExc_RuntimeError, "%s lacks an entry point", p);
   lib = l;
@@ -1103,6 +1582,8 @@ PyMethodDef methods[] = {
     LMOE_METHOD(gates_forward), LMOE_METHOD(gates_backward), LMOE_METHOD(mom_gather), LMOE_METHOD(mom_combine),
     LMOE_METHOD(mom_combine_backward), LMOE_METHOD(mom_plan), LMOE_METHOD(seq_tables),
     LMOE_METHOD(attn_forward), LMOE_METHOD(attn_backward), LMOE_METHOD(attn_node), LMOE_METHOD(paged_decode), LMOE_METHOD(paged_append),
+    LMOE_METHOD(paged4_decode), LMOE_METHOD(paged4_append), LMOE_METHOD(paged_read), LMOE_METHOD(pages_free), LMOE_METHOD(pages_fork), LMOE_METHOD(pages_reserve),
+    LMOE_METHOD(pages_compact), LMOE_METHOD(rope_forward), LMOE_METHOD(rope_node),
 #undef LMOE_METHOD
     {"intact", (PyCFunction)(void (*)(void))intact, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -167,10 +167,10 @@ def paged_attn_decode(
     name = "paged_attn_decode"
     _no_grad(name, q, k, v, k_pages, v_pages, slopes)
     scales = _both_scales(k_scales, v_scales, name)
-    if k_scales is None:
-        r = native_call("paged_decode", name, k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first)
-        if r is not None:
-            return r[0]
+    call = k_pages, v_pages, page_table, lens, q, k, v, scale, softcap, slopes, head_first
+    r = native_call("paged_decode", name, *call) if k_scales is None else native_call("paged4_decode", name, *call, k_scales, v_scales)
+    if r is not None:
+        return r[0]
     if (k is None) != (v is None):
         raise ValueError(f"{name}: k and v go together")
     a, held = _pages(k_pages, v_pages, page_table, lens, name, scales, q.dtype)
@@ -219,7 +219,8 @@ def paged_kv_append(
     name = "paged_kv_append"
     _no_grad(name, k, v, k_pages, v_pages)
     scales = _both_scales(k_scales, v_scales, name)
-    if k_scales is None and native_call("paged_append", name, k_pages, v_pages, page_table, lens, k, v, cu_seqlens, head_first) is not None:
+    call = k_pages, v_pages, page_table, lens, k, v, cu_seqlens, head_first
+    if (native_call("paged_append", name, *call) if k_scales is None else native_call("paged4_append", name, *call, k_scales, v_scales)) is not None:
         return
     a, held = _pages(k_pages, v_pages, page_table, lens, name, scales, k.dtype)
     if k.dim() != 4 or v.dim() != 4:
@@ -258,6 +259,10 @@ def paged_kv_read(
             raise ValueError(f"{name}: the pages are {k_pages.dtype}, not {dtype}")
         dtype = k_pages.dtype
     dtype, T = dtype or torch.bfloat16, int(T)
+    if dtype in _DT:
+        r = native_call("paged_read", name, k_pages, v_pages, page_table, starts, T, cu_seqlens, head_first, k_scales, v_scales, dtype == torch.float32)
+        if r is not None:
+            return r
     a, held = _pages(k_pages, v_pages, page_table, starts, name, scales, dtype)
     if not 0 <= T < 2 ** 31:
         raise ValueError(f"{name}: T={T}")

@@ -22,7 +22,7 @@ from typing import Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from ._host import ptr, stream_ptr
+from ._host import native_call, ptr, stream_ptr
 from .paged_kv import _no_grad, _written
 from .softmax_attn import ints_of, on_current_device, to_int32
 
@@ -99,6 +99,10 @@ def paged_reserve(
 
     lens itself is the caller's to advance."""
     name = "paged_reserve"
+    _no_grad(name, page_table)
+    r = native_call("pages_reserve", name, page_table, lens, refs, pages, tokens)
+    if r is not None:
+        return r[0]
     a = _state(page_table, refs, name, lens)
     dev = page_table.device
     pages, held = _bufs(pages, a, dev, name)
@@ -126,6 +130,9 @@ def paged_fork(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
     as a beam search does; the pages are shared from then on, and what a row of dst held before is given up.  src, dst: whole
     numbers on the device, ``[F]``.  Of several i with one dst the last counts; an i with a row outside 0 .. N - 1 is left out."""
     name = "paged_fork"
+    _no_grad(name, page_table)
+    if native_call("pages_fork", name, page_table, lens, refs, src, dst) is not None:
+        return
     a = _state(page_table, refs, name, lens)
     dev = page_table.device
     src, dst = _rows(src, name, "src", dev), _rows(dst, name, "dst", dev)
@@ -145,6 +152,9 @@ def paged_free(page_table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor,
     """The sequences ``rows`` (``[F]`` whole numbers on the device; the same one twice is as good as once, one outside 0 .. N - 1 is left
     out) give their pages back: entries become -1, ``lens`` 0."""
     name = "paged_free"
+    _no_grad(name, page_table)
+    if native_call("pages_free", name, page_table, lens, refs, rows) is not None:
+        return
     a = _state(page_table, refs, name, lens)
     rows = _rows(rows, name, "rows", page_table.device)
     a.F, a.rows = rows.numel(), rows.data_ptr()
@@ -161,6 +171,10 @@ def paged_compact(
     behind can go to another use; ``page_table`` and ``refs`` follow.  Returns live ``[1]`` and moved ``[P]``, int32: where each page went (itself,
     where it stayed), for what else a program keeps by their numbers."""
     name = "paged_compact"
+    _no_grad(name, page_table)
+    r = native_call("pages_compact", name, page_table, refs, pages)
+    if r is not None:
+        return r
     a = _state(page_table, refs, name)
     dev = page_table.device
     pages, held = _bufs(pages, a, dev, name)

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._host import _DT, _desc, has_tangent, no_node, ptr, stream_ptr
+from ._host import _DT, _desc, has_tangent, native_call, no_node, no_transform, ptr, stream_ptr
 from .softmax_attn import ints_of, on_current_device, to_int32
 
 MAX_ROPE_DIM = 256      # columns of a head
@@ -151,6 +151,12 @@ def qk_norm_rope(
     Forward and backward capture into a HIP graph; capture with leaves of which no graph of an eager step lives any more (torch's
     accumulation nodes belong to the stream of their first use)."""
     name = "qk_norm_rope"
+    grad = not no_node(q, k, q_weight, k_weight)
+    if not grad or no_transform():                   # (what the native path takes as it is, it also checks)
+        r = native_call("rope_node" if grad else "rope_forward", name, q, k, q_weight, k_weight, cos, sin, positions, offsets, cu_seqlens, eps, norm,
+                        interleaved, head_first)
+        if r is not None:
+            return r
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"{name}: q and k must be 4-dimensional")
     on_current_device(q.device, name)
@@ -213,6 +219,6 @@ def qk_norm_rope(
     if offsets is not None:
         offsets = ints_of(offsets, N, dev, f"{name}: offsets")
     call = _Call((B, T, HQ, HKV, D), head_first, cos, sin, R, positions, offsets, cu, N, float(eps), bool(norm), bool(interleaved))
-    if no_node(q, k, *weights):
+    if not grad:
         return call.forward(q, k, *(None if w is None else w.detach().contiguous() for w in (q_weight, k_weight)))[2:]
     return _QkNormRope.apply(q, k, q_weight, k_weight, call)
