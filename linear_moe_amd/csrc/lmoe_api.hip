@@ -832,6 +832,7 @@ static int check_rope(const lmoe_rope_args* a, const char* op, bool bwd) {
   if (a->R < 0 || a->R > a->D || a->R % 2) return fail(-3, "%s: R=%d must be even, 0 to D=%d", op, a->R, a->D);
   if (a->B < 0 || a->T < 0 || a->HQ <= 0 || a->HKV <= 0 || a->N < 0 || a->L < 0) return fail(-4, "%s: negative dimension", op);
   if (a->HQ > 65535 || a->HKV > 65535) return fail(-8, "%s: heads must be <= 65535", op);
+  if ((int64_t)a->B * a->T > 1 << 30) return fail(-8, "%s: more than 2^30 tokens", op);
   if (a->cu_seqlens && (a->B != 1 || a->positions)) return fail(-5, "%s: packed input needs B == 1 and no positions", op);
   if (a->positions && a->offsets) return fail(-5, "%s: positions and offsets exclude each other", op);
   if (!a->q.ptr || !a->k.ptr) return fail(-7, "%s: q and k must not be null", op);

@@ -195,8 +195,12 @@ static PagedPlan paged4_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
   const int64_t bound = (int64_t)a.M * a.S + 1, groups = (int64_t)a.N * a.HKV * p.blocks;
-  p.waves = 4;
-  const int64_t chunk = 512;
+  // A short cache: one stretch of eight waves and no second launch; else stretches of one length, whatever the call (us for stretches of
+  // 512, 1024, 2048 positions, with the join: 64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 55 54 58; 2 of 32 K and 128 K,
+  // 16 / 4 heads of 128: 33 29 39).
+  // (a launch has less than 2^32 threads: of 2^23 work-groups and more, which N * HQ < 2^24 allows, none has 512)
+  p.waves = bound <= 1024 && groups < 1 << 23 ? 8 : 4;
+  const int64_t chunk = 1024;
   const int64_t splits = (bound + chunk - 1) / chunk;
   const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;
   p.splits = (int)(splits < most ? splits : most);
@@ -221,8 +225,29 @@ template <int W> struct Tile4 {
   uint32_t live;                                   // which of the positions exist
 };
 
-template <typename T, int W, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
+// The B-th byte of the lane's keys of V, columns 2B and 2B + 1 of its own: as two products with P
+template <typename T, int W, int B>
+__device__ __forceinline__ void pv4(f32x4 (&o)[W / 16], const Tile4<W>& t, const typename ET<T>::frag& pf) {
+  typename ET<T>::frag lo, hi;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[e], scale_of(t.vs[e]), B);
+      lo[e] = x[0];
+      hi[e] = x[1];
+    } else {
+      const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t.v[e], scale_of(t.vs[e]), B);
+      if (e < 4) { lo.lo[e] = x[0]; hi.lo[e] = x[1]; } else { lo.hi[e - 4] = x[0]; hi.hi[e - 4] = x[1]; }
+    }
+  }
+  ET<T>::mma(o[2 * B], lo, pf);
+  ET<T>::mma(o[2 * B + 1], hi, pf);
+}
+
+// EVEN: 16 adjacent positions lie in one page (S a multiple of 16; no stride of a token passes 2^27 bytes), so that a step's rows are two
+// bases in scalar registers and offsets that stay the same; else every position's page is looked up by a lane and passed round.
+template <typename T, int W, int NW, bool EVEN, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
   const lmoe_paged_args& a = a4.p;
   typedef Tile4<W> Tile;
   constexpr int KW = Tile::KW, KC = W / 4, VW = W / 16;
@@ -247,45 +272,103 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn
   const uint8_t* vsp = (const uint8_t*)a4.vs.ptr + (int64_t)hk * a4.vs.sh;
   const bool kin = KC * g < a.K, vin = VW * c < a.V;           // columns behind the head dimension are zeros
 
-  // Where the lane's position (j0 + l % 32) lies; asked for two steps before its rows are used, as in k_paged_attn
-  struct Where { int id, slot; };
+  // Where the positions of a step lie: the lane's own (j0 + l % 32), or with EVEN those of each half, the same in all lanes.  Asked for two
+  // steps before its rows are used, as in k_paged_attn.
+  struct Where { int id[2], slot[2]; };
+  auto column = [&](int j) { return (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s); };
   auto ask = [&](int j0) {
-    Where x = {-1, 0};
-    const int j = j0 + (l & 31);
-    if (j < end) {
-      const int col = (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s);
-      x.slot = j - col * a.S;
-      x.id = table[col];
+    Where x = {{-1, -1}, {0, 0}};
+    if constexpr (EVEN) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int j = j0 + 16 * b;
+        if (j < end) {
+          const int col = column(j);
+          x.slot[b] = j - col * a.S;
+          x.id[b] = as_const(table)[col];
+        }
+      }
+    } else {
+      const int j = j0 + (l & 31);
+      if (j < end) {
+        const int col = column(j);
+        x.slot[0] = j - col * a.S;
+        x.id[0] = table[col];
+      }
     }
     return x;
   };
-  auto load = [&](Tile& t, const Where& x) {
-    const bool there = x.id >= 0 && x.id < a.P;
-    t.live = (uint32_t)__ballot(there);
+  const uint32_t kst = (uint32_t)a.kp.st, vst = (uint32_t)a.vp.st, kss = (uint32_t)a4.ks.st, vss = (uint32_t)a4.vs.st;
+  uint32_t vo[4], vso[4];               // EVEN: offsets of the lane's keys of V inside a half, and c's of K
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int64_t id = __shfl(x.id, 16 * b + c, 64), slot = __shfl(x.slot, 16 * b + c, 64);
-      words y;
-#pragma unroll
-      for (int i = 0; i < KW; ++i) y[i] = 0;
-      t.ks[b] = 127;
-      if ((t.live >> (16 * b + c) & 1) && kin) {
-        y = *(const words*)(kp + id * a.kp.sb + slot * a.kp.st + KC / 2 * g);
-        t.ks[b] = ksp[id * a4.ks.sb + slot * a4.ks.st + KC * g / 32];
-      }
+  for (int e = 0; e < 4; ++e) { vo[e] = (4 * g + e) * vst + VW / 2 * c; vso[e] = (4 * g + e) * vss + VW * c / 32; }
+  const uint32_t ko = c * kst + KC / 2 * g, kso = c * kss + KC * g / 32;
+  auto load = [&](Tile& t, int j0, const Where& x) {
+    auto k_row = [&](int b, const uint8_t* codes, const uint8_t* scale) {
+      const words y = *(const words*)codes;
 #pragma unroll
       for (int i = 0; i < KW; ++i) t.k[b][i] = y[i];
-    }
+      t.ks[b] = *scale;
+    };
+    auto v_row = [&](int e, const uint8_t* codes, const uint8_t* scale) {
+      if constexpr (VW == 8) t.v[e] = *(const uint32_t*)codes; else t.v[e] = *(const uint16_t*)codes;
+      t.vs[e] = *scale;
+    };
+    auto nothing = [&]() {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int at = 16 * (e >> 2) + 4 * g + (e & 3);
-      const int64_t id = __shfl(x.id, at, 64), slot = __shfl(x.slot, at, 64);
-      t.v[e] = 0;
-      t.vs[e] = 127;
-      if ((t.live >> at & 1) && vin) {
-        const uint8_t* row = vp + id * a.vp.sb + slot * a.vp.st + VW / 2 * c;
-        if constexpr (VW == 8) t.v[e] = *(const uint32_t*)row; else t.v[e] = *(const uint16_t*)row;
-        t.vs[e] = vsp[id * a4.vs.sb + slot * a4.vs.st + VW * c / 32];
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < KW; ++i) t.k[b][i] = 0;
+        t.ks[b] = 127;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { t.v[e] = 0; t.vs[e] = 127; }
+    };
+    if constexpr (EVEN) {
+      bool there[2];
+      const uint8_t *kb[2], *vb[2], *ksb[2], *vsb[2];
+      uint32_t live = 0;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        there[b] = x.id[b] >= 0 && x.id[b] < a.P;
+        const int64_t id = there[b] ? x.id[b] : 0, slot = x.slot[b];
+        kb[b] = kp + id * a.kp.sb + slot * a.kp.st;
+        vb[b] = vp + id * a.vp.sb + slot * a.vp.st;
+        ksb[b] = ksp + id * a4.ks.sb + slot * a4.ks.st;
+        vsb[b] = vsp + id * a4.vs.sb + slot * a4.vs.st;
+        const int left = min(16, end - j0 - 16 * b);          // positions of the half
+        if (there[b] && left > 0) live |= ((1u << left) - 1) << (16 * b);
+      }
+      t.live = live;
+      if (live == ~0u && (KC * 4 == a.K) && (VW * 16 == a.V)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) k_row(b, kb[b] + ko, ksb[b] + kso);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v_row(e, vb[e >> 2] + vo[e & 3], vsb[e >> 2] + vso[e & 3]);
+      } else {
+        nothing();
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          if (kin && (live >> (16 * b + c) & 1)) k_row(b, kb[b] + ko, ksb[b] + kso);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (vin && (live >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) v_row(e, vb[e >> 2] + vo[e & 3], vsb[e >> 2] + vso[e & 3]);
+      }
+    } else {
+      t.live = (uint32_t)__ballot(x.id[0] >= 0 && x.id[0] < a.P);
+      nothing();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int64_t id = __shfl(x.id[0], 16 * b + c, 64), slot = __shfl(x.slot[0], 16 * b + c, 64);
+        if ((t.live >> (16 * b + c) & 1) && kin)
+          k_row(b, kp + id * a.kp.sb + slot * a.kp.st + KC / 2 * g, ksp + id * a4.ks.sb + slot * a4.ks.st + KC * g / 32);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = 16 * (e >> 2) + 4 * g + (e & 3);
+        const int64_t id = __shfl(x.id[0], at, 64), slot = __shfl(x.slot[0], at, 64);
+        if ((t.live >> at & 1) && vin)
+          v_row(e, vp + id * a.vp.sb + slot * a.vp.st + VW / 2 * c, vsp + id * a4.vs.sb + slot * a4.vs.st + VW * c / 32);
       }
     }
   };
@@ -320,15 +403,29 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int j = j0 + 16 * b + 4 * g + e;
-        const float x = sc.of(s[b][e], CAP ? sc.squash(s[b][e]) : 0.f, (float)(total - 1 - j));
-        s[b][e] = t.live >> (16 * b + 4 * g + e) & 1 ? x : -INFINITY;
-        mx = fmaxf(mx, s[b][e]);
+        s[b][e] = sc.of(s[b][e], CAP ? sc.squash(s[b][e]) : 0.f, (float)(total - 1 - j));
       }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float next = fmaxf(m, mx), f = pow2(m - next);
-    m = next;
-    sum *= f;
+    if (t.live != ~0u) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[b][e] = t.live >> (16 * b + 4 * g + e) & 1 ? s[b][e] : -INFINITY;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[b][e]);
+    // The maximum moves only where a score passes it by 2^8: P is as exact at 2^8 as at 1, and most steps neither ask the other lanes nor
+    // touch the accumulators.
+    if (__any(mx > m + 8.0f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float next = fmaxf(m, mx), f = pow2(m - next);
+      m = next;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < VW; ++i) o[i] *= f;
+    }
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -339,28 +436,13 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn
     // (P rounded to the element type, as the products take it; the sum is of the numbers before)
     typename ET<T>::frag pf;
     if constexpr (FAST) pf = frag_of_blocks(s[0], s[1]); else { pf.lo = s[0]; pf.hi = s[1]; }
-    typename ET<T>::frag v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = from4<T>(t.v[e], scale_of(t.vs[e]));
-#pragma unroll
-    for (int i = 0; i < VW; ++i) {
-      o[i] *= f;
-      typename ET<T>::frag vf;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (FAST) vf[e] = v[e][i];
-        else {
-          const float x = i < 4 ? v[e].lo[i & 3] : v[e].hi[i & 3];
-          if (e < 4) vf.lo[e] = x; else vf.hi[e - 4] = x;
-        }
-      }
-      ET<T>::mma(o[i], vf, pf);
-    }
+    pv4<T, W, 0>(o, t, pf);
+    pv4<T, W, 1>(o, t, pf);
+    if constexpr (VW == 8) { pv4<T, W, 2>(o, t, pf); pv4<T, W, 3>(o, t, pf); }
   };
 
   Tile t[2];
-  if (j0 < end) load(t[0], at);
-  // the new token: the first of 32 positions that hold nothing else
+  // the new token, in front of the others (their registers are free then): the first of 32 positions that hold nothing else
   if (a.kn.ptr && stop == total && w == (end - begin + PSTEP - 1) / PSTEP % NW) {
     const T* kn = (const T*)a.kn.ptr + (int64_t)n * a.kn.sb + (int64_t)hk * a.kn.sh;
     const T* vn = (const T*)a.vn.ptr + (int64_t)n * a.vn.sb + (int64_t)hk * a.vn.sh;
@@ -416,16 +498,17 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn
     if (g != 0) { y.v[0] = 0; y.vs[0] = 127; }
     take(y, sq.len);
   }
+  if (j0 < end) load(t[0], j0, at);
   while (j0 < end) {
     at = ahead;
     ahead = ask(j0 + 2 * PGROUP);
-    if (j0 + PGROUP < end) load(t[1], at);
+    if (j0 + PGROUP < end) load(t[1], j0 + PGROUP, at);
     take(t[0], j0);
     j0 += PGROUP;
     if (j0 >= end) break;
     at = ahead;
     ahead = ask(j0 + 2 * PGROUP);
-    if (j0 + PGROUP < end) load(t[0], at);
+    if (j0 + PGROUP < end) load(t[0], j0 + PGROUP, at);
     take(t[1], j0);
     j0 += PGROUP;
   }
@@ -463,16 +546,24 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_paged4_attn
   }
 }
 
-template <typename T, int W, int NW> static void paged4_parts(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
+template <typename T, int W, int NW, bool EVEN> static void paged4_parts(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
   const dim3 grid((uint32_t)((int64_t)a.p.N * a.p.HKV * p.blocks * p.splits)), block(64 * NW);
   if (a.p.softcap > 0.f) {
-    if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, true, true>), grid, block, 0, st, a, p);
-    else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, true, false>), grid, block, 0, st, a, p);
-  } else if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, false, true>), grid, block, 0, st, a, p);
-  else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, false, false>), grid, block, 0, st, a, p);
+    if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, true>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, false>), grid, block, 0, st, a, p);
+  } else if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, false, true>), grid, block, 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, false, false>), grid, block, 0, st, a, p);
+}
+template <typename T, int W> static void paged4_wide(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
+  bool even = a.p.S % 16 == 0;
+  for (const lmoe_tensor* t : {&a.p.kp, &a.p.vp, &a.ks, &a.vs}) even = even && t->st < 1 << 27;
+  if (p.waves == 8) {
+    if (even) paged4_parts<T, W, 8, true>(a, p, st); else paged4_parts<T, W, 8, false>(a, p, st);
+  } else if (even) paged4_parts<T, W, 4, true>(a, p, st);
+  else paged4_parts<T, W, 4, false>(a, p, st);
 }
 template <typename T> static void paged4_decode(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
-  if (a.p.K <= 64 && a.p.V <= 64) paged4_parts<T, 64, 4>(a, p, st); else paged4_parts<T, 128, 4>(a, p, st);
+  if (a.p.K <= 64 && a.p.V <= 64) paged4_wide<T, 64>(a, p, st); else paged4_wide<T, 128>(a, p, st);
 }
 void launch_paged4_decode(const lmoe_paged4_args& a, hipStream_t st) {
   const PagedPlan p = paged4_plan(a.p);

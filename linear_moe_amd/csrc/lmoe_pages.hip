@@ -22,7 +22,6 @@ struct PagesWs {
   int32_t *src, *dst;                   // [P] their pages
   int32_t* list;                        // [P] free pages
   int32_t *claims, *last, *failed;      // [P] of a shared page: asked entries, the last of them, whether one gets no copy
-  int32_t* need;                        // [N] pages that the rows up to a row need
 };
 __host__ __device__ inline PagesWs pages_ws(const lmoe_pages_args& a) {
   PagesWs w;
@@ -33,11 +32,10 @@ __host__ __device__ inline PagesWs pages_ws(const lmoe_pages_args& a) {
   w.last = p; p += a.P;
   w.failed = p; p += a.P;
   w.src = p; p += a.P;
-  w.dst = p; p += a.P;
-  w.need = p;
+  w.dst = p;
   return w;
 }
-int64_t pages_ints(const lmoe_pages_args& a) { return 16 + 6 * (int64_t)a.P + a.N; }
+int64_t pages_ints(const lmoe_pages_args& a) { return 16 + 6 * (int64_t)a.P; }
 int64_t fork_ints(const lmoe_pages_args& a) { return (int64_t)a.F * (a.M + 1); }
 
 // memory that other waves of the work-group wrote, or that atomics count in: past this CU's cache
@@ -67,20 +65,39 @@ __device__ __forceinline__ int scan(int x, int& total, int* s_wave) {
 }
 
 // The numbers p in [begin, end) with (refs[p] > 0) == used, in their order, into list[0 .. most - 1]; how many there are (counting stops
-// behind the one that fills the list)
-__device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, bool used, int32_t* list, int most, int* s_wave) {
+// behind the tile that fills the list).  A tile is PAGES_VEC numbers for every thread, PAGES_NTHR apart, so that a load reads
+// adjacent ones and all of a tile are in flight at once.
+struct ListShared { int count[PAGES_VEC * PAGES_WAVES], wave[PAGES_WAVES]; };
+__device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, bool used, int32_t* list, int most, ListShared& sh) {
+  static_assert(PAGES_VEC * PAGES_WAVES <= PAGES_NTHR, "");
+  const int wave = wave_id();
   int before = 0;
   for (int p0 = begin; p0 < end && before < most; p0 += PAGES_NTHR * PAGES_VEC) {
-    const int first = p0 + (int)threadIdx.x * PAGES_VEC;
-    uint32_t hit = 0;
+    uint64_t hit[PAGES_VEC];
+    int r[PAGES_VEC];
 #pragma unroll
-    for (int i = 0; i < PAGES_VEC; ++i)
-      if (first + i < end && (refs[first + i] > 0) == used) hit |= 1u << i;
-    int total, at = before + scan(__popc(hit), total, s_wave);
+    for (int i = 0; i < PAGES_VEC; ++i) {
+      const int p = p0 + i * PAGES_NTHR + (int)threadIdx.x;
+      r[i] = p < end ? refs[p] : (used ? 0 : 1);
+    }
 #pragma unroll
-    for (int i = 0; i < PAGES_VEC; ++i)
-      if (hit >> i & 1) { if (at < most) put(list + at, first + i); ++at; }
+    for (int i = 0; i < PAGES_VEC; ++i) {
+      hit[i] = __ballot((r[i] > 0) == used);
+      if (lane_id() == 0) sh.count[i * PAGES_WAVES + wave] = __popcll(hit[i]);
+    }
+    __syncthreads();
+    const int slot = threadIdx.x;
+    int total;
+    const int at = scan(slot < PAGES_VEC * PAGES_WAVES ? sh.count[slot] : 0, total, sh.wave);
+    if (slot < PAGES_VEC * PAGES_WAVES) sh.count[slot] = at;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PAGES_VEC; ++i) {
+      const int k = before + sh.count[i * PAGES_WAVES + wave] + __popcll(hit[i] & ((1ull << lane_id()) - 1));
+      if ((hit[i] >> lane_id() & 1) && k < most) put(list + k, p0 + i * PAGES_NTHR + (int)threadIdx.x);
+    }
     before += total;
+    __syncthreads();                       // sh.count has been read
   }
   return before;
 }
@@ -141,120 +158,163 @@ __device__ __forceinline__ bool asked(const lmoe_pages_args& a, int n, int& firs
 // In the order of rows and columns, as if one after the other: an entry that names a page of refs r, of which e entries in front
 // of it are asked for too, has to be copied if r - e > 1, for those have taken their copies by then.  So of the asked entries of a page all are
 // copied, but the last where there are r of them.
+// The asked entries of PAGES_NTHR rows at a time are dealt to the threads; where the call has one for a thread, it stays in its registers
+// from the first step to the last (256 rows of one token, 41 thousand pages: 8 us; with a wave for every row, which waits for its entries again
+// in each step, 115).
+struct Asked { int n, c, x, refs; bool last; };      // row, column, entry, refs of its page (0: none), whether the row's last
 __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_args a) {
-  __shared__ int s_wave[PAGES_WAVES];
+  __shared__ ListShared sh;
+  __shared__ int s_first[PAGES_NTHR], s_start[PAGES_NTHR + 1], s_before[PAGES_NTHR], s_upto[PAGES_NTHR];
+  __shared__ uint8_t s_fits[PAGES_NTHR];
   const PagesWs w = pages_ws(a);
-  const int wave = wave_id(), l = lane_id();
-  auto each = [&](auto f) {                              // a wave per row, its columns over the lanes
-    for (int n = wave; n < a.N; n += PAGES_WAVES) {
-      int first, last;
-      if (asked(a, n, first, last)) f(n, first, last);
+  const int tid = threadIdx.x;
+  int row0 = 0, count = 0;                // rows from row0 on are dealt out, `count` entries of theirs
+  auto deal = [&](int n0) {
+    const int n = n0 + tid;
+    int first = 0, last = -1;
+    bool fits = false;
+    if (n < a.N) fits = asked(a, n, first, last);
+    const int at = scan(last - first + 1, count, sh.wave);
+    s_first[tid] = first;
+    s_start[tid] = at;
+    s_fits[tid] = fits;
+    if (tid == 0) s_start[PAGES_NTHR] = count;
+    row0 = n0;
+    __syncthreads();
+  };
+  auto entry = [&](int i) {
+    Asked e = {-1, 0, -1, 0, false};
+    if (i >= count) return e;
+    int lo = 0, hi = PAGES_NTHR;          // the last row that begins at or before entry i (rows without entries begin where the next does)
+#pragma unroll
+    for (int k = 0; k < 10; ++k) {
+      const int m = (lo + hi) >> 1;
+      if (s_start[m] <= i) lo = m; else hi = m;
+    }
+    e.n = row0 + lo;
+    e.c = s_first[lo] + i - s_start[lo];
+    e.last = i + 1 == s_start[lo + 1];
+    e.x = a.table[(int64_t)e.n * a.table_stride + e.c];
+    if (e.x < 0 || e.x >= a.P) e.x = -1;
+    else e.refs = a.refs[e.x];
+    return e;
+  };
+  static_assert(PAGES_NTHR == 1 << 10, "");
+  deal(0);
+  const bool whole = a.N <= PAGES_NTHR, single = whole && count <= PAGES_NTHR;
+  const Asked mine = single ? entry(tid) : Asked{-1, 0, -1, 0, false};
+  // f(entry, whether there is one), by all threads
+  auto entries = [&](auto f) {
+    for (int i0 = 0; i0 < count; i0 += PAGES_NTHR) {
+      const Asked e = single ? mine : entry(i0 + tid);
+      f(e);
     }
   };
-  auto entry = [&](int n, int c) { return a.table[(int64_t)n * a.table_stride + c]; };
-  auto is_page = [&](int x) { return x >= 0 && x < a.P; };
-  if (threadIdx.x == 0) put(w.count, 0);
-  each([&](int n, int first, int last) {
-    for (int c = first + l; c <= last; c += 64) {
-      const int x = entry(n, c);
-      if (is_page(x) && a.refs[x] > 1) { put(w.claims + x, 0); put(w.last + x, -1); put(w.failed + x, 0); }
+  auto every = [&](auto f) {
+    for (int n0 = 0; n0 < a.N; n0 += PAGES_NTHR) {
+      if (!whole) { __syncthreads(); deal(n0); }
+      entries(f);
     }
+  };
+  auto shared = [&](const Asked& e) { return e.x >= 0 && e.refs > 1; };
+  auto kept = [&](const Asked& e) { return seen(w.claims + e.x) == e.refs && seen(w.last + e.x) == e.n * a.M + e.c; };
+  if (tid == 0) put(w.count, 0);
+  every([&](const Asked& e) {
+    if (shared(e)) { put(w.claims + e.x, 0); put(w.last + e.x, -1); put(w.failed + e.x, 0); }
   });
   __syncthreads();
-  each([&](int n, int first, int last) {
-    for (int c = first + l; c <= last; c += 64) {
-      const int x = entry(n, c);
-      if (is_page(x) && a.refs[x] > 1) { atomicAdd(w.claims + x, 1); atomicMax(w.last + x, n * a.M + c); }
-    }
+  every([&](const Asked& e) {
+    if (shared(e)) { atomicAdd(w.claims + e.x, 1); atomicMax(w.last + e.x, e.n * a.M + e.c); }
   });
   __syncthreads();
-  auto shared = [&](int x) { return is_page(x) && a.refs[x] > 1; };
-  auto kept = [&](int n, int c, int x) { return seen(w.claims + x) == a.refs[x] && seen(w.last + x) == n * a.M + c; };
-  for (int n = threadIdx.x; n < a.N; n += PAGES_NTHR) put(w.need + n, 0);
+  auto copied = [&](const Asked& e) { return shared(e) && !kept(e); };
+  auto needs = [&](const Asked& e) { return e.n >= 0 && (e.x < 0 || copied(e)); };
+  int need = 0, all;
+  every([&](const Asked& e) { need += needs(e); });
+  scan(need, all, sh.wave);
+  const int free = listed(a.refs, 0, a.P, false, w.list, min(all, a.P), sh);
   __syncthreads();
-  each([&](int n, int first, int last) {
-    int need = 0;
-    for (int c0 = first; c0 <= last; c0 += 64) {
-      const int c = c0 + l, x = c <= last ? entry(n, c) : -1;
-      need += __popcll(__ballot(c <= last && (!is_page(x) || (shared(x) && !kept(n, c, x)))));
-    }
-    if (l == 0) put(w.need + n, need);
-  });
-  __syncthreads();
-  // how many pages up to each row
-  int all = 0;
-  for (int n0 = 0; n0 < a.N; n0 += PAGES_NTHR) {
-    const int n = n0 + threadIdx.x, need = n < a.N ? seen(w.need + n) : 0;
-    int total;
-    const int at = all + scan(need, total, s_wave);
-    if (n < a.N) put(w.need + n, at);
-    all += total;
-  }
-  const int free = listed(a.refs, 0, a.P, false, w.list, min(all, a.P), s_wave);
-  __syncthreads();
-  // rows that the free pages do not reach: the pages they do not copy stay shared
-  auto before = [&](int n) { return seen(w.need + n); };
-  auto upto = [&](int n) { return n + 1 < a.N ? seen(w.need + n + 1) : all; };
-  auto reached = [&](int n) { return upto(n) <= free || upto(n) == before(n); };
-  if (all > free) {
-    each([&](int n, int first, int last) {
-      if (reached(n)) return;
-      for (int c = first + l; c <= last; c += 64) {
-        const int x = entry(n, c);
-        if (shared(x) && !kept(n, c, x)) put(w.failed + x, 1);
-      }
+  // pages needed in front of and up to each row that is dealt out; before: by the rows in front of them
+  auto reach = [&](int before) {
+    s_before[tid] = s_upto[tid] = 0;
+    __syncthreads();
+    entries([&](const Asked& e) {
+      const int one = needs(e);
+      int total;
+      const int at = before + scan(one, total, sh.wave);
+      if (e.n >= 0 && e.c == s_first[e.n - row0]) s_before[e.n - row0] = at;
+      if (e.last) s_upto[e.n - row0] = at + one;
+      before += total;
     });
     __syncthreads();
+    return before;
+  };
+  auto reached = [&](int k) { return s_upto[k] <= free || s_upto[k] == s_before[k]; };
+  if (all > free) {
+    // rows that the free pages do not reach: the pages they do not copy stay shared
+    int before = 0;
+    for (int n0 = 0; n0 < a.N; n0 += PAGES_NTHR) {
+      if (!whole) { __syncthreads(); deal(n0); }
+      before = reach(before);
+      entries([&](const Asked& e) {
+        if (e.n >= 0 && !reached(e.n - row0) && copied(e)) put(w.failed + e.x, 1);
+      });
+      __syncthreads();
+    }
   }
-  for (int n = wave; n < a.N; n += PAGES_WAVES) {
-    int first, last;
-    bool fits = asked(a, n, first, last);
-    if (fits && all > free) {
-      fits = reached(n);
-      for (int c0 = first; fits && c0 <= last; c0 += 64) {
-        const int c = c0 + l, x = c <= last ? entry(n, c) : -1;
-        if (__ballot(c <= last && shared(x) && kept(n, c, x) && seen(w.failed + x))) fits = false;
-      }
+  int before = 0, given = 0;
+  for (int n0 = 0; n0 < a.N; n0 += PAGES_NTHR) {
+    if (!whole) { __syncthreads(); deal(n0); }
+    if (all > free) {
+      before = reach(before);
+      if (!reached(tid)) s_fits[tid] = false;
+      __syncthreads();
+      entries([&](const Asked& e) {
+        if (shared(e) && kept(e) && seen(w.failed + e.x)) s_fits[e.n - row0] = false;
+      });
+      __syncthreads();
     }
-    if (l == 0) a.fits[n] = fits;
-    // (refs of a shared page stays as it is until every wave has decided by it)
-    int at = before(n);
-    for (int c0 = first; fits && c0 <= last; c0 += 64) {
-      const int c = c0 + l, x = c <= last ? entry(n, c) : -1;
-      const bool copy = c <= last && shared(x) && !kept(n, c, x), take = copy || (c <= last && !is_page(x));
-      const uint64_t mask = __ballot(take);
-      if (take) {
-        const int page = seen(w.list + at + __popcll(mask & ((1ull << l) - 1)));
-        a.table[(int64_t)n * a.table_stride + c] = page;
-        a.refs[page] = 1;                                // (free or given out: no page is shared by it)
-        if (copy) {
-          const int i = atomicAdd(w.count, 1);           // (the order of the copies changes nothing)
-          put(w.src + i, x);
-          put(w.dst + i, page);
-        }
+    if (n0 + tid < a.N) a.fits[n0 + tid] = s_fits[tid];
+    // (refs of a shared page stays as it is until every thread has decided by it; the rows that fit take the free pages one by one, for
+    // those that do not lie behind them all, but for rows without needs)
+    entries([&](const Asked& e) {
+      const bool take = needs(e) && s_fits[e.n - row0];
+      int total;
+      const int at = given + scan(take, total, sh.wave);
+      given += total;
+      if (!take) return;
+      const int page = seen(w.list + at);
+      a.table[(int64_t)e.n * a.table_stride + e.c] = page;
+      a.refs[page] = 1;                    // (free or given out: no page is shared by it)
+      if (e.x >= 0) {
+        const int i = atomicAdd(w.count, 1);               // (the order of the copies changes nothing)
+        put(w.src + i, e.x);
+        put(w.dst + i, page);
       }
-      at += __popcll(mask);
-    }
+    });
   }
   __syncthreads();
   const int copies = seen(w.count);
-  for (int i = threadIdx.x; i < copies; i += PAGES_NTHR) atomicSub(a.refs + seen(w.src + i), 1);
+  for (int i = tid; i < copies; i += PAGES_NTHR) atomicSub(a.refs + seen(w.src + i), 1);
 }
 
 // ---- moved together ----
 __global__ __launch_bounds__(PAGES_NTHR) void k_pages_compact(const lmoe_pages_args a) {
-  __shared__ int s_wave[PAGES_WAVES];
+  __shared__ ListShared sh;
   const PagesWs w = pages_ws(a);
   int used = 0;
-  for (int p = threadIdx.x; p < a.P; p += PAGES_NTHR) {
-    used += a.refs[p] > 0;
-    put(a.moved + p, p);
+  for (int p0 = 0; p0 < a.P; p0 += PAGES_NTHR * PAGES_VEC) {
+#pragma unroll
+    for (int i = 0; i < PAGES_VEC; ++i) {
+      const int p = p0 + i * PAGES_NTHR + (int)threadIdx.x;
+      if (p < a.P) { used += a.refs[p] > 0; put(a.moved + p, p); }
+    }
   }
   int live;
-  scan(used, live, s_wave);
+  scan(used, live, sh.wave);
   // as many free numbers below as used pages above
-  const int count = listed(a.refs, 0, live, false, w.dst, live, s_wave);
-  listed(a.refs, live, a.P, true, w.src, count, s_wave);
+  const int count = listed(a.refs, 0, live, false, w.dst, live, sh);
+  listed(a.refs, live, a.P, true, w.src, count, sh);
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += PAGES_NTHR) {
     const int from = seen(w.src + i), to = seen(w.dst + i);
@@ -264,10 +324,11 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_compact(const lmoe_pages_a
   }
   if (threadIdx.x == 0) { a.live[0] = live; put(w.count, count); }
 }
-__global__ __launch_bounds__(NTHR) void k_pages_renamed(const lmoe_pages_args a) {
-  const int64_t all = (int64_t)a.N * a.M;
-  for (int64_t i = (int64_t)blockIdx.x * NTHR + threadIdx.x; i < all; i += (int64_t)gridDim.x * NTHR) {
-    int32_t* t = a.table + i / a.M * a.table_stride + i % a.M;
+// the table's entries after the move, by `groups` work-groups of which this is the k-th
+__device__ __forceinline__ void renamed(const lmoe_pages_args& a, int k, int groups) {
+  const int all = a.N * a.M;
+  for (int i = k * NTHR + threadIdx.x; i < all; i += groups * NTHR) {
+    int32_t* t = a.table + (int64_t)(i / a.M) * a.table_stride + i % a.M;
     const int x = *t;
     if (x >= 0 && x < a.P) *t = a.moved[x];
   }
@@ -276,6 +337,7 @@ __global__ __launch_bounds__(NTHR) void k_pages_renamed(const lmoe_pages_args a)
 // ---- the copies ----
 struct PageBufs {
   int n;
+  int renamers;                        // work-groups in front of the others that see to the table
   lmoe_page_buf b[COPY_BUFS];
   int32_t units[COPY_BUFS + 1];        // units of a page up to each tensor
   int32_t per[COPY_BUFS];              // units of a run
@@ -295,8 +357,9 @@ template <typename P> __device__ __forceinline__ void copy_run(uint8_t* to, cons
 __global__ __launch_bounds__(NTHR) void k_pages_copy(const lmoe_pages_args a, const PageBufs bufs) {
   const PagesWs w = pages_ws(a);
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  if ((int)blockIdx.x < bufs.renamers) return renamed(a, blockIdx.x, bufs.renamers);
   const int count = w.count[0], per_page = bufs.units[bufs.n];
-  for (int64_t x = blockIdx.x; x < (int64_t)count * per_page; x += gridDim.x) {
+  for (int64_t x = blockIdx.x - bufs.renamers; x < (int64_t)count * per_page; x += gridDim.x - bufs.renamers) {
     const int i = (int)(x / per_page), u = (int)(x % per_page);
     int k = 0;
     while (u >= bufs.units[k + 1]) ++k;
@@ -319,10 +382,12 @@ void launch_pages_fork(const lmoe_pages_args& a, hipStream_t st) {
   hipLaunchKernelGGL(k_pages_snapshot, dim3(a.F), dim3(NTHR), 0, st, a);
   hipLaunchKernelGGL(k_pages_fork, dim3(a.F), dim3(NTHR), 0, st, a);
 }
-static void pages_copies(const lmoe_pages_args& a, int64_t most, hipStream_t st) {
-  for (int k0 = 0; k0 < a.n_bufs; k0 += COPY_BUFS) {
-    PageBufs p;
+// at most so many pages; rename: the table's entries too
+static void pages_copies(const lmoe_pages_args& a, int64_t most, bool rename, hipStream_t st) {
+  for (int k0 = 0; k0 == 0 || k0 < a.n_bufs; k0 += COPY_BUFS) {
+    PageBufs p = {};
     p.n = std::min(COPY_BUFS, a.n_bufs - k0);
+    if (rename && k0 == 0) p.renamers = (int)std::min<int64_t>(((int64_t)a.N * a.M + 4 * NTHR - 1) / (4 * NTHR), 256);
     p.units[0] = 0;
     for (int k = 0; k < p.n; ++k) {
       const lmoe_page_buf& b = p.b[k] = a.bufs[k0 + k];
@@ -331,19 +396,17 @@ static void pages_copies(const lmoe_pages_args& a, int64_t most, hipStream_t st)
       const uint64_t bits = (uintptr_t)b.ptr | (uint64_t)(b.page_stride | b.stride0 | b.stride1 | b.bytes);
       p.vec[k] = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
     }
-    const int64_t units = most * p.units[p.n];
-    if (units > 0) hipLaunchKernelGGL(k_pages_copy, dim3((uint32_t)std::min<int64_t>(units, 2048)), dim3(NTHR), 0, st, a, p);
+    const int64_t units = most * p.units[p.n], groups = p.renamers + std::min<int64_t>(units, 2048);
+    if (groups > 0) hipLaunchKernelGGL(k_pages_copy, dim3((uint32_t)groups), dim3(NTHR), 0, st, a, p);
   }
 }
 void launch_pages_reserve(const lmoe_pages_args& a, hipStream_t st) {
   hipLaunchKernelGGL(k_pages_reserve, dim3(1), dim3(PAGES_NTHR), 0, st, a);
-  pages_copies(a, std::min<int64_t>(a.P, (int64_t)a.N * a.M), st);
+  pages_copies(a, std::min<int64_t>(a.P, (int64_t)a.N * a.M), false, st);
 }
 void launch_pages_compact(const lmoe_pages_args& a, hipStream_t st) {
   hipLaunchKernelGGL(k_pages_compact, dim3(1), dim3(PAGES_NTHR), 0, st, a);
-  const int64_t all = (int64_t)a.N * a.M;
-  if (all) hipLaunchKernelGGL(k_pages_renamed, dim3((uint32_t)std::min<int64_t>((all + NTHR - 1) / NTHR, 1024)), dim3(NTHR), 0, st, a);
-  pages_copies(a, a.P / 2, st);
+  pages_copies(a, a.P / 2, true, st);
 }
 
 }  // namespace lmoe

@@ -16,47 +16,56 @@
 
 namespace lmoe {
 
-constexpr int ROPE_HEADS = 4;          // heads of a token that a lane has in flight
-constexpr int ROPE_GROUPS = 2048, ROPE_BWD_GROUPS = 1024;        // work-groups of a launch at most (or what one token needs)
+constexpr int ROPE_FWD_HEADS = 4, ROPE_BWD_HEADS = 2;            // heads of a token that a lane has in flight
+constexpr int ROPE_GROUPS = 1 << 20, ROPE_BWD_GROUPS = 1024;     // work-groups of a launch at most (or what one token needs)
 
 struct RopePlan {
   int lanes;       // of a row
   int chunks;      // of a row: V pairs each
-  int runs;        // lane groups that share a token's heads
-  int heads;       // of them all
+  int runs_q;      // lane groups that share a token's query heads
+  int runs;        // and its key heads as well
   uint32_t grid;
 };
 
 template <typename T, int V> struct RopeVec { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct RopeVec<T, 1> { typedef T type; };
 
-// V columns each of the first (x[0 .. V - 1]) and second members of a lane's pairs
-template <typename T, int V, bool INTER> __device__ __forceinline__ void rope_load(float (&x)[2 * V], const T* row, int a, int b) {
-  typedef typename RopeVec<T, V>::type vec;
-  const vec lo = *(const vec*)(row + a), hi = *(const vec*)(row + b);
-  float y[2 * V];
-  if constexpr (V == 1) { y[0] = (float)lo; y[1] = (float)hi; }
-  else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) { y[i] = (float)lo[i]; y[V + i] = (float)hi[i]; }
+// V columns each of the first and second members of a lane's pairs, as they lie in memory
+template <typename T, int V> struct RopeRaw {
+  typename RopeVec<T, V>::type lo, hi;
+  __device__ __forceinline__ void load(const T* row, int a, int b) {
+    typedef typename RopeVec<T, V>::type vec;
+    lo = *(const vec*)(row + a);
+    hi = *(const vec*)(row + b);
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) { x[i] = INTER ? y[2 * i] : y[i]; x[V + i] = INTER ? y[2 * i + 1] : y[V + i]; }
-}
-template <typename T, int V, bool INTER> __device__ __forceinline__ void rope_store(T* row, int a, int b, const float (&x)[2 * V]) {
-  typedef typename RopeVec<T, V>::type vec;
-  float y[2 * V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) { y[INTER ? 2 * i : i] = x[i]; y[INTER ? 2 * i + 1 : V + i] = x[V + i]; }
-  vec lo, hi;
-  if constexpr (V == 1) { lo = (T)y[0]; hi = (T)y[1]; }
-  else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) { lo[i] = (T)y[i]; hi[i] = (T)y[V + i]; }
+  __device__ __forceinline__ void store(T* row, int a, int b) const {
+    typedef typename RopeVec<T, V>::type vec;
+    *(vec*)(row + a) = lo;
+    *(vec*)(row + b) = hi;
   }
-  *(vec*)(row + a) = lo;
-  *(vec*)(row + b) = hi;
-}
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (V == 1) return i ? (float)hi : (float)lo;
+    else return i < V ? (float)lo[i < V ? i : 0] : (float)hi[i < V ? 0 : i - V];
+  }
+  __device__ __forceinline__ void put(int i, float x) {
+    if constexpr (V == 1) { if (i) hi = (T)x; else lo = (T)x; }
+    else if (i < V) lo[i < V ? i : 0] = (T)x;
+    else hi[i < V ? 0 : i - V] = (T)x;
+  }
+  // the first (i < V) and second members of the pairs
+  template <bool INTER> __device__ __forceinline__ void members(float (&x)[2 * V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) { x[i] = at(INTER ? 2 * i : i); x[V + i] = at(INTER ? 2 * i + 1 : V + i); }
+  }
+  template <bool INTER> __device__ __forceinline__ void from(const float (&x)[2 * V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) { put(INTER ? 2 * i : i, x[i]); put(INTER ? 2 * i + 1 : V + i, x[V + i]); }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 2 * V; ++i) put(i, 0.f);
+  }
+};
 // the weights of a lane's columns (1 without them)
 template <int V, bool INTER> __device__ __forceinline__ void rope_weights(float (&w)[2 * V], const void* p, int dtype, int a, int b) {
 #pragma unroll
@@ -94,14 +103,19 @@ __device__ __forceinline__ bool rope_position(const lmoe_rope_args& a, int b, in
 
 template <typename T, int V, int L, int NC, bool INTER, bool BWD>
 __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, const RopePlan p) {
-  constexpr int HB = NC > 1 ? 1 : ROPE_HEADS;
+  constexpr int HB = NC > 1 ? 1 : BWD ? ROPE_BWD_HEADS : ROPE_FWD_HEADS;
+  typedef RopeRaw<T, V> Raw;
   const int l = threadIdx.x % L;
-  const int64_t group = (int64_t)blockIdx.x * (NTHR / L) + threadIdx.x / L, groups = (int64_t)gridDim.x * (NTHR / L) / p.runs;      // tokens at a time
-  const int run = (int)(group % p.runs);
+  const uint32_t group = blockIdx.x * (NTHR / L) + threadIdx.x / L, first = group / (uint32_t)p.runs;
+  const uint32_t step = gridDim.x * (NTHR / L) / (uint32_t)p.runs;      // tokens at a time
+  // a lane group takes heads of q or of k, the same ones of every token
+  const int run = (int)(group - first * p.runs);
+  const bool isq = run < p.runs_q;
+  const int h_first = isq ? run : run - p.runs_q, h_step = isq ? p.runs_q : p.runs - p.runs_q, heads = isq ? a.HQ : a.HKV;
   const int half = a.R / 2, rest = (a.D - a.R) / 2;
   int ca[NC], cb[NC], cr[NC];          // columns of the pairs' members, row of the angles (-1: not rotated)
   bool on[NC];
-  float wq[NC][2 * V], wk[NC][2 * V], sq[NC][2 * V], sk[NC][2 * V];
+  float w[NC][2 * V], sum[NC][2 * V];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
     const int c = (l + j * L) * V;
@@ -110,23 +124,23 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
     ca[j] = INTER ? 2 * c : c < half ? c : c + half;
     cb[j] = INTER ? 2 * c + V : c < half ? c + half : c + half + rest;
     if (!on[j]) ca[j] = cb[j] = 0;
+    rope_weights<V, INTER>(w[j], isq ? a.qw : a.kw, a.w_dtype, ca[j], cb[j]);
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) { wq[j][i] = wk[j][i] = 1.f; sq[j][i] = sk[j][i] = 0.f; }
-    if (on[j]) {
-      rope_weights<V, INTER>(wq[j], a.qw, a.w_dtype, ca[j], cb[j]);
-      rope_weights<V, INTER>(wk[j], a.kw, a.w_dtype, ca[j], cb[j]);
-    }
+    for (int i = 0; i < 2 * V; ++i) sum[j][i] = 0.f;
   }
+  const lmoe_tensor from = isq ? a.q : a.k, to = BWD ? (isq ? a.dq : a.dk) : (isq ? a.zq : a.zk), grad = isq ? a.dzq : a.dzk;
   const float over = 1.0f / (float)a.D;
-  const int64_t tokens = (int64_t)a.B * a.T;
-  const int64_t first = group / p.runs;
+  const uint32_t tokens = (uint32_t)a.B * (uint32_t)a.T;
   // (a group past the last whole set of runs has nothing to do; its lanes stay: sums over a row need them all)
-  for (int64_t tok0 = 0; tok0 < tokens; tok0 += groups) {
-    const int64_t tok = tok0 + first;
-    const bool mine = first < groups && tok < tokens;
-    const int b = mine ? (int)(tok / a.T) : 0, t = mine ? (int)(tok - (int64_t)b * a.T) : 0;
+  for (uint32_t tok0 = 0; tok0 < tokens; tok0 += step) {
+    const uint32_t tok = tok0 + first;
+    const bool mine = first < step && tok < tokens;
+    const int b = mine ? (int)(tok / (uint32_t)a.T) : 0, t = mine ? (int)(tok - (uint32_t)b * (uint32_t)a.T) : 0;
     int pos = -1;
     const bool live = mine && rope_position(a, b, t, pos);
+    const T* x_row = (const T*)from.ptr + b * from.sb + t * from.st;
+    const T* g_row = (const T*)grad.ptr + b * grad.sb + t * grad.st;
+    T* z_row = (T*)to.ptr + b * to.sb + t * to.st;
     float c[NC][V], s[NC][V];
 #pragma unroll
     for (int j = 0; j < NC; ++j)
@@ -136,81 +150,81 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
         c[j][i] = turn ? a.cos[(int64_t)pos * half + cr[j] + i] : 1.f;
         s[j][i] = turn ? a.sin[(int64_t)pos * half + cr[j] + i] : 0.f;
       }
-    for (int h0 = run; h0 < p.heads; h0 += HB * p.runs) {
-      float x[HB][NC][2 * V], g[HB][NC][2 * V];
+    for (int h0 = h_first; h0 < heads; h0 += HB * h_step) {
+      Raw rx[HB][NC], rg[HB][NC];
 #pragma unroll
       for (int y = 0; y < HB; ++y) {
-        const int h = h0 + y * p.runs;
-        const bool q = h < a.HQ;
-        const lmoe_tensor& from = q ? a.q : a.k;
-        const lmoe_tensor& grad = q ? a.dzq : a.dzk;
-        const int64_t hh = q ? h : h - a.HQ;
+        const int64_t h = h0 + y * h_step;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-#pragma unroll
-          for (int i = 0; i < 2 * V; ++i) x[y][j][i] = g[y][j][i] = 0.f;
-          if (!live || h >= p.heads || !on[j]) continue;
-          if (!BWD || a.norm) rope_load<T, V, INTER>(x[y][j], (const T*)from.ptr + b * from.sb + t * from.st + hh * from.sh, ca[j], cb[j]);
-          if (BWD) rope_load<T, V, INTER>(g[y][j], (const T*)grad.ptr + b * grad.sb + t * grad.st + hh * grad.sh, ca[j], cb[j]);
+          rx[y][j].clear();
+          rg[y][j].clear();
+          if (!live || h >= heads || !on[j]) continue;
+          if (!BWD || a.norm) rx[y][j].load(x_row + h * from.sh, ca[j], cb[j]);
+          if (BWD) rg[y][j].load(g_row + h * grad.sh, ca[j], cb[j]);
         }
       }
 #pragma unroll
       for (int y = 0; y < HB; ++y) {
-        const int h = h0 + y * p.runs;
-        const bool q = h < a.HQ;
+        const int64_t h = h0 + y * h_step;
+        float x[NC][2 * V], z[NC][2 * V];
         float r = 1.f;
         if (a.norm) {
           float ss = 0.f;
 #pragma unroll
-          for (int j = 0; j < NC; ++j)
+          for (int j = 0; j < NC; ++j) {
+            rx[y][j].template members<INTER>(x[j]);
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) ss += x[y][j][i] * x[y][j][i];
+            for (int i = 0; i < 2 * V; ++i) ss += x[j][i] * x[j][i];
+          }
           r = rsqrt_fast(lanes_of_row<L>(ss) * over + a.eps);
+        } else {
+#pragma unroll
+          for (int j = 0; j < NC; ++j) rx[y][j].template members<INTER>(x[j]);
         }
-        float z[NC][2 * V];
         if constexpr (!BWD) {
 #pragma unroll
           for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const float ya = x[y][j][i] * r * (q ? wq[j][i] : wk[j][i]), yb = x[y][j][V + i] * r * (q ? wq[j][V + i] : wk[j][V + i]);
+              const float ya = x[j][i] * r * w[j][i], yb = x[j][V + i] * r * w[j][V + i];
               z[j][i] = ya * c[j][i] - yb * s[j][i];
               z[j][V + i] = yb * c[j][i] + ya * s[j][i];
             }
         } else {
           float m = 0.f;
 #pragma unroll
-          for (int j = 0; j < NC; ++j)
+          for (int j = 0; j < NC; ++j) {
+            float g[2 * V];
+            rg[y][j].template members<INTER>(g);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const float ga = g[y][j][i] * c[j][i] + g[y][j][V + i] * s[j][i], gb = g[y][j][V + i] * c[j][i] - g[y][j][i] * s[j][i];
-              const float xa = x[y][j][i] * r, xb = x[y][j][V + i] * r;
-              if (q) { sq[j][i] += ga * xa; sq[j][V + i] += gb * xb; }
-              else { sk[j][i] += ga * xa; sk[j][V + i] += gb * xb; }
-              z[j][i] = ga * (q ? wq[j][i] : wk[j][i]);
-              z[j][V + i] = gb * (q ? wq[j][V + i] : wk[j][V + i]);
+              const float ga = g[i] * c[j][i] + g[V + i] * s[j][i], gb = g[V + i] * c[j][i] - g[i] * s[j][i];
+              const float xa = x[j][i] * r, xb = x[j][V + i] * r;
+              sum[j][i] += ga * xa;
+              sum[j][V + i] += gb * xb;
+              z[j][i] = ga * w[j][i];
+              z[j][V + i] = gb * w[j][V + i];
               m += z[j][i] * xa + z[j][V + i] * xb;
-              x[y][j][i] = xa; x[y][j][V + i] = xb;
+              x[j][i] = xa; x[j][V + i] = xb;
             }
+          }
           if (a.norm) {
             m = lanes_of_row<L>(m) * over;
 #pragma unroll
             for (int j = 0; j < NC; ++j)
 #pragma unroll
-              for (int i = 0; i < 2 * V; ++i) z[j][i] = r * (z[j][i] - x[y][j][i] * m);
+              for (int i = 0; i < 2 * V; ++i) z[j][i] = r * (z[j][i] - x[j][i] * m);
           }
         }
-        if (!mine || h >= p.heads) continue;
-        const lmoe_tensor& to = BWD ? (q ? a.dq : a.dk) : (q ? a.zq : a.zk);
-        T* row = (T*)to.ptr + b * to.sb + t * to.st + (int64_t)(q ? h : h - a.HQ) * to.sh;
+        if (!mine || h >= heads) continue;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
           if (!on[j]) continue;
-          if (!live) {
-#pragma unroll
-            for (int i = 0; i < 2 * V; ++i) z[j][i] = 0.f;
-          }
-          rope_store<T, V, INTER>(row, ca[j], cb[j], z[j]);
+          Raw out;
+          out.template from<INTER>(z[j]);
+          if (!live) out.clear();
+          out.store(z_row + h * to.sh, ca[j], cb[j]);
         }
       }
     }
@@ -219,18 +233,18 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
     // dw: the lane groups of a wave, then the waves, then a row of ws per work-group
     if (!a.ws) return;
     __shared__ float part[NTHR / 64][2][256];
-    const int w = wave_id();
+    const int wv = wave_id();
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
       for (int i = 0; i < 2 * V; ++i) {
-        float x = sq[j][i], y = sk[j][i];
+        float x = isq ? sum[j][i] : 0.f, y = isq ? 0.f : sum[j][i];
 #pragma unroll
         for (int d = L; d < 64; d <<= 1) { x += __shfl_xor(x, d, 64); y += __shfl_xor(y, d, 64); }
         if (lane_id() < L && on[j]) {
           const int e = i < V ? i : i - V, col = INTER ? ca[j] + 2 * e + (i >= V) : (i < V ? ca[j] : cb[j]) + e;
-          part[w][0][col] = x;
-          part[w][1][col] = y;
+          part[wv][0][col] = x;
+          part[wv][1][col] = y;
         }
       }
     __syncthreads();
@@ -241,22 +255,25 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
   }
 }
 
-// dw: the rows of ws, a work-group per 32 columns (of dqw and dkw in a row), 8 rows at a time
+// dw: the rows of ws, a work-group per four columns (of dqw and dkw in a row)
 __global__ __launch_bounds__(NTHR) void k_qk_norm_dw(const lmoe_rope_args a, int rows) {
-  __shared__ float s[8][32];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
-  float x = 0.f;
-  if (col < 2 * a.D)
-    for (int i = r; i < rows; i += 8) x += a.ws[(int64_t)i * 2 * a.D + col];
-  s[r][c] = x;
-  __syncthreads();
-  if (r || col >= 2 * a.D) return;
+  __shared__ f32x4 s_x[NTHR / 64];
+  const int col = blockIdx.x * 4;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int i = threadIdx.x; i < rows; i += NTHR) x += *(const f32x4*)(a.ws + (int64_t)i * 2 * a.D + col);
 #pragma unroll
-  for (int i = 1; i < 8; ++i) x += s[i][c];
-  void* to = col < a.D ? a.dqw : a.dkw;
-  const int at = col < a.D ? col : col - a.D;
+  for (int e = 0; e < 4; ++e) x[e] = wave_sum(x[e]);
+  if (lane_id() == 0) s_x[threadIdx.x >> 6] = x;
+  __syncthreads();
+  if (threadIdx.x >= 4) return;
+  const int at = col + threadIdx.x;
+  float y = 0.f;
+#pragma unroll
+  for (int i = 0; i < NTHR / 64; ++i) y += s_x[i][threadIdx.x];
+  void* to = at < a.D ? a.dqw : a.dkw;
+  const int e = at < a.D ? at : at - a.D;
   if (!to) return;
-  if (a.w_dtype == LMOE_F32) ((float*)to)[at] = x; else ((bf16*)to)[at] = (bf16)x;
+  if (a.w_dtype == LMOE_F32) ((float*)to)[e] = y; else ((bf16*)to)[e] = (bf16)y;
 }
 
 // Whether every row can be read in 16-byte pieces that hold whole pairs' members
@@ -275,19 +292,21 @@ static RopePlan rope_plan(const lmoe_rope_args& a, bool bwd) {
   p.lanes = 4;
   while (p.lanes < 64 && p.lanes < p.chunks) p.lanes *= 2;
   if (v == 1) p.lanes = 64;
-  p.heads = a.HQ + a.HKV;
-  const int64_t tokens = (int64_t)a.B * a.T, per = NTHR / p.lanes;
+  const int64_t tokens = (int64_t)a.B * a.T, per = NTHR / p.lanes, heads = (int64_t)a.HQ + a.HKV;
   // a head for each lane group while that leaves the card empty, else several
-  const bool few = tokens * p.heads <= 256 * 8 * per;
-  p.runs = few || v == 1 ? p.heads : (p.heads + ROPE_HEADS - 1) / ROPE_HEADS;
-  const int64_t want = (tokens * p.runs + per - 1) / per, least = (p.runs + per - 1) / per;
-  p.grid = (uint32_t)std::max(std::min<int64_t>(want, bwd ? ROPE_BWD_GROUPS : ROPE_GROUPS), least);
+  const int hb = v == 1 || tokens * heads <= 256 * 8 * per ? 1 : bwd ? ROPE_BWD_HEADS : ROPE_FWD_HEADS;
+  p.runs_q = (a.HQ + hb - 1) / hb;
+  p.runs = p.runs_q + (a.HKV + hb - 1) / hb;
+  // as many tokens for every lane group
+  const int64_t items = tokens * p.runs, most = bwd ? ROPE_BWD_GROUPS : ROPE_GROUPS;
+  const int64_t each = (items + most * per - 1) / (most * per), sets = (tokens + each - 1) / each;
+  p.grid = (uint32_t)((sets * p.runs + per - 1) / per);
   return p;
 }
 // (as many rows as a call of these sizes has work-groups at most, however its tensors lie)
 int64_t rope_floats(const lmoe_rope_args& a) {
   const int64_t heads = (int64_t)a.HQ + a.HKV, rows = (int64_t)a.B * a.T * heads;
-  return std::max(std::min<int64_t>(ROPE_BWD_GROUPS, rows), heads) * 2 * a.D;
+  return (std::min<int64_t>(ROPE_BWD_GROUPS, rows) + heads) * 2 * a.D;
 }
 
 template <typename T, int V, int L, int NC, bool BWD> static void rope_launch(const lmoe_rope_args& a, const RopePlan& p, hipStream_t st) {
@@ -308,7 +327,7 @@ void launch_qk_norm_rope(const lmoe_rope_args& a, bool bwd, hipStream_t st) {
   else if (bwd) rope_typed<float, true>(a, p, st);
   else rope_typed<float, false>(a, p, st);
   if (bwd && (a.dqw || a.dkw))
-    hipLaunchKernelGGL(k_qk_norm_dw, dim3((2 * a.D + 31) / 32), dim3(NTHR), 0, st, a, (int)p.grid);
+    hipLaunchKernelGGL(k_qk_norm_dw, dim3(a.D / 2), dim3(NTHR), 0, st, a, (int)p.grid);
 }
 
 }  // namespace lmoe
