@@ -244,8 +244,8 @@ __device__ __forceinline__ void pv4(f32x4 (&o)[W / 16], const Tile4<W>& t, const
   ET<T>::mma(o[2 * B + 1], hi, pf);
 }
 
-// EVEN: 16 adjacent positions lie in one page (S a multiple of 16; no stride of a token passes 2^27 bytes), so that a step's rows are two
-// bases in scalar registers and offsets that stay the same; else every position's page is looked up by a lane and passed round.
+// EVEN: 16 adjacent positions lie in one page (S a multiple of 16) and offsets inside a page and strides of pages hold in 32 bits, so that a
+// step's rows are two bases in scalar registers and offsets that stay the same; else every position's page is looked up by a lane and passed round.
 template <typename T, int W, int NW, bool EVEN, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
   const lmoe_paged_args& a = a4.p;
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   const PagedSeq sq = paged_seq(a, p, n);
   const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = part * sq.chunk;
   if (begin >= total && part > 0) return;
-  const int stop = min(total, begin + sq.chunk), end = min(stop, sq.len);       // the stretch, and its part in the cache
+  const int stop = min(total, begin + sq.chunk), end = a.P > 0 ? min(stop, sq.len) : begin;       // the stretch, and its part in the cache
   const int l = lane_id(), w = wave_id(), c = l & 15, g = l >> 4;
   const int32_t* table = a.table + (int64_t)n * a.table_stride;
   const uint8_t* kp = (const uint8_t*)a.kp.ptr + (int64_t)hk * a.kp.sh;
@@ -299,10 +299,14 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
     return x;
   };
   const uint32_t kst = (uint32_t)a.kp.st, vst = (uint32_t)a.vp.st, kss = (uint32_t)a4.ks.st, vss = (uint32_t)a4.vs.st;
+  // (columns behind the head dimension: the row's first, which no output and no product other than by 0 sees)
+  const uint32_t kc = kin ? KC * g : 0, vc = vin ? VW * c : 0;
   uint32_t vo[4], vso[4];               // EVEN: offsets of the lane's keys of V inside a half, and c's of K
 #pragma unroll
-  for (int e = 0; e < 4; ++e) { vo[e] = (4 * g + e) * vst + VW / 2 * c; vso[e] = (4 * g + e) * vss + VW * c / 32; }
-  const uint32_t ko = c * kst + KC / 2 * g, kso = c * kss + KC * g / 32;
+  for (int e = 0; e < 4; ++e) { vo[e] = (4 * g + e) * vst + vc / 2; vso[e] = (4 * g + e) * vss + vc / 32; }
+  const uint32_t ko = c * kst + kc / 2, kso = c * kss + kc / 32;
+  // A step's rows are asked for without a condition, so that waiting for one step's leaves the next one's in flight: positions that do not
+  // exist read a slot that does (behind the end: of their page; without a page: of page 0), and take() leaves them out.
   auto load = [&](Tile& t, int j0, const Where& x) {
     auto k_row = [&](int b, const uint8_t* codes, const uint8_t* scale) {
       const words y = *(const words*)codes;
@@ -314,61 +318,36 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
       if constexpr (VW == 8) t.v[e] = *(const uint32_t*)codes; else t.v[e] = *(const uint16_t*)codes;
       t.vs[e] = *scale;
     };
-    auto nothing = [&]() {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int i = 0; i < KW; ++i) t.k[b][i] = 0;
-        t.ks[b] = 127;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { t.v[e] = 0; t.vs[e] = 127; }
-    };
     if constexpr (EVEN) {
-      bool there[2];
-      const uint8_t *kb[2], *vb[2], *ksb[2], *vsb[2];
-      uint32_t live = 0;
+      const uint8_t *vb[2], *vsb[2];
+      t.live = 0;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        there[b] = x.id[b] >= 0 && x.id[b] < a.P;
-        const int64_t id = there[b] ? x.id[b] : 0, slot = x.slot[b];
-        kb[b] = kp + id * a.kp.sb + slot * a.kp.st;
-        vb[b] = vp + id * a.vp.sb + slot * a.vp.st;
-        ksb[b] = ksp + id * a4.ks.sb + slot * a4.ks.st;
-        vsb[b] = vsp + id * a4.vs.sb + slot * a4.vs.st;
+        const bool there = x.id[b] >= 0 && x.id[b] < a.P;
+        const uint32_t id = there ? x.id[b] : 0, slot = there ? x.slot[b] : 0;
+        auto row = [&](const uint8_t* base, const lmoe_tensor& y) { return base + (uint64_t)id * (uint32_t)y.sb + slot * (uint32_t)y.st; };
+        k_row(b, row(kp, a.kp) + ko, row(ksp, a4.ks) + kso);
+        vb[b] = row(vp, a.vp);
+        vsb[b] = row(vsp, a4.vs);
         const int left = min(16, end - j0 - 16 * b);          // positions of the half
-        if (there[b] && left > 0) live |= ((1u << left) - 1) << (16 * b);
+        if (there) t.live |= ((1u << left) - 1) << (16 * b);
       }
-      t.live = live;
-      if (live == ~0u && (KC * 4 == a.K) && (VW * 16 == a.V)) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) k_row(b, kb[b] + ko, ksb[b] + kso);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v_row(e, vb[e >> 2] + vo[e & 3], vsb[e >> 2] + vso[e & 3]);
-      } else {
-        nothing();
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          if (kin && (live >> (16 * b + c) & 1)) k_row(b, kb[b] + ko, ksb[b] + kso);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (vin && (live >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) v_row(e, vb[e >> 2] + vo[e & 3], vsb[e >> 2] + vso[e & 3]);
-      }
+      for (int e = 0; e < 8; ++e) v_row(e, vb[e >> 2] + vo[e & 3], vsb[e >> 2] + vso[e & 3]);
     } else {
-      t.live = (uint32_t)__ballot(x.id[0] >= 0 && x.id[0] < a.P);
-      nothing();
+      const bool there = x.id[0] >= 0 && x.id[0] < a.P;
+      t.live = (uint32_t)__ballot(there);
+      const int my_id = there ? x.id[0] : 0, my_slot = there ? x.slot[0] : 0;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int64_t id = __shfl(x.id[0], 16 * b + c, 64), slot = __shfl(x.slot[0], 16 * b + c, 64);
-        if ((t.live >> (16 * b + c) & 1) && kin)
-          k_row(b, kp + id * a.kp.sb + slot * a.kp.st + KC / 2 * g, ksp + id * a4.ks.sb + slot * a4.ks.st + KC * g / 32);
+        const int64_t id = __shfl(my_id, 16 * b + c, 64), slot = __shfl(my_slot, 16 * b + c, 64);
+        k_row(b, kp + id * a.kp.sb + slot * a.kp.st + kc / 2, ksp + id * a4.ks.sb + slot * a4.ks.st + kc / 32);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int at = 16 * (e >> 2) + 4 * g + (e & 3);
-        const int64_t id = __shfl(x.id[0], at, 64), slot = __shfl(x.slot[0], at, 64);
-        if ((t.live >> at & 1) && vin)
-          v_row(e, vp + id * a.vp.sb + slot * a.vp.st + VW / 2 * c, vsp + id * a4.vs.sb + slot * a4.vs.st + VW * c / 32);
+        const int64_t id = __shfl(my_id, at, 64), slot = __shfl(my_slot, at, 64);
+        v_row(e, vp + id * a.vp.sb + slot * a.vp.st + vc / 2, vsp + id * a4.vs.sb + slot * a4.vs.st + vc / 32);
       }
     }
   };
@@ -389,7 +368,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
 #pragma unroll
   for (int i = 0; i < VW; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = M_LOW, sum = 0.f;
-  auto take = [&](const Tile& t, int j0) {
+  auto take = [&](Tile& t, int j0) {
     f32x4 s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -409,7 +388,12 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[b][e] = t.live >> (16 * b + 4 * g + e) & 1 ? s[b][e] : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          const bool on = t.live >> (16 * b + 4 * g + e) & 1;
+          s[b][e] = on ? s[b][e] : -INFINITY;
+          t.v[4 * b + e] = on ? t.v[4 * b + e] : 0;             // (whatever lies there, 0 times it is 0)
+          t.vs[4 * b + e] = on ? t.vs[4 * b + e] : 127;
+        }
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -490,27 +474,24 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
         if (VW * c % 32 == 0) ((uint8_t*)vsp)[(int64_t)id * a4.vs.sb + (int64_t)slot * a4.vs.st + VW * c / 32] = (uint8_t)y.vs[0];
       }
     }
-    if (c != 0) {                     // (the other keys of the 16 and their scales: nothing)
-#pragma unroll
-      for (int j = 0; j < KW; ++j) y.k[0][j] = 0;
-      y.ks[0] = 127;
-    }
-    if (g != 0) { y.v[0] = 0; y.vs[0] = 127; }
     take(y, sq.len);
   }
-  if (j0 < end) load(t[0], j0, at);
-  while (j0 < end) {
-    at = ahead;
-    ahead = ask(j0 + 2 * PGROUP);
-    if (j0 + PGROUP < end) load(t[1], j0 + PGROUP, at);
-    take(t[0], j0);
-    j0 += PGROUP;
-    if (j0 >= end) break;
-    at = ahead;
-    ahead = ask(j0 + 2 * PGROUP);
-    if (j0 + PGROUP < end) load(t[0], j0 + PGROUP, at);
-    take(t[1], j0);
-    j0 += PGROUP;
+  if (j0 < end) {
+    load(t[0], j0, at);
+    for (;;) {
+      at = ahead;
+      ahead = ask(j0 + 2 * PGROUP);
+      load(t[1], j0 + PGROUP, at);
+      take(t[0], j0);
+      j0 += PGROUP;
+      if (j0 >= end) break;
+      at = ahead;
+      ahead = ask(j0 + 2 * PGROUP);
+      load(t[0], j0 + PGROUP, at);
+      take(t[1], j0);
+      j0 += PGROUP;
+      if (j0 >= end) break;
+    }
   }
 
   // the waves together: lane (c, g) holds head c, columns VW (4g + r) + i
@@ -556,7 +537,7 @@ template <typename T, int W, int NW, bool EVEN> static void paged4_parts(const l
 }
 template <typename T, int W> static void paged4_wide(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
   bool even = a.p.S % 16 == 0;
-  for (const lmoe_tensor* t : {&a.p.kp, &a.p.vp, &a.ks, &a.vs}) even = even && t->st < 1 << 27;
+  for (const lmoe_tensor* t : {&a.p.kp, &a.p.vp, &a.ks, &a.vs}) even = even && t->sb >> 32 == 0 && t->st < 1ll << 27 && (a.p.S * t->st) >> 32 == 0;
   if (p.waves == 8) {
     if (even) paged4_parts<T, W, 8, true>(a, p, st); else paged4_parts<T, W, 8, false>(a, p, st);
   } else if (even) paged4_parts<T, W, 4, true>(a, p, st);
