@@ -61,15 +61,19 @@ template <typename T> __device__ __forceinline__ typename ET<T>::frag from4(uint
   }
 }
 template <typename T> __device__ __forceinline__ float size_of(const typename ET<T>::frag& x) {
-  float m = 0.f;
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = larger(m, fabsf((float)x[i]));
+  if constexpr (sizeof(T) == 2) {          // (as whole numbers, two at a time: the order of their bits is that of the sizes)
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 y = __builtin_bit_cast(u32x4, x) & 0x7fff7fffu;
+    auto two = [](uint32_t z) { return __builtin_bit_cast(u16x2, z); };
+    const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(two(y[0]), two(y[1])), __builtin_elementwise_max(two(y[2]), two(y[3])));
+    return __builtin_bit_cast(float, (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16);
   } else {
+    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) m = larger(m, larger(fabsf(x.lo[i]), fabsf(x.hi[i])));
+    return m;
   }
-  return m;
 }
 template <typename T> __device__ __forceinline__ void store_frag(T* p, const typename ET<T>::frag& x) {
   if constexpr (sizeof(T) == 2) *(bf16x8*)p = x; else { *(f32x4*)p = x.lo; *(f32x4*)(p + 4) = x.hi; }
@@ -108,86 +112,144 @@ __device__ __forceinline__ int paged_slot(const lmoe_paged_args& a, const PagedT
   return id < 0 || id >= a.P ? -1 : id;
 }
 
-template <typename T> __global__ __launch_bounds__(NTHR) void k_paged4_append(const lmoe_paged4_args a4) {
+// The lanes of a wave go over the pieces (VEC columns) of a token's rows of k and of v, PIECES of each in flight for a lane.
+constexpr int PIECES = 2;
+struct TokenPlan {
+  int nk, nv;              // pieces of k and of v
+  uint32_t div_k, div_v;   // i / (pieces of a row) = umulhi(2 i, div) for i < 2^20
+};
+static TokenPlan token_plan(const lmoe_paged_args& a, int vec) {
+  const int pk = a.K / vec, pv = a.V / vec;
+  return {a.HKV * pk, a.HKV * pv, (uint32_t)((1ull << 31) / pk + 1), (uint32_t)((1ull << 31) / pv + 1)};
+}
+// pieces i0 + l + 64 u of a side (k or v): heads and places in a row
+struct Side {
+  int n, per;
+  uint32_t div;
+  int h[PIECES], c[PIECES];
+  bool on[PIECES];
+  __device__ __forceinline__ Side(int n, int per, uint32_t div) : n(n), per(per), div(div) {}
+  __device__ __forceinline__ void go(int i0) {
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
+      const int i = i0 + 64 * u + lane_id();
+      on[u] = i < n;
+      h[u] = (int)__umulhi(2 * (uint32_t)i, div);
+      c[u] = i - h[u] * per;
+    }
+  }
+};
+// the largest of four neighbouring lanes
+__device__ __forceinline__ float quad_larger(float x) {
+  x = larger(x, dpp_or_zero<0xB1, 0xf>(x));
+  return larger(x, dpp_or_zero<0x4E, 0xf>(x));
+}
+
+template <typename T> __global__ __launch_bounds__(NTHR) void k_paged4_append(const lmoe_paged4_args a4, const TokenPlan p) {
+  typedef typename ET<T>::frag frag;
   const lmoe_paged_args& a = a4.p;
   const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
   if (tok >= (int64_t)a.B * a.T) return;
+  const int b = a.cu_seqlens ? 0 : (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
+  const T* kn = (const T*)a.kn.ptr + (int64_t)b * a.kn.sb + (int64_t)t * a.kn.st;
+  const T* vn = (const T*)a.vn.ptr + (int64_t)b * a.vn.sb + (int64_t)t * a.vn.st;
+  Side sk(p.nk, a.K / 8, p.div_k), sv(p.nv, a.V / 8, p.div_v);                  // four pieces share a scale
+  frag yk[PIECES], yv[PIECES];
+  auto load = [&](Side& s, frag (&y)[PIECES], const T* row, int64_t sh, int i0) {
+    s.go(i0);
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
+      y[u] = zero_frag<T>();
+      if (s.on[u]) y[u] = ET<T>::load_frag(row + s.h[u] * sh + 8 * s.c[u]);
+    }
+  };
+  // (the rows are asked for before their place is)
+  load(sk, yk, kn, a.kn.sh, 0);
+  load(sv, yv, vn, a.vn.sh, 0);
   PagedToken x;
   if (!paged_token(a, tok, x)) return;
   int slot;
   const int id = paged_slot(a, x, slot);
   if (id < 0) return;
-  const int l = lane_id();
-  auto write = [&](const lmoe_tensor& from, const lmoe_tensor& to, const lmoe_tensor& scales, int D) {
-    const T* s = (const T*)from.ptr + (int64_t)x.b * from.sb + (int64_t)x.t * from.st;
-    uint8_t* d = (uint8_t*)to.ptr + (int64_t)id * to.sb + (int64_t)slot * to.st;
+  auto store = [&](const Side& s, const frag (&y)[PIECES], const lmoe_tensor& codes, const lmoe_tensor& scales) {
+    uint8_t* d = (uint8_t*)codes.ptr + (int64_t)id * codes.sb + (int64_t)slot * codes.st;
     uint8_t* e = (uint8_t*)scales.ptr + (int64_t)id * scales.sb + (int64_t)slot * scales.st;
-    const int per = D / 8;                 // lanes of a row: four for each scale
-    for (int i0 = 0; i0 < a.HKV * per; i0 += 64) {
-      const int i = i0 + l, h = i / per, c = i % per;
-      const bool on = i < a.HKV * per;
-      typename ET<T>::frag y = zero_frag<T>();
-      if (on) y = ET<T>::load_frag(s + (int64_t)h * from.sh + 8 * c);
-      float most = size_of<T>(y);
-      most = larger(most, __shfl_xor(most, 1, 64));
-      most = larger(most, __shfl_xor(most, 2, 64));
-      const uint32_t sc = scale4(most);
-      if (!on) continue;
-      *(uint32_t*)(d + (int64_t)h * to.sh + 4 * c) = to4<T>(y, scale_of(sc));
-      if ((c & 3) == 0) e[(int64_t)h * scales.sh + (c >> 2)] = (uint8_t)sc;
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
+      const uint32_t sc = scale4(quad_larger(size_of<T>(y[u])));
+      if (!s.on[u]) continue;
+      *(uint32_t*)(d + s.h[u] * codes.sh + 4 * s.c[u]) = to4<T>(y[u], scale_of(sc));
+      if ((s.c[u] & 3) == 0) e[s.h[u] * scales.sh + (s.c[u] >> 2)] = (uint8_t)sc;
     }
   };
-  write(a.kn, a.kp, a4.ks, a.K);
-  write(a.vn, a.vp, a4.vs, a.V);
+  store(sk, yk, a.kp, a4.ks);
+  store(sv, yv, a.vp, a4.vs);
+  for (int i0 = 64 * PIECES; i0 < max(p.nk, p.nv); i0 += 64 * PIECES) {
+    load(sk, yk, kn, a.kn.sh, i0);
+    load(sv, yv, vn, a.vn.sh, i0);
+    store(sk, yk, a.kp, a4.ks);
+    store(sv, yv, a.vp, a4.vs);
+  }
 }
 
 // BITS4: of a cache in 4 bits, else of elements of the same type
-template <typename T, bool BITS4> __global__ __launch_bounds__(NTHR) void k_paged_read(const lmoe_paged4_args a4) {
+template <typename T, bool BITS4> __global__ __launch_bounds__(NTHR) void k_paged_read(const lmoe_paged4_args a4, const TokenPlan p) {
   constexpr int VEC = BITS4 ? 8 : ET<T>::VEC;
+  typedef typename ET<T>::vec vec;
   const lmoe_paged_args& a = a4.p;
   const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
   if (tok >= (int64_t)a.B * a.T) return;
+  const int b = a.cu_seqlens ? 0 : (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
   PagedToken x;
   int slot = 0, id = -1;
   if (paged_token(a, tok, x)) id = paged_slot(a, x, slot);
-  const int l = lane_id();
-  auto read = [&](const lmoe_tensor& from, const lmoe_tensor& scales, const lmoe_tensor& to, int D) {
-    T* d = (T*)to.ptr + (int64_t)x.b * to.sb + (int64_t)x.t * to.st;
-    const int64_t page = id < 0 ? 0 : id;
-    const int per = D / VEC;
-    for (int i = l; i < a.HKV * per; i += 64) {
-      const int h = i / per, c = i % per;
-      T* row = d + (int64_t)h * to.sh + VEC * c;
+  Side sk(p.nk, a.K / VEC, p.div_k), sv(p.nv, a.V / VEC, p.div_v);
+  struct Held { uint32_t r, scale; vec y; } hk[PIECES], hv[PIECES];
+  auto load = [&](Side& s, Held (&y)[PIECES], const lmoe_tensor& codes, const lmoe_tensor& scales, int i0) {
+    s.go(i0);
+    const int64_t page = id < 0 ? 0 : id, at = page * codes.sb + (int64_t)slot * codes.st;
+    const uint8_t* e = (const uint8_t*)scales.ptr + page * scales.sb + (int64_t)slot * scales.st;
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
+      y[u].r = 0; y[u].scale = 127; y[u].y = ET<T>::zero();
+      if (!s.on[u] || id < 0) continue;
       if constexpr (BITS4) {
-        typename ET<T>::frag y = zero_frag<T>();
-        if (id >= 0) {
-          const uint32_t r = *(const uint32_t*)((const uint8_t*)from.ptr + page * from.sb + (int64_t)slot * from.st + (int64_t)h * from.sh + 4 * c);
-          y = from4<T>(r, scale_of(*((const uint8_t*)scales.ptr + page * scales.sb + (int64_t)slot * scales.st + (int64_t)h * scales.sh + (c >> 2))));
-        }
-        store_frag<T>(row, y);
-      } else {
-        typename ET<T>::vec y = ET<T>::zero();
-        if (id >= 0) y = *(const typename ET<T>::vec*)((const T*)from.ptr + page * from.sb + (int64_t)slot * from.st + (int64_t)h * from.sh + VEC * c);
-        *(typename ET<T>::vec*)row = y;
-      }
+        y[u].r = *(const uint32_t*)((const uint8_t*)codes.ptr + at + s.h[u] * codes.sh + 4 * s.c[u]);
+        y[u].scale = e[s.h[u] * scales.sh + (s.c[u] >> 2)];
+      } else y[u].y = *(const vec*)((const T*)codes.ptr + at + s.h[u] * codes.sh + VEC * s.c[u]);
     }
   };
-  read(a.kp, a4.ks, a.kn, a.K);
-  read(a.vp, a4.vs, a.vn, a.V);
+  auto store = [&](const Side& s, const Held (&y)[PIECES], const lmoe_tensor& to) {
+    T* row = (T*)to.ptr + (int64_t)b * to.sb + (int64_t)t * to.st;
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) {
+      if (!s.on[u]) continue;
+      T* d = row + s.h[u] * to.sh + VEC * s.c[u];
+      if constexpr (BITS4) store_frag<T>(d, from4<T>(y[u].r, scale_of(y[u].scale))); else *(vec*)d = y[u].y;
+    }
+  };
+  for (int i0 = 0; i0 < max(p.nk, p.nv); i0 += 64 * PIECES) {
+    load(sk, hk, a.kp, a4.ks, i0);
+    load(sv, hv, a.vp, a4.vs, i0);
+    store(sk, hk, a.kn);
+    store(sv, hv, a.vn);
+  }
 }
 
 static uint32_t token_groups(const lmoe_paged_args& a) { return (uint32_t)(((int64_t)a.B * a.T + NTHR / 64 - 1) / (NTHR / 64)); }
 void launch_paged4_append(const lmoe_paged4_args& a, hipStream_t st) {
-  if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged4_append<bf16>), dim3(token_groups(a.p)), dim3(NTHR), 0, st, a);
-  else hipLaunchKernelGGL((k_paged4_append<float>), dim3(token_groups(a.p)), dim3(NTHR), 0, st, a);
+  const TokenPlan p = token_plan(a.p, 8);
+  if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged4_append<bf16>), dim3(token_groups(a.p)), dim3(NTHR), 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged4_append<float>), dim3(token_groups(a.p)), dim3(NTHR), 0, st, a, p);
 }
 void launch_paged_read(const lmoe_paged4_args& a, bool bits4, hipStream_t st) {
   const dim3 grid(token_groups(a.p)), block(NTHR);
+  const TokenPlan p = token_plan(a.p, bits4 || a.p.dtype == LMOE_BF16 ? 8 : 4);
   if (bits4) {
-    if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_read<bf16, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_paged_read<float, true>), grid, block, 0, st, a);
-  } else if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_read<bf16, false>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((k_paged_read<float, false>), grid, block, 0, st, a);
+    if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_read<bf16, true>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged_read<float, true>), grid, block, 0, st, a, p);
+  } else if (a.p.dtype == LMOE_BF16) hipLaunchKernelGGL((k_paged_read<bf16, false>), grid, block, 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged_read<float, false>), grid, block, 0, st, a, p);
 }
 
 // ---- one new token ----

@@ -16,7 +16,7 @@
 
 namespace lmoe {
 
-constexpr int ROPE_FWD_HEADS = 4, ROPE_BWD_HEADS = 2;            // heads of a token that a lane has in flight
+constexpr int ROPE_FWD_HEADS = 4, ROPE_BWD_HEADS = 4;            // heads of a token that a lane has in flight
 constexpr int ROPE_GROUPS = 1 << 20, ROPE_BWD_GROUPS = 1024;     // work-groups of a launch at most (or what one token needs)
 
 struct RopePlan {
@@ -76,9 +76,11 @@ template <int V, bool INTER> __device__ __forceinline__ void rope_weights(float 
   }
 }
 
+// the sum over the lanes of a row (of which all or none are at work)
 template <int L> __device__ __forceinline__ float lanes_of_row(float x) {
+  x = group_sum<(L < 16 ? L : 16)>(x);
 #pragma unroll
-  for (int d = 1; d < L; d <<= 1) x += __shfl_xor(x, d, 64);
+  for (int d = 16; d < L; d <<= 1) x += __shfl_xor(x, d, 64);
   return x;
 }
 
