@@ -16,14 +16,16 @@
 
 namespace lmoe {
 
-constexpr int ROPE_FWD_HEADS = 4, ROPE_BWD_HEADS = 4;            // heads of a token that a lane has in flight
-constexpr int ROPE_GROUPS = 1 << 20, ROPE_BWD_GROUPS = 1024;     // work-groups of a launch at most (or what one token needs)
+constexpr int ROPE_HEADS = 4;                                    // heads of a token that a lane has in flight
+constexpr int ROPE_GROUPS = 1 << 20, ROPE_BWD_GROUPS = 2048;     // work-groups of a launch at most (or what one token needs)
 
 struct RopePlan {
   int lanes;       // of a row
   int chunks;      // of a row: V pairs each
   int runs_q;      // lane groups that share a token's query heads
   int runs;        // and its key heads as well
+  bool full;       // every lane of a row has columns
+  bool past;       // the results go past the caches
   uint32_t grid;
 };
 
@@ -38,10 +40,15 @@ template <typename T, int V> struct RopeRaw {
     lo = *(const vec*)(row + a);
     hi = *(const vec*)(row + b);
   }
-  __device__ __forceinline__ void store(T* row, int a, int b) const {
+  __device__ __forceinline__ void store(T* row, int a, int b, bool past) const {
     typedef typename RopeVec<T, V>::type vec;
-    *(vec*)(row + a) = lo;
-    *(vec*)(row + b) = hi;
+    if (past) {
+      __builtin_nontemporal_store(lo, (vec*)(row + a));
+      __builtin_nontemporal_store(hi, (vec*)(row + b));
+    } else {
+      *(vec*)(row + a) = lo;
+      *(vec*)(row + b) = hi;
+    }
   }
   __device__ __forceinline__ float at(int i) const {
     if constexpr (V == 1) return i ? (float)hi : (float)lo;
@@ -68,11 +75,30 @@ template <typename T, int V> struct RopeRaw {
 };
 // the weights of a lane's columns (1 without them)
 template <int V, bool INTER> __device__ __forceinline__ void rope_weights(float (&w)[2 * V], const void* p, int dtype, int a, int b) {
+  if (!p) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int ia = INTER ? a + 2 * i : a + i, ib = INTER ? a + 2 * i + 1 : b + i;
-    w[i] = !p ? 1.f : dtype == LMOE_F32 ? ((const float*)p)[ia] : (float)((const bf16*)p)[ia];
-    w[V + i] = !p ? 1.f : dtype == LMOE_F32 ? ((const float*)p)[ib] : (float)((const bf16*)p)[ib];
+    for (int i = 0; i < 2 * V; ++i) w[i] = 1.f;
+  } else if (dtype == LMOE_F32) {
+    RopeRaw<float, V> x;
+    x.load((const float*)p, a, b);
+    x.template members<INTER>(w);
+  } else {
+    RopeRaw<bf16, V> x;
+    x.load((const bf16*)p, a, b);
+    x.template members<INTER>(w);
+  }
+}
+// V numbers of a row of the table
+template <int V> __device__ __forceinline__ void rope_angles(float (&x)[V], const float* p) {
+  typedef float vec __attribute__((ext_vector_type(V < 4 ? V : 4)));
+  if constexpr (V == 1) x[0] = *p;
+  else {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const vec y = *(const vec*)(p + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i + e] = y[e];
+    }
   }
 }
 
@@ -104,8 +130,8 @@ __device__ __forceinline__ bool rope_position(const lmoe_rope_args& a, int b, in
 }
 
 template <typename T, int V, int L, int NC, bool INTER, bool BWD>
-__global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, const RopePlan p) {
-  constexpr int HB = NC > 1 ? 1 : BWD ? ROPE_BWD_HEADS : ROPE_FWD_HEADS;
+__global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a, const RopePlan p) {
+  constexpr int HB = NC > 1 ? 1 : ROPE_HEADS;
   typedef RopeRaw<T, V> Raw;
   const int l = threadIdx.x % L;
   const uint32_t group = blockIdx.x * (NTHR / L) + threadIdx.x / L, first = group / (uint32_t)p.runs;
@@ -133,56 +159,70 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
   const lmoe_tensor from = isq ? a.q : a.k, to = BWD ? (isq ? a.dq : a.dk) : (isq ? a.zq : a.zk), grad = isq ? a.dzq : a.dzk;
   const float over = 1.0f / (float)a.D;
   const uint32_t tokens = (uint32_t)a.B * (uint32_t)a.T;
-  // (a group past the last whole set of runs has nothing to do; its lanes stay: sums over a row need them all)
-  for (uint32_t tok0 = 0; tok0 < tokens; tok0 += step) {
-    const uint32_t tok = tok0 + first;
-    const bool mine = first < step && tok < tokens;
-    const int b = mine ? (int)(tok / (uint32_t)a.T) : 0, t = mine ? (int)(tok - (uint32_t)b * (uint32_t)a.T) : 0;
-    int pos = -1;
-    const bool live = mine && rope_position(a, b, t, pos);
+  // (all lanes of a row go the same way; a group past the last whole set of runs has nothing to do)
+  for (uint32_t tok = first < step ? first : tokens; tok < tokens; tok += step) {
+    const int b = (int)(tok / (uint32_t)a.T), t = (int)(tok - (uint32_t)b * (uint32_t)a.T);
     const T* x_row = (const T*)from.ptr + b * from.sb + t * from.st;
     const T* g_row = (const T*)grad.ptr + b * grad.sb + t * grad.st;
     T* z_row = (T*)to.ptr + b * to.sb + t * to.st;
-    float c[NC][V], s[NC][V];
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const bool turn = pos >= 0 && cr[j] >= 0;
-        c[j][i] = turn ? a.cos[(int64_t)pos * half + cr[j] + i] : 1.f;
-        s[j][i] = turn ? a.sin[(int64_t)pos * half + cr[j] + i] : 0.f;
-      }
-    for (int h0 = h_first; h0 < heads; h0 += HB * h_step) {
-      Raw rx[HB][NC], rg[HB][NC];
+    Raw rx[HB][NC], rg[HB][NC];
+    // (without a condition: behind the last head that one again, behind the last column the first)
+    auto load = [&](int h0) {
 #pragma unroll
       for (int y = 0; y < HB; ++y) {
-        const int64_t h = h0 + y * h_step;
+        const int64_t h = min(h0 + y * h_step, heads - 1);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-          rx[y][j].clear();
-          rg[y][j].clear();
-          if (!live || h >= heads || !on[j]) continue;
-          if (!BWD || a.norm) rx[y][j].load(x_row + h * from.sh, ca[j], cb[j]);
-          if (BWD) rg[y][j].load(g_row + h * grad.sh, ca[j], cb[j]);
+          rx[y][j].load(x_row + h * from.sh, ca[j], cb[j]);
+          if constexpr (BWD) rg[y][j].load(g_row + h * grad.sh, ca[j], cb[j]);
         }
       }
+    };
+    load(h_first);                       // (in front of the search for the position)
+    int pos;
+    const bool live = rope_position(a, b, t, pos);
+    if (!live) {                         // behind the last sequence: zeros, whatever lies there
+      Raw none;
+      none.clear();
+      for (int h = h_first; h < heads; h += h_step)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) if (on[j]) none.store(z_row + h * to.sh, ca[j], cb[j], p.past);
+      continue;
+    }
+    float c[NC][V], s[NC][V];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const bool turn = pos >= 0 && cr[j] >= 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) { c[j][i] = 1.f; s[j][i] = 0.f; }
+      if (turn) {
+        rope_angles<V>(c[j], a.cos + (int64_t)pos * half + cr[j]);
+        rope_angles<V>(s[j], a.sin + (int64_t)pos * half + cr[j]);
+      }
+    }
+    for (int h0 = h_first; h0 < heads; h0 += HB * h_step) {
+      if (h0 != h_first) load(h0);
 #pragma unroll
       for (int y = 0; y < HB; ++y) {
         const int64_t h = h0 + y * h_step;
+        if (h >= heads) break;
         float x[NC][2 * V], z[NC][2 * V];
         float r = 1.f;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          rx[y][j].template members<INTER>(x[j]);
+          if (!p.full && !on[j]) {
+#pragma unroll
+            for (int i = 0; i < 2 * V; ++i) x[j][i] = 0.f;
+          }
+        }
         if (a.norm) {
           float ss = 0.f;
 #pragma unroll
-          for (int j = 0; j < NC; ++j) {
-            rx[y][j].template members<INTER>(x[j]);
+          for (int j = 0; j < NC; ++j)
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) ss += x[j][i] * x[j][i];
-          }
           r = rsqrt_fast(lanes_of_row<L>(ss) * over + a.eps);
-        } else {
-#pragma unroll
-          for (int j = 0; j < NC; ++j) rx[y][j].template members<INTER>(x[j]);
         }
         if constexpr (!BWD) {
 #pragma unroll
@@ -199,6 +239,10 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
           for (int j = 0; j < NC; ++j) {
             float g[2 * V];
             rg[y][j].template members<INTER>(g);
+            if (!p.full && !on[j]) {
+#pragma unroll
+              for (int i = 0; i < 2 * V; ++i) g[i] = 0.f;
+            }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               const float ga = g[i] * c[j][i] + g[V + i] * s[j][i], gb = g[V + i] * c[j][i] - g[i] * s[j][i];
@@ -219,40 +263,40 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_rope(const lmoe_rope_args a, c
               for (int i = 0; i < 2 * V; ++i) z[j][i] = r * (z[j][i] - x[j][i] * m);
           }
         }
-        if (!mine || h >= heads) continue;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-          if (!on[j]) continue;
           Raw out;
           out.template from<INTER>(z[j]);
-          if (!live) out.clear();
-          out.store(z_row + h * to.sh, ca[j], cb[j]);
+          if (on[j]) out.store(z_row + h * to.sh, ca[j], cb[j], p.past);
         }
+        __builtin_amdgcn_sched_barrier(0);             // (one head after the other: their registers)
       }
     }
   }
   if constexpr (BWD) {
-    // dw: the lane groups of a wave, then the waves, then a row of ws per work-group
+    // dw: the lane groups of the work-group in their order, into its row of ws
     if (!a.ws) return;
-    __shared__ float part[NTHR / 64][2][256];
-    const int wv = wave_id();
+    constexpr int E = 2 * V * NC;
+    __shared__ float part[NTHR][E + 1];
+    __shared__ uint8_t of_q[NTHR / L];
 #pragma unroll
     for (int j = 0; j < NC; ++j)
 #pragma unroll
-      for (int i = 0; i < 2 * V; ++i) {
-        float x = isq ? sum[j][i] : 0.f, y = isq ? 0.f : sum[j][i];
-#pragma unroll
-        for (int d = L; d < 64; d <<= 1) { x += __shfl_xor(x, d, 64); y += __shfl_xor(y, d, 64); }
-        if (lane_id() < L && on[j]) {
-          const int e = i < V ? i : i - V, col = INTER ? ca[j] + 2 * e + (i >= V) : (i < V ? ca[j] : cb[j]) + e;
-          part[wv][0][col] = x;
-          part[wv][1][col] = y;
-        }
-      }
+      for (int i = 0; i < 2 * V; ++i) part[threadIdx.x][2 * V * j + i] = sum[j][i];
+    if (l == 0) of_q[threadIdx.x / L] = isq;
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * a.D; i += NTHR) {
-      const int which = i / a.D, col = i % a.D;
-      a.ws[(int64_t)blockIdx.x * 2 * a.D + i] = (part[0][which][col] + part[1][which][col]) + (part[2][which][col] + part[3][which][col]);
+      const bool q = i < a.D;
+      const int at = q ? i : i - a.D, chunk = at / (2 * V), e = at % (2 * V), c = chunk * V;         // member e of the chunk's pairs
+      float x = 0.f;
+#pragma unroll 8
+      for (int g = 0; g < NTHR / L; ++g) {
+        const float y = part[g * L + chunk % L][2 * V * (chunk / L) + e];
+        x += of_q[g] == q ? y : 0.f;
+      }
+      const int k = e < V ? e : e - V;
+      const int col = INTER ? 2 * (c + k) + (e >= V) : (c < half ? c : c + half) + k + (e < V ? 0 : c < half ? half : rest);
+      a.ws[(int64_t)blockIdx.x * 2 * a.D + (q ? 0 : a.D) + col] = x;
     }
   }
 }
@@ -278,8 +322,9 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_dw(const lmoe_rope_args a, int
   if (a.w_dtype == LMOE_F32) ((float*)to)[e] = y; else ((bf16*)to)[e] = (bf16)y;
 }
 
-// Whether every row can be read in 16-byte pieces that hold whole pairs' members
+// Whether every row can be read in 16-byte pieces that hold whole pairs' members, and the table and the weights with it
 static bool rope_wide(const lmoe_rope_args& a) {
+  for (const void* x : {(const void*)a.cos, (const void*)a.sin, a.qw, a.kw}) if ((uintptr_t)x & 15) return false;
   const int v = a.dtype == LMOE_BF16 ? 8 : 4;
   if (a.interleaved ? a.R % (2 * v) || a.D % (2 * v) : a.R % (2 * v) || (a.D - a.R) % (2 * v)) return false;
   const lmoe_tensor* all[] = {&a.q, &a.k, &a.zq, &a.zk, &a.dzq, &a.dzk, &a.dq, &a.dk};
@@ -294,11 +339,15 @@ static RopePlan rope_plan(const lmoe_rope_args& a, bool bwd) {
   p.lanes = 4;
   while (p.lanes < 64 && p.lanes < p.chunks) p.lanes *= 2;
   if (v == 1) p.lanes = 64;
+  p.full = p.chunks == p.lanes * (v == 1 ? 2 : 1);
   const int64_t tokens = (int64_t)a.B * a.T, per = NTHR / p.lanes, heads = (int64_t)a.HQ + a.HKV;
   // a head for each lane group while that leaves the card empty, else several
-  const int hb = v == 1 || tokens * heads <= 256 * 8 * per ? 1 : bwd ? ROPE_BWD_HEADS : ROPE_FWD_HEADS;
+  const int hb = v == 1 || tokens * heads <= 256 * 8 * per ? 1 : ROPE_HEADS;
   p.runs_q = (a.HQ + hb - 1) / hb;
   p.runs = p.runs_q + (a.HKV + hb - 1) / hb;
+  // Results of which the last-level cache would keep less than half by the time they are read go past it: 4 x 8192 tokens of 20 heads of
+  // 128 (168 MB each way), forward and backward, 192 -> 176 us; 8192 of 40 (84 MB), forward, 39 either way.
+  p.past = tokens * heads * a.D * (a.dtype == LMOE_BF16 ? 2 : 4) > 128 << 20;
   // as many tokens for every lane group
   const int64_t items = tokens * p.runs, most = bwd ? ROPE_BWD_GROUPS : ROPE_GROUPS;
   const int64_t each = (items + most * per - 1) / (most * per), sets = (tokens + each - 1) / each;
