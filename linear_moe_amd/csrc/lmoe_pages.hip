@@ -42,14 +42,18 @@ int64_t fork_ints(const lmoe_pages_args& a) { return (int64_t)a.F * (a.M + 1); }
 __device__ __forceinline__ int32_t seen(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void put(int32_t* p, int32_t x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+template <int N> struct Int { static constexpr int value = N; };
 // sum over the threads in front of this one, and over all (every thread of the work-group calls it)
 __device__ __forceinline__ int scan(int x, int& total, int* s_wave) {
+  // (shifts inside rows of 16 lanes, then the last lanes of rows into the next ones, as in wave_incl_scan)
+  auto dpp = [](int v, auto ctrl, auto rows) { return __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
   int y = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int z = __shfl_up(y, d, 64);
-    if (lane_id() >= d) y += z;
-  }
+  y += dpp(y, Int<0x111>(), Int<0xf>());
+  y += dpp(y, Int<0x112>(), Int<0xf>());
+  y += dpp(y, Int<0x114>(), Int<0xf>());
+  y += dpp(y, Int<0x118>(), Int<0xf>());
+  y += dpp(y, Int<0x142>(), Int<0xa>());
+  y += dpp(y, Int<0x143>(), Int<0xc>());
   __syncthreads();                         // s_wave of the scan before has been read
   if (lane_id() == 63) s_wave[threadIdx.x >> 6] = y;
   __syncthreads();
@@ -68,23 +72,30 @@ __device__ __forceinline__ int scan(int x, int& total, int* s_wave) {
 // behind the tile that fills the list).  A tile is PAGES_VEC numbers for every thread, PAGES_NTHR apart, so that a load reads
 // adjacent ones and all of a tile are in flight at once.
 struct ListShared { int count[PAGES_VEC * PAGES_WAVES], wave[PAGES_WAVES]; };
-__device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, bool used, int32_t* list, int most, ListShared& sh) {
-  static_assert(PAGES_VEC * PAGES_WAVES <= PAGES_NTHR, "");
-  const int wave = wave_id();
-  int before = 0;
-  for (int p0 = begin; p0 < end && before < most; p0 += PAGES_NTHR * PAGES_VEC) {
-    uint64_t hit[PAGES_VEC];
-    int r[PAGES_VEC];
+struct ListTile {
+  int r[PAGES_VEC];
+  __device__ __forceinline__ void load(const int32_t* refs, int p0, int end, bool used) {
 #pragma unroll
     for (int i = 0; i < PAGES_VEC; ++i) {
       const int p = p0 + i * PAGES_NTHR + (int)threadIdx.x;
       r[i] = p < end ? refs[p] : (used ? 0 : 1);
     }
+  }
+};
+// next: the first tile, asked for by the caller
+__device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, bool used, int32_t* list, int most, ListShared& sh, ListTile next) {
+  static_assert(PAGES_VEC * PAGES_WAVES <= PAGES_NTHR, "");
+  constexpr int TILE = PAGES_NTHR * PAGES_VEC;
+  const int wave = wave_id();
+  int before = 0;
+  for (int p0 = begin; p0 < end && before < most; p0 += TILE) {
+    uint64_t hit[PAGES_VEC];
 #pragma unroll
     for (int i = 0; i < PAGES_VEC; ++i) {
-      hit[i] = __ballot((r[i] > 0) == used);
+      hit[i] = __ballot((next.r[i] > 0) == used);
       if (lane_id() == 0) sh.count[i * PAGES_WAVES + wave] = __popcll(hit[i]);
     }
+    if (p0 + TILE < end) next.load(refs, p0 + TILE, end, used);
     __syncthreads();
     const int slot = threadIdx.x;
     int total;
@@ -168,6 +179,8 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
   __shared__ uint8_t s_fits[PAGES_NTHR];
   const PagesWs w = pages_ws(a);
   const int tid = threadIdx.x;
+  ListTile tile;
+  tile.load(a.refs, 0, a.P, false);       // (used last, asked for first)
   int row0 = 0, count = 0;                // rows from row0 on are dealt out, `count` entries of theirs
   auto deal = [&](int n0) {
     const int n = n0 + tid;
@@ -219,20 +232,22 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
   auto shared = [&](const Asked& e) { return e.x >= 0 && e.refs > 1; };
   auto kept = [&](const Asked& e) { return seen(w.claims + e.x) == e.refs && seen(w.last + e.x) == e.n * a.M + e.c; };
   if (tid == 0) put(w.count, 0);
+  int any = 0;
   every([&](const Asked& e) {
-    if (shared(e)) { put(w.claims + e.x, 0); put(w.last + e.x, -1); put(w.failed + e.x, 0); }
+    if (shared(e)) { put(w.claims + e.x, 0); put(w.last + e.x, -1); put(w.failed + e.x, 0); any = 1; }
   });
-  __syncthreads();
-  every([&](const Asked& e) {
-    if (shared(e)) { atomicAdd(w.claims + e.x, 1); atomicMax(w.last + e.x, e.n * a.M + e.c); }
-  });
-  __syncthreads();
+  if (__syncthreads_or(any)) {
+    every([&](const Asked& e) {
+      if (shared(e)) { atomicAdd(w.claims + e.x, 1); atomicMax(w.last + e.x, e.n * a.M + e.c); }
+    });
+    __syncthreads();
+  }
   auto copied = [&](const Asked& e) { return shared(e) && !kept(e); };
   auto needs = [&](const Asked& e) { return e.n >= 0 && (e.x < 0 || copied(e)); };
   int need = 0, all;
   every([&](const Asked& e) { need += needs(e); });
   scan(need, all, sh.wave);
-  const int free = listed(a.refs, 0, a.P, false, w.list, min(all, a.P), sh);
+  const int free = listed(a.refs, 0, a.P, false, w.list, min(all, a.P), sh, tile);
   __syncthreads();
   // pages needed in front of and up to each row that is dealt out; before: by the rows in front of them
   auto reach = [&](int before) {
@@ -303,18 +318,27 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_compact(const lmoe_pages_a
   __shared__ ListShared sh;
   const PagesWs w = pages_ws(a);
   int used = 0;
+  ListTile first, tile;
+  first.load(a.refs, 0, a.P, true);
+  tile = first;
   for (int p0 = 0; p0 < a.P; p0 += PAGES_NTHR * PAGES_VEC) {
+    const ListTile t = tile;
+    if (p0 + PAGES_NTHR * PAGES_VEC < a.P) tile.load(a.refs, p0 + PAGES_NTHR * PAGES_VEC, a.P, true);
 #pragma unroll
     for (int i = 0; i < PAGES_VEC; ++i) {
       const int p = p0 + i * PAGES_NTHR + (int)threadIdx.x;
-      if (p < a.P) { used += a.refs[p] > 0; put(a.moved + p, p); }
+      used += t.r[i] > 0;
+      if (p < a.P) put(a.moved + p, p);
     }
   }
   int live;
   scan(used, live, sh.wave);
-  // as many free numbers below as used pages above
-  const int count = listed(a.refs, 0, live, false, w.dst, live, sh);
-  listed(a.refs, live, a.P, true, w.src, count, sh);
+  // as many free numbers below as used pages above (numbers from live on are as good as used for the first list)
+  tile.load(a.refs, live, a.P, true);
+#pragma unroll
+  for (int i = 0; i < PAGES_VEC; ++i) if (i * PAGES_NTHR + (int)threadIdx.x >= live) first.r[i] = 1;
+  const int count = listed(a.refs, 0, live, false, w.dst, live, sh, first);
+  listed(a.refs, live, a.P, true, w.src, count, sh, tile);
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += PAGES_NTHR) {
     const int from = seen(w.src + i), to = seen(w.dst + i);
