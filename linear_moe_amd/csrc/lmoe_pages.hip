@@ -367,6 +367,7 @@ struct PageBufs {
   int32_t per[COPY_BUFS];              // units of a run
   int8_t vec[COPY_BUFS];               // bytes of a piece: 16, 4 or 1
 };
+// (stores past the caches: 320 pages of 2 x 131 KB, 37 -> 29 us; a few pages, either way)
 template <typename P> __device__ __forceinline__ void copy_run(uint8_t* to, const uint8_t* from, int64_t bytes) {
   constexpr int U = 4;
   const int64_t n = bytes / sizeof(P);
@@ -375,7 +376,7 @@ template <typename P> __device__ __forceinline__ void copy_run(uint8_t* to, cons
 #pragma unroll
     for (int u = 0; u < U; ++u) if (i0 + u * NTHR < n) x[u] = ((const P*)from)[i0 + u * NTHR];
 #pragma unroll
-    for (int u = 0; u < U; ++u) if (i0 + u * NTHR < n) ((P*)to)[i0 + u * NTHR] = x[u];
+    for (int u = 0; u < U; ++u) if (i0 + u * NTHR < n) __builtin_nontemporal_store(x[u], (P*)to + i0 + u * NTHR);
   }
 }
 __global__ __launch_bounds__(NTHR) void k_pages_copy(const lmoe_pages_args a, const PageBufs bufs) {
@@ -420,7 +421,7 @@ static void pages_copies(const lmoe_pages_args& a, int64_t most, bool rename, hi
       const uint64_t bits = (uintptr_t)b.ptr | (uint64_t)(b.page_stride | b.stride0 | b.stride1 | b.bytes);
       p.vec[k] = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
     }
-    const int64_t units = most * p.units[p.n], groups = p.renamers + std::min<int64_t>(units, 2048);
+    const int64_t units = most * p.units[p.n], groups = p.renamers + std::min<int64_t>(units, 1024);
     if (groups > 0) hipLaunchKernelGGL(k_pages_copy, dim3((uint32_t)groups), dim3(NTHR), 0, st, a, p);
   }
 }
