@@ -253,6 +253,14 @@ void launch_paged_read(const lmoe_paged4_args& a, bool bits4, hipStream_t st) {
 }
 
 // ---- one new token ----
+// Work-groups go round the eight XCDs.  Where the heads of a token lie next to each other, two rows of 64 bytes share a cache line: then the
+// heads of a stretch follow each other on one XCD, and the line comes once from memory (64 sequences of 1024 to 4096 tokens, 32 / 8
+// heads of 128: 72 -> 62 us; where the tokens of a head lie next to each other, 49 -> 50).
+constexpr int XCDS = 8;
+__host__ __device__ inline bool heads_near(const lmoe_paged_args& a, const PagedPlan& p) {
+  const int64_t units = (int64_t)a.N * p.splits;
+  return a.HKV > 1 && a.kp.sh < a.kp.st && units >= XCDS && units * a.HKV * p.blocks <= 1 << 22;
+}
 static PagedPlan paged4_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
@@ -318,9 +326,18 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   typedef uint32_t words __attribute__((ext_vector_type(KW)));
   __shared__ __attribute__((aligned(16))) float s_o[NW][PHEADS][W + 4];
   __shared__ float s_m[NW][PHEADS], s_l[NW][PHEADS];
-  // (the order of the work-groups as in k_paged_attn)
-  const int part = blockIdx.x % p.splits, group = blockIdx.x / p.splits;
-  const int n = group / (a.HKV * p.blocks), hb = group % (a.HKV * p.blocks), hk = hb / p.blocks, G = a.HQ / a.HKV;
+  const int G = a.HQ / a.HKV, per = a.HKV * p.blocks;
+  int unit, hb;
+  if (heads_near(a, p)) {
+    const int y = blockIdx.x / XCDS;
+    unit = y / per * XCDS + blockIdx.x % XCDS;
+    hb = y % per;
+    if (unit >= a.N * p.splits) return;
+  } else {                               // (the order of k_paged_attn)
+    unit = blockIdx.x / p.splits / per * p.splits + blockIdx.x % p.splits;
+    hb = blockIdx.x / p.splits % per;
+  }
+  const int part = unit % p.splits, n = unit / p.splits, hk = hb / p.blocks;
   const int h0 = hb % p.blocks * PHEADS, heads = min(PHEADS, G - h0);      // of the key head's group
   const PagedSeq sq = paged_seq(a, p, n);
   const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = part * sq.chunk;
@@ -590,7 +607,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
 }
 
 template <typename T, int W, int NW, bool EVEN> static void paged4_parts(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
-  const dim3 grid((uint32_t)((int64_t)a.p.N * a.p.HKV * p.blocks * p.splits)), block(64 * NW);
+  const int64_t units = (int64_t)a.p.N * p.splits;
+  const dim3 grid((uint32_t)((heads_near(a.p, p) ? (units + XCDS - 1) / XCDS * XCDS : units) * a.p.HKV * p.blocks)), block(64 * NW);
   if (a.p.softcap > 0.f) {
     if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, true>), grid, block, 0, st, a, p);
     else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, false>), grid, block, 0, st, a, p);
