@@ -231,7 +231,6 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
   };
   auto shared = [&](const Asked& e) { return e.x >= 0 && e.refs > 1; };
   auto kept = [&](const Asked& e) { return seen(w.claims + e.x) == e.refs && seen(w.last + e.x) == e.n * a.M + e.c; };
-  if (tid == 0) put(w.count, 0);
   int any = 0;
   every([&](const Asked& e) {
     if (shared(e)) { put(w.claims + e.x, 0); put(w.last + e.x, -1); put(w.failed + e.x, 0); any = 1; }
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
       __syncthreads();
     }
   }
-  int before = 0, given = 0;
+  int before = 0, given = 0, copies = 0;
   for (int n0 = 0; n0 < a.N; n0 += PAGES_NTHR) {
     if (!whole) { __syncthreads(); deal(n0); }
     if (all > free) {
@@ -293,23 +292,26 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
     // (refs of a shared page stays as it is until every thread has decided by it; the rows that fit take the free pages one by one, for
     // those that do not lie behind them all, but for rows without needs)
     entries([&](const Asked& e) {
-      const bool take = needs(e) && s_fits[e.n - row0];
+      // (pages taken and, of them, copies: both counts in one sum)
+      const bool take = needs(e) && s_fits[e.n - row0], copy = take && e.x >= 0;
       int total;
-      const int at = given + scan(take, total, sh.wave);
-      given += total;
+      const int both = scan(take + (copy << 16), total, sh.wave), at = given + (both & 0xffff), i = copies + (both >> 16);
+      given += total & 0xffff;
+      copies += total >> 16;
       if (!take) return;
       const int page = seen(w.list + at);
       a.table[(int64_t)e.n * a.table_stride + e.c] = page;
       a.refs[page] = 1;                    // (free or given out: no page is shared by it)
-      if (e.x >= 0) {
-        const int i = atomicAdd(w.count, 1);               // (the order of the copies changes nothing)
+      if (copy) {
         put(w.src + i, e.x);
         put(w.dst + i, page);
+        if (single) atomicSub(a.refs + e.x, 1);            // (everybody has decided)
       }
     });
   }
+  if (tid == 0) put(w.count, copies);
+  if (single) return;
   __syncthreads();
-  const int copies = seen(w.count);
   for (int i = tid; i < copies; i += PAGES_NTHR) atomicSub(a.refs + seen(w.src + i), 1);
 }
 
