@@ -75,52 +75,52 @@ template <typename T> __device__ __forceinline__ float size_of(const typename ET
     return m;
   }
 }
-template <typename T> __device__ __forceinline__ void store_frag(T* p, const typename ET<T>::frag& x) {
-  if constexpr (sizeof(T) == 2) *(bf16x8*)p = x; else { *(f32x4*)p = x.lo; *(f32x4*)(p + 4) = x.hi; }
+template <typename T> __device__ __forceinline__ void store_frag(T* p, const typename ET<T>::frag& x, bool past) {
+  if constexpr (sizeof(T) == 2) { if (past) __builtin_nontemporal_store(x, (bf16x8*)p); else *(bf16x8*)p = x; }
+  else if (past) { __builtin_nontemporal_store(x.lo, (f32x4*)p); __builtin_nontemporal_store(x.hi, (f32x4*)(p + 4)); }
+  else { *(f32x4*)p = x.lo; *(f32x4*)(p + 4) = x.hi; }
 }
 
 // ---- written and read: a wave per token ----
-// Token `tok` of a call: its sequence n, its row and place in memory, and its place in the sequence; false: behind the last one
-struct PagedToken { int n, b, t, at; };
-__device__ __forceinline__ bool paged_token(const lmoe_paged_args& a, int64_t tok, PagedToken& x) {
-  if (a.cu_seqlens) {
-    // the last sequence that begins at or before the token (of several, all but the last are empty): 64 candidates a round
-    x.b = 0; x.t = (int)tok;
-    if (x.t >= a.cu_seqlens[a.N] || x.t < a.cu_seqlens[0]) return false;
-    int lo = 0, hi = a.N;
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 63) / 64, i = lo + lane_id() * step;
-      const int cnt = __popcll(__ballot(i < hi && a.cu_seqlens[min(i, a.N)] <= x.t));
-      lo += (cnt - 1) * step;
-      hi = min(hi, lo + step);
-    }
-    x.n = lo;
-    x.at = x.t - a.cu_seqlens[lo];
-  } else {
-    x.n = x.b = (int)(tok / a.T);
-    x.t = x.at = (int)(tok - (int64_t)x.b * a.T);
+// The sequence of token t of row b, and its place in it; n = -1: behind the last sequence
+struct PagedToken { int n, at; };
+__device__ __forceinline__ PagedToken paged_token(const lmoe_paged_args& a, int b, int t) {
+  if (!a.cu_seqlens) return {b, t};
+  // the last sequence that begins at or before the token (of several, all but the last are empty): 64 candidates a round
+  if (t >= a.cu_seqlens[a.N] || t < a.cu_seqlens[0]) return {-1, 0};
+  int lo = 0, hi = a.N;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, i = lo + lane_id() * step;
+    const int cnt = __popcll(__ballot(i < hi && a.cu_seqlens[min(i, a.N)] <= t));
+    lo += (cnt - 1) * step;
+    hi = min(hi, lo + step);
   }
-  return true;
+  return {lo, t - a.cu_seqlens[lo]};
 }
-// page and slot of a token; -1: it has none
-__device__ __forceinline__ int paged_slot(const lmoe_paged_args& a, const PagedToken& x, int& slot) {
-  const int64_t pos = (int64_t)a.lens[x.n] + x.at;
-  slot = 0;
-  if (a.lens[x.n] < 0 || pos >= (int64_t)a.M * a.S) return -1;
-  const int id = a.table[(int64_t)x.n * a.table_stride + (int)pos / a.S];
-  slot = (int)pos % a.S;
-  return id < 0 || id >= a.P ? -1 : id;
+// page and slot of a token; page -1: it has none
+struct PagedSlot { int page, slot; };
+__device__ __forceinline__ PagedSlot paged_slot(const lmoe_paged_args& a, const PagedToken& x) {
+  if (x.n < 0) return {-1, 0};
+  const int len = a.lens[x.n];
+  const int64_t pos = (int64_t)len + x.at;
+  if (len < 0 || pos >= (int64_t)a.M * a.S) return {-1, 0};
+  const uint32_t col = (uint32_t)pos / (uint32_t)a.S;
+  const int id = a.table[(int64_t)x.n * a.table_stride + col];
+  return id < 0 || id >= a.P ? PagedSlot{-1, 0} : PagedSlot{id, (int)((uint32_t)pos - col * (uint32_t)a.S)};
 }
 
 // The lanes of a wave go over the pieces (VEC columns) of a token's rows of k and of v, PIECES of each in flight for a lane.
 constexpr int PIECES = 2;
 struct TokenPlan {
   int nk, nv;              // pieces of k and of v
-  uint32_t div_k, div_v;   // i / (pieces of a row) = umulhi(2 i, div) for i < 2^20
+  bool past;               // what is read goes past the caches: more of it than an eighth of the last-level cache (16384 tokens, 8 heads of 128,
+                           // 67 MB: 19 -> 15 us; 64 tokens: either way)
+  uint32_t div_k, div_v;   // i / (pieces of a row) = umulhi(2 i, div) for i < 2^26, at most 32 of them
 };
 static TokenPlan token_plan(const lmoe_paged_args& a, int vec) {
   const int pk = a.K / vec, pv = a.V / vec;
-  return {a.HKV * pk, a.HKV * pv, (uint32_t)((1ull << 31) / pk + 1), (uint32_t)((1ull << 31) / pv + 1)};
+  const bool past = (int64_t)a.B * a.T * a.HKV * (a.K + a.V) * (a.dtype == LMOE_BF16 ? 2 : 4) > 32 << 20;
+  return {a.HKV * pk, a.HKV * pv, past, (uint32_t)((1ull << 31) / pk + 1), (uint32_t)((1ull << 31) / pv + 1)};
 }
 // pieces i0 + l + 64 u of a side (k or v): heads and places in a row
 struct Side {
@@ -148,9 +148,9 @@ __device__ __forceinline__ float quad_larger(float x) {
 template <typename T> __global__ __launch_bounds__(NTHR) void k_paged4_append(const lmoe_paged4_args a4, const TokenPlan p) {
   typedef typename ET<T>::frag frag;
   const lmoe_paged_args& a = a4.p;
-  const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
-  if (tok >= (int64_t)a.B * a.T) return;
-  const int b = a.cu_seqlens ? 0 : (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
+  const uint32_t tok = blockIdx.x * (NTHR / 64) + wave_id();             // (less than 2^26)
+  if (tok >= (uint32_t)a.B * (uint32_t)a.T) return;
+  const int b = a.cu_seqlens ? 0 : (int)(tok / (uint32_t)a.T), t = (int)(tok - (uint32_t)b * (uint32_t)a.T);
   const T* kn = (const T*)a.kn.ptr + (int64_t)b * a.kn.sb + (int64_t)t * a.kn.st;
   const T* vn = (const T*)a.vn.ptr + (int64_t)b * a.vn.sb + (int64_t)t * a.vn.st;
   Side sk(p.nk, a.K / 8, p.div_k), sv(p.nv, a.V / 8, p.div_v);                  // four pieces share a scale
@@ -166,10 +166,8 @@ template <typename T> __global__ __launch_bounds__(NTHR) void k_paged4_append(co
   // (the rows are asked for before their place is)
   load(sk, yk, kn, a.kn.sh, 0);
   load(sv, yv, vn, a.vn.sh, 0);
-  PagedToken x;
-  if (!paged_token(a, tok, x)) return;
-  int slot;
-  const int id = paged_slot(a, x, slot);
+  const PagedSlot place = paged_slot(a, paged_token(a, b, t));
+  const int id = place.page, slot = place.slot;
   if (id < 0) return;
   auto store = [&](const Side& s, const frag (&y)[PIECES], const lmoe_tensor& codes, const lmoe_tensor& scales) {
     uint8_t* d = (uint8_t*)codes.ptr + (int64_t)id * codes.sb + (int64_t)slot * codes.st;
@@ -197,12 +195,11 @@ template <typename T, bool BITS4> __global__ __launch_bounds__(NTHR) void k_page
   constexpr int VEC = BITS4 ? 8 : ET<T>::VEC;
   typedef typename ET<T>::vec vec;
   const lmoe_paged_args& a = a4.p;
-  const int64_t tok = (int64_t)blockIdx.x * (NTHR / 64) + wave_id();
-  if (tok >= (int64_t)a.B * a.T) return;
-  const int b = a.cu_seqlens ? 0 : (int)(tok / a.T), t = (int)(tok - (int64_t)b * a.T);
-  PagedToken x;
-  int slot = 0, id = -1;
-  if (paged_token(a, tok, x)) id = paged_slot(a, x, slot);
+  const uint32_t tok = blockIdx.x * (NTHR / 64) + wave_id();             // (less than 2^26)
+  if (tok >= (uint32_t)a.B * (uint32_t)a.T) return;
+  const int b = a.cu_seqlens ? 0 : (int)(tok / (uint32_t)a.T), t = (int)(tok - (uint32_t)b * (uint32_t)a.T);
+  const PagedSlot place = paged_slot(a, paged_token(a, b, t));
+  const int id = place.page, slot = place.slot;
   Side sk(p.nk, a.K / VEC, p.div_k), sv(p.nv, a.V / VEC, p.div_v);
   struct Held { uint32_t r, scale; vec y; } hk[PIECES], hv[PIECES];
   auto load = [&](Side& s, Held (&y)[PIECES], const lmoe_tensor& codes, const lmoe_tensor& scales, int i0) {
@@ -225,7 +222,9 @@ template <typename T, bool BITS4> __global__ __launch_bounds__(NTHR) void k_page
     for (int u = 0; u < PIECES; ++u) {
       if (!s.on[u]) continue;
       T* d = row + s.h[u] * to.sh + VEC * s.c[u];
-      if constexpr (BITS4) store_frag<T>(d, from4<T>(y[u].r, scale_of(y[u].scale))); else *(vec*)d = y[u].y;
+      if constexpr (BITS4) store_frag<T>(d, from4<T>(y[u].r, scale_of(y[u].scale)), p.past);
+      else if (p.past) __builtin_nontemporal_store(y[u].y, (vec*)d);
+      else *(vec*)d = y[u].y;
     }
   };
   for (int i0 = 0; i0 < max(p.nk, p.nv); i0 += 64 * PIECES) {

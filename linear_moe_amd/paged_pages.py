@@ -70,7 +70,7 @@ def _bufs(pages, a, dev, name):
                 runs[-1] = runs[-1][0], runs[-1][1] * count
             else:
                 runs.append((step, count))
-        if runs[0][0] != size or len(runs) > 3:
+        if len(runs) > 3 or max(n for _, n in runs[1:] or [(0, 0)]) > 2 ** 24:
             raise ValueError(f"{name}: a page must be runs of adjacent numbers at one or two strides: {tuple(x.shape)} with strides {x.stride()}")
         buf.ptr, buf.page_stride = x.data_ptr(), x.stride(0) * size if a.P > 1 else 0
         buf.bytes = size * runs[0][1] if x.numel() else 0

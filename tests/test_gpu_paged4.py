@@ -154,6 +154,32 @@ def test_pages_that_are_none(cuda):
     assert (o == 0).all()
 
 
+def test_many_sequences_and_heads_next_to_each_other(cuda):
+    """Both orders of the work-groups, with stretches of their own for every head."""
+    lens = [(37 * i) % 70 for i in range(50)]
+    for heads_first in (True, False):
+        decode_and_check(cuda, Cache4(14, lens, 16, 3, 64, 64, heads_first=heads_first), 6, 64, 64, BF16, append=True)
+        decode_and_check(cuda, Cache4(15, [2500, 1, 1100, 40, 2048, 1024, 0, 7, 1025], 16, 2, 64, 64, heads_first=heads_first), 2, 64, 64, BF16)
+
+
+def test_a_score_that_grows(cuda):
+    """Maxima that move late and by much, and ones that move by less than 2^8: the sums stay those of the definition."""
+    for step, scale in ((0.02, 1.0), (0.3, 1.0), (3.0, 1.0), (-3.0, 1.0)):
+        c = Cache4(16, [700], 16, 1, 64, 64)
+        q = gen(80, 1, 1, 2, 64, dtype=BF16)
+        # keys along q, longer and longer (in 4 bits: what the format keeps of them)
+        grow = (1 + step * torch.arange(700).float() / 50) * scale
+        kk = kv4.pack(q[0, 0, :1].float() * grow[:, None, None])
+        c.rows[0][:2] = kk
+        for j in range(700):
+            c.put(0, j, [p[j] for p in c.rows[0]])
+        (kp, ks, vp, vs), table, lens = c.to(cuda)
+        o = L.paged_attn_decode(q.to(cuda), kp, vp, table, lens, head_first=False, k_scales=ks, v_scales=vs)
+        for h in range(2):
+            ref, tol = softmax.head(q[0, :, h], kv4.values(*c.rows[0][:2])[:, 0], kv4.values(*c.rows[0][2:])[:, 0], 0.125, dtype=BF16)
+            assert ((o[0, :, h].cpu().double() - ref).abs() <= tol).all()
+
+
 def test_nan_in_a_token_that_nobody_sees(cuda):
     """Slots behind a sequence hold NaN in all these tests; one that is seen makes its head NaN."""
     c = Cache4(11, [50], 16, 2, 64, 64)
@@ -259,6 +285,22 @@ def test_append_and_read(cuda, dtype, bits4, K, V, HKV, S):
         assert all(torch.equal(a, b) for a, b in zip(before, (kp, vp)))
 
 
+def test_large_results_are_read(cuda):
+    """More than goes through the caches."""
+    P, S, H, D = 80, 64, 16, 128
+    for bits4 in (True, False):
+        k, v = (gen(72 + i, 1, P * S, H, D, dtype=BF16).to(cuda) for i in range(2))
+        table, zero = torch.arange(P, dtype=torch.int32, device=cuda)[None], torch.zeros(1, dtype=torch.int32, device=cuda)
+        sc = dict(zip(("k_scales", "v_scales"), (torch.empty(P, S, H, D // 32, dtype=torch.uint8, device=cuda) for _ in range(2)))) if bits4 else {}
+        kp, vp = (torch.empty(P, S, H, D // 2, dtype=torch.uint8, device=cuda) if bits4 else torch.empty(P, S, H, D, dtype=BF16, device=cuda) for _ in range(2))
+        L.paged_kv_append(kp, vp, k, v, table, zero, head_first=False, **sc)
+        for f32 in (False, True) if bits4 else (False,):
+            got = L.paged_kv_read(kp, vp, table, zero, P * S, head_first=False, dtype=F32 if f32 else BF16, **sc)
+            for x, y in zip(got, (k, v)):
+                want = kv4.values(*kv4.pack(y)) if bits4 else y.double()
+                assert torch.equal(x.double(), want)
+
+
 def test_strides(cuda):
     """Pages as parts of larger tensors: keys and values of one buffer, every second page, heads in another order; scales with any strides."""
     c = Cache4(12, [70, 3], 16, 2, 64, 64)
@@ -281,9 +323,10 @@ def test_strides(cuda):
     assert torch.equal(a, c2)
 
 
-def test_far_pages(cuda):
+@pytest.mark.parametrize("S", [64, 60])
+def test_far_pages(cuda, S):
     """Offsets beyond 2^32 bytes."""
-    P, S, H, D = 40000, 64, 16, 128                      # 2.6e9 bytes of codes
+    P, H, D = 40000, 16, 128                             # 2.6e9 bytes of codes
     k = torch.empty(P, H, S, D // 2, dtype=torch.uint8, device=cuda).transpose(1, 2)
     v = torch.empty(P, H, S, D // 2, dtype=torch.uint8, device=cuda).transpose(1, 2)
     ks, vs = (torch.empty(P, H, S, D // 32, dtype=torch.uint8, device=cuda).transpose(1, 2) for _ in range(2))

@@ -1,0 +1,257 @@
+"""Norm and rotation, the cache in 4 bits and the pages of a cache, as far as the host goes: blocks as the library reads them, what it
+refuses without a launch, the tables of angles, how tensors of pages are taken apart, and the oracles against themselves."""
+import ctypes as C
+import os
+import subprocess
+import tempfile
+
+import pytest
+import torch
+
+import linear_moe_amd as L
+from linear_moe_amd import _lib
+from linear_moe_amd.paged_pages import _bufs
+from oracle import kv4, pages, rope
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "lmoe.h")
+FAKE = 1 << 20          # an aligned address that nothing reads
+
+
+@pytest.mark.parametrize("struct,cls", [("lmoe_paged4_args", _lib.Paged4Args), ("lmoe_rope_args", _lib.RopeArgs), ("lmoe_page_buf", _lib.PageBuf),
+                                        ("lmoe_pages_args", _lib.PagesArgs)])
+def test_blocks_match_the_header(struct, cls):
+    fields = [f[0] for f in cls._fields_]
+    prog = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{HEADER}"', 'int main(void){', f'printf("%zu\\n", sizeof({struct}));']
+    prog += [f'printf("%zu\\n", offsetof({struct}, {f}));' for f in fields] + ['return 0;}']
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "t.c"), os.path.join(d, "t")
+        open(src, "w").write("\n".join(prog))
+        subprocess.check_call(["gcc", "-o", exe, src])
+        out = [int(x) for x in subprocess.check_output([exe]).split()]
+    assert out == [C.sizeof(cls)] + [getattr(cls, f).offset for f in fields]
+
+
+def rope_args(**kw):
+    a = _lib.RopeArgs()
+    a.dtype, a.w_dtype, a.B, a.T, a.HQ, a.HKV, a.D, a.R, a.N, a.L, a.norm, a.eps = _lib.LMOE_BF16, _lib.LMOE_F32, 2, 3, 4, 2, 64, 64, 2, 10, 1, 1e-6
+    a.cos = a.sin = a.qw = a.kw = a.dqw = a.dkw = a.ws = FAKE
+    for n in ("q", "k", "zq", "zk", "dzq", "dzk", "dq", "dk"):
+        setattr(a, n, _lib.Tensor4(FAKE, 2048, 256, 64))
+    for n, x in kw.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("code,kw", [
+    (-2, dict(dtype=3)), (-2, dict(w_dtype=2)), (-3, dict(D=63)), (-3, dict(D=258)), (-3, dict(D=0)), (-3, dict(R=66)), (-3, dict(R=3)), (-3, dict(R=-2)), (-4, dict(T=-1)),
+    (-4, dict(HKV=0)), (-4, dict(L=-1)), (-8, dict(HQ=65536)), (-8, dict(B=2 ** 16, T=2 ** 15)), (-5, dict(cu_seqlens=FAKE)),
+    (-5, dict(cu_seqlens=FAKE, B=1, positions=FAKE)), (-5, dict(positions=FAKE, offsets=FAKE)), (-7, dict(k=_lib.Tensor4())), (-7, dict(cos=None)), (-15, dict(eps=-1.0)),
+    (-15, dict(eps=float("nan"))), (-15, dict(norm=0))])
+def test_norm_and_rotation_blocks_that_are_refused(code, kw):
+    lib = _lib.load()
+    for fn in (lib.lmoe_qk_norm_rope_fwd, lib.lmoe_qk_norm_rope_bwd):
+        assert fn(C.byref(rope_args(**kw)), None) == code, lib.lmoe_last_error()
+        assert fn(None, None) == -1
+    assert lib.lmoe_qk_norm_rope_floats(C.byref(rope_args(**kw))) == code
+
+
+def test_norm_and_rotation_blocks_of_one_way():
+    lib = _lib.load()
+    fwd, bwd = lib.lmoe_qk_norm_rope_fwd, lib.lmoe_qk_norm_rope_bwd
+    assert fwd(C.byref(rope_args(zq=_lib.Tensor4())), None) == -7
+    assert bwd(C.byref(rope_args(dzk=_lib.Tensor4())), None) == -11
+    for ws in (None, FAKE + 4):
+        assert bwd(C.byref(rope_args(ws=ws)), None) == -11
+    for kw in (dict(T=0), dict(B=0, N=0)):                     # no tokens: checked, and nothing launched
+        assert fwd(C.byref(rope_args(**kw)), None) == 0 and bwd(C.byref(rope_args(**kw)), None) == 0
+    assert lib.lmoe_qk_norm_rope_floats(C.byref(rope_args(dqw=None, dkw=None))) == 0
+    # as many rows as a call has work-groups at most, whatever its tensors' alignment
+    assert lib.lmoe_qk_norm_rope_floats(C.byref(rope_args())) == (2 * 3 * 6 + 6) * 2 * 64
+
+
+def paged4_args(**kw):
+    a = _lib.Paged4Args()
+    p = a.p
+    p.dtype, p.N, p.HQ, p.HKV, p.K, p.V, p.P, p.S, p.M, p.B, p.T = _lib.LMOE_BF16, 3, 4, 2, 64, 64, 10, 16, 4, 3, 5
+    p.scale, p.table_stride, p.table, p.lens, p.ws = 1.0, 4, FAKE, FAKE, FAKE
+    for n in ("q", "o", "kp", "vp", "kn", "vn"):
+        setattr(p, n, _lib.Tensor4(FAKE, 2048, 128, 64))
+    a.ks, a.vs = _lib.Tensor4(FAKE + 1, 70, 5, 3), _lib.Tensor4(FAKE + 3, 70, 5, 3)
+    for n, x in kw.items():
+        setattr(a if n in ("ks", "vs") else p, n, x)
+    return a
+
+
+@pytest.mark.parametrize("code,kw", [
+    (-2, dict(dtype=5)), (-3, dict(K=160)), (-3, dict(V=48)), (-3, dict(K=16)), (-4, dict(S=0)), (-4, dict(M=-1)), (-8, dict(N=70000)), (-8, dict(M=2 ** 20, S=2 ** 12)),
+    (-7, dict(lens=None)), (-7, dict(table=None)), (-7, dict(ks=_lib.Tensor4())), (-11, dict(vn=_lib.Tensor4())), (-9, dict(kp=_lib.Tensor4(FAKE, 2048, 136, 64))),
+    (-9, dict(vp=_lib.Tensor4(FAKE + 8, 2048, 128, 64))), (-9, dict(kn=_lib.Tensor4(FAKE + 8, 2048, 128, 64)))])
+def test_blocks_of_a_cache_in_4_bits_that_are_refused(code, kw):
+    lib = _lib.load()
+    for fn in (lib.lmoe_paged4_attn_decode, lib.lmoe_paged4_kv_append, lib.lmoe_paged4_kv_read):
+        assert fn(C.byref(paged4_args(**kw)), None) == code, lib.lmoe_last_error()
+        assert fn(None, None) == -1
+    assert lib.lmoe_paged4_attn_floats(C.byref(paged4_args(**kw))) == code
+
+
+def test_blocks_of_one_op_on_a_cache_in_4_bits():
+    lib = _lib.load()
+    decode, append, read = lib.lmoe_paged4_attn_decode, lib.lmoe_paged4_kv_append, lib.lmoe_paged4_kv_read
+    assert decode(C.byref(paged4_args(HQ=3)), None) == -3
+    assert decode(C.byref(paged4_args(HQ=60000, HKV=1, N=60000)), None) == -8
+    assert decode(C.byref(paged4_args(softcap=-2.0)), None) == -15
+    assert decode(C.byref(paged4_args(o=_lib.Tensor4())), None) == -7
+    for fn in (append, read):
+        assert fn(C.byref(paged4_args(kn=_lib.Tensor4(), vn=_lib.Tensor4())), None) == -7
+        assert fn(C.byref(paged4_args(B=2)), None) == -6
+        assert fn(C.byref(paged4_args(T=2 ** 26)), None) == -8
+        assert fn(C.byref(paged4_args(T=0)), None) == 0
+    a = paged4_args(M=1000, N=1)
+    n = lib.lmoe_paged4_attn_floats(C.byref(a))
+    assert n > 0 and n % ((64 + 2) * 4) == 0
+    a.p.ws = None
+    assert decode(C.byref(a), None) == -11
+    assert lib.lmoe_paged_kv_read(C.byref(paged4_args(B=2).p), None) == -6 and lib.lmoe_paged_kv_read(None, None) == -1
+
+
+def pages_args(**kw):
+    a = _lib.PagesArgs()
+    a.N, a.M, a.P, a.S, a.F, a.each, a.n_bufs, a.table_stride = 3, 4, 10, 16, 2, 1, 1, 4
+    for n in ("table", "lens", "refs", "rows", "src", "tokens", "fits", "live", "moved", "ws"):
+        setattr(a, n, FAKE)
+    buf = (_lib.PageBuf * 1)(_lib.PageBuf(FAKE, 1024, 0, 0, 1024, 1, 1))
+    a.bufs = buf
+    for n, x in kw.items():
+        if n in ("ptr", "bytes", "rows0"):
+            setattr(buf[0], n, x)
+        else:
+            setattr(a, n, x)
+    return a, buf
+
+
+@pytest.mark.parametrize("code,kw,ops", [
+    (-4, dict(N=-1), "free fork reserve compact"), (-4, dict(F=-1), "free fork"), (-4, dict(S=0), "reserve compact"), (-8, dict(N=2 ** 16, M=2 ** 15, table_stride=2 ** 15), "free fork reserve compact"),
+    (-8, dict(F=2 ** 24), "free fork"), (-8, dict(M=2 ** 16, S=2 ** 15, table_stride=2 ** 16), "reserve compact"), (-7, dict(table=None), "free fork reserve compact"), (-7, dict(refs=None), "free fork reserve compact"),
+    (-9, dict(table_stride=3), "free fork reserve compact"), (-7, dict(rows=None), "free fork"), (-7, dict(src=None), "fork"), (-11, dict(ws=None), "fork reserve compact"), (-7, dict(fits=None), "reserve"),
+    (-7, dict(lens=None), "free fork reserve"), (-7, dict(live=None), "compact"), (-7, dict(moved=None), "compact"), (-7, dict(ptr=None), "reserve compact"), (-8, dict(bytes=-1), "reserve compact"),
+    (-8, dict(rows0=2 ** 25), "reserve compact")])
+def test_blocks_of_pages_that_are_refused(code, kw, ops):
+    lib = _lib.load()
+    for op in ops.split():
+        fn = getattr(lib, f"lmoe_paged_{op}")
+        a, buf = pages_args(**kw)
+        assert fn(C.byref(a), None) == code, (op, lib.lmoe_last_error())
+        assert fn(None, None) == -1
+
+
+def test_calls_on_pages_without_work():
+    lib = _lib.load()
+    a, buf = pages_args(F=0)
+    assert lib.lmoe_paged_free(C.byref(a), None) == 0 and lib.lmoe_paged_fork(C.byref(a), None) == 0
+    a, buf = pages_args(N=0)
+    assert lib.lmoe_paged_reserve(C.byref(a), None) == 0
+    a, buf = pages_args()
+    assert lib.lmoe_paged_fork_ints(C.byref(a)) == 2 * 5 and lib.lmoe_paged_pages_ints(C.byref(a)) > 6 * 10
+
+
+def test_angles_are_formed_in_64_bits():
+    cos, sin = L.rope_table(200001, 8, base=10000.0)
+    assert cos.dtype == torch.float32 and cos.shape == (200001, 4)
+    import math
+    for p in (0, 1, 77, 4096, 131071, 200000):
+        for i in range(4):
+            a = p * 10000.0 ** (-2 * i / 8)
+            assert abs(float(cos[p, i]) - math.cos(a)) <= 2.0 ** -24 and abs(float(sin[p, i]) - math.sin(a)) <= 2.0 ** -24
+    assert L.rope_table(3, 0)[0].shape == (3, 0) and L.rope_table(0, 4)[0].shape == (0, 2)
+    for bad in ((3, 5), (-1, 4), (3, -2)):
+        with pytest.raises(ValueError):
+            L.rope_table(*bad)
+
+
+def test_calls_off_the_gpu_are_refused():
+    q, k, i32 = torch.zeros(2, 3, 4, 64), torch.zeros(2, 3, 2, 64), torch.zeros(2, dtype=torch.int32)
+    table = torch.zeros(2, 3, dtype=torch.int32)
+    u8 = torch.zeros(4, 16, 2, 32, dtype=torch.uint8)
+    for f in (lambda: L.qk_norm_rope(q, k), lambda: L.paged_kv_read(u8, u8, table, i32, 2, k_scales=u8[..., :2], v_scales=u8[..., :2]),
+              lambda: L.paged_free(table, i32, i32, i32), lambda: L.paged_fork(table, i32, i32, i32, i32), lambda: L.paged_reserve(u8, table, i32, i32, 1),
+              lambda: L.paged_compact(u8, table, i32)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            f()
+
+
+def taken(x, P=None):
+    a = _lib.PagesArgs()
+    a.P = x.shape[0] if P is None else P
+    pages_, bufs = _bufs(x, a, x.device, "t")
+    return a, bufs[0]
+
+
+def test_tensors_of_pages_are_taken_apart():
+    """Every byte of a page is in one run, and none of another page: told by copying page 1 as the block says."""
+    make = [torch.zeros(3, 4, 2, 8), torch.zeros(3, 2, 4, 8).transpose(1, 2), torch.zeros(6, 4, 3, 8)[::2, :, 1:], torch.zeros(4, 3, 8).transpose(0, 1),
+            torch.zeros(3, 4), torch.zeros(3, 4, 5, 2, 8)[:, :, :, 1], torch.zeros(3, 4, 2, 2)[..., 0], torch.zeros(3, 4, 2, 7, dtype=torch.uint8)[..., 1:4]]
+    for x in make:
+        base = x._base if x._base is not None else x
+        a, b = taken(x)
+        size, start = x.element_size(), x.data_ptr() - base.data_ptr()
+        flat = base.view(-1).view(torch.uint8) if base.is_contiguous() else None
+        x[1] = 1
+        want = base.clone()
+        x[1] = 0
+        mark = torch.zeros(base.numel() * size, dtype=torch.uint8)
+        for i in range(b.rows0):
+            for j in range(b.rows1):
+                at = start + b.page_stride + i * b.stride0 + j * b.stride1
+                mark[at:at + b.bytes] += 1
+        assert a.S == x.shape[1] and int(mark.max()) == 1
+        assert torch.equal(mark.view(-1, size)[:, 0].bool(), want.view(-1) != 0) and flat is not None
+
+
+def test_tensors_of_pages_that_are_refused():
+    for x in (torch.zeros(3), torch.zeros(1, 4, 2).expand(3, 4, 2), torch.zeros(3, 4, 1).expand(3, 4, 2), torch.zeros(6, 5, 3, 4, 9)[:, :4, :2, :3, :8], torch.zeros(3, 0, 2)):
+        with pytest.raises(ValueError):
+            taken(x)
+    with pytest.raises(ValueError):
+        taken(torch.zeros(3, 4), P=4)
+
+
+def test_the_format_of_4_bits():
+    """Nearest of the fifteen numbers by trying them all; nothing above 6 but at the last scale; what was read packs to itself."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(40, 64, generator=g, dtype=torch.float64) * torch.exp2(torch.randint(-30, 30, (40, 1), generator=g).double())
+    codes, scales = kv4.pack(x)
+    y = kv4.values(codes, scales)
+    step = torch.exp2(scales.double() - 127).repeat_interleave(32, -1)
+    grid = torch.tensor(kv4.GRID + tuple(-v for v in kv4.GRID), dtype=torch.float64)
+    best = (x[..., None] - grid * step[..., None]).abs().amin(-1)
+    assert torch.equal((x - y).abs(), best)
+    most = x.unflatten(-1, (-1, 32)).abs().amax(-1) / torch.exp2(scales.double() - 127)
+    assert ((most <= 6) & (most > 3)).all()
+    assert all(torch.equal(a, b) for a, b in zip(kv4.pack(y), (codes, scales))) or torch.equal(kv4.values(*kv4.pack(y)), y)
+
+
+def test_the_oracle_of_pages():
+    """Forks share, a write to a shared page takes a copy, the last holder keeps it, and what is given back can be given out again."""
+    table, lens, refs = [[0, 1, -1], [-1] * 3, [-1] * 3], [6, 0, 0], [1, 1, 0, 0, 0]
+    pages.fork(table, lens, refs, [0, 0], [1, 2])
+    assert refs == [3, 3, 0, 0, 0] and lens == [6, 6, 6] and table[1] == table[2] == [0, 1, -1]
+    fits, copies = pages.reserve(table, lens, refs, [1, 1, 1], 4)
+    assert fits == [True] * 3 and copies == [(1, 2), (1, 3)] and refs == [3, 1, 1, 1, 0] and [r[1] for r in table] == [2, 3, 1]
+    pages.free(table, lens, refs, [0, 0, 7])
+    assert refs == [2, 1, 0, 1, 0] and lens[0] == 0
+    live, moved, copies = pages.compact(table, refs)
+    assert live == 3 and copies == [(3, 2)] and table[1] == [0, 2, -1] and refs == [2, 1, 1, 0, 0]
+    fits, copies = pages.reserve(table, lens, refs, [9, 4, 99], 4)
+    assert fits == [False] * 3 and refs == [2, 1, 1, 0, 0]     # (row 0 needs three pages of two, and row 1 comes behind it)
+    fits, copies = pages.reserve(table, lens, refs, [0, 4, 99], 4)
+    assert fits == [True, True, False] and refs == [2, 1, 1, 1, 0] and table[1] == [0, 2, 3]
+
+
+def test_the_oracle_of_the_rotation_keeps_lengths():
+    x = torch.randn(2, 3, 4, 16, dtype=torch.float64)
+    cos, sin = L.rope_table(3, 8)
+    c, s = (y.double()[None, :, None] for y in (cos, sin))
+    for inter in (False, True):
+        z = rope.turn(x, c, s, 8, inter)
+        assert torch.equal(z[..., 8:], x[..., 8:]) and torch.allclose(z.norm(dim=-1), x.norm(dim=-1), rtol=1e-6)
+        assert torch.allclose(rope.turn(z, c, -s, 8, inter), x, atol=1e-6)
