@@ -49,6 +49,15 @@ __device__ __forceinline__ void wait_all_loads() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// A store that goes past the caches where `past` says so.  (The empty statements keep the compiler from making one plain store of the two.)
+template <typename V> __device__ __forceinline__ void store_past(V* p, const V& x, bool past) {
+  if (past) {
+    asm volatile("");
+    __builtin_nontemporal_store(x, p);
+    asm volatile("");
+  } else *p = x;
+}
+
 // x, in a form the compiler cannot prove loop-invariant
 __device__ __forceinline__ int fresh_index(int x) {
   asm volatile("" : "+v"(x));

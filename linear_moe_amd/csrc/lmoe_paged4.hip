@@ -76,9 +76,8 @@ template <typename T> __device__ __forceinline__ float size_of(const typename ET
   }
 }
 template <typename T> __device__ __forceinline__ void store_frag(T* p, const typename ET<T>::frag& x, bool past) {
-  if constexpr (sizeof(T) == 2) { if (past) __builtin_nontemporal_store(x, (bf16x8*)p); else *(bf16x8*)p = x; }
-  else if (past) { __builtin_nontemporal_store(x.lo, (f32x4*)p); __builtin_nontemporal_store(x.hi, (f32x4*)(p + 4)); }
-  else { *(f32x4*)p = x.lo; *(f32x4*)(p + 4) = x.hi; }
+  if constexpr (sizeof(T) == 2) store_past((bf16x8*)p, x, past);
+  else { store_past((f32x4*)p, x.lo, past); store_past((f32x4*)(p + 4), x.hi, past); }
 }
 
 // ---- written and read: a wave per token ----
@@ -114,7 +113,7 @@ constexpr int PIECES = 2;
 struct TokenPlan {
   int nk, nv;              // pieces of k and of v
   bool past;               // what is read goes past the caches: more of it than an eighth of the last-level cache (16384 tokens, 8 heads of 128,
-                           // 67 MB: 19 -> 15 us; 64 tokens: either way)
+                           // 67 MB: 19 -> 16.5 us; 64 tokens: either way)
   uint32_t div_k, div_v;   // i / (pieces of a row) = umulhi(2 i, div) for i < 2^26, at most 32 of them
 };
 static TokenPlan token_plan(const lmoe_paged_args& a, int vec) {
@@ -223,8 +222,7 @@ template <typename T, bool BITS4> __global__ __launch_bounds__(NTHR) void k_page
       if (!s.on[u]) continue;
       T* d = row + s.h[u] * to.sh + VEC * s.c[u];
       if constexpr (BITS4) store_frag<T>(d, from4<T>(y[u].r, scale_of(y[u].scale)), p.past);
-      else if (p.past) __builtin_nontemporal_store(y[u].y, (vec*)d);
-      else *(vec*)d = y[u].y;
+      else store_past((vec*)d, y[u].y, p.past);
     }
   };
   for (int i0 = 0; i0 < max(p.nk, p.nv); i0 += 64 * PIECES) {

@@ -42,13 +42,8 @@ template <typename T, int V> struct RopeRaw {
   }
   __device__ __forceinline__ void store(T* row, int a, int b, bool past) const {
     typedef typename RopeVec<T, V>::type vec;
-    if (past) {
-      __builtin_nontemporal_store(lo, (vec*)(row + a));
-      __builtin_nontemporal_store(hi, (vec*)(row + b));
-    } else {
-      *(vec*)(row + a) = lo;
-      *(vec*)(row + b) = hi;
-    }
+    store_past((vec*)(row + a), lo, past);
+    store_past((vec*)(row + b), hi, past);
   }
   __device__ __forceinline__ float at(int i) const {
     if constexpr (V == 1) return i ? (float)hi : (float)lo;
@@ -346,7 +341,7 @@ static RopePlan rope_plan(const lmoe_rope_args& a, bool bwd) {
   p.runs_q = (a.HQ + hb - 1) / hb;
   p.runs = p.runs_q + (a.HKV + hb - 1) / hb;
   // Results of which the last-level cache would keep less than half by the time they are read go past it: 4 x 8192 tokens of 20 heads of
-  // 128 (168 MB each way), forward and backward, 192 -> 176 us; 8192 of 40 (84 MB), forward, 39 either way.
+  // 128 (168 MB each way), forward and backward, 171 -> 156 us; 8192 of 40 (84 MB), forward, 34 either way.
   p.past = tokens * heads * a.D * (a.dtype == LMOE_BF16 ? 2 : 4) > 128 << 20;
   // as many tokens for every lane group
   const int64_t items = tokens * p.runs, most = bwd ? ROPE_BWD_GROUPS : ROPE_GROUPS;
