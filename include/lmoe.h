@@ -482,7 +482,8 @@ int lmoe_paged_kv_read(const lmoe_paged_args* a, void* stream);
  * low half of byte i, 16-byte aligned rows; ks, vs [P, S, HKV, K/32 | V/32] bytes; the strides of these in bytes.  A half byte is a
  * sign (8) and one of 0 0.5 1 1.5 2 3 4 6; the 32 columns of a scale byte x stand for that times 2^(x - 127), for x = 255 for NaN.  What is
  * written: the least x in 7 .. 252 for which nothing is above 6 (above 6 at 252: 6), the nearest number, of two as near the one whose half
- * byte is even; 255 where one of the 32 is infinite or NaN.  The new token is attended to as the cache holds it. */
+ * byte is even; 255 where one of the 32 is infinite or NaN.  The new token is attended to as the cache holds it.  Two tokens of one call
+ * that share a position leave bytes of either there. */
 typedef struct lmoe_paged4_args {
   lmoe_paged_args p;
   lmoe_tensor ks, vs;
@@ -521,7 +522,7 @@ int lmoe_qk_norm_rope_bwd(const lmoe_rope_args* a, void* stream);
 
 /* The pages of a cache, kept by a table [N, M] (row stride table_stride) of page numbers, lens [N] and refs [P]: how many entries (and
  * holds of the program itself) name a page, 0 for a free one.  A number outside 0 .. P - 1 names no page.  Every result is the same
- * whatever order the card takes; nothing is read by the host.
+ * whatever order the card takes; nothing is read by the host.  N <= 65535, forks at most as many, N * M <= 2^30.
  * lmoe_paged_free: the rows rows[F] give their pages back (refs - 1, entry -1) and get lens 0; a number outside 0 .. N - 1 is left out.
  * lmoe_paged_fork: for all i at once row rows[i] becomes what row src[i] was (entries and lens), refs follow; of several for one
  *   row the last counts.  ws: lmoe_paged_fork_ints int32.

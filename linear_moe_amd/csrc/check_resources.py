@@ -32,6 +32,8 @@ GUARDED = {
     "k_attn_fwd": 2,          # two work-groups of 4 waves per CU, or one of 8: a spill in the loop waits for the tiles in flight
     "k_attn_bwd_dq": 2,
     "k_attn_bwd_dkv": 2,      # one work-group of 8 waves per CU; 64 columns: three of 4, see FLOORS
+    "k_paged4_attn": 2,       # two work-groups of 4 waves per CU at least, three with 128 columns in 2-byte elements
+    "k_qk_norm_rope": 2,      # backward: two work-groups of 4 waves per CU
     "k_bwd_dqkv": 2,          # one work-group of 8 waves per CU; its first version spilled loop-invariant lane arithmetic
 }
 ANY_TYPE = ("k_state_bwd", "k_state_fwd_chunks")

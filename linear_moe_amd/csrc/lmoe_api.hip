@@ -866,6 +866,7 @@ int lmoe_qk_norm_rope_bwd(const lmoe_rope_args* a, void* stream) {
 static int check_pages(const lmoe_pages_args* a, const char* op, bool rows, bool bufs) {
   if (!a) return fail(-1, "%s: null argument block", op);
   if (a->N < 0 || a->M < 0 || a->P < 0 || a->F < 0 || a->n_bufs < 0 || (bufs && a->S <= 0)) return fail(-4, "%s: negative dimension", op);
+  if (a->N > 65535) return fail(-8, "%s: N must be <= 65535", op);
   if ((int64_t)a->N * a->M > 1 << 30) return fail(-8, "%s: a table of %d x %d: at most 2^30 entries", op, a->N, a->M);
   if (a->F >= MAX_GROUPS) return fail(-8, "%s: more than 2^24 - 1 rows", op);
   if (bufs && (int64_t)a->M * a->S > 1 << 30) return fail(-8, "%s: %d pages of %d tokens per sequence: positions must stay below 2^30", op, a->M, a->S);
@@ -901,6 +902,7 @@ int lmoe_paged_fork(const lmoe_pages_args* a, void* stream) {
   const char* op = "lmoe_paged_fork";
   if (int r = check_pages(a, op, true, false)) return r;
   if (a->F == 0 || a->N == 0) return 0;
+  if (a->F > 65535) return fail(-8, "%s: more than 65535 forks", op);
   if (!a->src) return fail(-7, "%s: src must not be null", op);
   if (!a->ws) return fail(-11, "%s: ws must not be null", op);
   lmoe::launch_pages_fork(*a, (hipStream_t)stream);

@@ -493,7 +493,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
         s[b][e] = pow2(s[b][e] - m);
         sum += s[b][e];
       }
-    // (P rounded to the element type, as the products take it; the sum is of the numbers before)
+    // (P rounded to the element type, as the products take it; the sum is of the numbers before.  What the rounding leaves, as two more
+    // products, would take the error of o from 0.0023 of its size to the 0.0017 of its own rounding: 49 -> 51 us, and 49 it is, as in a
+    // cache of 2-byte elements.)
     typename ET<T>::frag pf;
     if constexpr (FAST) pf = frag_of_blocks(s[0], s[1]); else { pf.lo = s[0]; pf.hi = s[1]; }
     pv4<T, W, 0>(o, t, pf);

@@ -18,7 +18,8 @@ In 4 bits (``k_scales``, ``v_scales`` given): ``k_pages`` ``[P, S, HKV, K/2]`` a
 multiples of 32.  32 columns share a power of two 2^(scale - 127); a column is one of 0 0.5 1 1.5 2 3 4 6 times it, with a sign (8), the even
 column in the low half of a byte.  Written is the least scale for which no column is above 6 (7 to 252), and of the numbers the
 nearest, of two as near the even one; a NaN or infinity makes the 32 columns NaN.  The new token of ``paged_attn_decode`` is attended to as the
-cache holds it.  A row takes 17/64 of the bytes of bfloat16.  Fastest are pages in which all tokens of a head lie next to each other
+cache holds it.  A row takes 17/64 of the bytes of bfloat16.  Two tokens of one call that share a
+position (a page that two sequences share: ``paged_reserve`` parts them) leave bytes of either there.  Fastest are pages in which all tokens of a head lie next to each other
 (``torch.empty(P, HKV, S, K // 2).transpose(1, 2)``).
 """
 from __future__ import annotations

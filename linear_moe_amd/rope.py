@@ -142,6 +142,7 @@ def qk_norm_rope(
     q ``[B,HQ,T,D]``, k ``[B,HKV,T,D]`` (``[B,T,H,D]`` with ``head_first=False``), bfloat16 or float32, any strides (views of one projection are
     read in place); any numbers of heads; D even, up to 256.  Returns both, laid out like q and k, contiguous.
 
+    The squares of a row are summed in float32: for sizes from 1e-18 to 1e18.
     q_weight, k_weight: ``[D]``, bfloat16 or float32, or none; ``norm=False``: rotation alone.
     cos, sin: ``[L, R/2]`` (``rope_table``; float32, others are converted), not trained; none: norm alone.  A token's row is its position inside its
     sequence, and so many more as ``offsets`` (``[N]`` whole numbers on the device: what the cache holds already) says; or what ``positions``
