@@ -250,10 +250,20 @@ void launch_paged_read(const lmoe_paged4_args& a, bool bits4, hipStream_t st) {
 }
 
 // ---- one new token ----
-// Work-groups go round the eight XCDs.  Where the heads of a token lie next to each other, two rows of 64 bytes share a cache line: then the
-// heads of a stretch follow each other on one XCD, and the line comes once from memory (64 sequences of 1024 to 4096 tokens, 32 / 8
-// heads of 128: 72 -> 62 us; where the tokens of a head lie next to each other, 49 -> 50).
+// Work-groups go round the eight XCDs in the order of their index.  First come the first stretches of all, then the second ones: those that a
+// sequence does not have come last, and what each XCD gets does not depend on how many stretches the table has room for (192 sequences
+// of 1024 tokens in a table of one page more, two stretches of which one is empty: with the stretches of a head next to each other half of
+// the XCDs had nothing to do, 71 us, so 60).  Every so many stretches they shift by one, so that a long sequence is on all XCDs.
+// Where the heads of a token lie next to each other, two rows of 64 bytes share a cache line: then the heads of a stretch follow each
+// other on one XCD, and the line comes once from memory (64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 72 -> 62 us; where the
+// tokens of a head lie next to each other, 49 -> 50).
 constexpr int XCDS = 8;
+// place x of the `count` that share stretch `part` (count is a multiple of some power of two up to 8: after 8 / that many stretches an
+// XCD would meet the same ones again)
+__device__ __forceinline__ uint32_t shifted(uint32_t x, uint32_t part, uint32_t count) {
+  const uint32_t same = min(count & -count, (uint32_t)XCDS);
+  return (x + part * same / XCDS) % count;
+}
 __host__ __device__ inline bool heads_near(const lmoe_paged_args& a, const PagedPlan& p) {
   const int64_t units = (int64_t)a.N * p.splits;
   return a.HKV > 1 && a.kp.sh < a.kp.st && units >= XCDS && units * a.HKV * p.blocks <= 1 << 22;
@@ -261,14 +271,15 @@ __host__ __device__ inline bool heads_near(const lmoe_paged_args& a, const Paged
 static PagedPlan paged4_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
-  const int64_t bound = (int64_t)a.M * a.S + 1, groups = (int64_t)a.N * a.HKV * p.blocks;
+  const int64_t bound = (int64_t)a.M * a.S + (a.kn.ptr ? 1 : 0), groups = (int64_t)a.N * a.HKV * p.blocks;
   // A short cache: one stretch of eight waves and no second launch; else stretches of one length, whatever the call (us for stretches of
   // 512, 1024, 2048 positions, with the join: 64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 55 54 58; 2 of 32 K and 128 K,
   // 16 / 4 heads of 128: 33 29 39).
-  // (a launch has less than 2^32 threads: of 2^23 work-groups and more, which N * HQ < 2^24 allows, none has 512)
-  p.waves = bound <= 1024 && groups < 1 << 23 ? 8 : 4;
+  // Eight waves leave a CU one work-group: for one a CU at most (16 / 4 heads of 128, with eight and with four waves: 1 sequence of 500 tokens
+  // 7.4 and 7.9 us, 64 of 1000 11.4 and 12.2, 100 of 1000 19.0 and 15.7).
+  p.waves = bound <= 1024 && groups <= 256 ? 8 : 4;
   const int64_t chunk = 1024;
-  const int64_t splits = (bound + chunk - 1) / chunk;
+  const int64_t splits = bound > 0 ? (bound + chunk - 1) / chunk : 1;
   const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;
   p.splits = (int)(splits < most ? splits : most);
   p.chunk = (int)chunk;
@@ -324,24 +335,28 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   __shared__ __attribute__((aligned(16))) float s_o[NW][PHEADS][W + 4];
   __shared__ float s_m[NW][PHEADS], s_l[NW][PHEADS];
   const int G = a.HQ / a.HKV, per = a.HKV * p.blocks;
-  int unit, hb;
+  int part, n, hb;
   if (heads_near(a, p)) {
-    const int y = blockIdx.x / XCDS;
-    unit = y / per * XCDS + blockIdx.x % XCDS;
+    const int y = blockIdx.x / XCDS, unit = y / per * XCDS + blockIdx.x % XCDS;
     hb = y % per;
-    if (unit >= a.N * p.splits) return;
-  } else {                               // (the order of k_paged_attn)
-    unit = blockIdx.x / p.splits / per * p.splits + blockIdx.x % p.splits;
-    hb = blockIdx.x / p.splits % per;
+    part = unit / a.N;
+    n = shifted(unit % a.N, part, a.N);
+    if (part >= p.splits) return;
+  } else {
+    const uint32_t groups = (uint32_t)a.N * per;
+    part = blockIdx.x / groups;
+    const int group = shifted(blockIdx.x % groups, part, groups);
+    n = group / per;
+    hb = group % per;
   }
-  const int part = unit % p.splits, n = unit / p.splits, hk = hb / p.blocks;
+  const int hk = hb / p.blocks;
   const int h0 = hb % p.blocks * PHEADS, heads = min(PHEADS, G - h0);      // of the key head's group
+  const int32_t* table = a.table + (int64_t)n * a.table_stride;
   const PagedSeq sq = paged_seq(a, p, n);
   const int total = sq.len + (a.kn.ptr ? 1 : 0), begin = part * sq.chunk;
   if (begin >= total && part > 0) return;
   const int stop = min(total, begin + sq.chunk), end = a.P > 0 ? min(stop, sq.len) : begin;       // the stretch, and its part in the cache
   const int l = lane_id(), w = wave_id(), c = l & 15, g = l >> 4;
-  const int32_t* table = a.table + (int64_t)n * a.table_stride;
   const uint8_t* kp = (const uint8_t*)a.kp.ptr + (int64_t)hk * a.kp.sh;
   const uint8_t* vp = (const uint8_t*)a.vp.ptr + (int64_t)hk * a.vp.sh;
   const uint8_t* ksp = (const uint8_t*)a4.ks.ptr + (int64_t)hk * a4.ks.sh;
@@ -352,25 +367,21 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   // steps before its rows are used, as in k_paged_attn.
   struct Where { int id[2], slot[2]; };
   auto column = [&](int j) { return (int)((__umulhi((uint32_t)j, p.div_m) + (uint32_t)j) >> p.div_s); };
+  // (without a condition: behind the stretch, the last column's)
   auto ask = [&](int j0) {
-    Where x = {{-1, -1}, {0, 0}};
+    Where x;
     if constexpr (EVEN) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int j = j0 + 16 * b;
-        if (j < end) {
-          const int col = column(j);
-          x.slot[b] = j - col * a.S;
-          x.id[b] = as_const(table)[col];
-        }
+        const int col = min(column(j0 + 16 * b), a.M - 1);
+        x.slot[b] = j0 + 16 * b - col * a.S;
+        x.id[b] = as_const(table)[col];
       }
     } else {
-      const int j = j0 + (l & 31);
-      if (j < end) {
-        const int col = column(j);
-        x.slot[0] = j - col * a.S;
-        x.id[0] = table[col];
-      }
+      const int j = j0 + (l & 31), col = min(column(j), a.M - 1);
+      x.slot[0] = j - col * a.S;
+      x.id[0] = table[col];
+      x.id[1] = x.slot[1] = 0;
     }
     return x;
   };
@@ -399,19 +410,19 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
       t.live = 0;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const bool there = x.id[b] >= 0 && x.id[b] < a.P;
+        const int left = min(16, end - j0 - 16 * b);          // positions of the half
+        const bool there = left > 0 && x.id[b] >= 0 && x.id[b] < a.P;
         const uint32_t id = there ? x.id[b] : 0, slot = there ? x.slot[b] : 0;
         auto row = [&](const uint8_t* base, const lmoe_tensor& y) { return base + (uint64_t)id * (uint32_t)y.sb + slot * (uint32_t)y.st; };
         k_row(b, row(kp, a.kp) + ko, row(ksp, a4.ks) + kso);
         vb[b] = row(vp, a.vp);
         vsb[b] = row(vsp, a4.vs);
-        const int left = min(16, end - j0 - 16 * b);          // positions of the half
         if (there) t.live |= ((1u << left) - 1) << (16 * b);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) v_row(e, vb[e >> 2] + vo[e & 3], vsb[e >> 2] + vso[e & 3]);
     } else {
-      const bool there = x.id[0] >= 0 && x.id[0] < a.P;
+      const bool there = j0 + (l & 31) < end && x.id[0] >= 0 && x.id[0] < a.P;
       t.live = (uint32_t)__ballot(there);
       const int my_id = there ? x.id[0] : 0, my_slot = there ? x.slot[0] : 0;
 #pragma unroll
@@ -429,7 +440,12 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   };
 
   int j0 = begin + PSTEP * w;
-  Where at = ask(j0), ahead = ask(j0 + PGROUP);
+  if (a.M == 0) j0 = end;
+  Where at = {}, ahead = {};
+  if (a.M > 0) {
+    at = ask(j0);
+    ahead = ask(j0 + PGROUP);
+  }
 
   typename ET<T>::frag q[KW];
   const int hq = hk * G + h0 + min(c, heads - 1);
