@@ -170,8 +170,8 @@ __device__ __forceinline__ bool asked(const lmoe_pages_args& a, int n, int& firs
 // of it are asked for too, has to be copied if r - e > 1, for those have taken their copies by then.  So of the asked entries of a page all are
 // copied, but the last where there are r of them.
 // The asked entries of PAGES_NTHR rows at a time are dealt to the threads; where the call has one for a thread, it stays in its registers
-// from the first step to the last (256 rows of one token, 41 thousand pages: 8 us; with a wave for every row, which waits for its entries again
-// in each step, 115).
+// from the first step to the last (256 rows of one token, 128 of them forks, 41 thousand pages: 12 us; with a wave for every row, which waits
+// for its entries again in each step, 115).
 struct Asked { int n, c, x, refs; bool last; };      // row, column, entry, refs of its page (0: none), whether the row's last
 __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_args a) {
   __shared__ ListShared sh;

@@ -5,7 +5,7 @@ layers' rotary autograd function, never by the linear-attention layers): resolve
 def apply_rotary(*args, **kwargs):
     raise NotImplementedError(
         "fla.ops.rotary.apply_rotary: rotary embeddings are not on the linear-attention path and are not provided "
-        "by linear_moe_amd")
+        "under this name: linear_moe_amd.qk_norm_rope turns queries and keys")
 
 
 __all__ = ["apply_rotary"]
