@@ -1443,10 +1443,10 @@ struct RopeNode : torch::autograd::Node {
   std::string name() const override { return "QkNormRopeBackward"; }
   void save(int i, const Tensor& x) {
     if (!x.defined()) return;
-    given[i] = true;
     types[i] = x.scalar_type();
     shapes[i].assign(x.sizes().begin(), x.sizes().end());
-    saved[i] = torch::autograd::SavedVariable(x, false);
+    given[i] = a.norm || i > K;                    // (a rotation alone is turned back without q and k)
+    if (given[i]) saved[i] = torch::autograd::SavedVariable(x, false);
   }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
@@ -1480,7 +1480,8 @@ struct RopeNode : torch::autograd::Node {
         if (grads[i].defined()) {
           TORCH_CHECK(grads[i].sizes() == at::IntArrayRef(shapes[i]) && grads[i].device() == device, "qk_norm_rope backward: a gradient of another shape or device");
           dz[i] = as(grads[i], types[i]);
-        } else dz[i] = at::zeros(shapes[i], x[i].options().requires_grad(false));
+        } else dz[i] = at::zeros(shapes[i], grads[1 - i].options().dtype(types[i]).requires_grad(false));
+        if (!given[i]) x[i] = dz[i];
       }
       lmoe_rope_args b = a;
       b.q = desc(x[Q], head_first); b.k = desc(x[K], head_first); b.qw = ptr(x[QW]); b.kw = ptr(x[KW]);

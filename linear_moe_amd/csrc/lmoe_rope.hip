@@ -152,7 +152,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
 #pragma unroll
     for (int i = 0; i < 2 * V; ++i) sum[j][i] = 0.f;
   }
-  const lmoe_tensor from = isq ? a.q : a.k, to = BWD ? (isq ? a.dq : a.dk) : (isq ? a.zq : a.zk), grad = isq ? a.dzq : a.dzk;
+  // (a rotation alone has no use for x on the way back: the gradient again, which costs nothing)
+  const lmoe_tensor from = BWD && !a.norm ? (isq ? a.dzq : a.dzk) : (isq ? a.q : a.k), to = BWD ? (isq ? a.dq : a.dk) : (isq ? a.zq : a.zk), grad = isq ? a.dzq : a.dzk;
   const float over = 1.0f / (float)a.D;
   const uint32_t tokens = (uint32_t)a.B * (uint32_t)a.T;
   // (all lanes of a row go the same way; a group past the last whole set of runs has nothing to do)

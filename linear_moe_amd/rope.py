@@ -90,9 +90,10 @@ class _QkNormRope(torch.autograd.Function):
         ws = [None if w is None else w.detach().contiguous() for w in (qw, kw)]
         q_, k_, zq, zk = call.forward(q, k, *ws)
         ctx.call = call
-        saved = (q_, k_, *ws, *call.tables)
+        saved = (*((q_, k_) if call.norm else (None, None)), *ws, *call.tables)         # (a rotation alone is turned back without q and k)
         ctx.save_for_backward(*saved)
         ctx.like = [None if x is None else (tuple(x.shape), x.dtype) for x in saved]
+        ctx.shapes, ctx.dtype = (q.shape, k.shape), q.dtype
         return zq, zk
 
     @staticmethod
@@ -101,7 +102,9 @@ class _QkNormRope(torch.autograd.Function):
         call, dev = ctx.call, dzq.device
         names = "q k q_weight k_weight cos sin positions offsets cu_seqlens".split()
         q, k, qw, kw, *tables = (None if like is None else _back(x, *like, dev, n) for x, like, n in zip(ctx.saved_tensors, ctx.like, names))
-        dzq, dzk = _back(dzq, q.shape, q.dtype, dev, "the gradient of q"), _back(dzk, k.shape, k.dtype, dev, "the gradient of k")
+        dzq, dzk = (_back(x, s, ctx.dtype, dev, f"the gradient of {n}") for x, s, n in zip((dzq, dzk), ctx.shapes, "qk"))
+        if not call.norm:
+            q, k = dzq, dzk
         dq, dk = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
         dqw, dkw = (torch.empty_like(w) if w is not None and ctx.needs_input_grad[i] else None for i, w in ((2, qw), (3, kw)))
         if q.numel():

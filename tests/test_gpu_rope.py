@@ -198,6 +198,39 @@ def test_one_weight_and_one_gradient(cuda):
     assert torch.equal(g[0], full[0]) and (g[1] is None or (g[1] == 0).all())
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_a_rotation_alone_keeps_nothing_of_its_input(cuda, interleaved):
+    """Its gradient is the gradient turned back: q and k may be overwritten in between, in the node in native code and the one in Python."""
+    cos, sin = L.rope_table(7, 64, device=cuda)
+    for table in ((cos, sin), (cos.double(), sin.double())):             # (a table in 64 bits takes the path in Python)
+        leaf = [gen(70 + i, 2, 7, h, 64, dtype=BF16).to(cuda).requires_grad_(True) for i, h in enumerate((4, 2))]
+        q, k = (x * 1.0 for x in leaf)
+        z = L.qk_norm_rope(q, k, None, None, *table, norm=False, interleaved=interleaved, head_first=False)
+        with torch.no_grad():
+            q.zero_(), k.fill_(float("nan"))
+        dz = [gen(75 + i, *x.shape, dtype=BF16).to(cuda) for i, x in enumerate(z)]
+        got = torch.autograd.grad(z, leaf, dz)
+        back = L.qk_norm_rope(*dz, None, None, cos, -sin, norm=False, interleaved=interleaved, head_first=False)
+        assert all(torch.equal(a, b) for a, b in zip(got, back))
+        z = L.qk_norm_rope(*(x * 1.0 for x in leaf), None, None, *table, norm=False, interleaved=interleaved, head_first=False)
+        g = torch.autograd.grad(z[1], leaf, dz[1], allow_unused=True)
+        assert torch.equal(g[1], back[1]) and (g[0] is None or (g[0] == 0).all())
+
+
+def test_the_node_in_python_gives_the_same_bits(cuda):
+    """A call that needs a conversion takes the steps in Python."""
+    q, k, w = (gen(90 + i, *s, dtype=BF16).to(cuda) for i, s in enumerate(((2, 9, 4, 64), (2, 9, 2, 64), (64,))))
+    cos, sin = L.rope_table(40, 64, device=cuda)
+    offs = torch.tensor([3, 30], dtype=torch.int32, device=cuda)
+    out = []
+    for c, s, o in ((cos, sin, offs), (cos.double(), sin.double(), offs.long())):
+        leaves = [x.clone().requires_grad_(True) for x in (q, k, w, w)]
+        z = L.qk_norm_rope(*leaves, c, s, offsets=o, head_first=False)
+        out.append([*z, *torch.autograd.grad(z, leaves, [torch.ones_like(x) for x in z])])
+    assert type(out[0][0].grad_fn) is not type(out[1][0].grad_fn)
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def test_no_tokens(cuda):
     cos, sin = L.rope_table(4, 64, device=cuda)
     w = torch.ones(64, device=cuda, requires_grad=True)
