@@ -1215,11 +1215,12 @@ struct Pages {
     a.table = (int32_t*)table.data_ptr(); a.lens = (int32_t*)ptr(lens); a.refs = (int32_t*)refs.data_ptr();
     return true;
   }
-  // the tensors of the pages: as paged_pages.py takes them apart
-  bool take_pages(PyObject* o) {
+  // the tensors of the pages: as paged_pages.py takes them apart; least: of them
+  bool take_pages(PyObject* o, Py_ssize_t least) {
     const bool one = THPVariable_CheckExact(o);
     NEED(one || PyTuple_CheckExact(o) || PyList_CheckExact(o));
     const Py_ssize_t count = one ? 1 : PySequence_Fast_GET_SIZE(o);
+    NEED(count >= least);
     pages.resize(count); bufs.resize(count);
     for (Py_ssize_t i = 0; i < count; ++i) {
       Tensor& x = pages[i];
@@ -1302,7 +1303,7 @@ PyObject* pages_reserve(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pages c;
   Tensor tokens;
-  if (n != 6 || !c.take(o[0], o[1], o[2]) || !c.take_pages(o[3])) return elsewhere();
+  if (n != 6 || !c.take(o[0], o[1], o[2]) || !c.take_pages(o[3], 1)) return elsewhere();
   if (PyLong_CheckExact(o[4])) {
     const int64_t each = PyLong_AsLongLong(o[4]);
     if (PyErr_Occurred() || !fits(each)) return elsewhere();
@@ -1333,7 +1334,7 @@ PyObject* pages_reserve(PyObject*, PyObject* const* o, Py_ssize_t n) {
 PyObject* pages_compact(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pages c;
-  if (n != 4 || !c.take(o[0], nullptr, o[1]) || !c.take_pages(o[2])) return elsewhere();
+  if (n != 4 || !c.take(o[0], nullptr, o[1]) || !c.take_pages(o[2], 0)) return elsewhere();
   void* st = stream_of(o[3]);
   if (PyErr_Occurred()) return elsewhere();
   const int64_t ints = lib.pages_ints(&c.a);

@@ -107,6 +107,8 @@ def paged_reserve(
     dev = page_table.device
     pages, held = _bufs(pages, a, dev, name)
     _no_grad(name, *pages)
+    if not pages:
+        raise ValueError(f"{name}: at least one tensor of the pages is needed, which says how many tokens a page has")
     if isinstance(tokens, torch.Tensor):
         tokens = ints_of(tokens, a.N, dev, f"{name}: tokens")
         a.tokens = tokens.data_ptr()

@@ -241,6 +241,22 @@ def test_graph(cuda):
             d[1].add_(more).clamp_(max=M * S - 1)
 
 
+def test_the_path_in_python_does_the_same(cuda):
+    """Calls that need a conversion (numbers of 64 bits, a generator of tensors)."""
+    for native in (True, False):
+        st = State(cuda, 80, 6, 8, 60, 4, shapes=((2, 16), (3,)), dtypes=(torch.bfloat16, torch.uint8))
+        conv = (lambda x: x) if native else (lambda x: x.long())
+        pages = lambda: tuple(st.d_pages) if native else (p for p in st.d_pages)
+        L.paged_free(st.d_table, st.d_lens, st.d_refs, conv(st.ints([1, 1, 9])))
+        L.paged_fork(st.d_table, st.d_lens, st.d_refs, conv(st.ints([0, 2])), conv(st.ints([1, 4])))
+        fits = L.paged_reserve(pages(), st.d_table, st.d_lens, st.d_refs, conv(st.ints([1, 2, 3, 4, 5, 6])))
+        live, moved = L.paged_compact(pages(), st.d_table, st.d_refs)
+        got = [st.d_table, st.d_lens, st.d_refs, fits, live, moved, *st.d_pages]
+        if native:
+            first = got
+    assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
 def test_nothing(cuda):
     i32 = dict(dtype=torch.int32, device=cuda)
     none = torch.zeros(0, **i32)
@@ -275,6 +291,8 @@ def test_refusals(cuda):
     for change in (dict(src=rows[:1]), dict(src=rows.float()), dict(dst=rows[None]), dict(dst=rows.cpu())):
         with pytest.raises(ValueError):
             L.paged_fork(**{**state, **dict(src=rows, dst=rows), **change})
+    with pytest.raises(ValueError):
+        L.paged_reserve((), **state, tokens=1)
     with pytest.raises(ValueError):
         L.paged_free(**state, rows=rows[None])
     with pytest.raises(RuntimeError):
