@@ -499,8 +499,8 @@ int lmoe_paged4_kv_read(const lmoe_paged4_args* a, void* stream);
  * i < R / 2 (R = 0: no rotation); columns from R on as they are.  The position p of token t of row b: positions[b * pos_stride + t] where
  * given, else t + offsets[b] (offsets NULL: 0); packed input (cu_seqlens [N + 1], B = 1): that inside its sequence.  p outside 0 .. L - 1:
  * not rotated.  Rows behind the last sequence are zero in every result.  D <= 256, D and R even; any strides with adjacent columns.
- * bwd: q, k (without norm: not read) and the gradients dzq, dzk in; dq, dk and (where their pointers are given) dqw, dkw out; ws: lmoe_qk_norm_rope_floats fp32 numbers
- * (0: may be NULL).  The reference's rotary: linear_moe/model/common_modules/rotary.py:40-98. */
+ * bwd: q, k (without norm: not read, may be NULL) and the gradients dzq, dzk in; dq, dk and (where their pointers are given) dqw, dkw
+ * out; ws: lmoe_qk_norm_rope_floats fp32 numbers (0: not touched, may be NULL).  Without tokens nothing is done: dqw, dkw stay as they were.  The reference's rotary: linear_moe/model/common_modules/rotary.py:40-98. */
 typedef struct lmoe_rope_args {
   int32_t dtype;       /* of q, k, their results and gradients                         */
   int32_t w_dtype;     /* of qw, kw, dqw, dkw                                          */

@@ -835,7 +835,7 @@ static int check_rope(const lmoe_rope_args* a, const char* op, bool bwd) {
   if ((int64_t)a->B * a->T > 1 << 30) return fail(-8, "%s: more than 2^30 tokens", op);
   if (a->cu_seqlens && (a->B != 1 || a->positions)) return fail(-5, "%s: packed input needs B == 1 and no positions", op);
   if (a->positions && a->offsets) return fail(-5, "%s: positions and offsets exclude each other", op);
-  if (!a->q.ptr || !a->k.ptr) return fail(-7, "%s: q and k must not be null", op);
+  if ((!bwd || a->norm) && (!a->q.ptr || !a->k.ptr)) return fail(-7, "%s: q and k must not be null", op);
   if (a->R > 0 && a->L > 0 && (!a->cos || !a->sin)) return fail(-7, "%s: cos and sin must not be null", op);
   if (!(a->eps >= 0.f)) return fail(-15, "%s: eps must not be negative", op);
   if (!a->norm && (a->qw || a->kw || a->dqw || a->dkw)) return fail(-15, "%s: weights belong to the norm", op);

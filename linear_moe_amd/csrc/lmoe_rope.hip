@@ -272,7 +272,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
   }
   if constexpr (BWD) {
     // dw: the lane groups of the work-group in their order, into its row of ws
-    if (!a.ws) return;
+    if (!a.dqw && !a.dkw) return;
     constexpr int E = 2 * V * NC;
     __shared__ float part[NTHR][E + 1];
     __shared__ uint8_t of_q[NTHR / L];

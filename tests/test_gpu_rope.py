@@ -1,8 +1,11 @@
 """Norm and rotation of queries and keys on the GPU, against float64 within derived bounds (oracle/rope.py)."""
+import ctypes as C
+
 import pytest
 import torch
 
 import linear_moe_amd as L
+from linear_moe_amd import _lib
 from oracle import rope
 from tests.util import gen
 
@@ -231,6 +234,24 @@ def test_the_node_in_python_gives_the_same_bits(cuda):
     assert all(torch.equal(a, b) for a, b in zip(*out))
 
 
+def test_a_workspace_that_is_not_needed_is_left_alone(cuda):
+    """The block of a backward pass without gradients of weights asks for no workspace; one that is given all the same is not written."""
+    q, k, dq, dk = (gen(100 + i, 2, 5, h, 64, dtype=BF16).to(cuda) for i, h in enumerate((4, 2, 4, 2)))
+    a, out, ws = _lib.RopeArgs(), [torch.empty_like(q), torch.empty_like(k)], torch.full((4096,), 7.0, device=cuda)
+    a.dtype = a.w_dtype = _lib.LMOE_BF16
+    a.B, a.T, a.HQ, a.HKV, a.D, a.N, a.norm, a.eps = 2, 5, 4, 2, 64, 2, 1, 1e-6
+    for n, x in dict(q=q, k=k, dzq=dq, dzk=dk, dq=out[0], dk=out[1]).items():
+        setattr(a, n, _lib.Tensor4(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)))
+    lib = _lib.load()
+    assert lib.lmoe_qk_norm_rope_floats(C.byref(a)) == 0
+    a.ws = ws.data_ptr()
+    assert lib.lmoe_qk_norm_rope_bwd(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    assert (ws == 7).all()
+    leaves = [x.clone().requires_grad_(True) for x in (q, k)]
+    got = torch.autograd.grad(L.qk_norm_rope(*leaves, head_first=False), leaves, [dq, dk])
+    assert all(torch.equal(x, y) for x, y in zip(got, out))
+
+
 def test_no_tokens(cuda):
     cos, sin = L.rope_table(4, 64, device=cuda)
     w = torch.ones(64, device=cuda, requires_grad=True)
@@ -315,3 +336,56 @@ def test_refusals(cuda):
     offs += 1
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         z.sum().backward()
+
+
+def test_transforms_are_refused(cuda):
+    from torch.autograd import forward_ad as fw
+    q, k = gen(110, 2, 3, 4, 64).to(cuda), gen(111, 2, 3, 2, 64).to(cuda)
+    cos, sin = L.rope_table(3, 64, device=cuda)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: L.qk_norm_rope(x, k, None, None, cos, sin, head_first=False)[0])(q[None])
+    with pytest.raises(RuntimeError), fw.dual_level():
+        L.qk_norm_rope(fw.make_dual(q, torch.ones_like(q)), k, None, None, cos, sin, head_first=False)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_hooks_on_what_is_saved(cuda, native):
+    """What a hook hands back may lie anywhere and have another type; another shape is noticed."""
+    q, k, w = gen(120, 2, 3, 4, 64).to(cuda), gen(121, 2, 3, 2, 64).to(cuda), gen(122, 64).to(cuda)
+    cos, sin = L.rope_table(9, 64, device=cuda)
+    offs = torch.tensor([1, 6], dtype=torch.int32 if native else torch.int64, device=cuda)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, w)]
+    call = lambda: L.qk_norm_rope(*leaves, None, cos, sin, offsets=offs, head_first=False)
+    ones = lambda z: [torch.ones_like(x) for x in z]
+    z = call()
+    want = torch.autograd.grad(z, leaves, ones(z))
+    away = lambda x: (x.cpu().double() if x.is_floating_point() else x.cpu().long()).transpose(0, -1).contiguous()
+    with torch.autograd.graph.saved_tensors_hooks(away, lambda x: x.transpose(0, -1).to(cuda)):
+        z = call()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(z, leaves, ones(z)), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x[:1]):
+        z = call()
+    with pytest.raises(RuntimeError, match="came back as"):
+        torch.autograd.grad(z, leaves, ones(z))
+
+
+def test_two_at_once(cuda):
+    """Calls on two streams at the same time, forward and backward, and in inference mode: the bits of each by itself."""
+    q, k, w = gen(130, 4, 700, 8, 128, dtype=BF16).to(cuda), gen(131, 4, 700, 2, 128, dtype=BF16).to(cuda), gen(132, 128, dtype=BF16).to(cuda)
+    cos, sin = L.rope_table(700, 128, device=cuda)
+
+    def step():
+        leaves = [x.clone().requires_grad_(True) for x in (q, k, w, w)]
+        z = L.qk_norm_rope(*leaves, cos, sin, head_first=False)
+        return [*z, *torch.autograd.grad(z, leaves, [q, k])]
+    want = step()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for x in got for a, b in zip(x, want))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(L.qk_norm_rope(q, k, w, w, cos, sin, head_first=False), want))

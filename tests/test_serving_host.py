@@ -55,6 +55,13 @@ def test_norm_and_rotation_blocks_that_are_refused(code, kw):
     assert lib.lmoe_qk_norm_rope_floats(C.byref(rope_args(**kw))) == code
 
 
+def test_a_rotation_alone_needs_no_input_on_the_way_back():
+    lib = _lib.load()
+    a = rope_args(norm=0, qw=None, kw=None, dqw=None, dkw=None, ws=None, q=_lib.Tensor4(), k=_lib.Tensor4(), T=0)
+    assert lib.lmoe_qk_norm_rope_bwd(C.byref(a), None) == 0 and lib.lmoe_qk_norm_rope_floats(C.byref(a)) == 0
+    assert lib.lmoe_qk_norm_rope_fwd(C.byref(a), None) == -7
+
+
 def test_norm_and_rotation_blocks_of_one_way():
     lib = _lib.load()
     fwd, bwd = lib.lmoe_qk_norm_rope_fwd, lib.lmoe_qk_norm_rope_bwd
