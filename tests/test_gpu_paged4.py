@@ -162,6 +162,68 @@ def test_many_sequences_and_heads_next_to_each_other(cuda):
         decode_and_check(cuda, Cache4(15, [2500, 1, 1100, 40, 2048, 1024, 0, 7, 1025], 16, 2, 64, 64, heads_first=heads_first), 2, 64, 64, BF16)
 
 
+@pytest.mark.parametrize("heads_first", [True, False])
+@pytest.mark.parametrize("cols", [129, 257, 1100, 12800])
+def test_tables_wider_than_their_sequences(cuda, cols, heads_first):
+    """2 to 64 stretches that the table has room for, of which the sequences have none to four."""
+    c = Cache4(19, [2500, 1, 0, 1024, 1025, 4000], 16, 2, 64, 64, heads_first=heads_first)
+    if cols < c.table.shape[1]:
+        c = Cache4(20, [2000, 1, 0, 1024, 1025], 16, 2, 64, 64, heads_first=heads_first)
+    c.table = torch.cat([c.table, torch.full((len(c.lens), max(cols - c.table.shape[1], 0)), -1, dtype=torch.int32)], 1)
+    decode_and_check(cuda, c, 4, 64, 64, BF16, append=True)
+
+
+def test_fewer_stretches_than_a_long_sequence_would_have(cuda):
+    """So many sequences and heads that a stretch is longer than it is for a few."""
+    decode_and_check(cuda, Cache4(21, [9000] + [i % 4 for i in range(1499)], 16, 2, 32, 32), 2, 32, 32, BF16)
+    N, HKV, D, S = 256, 64, 32, 16                                       # one stretch each, whatever its length
+    lens = [1500] + [(5 * i) % 40 for i in range(1, N - 1)] + [1300]
+    need = [(n + S - 1) // S for n in lens]
+    table = torch.full((N, max(need)), -1, dtype=torch.int32)
+    at = 0
+    for n, m in enumerate(need):
+        table[n, :m] = torch.arange(at, at + m)
+        at += m
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32)
+    k, v, q = gen(300, 1, sum(lens), HKV, D, dtype=BF16), gen(301, 1, sum(lens), HKV, D, dtype=BF16), gen(302, N, 1, HKV, D, dtype=BF16)
+    kp, ks, vp, vs = (torch.empty(at, HKV, S, d, dtype=torch.uint8, device=cuda).transpose(1, 2) for d in (D // 2, 1, D // 2, 1))
+    sc = dict(k_scales=ks, v_scales=vs, head_first=False)
+    L.paged_kv_append(kp, vp, k.to(cuda), v.to(cuda), table.to(cuda), torch.zeros(N, dtype=torch.int32, device=cuda), cu_seqlens=cu, **sc)
+    o = L.paged_attn_decode(q.to(cuda), kp, vp, table.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda), **sc).cpu().double()
+    for n in (0, 1, 8, 100, N - 2, N - 1):
+        if not lens[n]:
+            assert (o[n] == 0).all()
+            continue
+        kk, vv = (kv4.values(*kv4.pack(x[0, cu[n]:cu[n + 1]])) for x in (k, v))
+        for h in range(0, HKV, 9):
+            ref, tol = softmax.head(q[n, :, h], kk[:, h], vv[:, h], D ** -0.5, dtype=BF16)
+            assert ((o[n, :, h] - ref).abs() <= tol).all(), (n, h)
+
+
+def test_two_at_once(cuda):
+    """Steps of two caches on two streams at the same time, and in inference mode: the bits of each by itself."""
+    caches = [Cache4(22 + i, [4000, 70, 1500], 16, 2, 128, 128, spare=8) for i in range(2)]
+    held = [c.to(cuda) for c in caches]
+    q, k, v = (gen(310 + i, 3, 1, h, 128, dtype=BF16).to(cuda) for i, h in enumerate((8, 2, 2)))
+
+    def steps(h, i):
+        (kp, ks, vp, vs), table, lens = h
+        out = []
+        for j in range(4):
+            out.append(L.paged_attn_decode(q * (i + 1), kp, vp, table, lens, k=k + j, v=v - j, head_first=False, k_scales=ks, v_scales=vs))
+            lens += 1
+        return out + list(L.paged_kv_read(kp, vp, table, lens - 20, 20, head_first=False, k_scales=ks, v_scales=vs))
+    with torch.inference_mode():
+        want = [steps(c.to(cuda), i) for i, c in enumerate(caches)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            got.append(steps(held[i], i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for x, y in zip(want, got) for a, b in zip(x, y))
+
+
 def test_a_score_that_grows(cuda):
     """Maxima that move late and by much, and ones that move by less than 2^8: the sums stay those of the definition."""
     for step, scale in ((0.02, 1.0), (0.3, 1.0), (3.0, 1.0), (-3.0, 1.0)):

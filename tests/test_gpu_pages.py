@@ -241,6 +241,31 @@ def test_graph(cuda):
             d[1].add_(more).clamp_(max=M * S - 1)
 
 
+def test_two_at_once(cuda):
+    """Two caches on two streams at the same time: each as by itself."""
+    N, M, P, S = 40, 12, 700, 8
+    states = [State(cuda, 90 + i, N, M, P, S) for i in range(2)]
+    twins = [tuple(x.clone() for x in (st.d_table, st.d_lens, st.d_refs)) + ([p.clone() for p in st.d_pages],) for st in states]
+    rows, src, dst = states[0].ints([1, 5, 39]), states[0].ints([0, 2, 2]), states[0].ints([1, 5, 7])
+
+    def life(d):
+        out = []
+        for j in range(3):
+            L.paged_free(d[0], d[1], d[2], rows)
+            L.paged_fork(d[0], d[1], d[2], src, dst)
+            out.append(L.paged_reserve(d[3], d[0], d[1], d[2], j + 1))
+            out += L.paged_compact(d[3], d[0], d[2])
+        return out + [x.clone() for x in (*d[:3], *d[3])]
+    want = [life(d) for d in twins]
+    torch.cuda.synchronize()
+    got = []
+    for st in states:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(life((st.d_table, st.d_lens, st.d_refs, st.d_pages)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for x, y in zip(want, got) for a, b in zip(x, y))
+
+
 def test_the_path_in_python_does_the_same(cuda):
     """Calls that need a conversion (numbers of 64 bits, a generator of tensors)."""
     for native in (True, False):
