@@ -21,6 +21,7 @@ constexpr int ROPE_HEADS = 4;                                    // heads of a t
 constexpr int ROPE_GROUPS = 1 << 20, ROPE_BWD_GROUPS = 2048;     // work-groups of a launch at most (or what one token needs)
 
 struct RopePlan {
+  int v, nc;       // the kernel's V and NC
   int lanes;       // of a row
   int chunks;      // of a row: V pairs each
   int runs_q;      // lane groups that share a token's query heads
@@ -85,17 +86,26 @@ template <int V, bool INTER> __device__ __forceinline__ void rope_weights(float 
   }
 }
 // V numbers of a row of the table
-template <int V> __device__ __forceinline__ void rope_angles(float (&x)[V], const float* p) {
-  typedef float vec __attribute__((ext_vector_type(V < 4 ? V : 4)));
+template <int V> __device__ __forceinline__ void rope_angles(float* x, const float* p) {
   if constexpr (V == 1) x[0] = *p;
   else {
+    constexpr int E = V < 4 ? V : 4;
+    typedef float vec __attribute__((ext_vector_type(E)));
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
+    for (int i = 0; i < V; i += E) {
       const vec y = *(const vec*)(p + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[i + e] = y[e];
+      for (int e = 0; e < E; ++e) x[i + e] = y[e];
     }
   }
+}
+
+// The number of pair k of a lane's chunk, where pairs lie next to each other: V / 2 pairs of the row's first half and as many of the second, so that
+// the lanes of a row read and write adjacent pieces (with 2 V adjacent columns to a lane, stores past the caches took twice the time: 4 x 8192
+// tokens of 20 heads of 128, 127 us forward in place of 65)
+template <int V> __device__ __forceinline__ int near_pair(int chunk, int k, int D) {
+  if constexpr (V == 1) return chunk;
+  else return k < V / 2 ? V / 2 * chunk + k : D / 4 + V / 2 * chunk + k - V / 2;
 }
 
 // the sum over the lanes of a row (of which all or none are at work)
@@ -127,7 +137,7 @@ __device__ __forceinline__ bool rope_position(const lmoe_rope_args& a, int b, in
 
 template <typename T, int V, int L, int NC, bool INTER, bool BWD>
 __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a, const RopePlan p) {
-  constexpr int HB = NC > 1 ? 1 : ROPE_HEADS;
+  constexpr int HB = ROPE_HEADS;
   typedef RopeRaw<T, V> Raw;
   const int l = threadIdx.x % L;
   const uint32_t group = blockIdx.x * (NTHR / L) + threadIdx.x / L, first = group / (uint32_t)p.runs;
@@ -145,8 +155,8 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
     const int c = (l + j * L) * V;
     on[j] = l + j * L < p.chunks;
     cr[j] = on[j] && c < half ? c : -1;
-    ca[j] = INTER ? 2 * c : c < half ? c : c + half;
-    cb[j] = INTER ? 2 * c + V : c < half ? c + half : c + half + rest;
+    ca[j] = INTER ? 2 * near_pair<V>(l + j * L, 0, a.D) : c < half ? c : c + half;
+    cb[j] = INTER ? (V == 1 ? ca[j] + 1 : 2 * near_pair<V>(l + j * L, V / 2, a.D)) : c < half ? c + half : c + half + rest;
     if (!on[j]) ca[j] = cb[j] = 0;
     rope_weights<V, INTER>(w[j], isq ? a.qw : a.kw, a.w_dtype, ca[j], cb[j]);
 #pragma unroll
@@ -192,7 +202,17 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
       const bool turn = pos >= 0 && cr[j] >= 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) { c[j][i] = 1.f; s[j][i] = 0.f; }
-      if (turn) {
+      if constexpr (INTER && V > 1) {
+        const int64_t row = (int64_t)pos * half;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int at = (y ? cb[j] : ca[j]) / 2;
+          if (pos >= 0 && on[j] && at < half) {
+            rope_angles<V / 2>(c[j] + V / 2 * y, a.cos + row + at);
+            rope_angles<V / 2>(s[j] + V / 2 * y, a.sin + row + at);
+          }
+        }
+      } else if (turn) {
         rope_angles<V>(c[j], a.cos + (int64_t)pos * half + cr[j]);
         rope_angles<V>(s[j], a.sin + (int64_t)pos * half + cr[j]);
       }
@@ -292,7 +312,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
         x += of_q[g] == q ? y : 0.f;
       }
       const int k = e < V ? e : e - V;
-      const int col = INTER ? 2 * (c + k) + (e >= V) : (c < half ? c : c + half) + k + (e < V ? 0 : c < half ? half : rest);
+      const int col = INTER ? 2 * near_pair<V>(chunk, k, a.D) + (e >= V) : (c < half ? c : c + half) + k + (e < V ? 0 : c < half ? half : rest);
       a.ws[(int64_t)blockIdx.x * 2 * a.D + (q ? 0 : a.D) + col] = x;
     }
   }
@@ -319,32 +339,39 @@ __global__ __launch_bounds__(NTHR) void k_qk_norm_dw(const lmoe_rope_args a, int
   if (a.w_dtype == LMOE_F32) ((float*)to)[e] = y; else ((bf16*)to)[e] = (bf16)y;
 }
 
-// Whether every row can be read in 16-byte pieces that hold whole pairs' members, and the table and the weights with it
-static bool rope_wide(const lmoe_rope_args& a) {
-  for (const void* x : {(const void*)a.cos, (const void*)a.sin, a.qw, a.kw}) if ((uintptr_t)x & 15) return false;
-  const int v = a.dtype == LMOE_BF16 ? 8 : 4;
-  if (a.interleaved ? a.R % (2 * v) || a.D % (2 * v) : a.R % (2 * v) || (a.D - a.R) % (2 * v)) return false;
-  const lmoe_tensor* all[] = {&a.q, &a.k, &a.zq, &a.zk, &a.dzq, &a.dzk, &a.dq, &a.dk};
-  for (const lmoe_tensor* t : all)
-    if (t->ptr && (((uintptr_t)t->ptr & 15) || (t->sb | t->st | t->sh) % v)) return false;
-  return true;
+// The most columns (16 bytes of them, 2 or 1) in which every row can be read, with the weights and the table's rows, so that a piece holds whole
+// pairs (interleaved) or members of one kind (4 x 8192 tokens of 20 heads, forward and backward, us: 128 columns 156; 36, in pieces of 2, 109, column by
+// column 169 of half of them turned; 118, column by column, 340)
+static int rope_vec(const lmoe_rope_args& a) {
+  const int size = a.dtype == LMOE_BF16 ? 2 : 4;
+  for (const int v : {16 / size, 2}) {
+    const uint64_t bytes = (uint64_t)v * size;
+    bool ok = a.interleaved ? a.D % (2 * v) == 0 && a.R % v == 0 : a.R % (2 * v) == 0 && (a.D - a.R) % (2 * v) == 0;
+    for (const void* x : {(const void*)a.cos, (const void*)a.sin, a.qw, a.kw}) ok = ok && (uintptr_t)x % (v == 2 ? 8 : 16) == 0;
+    for (const lmoe_tensor* t : {&a.q, &a.k, &a.zq, &a.zk, &a.dzq, &a.dzk, &a.dq, &a.dk})
+      ok = ok && (!t->ptr || ((uintptr_t)t->ptr % bytes == 0 && (t->sb | t->st | t->sh) % v == 0));
+    if (ok) return v;
+  }
+  return 1;
 }
 static RopePlan rope_plan(const lmoe_rope_args& a, bool bwd) {
   RopePlan p;
-  const int v = rope_wide(a) ? (a.dtype == LMOE_BF16 ? 8 : 4) : 1;
+  const int v = p.v = rope_vec(a);
   p.chunks = a.D / (2 * v);
-  p.lanes = 4;
+  p.lanes = v > 2 ? 4 : v == 2 ? 16 : 32;
   while (p.lanes < 64 && p.lanes < p.chunks) p.lanes *= 2;
-  if (v == 1) p.lanes = 64;
-  p.full = p.chunks == p.lanes * (v == 1 ? 2 : 1);
+  p.nc = p.chunks > p.lanes ? 2 : 1;
+  p.full = p.chunks == p.lanes * p.nc;
   const int64_t tokens = (int64_t)a.B * a.T, per = NTHR / p.lanes, heads = (int64_t)a.HQ + a.HKV;
   // a head for each lane group while that leaves the card empty, else several
-  const int hb = v == 1 || tokens * heads <= 256 * 8 * per ? 1 : ROPE_HEADS;
+  const int hb = tokens * heads <= 256 * 8 * per ? 1 : ROPE_HEADS;
   p.runs_q = (a.HQ + hb - 1) / hb;
   p.runs = p.runs_q + (a.HKV + hb - 1) / hb;
-  // Results of which the last-level cache would keep less than half by the time they are read go past it: 4 x 8192 tokens of 20 heads of
-  // 128 (168 MB each way), forward and backward, 171 -> 156 us; 8192 of 40 (84 MB), forward, 34 either way.
-  p.past = tokens * heads * a.D * (a.dtype == LMOE_BF16 ? 2 : 4) > 128 << 20;
+  // Results of which the last-level cache would keep less than half by the time they are read go past it, in whole cache lines: 4 x 8192
+  // tokens of 20 heads of 128 (168 MB each way), forward and backward, 171 -> 156 us; 8192 of 40 (84 MB), forward, 34 either way; in pieces of
+  // 64 bytes (65536 tokens of 24 heads of 64) 205 -> 211, of 96 235 -> 257.
+  const int size = a.dtype == LMOE_BF16 ? 2 : 4, rest = (a.D - a.R) / 2, piece = a.interleaved || a.R == 0 || rest == 0 ? a.D / 2 : std::min(a.R / 2, rest);
+  p.past = v > 1 && tokens * heads * a.D * size > 128 << 20 && piece * size % 128 == 0;
   // as many tokens for every lane group
   const int64_t items = tokens * p.runs, most = bwd ? ROPE_BWD_GROUPS : ROPE_GROUPS;
   const int64_t each = (items + most * per - 1) / (most * per), sets = (tokens + each - 1) / each;
@@ -363,11 +390,18 @@ template <typename T, int V, int L, int NC, bool BWD> static void rope_launch(co
 }
 template <typename T, bool BWD> static void rope_typed(const lmoe_rope_args& a, const RopePlan& p, hipStream_t st) {
   constexpr int V = ET<T>::VEC;
-  if (p.chunks * 2 * V != a.D || !rope_wide(a)) rope_launch<T, 1, 64, 2, BWD>(a, p, st);
-  else if (p.lanes == 4) rope_launch<T, V, 4, 1, BWD>(a, p, st);
-  else if (p.lanes == 8) rope_launch<T, V, 8, 1, BWD>(a, p, st);
-  else if (p.lanes == 16) rope_launch<T, V, 16, 1, BWD>(a, p, st);
-  else if constexpr (V == 4) rope_launch<T, V, 32, 1, BWD>(a, p, st);
+  if (p.v == V) {
+    if (p.lanes == 4) rope_launch<T, V, 4, 1, BWD>(a, p, st);
+    else if (p.lanes == 8) rope_launch<T, V, 8, 1, BWD>(a, p, st);
+    else if (p.lanes == 16) rope_launch<T, V, 16, 1, BWD>(a, p, st);
+    else if constexpr (V == 4) rope_launch<T, V, 32, 1, BWD>(a, p, st);
+  } else if (p.v == 2) {
+    if (p.lanes == 16) rope_launch<T, 2, 16, 1, BWD>(a, p, st);
+    else if (p.lanes == 32) rope_launch<T, 2, 32, 1, BWD>(a, p, st);
+    else rope_launch<T, 2, 64, 1, BWD>(a, p, st);
+  } else if (p.lanes == 32) rope_launch<T, 1, 32, 1, BWD>(a, p, st);
+  else if (p.nc == 1) rope_launch<T, 1, 64, 1, BWD>(a, p, st);
+  else rope_launch<T, 1, 64, 2, BWD>(a, p, st);
 }
 void launch_qk_norm_rope(const lmoe_rope_args& a, bool bwd, hipStream_t st) {
   const RopePlan p = rope_plan(a, bwd);

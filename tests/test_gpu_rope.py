@@ -83,6 +83,18 @@ def test_dims(cuda, dtype, interleaved, D, R):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,R,off", [(36, 36, 0), (80, 40, 0), (80, 40, 4), (128, 96, 2), (128, 128, 1), (200, 100, 2), (256, 64, 2), (118, 118, 0), (254, 100, 0), (64, 40, 0), (62, 2, 0)])
+def test_pieces_of_a_row(cuda, dtype, interleaved, D, R, off):
+    """Rows that begin anywhere and columns that no 16 bytes divide; few tokens, and enough of them for several heads at a time."""
+    def shifted(y):
+        out = torch.zeros(y.numel() + 8, dtype=y.dtype, device=cuda)[off:off + y.numel()].view(y.shape)
+        return out.copy_(y)
+    for B, T, HQ, HKV in ((2, 3, 5, 2), (1, 1501, 9, 3)):
+        check(cuda, B, T, HQ, HKV, D, dtype, R, interleaved, wdtype=F32, make=shifted)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("B,T,HQ,HKV", [(1, 1, 1, 1), (1, 1, 16, 4), (3, 1, 5, 1), (1, 333, 4, 4), (2, 129, 7, 3), (1, 1111, 12, 12), (5, 64, 1, 9)])
 def test_sizes(cuda, dtype, B, T, HQ, HKV):
     check(cuda, B, T, HQ, HKV, 64, dtype, wdtype=F32, head_first=T % 2 == 0)
