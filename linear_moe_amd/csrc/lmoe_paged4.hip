@@ -305,23 +305,50 @@ template <int W> struct Tile4 {
   uint32_t live;                                   // which of the positions exist
 };
 
-// The B-th byte of the lane's keys of V, columns 2B and 2B + 1 of its own: as two products with P
-template <typename T, int W, int B>
-__device__ __forceinline__ void pv4(f32x4 (&o)[W / 16], const Tile4<W>& t, const typename ET<T>::frag& pf) {
-  typename ET<T>::frag lo, hi;
+// What the cache holds is exact in a bfloat16, so that numbers of 32 bits go into the products with it as three of them, x = a + b + c with the
+// upper, middle and lower 8 of its 24 bits: each product is exact as in one of 32 bits, whose matrix instructions take sixteen times as long
+// per number (16 sequences of 1024 to 4096 tokens, 16 / 8 heads of 128: 46 -> 22 us).
+template <typename T> struct Parts {
+  static constexpr int N = sizeof(T) == 2 ? 1 : 3;
+  bf16x8 x[N];
+};
+__device__ __forceinline__ f32x4 upper8(const f32x4& x) {
+  f32x4 r;
+#pragma unroll                                 // (a copy: the bits of an element of a vector in place are those of its first)
+  for (int i = 0; i < 4; ++i) { const float y = x[i]; r[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & 0xffff0000u); }
+  return r;
+}
+template <typename T> __device__ __forceinline__ Parts<T> parts_of(f32x4 lo, f32x4 hi) {
+  Parts<T> r;
+  if constexpr (Parts<T>::N == 1) r.x[0] = frag_of_blocks(lo, hi);
+  else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (sizeof(T) == 2) {
-      const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[e], scale_of(t.vs[e]), B);
-      lo[e] = x[0];
-      hi[e] = x[1];
-    } else {
-      const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(t.v[e], scale_of(t.vs[e]), B);
-      if (e < 4) { lo.lo[e] = x[0]; hi.lo[e] = x[1]; } else { lo.hi[e - 4] = x[0]; hi.hi[e - 4] = x[1]; }
+    for (int i = 0; i < 3; ++i) {
+      const f32x4 a = upper8(lo), b = upper8(hi);
+      r.x[i] = frag_of_blocks(a, b);
+      lo -= a;
+      hi -= b;
     }
   }
-  ET<T>::mma(o[2 * B], lo, pf);
-  ET<T>::mma(o[2 * B + 1], hi, pf);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void mma_parts(f32x4& c, const bf16x8& a, const Parts<T>& b) {
+#pragma unroll
+  for (int i = 0; i < Parts<T>::N; ++i) ET<bf16>::mma(c, a, b.x[i]);
+}
+
+// The B-th byte of the lane's keys of V, columns 2B and 2B + 1 of its own: as two products with P
+template <typename T, int W, int B>
+__device__ __forceinline__ void pv4(f32x4 (&o)[W / 16], const Tile4<W>& t, const Parts<T>& pf) {
+  bf16x8 lo, hi;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(t.v[e], scale_of(t.vs[e]), B);
+    lo[e] = x[0];
+    hi[e] = x[1];
+  }
+  mma_parts<T>(o[2 * B], lo, pf);
+  mma_parts<T>(o[2 * B + 1], hi, pf);
 }
 
 // EVEN: 16 adjacent positions lie in one page (S a multiple of 16) and offsets inside a page and strides of pages hold in 32 bits, so that a
@@ -449,12 +476,15 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
     ahead = ask(j0 + PGROUP);
   }
 
-  typename ET<T>::frag q[KW];
+  Parts<T> q[KW];
   const int hq = hk * G + h0 + min(c, heads - 1);
   {
     const T* row = (const T*)a.q.ptr + (int64_t)n * a.q.sb + (int64_t)hq * a.q.sh;
 #pragma unroll
-    for (int j = 0; j < KW; ++j) q[j] = kin ? ET<T>::load_frag(row + KC * g + 8 * j) : zero_frag<T>();
+    for (int j = 0; j < KW; ++j) {
+      const typename ET<T>::frag x = kin ? ET<T>::load_frag(row + KC * g + 8 * j) : zero_frag<T>();
+      if constexpr (FAST) q[j].x[0] = x; else q[j] = parts_of<T>(x.lo, x.hi);
+    }
   }
   const Score<CAP, BIAS, FAST> sc(a.scale, a.softcap, a.slopes, hq);
 
@@ -468,7 +498,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
     for (int b = 0; b < 2; ++b) {
       s[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < KW; ++j) ET<T>::mma(s[b], from4<T>(t.k[b][j], scale_of(t.ks[b])), q[j]);
+      for (int j = 0; j < KW; ++j) mma_parts<T>(s[b], from4<bf16>(t.k[b][j], scale_of(t.ks[b])), q[j]);
     }
     float mx = M_LOW;
 #pragma unroll
@@ -514,8 +544,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
     // (P rounded to the element type, as the products take it; the sum is of the numbers before.  What the rounding leaves, as two more
     // products, would take the error of o from 0.0023 of its size to the 0.0017 of its own rounding: 49 -> 51 us, and 49 it is, as in a
     // cache of 2-byte elements.)
-    typename ET<T>::frag pf;
-    if constexpr (FAST) pf = frag_of_blocks(s[0], s[1]); else { pf.lo = s[0]; pf.hi = s[1]; }
+    const Parts<T> pf = parts_of<T>(s[0], s[1]);
     pv4<T, W, 0>(o, t, pf);
     pv4<T, W, 1>(o, t, pf);
     if constexpr (VW == 8) { pv4<T, W, 2>(o, t, pf); pv4<T, W, 3>(o, t, pf); }
