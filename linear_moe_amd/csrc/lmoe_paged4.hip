@@ -274,13 +274,14 @@ static PagedPlan paged4_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
   const int64_t bound = (int64_t)a.M * a.S + (a.kn.ptr ? 1 : 0), groups = (int64_t)a.N * a.HKV * p.blocks;
-  // A short cache: one stretch of eight waves and no second launch; else stretches of one length, whatever the call (us for stretches of
-  // 512, 1024, 2048 positions, with the join: 64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 55 54 58; 2 of 32 K and 128 K,
-  // 16 / 4 heads of 128: 33 29 39).
-  // Eight waves leave a CU one work-group: for one a CU at most (16 / 4 heads of 128, with eight and with four waves: 1 sequence of 500 tokens
-  // 7.4 and 7.9 us, 64 of 1000 11.4 and 12.2, 100 of 1000 19.0 and 15.7).
-  p.waves = bound <= 1024 && groups <= 256 ? 8 : 4;
-  const int64_t chunk = 1024;
+  // A short cache: one stretch and no second launch; else stretches of one length, whatever the call (us for stretches of 512, 1024, 2048
+  // positions of four waves, with the join: 64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 55 54 58; 2 of 32 K and 128 K, 16 / 4
+  // heads of 128: 33 29 39).  Eight waves leave a CU one work-group: for one a CU at most, which then have half the steps (16 / 4 heads of
+  // 128: 64 of 1000 tokens 12.2 -> 11.4, 100 of 1000 15.7 -> 19.0), and half the positions where that leaves them one a CU (4 of 3000, 32 / 8 heads
+  // of 128: 14.6, with eight waves 13.4, and 512 positions 11.3; of 256 positions 12.4).
+  auto pieces = [&](int64_t chunk) { return groups * ((bound + chunk - 1) / chunk); };
+  const int64_t chunk = bound > 1024 && pieces(512) <= 256 ? 512 : 1024;
+  p.waves = pieces(chunk) <= 256 ? 8 : 4;
   const int64_t splits = bound > 0 ? (bound + chunk - 1) / chunk : 1;
   const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;
   p.splits = (int)(splits < most ? splits : most);
