@@ -68,7 +68,7 @@ __device__ __forceinline__ int scan(int x, int& total, int* s_wave) {
   return before + y - x;
 }
 
-// The numbers p in [begin, end) with (refs[p] > 0) == used, in their order, into list[0 .. most - 1]; how many there are (counting stops
+// The numbers p in [begin, end) with (refs[p] > 0) == used, in their order, the first `most` of them; how many there are (counting stops
 // behind the tile that fills the list).  A tile is PAGES_VEC numbers for every thread, PAGES_NTHR apart, so that a load reads
 // adjacent ones and all of a tile are in flight at once.
 struct ListShared { int count[PAGES_VEC * PAGES_WAVES], wave[PAGES_WAVES]; };
@@ -82,8 +82,8 @@ struct ListTile {
     }
   }
 };
-// next: the first tile, asked for by the caller
-__device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, bool used, int32_t* list, int most, ListShared& sh, ListTile next) {
+// next: the first tile, asked for by the caller; to(k, p): takes the k-th of them
+template <typename F> __device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, bool used, F to, int most, ListShared& sh, ListTile next) {
   static_assert(PAGES_VEC * PAGES_WAVES <= PAGES_NTHR, "");
   constexpr int TILE = PAGES_NTHR * PAGES_VEC;
   const int wave = wave_id();
@@ -105,7 +105,7 @@ __device__ __forceinline__ int listed(const int32_t* refs, int begin, int end, b
 #pragma unroll
     for (int i = 0; i < PAGES_VEC; ++i) {
       const int k = before + sh.count[i * PAGES_WAVES + wave] + __popcll(hit[i] & ((1ull << lane_id()) - 1));
-      if ((hit[i] >> lane_id() & 1) && k < most) put(list + k, p0 + i * PAGES_NTHR + (int)threadIdx.x);
+      if ((hit[i] >> lane_id() & 1) && k < most) to(k, p0 + i * PAGES_NTHR + (int)threadIdx.x);
     }
     before += total;
     __syncthreads();                       // sh.count has been read
@@ -170,17 +170,36 @@ __device__ __forceinline__ bool asked(const lmoe_pages_args& a, int n, int& firs
 // of it are asked for too, has to be copied if r - e > 1, for those have taken their copies by then.  So of the asked entries of a page all are
 // copied, but the last where there are r of them.
 // The asked entries of PAGES_NTHR rows at a time are dealt to the threads; where the call has one for a thread, it stays in its registers
-// from the first step to the last (256 rows of one token, 128 of them forks, 41 thousand pages: 12 us; with a wave for every row, which waits
+// from the first step to the last (256 rows of one token, 128 of them forks, 41 thousand pages: 9.8 us; with a wave for every row, which waits
 // for its entries again in each step, 115).
 struct Asked { int n, c, x, refs; bool last; };      // row, column, entry, refs of its page (0: none), whether the row's last
+// What is counted of the shared pages that entries ask for, in shared memory where the call has one entry for a thread (the rows above,
+// with the list of free pages there too: 12.0 -> 9.8 us): a table that is half full at most, places by open addressing.
+struct AskedPages {
+  static constexpr int PLACES = 2 * PAGES_NTHR;
+  int page[PLACES], claims[PLACES], last[PLACES], failed[PLACES], free[PAGES_NTHR];
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < PLACES; i += PAGES_NTHR) { page[i] = last[i] = -1; claims[i] = failed[i] = 0; }
+  }
+  __device__ __forceinline__ int place(int x) {
+    uint32_t i = (uint32_t)x * 2654435761u % PLACES;
+    for (;;) {
+      const int y = atomicCAS(&page[i], -1, x);
+      if (y == -1 || y == x) return (int)i;
+      i = (i + 1) % PLACES;
+    }
+  }
+};
 __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_args a) {
   __shared__ ListShared sh;
   __shared__ int s_first[PAGES_NTHR], s_start[PAGES_NTHR + 1], s_before[PAGES_NTHR], s_upto[PAGES_NTHR];
   __shared__ uint8_t s_fits[PAGES_NTHR];
+  __shared__ AskedPages s_asked;
   const PagesWs w = pages_ws(a);
   const int tid = threadIdx.x;
   ListTile tile;
   tile.load(a.refs, 0, a.P, false);       // (used last, asked for first)
+  s_asked.clear();
   int row0 = 0, count = 0;                // rows from row0 on are dealt out, `count` entries of theirs
   auto deal = [&](int n0) {
     const int n = n0 + tid;
@@ -230,23 +249,36 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
     }
   };
   auto shared = [&](const Asked& e) { return e.x >= 0 && e.refs > 1; };
-  auto kept = [&](const Asked& e) { return seen(w.claims + e.x) == e.refs && seen(w.last + e.x) == e.n * a.M + e.c; };
-  int any = 0;
-  every([&](const Asked& e) {
-    if (shared(e)) { put(w.claims + e.x, 0); put(w.last + e.x, -1); put(w.failed + e.x, 0); any = 1; }
-  });
-  if (__syncthreads_or(any)) {
-    every([&](const Asked& e) {
-      if (shared(e)) { atomicAdd(w.claims + e.x, 1); atomicMax(w.last + e.x, e.n * a.M + e.c); }
-    });
+  int place = 0;                          // of `mine` in s_asked
+  auto kept = [&](const Asked& e) {
+    if (single) return s_asked.claims[place] == e.refs && s_asked.last[place] == e.n * a.M + e.c;
+    return seen(w.claims + e.x) == e.refs && seen(w.last + e.x) == e.n * a.M + e.c;
+  };
+  if (single) {                           // (cleared in front of a barrier of deal())
+    if (shared(mine)) {
+      place = s_asked.place(mine.x);
+      atomicAdd(&s_asked.claims[place], 1);
+      atomicMax(&s_asked.last[place], mine.n * a.M + mine.c);
+    }
     __syncthreads();
+  } else {
+    int any = 0;
+    every([&](const Asked& e) {
+      if (shared(e)) { put(w.claims + e.x, 0); put(w.last + e.x, -1); put(w.failed + e.x, 0); any = 1; }
+    });
+    if (__syncthreads_or(any)) {
+      every([&](const Asked& e) {
+        if (shared(e)) { atomicAdd(w.claims + e.x, 1); atomicMax(w.last + e.x, e.n * a.M + e.c); }
+      });
+      __syncthreads();
+    }
   }
   auto copied = [&](const Asked& e) { return shared(e) && !kept(e); };
   auto needs = [&](const Asked& e) { return e.n >= 0 && (e.x < 0 || copied(e)); };
   int need = 0, all;
   every([&](const Asked& e) { need += needs(e); });
   scan(need, all, sh.wave);
-  const int free = listed(a.refs, 0, a.P, false, w.list, min(all, a.P), sh, tile);
+  const int free = listed(a.refs, 0, a.P, false, [&](int k, int p) { if (single) s_asked.free[k] = p; else put(w.list + k, p); }, min(all, a.P), sh, tile);
   __syncthreads();
   // pages needed in front of and up to each row that is dealt out; before: by the rows in front of them
   auto reach = [&](int before) {
@@ -271,7 +303,7 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
       if (!whole) { __syncthreads(); deal(n0); }
       before = reach(before);
       entries([&](const Asked& e) {
-        if (e.n >= 0 && !reached(e.n - row0) && copied(e)) put(w.failed + e.x, 1);
+        if (e.n >= 0 && !reached(e.n - row0) && copied(e)) { if (single) s_asked.failed[place] = 1; else put(w.failed + e.x, 1); }
       });
       __syncthreads();
     }
@@ -284,7 +316,7 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
       if (!reached(tid)) s_fits[tid] = false;
       __syncthreads();
       entries([&](const Asked& e) {
-        if (shared(e) && kept(e) && seen(w.failed + e.x)) s_fits[e.n - row0] = false;
+        if (shared(e) && kept(e) && (single ? s_asked.failed[place] : seen(w.failed + e.x))) s_fits[e.n - row0] = false;
       });
       __syncthreads();
     }
@@ -299,7 +331,7 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_reserve(const lmoe_pages_a
       given += total & 0xffff;
       copies += total >> 16;
       if (!take) return;
-      const int page = seen(w.list + at);
+      const int page = single ? s_asked.free[at] : seen(w.list + at);
       a.table[(int64_t)e.n * a.table_stride + e.c] = page;
       a.refs[page] = 1;                    // (free or given out: no page is shared by it)
       if (copy) {
@@ -339,8 +371,8 @@ __global__ __launch_bounds__(PAGES_NTHR) void k_pages_compact(const lmoe_pages_a
   tile.load(a.refs, live, a.P, true);
 #pragma unroll
   for (int i = 0; i < PAGES_VEC; ++i) if (i * PAGES_NTHR + (int)threadIdx.x >= live) first.r[i] = 1;
-  const int count = listed(a.refs, 0, live, false, w.dst, live, sh, first);
-  listed(a.refs, live, a.P, true, w.src, count, sh, tile);
+  const int count = listed(a.refs, 0, live, false, [&](int k, int p) { put(w.dst + k, p); }, live, sh, first);
+  listed(a.refs, live, a.P, true, [&](int k, int p) { put(w.src + k, p); }, count, sh, tile);
   __syncthreads();
   for (int i = threadIdx.x; i < count; i += PAGES_NTHR) {
     const int from = seen(w.src + i), to = seen(w.dst + i);

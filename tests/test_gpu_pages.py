@@ -168,6 +168,17 @@ def test_many(cuda):
         st.reserve(1)
 
 
+@pytest.mark.parametrize("N,M,F", [(300, 2, 256), (300, 2, 257), (40, 1024, 8), (40, 1025, 8), (260, 32, 256), (260, 33, 256), (5, 3000, 4), (200, 1, 200), (3, 1, 40)])
+def test_forks_of_many_rows(cuda, N, M, F):
+    """Chains and rings of rows, rows twice, rows that are none."""
+    r = random.Random(N * M + F)
+    st = State(cuda, 60, N, M, 3 * N + M, 2)
+    for _ in range(3):
+        st.fork([r.randrange(-1, N + 1) for _ in range(F)], [r.randrange(-1, N + 1) for _ in range(F)])
+    ring = [i % N for i in range(min(F, N))]
+    st.fork(ring, ring[1:] + ring[:1])
+
+
 def test_layouts_of_pages(cuda):
     """Tensors of pages in other orders and as parts of others; what lies between stays."""
     N, M, P, S = 5, 6, 40, 8
