@@ -116,18 +116,23 @@ template <int L> __device__ __forceinline__ float lanes_of_row(float x) {
   return x;
 }
 
-// The position of token t (of row b), and whether it belongs to a sequence
-__device__ __forceinline__ bool rope_position(const lmoe_rope_args& a, int b, int t, int& pos) {
+// The position of token t (of row b), and whether it belongs to a sequence; s_cu: a copy of the sequences' offsets, where they are few
+constexpr int ROPE_DOCS = 1024;
+__device__ __forceinline__ bool rope_position(const lmoe_rope_args& a, const int32_t* s_cu, int b, int t, int& pos) {
   int n = b, at = t;
   if (a.cu_seqlens) {
-    if (t < a.cu_seqlens[0] || t >= a.cu_seqlens[a.N]) return false;
-    int lo = 0, hi = a.N;                       // the last sequence that begins at or before the token (of several, all but it are empty)
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (a.cu_seqlens[m] <= t) lo = m; else hi = m;
-    }
-    n = lo;
-    at = t - a.cu_seqlens[n];
+    auto find = [&](auto cu) {
+      if (t < cu[0] || t >= cu[a.N]) return false;
+      int lo = 0, hi = a.N;                     // the last sequence that begins at or before the token (of several, all but it are empty)
+      while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (cu[m] <= t) lo = m; else hi = m;
+      }
+      n = lo;
+      at = t - cu[n];
+      return true;
+    };
+    if (!(a.N <= ROPE_DOCS ? find((const __attribute__((address_space(3))) int32_t*)s_cu) : find(a.cu_seqlens))) return false;
   }
   // (in 64 bits: an offset may be any number)
   int64_t p = a.positions ? a.positions[b * a.pos_stride + t] : (int64_t)at + (a.offsets ? a.offsets[n] : 0);
@@ -164,6 +169,12 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
   }
   // (a rotation alone has no use for x on the way back: the gradient again, which costs nothing)
   const lmoe_tensor from = BWD && !a.norm ? (isq ? a.dzq : a.dzk) : (isq ? a.q : a.k), to = BWD ? (isq ? a.dq : a.dk) : (isq ? a.zq : a.zk), grad = isq ? a.dzq : a.dzk;
+  // (the search for a token's sequence is a chain of reads: 16381 tokens of 24 heads of 64 in 23 documents, forward 27 -> 25 us, backward 42 -> 37)
+  __shared__ int32_t s_cu[ROPE_DOCS + 1];
+  if (a.cu_seqlens && a.N <= ROPE_DOCS) {
+    for (int i = threadIdx.x; i <= a.N; i += NTHR) s_cu[i] = a.cu_seqlens[i];
+    __syncthreads();
+  }
   const float over = 1.0f / (float)a.D;
   const uint32_t tokens = (uint32_t)a.B * (uint32_t)a.T;
   // (all lanes of a row go the same way; a group past the last whole set of runs has nothing to do)
@@ -187,7 +198,7 @@ __global__ __launch_bounds__(NTHR, 2) void k_qk_norm_rope(const lmoe_rope_args a
     };
     load(h_first);                       // (in front of the search for the position)
     int pos;
-    const bool live = rope_position(a, b, t, pos);
+    const bool live = rope_position(a, s_cu, b, t, pos);
     if (!live) {                         // behind the last sequence: zeros, whatever lies there
       Raw none;
       none.clear();

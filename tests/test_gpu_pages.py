@@ -168,6 +168,22 @@ def test_many(cuda):
         st.reserve(1)
 
 
+def test_shared_pages_whose_numbers_are_alike(cuda):
+    """Rows of one token that share pages 512, 1024, 2048 and 4096 apart, and neighbours."""
+    for step in (1, 512, 1024, 2048, 4096):
+        n, r = 15, random.Random(step)
+        st = State(cuda, 2, 4 * n, 3, 15 * 4096 + 1, 4, full=0.0, shapes=((1,),), dtypes=(torch.uint8,))
+        pages = [step * i for i in range(n)] * 4
+        r.shuffle(pages)
+        st.table = [[p, -1, -1] for p in pages]
+        st.lens, st.refs = [r.randrange(1, 4) for _ in pages], [0] * st.P
+        for i in range(n):
+            st.refs[step * i] = 4 + (i % 5 == 0)                               # (some held by the program as well)
+        st.d_table.copy_(st.ints(st.table)), st.d_lens.copy_(st.ints(st.lens)), st.d_refs.copy_(st.ints(st.refs))
+        st.reserve([r.choice((0, 1, 1, 1)) for _ in pages])
+        st.reserve(2)
+
+
 @pytest.mark.parametrize("N,M,F", [(300, 2, 256), (300, 2, 257), (40, 1024, 8), (40, 1025, 8), (260, 32, 256), (260, 33, 256), (5, 3000, 4), (200, 1, 200), (3, 1, 40)])
 def test_forks_of_many_rows(cuda, N, M, F):
     """Chains and rings of rows, rows twice, rows that are none."""

@@ -113,6 +113,8 @@ def test_packed_documents_offsets_and_rows_behind(cuda, cu_dtype):
     check(cuda, 1, 60, 4, 2, 64, BF16, lens=[0, 1, 17, 12, 30, 0], offsets=[5, 0, 1000, 3, 2, 9], wdtype=F32, cu_dtype=cu_dtype)
     check(cuda, 1, 40, 3, 1, 36, F32, lens=[0, 0], wdtype=F32, L_table=1, cu_dtype=cu_dtype)                          # nothing but rows behind
     check(cuda, 1, 300, 3, 1, 64, F32, lens=[1] * 300, offsets=list(range(300)), cu_dtype=cu_dtype)
+    for n in (1023, 1024, 1025, 2100):                                                                                # as many as a work-group keeps, and more
+        check(cuda, 1, n + 9, 3, 1, 64, BF16, lens=[(3 * i) % 4 and 1 for i in range(n)], offsets=[i % 50 for i in range(n)], cu_dtype=cu_dtype)
 
 
 def test_rows_behind_the_last_document_do_not_spread(cuda):
