@@ -13,6 +13,8 @@
 //   The new token is made into 4 bits by the wave that attends to it, in the registers it is attended from.
 // HBM-bound while its stretches last (64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128, 179 MB: 44 us and a join of 5; of twice the
 // tokens the second half takes 5.2 TB/s); writing and reading, a wave per token, likewise (16384 tokens, 85 MB each way: 18 and 17 us).
+#include <algorithm>
+
 #include "lmoe_paged.hpp"
 
 namespace lmoe {
@@ -266,21 +268,26 @@ __device__ __forceinline__ uint32_t shifted(uint32_t x, uint32_t part, uint32_t 
   const uint32_t same = min(count & -count, (uint32_t)XCDS);
   return (x + part * same / XCDS) % count;
 }
+__host__ __device__ inline bool heads_adjacent(const lmoe_paged_args& a) { return a.HKV > 1 && a.kp.sh < a.kp.st; }
 __host__ __device__ inline bool heads_near(const lmoe_paged_args& a, const PagedPlan& p) {
   const int64_t units = (int64_t)a.N * p.splits;
-  return a.HKV > 1 && a.kp.sh < a.kp.st && units >= XCDS && units * a.HKV * p.blocks <= 1 << 22;
+  return heads_adjacent(a) && units >= XCDS && units * a.HKV * p.blocks <= 1 << 22;
 }
 static PagedPlan paged4_plan(const lmoe_paged_args& a) {
   PagedPlan p;
   p.blocks = (a.HQ / a.HKV + PHEADS - 1) / PHEADS;
   const int64_t bound = (int64_t)a.M * a.S + (a.kn.ptr ? 1 : 0), groups = (int64_t)a.N * a.HKV * p.blocks;
-  // A short cache: one stretch and no second launch; else stretches of one length, whatever the call (us for stretches of 512, 1024, 2048
-  // positions of four waves, with the join: 64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 55 54 58; 2 of 32 K and 128 K, 16 / 4
-  // heads of 128: 33 29 39).  Eight waves leave a CU one work-group: for one a CU at most, which then have half the steps (16 / 4 heads of
-  // 128: 64 of 1000 tokens 12.2 -> 11.4, 100 of 1000 15.7 -> 19.0), and half the positions where that leaves them one a CU (4 of 3000, 32 / 8 heads
+  // One stretch and no second launch for a short cache, and up to 5120 positions where there are two work-groups a CU: sequences that fill
+  // the table take as long together as the longest by itself (us with stretches of 1024 and with one, 32 / 8 heads of 128: 16 sequences of 375
+  // to 1500 tokens 14.7 and 12.0, 100 of 512 to 2048 43 and 37, 64 of 1024 to 4096 49 and 44, 45 of 1616 to 6464 53 and 56; where the heads of a
+  // token lie next to each other, 60 and 63).
+  // Else stretches of one length, whatever the call (of 512, 1024, 2048 positions: 2 sequences of 32 K and 128 K, 16 / 4 heads of 128, 33 29 39).
+  // Eight waves leave a CU one work-group: for one a CU at most, which then have half the steps (16 / 4 heads of
+  // 128: 64 of 1000 tokens 12.2 -> 11.4, 100 of 1000 15.7 -> 19.0), and 512 positions where that leaves them one a CU (4 of 3000, 32 / 8 heads
   // of 128: 14.6, with eight waves 13.4, and 512 positions 11.3; of 256 positions 12.4).
   auto pieces = [&](int64_t chunk) { return groups * ((bound + chunk - 1) / chunk); };
-  const int64_t chunk = bound > 1024 && pieces(512) <= 256 ? 512 : 1024;
+  const bool one = bound <= 2048 || (bound <= 5120 && groups >= 512 && !heads_adjacent(a));
+  const int64_t chunk = bound > 1024 && pieces(512) <= 256 ? 512 : one ? std::max<int64_t>(bound, 1) : 1024;
   p.waves = pieces(chunk) <= 256 ? 8 : 4;
   const int64_t splits = bound > 0 ? (bound + chunk - 1) / chunk : 1;
   const int64_t most = groups * PSPLITS <= 16384 ? PSPLITS : groups >= 16384 ? 1 : 16384 / groups;

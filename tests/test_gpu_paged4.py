@@ -200,6 +200,13 @@ def test_fewer_stretches_than_a_long_sequence_would_have(cuda):
             assert ((o[n, :, h] - ref).abs() <= tol).all(), (n, h)
 
 
+@pytest.mark.parametrize("heads_first", [True, False])
+def test_one_stretch_for_many_work_groups(cuda, heads_first):
+    """Tables of up to 5120 positions and two work-groups a CU; with the heads of a token next to each other, several stretches."""
+    decode_and_check(cuda, Cache4(24, [5000, 2049, 0] + [i % 4 for i in range(300)], 16, 2, 32, 32, heads_first=heads_first), 2, 32, 32, BF16, append=True)
+    decode_and_check(cuda, Cache4(25, [2000] + [i % 3 for i in range(40)], 24, 3, 64, 64, heads_first=heads_first), 3, 64, 64, F32)
+
+
 def test_two_at_once(cuda):
     """Steps of two caches on two streams at the same time, and in inference mode: the bits of each by itself."""
     caches = [Cache4(22 + i, [4000, 70, 1500], 16, 2, 128, 128, spare=8) for i in range(2)]
