@@ -7,7 +7,7 @@
 // same bits.  A row of D columns is D / 2 + D / 32 bytes in place of 2 D.
 //
 // k_paged4_attn lies in registers as k_paged_attn does (lmoe_paged.hip); what differs:
-//   K: the contraction index may be numbered freely, so lane (c, g) holds a quarter of key c's columns, W / 4 from W / 4 g on: 16 (8)
+//   K: the contraction index may be numbered freely, so lane (c, g) holds a quarter of key c's columns, W / 4 from W / 4 g on: W / 8
 //     adjacent bytes and, with 128 columns, one scale.  Eight columns of them are the A operand of a product.
 //   V: lane (c, g) holds its eight keys at columns VW c .. + VW - 1, VW / 2 bytes and a scale each.
 //   The new token is made into 4 bits by the wave that attends to it, in the registers it is attended from.
@@ -308,7 +308,7 @@ template <int W> struct Tile4 {
   static constexpr int KW = W / 32;                // words of a lane's columns of a key
   uint32_t k[2][KW];
   uint32_t ks[2];
-  uint32_t v[8];                                   // the low half alone with 64 columns
+  uint32_t v[8];                                   // W / 4 bits of it
   uint32_t vs[8];
   uint32_t live;                                   // which of the positions exist
 };
@@ -439,7 +439,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
       t.ks[b] = *scale;
     };
     auto v_row = [&](int e, const uint8_t* codes, const uint8_t* scale) {
-      if constexpr (VW == 8) t.v[e] = *(const uint32_t*)codes; else t.v[e] = *(const uint16_t*)codes;
+      if constexpr (VW == 8) t.v[e] = *(const uint32_t*)codes;
+      else if constexpr (VW == 4) t.v[e] = *(const uint16_t*)codes;
+      else t.v[e] = *codes;
       t.vs[e] = *scale;
     };
     if constexpr (EVEN) {
@@ -554,7 +556,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
     // cache of 2-byte elements.)
     const Parts<T> pf = parts_of<T>(s[0], s[1]);
     pv4<T, W, 0>(o, t, pf);
-    pv4<T, W, 1>(o, t, pf);
+    if constexpr (VW > 2) pv4<T, W, 1>(o, t, pf);
     if constexpr (VW == 8) { pv4<T, W, 2>(o, t, pf); pv4<T, W, 3>(o, t, pf); }
   };
 
@@ -573,6 +575,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
       most = larger(most, size_of<T>(x[j]));
     }
     if constexpr (KC < 32) most = larger(most, __shfl_xor(most, 16, 64));
+    if constexpr (KC < 16) most = larger(most, __shfl_xor(most, 32, 64));
     y.ks[0] = scale4(most);
     y.ks[1] = 127;
 #pragma unroll
@@ -580,6 +583,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
     typename ET<T>::frag z = zero_frag<T>();
     if (vin) {
       if constexpr (VW == 8) z = ET<T>::load_frag(vn + VW * c);
+      else if constexpr (VW == 2 && FAST) { const bf16x2 u = *(const bf16x2*)(vn + VW * c); z[0] = u[0]; z[1] = u[1]; }
+      else if constexpr (VW == 2) { const f32x2 u = *(const f32x2*)(vn + VW * c); z.lo[0] = u[0]; z.lo[1] = u[1]; }
       else if constexpr (FAST) { const bf16x4 u = *(const bf16x4*)(vn + VW * c); z[0] = u[0]; z[1] = u[1]; z[2] = u[2]; z[3] = u[3]; }
       else z.lo = *(const f32x4*)(vn + VW * c);
     }
@@ -603,7 +608,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
       }
       if (g == 0 && vin) {
         uint8_t* row = (uint8_t*)vp + (int64_t)id * a.vp.sb + (int64_t)slot * a.vp.st + VW / 2 * c;
-        if constexpr (VW == 8) *(uint32_t*)row = y.v[0]; else *(uint16_t*)row = (uint16_t)y.v[0];
+        if constexpr (VW == 8) *(uint32_t*)row = y.v[0];
+        else if constexpr (VW == 4) *(uint16_t*)row = (uint16_t)y.v[0];
+        else *row = (uint8_t)y.v[0];
         if (VW * c % 32 == 0) ((uint8_t*)vsp)[(int64_t)id * a4.vs.sb + (int64_t)slot * a4.vs.st + VW * c / 32] = (uint8_t)y.vs[0];
       }
     }
@@ -678,7 +685,9 @@ template <typename T, int W> static void paged4_wide(const lmoe_paged4_args& a, 
   else paged4_parts<T, W, 4, false>(a, p, st);
 }
 template <typename T> static void paged4_decode(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
-  if (a.p.K <= 64 && a.p.V <= 64) paged4_wide<T, 64>(a, p, st); else paged4_wide<T, 128>(a, p, st);
+  if (a.p.K <= 32 && a.p.V <= 32) paged4_wide<T, 32>(a, p, st);          // (62 sequences of 12 to 46 K tokens, 10 / 2 heads of 32: 90 -> 80 us)
+  else if (a.p.K <= 64 && a.p.V <= 64) paged4_wide<T, 64>(a, p, st);
+  else paged4_wide<T, 128>(a, p, st);
 }
 void launch_paged4_decode(const lmoe_paged4_args& a, hipStream_t st) {
   const PagedPlan p = paged4_plan(a.p);
