@@ -11,8 +11,8 @@
 //     adjacent bytes and, with 128 columns, one scale.  Eight columns of them are the A operand of a product.
 //   V: lane (c, g) holds its eight keys at columns VW c .. + VW - 1, VW / 2 bytes and a scale each.
 //   The new token is made into 4 bits by the wave that attends to it, in the registers it is attended from.
-// HBM-bound while its stretches last (64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128, 179 MB: 44 us and a join of 5; of twice the
-// tokens the second half takes 5.2 TB/s); writing and reading, a wave per token, likewise (16384 tokens, 85 MB each way: 18 and 17 us).
+// HBM-bound where it lasts (64 sequences of 4096 tokens, 32 / 8 heads of 128, 287 MB: 55 us, 5.1 TB/s; of 1024 to 4096, 179 MB, 43); with rows of
+// 32 columns by its steps; writing and reading, a wave per token, likewise HBM-bound (16384 tokens, 85 MB each way: 18 and 17 us).
 #include <algorithm>
 
 #include "lmoe_paged.hpp"
@@ -256,7 +256,7 @@ void launch_paged_read(const lmoe_paged4_args& a, bool bits4, hipStream_t st) {
 // ---- one new token ----
 // Work-groups go round the eight XCDs in the order of their index.  First come the first stretches of all, then the second ones: those that a
 // sequence does not have come last, and what each XCD gets does not depend on how many stretches the table has room for (192 sequences
-// of 1024 tokens in a table of one page more, two stretches of which one is empty: with the stretches of a head next to each other half of
+// of 1024 tokens, two stretches of which one is empty: with the stretches of a head next to each other half of
 // the XCDs had nothing to do, 71 us, so 60).  Every so many stretches they shift by one, so that a long sequence is on all XCDs.
 // Where the heads of a token lie next to each other, two rows of 64 bytes share a cache line: then the heads of a stretch follow each
 // other on one XCD, and the line comes once from memory (64 sequences of 1024 to 4096 tokens, 32 / 8 heads of 128: 72 -> 62 us; where the
@@ -552,8 +552,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
         sum += s[b][e];
       }
     // (P rounded to the element type, as the products take it; the sum is of the numbers before.  What the rounding leaves, as two more
-    // products, would take the error of o from 0.0023 of its size to the 0.0017 of its own rounding: 49 -> 51 us, and 49 it is, as in a
-    // cache of 2-byte elements.)
+    // products, would take the error of o from 0.0023 of its size to the 0.0017 of its own rounding: 49 -> 51 us with stretches of 1024, and it
+    // stays out, as in a cache of 2-byte elements.)
     const Parts<T> pf = parts_of<T>(s[0], s[1]);
     pv4<T, W, 0>(o, t, pf);
     if constexpr (VW > 2) pv4<T, W, 1>(o, t, pf);
