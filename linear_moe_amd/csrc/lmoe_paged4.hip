@@ -361,7 +361,11 @@ __device__ __forceinline__ void pv4(f32x4 (&o)[W / 16], const Tile4<W>& t, const
 
 // EVEN: 16 adjacent positions lie in one page (S a multiple of 16) and offsets inside a page and strides of pages hold in 32 bits, so that a
 // step's rows are two bases in scalar registers and offsets that stay the same; else every position's page is looked up by a lane and passed round.
-template <typename T, int W, int NW, bool EVEN, bool CAP, bool BIAS>
+// FAR: the codes are read past the caches.
+template <bool FAR, typename V> __device__ __forceinline__ V fetch(const V* p) {
+  if constexpr (FAR) return __builtin_nontemporal_load(p); else return *p;
+}
+template <typename T, int W, int NW, bool EVEN, bool CAP, bool BIAS, bool FAR>
 __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
   const lmoe_paged_args& a = a4.p;
   typedef Tile4<W> Tile;
@@ -433,13 +437,13 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   // exist read a slot that does (behind the end: of their page; without a page: of page 0), and take() leaves them out.
   auto load = [&](Tile& t, int j0, const Where& x) {
     auto k_row = [&](int b, const uint8_t* codes, const uint8_t* scale) {
-      const words y = *(const words*)codes;
+      const words y = fetch<FAR>((const words*)codes);
 #pragma unroll
       for (int i = 0; i < KW; ++i) t.k[b][i] = y[i];
       t.ks[b] = *scale;
     };
     auto v_row = [&](int e, const uint8_t* codes, const uint8_t* scale) {
-      if constexpr (VW == 8) t.v[e] = *(const uint32_t*)codes;
+      if constexpr (VW == 8) t.v[e] = fetch<FAR>((const uint32_t*)codes);
       else if constexpr (VW == 4) t.v[e] = *(const uint16_t*)codes;
       else t.v[e] = *codes;
       t.vs[e] = *scale;
@@ -667,22 +671,31 @@ __global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_ar
   }
 }
 
-template <typename T, int W, int NW, bool EVEN> static void paged4_parts(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
+template <typename T, int W, int NW, bool EVEN, bool FAR = false> static void paged4_parts(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
   const int64_t units = (int64_t)a.p.N * p.splits;
   const dim3 grid((uint32_t)((heads_near(a.p, p) ? (units + XCDS - 1) / XCDS * XCDS : units) * a.p.HKV * p.blocks)), block(64 * NW);
   if (a.p.softcap > 0.f) {
-    if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, true>), grid, block, 0, st, a, p);
-    else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, false>), grid, block, 0, st, a, p);
-  } else if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, false, true>), grid, block, 0, st, a, p);
-  else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, false, false>), grid, block, 0, st, a, p);
+    if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, true, FAR>), grid, block, 0, st, a, p);
+    else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, true, false, FAR>), grid, block, 0, st, a, p);
+  } else if (a.p.slopes) hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, false, true, FAR>), grid, block, 0, st, a, p);
+  else hipLaunchKernelGGL((k_paged4_attn<T, W, NW, EVEN, false, false, FAR>), grid, block, 0, st, a, p);
 }
 template <typename T, int W> static void paged4_wide(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
   bool even = a.p.S % 16 == 0;
   for (const lmoe_tensor* t : {&a.p.kp, &a.p.vp, &a.ks, &a.vs}) even = even && t->sb >> 32 == 0 && t->st < 1ll << 27 && (a.p.S * t->st) >> 32 == 0;
+  // What the last-level cache would not keep until the next call is read past the caches: a table of more than it (256 MB), whole rows of 128
+  // columns, the tokens of a head next to each other (64 sequences of 1024 to 4096 tokens, 32 / 8 heads: 43 -> 41 us; heads of a token next to each
+  // other 60 -> 65, rows of 96 columns 37 -> 40, 2 sequences of 32 K and 128 K in a table of 142 MB 26.2 -> 26.9;
+  // 64 of 4096, 61 -> 58, and where eight each share their pages 44 -> 45).
+  const bool far = a.p.K == 128 && a.p.V == 128 && !heads_adjacent(a.p) && (int64_t)a.p.N * a.p.M * a.p.S * a.p.HKV * 136 > 256 << 20;
   if (p.waves == 8) {
     if (even) paged4_parts<T, W, 8, true>(a, p, st); else paged4_parts<T, W, 8, false>(a, p, st);
-  } else if (even) paged4_parts<T, W, 4, true>(a, p, st);
-  else paged4_parts<T, W, 4, false>(a, p, st);
+  } else if (even) {
+    if constexpr (W == 128) {
+      if (far) return paged4_parts<T, W, 4, true, true>(a, p, st);
+    }
+    paged4_parts<T, W, 4, true>(a, p, st);
+  } else paged4_parts<T, W, 4, false>(a, p, st);
 }
 template <typename T> static void paged4_decode(const lmoe_paged4_args& a, const PagedPlan& p, hipStream_t st) {
   if (a.p.K <= 32 && a.p.V <= 32) paged4_wide<T, 32>(a, p, st);          // (62 sequences of 12 to 46 K tokens, 10 / 2 heads of 32: 90 -> 80 us)

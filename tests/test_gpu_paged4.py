@@ -207,6 +207,18 @@ def test_one_stretch_for_many_work_groups(cuda, heads_first):
     decode_and_check(cuda, Cache4(25, [2000] + [i % 3 for i in range(40)], 24, 3, 64, 64, heads_first=heads_first), 3, 64, 64, F32)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_tables_past_the_caches(cuda, dtype):
+    """Tables of more than 256 MB of positions, most of them of no page: whole rows of 128 columns, and 96."""
+    for D in (128, 96):
+        c = Cache4(26, [300, 0, 1100, 33], 16, 2, D, D)
+        c.table = torch.cat([c.table, torch.full((4, 16000), -1, dtype=torch.int32)], 1)
+        decode_and_check(cuda, c, 4, D, D, dtype, append=True)
+    c = Cache4(27, [4000, 1] + [i % 3 for i in range(300)], 16, 2, 128, 128)
+    c.table = torch.cat([c.table, torch.full((302, 319 - c.table.shape[1]), -1, dtype=torch.int32)], 1)
+    decode_and_check(cuda, c, 2, 128, 128, dtype, softcap=20.0, slopes=alibi(2))
+
+
 def test_two_at_once(cuda):
     """Steps of two caches on two streams at the same time, and in inference mode: the bits of each by itself."""
     caches = [Cache4(22 + i, [4000, 70, 1500], 16, 2, 128, 128, spare=8) for i in range(2)]
