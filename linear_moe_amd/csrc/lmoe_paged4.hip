@@ -11,7 +11,7 @@
 //     adjacent bytes and, with 128 columns, one scale.  Eight columns of them are the A operand of a product.
 //   V: lane (c, g) holds its eight keys at columns VW c .. + VW - 1, VW / 2 bytes and a scale each.
 //   The new token is made into 4 bits by the wave that attends to it, in the registers it is attended from.
-// HBM-bound where it lasts (64 sequences of 4096 tokens, 32 / 8 heads of 128, 287 MB: 55 us, 5.1 TB/s; of 1024 to 4096, 179 MB, 43); with rows of
+// HBM-bound where it lasts (64 sequences of 4096 tokens, 32 / 8 heads of 128, 287 MB: 53 us, 5.4 TB/s; of 1024 to 4096, 179 MB, 41); with rows of
 // 32 columns by its steps; writing and reading, a wave per token, likewise HBM-bound (16384 tokens, 85 MB each way: 18 and 17 us).
 #include <algorithm>
 
