@@ -359,6 +359,9 @@ __device__ __forceinline__ void pv4(f32x4 (&o)[W / 16], const Tile4<W>& t, const
   mma_parts<T>(o[2 * B + 1], hi, pf);
 }
 
+// Waves of a SIMD that the registers have to do for at least: four where a step has few bytes and they suffice (60 sequences of 5 to 20 K tokens,
+// 16 / 4 heads of 64, three and four: 68.5 and 65 us)
+template <typename T, int W, int NW, bool EVEN> constexpr int paged4_waves() { return W == 64 && NW == 4 && EVEN && sizeof(T) == 2 ? 4 : 2; }
 // EVEN: 16 adjacent positions lie in one page (S a multiple of 16) and offsets inside a page and strides of pages hold in 32 bits, so that a
 // step's rows are two bases in scalar registers and offsets that stay the same; else every position's page is looked up by a lane and passed round.
 // FAR: the codes are read past the caches.
@@ -366,7 +369,7 @@ template <bool FAR, typename V> __device__ __forceinline__ V fetch(const V* p) {
   if constexpr (FAR) return __builtin_nontemporal_load(p); else return *p;
 }
 template <typename T, int W, int NW, bool EVEN, bool CAP, bool BIAS, bool FAR>
-__global__ __launch_bounds__(64 * NW, 2) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
+__global__ __launch_bounds__(64 * NW, (paged4_waves<T, W, NW, EVEN>())) void k_paged4_attn(const lmoe_paged4_args a4, const PagedPlan p) {
   const lmoe_paged_args& a = a4.p;
   typedef Tile4<W> Tile;
   constexpr int KW = Tile::KW, KC = W / 4, VW = W / 16;
